@@ -36,6 +36,7 @@ extern "C" {
 #define MHC_DTYPE_F32 0
 #define MHC_DTYPE_BF16 1
 #define MHC_DTYPE_F16 2
+#define MHC_DTYPE_U8 3 /* bytes or bools; taken where a comment says so */
 
 #define MHC_OK 0
 #define MHC_ERR_INVALID_ARG (-1)
@@ -307,6 +308,130 @@ int mhc_residual_add_agg_bwd(const void* x, const void* res, int dtype, const vo
                              int dout_dtype, const float* dy_agg, const float* h_pre, int h_mode,
                              void* dx, void* dres, float* dh_pre, void* workspace,
                              size_t workspace_bytes, int64_t T, int n, int C, void* stream);
+
+/* --------------------------------------------------------------------- */
+/* AdamW                                                                   */
+/* --------------------------------------------------------------------- */
+
+/* One tensor of an AdamW step: numel elements at each address, in the same
+ * order.  param and grad are of the call's dtype; master (fp32) is the copy
+ * that a 16-bit parameter is updated through, or NULL.  exp_avg / exp_avg_sq
+ * are fp32, or, with states in 8 bits, e4m3 codes of m and of sqrt(v), with
+ * scales[2 b] and scales[2 b + 1] the fp32 units of elements [256 b, 256 b +
+ * 256) of each (2 * ceil(numel / 256) floats). */
+typedef struct {
+  void* param;
+  const void* grad;
+  float* master;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* scales;
+  int64_t numel;
+} mhc_adamw_tensor;
+
+/* One step over `count` tensors, in place (`tensors` is host memory, read
+ * before the call returns):
+ *   g = grad * grad_scale (* *grad_scale_ptr, a device float, if not NULL)
+ *   p *= 1 - lr weight_decay;  m = beta1 m + (1 - beta1) g;
+ *   v = beta2 v + (1 - beta2) g g;
+ *   p -= lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * in fp32, each operation rounded by itself.  state_bits is 32 or 8.  With a
+ * master copy p is the master, and param its rounding.  The tensors of one
+ * call all have a master copy or none; they must not overlap.  An 8-bit
+ * block with a non-finite gradient is lost (its scale becomes inf or NaN). */
+int mhc_adamw_step(const mhc_adamw_tensor* tensors, int64_t count, int dtype, int state_bits,
+                   double lr, double beta1, double beta2, double eps, double weight_decay,
+                   int64_t step, double grad_scale, const float* grad_scale_ptr, void* stream);
+
+/* --------------------------------------------------------------------- */
+/* Clipped policy loss                                                     */
+/* --------------------------------------------------------------------- */
+
+/* Arguments shared by the policy-loss calls.  logits [T, V] of `dtype` with
+ * rows row_stride elements apart; actions [T] int64 in [0, V); old_logp,
+ * advantages [T] fp32; ref_logp [T] fp32 or NULL (no KL term); weights [T] of
+ * weights_dtype (fp32, or MHC_DTYPE_U8: 0 or 1) or NULL (all one), and 0
+ * leaves a token out: none of its other inputs counts.  denominator > 0
+ * divides the sum; 0: the sum of the weights (1 if that is 0). */
+typedef struct {
+  const void* logits;
+  int64_t row_stride;
+  const int64_t* actions;
+  const float* old_logp;
+  const float* advantages;
+  const float* ref_logp;
+  const void* weights;
+  int weights_dtype;
+  int64_t T;
+  int64_t V;
+  int dtype;
+  float clip_low;
+  float clip_high;
+  float kl_coef;
+  float denominator;
+} mhc_policy_args;
+
+/* Bytes of workspace of the calls that take one. */
+size_t mhc_policy_loss_workspace_bytes(int64_t T);
+
+/* loss[0] = sum_t w_t L_t / D, with lp = log softmax(logits_t)[a_t] and
+ *   r = exp(lp - old);  q = exp(ref - lp)
+ *   L = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (q - 1 - log q)
+ * logp [T] = lp (0 for a token left out).  stats [3 T + 1] is what the
+ * backward reads: each row's largest logit, the inverse of its sum of
+ * exponentials and w_t dL_t / dlp, then 1 / D.  An action outside [0, V) makes its token's values NaN. */
+int mhc_policy_loss_fwd(const mhc_policy_args* args, float* loss, float* logp, float* stats,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* dlogits [T, V] (contiguous, of the logits' dtype) = *dloss (or 1 if NULL)
+ * times the gradient of the loss; 0 in the rows of tokens left out. */
+int mhc_policy_loss_bwd(const mhc_policy_args* args, const float* stats, const float* dloss,
+                        void* dlogits, void* stream);
+
+/* Loss, logp and grad_scale times the gradient in one call, which reads the
+ * logits from memory once where a row fits the registers of a workgroup. */
+int mhc_policy_loss_fwd_bwd(const mhc_policy_args* args, float grad_scale, float* loss,
+                            float* logp, void* dlogits, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* --------------------------------------------------------------------- */
+/* Matrix product with bias, activation and residual                       */
+/* --------------------------------------------------------------------- */
+
+#define MHC_ACT_NONE 0
+#define MHC_ACT_RELU 1
+#define MHC_ACT_GELU 2      /* z Phi(z) */
+#define MHC_ACT_GELU_TANH 3 /* z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2 */
+#define MHC_ACT_SILU 4
+
+/* Bytes of workspace of mhc_linear_act_fwd (partial sums of a product whose
+ * reduction is split; 0 for most shapes). */
+size_t mhc_linear_act_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype);
+
+/* out [M, N] = act(x W^T + bias) + residual.  x [M, K] with rows ldx elements
+ * apart, w [N, K] with rows ldw apart, bias [N] or NULL, all of `dtype`;
+ * residual [M, N] or NULL and out of out_dtype (`dtype` or fp32), contiguous.
+ * dact [M, N] or NULL receives act'(x W^T + bias) for the backward: fp32 for
+ * fp32, else fp16, whose rounding of a value below 1.13 is an eighth of
+ * bf16's.  Sums are held in fp32. */
+int mhc_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
+                       const void* residual, void* out, int out_dtype, void* dact, int act,
+                       int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+size_t mhc_linear_act_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype,
+                                          int dout_dtype, int has_dact, int want_dx, int want_dw,
+                                          int want_db);
+
+/* Gradients of mhc_linear_act_fwd for dout [M, N] (contiguous, out_dtype):
+ *   dz = dout * dact (dact NULL: dz = dout), rounded to `dtype` for the products
+ *   dx [M, K] = dz W, dw [N, K] = dz^T x, db [N] = sum_m dz (unrounded)
+ * each contiguous, of `dtype`, written if not NULL.  The residual's gradient
+ * is dout. */
+int mhc_linear_act_bwd(const void* dout, int dout_dtype, const void* dact, const void* x,
+                       int64_t ldx, const void* w, int64_t ldw, void* dx, void* dw, void* db,
+                       int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
+                       size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

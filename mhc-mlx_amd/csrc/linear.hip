@@ -1,0 +1,165 @@
+// linear_act: out = act(x W^T + bias) + residual and its gradients.
+//
+// The forward is one product with the epilogue in its kernel; for a training
+// step it also stores d = act'(z), so that the backward needs neither z nor
+// an exponential: dz = dout d is one streaming pass, which also forms db from
+// the unrounded dz, and dx = dz W and dW = dz^T x are two more products.
+#include "mhc_gemm.hpp"
+
+namespace mhc {
+namespace {
+
+using gemm::Product;
+
+constexpr int kDzCols = 64 * 8;   // columns of a workgroup of dz_kernel: eight a lane of each wave
+constexpr int kDzRows = 64;       // rows: sixteen each wave
+
+// dz = dout dact (dact NULL: dout), rounded to T (not stored if dz is NULL),
+// and sums of dz over this workgroup's rows, before rounding, to part[block of rows][N] (if not NULL)
+template <typename T, typename G>
+__global__ __launch_bounds__(256) void dz_kernel(const G* dout, const void* dact, T* dz, float* part, int64_t M, int64_t N) {
+  using D = typename gemm::DactOf<T>::Type;
+  __shared__ float lds[4][kDzCols];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int64_t n = (int64_t)blockIdx.x * kDzCols + lane * 8, m0 = (int64_t)blockIdx.y * kDzRows;
+  const int left = (int)max((int64_t)0, min((int64_t)8, N - n));
+  float sum[8] = {};
+  for (int64_t m = m0 + wave; m < min(m0 + kDzRows, M); m += 4) {
+    for (int k = 0; k < left; ++k) {
+      const int64_t at = m * N + n + k;
+      float v = load1(dout + at);
+      if (dact != nullptr) v *= load1(static_cast<const D*>(dact) + at);
+      sum[k] += v;
+      if (dz != nullptr) store1(dz + at, v);
+    }
+  }
+  if (part == nullptr) return;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) lds[wave][lane * 8 + k] = sum[k];
+  __syncthreads();
+  for (int c = threadIdx.x; c < kDzCols; c += 256) {
+    const int64_t at = (int64_t)blockIdx.x * kDzCols + c;
+    if (at < N) part[(int64_t)blockIdx.y * N + at] = (lds[0][c] + lds[1][c]) + (lds[2][c] + lds[3][c]);
+  }
+}
+
+// db[n] = sum over the blocks of rows, in order
+template <typename T>
+__global__ __launch_bounds__(256) void db_kernel(const float* part, T* db, int64_t blocks, int64_t N) {
+  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (n >= N) return;
+  float s = 0.f;
+  for (int64_t b = 0; b < blocks; ++b) s += part[b * N + n];
+  store1(db + n, s);
+}
+
+int elem_bytes(int dtype) { return dtype == kF32 ? 4 : 2; }
+
+int run_product(const Product& p, bool a_k, bool b_k, int dtype, hipStream_t s) {
+  if (dtype == kF32) return gemm::run_product_f32(p, a_k, b_k, s);
+  if (dtype == kBF16) return gemm::run_product_bf16(p, a_k, b_k, s);
+  return gemm::run_product_f16(p, a_k, b_k, s);
+}
+
+size_t up256(size_t b) { return (b + 255) / 256 * 256; }
+
+struct BwdPlan {
+  size_t dz, part, total;  // bytes
+};
+
+BwdPlan plan_bwd(int64_t M, int64_t N, int dtype, int dout_dtype, bool dact, bool dx, bool dw, bool db) {
+  BwdPlan b = {};
+  if ((dx || dw) && (dact || dout_dtype != dtype)) b.dz = up256((size_t)(M * N) * elem_bytes(dtype));
+  if (db) b.part = up256((size_t)(ceil_div(M, kDzRows) * N) * sizeof(float));
+  b.total = b.dz + b.part;
+  return b;
+}
+
+template <typename T, typename G>
+int run_dz(const void* dout, const void* dact, void* dz, float* part, void* db, int64_t M, int64_t N, hipStream_t s) {
+  const int64_t blocks = ceil_div(M, kDzRows);
+  hipLaunchKernelGGL((dz_kernel<T, G>), dim3((unsigned)ceil_div(N, kDzCols), (unsigned)blocks), dim3(256), 0, s,
+                     static_cast<const G*>(dout), dact, static_cast<T*>(dz), part, M, N);
+  MHC_CHECK_LAUNCH("dz_kernel");
+  if (db != nullptr) {
+    hipLaunchKernelGGL((db_kernel<T>), dim3((unsigned)ceil_div(N, 256)), dim3(256), 0, s, (const float*)part, static_cast<T*>(db),
+                       blocks, N);
+    MHC_CHECK_LAUNCH("db_kernel");
+  }
+  return MHC_OK;
+}
+
+int check_shape(int64_t M, int64_t N, int64_t K, int dtype) {
+  MHC_CHECK_ARG(M >= 0 && N >= 1 && K >= 1, "M must be >= 0, N and K >= 1 (got %lld, %lld, %lld)", (long long)M,
+                (long long)N, (long long)K);
+  MHC_CHECK_ARG(M < ((int64_t)1 << 22) && N < ((int64_t)1 << 22) && K < ((int64_t)1 << 22), "M, N and K must be below 2^22");
+  MHC_CHECK_ARG(dtype == kF32 || dtype == kBF16 || dtype == kF16, "unsupported dtype %d", dtype);
+  return MHC_OK;
+}
+
+}  // namespace
+}  // namespace mhc
+
+extern "C" size_t mhc_linear_act_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) { return 0; }
+
+extern "C" int mhc_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
+                                  const void* residual, void* out, int out_dtype, void* dact, int act, int64_t M,
+                                  int64_t N, int64_t K, int dtype, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+  using namespace mhc;
+  clear_error();
+  if (const int rc = check_shape(M, N, K, dtype)) return rc;
+  MHC_CHECK_ARG(out_dtype == dtype || out_dtype == kF32, "out_dtype must be the operands' or fp32 (got %d)", out_dtype);
+  MHC_CHECK_ARG(act >= MHC_ACT_NONE && act <= MHC_ACT_SILU, "unknown activation %d", act);
+  if (M == 0) return MHC_OK;
+  MHC_CHECK_ARG(x && w && out, "null pointer");
+  MHC_CHECK_ARG((ldx >= K || M == 1) && (ldw >= K || N == 1), "ldx and ldw must be at least K");
+  const Product p = {x, w, ldx, ldw, M, N, K, gemm::epilogue(bias, residual, out, dact, act, out_dtype, dtype, N)};
+  return run_product(p, true, true, dtype, static_cast<hipStream_t>(stream));
+}
+
+extern "C" size_t mhc_linear_act_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int dout_dtype,
+                                                     int has_dact, int want_dx, int want_dw, int want_db) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return mhc::plan_bwd(M, N, dtype, dout_dtype, has_dact != 0, want_dx != 0, want_dw != 0, want_db != 0).total;
+}
+
+extern "C" int mhc_linear_act_bwd(const void* dout, int dout_dtype, const void* dact, const void* x, int64_t ldx,
+                                  const void* w, int64_t ldw, void* dx, void* dw, void* db, int64_t M, int64_t N,
+                                  int64_t K, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace mhc;
+  clear_error();
+  if (const int rc = check_shape(M, N, K, dtype)) return rc;
+  MHC_CHECK_ARG(dout_dtype == dtype || dout_dtype == kF32, "dout_dtype must be the operands' or fp32 (got %d)", dout_dtype);
+  MHC_CHECK_ARG(M > 0, "M must be > 0");
+  MHC_CHECK_ARG(dout && (dw == nullptr || x) && (dx == nullptr || w), "null pointer");
+  MHC_CHECK_ARG((dw == nullptr || ldx >= K || M == 1) && (dx == nullptr || ldw >= K || N == 1), "ldx and ldw must be at least K");
+  const BwdPlan b = plan_bwd(M, N, dtype, dout_dtype, dact != nullptr, dx != nullptr, dw != nullptr, db != nullptr);
+  MHC_CHECK_ARG(workspace_bytes >= b.total && (b.total == 0 || workspace != nullptr), "workspace too small");
+  MHC_CHECK_ARG(aligned(workspace, 16), "workspace must be 16-byte aligned");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char* const ws = static_cast<char*>(workspace);
+  void* const dz = b.dz > 0 ? ws : nullptr;
+  float* const part = b.part > 0 ? reinterpret_cast<float*>(ws + b.dz) : nullptr;
+  if (dz != nullptr || db != nullptr) {
+    int rc;
+    if (dtype == kF32) rc = run_dz<float, float>(dout, dact, dz, part, db, M, N, s);
+    else if (dtype == kBF16)
+      rc = dout_dtype == kF32 ? run_dz<__bf16, float>(dout, dact, dz, part, db, M, N, s)
+                              : run_dz<__bf16, __bf16>(dout, dact, dz, part, db, M, N, s);
+    else
+      rc = dout_dtype == kF32 ? run_dz<_Float16, float>(dout, dact, dz, part, db, M, N, s)
+                              : run_dz<_Float16, _Float16>(dout, dact, dz, part, db, M, N, s);
+    if (rc != MHC_OK) return rc;
+  }
+  const void* const g = dz != nullptr ? dz : dout;
+  if (dx != nullptr) {  // dx[m, k] = sum_n dz[m, n] W[n, k]
+    const Product p = {g, w, N, ldw, M, K, N, gemm::epilogue(nullptr, nullptr, dx, nullptr, MHC_ACT_NONE, dtype, dtype, K)};
+    if (const int rc = run_product(p, true, false, dtype, s)) return rc;
+  }
+  if (dw != nullptr) {  // dw[n, k] = sum_m dz[m, n] x[m, k]
+    const Product p = {g, x, N, ldx, N, K, M, gemm::epilogue(nullptr, nullptr, dw, nullptr, MHC_ACT_NONE, dtype, dtype, K)};
+    if (const int rc = run_product(p, false, false, dtype, s)) return rc;
+  }
+  return MHC_OK;
+}

@@ -1,0 +1,10 @@
+// The matrix products' kernels for f32 operands.
+#include "mhc_gemm.hpp"
+
+namespace mhc {
+namespace gemm {
+
+int run_product_f32(const Product& p, bool a_k, bool b_k, hipStream_t s) { return run_product<float>(p, a_k, b_k, s); }
+
+}  // namespace gemm
+}  // namespace mhc

@@ -473,6 +473,8 @@ at::Tensor module_call(py::handle mod, py::handle x_obj, py::handle rd_obj) {
 
 }  // namespace
 
+void bind_train(py::module_& m);  // torch_train.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "torch binding of libmhc_hip for MHCLayer's forward and backward";
   m.def("layer_apply", &layer_apply, "MHCLayer forward with its backward as a C++ autograd Function");
@@ -482,4 +484,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("residual_add_agg_nograd", &residual_add_agg_nograd, "residual_add_agg without autograd");
   m.def("module_forward", &module_forward, "MHCLayer.forward's accelerated path (None: take the general path)");
   m.def("module_call", &module_call, "module_forward with the arguments read from the MHCLayer instance");
+  bind_train(m);
 }

@@ -26,7 +26,9 @@ SOURCES = ["capi.hip", "sinkhorn.hip", "fused_fwd.hip", "fused_bwd.hip", "stream
            "mfma32.hip", "mix32.hip", "lf32_fwd.hip",
            "lf32_bwd_f32.hip", "lf32_bwd_bf16.hip", "lf32_bwd_f16.hip", "mxf32_f32.hip", "mxf32_bf16.hip", "mxf32_f16.hip",
            "lv_fwd_f32.hip", "lv_fwd_bf16.hip", "lv_fwd_f16.hip", "lv_bwd_f32.hip", "lv_bwd_bf16.hip", "lv_bwd_f16.hip",
-           "noalloc.hip"]
+           "noalloc.hip", "adamw.hip", "policy.hip", "linear.hip", "linear_f32.hip", "linear_bf16.hip", "linear_f16.hip"]
+
+EXT_SOURCES = ["torch_ext.cpp", "torch_train.cpp"]
 
 # Packed-FP32 VALU forms are disabled for every device pass (hipcc only; the
 # host pass prints a harmless "not a recognized feature" warning).
@@ -59,7 +61,7 @@ EXT_PATH = PKG_DIR / (EXT_NAME + ".so")
 
 
 def build_ext(verbose: bool = True) -> Path:
-    """Compile the torch binding (csrc/torch_ext.cpp) into _mhc_torch.so next to libmhc_hip.so.
+    """Compile the torch binding (csrc/torch_ext.cpp, csrc/torch_train.cpp) into _mhc_torch.so next to libmhc_hip.so.
 
     A plain C++ torch extension (g++, torch's headers and c10_hip for the current HIP stream); its
     calls into libmhc_hip resolve against the library, which _lib.load() opens with RTLD_GLOBAL
@@ -76,7 +78,7 @@ def build_ext(verbose: bool = True) -> Path:
     bdir.mkdir(parents=True, exist_ok=True)
     torch_lib = Path(torch.__file__).resolve().parent / "lib"
     rocm = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
-    ce.load(name=EXT_NAME, sources=[str(CSRC / "torch_ext.cpp")],
+    ce.load(name=EXT_NAME, sources=[str(CSRC / s) for s in EXT_SOURCES],
             extra_include_paths=[str(INCLUDE), str(rocm / "include")],
             extra_cflags=["-O2", "-D__HIP_PLATFORM_AMD__=1"],
             extra_ldflags=[f"-L{torch_lib}", "-lc10_hip"],

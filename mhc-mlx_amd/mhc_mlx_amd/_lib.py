@@ -16,6 +16,13 @@ LIB_PATH = Path(__file__).resolve().parent / "libmhc_hip.so"
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
 DTYPE_F16 = 2
+DTYPE_U8 = 3
+
+ACT_NONE = 0
+ACT_RELU = 1
+ACT_GELU = 2
+ACT_GELU_TANH = 3
+ACT_SILU = 4
 
 H_NONE = 0
 H_ACTIVATED = 1
@@ -28,7 +35,26 @@ _I32 = ctypes.c_int
 _I64 = ctypes.c_int64
 _F32 = ctypes.c_float
 _SZ = ctypes.c_size_t
+_F64 = ctypes.c_double
 _PI64 = ctypes.POINTER(ctypes.c_int64)
+
+
+class AdamWTensor(ctypes.Structure):
+    """mhc_adamw_tensor: one tensor of an AdamW step."""
+
+    _fields_ = [("param", _VP), ("grad", _VP), ("master", _VP), ("exp_avg", _VP), ("exp_avg_sq", _VP), ("scales", _VP),
+                ("numel", _I64)]
+
+
+class PolicyArgs(ctypes.Structure):
+    """mhc_policy_args: the inputs of the policy-loss calls."""
+
+    _fields_ = [("logits", _VP), ("row_stride", _I64), ("actions", _VP), ("old_logp", _VP), ("advantages", _VP),
+                ("ref_logp", _VP), ("weights", _VP), ("weights_dtype", _I32), ("T", _I64), ("V", _I64), ("dtype", _I32),
+                ("clip_low", _F32), ("clip_high", _F32), ("kl_coef", _F32), ("denominator", _F32)]
+
+
+_PPOL = ctypes.POINTER(PolicyArgs)
 
 # name -> (argtypes, restype); must list exactly the functions of mhc_hip.h
 SIGNATURES = {
@@ -76,6 +102,18 @@ SIGNATURES = {
     "mhc_residual_add_agg_bwd_workspace_bytes": ([_I64, _I32, _I32], _SZ),
     "mhc_residual_add_agg_bwd": ([_VP, _VP, _I32, _VP, _I32, _VP, _VP, _I32, _VP, _VP, _VP, _VP, _SZ, _I64,
                                   _I32, _I32, _VP], _I32),
+    "mhc_adamw_step": ([ctypes.POINTER(AdamWTensor), _I64, _I32, _I32, _F64, _F64, _F64, _F64, _F64, _I64, _F64, _VP, _VP],
+                       _I32),
+    "mhc_policy_loss_workspace_bytes": ([_I64], _SZ),
+    "mhc_policy_loss_fwd": ([_PPOL, _VP, _VP, _VP, _VP, _SZ, _VP], _I32),
+    "mhc_policy_loss_bwd": ([_PPOL, _VP, _VP, _VP, _VP], _I32),
+    "mhc_policy_loss_fwd_bwd": ([_PPOL, _F32, _VP, _VP, _VP, _VP, _SZ, _VP], _I32),
+    "mhc_linear_act_fwd_workspace_bytes": ([_I64, _I64, _I64, _I32], _SZ),
+    "mhc_linear_act_fwd": ([_VP, _I64, _VP, _I64, _VP, _VP, _VP, _I32, _VP, _I32, _I64, _I64, _I64, _I32, _VP, _SZ, _VP],
+                           _I32),
+    "mhc_linear_act_bwd_workspace_bytes": ([_I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _I32], _SZ),
+    "mhc_linear_act_bwd": ([_VP, _I32, _VP, _VP, _I64, _VP, _I64, _VP, _VP, _VP, _I64, _I64, _I64, _I32, _VP, _SZ, _VP],
+                           _I32),
 }
 
 _lock = threading.Lock()
