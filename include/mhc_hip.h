@@ -404,24 +404,26 @@ int mhc_policy_loss_fwd_bwd(const mhc_policy_args* args, float grad_scale, float
 #define MHC_ACT_GELU_TANH 3 /* z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2 */
 #define MHC_ACT_SILU 4
 
-/* Bytes of workspace of mhc_linear_act_fwd (partial sums of a product whose
- * reduction is split; 0 for most shapes). */
-size_t mhc_linear_act_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype);
+/* Bytes of workspace of mhc_linear_act_fwd for these operands: copies of
+ * those whose rows do not start on 16 bytes or are no multiple of it. */
+size_t mhc_linear_act_fwd_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                          int64_t M, int64_t N, int64_t K, int dtype);
 
 /* out [M, N] = act(x W^T + bias) + residual.  x [M, K] with rows ldx elements
  * apart, w [N, K] with rows ldw apart, bias [N] or NULL, all of `dtype`;
  * residual [M, N] or NULL and out of out_dtype (`dtype` or fp32), contiguous.
- * dact [M, N] or NULL receives act'(x W^T + bias) for the backward: fp32 for
- * fp32, else fp16, whose rounding of a value below 1.13 is an eighth of
- * bf16's.  Sums are held in fp32. */
+ * dact [M, N] or NULL (only NULL for MHC_ACT_NONE) receives act'(x W^T +
+ * bias) for the backward: fp32 for fp32, else int16, (act' - 1/2) 2^15 with
+ * -2^15 for NaN.  Sums are held in fp32. */
 int mhc_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
                        const void* residual, void* out, int out_dtype, void* dact, int act,
                        int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
                        size_t workspace_bytes, void* stream);
 
-size_t mhc_linear_act_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype,
-                                          int dout_dtype, int has_dact, int want_dx, int want_dw,
-                                          int want_db);
+size_t mhc_linear_act_bwd_workspace_bytes(const void* dout, int dout_dtype, const void* dact,
+                                          const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                          int want_dx, int want_dw, int want_db, int64_t M,
+                                          int64_t N, int64_t K, int dtype);
 
 /* Gradients of mhc_linear_act_fwd for dout [M, N] (contiguous, out_dtype):
  *   dz = dout * dact (dact NULL: dz = dout), rounded to `dtype` for the products

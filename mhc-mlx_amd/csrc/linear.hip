@@ -9,15 +9,17 @@
 namespace mhc {
 namespace {
 
+using gemm::Operand;
 using gemm::Product;
 
 constexpr int kDzCols = 64 * 8;   // columns of a workgroup of dz_kernel: eight a lane of each wave
 constexpr int kDzRows = 64;       // rows: sixteen each wave
 
-// dz = dout dact (dact NULL: dout), rounded to T (not stored if dz is NULL),
-// and sums of dz over this workgroup's rows, before rounding, to part[block of rows][N] (if not NULL)
+// dz = dout dact (dact NULL: dout), rounded to T, in rows of N elements `ld`
+// apart with zeros between (not stored if dz is NULL), and sums of dz over this workgroup's rows, before rounding, to part[block of rows][N] (if not NULL)
 template <typename T, typename G>
-__global__ __launch_bounds__(256) void dz_kernel(const G* dout, const void* dact, T* dz, float* part, int64_t M, int64_t N) {
+__global__ __launch_bounds__(256) void dz_kernel(const G* dout, const void* dact, T* dz, int64_t ld, float* part, int64_t M,
+                                                 int64_t N) {
   using D = typename gemm::DactOf<T>::Type;
   __shared__ float lds[4][kDzCols];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
@@ -28,10 +30,11 @@ __global__ __launch_bounds__(256) void dz_kernel(const G* dout, const void* dact
     for (int k = 0; k < left; ++k) {
       const int64_t at = m * N + n + k;
       float v = load1(dout + at);
-      if (dact != nullptr) v *= load1(static_cast<const D*>(dact) + at);
+      if (dact != nullptr) v *= gemm::dact_value(static_cast<const D*>(dact)[at]);
       sum[k] += v;
-      if (dz != nullptr) store1(dz + at, v);
+      if (dz != nullptr) store1(dz + m * ld + n + k, v);
     }
+    for (int k = left; k < 8 && dz != nullptr && n + k < ld; ++k) dz[m * ld + n + k] = (T)0;
   }
   if (part == nullptr) return;
 #pragma unroll
@@ -53,6 +56,26 @@ __global__ __launch_bounds__(256) void db_kernel(const float* part, T* db, int64
   store1(db + n, s);
 }
 
+// rows of `width` elements, `ld` apart, into rows of a multiple of 16 bytes, with zeros after the last element
+template <typename T>
+__global__ __launch_bounds__(256) void pack_kernel(const T* src, int64_t ld, T* dst, int64_t rows, int64_t width, int64_t chunks) {
+  constexpr int kE = 16 / (int)sizeof(T);
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < rows * chunks; at += (int64_t)gridDim.x * 256) {
+    const int64_t row = at / chunks, k = at % chunks * kE;
+    const T* const p = src + row * ld + k;
+    u32x4 v = {0, 0, 0, 0};
+    if (k + kE <= width) {
+      __builtin_memcpy(&v, p, 16);
+    } else {
+      T e[kE];
+#pragma unroll
+      for (int j = 0; j < kE; ++j) e[j] = k + j < width ? p[j] : (T)0;
+      __builtin_memcpy(&v, e, 16);
+    }
+    reinterpret_cast<u32x4*>(dst)[at] = v;
+  }
+}
+
 int elem_bytes(int dtype) { return dtype == kF32 ? 4 : 2; }
 
 int run_product(const Product& p, bool a_k, bool b_k, int dtype, hipStream_t s) {
@@ -63,23 +86,63 @@ int run_product(const Product& p, bool a_k, bool b_k, int dtype, hipStream_t s) 
 
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
+int64_t padded(int64_t width, int dtype) {
+  const int64_t e = 16 / elem_bytes(dtype);
+  return (width + e - 1) / e * e;
+}
+
+// bytes of an operand's copy in rows of whole chunks; 0: it is read as it is
+size_t pack_bytes(const void* p, int64_t rows, int64_t ld, int64_t width, int dtype) {
+  if (gemm::in_chunks(p, ld, width, elem_bytes(dtype))) return 0;
+  return up256((size_t)(rows * padded(width, dtype)) * elem_bytes(dtype));
+}
+
+template <typename T>
+int run_pack(const void* p, int64_t ld, void* to, int64_t rows, int64_t width, int64_t wide, hipStream_t s) {
+  const int64_t chunks = wide * (int64_t)sizeof(T) / 16;
+  const int64_t blocks = std::min(ceil_div(rows * chunks, 256), (int64_t)device_cu_count() * 16);
+  hipLaunchKernelGGL((pack_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, static_cast<const T*>(p), ld,
+                     static_cast<T*>(to), rows, width, chunks);
+  MHC_CHECK_LAUNCH("pack_kernel");
+  return MHC_OK;
+}
+
+// The operand, copied to `ws` first (which moves on) where its rows are not whole chunks.
+int operand(Operand& o, const void* p, int64_t rows, int64_t ld, int64_t width, int dtype, char*& ws, hipStream_t s) {
+  const size_t bytes = pack_bytes(p, rows, ld, width, dtype);
+  if (bytes == 0) {
+    o = Operand{p, ld, width};
+    return MHC_OK;
+  }
+  const int64_t wide = padded(width, dtype);
+  o = Operand{ws, wide, wide};
+  const int rc = dtype == kF32 ? run_pack<float>(p, ld, ws, rows, width, wide, s)
+                               : run_pack<uint16_t>(p, ld, ws, rows, width, wide, s);
+  ws += bytes;
+  return rc;
+}
+
 struct BwdPlan {
-  size_t dz, part, total;  // bytes
+  size_t dz, part, x, w, total;  // bytes
 };
 
-BwdPlan plan_bwd(int64_t M, int64_t N, int dtype, int dout_dtype, bool dact, bool dx, bool dw, bool db) {
+BwdPlan plan_bwd(const void* dout, int dout_dtype, bool dact, const void* x, int64_t ldx, const void* w, int64_t ldw, bool dx, bool dw,
+                 bool db, int64_t M, int64_t N, int64_t K, int dtype) {
   BwdPlan b = {};
-  if ((dx || dw) && (dact || dout_dtype != dtype)) b.dz = up256((size_t)(M * N) * elem_bytes(dtype));
+  if ((dx || dw) && (dact || dout_dtype != dtype || !gemm::in_chunks(dout, N, N, elem_bytes(dtype))))
+    b.dz = up256((size_t)(M * padded(N, dtype)) * elem_bytes(dtype));
   if (db) b.part = up256((size_t)(ceil_div(M, kDzRows) * N) * sizeof(float));
-  b.total = b.dz + b.part;
+  if (dx) b.w = pack_bytes(w, N, ldw, K, dtype);
+  if (dw) b.x = pack_bytes(x, M, ldx, K, dtype);
+  b.total = b.dz + b.part + b.x + b.w;
   return b;
 }
 
 template <typename T, typename G>
-int run_dz(const void* dout, const void* dact, void* dz, float* part, void* db, int64_t M, int64_t N, hipStream_t s) {
+int run_dz(const void* dout, const void* dact, void* dz, int64_t ld, float* part, void* db, int64_t M, int64_t N, hipStream_t s) {
   const int64_t blocks = ceil_div(M, kDzRows);
   hipLaunchKernelGGL((dz_kernel<T, G>), dim3((unsigned)ceil_div(N, kDzCols), (unsigned)blocks), dim3(256), 0, s,
-                     static_cast<const G*>(dout), dact, static_cast<T*>(dz), part, M, N);
+                     static_cast<const G*>(dout), dact, static_cast<T*>(dz), ld, part, M, N);
   MHC_CHECK_LAUNCH("dz_kernel");
   if (db != nullptr) {
     hipLaunchKernelGGL((db_kernel<T>), dim3((unsigned)ceil_div(N, 256)), dim3(256), 0, s, (const float*)part, static_cast<T*>(db),
@@ -100,7 +163,11 @@ int check_shape(int64_t M, int64_t N, int64_t K, int dtype) {
 }  // namespace
 }  // namespace mhc
 
-extern "C" size_t mhc_linear_act_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) { return 0; }
+extern "C" size_t mhc_linear_act_fwd_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M,
+                                                     int64_t N, int64_t K, int dtype) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return mhc::pack_bytes(x, M, ldx, K, dtype) + mhc::pack_bytes(w, N, ldw, K, dtype);
+}
 
 extern "C" int mhc_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
                                   const void* residual, void* out, int out_dtype, void* dact, int act, int64_t M,
@@ -111,17 +178,26 @@ extern "C" int mhc_linear_act_fwd(const void* x, int64_t ldx, const void* w, int
   if (const int rc = check_shape(M, N, K, dtype)) return rc;
   MHC_CHECK_ARG(out_dtype == dtype || out_dtype == kF32, "out_dtype must be the operands' or fp32 (got %d)", out_dtype);
   MHC_CHECK_ARG(act >= MHC_ACT_NONE && act <= MHC_ACT_SILU, "unknown activation %d", act);
+  MHC_CHECK_ARG(act != MHC_ACT_NONE || dact == nullptr, "dact is for an activation");
   if (M == 0) return MHC_OK;
   MHC_CHECK_ARG(x && w && out, "null pointer");
   MHC_CHECK_ARG((ldx >= K || M == 1) && (ldw >= K || N == 1), "ldx and ldw must be at least K");
-  const Product p = {x, w, ldx, ldw, M, N, K, gemm::epilogue(bias, residual, out, dact, act, out_dtype, dtype, N)};
-  return run_product(p, true, true, dtype, static_cast<hipStream_t>(stream));
+  MHC_CHECK_ARG(workspace_bytes >= mhc_linear_act_fwd_workspace_bytes(x, ldx, w, ldw, M, N, K, dtype), "workspace too small");
+  MHC_CHECK_ARG(aligned(workspace, 16), "workspace must be 16-byte aligned");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  Product p = {{}, {}, M, N, K, gemm::epilogue(bias, residual, out, dact, act, out_dtype, dtype, N)};
+  if (const int rc = operand(p.a, x, M, ldx, K, dtype, ws, s)) return rc;
+  if (const int rc = operand(p.b, w, N, ldw, K, dtype, ws, s)) return rc;
+  return run_product(p, true, true, dtype, s);
 }
 
-extern "C" size_t mhc_linear_act_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype, int dout_dtype,
-                                                     int has_dact, int want_dx, int want_dw, int want_db) {
+extern "C" size_t mhc_linear_act_bwd_workspace_bytes(const void* dout, int dout_dtype, const void* dact, const void* x,
+                                                     int64_t ldx, const void* w, int64_t ldw, int want_dx, int want_dw,
+                                                     int want_db, int64_t M, int64_t N, int64_t K, int dtype) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  return mhc::plan_bwd(M, N, dtype, dout_dtype, has_dact != 0, want_dx != 0, want_dw != 0, want_db != 0).total;
+  return mhc::plan_bwd(dout, dout_dtype, dact != nullptr, x, ldx, w, ldw, want_dx != 0, want_dw != 0, want_db != 0, M, N, K, dtype)
+      .total;
 }
 
 extern "C" int mhc_linear_act_bwd(const void* dout, int dout_dtype, const void* dact, const void* x, int64_t ldx,
@@ -134,31 +210,35 @@ extern "C" int mhc_linear_act_bwd(const void* dout, int dout_dtype, const void* 
   MHC_CHECK_ARG(M > 0, "M must be > 0");
   MHC_CHECK_ARG(dout && (dw == nullptr || x) && (dx == nullptr || w), "null pointer");
   MHC_CHECK_ARG((dw == nullptr || ldx >= K || M == 1) && (dx == nullptr || ldw >= K || N == 1), "ldx and ldw must be at least K");
-  const BwdPlan b = plan_bwd(M, N, dtype, dout_dtype, dact != nullptr, dx != nullptr, dw != nullptr, db != nullptr);
+  const BwdPlan b = plan_bwd(dout, dout_dtype, dact != nullptr, x, ldx, w, ldw, dx != nullptr, dw != nullptr, db != nullptr, M, N, K,
+                             dtype);
   MHC_CHECK_ARG(workspace_bytes >= b.total && (b.total == 0 || workspace != nullptr), "workspace too small");
   MHC_CHECK_ARG(aligned(workspace, 16), "workspace must be 16-byte aligned");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  char* const ws = static_cast<char*>(workspace);
+  char* ws = static_cast<char*>(workspace);
   void* const dz = b.dz > 0 ? ws : nullptr;
   float* const part = b.part > 0 ? reinterpret_cast<float*>(ws + b.dz) : nullptr;
   if (dz != nullptr || db != nullptr) {
     int rc;
-    if (dtype == kF32) rc = run_dz<float, float>(dout, dact, dz, part, db, M, N, s);
+    if (dtype == kF32) rc = run_dz<float, float>(dout, dact, dz, padded(N, dtype), part, db, M, N, s);
     else if (dtype == kBF16)
-      rc = dout_dtype == kF32 ? run_dz<__bf16, float>(dout, dact, dz, part, db, M, N, s)
-                              : run_dz<__bf16, __bf16>(dout, dact, dz, part, db, M, N, s);
+      rc = dout_dtype == kF32 ? run_dz<__bf16, float>(dout, dact, dz, padded(N, dtype), part, db, M, N, s)
+                              : run_dz<__bf16, __bf16>(dout, dact, dz, padded(N, dtype), part, db, M, N, s);
     else
-      rc = dout_dtype == kF32 ? run_dz<_Float16, float>(dout, dact, dz, part, db, M, N, s)
-                              : run_dz<_Float16, _Float16>(dout, dact, dz, part, db, M, N, s);
+      rc = dout_dtype == kF32 ? run_dz<_Float16, float>(dout, dact, dz, padded(N, dtype), part, db, M, N, s)
+                              : run_dz<_Float16, _Float16>(dout, dact, dz, padded(N, dtype), part, db, M, N, s);
     if (rc != MHC_OK) return rc;
   }
-  const void* const g = dz != nullptr ? dz : dout;
+  ws += b.dz + b.part;
+  const Operand g = dz != nullptr ? Operand{dz, padded(N, dtype), padded(N, dtype)} : Operand{dout, N, N};
   if (dx != nullptr) {  // dx[m, k] = sum_n dz[m, n] W[n, k]
-    const Product p = {g, w, N, ldw, M, K, N, gemm::epilogue(nullptr, nullptr, dx, nullptr, MHC_ACT_NONE, dtype, dtype, K)};
+    Product p = {g, {}, M, K, N, gemm::epilogue(nullptr, nullptr, dx, nullptr, MHC_ACT_NONE, dtype, dtype, K)};
+    if (const int rc = operand(p.b, w, N, ldw, K, dtype, ws, s)) return rc;
     if (const int rc = run_product(p, true, false, dtype, s)) return rc;
   }
   if (dw != nullptr) {  // dw[n, k] = sum_m dz[m, n] x[m, k]
-    const Product p = {g, x, N, ldx, N, K, M, gemm::epilogue(nullptr, nullptr, dw, nullptr, MHC_ACT_NONE, dtype, dtype, K)};
+    Product p = {g, {}, N, K, M, gemm::epilogue(nullptr, nullptr, dw, nullptr, MHC_ACT_NONE, dtype, dtype, K)};
+    if (const int rc = operand(p.b, x, M, ldx, K, dtype, ws, s)) return rc;
     if (const int rc = run_product(p, false, false, dtype, s)) return rc;
   }
   return MHC_OK;

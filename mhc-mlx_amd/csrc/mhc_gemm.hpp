@@ -22,17 +22,16 @@ struct Epilogue {
   const void* bias;      // [N] of the operands' type, or NULL
   const void* residual;  // [M, N] of the output's type, or NULL
   void* out;             // [M, N]
-  void* dact;            // [M, N] fp32 (fp32 operands) or fp16, or NULL
+  void* dact;            // [M, N] as DactOf has it, or NULL; act is not none then
   int act;               // MHC_ACT_*
   int out_f32;           // out and residual are fp32, else of the operands' type
-  int vec;               // four outputs from a column that is a multiple of four are one vector of each array
+  int vec;               // eight outputs from a column that is a multiple of eight are whole 16-byte vectors
 };
 
 // an epilogue whose `vec` goes by the row length and the addresses (residuals start anywhere)
 inline Epilogue epilogue(const void* bias, const void* residual, void* out, void* dact, int act, int out_dtype, int dtype,
                          int64_t N) {
-  const int eo = out_dtype == kF32 ? 16 : 8, ed = dtype == kF32 ? 16 : 8;
-  const bool vec = N % 4 == 0 && aligned(out, eo) && aligned(residual, eo) && aligned(dact, ed);
+  const bool vec = N % 8 == 0 && aligned(out, 16) && aligned(residual, 16) && aligned(dact, 16);
   return Epilogue{bias, residual, out, dact, act, out_dtype == kF32, vec};
 }
 
@@ -62,67 +61,72 @@ MHC_DEV Act activate(float z, int act) {
   }
 }
 
-template <typename T> struct DactOf { using Type = _Float16; };
+// act'(z) as a backward reads it: fp32 for fp32 operands, else 16 bits in fixed
+// point, (act' - 1/2) 2^15.  All of the derivatives lie in [-0.13, 1.13], so
+// that 2^-16 is the largest error, where fp16 has 2^-11 of the value and more
+// of the gradients' error would be act's than the one rounding of dz; 0 and 1
+// are exact.  The lowest code is NaN.
+template <typename T> struct DactOf { using Type = int16_t; };
 template <> struct DactOf<float> { using Type = float; };
 
-// `C` consecutive outputs of one row, from column n; vec: all C are stored as one vector
-template <typename T, int C>
-MHC_DEV void finish(const Epilogue& e, int64_t m, int64_t n, int64_t N, float (&z)[C], bool vec) {
-  using D = typename DactOf<T>::Type;
-  const int64_t at = m * N + n;
-  const int left = vec ? C : (int)min((int64_t)C, N - n);
-  float d[C];
+MHC_DEV uint32_t dact_code(float d) {
+  return (uint32_t)(d == d ? (int)rintf((d - 0.5f) * 32768.f) : -32768) & 0xffffu;
+}
+MHC_DEV float dact_value(int16_t q) { return q == -32768 ? __builtin_nanf("") : 0.5f + (float)q * 0x1p-15f; }
+MHC_DEV float dact_value(float d) { return d; }
+
+// V values to p: as 16-byte vectors (of 16-bit values: one for eight)
+template <typename O, int V>
+MHC_DEV void put(O* p, const float (&z)[V]) {
+  if constexpr (V == 1) {
+    if constexpr (__is_same(O, int16_t)) *p = (int16_t)dact_code(z[0]);
+    else store1(p, z[0]);
+  } else if constexpr (sizeof(O) == 4) {
 #pragma unroll
-  for (int k = 0; k < C; ++k) {
-    if (e.bias != nullptr && k < left) z[k] += load1(static_cast<const T*>(e.bias) + n + k);
-    const Act a = activate(z[k], e.act);
-    z[k] = a.y;
-    d[k] = a.d;
-  }
-  if (vec) {
-    if (e.out_f32) {
-      if (e.residual != nullptr) {
-        Vec<float, C> r;
-        r.load(static_cast<const float*>(e.residual) + at);
-#pragma unroll
-        for (int k = 0; k < C; ++k) z[k] += r.get(k);
-      }
-      float* const o = static_cast<float*>(e.out) + at;
-#pragma unroll
-      for (int k = 0; k < C; k += 4) *reinterpret_cast<f32x4*>(o + k) = f32x4{z[k], z[k + 1], z[k + 2], z[k + 3]};
-    } else if constexpr (sizeof(T) == 2) {
-      if (e.residual != nullptr) {
-        Vec<T, C> r;
-        r.load(static_cast<const T*>(e.residual) + at);
-#pragma unroll
-        for (int k = 0; k < C; ++k) z[k] += r.get(k);
-      }
-      T* const o = static_cast<T*>(e.out) + at;
-#pragma unroll
-      for (int k = 0; k < C; k += 4)
-        *reinterpret_cast<u32x2*>(o + k) = u32x2{pack2<T>(z[k], z[k + 1]), pack2<T>(z[k + 2], z[k + 3])};
-    }
-    if (e.dact != nullptr) {
-      D* const o = static_cast<D*>(e.dact) + at;
-#pragma unroll
-      for (int k = 0; k < C; k += 4) {
-        if constexpr (sizeof(D) == 4) *reinterpret_cast<f32x4*>(o + k) = f32x4{d[k], d[k + 1], d[k + 2], d[k + 3]};
-        else *reinterpret_cast<u32x2*>(o + k) = u32x2{pack2<D>(d[k], d[k + 1]), pack2<D>(d[k + 2], d[k + 3])};
-      }
-    }
+    for (int k = 0; k < V; k += 4) *reinterpret_cast<f32x4*>(p + k) = f32x4{z[k], z[k + 1], z[k + 2], z[k + 3]};
   } else {
+    u32x4 w;
 #pragma unroll
-    for (int k = 0; k < C; ++k) {
-      if (k >= left) break;
-      if (e.out_f32) {
-        if (e.residual != nullptr) z[k] += static_cast<const float*>(e.residual)[at + k];
-        static_cast<float*>(e.out)[at + k] = z[k];
-      } else {
-        if (e.residual != nullptr) z[k] += load1(static_cast<const T*>(e.residual) + at + k);
-        store1(static_cast<T*>(e.out) + at + k, z[k]);
-      }
-      if (e.dact != nullptr) store1(static_cast<D*>(e.dact) + at + k, d[k]);
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (__is_same(O, int16_t)) w[k] = dact_code(z[2 * k]) | dact_code(z[2 * k + 1]) << 16;
+      else w[k] = pack2<O>(z[2 * k], z[2 * k + 1]);
     }
+    *reinterpret_cast<u32x4*>(p) = w;
+  }
+}
+
+template <typename O, int V>
+MHC_DEV void add(const O* p, float (&z)[V]) {
+  Vec<O, V> r;
+  r.load(p);
+#pragma unroll
+  for (int k = 0; k < V; ++k) z[k] += r.get(k);
+}
+
+// V outputs of row m from column n on, from their sums; V > 1: each array's are whole vectors
+template <typename T, int V>
+MHC_DEV void finish(const Epilogue& e, int64_t m, int64_t n, int64_t N, float (&z)[V]) {
+  const int64_t at = m * N + n;
+  if (e.bias != nullptr) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) z[k] += load1(static_cast<const T*>(e.bias) + n + k);
+  }
+  if (e.act != MHC_ACT_NONE) {
+    float d[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const Act a = activate(z[k], e.act);
+      z[k] = a.y;
+      d[k] = a.d;
+    }
+    if (e.dact != nullptr) put(static_cast<typename DactOf<T>::Type*>(e.dact) + at, d);
+  }
+  if (e.out_f32) {
+    if (e.residual != nullptr) add(static_cast<const float*>(e.residual) + at, z);
+    put(static_cast<float*>(e.out) + at, z);
+  } else if constexpr (sizeof(T) == 2) {
+    if (e.residual != nullptr) add(static_cast<const T*>(e.residual) + at, z);
+    put(static_cast<T*>(e.out) + at, z);
   }
 }
 
@@ -149,112 +153,292 @@ MHC_DEV f32x4 mfma16(const u32x4& a, const u32x4& b, f32x4 c) {
 }
 
 // --------------------------------------------------------------------------
-// The tile kernel: 128 x 128 outputs a workgroup, four waves of 64 x 64
+// The tile kernel: BM x BN outputs a workgroup, WM x WN waves
 // --------------------------------------------------------------------------
 
+// An operand as it is stored: rows of `width` elements, `ld` elements apart.
+// Rows and width are a multiple of 16 bytes long and start on one.
+struct Operand {
+  const void* p;
+  int64_t ld, width;
+};
+
+constexpr int64_t kMaxRowBytes = 1 << 23;  // between rows: 256 of them stay below 2^31
+
+// Whether rows of `width` elements, `ld` apart, can be an Operand as they are.
+inline bool in_chunks(const void* p, int64_t ld, int64_t width, int bytes) {
+  return aligned(p, 16) && ld * bytes % 16 == 0 && width * bytes % 16 == 0 && ld * bytes <= kMaxRowBytes;
+}
+
 struct Product {
-  const void* a;
-  const void* b;
-  int64_t lda, ldb;  // elements between rows as they are stored
+  Operand a, b;
   int64_t M, N, K;
   Epilogue e;
 };
 
-constexpr int kTile = 128;
-constexpr int kTileThreads = 256;
-
-// LDS holds an operand's tile as rows of its index with eight 16-byte chunks
-// of k each; chunk c of row r is at c ^ (r % 8), so that 16 lanes that read
-// the same chunk of 16 rows meet different banks.
+// LDS holds an operand's tile of a stage, 128 bytes of k for each index, in
+// 16-byte chunks that the wave's loads put there directly.
+//
+// k-major: a row for each index, with eight chunks of k.  Chunk c of row r is
+// at c ^ (r % 8), so that lanes that read the same chunk of 16 rows meet
+// different banks.
+//
+// Otherwise: a row for each k, with chunks of the index.  16-bit operands are
+// read with a transposing load (four k of one index a lane): its 16 lanes
+// take 32 bytes of each of four rows, and chunk c of row k is at
+// c ^ (2 (k % 4) + k & 8), which spreads the eight rows of half a wave over
+// all banks.  fp32 operands are read one by one, four groups of lanes from
+// rows four apart: chunk c of row k is at c ^ 4 (k / 4 % 4).
 template <typename T>
 struct Stage {
   static constexpr int kE = 16 / (int)sizeof(T);  // elements of a chunk
   static constexpr int kK = 8 * kE;               // k of a stage
-  static constexpr int kElems = kTile * kK;
 };
 
 template <typename T>
-MHC_DEV int lds_at(int row, int chunk) { return (row * 8 + (chunk ^ (row & 7))) * Stage<T>::kE; }
-
-// a chunk of kE elements along k of row i (zeros past the ends)
-template <typename T, bool KMAJOR>
-MHC_DEV u32x4 fetch(const T* p, int64_t ld, int64_t i, int64_t rows, int64_t k, int64_t K) {
-  constexpr int kE = Stage<T>::kE;
-  u32x4 r = {0, 0, 0, 0};
-  if (i >= rows) return r;
-  if (KMAJOR && k + kE <= K) {
-    __builtin_memcpy(&r, p + i * ld + k, 16);
-    return r;
-  }
-  T v[kE];
-#pragma unroll
-  for (int j = 0; j < kE; ++j) v[j] = k + j < K ? (KMAJOR ? p[i * ld + k + j] : p[(k + j) * ld + i]) : (T)0;
-  __builtin_memcpy(&r, v, 16);
-  return r;
+MHC_DEV int row_key(int k) {
+  return sizeof(T) == 4 ? ((k >> 2) & 3) << 2 : ((k & 3) << 1) | (k & 8);
 }
 
-template <typename T, bool AK, bool BK>
-__global__ __launch_bounds__(kTileThreads) void tile_kernel(const Product p) {
+// Sixteen bytes a lane from memory to LDS, in the order of the lanes, without
+// passing through registers; past the end of `rs` zeros are stored.  In
+// assembly, since the compiler would wait for it before every LDS read.  The
+// caller waits (wait_loads) before the barrier that hands the stage over.
+MHC_DEV void load_to_lds(u32x4 rs, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rs), "s"(lds));
+}
+
+MHC_DEV void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+MHC_DEV uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+
+// One operand's side of a workgroup's tile: R indices from i0.
+template <typename T, bool KM, int R, int WAVES>
+struct Loader {
   using S = Stage<T>;
-  __shared__ T sa[S::kElems];
-  __shared__ T sb[S::kElems];
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const int64_t m0 = (int64_t)blockIdx.y * kTile, n0 = (int64_t)blockIdx.x * kTile;
-  const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-  f32x4 acc[4][4] = {};  // [n][m]: the first operand's index runs over a lane's four values
+  static constexpr int kLoads = R * 128 / 1024 / WAVES;  // of a wave, each 64 chunks
+  uint64_t base;
+  int64_t left;       // bytes from base to the operand's end
+  int64_t step;       // bytes of base from stage to stage
+  uint32_t off[kLoads];
+  uint32_t lds;       // of the wave's first chunk in a stage
+
+  MHC_DEV void init(const Operand& o, int64_t i0, int64_t count, int64_t k0, int64_t k1, int wave, int lane, uint32_t lds0) {
+    const int64_t ld = o.ld * (int64_t)sizeof(T);
+    if constexpr (KM) {
+      base = reinterpret_cast<uint64_t>(o.p) + (uint64_t)(i0 * ld + k0 * (int64_t)sizeof(T));
+      left = (count - i0 - 1) * ld + (o.width - k0) * (int64_t)sizeof(T);
+      step = 128;
+    } else {
+      base = reinterpret_cast<uint64_t>(o.p) + (uint64_t)(k0 * ld + i0 * (int64_t)sizeof(T));
+      left = (k1 - k0 - 1) * ld + (o.width - i0) * (int64_t)sizeof(T);
+      step = S::kK * ld;
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int at = (wave * kLoads + i) * 64 + lane;
+      if constexpr (KM) {
+        const int row = at >> 3;
+        off[i] = (uint32_t)(row * ld) + (((at & 7) ^ (row & 7)) << 4);
+      } else {
+        constexpr int kC = R / S::kE;  // chunks of a row
+        const int k = at / kC;
+        off[i] = (uint32_t)(k * ld) + (((at % kC) ^ row_key<T>(k)) << 4);
+      }
+    }
+    lds = lds0 + wave * kLoads * 1024;
+  }
+
+  // the stage at base; kleft: k from it to the end
+  MHC_DEV void load(uint32_t stage, int64_t kleft, int lane) const {
+    // (offsets of the tile stay below 2^31, see kMaxRowBytes)
+    const uint32_t n = left <= 0 ? 0u : left > 0x80000000ll ? 0x80000000u : (uint32_t)left;
+    const u32x4 rs = {(uint32_t)base, (uint32_t)(base >> 32) & 0xffffu, n, 0x00020000u};
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      uint32_t v = off[i];
+      if constexpr (KM) {  // in the last stage, chunks past the end of a row are the next row's
+        if (kleft < S::kK && ((lane & 7) ^ (lane >> 3)) * S::kE >= kleft) v = 0xfffffff0u;
+      }
+      load_to_lds(rs, v, lds + stage + i * 1024);
+    }
+  }
+
+  MHC_DEV void next() {
+    base += (uint64_t)step;
+    left -= step;
+  }
+};
+
+// A wave's fragments of one operand: J times 16 indices from w0 of a tile
+// R indices wide.  Lane l has index l % 16 and the k of group l / 16.
+template <typename T, bool KM, int R, int J>
+struct Reader {
+  using S = Stage<T>;
+  int at[KM ? 2 : J];
+
+  MHC_DEV void init(int w0, int lane) {
+    const int r = lane & 15, g = lane >> 4;
+    if constexpr (KM) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) at[s] = (w0 + r) * 128 + (((s * 4 + g) ^ (r & 7)) << 4);
+    } else if constexpr (sizeof(T) == 2) {
+      const int k = g * 8 + (r >> 2);
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int col = w0 + j * 16 + (r & 3) * 4;
+        at[j] = k * R * 2 + (((col >> 3) ^ row_key<T>(k)) << 4) + (col & 7) * 2;
+      }
+    } else {
+      const int k = g * 4;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int col = w0 + j * 16 + r;
+        at[j] = k * R * 4 + (((col >> 2) ^ row_key<T>(k)) << 4) + (col & 3) * 4;
+      }
+    }
+  }
+
+  // the fragment of step s (half a stage) and tile j
+  MHC_DEV u32x4 get(const char* stage, int s, int j) const {
+    if constexpr (KM) {
+      return *reinterpret_cast<const u32x4*>(stage + at[s] + j * 2048);
+    } else if constexpr (sizeof(T) == 2) {
+      typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+      const char* const p = stage + at[j] + s * 32 * R * 2;
+      // (32 k and 4 k further the key is the same)
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)p);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + 4 * R * 2));
+      const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
+      return u32x4{a.x, a.y, b.x, b.y};
+    } else {
+      u32x4 v;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const uint32_t*>(stage + at[j] + (s * 16 + k) * R * 4);
+      return v;
+    }
+  }
+};
+
+// The tile of a workgroup.  Workgroups go round the eight XCDs, each with an
+// L2 of its own: one XCD takes a run of consecutive tiles, in bands of eight
+// rows of tiles, so that its tiles share rows of A and B.
+MHC_DEV void tile_of(uint32_t id, uint32_t tm, uint32_t tn, uint32_t& m, uint32_t& n) {
+  const uint32_t total = tm * tn, per = total / 8, more = total % 8, xcd = id % 8;
+  const uint32_t t = xcd * per + min(xcd, more) + id / 8;
+  const uint32_t band = t / (8 * tn), first = band * 8, rows = min(8u, tm - first);
+  m = first + (t % (8 * tn)) % rows;
+  n = (t % (8 * tn)) / rows;
+}
+
+template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const Product p) {
+  using S = Stage<T>;
+  constexpr int kWaves = WM * WN, JM = BM / WM / 16, JN = BN / WN / 16;
+  constexpr int kA = BM * 128, kStage = kA + BN * 128;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * kStage];
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  uint32_t tm, tn;
+  tile_of(blockIdx.x, (uint32_t)ceil_div(p.M, BM), (uint32_t)ceil_div(p.N, BN), tm, tn);
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+  Loader<T, AK, BM, kWaves> la;
+  Loader<T, BK, BN, kWaves> lb;
+  const uint32_t lds = lds_address(smem);
+  la.init(p.a, m0, p.M, 0, p.K, wave, lane, lds);
+  lb.init(p.b, n0, p.N, 0, p.K, wave, lane, lds + kA);
+  Reader<T, AK, BM, JM> ra;
+  Reader<T, BK, BN, JN> rb;
+  ra.init(wm, lane);
+  rb.init(wn, lane);
+  f32x4 acc[JN][JM] = {};  // the first operand's index, n, runs over a lane's four values
+  la.load(0, p.K, lane);
+  lb.load(0, p.K, lane);
+  int cur = 0;
   for (int64_t k0 = 0; k0 < p.K; k0 += S::kK) {
-    u32x4 ra[4], rb[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int row = j * 32 + tid / 8, chunk = tid % 8;
-      ra[j] = fetch<T, AK>(static_cast<const T*>(p.a), p.lda, m0 + row, p.M, k0 + chunk * S::kE, p.K);
-      rb[j] = fetch<T, BK>(static_cast<const T*>(p.b), p.ldb, n0 + row, p.N, k0 + chunk * S::kE, p.K);
+    wait_loads();
+    __syncthreads();  // every wave's part of this stage is there, and nobody reads the other one any more
+    if (k0 + S::kK < p.K) {
+      la.next();
+      lb.next();
+      la.load((cur ^ 1) * kStage, p.K - k0 - S::kK, lane);
+      lb.load((cur ^ 1) * kStage, p.K - k0 - S::kK, lane);
     }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int row = j * 32 + tid / 8, chunk = tid % 8;
-      *reinterpret_cast<u32x4*>(sa + lds_at<T>(row, chunk)) = ra[j];
-      *reinterpret_cast<u32x4*>(sb + lds_at<T>(row, chunk)) = rb[j];
-    }
-    __syncthreads();
+    const char* const sa = smem + cur * kStage;
+    const char* const sb = sa + kA;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      u32x4 fa[4], fb[4];
+      u32x4 fa[JM], fb[JN];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        fa[j] = *reinterpret_cast<const u32x4*>(sa + lds_at<T>(wm + j * 16 + lane % 16, s * 4 + lane / 16));
-        fb[j] = *reinterpret_cast<const u32x4*>(sb + lds_at<T>(wn + j * 16 + lane % 16, s * 4 + lane / 16));
+      for (int j = 0; j < JN; ++j) fb[j] = rb.get(sb, s, j);
+#pragma unroll
+      for (int j = 0; j < JM; ++j) fa[j] = ra.get(sa, s, j);
+#pragma unroll
+      for (int j = 0; j < JM; ++j)
+#pragma unroll
+        for (int i = 0; i < JN; ++i) acc[i][j] = mfma16<T>(fb[i], fa[j], acc[i][j]);
+    }
+    cur ^= 1;
+  }
+  // The sums go through LDS, where each wave has 16 KB for 64 rows of 64
+  // columns, so that rows of the outputs are written as whole vectors of
+  // consecutive lanes.  The 16-byte chunk c of row r is at c ^ (r % 16).
+  static_assert(JN == 4 && JM % 4 == 0 && kWaves * 16384 <= 2 * kStage, "64 columns a wave");
+  char* const mine = smem + wave * 16384;
+#pragma unroll
+  for (int h = 0; h < JM; h += 4) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < JN; ++i)
+        *reinterpret_cast<f32x4*>(mine + (j * 16 + lane % 16) * 256 + (((i * 4 + lane / 16) ^ (lane % 16)) << 4)) = acc[i][h + j];
+    __syncthreads();
+    const int64_t mh = m0 + wm + h * 16;
+    if (p.e.vec) {
+      const int c = lane % 8 * 2;
+      const int64_t n = n0 + wn + c * 4;
+      for (int r = lane / 8; r < 64; r += 8) {
+        const f32x4 u = *reinterpret_cast<const f32x4*>(mine + r * 256 + ((c ^ (r % 16)) << 4));
+        const f32x4 v = *reinterpret_cast<const f32x4*>(mine + r * 256 + (((c + 1) ^ (r % 16)) << 4));
+        float z[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
+        if (mh + r < p.M && n < p.N) finish<T>(p.e, mh + r, n, p.N, z);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = mfma16<T>(fb[i], fa[j], acc[i][j]);
+    } else {
+      const int64_t n = n0 + wn + lane;
+      for (int r = 0; r < 64; ++r) {
+        float z[1] = {*reinterpret_cast<const float*>(mine + r * 256 + (((lane / 4) ^ (r % 16)) << 4) + lane % 4 * 4)};
+        if (mh + r < p.M && n < p.N) finish<T>(p.e, mh + r, n, p.N, z);
+      }
     }
   }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int64_t m = m0 + wm + j * 16 + lane % 16;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t n = n0 + wn + i * 16 + lane / 16 * 4;
-      if (m < p.M && n < p.N) {
-        float z[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-        finish<T, 4>(p.e, m, n, p.N, z, p.e.vec != 0);
-      }
-    }
-  }
+}
+
+template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN>
+int launch_tile(const Product& p, hipStream_t s) {
+  const int64_t tiles = ceil_div(p.M, BM) * ceil_div(p.N, BN);
+  hipLaunchKernelGGL((tile_kernel<T, AK, BK, BM, BN, WM, WN>), dim3((unsigned)tiles), dim3(64 * WM * WN), 0, s, p);
+  MHC_CHECK_LAUNCH("tile_kernel");
+  return MHC_OK;
+}
+
+// 256 x 256 where its tiles keep most of the CUs busy (each workgroup takes a
+// whole one), else 128 x 128.
+template <typename T, bool AK, bool BK>
+int run_layout(const Product& p, hipStream_t s) {
+  const int64_t big = ceil_div(p.M, 256) * ceil_div(p.N, 256), cus = device_cu_count();
+  if (big * 8 >= cus * 6) return launch_tile<T, AK, BK, 256, 256, 2, 4>(p, s);
+  return launch_tile<T, AK, BK, 128, 128, 2, 2>(p, s);
 }
 
 // The product of one type; a_k / b_k: the operand's k are contiguous.
 template <typename T>
 int run_product(const Product& p, bool a_k, bool b_k, hipStream_t s) {
-  const dim3 grid((unsigned)ceil_div(p.N, kTile), (unsigned)ceil_div(p.M, kTile));
-  if (a_k && b_k) hipLaunchKernelGGL((tile_kernel<T, true, true>), grid, dim3(kTileThreads), 0, s, p);
-  else if (a_k) hipLaunchKernelGGL((tile_kernel<T, true, false>), grid, dim3(kTileThreads), 0, s, p);
-  else hipLaunchKernelGGL((tile_kernel<T, false, false>), grid, dim3(kTileThreads), 0, s, p);
-  MHC_CHECK_LAUNCH("tile_kernel");
-  return MHC_OK;
+  if (a_k && b_k) return run_layout<T, true, true>(p, s);
+  if (a_k) return run_layout<T, true, false>(p, s);
+  return run_layout<T, false, false>(p, s);
 }
 
 int run_product_f32(const Product& p, bool a_k, bool b_k, hipStream_t s);

@@ -127,11 +127,11 @@ std::tuple<at::Tensor, at::Tensor> linear_fwd(const at::Tensor& x, const at::Ten
   const int code = dtype_code(x.scalar_type(), "x");
   const auto plain = x.options().requires_grad(false);
   at::Tensor out = at::empty(s.out, plain.dtype(scalar_type(out_code))), dact;
-  if (want_dact && act != MHC_ACT_NONE) dact = at::empty({s.M, s.N}, plain.dtype(code == MHC_DTYPE_F32 ? at::kFloat : at::kHalf));
+  if (want_dact && act != MHC_ACT_NONE) dact = at::empty({s.M, s.N}, plain.dtype(code == MHC_DTYPE_F32 ? at::kFloat : at::kShort));
   if (s.M == 0) return {out, dact};
   const at::Tensor xr = rows_of(x, s.K), wr = rows_of(w, s.K);
   const at::Tensor b = bias.defined() ? bias.contiguous() : bias, r = residual.defined() ? residual.contiguous() : residual;
-  const size_t nb = mhc_linear_act_fwd_workspace_bytes(s.M, s.N, s.K, code);
+  const size_t nb = mhc_linear_act_fwd_workspace_bytes(xr.data_ptr(), row_stride(xr), wr.data_ptr(), row_stride(wr), s.M, s.N, s.K, code);
   const at::Tensor ws = nb > 0 ? workspace(nb, x) : at::Tensor();
   check(mhc_linear_act_fwd(xr.data_ptr(), row_stride(xr), wr.data_ptr(), row_stride(wr), ptr(b), ptr(r), out.data_ptr(),
                            (int)out_code, ptr(dact), (int)act, s.M, s.N, s.K, code, ptr(ws), nb, stream_of(x)),
@@ -160,7 +160,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_bwd(const at::Tensor& dout
   const at::Tensor dact = get(dact_), xr = rows_of(x, K), wr = rows_of(w, K);
   const at::Tensor g = (dout.scalar_type() == x.scalar_type() ? dout : dout.to(at::kFloat)).contiguous();
   const int gc = dtype_code(g.scalar_type(), "dout");
-  const size_t nb = mhc_linear_act_bwd_workspace_bytes(M, N, K, code, gc, dact.defined(), want_dx, want_dw, want_db);
+  const size_t nb = mhc_linear_act_bwd_workspace_bytes(g.data_ptr(), gc, ptr(dact), xr.data_ptr(), row_stride(xr), wr.data_ptr(),
+                                                       row_stride(wr), want_dx, want_dw, want_db, M, N, K, code);
   const at::Tensor ws = workspace(nb, x);
   check(mhc_linear_act_bwd(g.data_ptr(), gc, ptr(dact), xr.data_ptr(), row_stride(xr), wr.data_ptr(), row_stride(wr), ptr(dx),
                            ptr(dw), ptr(db), M, N, K, code, ws.data_ptr(), nb, stream_of(x)),

@@ -108,10 +108,11 @@ SIGNATURES = {
     "mhc_policy_loss_fwd": ([_PPOL, _VP, _VP, _VP, _VP, _SZ, _VP], _I32),
     "mhc_policy_loss_bwd": ([_PPOL, _VP, _VP, _VP, _VP], _I32),
     "mhc_policy_loss_fwd_bwd": ([_PPOL, _F32, _VP, _VP, _VP, _VP, _SZ, _VP], _I32),
-    "mhc_linear_act_fwd_workspace_bytes": ([_I64, _I64, _I64, _I32], _SZ),
+    "mhc_linear_act_fwd_workspace_bytes": ([_VP, _I64, _VP, _I64, _I64, _I64, _I64, _I32], _SZ),
     "mhc_linear_act_fwd": ([_VP, _I64, _VP, _I64, _VP, _VP, _VP, _I32, _VP, _I32, _I64, _I64, _I64, _I32, _VP, _SZ, _VP],
                            _I32),
-    "mhc_linear_act_bwd_workspace_bytes": ([_I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _I32], _SZ),
+    "mhc_linear_act_bwd_workspace_bytes": ([_VP, _I32, _VP, _VP, _I64, _VP, _I64, _I32, _I32, _I32, _I64, _I64, _I64, _I32],
+                                           _SZ),
     "mhc_linear_act_bwd": ([_VP, _I32, _VP, _VP, _I64, _VP, _I64, _VP, _VP, _VP, _I64, _I64, _I64, _I32, _VP, _SZ, _VP],
                            _I32),
 }

@@ -49,14 +49,13 @@ def linear64(x, w, b, r, act, out_dtype):
 
 
 def linear_grads64(x, w, g, d, dz, dtype, has_act):
-    """((dx, bound), (dw, bound), (db, bound)): dz is rounded to dtype, act' to fp16 (fp32 for fp32)."""
+    """((dx, bound), (dw, bound), (db, bound)): dz is rounded to dtype, act' to 2^-15 steps (fp32 for fp32)."""
     x, w, g = x.detach().double(), w.detach().double(), g.double()
     t = g * d
     # |act''| <= 1; act' takes a few roundings of values up to 2
     off = g.abs() * (dz + 32 * U32) + t.abs() * 4 * U32
     if has_act:
-        half = torch.float32 if dtype == torch.float32 else torch.float16
-        off = off + t.abs() * UNIT[half] + g.abs() * LEAST[half]
+        off = off + (t.abs() * U32 if dtype == torch.float32 else g.abs() * 2.0 ** -16)
     sum_off = off
     off = off + t.abs() * 1.01 * UNIT[dtype] + LEAST[dtype]
     M, N = t.shape

@@ -183,4 +183,4 @@ def test_linear_rejects_bad_arguments_on_the_host(lib):
 
     for bad in [dict(g=None), dict(x=None), dict(w=None), dict(gdt=2), dict(ldx=63), dict(M=0), dict(ws=None), dict(nb=0), dict(ws=257)]:
         assert bwd(**bad) == -1, bad
-    assert lib.mhc_linear_act_bwd_workspace_bytes(0, 8, 64, 1, 1, 0, 1, 1, 1) == 0
+    assert lib.mhc_linear_act_bwd_workspace_bytes(16, 1, None, 16, 64, 16, 64, 1, 1, 1, 0, 8, 64, 1) == 0
