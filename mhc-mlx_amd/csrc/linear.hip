@@ -78,10 +78,19 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* src, int64_t ld, T* 
 
 int elem_bytes(int dtype) { return dtype == kF32 ? 4 : 2; }
 
-int run_product(const Product& p, bool a_k, bool b_k, int dtype, hipStream_t s) {
-  if (dtype == kF32) return gemm::run_product_f32(p, a_k, b_k, s);
-  if (dtype == kBF16) return gemm::run_product_bf16(p, a_k, b_k, s);
-  return gemm::run_product_f16(p, a_k, b_k, s);
+// ws: part_bytes of the product
+int run_product(const Product& p, bool a_k, bool b_k, int dtype, char* ws, hipStream_t s) {
+  const gemm::Cut c = gemm::cut_of(p.M, p.N, p.K, dtype);
+  float* const part = reinterpret_cast<float*>(ws);
+  if (dtype == kF32) return gemm::run_product_f32(p, a_k, b_k, c, part, s);
+  if (dtype == kBF16) return gemm::run_product_bf16(p, a_k, b_k, c, part, s);
+  return gemm::run_product_f16(p, a_k, b_k, c, part, s);
+}
+
+// bytes of the sums of a product whose reduction is split
+size_t part_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
+  const gemm::Cut c = gemm::cut_of(M, N, K, dtype);
+  return c.splits > 1 ? (size_t)(c.splits * M * N) * sizeof(float) : 0;
 }
 
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
@@ -123,7 +132,7 @@ int operand(Operand& o, const void* p, int64_t rows, int64_t ld, int64_t width, 
 }
 
 struct BwdPlan {
-  size_t dz, part, x, w, total;  // bytes
+  size_t dz, part, x, w, total;  // bytes; the products' sums, one after the other, come last
 };
 
 BwdPlan plan_bwd(const void* dout, int dout_dtype, bool dact, const void* x, int64_t ldx, const void* w, int64_t ldw, bool dx, bool dw,
@@ -134,7 +143,8 @@ BwdPlan plan_bwd(const void* dout, int dout_dtype, bool dact, const void* x, int
   if (db) b.part = up256((size_t)(ceil_div(M, kDzRows) * N) * sizeof(float));
   if (dx) b.w = pack_bytes(w, N, ldw, K, dtype);
   if (dw) b.x = pack_bytes(x, M, ldx, K, dtype);
-  b.total = b.dz + b.part + b.x + b.w;
+  b.total = b.dz + b.part + b.x + b.w +
+            std::max(dx ? part_bytes(M, K, N, dtype) : 0, dw ? part_bytes(N, K, M, dtype) : 0);
   return b;
 }
 
@@ -166,7 +176,7 @@ int check_shape(int64_t M, int64_t N, int64_t K, int dtype) {
 extern "C" size_t mhc_linear_act_fwd_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M,
                                                      int64_t N, int64_t K, int dtype) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  return mhc::pack_bytes(x, M, ldx, K, dtype) + mhc::pack_bytes(w, N, ldw, K, dtype);
+  return mhc::pack_bytes(x, M, ldx, K, dtype) + mhc::pack_bytes(w, N, ldw, K, dtype) + mhc::part_bytes(M, N, K, dtype);
 }
 
 extern "C" int mhc_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
@@ -186,10 +196,10 @@ extern "C" int mhc_linear_act_fwd(const void* x, int64_t ldx, const void* w, int
   MHC_CHECK_ARG(aligned(workspace, 16), "workspace must be 16-byte aligned");
   hipStream_t s = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
-  Product p = {{}, {}, M, N, K, gemm::epilogue(bias, residual, out, dact, act, out_dtype, dtype, N)};
+  Product p = {{}, {}, M, N, K, gemm::epilogue(bias, residual, out, dact, act, out_dtype, dtype, N), 1, 0};
   if (const int rc = operand(p.a, x, M, ldx, K, dtype, ws, s)) return rc;
   if (const int rc = operand(p.b, w, N, ldw, K, dtype, ws, s)) return rc;
-  return run_product(p, true, true, dtype, s);
+  return run_product(p, true, true, dtype, ws, s);
 }
 
 extern "C" size_t mhc_linear_act_bwd_workspace_bytes(const void* dout, int dout_dtype, const void* dact, const void* x,
@@ -232,14 +242,14 @@ extern "C" int mhc_linear_act_bwd(const void* dout, int dout_dtype, const void* 
   ws += b.dz + b.part;
   const Operand g = dz != nullptr ? Operand{dz, padded(N, dtype), padded(N, dtype)} : Operand{dout, N, N};
   if (dx != nullptr) {  // dx[m, k] = sum_n dz[m, n] W[n, k]
-    Product p = {g, {}, M, K, N, gemm::epilogue(nullptr, nullptr, dx, nullptr, MHC_ACT_NONE, dtype, dtype, K)};
+    Product p = {g, {}, M, K, N, gemm::epilogue(nullptr, nullptr, dx, nullptr, MHC_ACT_NONE, dtype, dtype, K), 1, 0};
     if (const int rc = operand(p.b, w, N, ldw, K, dtype, ws, s)) return rc;
-    if (const int rc = run_product(p, true, false, dtype, s)) return rc;
+    if (const int rc = run_product(p, true, false, dtype, ws + (dw != nullptr ? b.x : 0), s)) return rc;
   }
   if (dw != nullptr) {  // dw[n, k] = sum_m dz[m, n] x[m, k]
-    Product p = {g, {}, N, K, M, gemm::epilogue(nullptr, nullptr, dw, nullptr, MHC_ACT_NONE, dtype, dtype, K)};
+    Product p = {g, {}, N, K, M, gemm::epilogue(nullptr, nullptr, dw, nullptr, MHC_ACT_NONE, dtype, dtype, K), 1, 0};
     if (const int rc = operand(p.b, x, M, ldx, K, dtype, ws, s)) return rc;
-    if (const int rc = run_product(p, false, false, dtype, s)) return rc;
+    if (const int rc = run_product(p, false, false, dtype, ws, s)) return rc;
   }
   return MHC_OK;
 }

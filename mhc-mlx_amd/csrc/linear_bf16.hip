@@ -4,7 +4,9 @@
 namespace mhc {
 namespace gemm {
 
-int run_product_bf16(const Product& p, bool a_k, bool b_k, hipStream_t s) { return run_product<__bf16>(p, a_k, b_k, s); }
+int run_product_bf16(const Product& p, bool a_k, bool b_k, const Cut& c, float* part, hipStream_t s) {
+  return run_product<__bf16>(p, a_k, b_k, c, part, s);
+}
 
 }  // namespace gemm
 }  // namespace mhc

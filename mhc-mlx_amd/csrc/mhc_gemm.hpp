@@ -174,6 +174,8 @@ struct Product {
   Operand a, b;
   int64_t M, N, K;
   Epilogue e;
+  int splits;   // of the reduction, each of kper k; more than one: `out` of the epilogue holds the sums of each
+  int kper;     // a multiple of a stage
 };
 
 // LDS holds an operand's tile of a stage, 128 bytes of k for each index, in
@@ -208,7 +210,9 @@ MHC_DEV void load_to_lds(u32x4 rs, uint32_t voff, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rs), "s"(lds));
 }
 
-MHC_DEV void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// until at most N of the wave's loads are under way
+template <int N>
+MHC_DEV void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
 MHC_DEV uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
@@ -252,7 +256,7 @@ struct Loader {
   }
 
   // the stage at base; kleft: k from it to the end
-  MHC_DEV void load(uint32_t stage, int64_t kleft, int lane) const {
+  MHC_DEV void load(uint32_t stage, int kleft, int lane) const {
     // (offsets of the tile stay below 2^31, see kMaxRowBytes)
     const uint32_t n = left <= 0 ? 0u : left > 0x80000000ll ? 0x80000000u : (uint32_t)left;
     const u32x4 rs = {(uint32_t)base, (uint32_t)(base >> 32) & 0xffffu, n, 0x00020000u};
@@ -322,6 +326,39 @@ struct Reader {
   }
 };
 
+// A wave's fragments of half a stage, and their products.
+template <int JM, int JN>
+struct Fragments {
+  u32x4 a[JM], b[JN];
+
+  template <typename RA, typename RB>
+  MHC_DEV void read(const RA& ra, const RB& rb, const char* sa, const char* sb, int s) {
+#pragma unroll
+    for (int j = 0; j < JN; ++j) b[j] = rb.get(sb, s, j);
+#pragma unroll
+    for (int j = 0; j < JM; ++j) a[j] = ra.get(sa, s, j);
+  }
+
+  template <typename T>
+  MHC_DEV void multiply(f32x4 (&acc)[JN][JM]) const {
+#pragma unroll
+    for (int j = 0; j < JM; ++j)
+#pragma unroll
+      for (int i = 0; i < JN; ++i) acc[i][j] = mfma16<T>(b[i], a[j], acc[i][j]);
+  }
+};
+
+// Spreads READS LDS reads evenly over PRODUCTS matrix instructions.
+template <int READS, int PRODUCTS>
+MHC_DEV void interleave() {
+#pragma unroll
+  for (int r = 0; r < READS; ++r) {
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    constexpr int kEach = PRODUCTS / READS > 0 ? PRODUCTS / READS : 1;
+    __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
+  }
+}
+
 // The tile of a workgroup.  Workgroups go round the eight XCDs, each with an
 // L2 of its own: one XCD takes a run of consecutive tiles, in bands of eight
 // rows of tiles, so that its tiles share rows of A and B.
@@ -333,117 +370,184 @@ MHC_DEV void tile_of(uint32_t id, uint32_t tm, uint32_t tn, uint32_t& m, uint32_
   n = (t % (8 * tn)) / rows;
 }
 
-template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN>
+template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
 __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const Product p) {
   using S = Stage<T>;
   constexpr int kWaves = WM * WN, JM = BM / WM / 16, JN = BN / WN / 16;
   constexpr int kA = BM * 128, kStage = kA + BN * 128;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * kStage];
+  __shared__ __attribute__((aligned(1024))) char smem[NS * kStage];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   uint32_t tm, tn;
   tile_of(blockIdx.x, (uint32_t)ceil_div(p.M, BM), (uint32_t)ceil_div(p.N, BN), tm, tn);
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+  const int k0 = (int)blockIdx.y * p.kper, k1 = min((int)p.K, k0 + p.kper);
   Loader<T, AK, BM, kWaves> la;
   Loader<T, BK, BN, kWaves> lb;
+  constexpr int kLoads = decltype(la)::kLoads + decltype(lb)::kLoads;
   const uint32_t lds = lds_address(smem);
-  la.init(p.a, m0, p.M, 0, p.K, wave, lane, lds);
-  lb.init(p.b, n0, p.N, 0, p.K, wave, lane, lds + kA);
+  la.init(p.a, m0, p.M, k0, k1, wave, lane, lds);
+  lb.init(p.b, n0, p.N, k0, k1, wave, lane, lds + kA);
   Reader<T, AK, BM, JM> ra;
   Reader<T, BK, BN, JN> rb;
   ra.init(wm, lane);
   rb.init(wn, lane);
   f32x4 acc[JN][JM] = {};  // the first operand's index, n, runs over a lane's four values
-  la.load(0, p.K, lane);
-  lb.load(0, p.K, lane);
-  int cur = 0;
-  for (int64_t k0 = 0; k0 < p.K; k0 += S::kK) {
-    wait_loads();
-    __syncthreads();  // every wave's part of this stage is there, and nobody reads the other one any more
-    if (k0 + S::kK < p.K) {
-      la.next();
-      lb.next();
-      la.load((cur ^ 1) * kStage, p.K - k0 - S::kK, lane);
-      lb.load((cur ^ 1) * kStage, p.K - k0 - S::kK, lane);
-    }
-    const char* const sa = smem + cur * kStage;
-    const char* const sb = sa + kA;
+  // The fragments of half a stage are read while the products of the half
+  // before are formed; in the middle of a stage its last reads are done, so
+  // that the barrier there frees its place and hands over the next one.
+  // NS stages are under way.  (Those past the end read nothing: every pass
+  // issues the same number of loads.)
+  int kleft = k1 - k0;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      u32x4 fa[JM], fb[JN];
-#pragma unroll
-      for (int j = 0; j < JN; ++j) fb[j] = rb.get(sb, s, j);
-#pragma unroll
-      for (int j = 0; j < JM; ++j) fa[j] = ra.get(sa, s, j);
-#pragma unroll
-      for (int j = 0; j < JM; ++j)
-#pragma unroll
-        for (int i = 0; i < JN; ++i) acc[i][j] = mfma16<T>(fb[i], fa[j], acc[i][j]);
-    }
-    cur ^= 1;
+  for (int q = 0; q < NS; ++q) {
+    la.load(q * kStage, kleft - q * S::kK, lane);
+    lb.load(q * kStage, kleft - q * S::kK, lane);
+    la.next();
+    lb.next();
   }
-  // The sums go through LDS, where each wave has 16 KB for 64 rows of 64
-  // columns, so that rows of the outputs are written as whole vectors of
+  wait_loads<(NS - 1) * kLoads>();
+  __syncthreads();
+  int cur = 0;
+  Fragments<JM, JN> f0, f1;
+  f0.read(ra, rb, smem, smem + kA, 0);
+  for (; kleft > 0; kleft -= S::kK) {
+    f1.read(ra, rb, smem + cur, smem + cur + kA, 1);
+    f0.template multiply<T>(acc);
+    interleave<(JM * (AK ? 1 : S::kE / 4) + JN * (BK ? 1 : S::kE / 4)), JM * JN * (sizeof(T) == 4 ? 4 : 1)>();
+    wait_loads<(NS - 2) * kLoads>();
+    __syncthreads();
+    la.load(cur, kleft - NS * S::kK, lane);
+    lb.load(cur, kleft - NS * S::kK, lane);
+    la.next();
+    lb.next();
+    cur = cur == (NS - 1) * kStage ? 0 : cur + kStage;
+    f0.read(ra, rb, smem + cur, smem + cur + kA, 0);
+    f1.template multiply<T>(acc);
+    interleave<(JM * (AK ? 1 : S::kE / 4) + JN * (BK ? 1 : S::kE / 4)), JM * JN * (sizeof(T) == 4 ? 4 : 1)>();
+  }
+  wait_loads<0>();  // (the last ones store zeros where the sums go next)
+  Epilogue e = p.e;
+  if (p.splits > 1) e.out = static_cast<float*>(e.out) + (int64_t)blockIdx.y * p.M * p.N;
+  // The sums go through LDS, where each wave has room for up to 64 rows
+  // of 64 columns, so that rows of the outputs are written as whole vectors of
   // consecutive lanes.  The 16-byte chunk c of row r is at c ^ (r % 16).
-  static_assert(JN == 4 && JM % 4 == 0 && kWaves * 16384 <= 2 * kStage, "64 columns a wave");
-  char* const mine = smem + wave * 16384;
+  constexpr int kFit = NS * kStage / (kWaves * 4096);  // sets of 16 rows that every wave has room for
+  constexpr int kRound = JM >= 4 && kFit >= 4 ? 4 : JM >= 2 && kFit >= 2 ? 2 : 1, kRows = kRound * 16;
+  static_assert(JN == 4 && JM % kRound == 0 && kFit >= 1, "64 columns a wave");
+  char* const mine = smem + wave * kRows * 256;
 #pragma unroll
-  for (int h = 0; h < JM; h += 4) {
+  for (int h = 0; h < JM; h += kRound) {
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < kRound; ++j)
 #pragma unroll
       for (int i = 0; i < JN; ++i)
         *reinterpret_cast<f32x4*>(mine + (j * 16 + lane % 16) * 256 + (((i * 4 + lane / 16) ^ (lane % 16)) << 4)) = acc[i][h + j];
     __syncthreads();
     const int64_t mh = m0 + wm + h * 16;
-    if (p.e.vec) {
+    if (e.vec) {
       const int c = lane % 8 * 2;
       const int64_t n = n0 + wn + c * 4;
-      for (int r = lane / 8; r < 64; r += 8) {
+      for (int r = lane / 8; r < kRows; r += 8) {
         const f32x4 u = *reinterpret_cast<const f32x4*>(mine + r * 256 + ((c ^ (r % 16)) << 4));
         const f32x4 v = *reinterpret_cast<const f32x4*>(mine + r * 256 + (((c + 1) ^ (r % 16)) << 4));
         float z[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
-        if (mh + r < p.M && n < p.N) finish<T>(p.e, mh + r, n, p.N, z);
+        if (mh + r < p.M && n < p.N) finish<T>(e, mh + r, n, p.N, z);
       }
     } else {
       const int64_t n = n0 + wn + lane;
-      for (int r = 0; r < 64; ++r) {
+      for (int r = 0; r < kRows; ++r) {
         float z[1] = {*reinterpret_cast<const float*>(mine + r * 256 + (((lane / 4) ^ (r % 16)) << 4) + lane % 4 * 4)};
-        if (mh + r < p.M && n < p.N) finish<T>(p.e, mh + r, n, p.N, z);
+        if (mh + r < p.M && n < p.N) finish<T>(e, mh + r, n, p.N, z);
       }
     }
   }
 }
 
-template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN>
+// The sum over the splits, in order, and the epilogue.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void join_kernel(const float* part, int splits, int64_t M, int64_t N, const Epilogue e) {
+  const int64_t total = M * N / V;
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * 256) {
+    const int64_t m = at * V / N, n = at * V % N;
+    float z[V] = {};
+    for (int k = 0; k < splits; ++k) {
+      const float* const p = part + ((int64_t)k * M + m) * N + n;
+      if constexpr (V == 1) z[0] += *p;
+      else add(p, z);
+    }
+    finish<T>(e, m, n, N, z);
+  }
+}
+
+template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
 int launch_tile(const Product& p, hipStream_t s) {
   const int64_t tiles = ceil_div(p.M, BM) * ceil_div(p.N, BN);
-  hipLaunchKernelGGL((tile_kernel<T, AK, BK, BM, BN, WM, WN>), dim3((unsigned)tiles), dim3(64 * WM * WN), 0, s, p);
+  hipLaunchKernelGGL((tile_kernel<T, AK, BK, BM, BN, WM, WN, NS>), dim3((unsigned)tiles, (unsigned)p.splits),
+                     dim3(64 * WM * WN), 0, s, p);
   MHC_CHECK_LAUNCH("tile_kernel");
   return MHC_OK;
 }
 
-// 256 x 256 where its tiles keep most of the CUs busy (each workgroup takes a
-// whole one), else 128 x 128.
-template <typename T, bool AK, bool BK>
-int run_layout(const Product& p, hipStream_t s) {
-  const int64_t big = ceil_div(p.M, 256) * ceil_div(p.N, 256), cus = device_cu_count();
-  if (big * 8 >= cus * 6) return launch_tile<T, AK, BK, 256, 256, 2, 4>(p, s);
-  return launch_tile<T, AK, BK, 128, 128, 2, 2>(p, s);
-}
-
-// The product of one type; a_k / b_k: the operand's k are contiguous.
 template <typename T>
-int run_product(const Product& p, bool a_k, bool b_k, hipStream_t s) {
-  if (a_k && b_k) return run_layout<T, true, true>(p, s);
-  if (a_k) return run_layout<T, true, false>(p, s);
-  return run_layout<T, false, false>(p, s);
+int launch_join(const Epilogue& e, const float* part, int splits, int64_t M, int64_t N, hipStream_t s) {
+  const int V = e.vec ? 8 : 1;
+  const unsigned blocks = (unsigned)std::min(ceil_div(M * N / V, 256), (int64_t)device_cu_count() * 16);
+  if (e.vec) hipLaunchKernelGGL((join_kernel<T, 8>), dim3(blocks), dim3(256), 0, s, part, splits, M, N, e);
+  else hipLaunchKernelGGL((join_kernel<T, 1>), dim3(blocks), dim3(256), 0, s, part, splits, M, N, e);
+  MHC_CHECK_LAUNCH("join_kernel");
+  return MHC_OK;
 }
 
-int run_product_f32(const Product& p, bool a_k, bool b_k, hipStream_t s);
-int run_product_bf16(const Product& p, bool a_k, bool b_k, hipStream_t s);
-int run_product_f16(const Product& p, bool a_k, bool b_k, hipStream_t s);
+template <typename T, bool AK, bool BK>
+int run_layout(const Product& p, int tile, hipStream_t s) {
+  switch (tile) {
+    case 0: return launch_tile<T, AK, BK, 256, 256, 2, 4, 2>(p, s);
+    case 1: return launch_tile<T, AK, BK, 128, 128, 2, 2, 2>(p, s);
+    case 2: return launch_tile<T, AK, BK, 128, 128, 2, 2, 4>(p, s);
+    case 3: return launch_tile<T, AK, BK, 64, 128, 2, 2, 3>(p, s);
+    case 4: return launch_tile<T, AK, BK, 64, 128, 2, 2, 6>(p, s);
+    case 5: return launch_tile<T, AK, BK, 128, 128, 2, 2, 3>(p, s);
+    default: return launch_tile<T, AK, BK, 128, 256, 2, 4, 2>(p, s);
+  }
+}
+
+// How a product is cut up: its tile, and into how many parts its reduction.
+struct Cut {
+  int tile, splits, kper;
+};
+
+inline Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype) {
+  const char* t = getenv("X_TILE");
+  const char* sp = getenv("X_SPLIT");
+  const int kK = dtype == kF32 ? 32 : 64;
+  const int64_t big = ceil_div(M, 256) * ceil_div(N, 256), cus = device_cu_count();
+  Cut c = {t ? atoi(t) : big * 8 >= cus * 6 ? 0 : 1, sp ? atoi(sp) : 1, 0};
+  const int64_t stages = ceil_div(K, kK);
+  c.splits = (int)std::min<int64_t>(c.splits, stages);
+  c.kper = (int)(ceil_div(stages, c.splits) * kK);
+  c.splits = (int)ceil_div(K, c.kper);
+  return c;
+}
+
+// The product of one type; a_k / b_k: the operand's k are contiguous.  part: splits * M * N floats where it is split.
+template <typename T>
+int run_product(Product p, bool a_k, bool b_k, const Cut& c, float* part, hipStream_t s) {
+  const Epilogue e = p.e;
+  p.splits = c.splits;
+  p.kper = c.kper;
+  if (c.splits > 1) p.e = Epilogue{nullptr, nullptr, part, nullptr, MHC_ACT_NONE, 1, p.N % 8 == 0};
+  const int rc = a_k && b_k ? run_layout<T, true, true>(p, c.tile, s)
+                 : a_k      ? run_layout<T, true, false>(p, c.tile, s)
+                            : run_layout<T, false, false>(p, c.tile, s);
+  if (rc != MHC_OK || c.splits == 1) return rc;
+  return launch_join<T>(e, part, c.splits, p.M, p.N, s);
+}
+
+int run_product_f32(const Product& p, bool a_k, bool b_k, const Cut& c, float* part, hipStream_t s);
+int run_product_bf16(const Product& p, bool a_k, bool b_k, const Cut& c, float* part, hipStream_t s);
+int run_product_f16(const Product& p, bool a_k, bool b_k, const Cut& c, float* part, hipStream_t s);
 
 }  // namespace gemm
 }  // namespace mhc
