@@ -93,6 +93,12 @@ size_t part_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
   return c.splits > 1 ? (size_t)(c.splits * M * N) * sizeof(float) : 0;
 }
 
+// Up to 64 rows of x go to the kernel that only streams W.
+bool few_rows(int64_t M, int64_t N, int64_t K, int dtype) {
+  const char* t = getenv("X_FEW");
+  return M <= (t ? atoi(t) : 64);
+}
+
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
 int64_t padded(int64_t width, int dtype) {
@@ -175,7 +181,7 @@ int check_shape(int64_t M, int64_t N, int64_t K, int dtype) {
 
 extern "C" size_t mhc_linear_act_fwd_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M,
                                                      int64_t N, int64_t K, int dtype) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || mhc::few_rows(M, N, K, dtype)) return 0;
   return mhc::pack_bytes(x, M, ldx, K, dtype) + mhc::pack_bytes(w, N, ldw, K, dtype) + mhc::part_bytes(M, N, K, dtype);
 }
 
@@ -196,6 +202,12 @@ extern "C" int mhc_linear_act_fwd(const void* x, int64_t ldx, const void* w, int
   MHC_CHECK_ARG(aligned(workspace, 16), "workspace must be 16-byte aligned");
   hipStream_t s = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
+  if (few_rows(M, N, K, dtype)) {
+    const gemm::Epilogue e = gemm::epilogue(bias, residual, out, dact, act, out_dtype, dtype, N);
+    if (dtype == kF32) return gemm::run_few_rows_f32(x, ldx, w, ldw, M, N, K, e, s);
+    if (dtype == kBF16) return gemm::run_few_rows_bf16(x, ldx, w, ldw, M, N, K, e, s);
+    return gemm::run_few_rows_f16(x, ldx, w, ldw, M, N, K, e, s);
+  }
   Product p = {{}, {}, M, N, K, gemm::epilogue(bias, residual, out, dact, act, out_dtype, dtype, N), 1, 0};
   if (const int rc = operand(p.a, x, M, ldx, K, dtype, ws, s)) return rc;
   if (const int rc = operand(p.b, w, N, ldw, K, dtype, ws, s)) return rc;

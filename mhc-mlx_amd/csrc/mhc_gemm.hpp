@@ -5,6 +5,8 @@
 // or not (its rows are k: W of dz W, and both operands of dz^T x).
 #pragma once
 
+#include <cmath>
+
 #include "mhc_device.hpp"
 #include "mhc_host.hpp"
 
@@ -25,13 +27,15 @@ struct Epilogue {
   void* dact;            // [M, N] as DactOf has it, or NULL; act is not none then
   int act;               // MHC_ACT_*
   int out_f32;           // out and residual are fp32, else of the operands' type
-  int vec;               // eight outputs from a column that is a multiple of eight are whole 16-byte vectors
+  int vec;               // 8, 4 or 1: so many outputs, from a column that is a multiple of it, are whole vectors of each array
 };
 
 // an epilogue whose `vec` goes by the row length and the addresses (residuals start anywhere)
 inline Epilogue epilogue(const void* bias, const void* residual, void* out, void* dact, int act, int out_dtype, int dtype,
                          int64_t N) {
-  const bool vec = N % 8 == 0 && aligned(out, 16) && aligned(residual, 16) && aligned(dact, 16);
+  const int v4 = out_dtype == kF32 ? 16 : 8, d4 = dtype == kF32 ? 16 : 8;  // bytes of four
+  const int vec = N % 8 == 0 && aligned(out, 16) && aligned(residual, 16) && aligned(dact, 16) ? 8
+                  : N % 4 == 0 && aligned(out, v4) && aligned(residual, v4) && aligned(dact, d4) ? 4 : 1;
   return Epilogue{bias, residual, out, dact, act, out_dtype == kF32, vec};
 }
 
@@ -75,7 +79,7 @@ MHC_DEV uint32_t dact_code(float d) {
 MHC_DEV float dact_value(int16_t q) { return q == -32768 ? __builtin_nanf("") : 0.5f + (float)q * 0x1p-15f; }
 MHC_DEV float dact_value(float d) { return d; }
 
-// V values to p: as 16-byte vectors (of 16-bit values: one for eight)
+// V values to p, as vectors
 template <typename O, int V>
 MHC_DEV void put(O* p, const float (&z)[V]) {
   if constexpr (V == 1) {
@@ -85,13 +89,14 @@ MHC_DEV void put(O* p, const float (&z)[V]) {
 #pragma unroll
     for (int k = 0; k < V; k += 4) *reinterpret_cast<f32x4*>(p + k) = f32x4{z[k], z[k + 1], z[k + 2], z[k + 3]};
   } else {
-    u32x4 w;
+    typedef uint32_t words __attribute__((ext_vector_type(V / 2)));
+    words w;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < V / 2; ++k) {
       if constexpr (__is_same(O, int16_t)) w[k] = dact_code(z[2 * k]) | dact_code(z[2 * k + 1]) << 16;
       else w[k] = pack2<O>(z[2 * k], z[2 * k + 1]);
     }
-    *reinterpret_cast<u32x4*>(p) = w;
+    *reinterpret_cast<words*>(p) = w;
   }
 }
 
@@ -189,7 +194,8 @@ struct Product {
 // read with a transposing load (four k of one index a lane): its 16 lanes
 // take 32 bytes of each of four rows, and chunk c of row k is at
 // c ^ (2 (k % 4) + k & 8), which spreads the eight rows of half a wave over
-// all banks.  fp32 operands are read one by one, four groups of lanes from
+// all banks (tiles of 64 have rows of half as many banks, two to a line:
+// c ^ 2 (k % 4) ^ k & 8 / 4).  fp32 operands are read one by one, four groups of lanes from
 // rows four apart: chunk c of row k is at c ^ 4 (k / 4 % 4).
 template <typename T>
 struct Stage {
@@ -197,9 +203,11 @@ struct Stage {
   static constexpr int kK = 8 * kE;               // k of a stage
 };
 
-template <typename T>
+template <typename T, int R>
 MHC_DEV int row_key(int k) {
-  return sizeof(T) == 4 ? ((k >> 2) & 3) << 2 : ((k & 3) << 1) | (k & 8);
+  static_assert(R >= 64, "a row has more chunks than a key has values");
+  if constexpr (sizeof(T) == 4) return ((k >> 2) & 3) << 2;
+  else return R >= 128 ? ((k & 3) << 1) | (k & 8) : ((k & 3) << 1) ^ ((k & 8) >> 2);
 }
 
 // Sixteen bytes a lane from memory to LDS, in the order of the lanes, without
@@ -249,7 +257,7 @@ struct Loader {
       } else {
         constexpr int kC = R / S::kE;  // chunks of a row
         const int k = at / kC;
-        off[i] = (uint32_t)(k * ld) + (((at % kC) ^ row_key<T>(k)) << 4);
+        off[i] = (uint32_t)(k * ld) + (((at % kC) ^ row_key<T, R>(k)) << 4);
       }
     }
     lds = lds0 + wave * kLoads * 1024;
@@ -293,14 +301,14 @@ struct Reader {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         const int col = w0 + j * 16 + (r & 3) * 4;
-        at[j] = k * R * 2 + (((col >> 3) ^ row_key<T>(k)) << 4) + (col & 7) * 2;
+        at[j] = k * R * 2 + (((col >> 3) ^ row_key<T, R>(k)) << 4) + (col & 7) * 2;
       }
     } else {
       const int k = g * 4;
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         const int col = w0 + j * 16 + r;
-        at[j] = k * R * 4 + (((col >> 2) ^ row_key<T>(k)) << 4) + (col & 3) * 4;
+        at[j] = k * R * 4 + (((col >> 2) ^ row_key<T, R>(k)) << 4) + (col & 3) * 4;
       }
     }
   }
@@ -356,6 +364,29 @@ MHC_DEV void interleave() {
     __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     constexpr int kEach = PRODUCTS / READS > 0 ? PRODUCTS / READS : 1;
     __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
+  }
+}
+
+// ROWS rows of 64 sums in LDS, as tile_kernel puts them there, to the outputs
+// from (m0, n0) on: V columns a lane.
+template <typename T, int V, int ROWS>
+MHC_DEV void store_rows(const Epilogue& e, const char* sums, int lane, int64_t m0, int64_t M, int64_t n0, int64_t N) {
+  constexpr int kLanes = 64 / V;  // of a row
+  const int c = lane % kLanes * V;
+  if (n0 + c >= N) return;
+  for (int r = lane / kLanes; r < ROWS && m0 + r < M; r += kWave / kLanes) {
+    float z[V];
+    if constexpr (V == 1) {
+      z[0] = *reinterpret_cast<const float*>(sums + r * 256 + (((c / 4) ^ (r % 16)) << 4) + c % 4 * 4);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V / 4; ++k) {
+        const f32x4 u = *reinterpret_cast<const f32x4*>(sums + r * 256 + (((c / 4 + k) ^ (r % 16)) << 4));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) z[4 * k + j] = u[j];
+      }
+    }
+    finish<T>(e, m0 + r, n0 + c, N, z);
   }
 }
 
@@ -446,23 +477,97 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const Product p) {
         *reinterpret_cast<f32x4*>(mine + (j * 16 + lane % 16) * 256 + (((i * 4 + lane / 16) ^ (lane % 16)) << 4)) = acc[i][h + j];
     __syncthreads();
     const int64_t mh = m0 + wm + h * 16;
-    if (e.vec) {
-      const int c = lane % 8 * 2;
-      const int64_t n = n0 + wn + c * 4;
-      for (int r = lane / 8; r < kRows; r += 8) {
-        const f32x4 u = *reinterpret_cast<const f32x4*>(mine + r * 256 + ((c ^ (r % 16)) << 4));
-        const f32x4 v = *reinterpret_cast<const f32x4*>(mine + r * 256 + (((c + 1) ^ (r % 16)) << 4));
-        float z[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
-        if (mh + r < p.M && n < p.N) finish<T>(e, mh + r, n, p.N, z);
-      }
-    } else {
-      const int64_t n = n0 + wn + lane;
-      for (int r = 0; r < kRows; ++r) {
-        float z[1] = {*reinterpret_cast<const float*>(mine + r * 256 + (((lane / 4) ^ (r % 16)) << 4) + lane % 4 * 4)};
-        if (mh + r < p.M && n < p.N) finish<T>(e, mh + r, n, p.N, z);
-      }
-    }
+    if (e.vec == 8) store_rows<T, 8, kRows>(e, mine, lane, mh, p.M, n0 + wn, p.N);
+    else if (e.vec == 4) store_rows<T, 4, kRows>(e, mine, lane, mh, p.M, n0 + wn, p.N);
+    else store_rows<T, 1, kRows>(e, mine, lane, mh, p.M, n0 + wn, p.N);
   }
+}
+
+// --------------------------------------------------------------------------
+// Few rows: x W^T with M <= 64, bound by reading W
+// --------------------------------------------------------------------------
+
+// A workgroup has 16 rows of W and all of x; its eight waves take the k in
+// turn, straight from memory to the matrix instructions (each element of W is
+// used once, so LDS would only be a detour), with kDepth steps of loads under
+// way: 16 waves of a CU hold 64 KB of W in flight at M <= 16.  The waves'
+// sums meet in LDS, in order.  Rows may start anywhere.
+constexpr int kFewWaves = 8;
+
+template <typename T>
+MHC_DEV u32x4 load_any(const T* p) {
+  u32x4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+
+// a chunk of a row that ends before `left` elements, zeros after
+template <typename T>
+MHC_DEV u32x4 load_end(const T* p, int left) {
+  constexpr int kE = 16 / (int)sizeof(T);
+  T v[kE];
+#pragma unroll
+  for (int j = 0; j < kE; ++j) v[j] = j < left ? p[j] : (T)0;
+  return __builtin_bit_cast(u32x4, v);
+}
+
+template <typename T, int MT>
+__global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const T* x, int64_t ldx, const T* w, int64_t ldw, int M, int64_t N,
+                                                                  int K, const Epilogue e) {
+  constexpr int kE = 16 / (int)sizeof(T), kStep = 4 * kE;  // k of a step: a chunk for each of four groups of lanes
+  constexpr int kDepth = MT == 1 ? 8 : MT == 2 ? 4 : 2;
+  __shared__ __attribute__((aligned(16))) float sums[kFewWaves][MT * 16][16];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, r = lane & 15, g = lane >> 4;
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  // (lanes of rows that are not there read another one; their sums are not stored)
+  const T* const wr = w + min(n0 + r, N - 1) * ldw + g * kE;
+  const T* xr[MT];
+#pragma unroll
+  for (int j = 0; j < MT; ++j) xr[j] = x + (int64_t)min(j * 16 + r, M - 1) * ldx + g * kE;
+  f32x4 acc[MT] = {};
+  const int whole = K / (kStep * kDepth) * (kStep * kDepth);
+  for (int k = wave * kStep * kDepth; k < whole; k += kFewWaves * kStep * kDepth) {
+    u32x4 fw[kDepth], fx[MT][kDepth];
+#pragma unroll
+    for (int q = 0; q < kDepth; ++q) {
+      fw[q] = load_any(wr + k + q * kStep);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) fx[j][q] = load_any(xr[j] + k + q * kStep);
+    }
+#pragma unroll
+    for (int q = 0; q < kDepth; ++q)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) acc[j] = mfma16<T>(fw[q], fx[j][q], acc[j]);
+  }
+  for (int k = whole + wave * kStep; k < K; k += kFewWaves * kStep) {
+    const int left = K - k - g * kE;
+    const bool full = left >= kE;
+    const u32x4 fw = full ? load_any(wr + k) : load_end(wr + k, left);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[j] = mfma16<T>(fw, full ? load_any(xr[j] + k) : load_end(xr[j] + k, left), acc[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(&sums[wave][j * 16 + r][g * 4]) = acc[j];
+  __syncthreads();
+  for (int at = threadIdx.x; at < MT * 256; at += 64 * kFewWaves) {
+    const int m = at / 16, n = at % 16;
+    float z[1] = {0.f};
+#pragma unroll
+    for (int v = 0; v < kFewWaves; ++v) z[0] += sums[v][m][n];
+    if (m < M && n0 + n < N) finish<T>(e, m, n0 + n, N, z);
+  }
+}
+
+template <typename T>
+int run_few_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K, const Epilogue& e, hipStream_t s) {
+  const dim3 grid((unsigned)ceil_div(N, 16)), block(64 * kFewWaves);
+  const T* const xt = static_cast<const T*>(x);
+  const T* const wt = static_cast<const T*>(w);
+  if (M <= 16) hipLaunchKernelGGL((few_rows_kernel<T, 1>), grid, block, 0, s, xt, ldx, wt, ldw, (int)M, N, (int)K, e);
+  else if (M <= 32) hipLaunchKernelGGL((few_rows_kernel<T, 2>), grid, block, 0, s, xt, ldx, wt, ldw, (int)M, N, (int)K, e);
+  else hipLaunchKernelGGL((few_rows_kernel<T, 4>), grid, block, 0, s, xt, ldx, wt, ldw, (int)M, N, (int)K, e);
+  MHC_CHECK_LAUNCH("few_rows_kernel");
+  return MHC_OK;
 }
 
 // The sum over the splits, in order, and the epilogue.
@@ -492,25 +597,12 @@ int launch_tile(const Product& p, hipStream_t s) {
 
 template <typename T>
 int launch_join(const Epilogue& e, const float* part, int splits, int64_t M, int64_t N, hipStream_t s) {
-  const int V = e.vec ? 8 : 1;
-  const unsigned blocks = (unsigned)std::min(ceil_div(M * N / V, 256), (int64_t)device_cu_count() * 16);
-  if (e.vec) hipLaunchKernelGGL((join_kernel<T, 8>), dim3(blocks), dim3(256), 0, s, part, splits, M, N, e);
+  const unsigned blocks = (unsigned)std::min(ceil_div(M * N / e.vec, 256), (int64_t)device_cu_count() * 16);
+  if (e.vec == 8) hipLaunchKernelGGL((join_kernel<T, 8>), dim3(blocks), dim3(256), 0, s, part, splits, M, N, e);
+  else if (e.vec == 4) hipLaunchKernelGGL((join_kernel<T, 4>), dim3(blocks), dim3(256), 0, s, part, splits, M, N, e);
   else hipLaunchKernelGGL((join_kernel<T, 1>), dim3(blocks), dim3(256), 0, s, part, splits, M, N, e);
   MHC_CHECK_LAUNCH("join_kernel");
   return MHC_OK;
-}
-
-template <typename T, bool AK, bool BK>
-int run_layout(const Product& p, int tile, hipStream_t s) {
-  switch (tile) {
-    case 0: return launch_tile<T, AK, BK, 256, 256, 2, 4, 2>(p, s);
-    case 1: return launch_tile<T, AK, BK, 128, 128, 2, 2, 2>(p, s);
-    case 2: return launch_tile<T, AK, BK, 128, 128, 2, 2, 4>(p, s);
-    case 3: return launch_tile<T, AK, BK, 64, 128, 2, 2, 3>(p, s);
-    case 4: return launch_tile<T, AK, BK, 64, 128, 2, 2, 6>(p, s);
-    case 5: return launch_tile<T, AK, BK, 128, 128, 2, 2, 3>(p, s);
-    default: return launch_tile<T, AK, BK, 128, 256, 2, 4, 2>(p, s);
-  }
 }
 
 // How a product is cut up: its tile, and into how many parts its reduction.
@@ -518,17 +610,61 @@ struct Cut {
   int tile, splits, kper;
 };
 
+// The tiles, and what a stage of them takes in us on an MI355X: `alone` with
+// few workgroups on the card (its latencies), `busy` for each workgroup of a
+// CU that has `fit` of them (its matrix instructions and LDS reads).  From
+// x W^T over 64 to 512 stages: 256 x 256 16-bit at 1.18 alone, 1.6 with all
+// CUs at it (1.3 PFLOP/s); fp32 stages have half the k at 1/16 the rate.
+struct TileCost {
+  int bm, bn, fit;
+  float alone16, busy16, alone32, busy32;
+};
+constexpr TileCost kTiles[] = {
+    {256, 256, 1, 1.18f, 1.60f, 7.20f, 7.35f}, {128, 256, 1, 0.71f, 0.92f, 3.68f, 3.84f},
+    {128, 128, 2, 0.57f, 0.54f, 1.96f, 1.88f}, {64, 128, 2, 0.43f, 0.34f, 1.07f, 0.98f},
+    {64, 64, 3, 0.26f, 0.21f, 0.57f, 0.53f},
+};
+
+// The cut with the least estimated time.  Large tiles read least, small ones
+// give every CU work; a reduction is split where even those are too few,
+// which costs a launch and its sums' way through memory.
 inline Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype) {
-  const char* t = getenv("X_TILE");
-  const char* sp = getenv("X_SPLIT");
-  const int kK = dtype == kF32 ? 32 : 64;
-  const int64_t big = ceil_div(M, 256) * ceil_div(N, 256), cus = device_cu_count();
-  Cut c = {t ? atoi(t) : big * 8 >= cus * 6 ? 0 : 1, sp ? atoi(sp) : 1, 0};
-  const int64_t stages = ceil_div(K, kK);
-  c.splits = (int)std::min<int64_t>(c.splits, stages);
-  c.kper = (int)(ceil_div(stages, c.splits) * kK);
-  c.splits = (int)ceil_div(K, c.kper);
-  return c;
+  const bool f32 = dtype == kF32;
+  const int kK = f32 ? 32 : 64;
+  const int stages = (int)ceil_div(K, kK);
+  const float cus = (float)device_cu_count();
+  Cut best = {0, 1, stages * kK};
+  float least = 0.f;
+  for (int t = 0; t < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++t) {
+    const TileCost& c = kTiles[t];
+    const float tiles = (float)ceil_div(M, c.bm) * (float)ceil_div(N, c.bn);
+    const float alone = f32 ? c.alone32 : c.alone16, busy = f32 ? c.busy32 : c.busy16;
+    for (int want = 1; want <= 16; ++want) {
+      if (want > 1 && (tiles * (want - 1) > 4.f * cus || stages < 2 * want)) break;
+      const int per = (stages + want - 1) / want, splits = (stages + per - 1) / per;
+      if (splits < want) continue;
+      const float of_cu = tiles * splits / cus, q = ceilf(of_cu);  // workgroups of a CU
+      const float stage = of_cu <= 1.f ? alone + std::max(0.f, busy - alone) * of_cu : std::max(alone * ceilf(q / c.fit), busy * q);
+      float us = 3.f + per * stage;
+      if (splits > 1) us += 4.f + 2.f * splits * (float)M * (float)N / 1e6f;  // 8 bytes each at 4 TB/s
+      if (least == 0.f || us < least) {
+        least = us;
+        best = {t, splits, per * kK};
+      }
+    }
+  }
+  return best;
+}
+
+template <typename T, bool AK, bool BK>
+int run_layout(const Product& p, int tile, hipStream_t s) {
+  switch (tile) {
+    case 0: return launch_tile<T, AK, BK, 256, 256, 2, 4, 2>(p, s);
+    case 1: return launch_tile<T, AK, BK, 128, 256, 2, 4, 2>(p, s);
+    case 2: return launch_tile<T, AK, BK, 128, 128, 2, 2, 2>(p, s);
+    case 3: return launch_tile<T, AK, BK, 64, 128, 2, 2, 3>(p, s);
+    default: return launch_tile<T, AK, BK, 64, 64, 4, 1, 3>(p, s);
+  }
 }
 
 // The product of one type; a_k / b_k: the operand's k are contiguous.  part: splits * M * N floats where it is split.
@@ -537,7 +673,7 @@ int run_product(Product p, bool a_k, bool b_k, const Cut& c, float* part, hipStr
   const Epilogue e = p.e;
   p.splits = c.splits;
   p.kper = c.kper;
-  if (c.splits > 1) p.e = Epilogue{nullptr, nullptr, part, nullptr, MHC_ACT_NONE, 1, p.N % 8 == 0};
+  if (c.splits > 1) p.e = epilogue(nullptr, nullptr, part, nullptr, MHC_ACT_NONE, kF32, kF32, p.N);
   const int rc = a_k && b_k ? run_layout<T, true, true>(p, c.tile, s)
                  : a_k      ? run_layout<T, true, false>(p, c.tile, s)
                             : run_layout<T, false, false>(p, c.tile, s);
@@ -545,6 +681,9 @@ int run_product(Product p, bool a_k, bool b_k, const Cut& c, float* part, hipStr
   return launch_join<T>(e, part, c.splits, p.M, p.N, s);
 }
 
+int run_few_rows_f32(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K, const Epilogue& e, hipStream_t s);
+int run_few_rows_bf16(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K, const Epilogue& e, hipStream_t s);
+int run_few_rows_f16(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K, const Epilogue& e, hipStream_t s);
 int run_product_f32(const Product& p, bool a_k, bool b_k, const Cut& c, float* part, hipStream_t s);
 int run_product_bf16(const Product& p, bool a_k, bool b_k, const Cut& c, float* part, hipStream_t s);
 int run_product_f16(const Product& p, bool a_k, bool b_k, const Cut& c, float* part, hipStream_t s);
