@@ -404,8 +404,9 @@ int mhc_policy_loss_fwd_bwd(const mhc_policy_args* args, float grad_scale, float
 #define MHC_ACT_GELU_TANH 3 /* z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2 */
 #define MHC_ACT_SILU 4
 
-/* Bytes of workspace of mhc_linear_act_fwd for these operands: copies of
- * those whose rows do not start on 16 bytes or are no multiple of it. */
+/* Bytes of workspace of mhc_linear_act_fwd for these operands: sums of a
+ * reduction that is split, and copies of operands whose rows are no whole
+ * four-byte words. */
 size_t mhc_linear_act_fwd_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw,
                                           int64_t M, int64_t N, int64_t K, int dtype);
 

@@ -12,47 +12,94 @@ namespace {
 using gemm::Operand;
 using gemm::Product;
 
-constexpr int kDzCols = 64 * 8;   // columns of a workgroup of dz_kernel: eight a lane of each wave
-constexpr int kDzRows = 64;       // rows: sixteen each wave
+constexpr int kDzCols = 64 * 8;   // columns of a workgroup of dz_kernel: eight for each lane of a wave
+constexpr int kDzRows = 64;       // rows: sixteen for each wave
 
 // dz = dout dact (dact NULL: dout), rounded to T, in rows of N elements `ld`
-// apart with zeros between (not stored if dz is NULL), and sums of dz over this workgroup's rows, before rounding, to part[block of rows][N] (if not NULL)
-template <typename T, typename G>
+// apart with zeros between (not stored if dz is NULL), and sums of dz over
+// this workgroup's rows, before rounding, to part[block of rows][N] (if not
+// NULL).  One pass at the card's streaming rate: a lane has eight consecutive
+// columns (VEC: every array's are 16-byte vectors), else eight 64 apart, of
+// every fourth row, four of which are loaded at a time.
+template <typename T, typename G, bool VEC>
 __global__ __launch_bounds__(256) void dz_kernel(const G* dout, const void* dact, T* dz, int64_t ld, float* part, int64_t M,
                                                  int64_t N) {
   using D = typename gemm::DactOf<T>::Type;
   __shared__ float lds[4][kDzCols];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int64_t n = (int64_t)blockIdx.x * kDzCols + lane * 8, m0 = (int64_t)blockIdx.y * kDzRows;
-  const int left = (int)max((int64_t)0, min((int64_t)8, N - n));
+  const int64_t n0 = (int64_t)blockIdx.x * kDzCols, m0 = (int64_t)blockIdx.y * kDzRows;
+  const auto column = [&](int k) { return VEC ? lane * 8 + k : k * kWave + lane; };
+  const D* const d = static_cast<const D*>(dact);
   float sum[8] = {};
-  for (int64_t m = m0 + wave; m < min(m0 + kDzRows, M); m += 4) {
-    for (int k = 0; k < left; ++k) {
-      const int64_t at = m * N + n + k;
-      float v = load1(dout + at);
-      if (dact != nullptr) v *= gemm::dact_value(static_cast<const D*>(dact)[at]);
-      sum[k] += v;
-      if (dz != nullptr) store1(dz + m * ld + n + k, v);
+  const bool in = !VEC || n0 + lane * 8 < N;
+  for (int64_t m = m0 + wave; in && m < min(m0 + kDzRows, M); m += 16) {
+    float v[4][8], f[4][8];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t row = min(m + 4 * q, M - 1);
+      if constexpr (VEC) {
+        gemm::take(dout + row * N + n0 + lane * 8, v[q]);
+        if (d != nullptr) {
+          if constexpr (sizeof(D) == 4) {
+            gemm::take(d + row * N + n0 + lane * 8, f[q]);
+          } else {
+            const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(d + row * N + n0 + lane * 8));
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[q][k] = gemm::dact_value((int16_t)(w[k / 2] >> (16 * (k % 2))));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int64_t at = row * N + min(n0 + column(k), N - 1);
+          v[q][k] = load1(dout + at);
+          if (d != nullptr) f[q][k] = gemm::dact_value(d[at]);
+        }
+      }
     }
-    for (int k = left; k < 8 && dz != nullptr && n + k < ld; ++k) dz[m * ld + n + k] = (T)0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t row = m + 4 * q;
+      if (row >= min(m0 + kDzRows, M)) break;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (d != nullptr) v[q][k] *= f[q][k];
+        sum[k] += v[q][k];
+      }
+      if (dz == nullptr) continue;
+      if constexpr (VEC) {
+        gemm::put(dz + row * ld + n0 + lane * 8, v[q]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const int64_t n = n0 + column(k);
+          if (n < ld) store1(dz + row * ld + n, n < N ? v[q][k] : 0.f);
+        }
+      }
+    }
   }
   if (part == nullptr) return;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) lds[wave][lane * 8 + k] = sum[k];
+  for (int k = 0; k < 8; ++k) lds[wave][column(k)] = sum[k];
   __syncthreads();
-  for (int c = threadIdx.x; c < kDzCols; c += 256) {
-    const int64_t at = (int64_t)blockIdx.x * kDzCols + c;
-    if (at < N) part[(int64_t)blockIdx.y * N + at] = (lds[0][c] + lds[1][c]) + (lds[2][c] + lds[3][c]);
-  }
+  for (int c = threadIdx.x; c < kDzCols; c += 256)
+    if (n0 + c < N) part[(int64_t)blockIdx.y * N + n0 + c] = (lds[0][c] + lds[1][c]) + (lds[2][c] + lds[3][c]);
 }
 
-// db[n] = sum over the blocks of rows, in order
+// db[n] = sum over the blocks of rows: 32 columns a workgroup, each in eight parts that are joined in order
 template <typename T>
 __global__ __launch_bounds__(256) void db_kernel(const float* part, T* db, int64_t blocks, int64_t N) {
-  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (n >= N) return;
+  __shared__ float lds[8][32];
+  const int c = threadIdx.x % 32, q = threadIdx.x / 32;
+  const int64_t n = (int64_t)blockIdx.x * 32 + c;
   float s = 0.f;
-  for (int64_t b = 0; b < blocks; ++b) s += part[b * N + n];
+#pragma unroll 8
+  for (int64_t b = q; b < blocks; b += 8) s += part[b * N + min(n, N - 1)];
+  lds[q][c] = s;
+  __syncthreads();
+  if (q != 0 || n >= N) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) s += lds[k][c];
   store1(db + n, s);
 }
 
@@ -93,12 +140,6 @@ size_t part_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
   return c.splits > 1 ? (size_t)(c.splits * M * N) * sizeof(float) : 0;
 }
 
-// Up to 64 rows of x go to the kernel that only streams W.
-bool few_rows(int64_t M, int64_t N, int64_t K, int dtype) {
-  const char* t = getenv("X_FEW");
-  return M <= (t ? atoi(t) : 64);
-}
-
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
 int64_t padded(int64_t width, int dtype) {
@@ -108,7 +149,7 @@ int64_t padded(int64_t width, int dtype) {
 
 // bytes of an operand's copy in rows of whole chunks; 0: it is read as it is
 size_t pack_bytes(const void* p, int64_t rows, int64_t ld, int64_t width, int dtype) {
-  if (gemm::in_chunks(p, ld, width, elem_bytes(dtype))) return 0;
+  if (gemm::in_words(p, ld, width, elem_bytes(dtype))) return 0;
   return up256((size_t)(rows * padded(width, dtype)) * elem_bytes(dtype));
 }
 
@@ -122,7 +163,7 @@ int run_pack(const void* p, int64_t ld, void* to, int64_t rows, int64_t width, i
   return MHC_OK;
 }
 
-// The operand, copied to `ws` first (which moves on) where its rows are not whole chunks.
+// The operand, copied to `ws` first (which moves on) where its rows are no whole words.
 int operand(Operand& o, const void* p, int64_t rows, int64_t ld, int64_t width, int dtype, char*& ws, hipStream_t s) {
   const size_t bytes = pack_bytes(p, rows, ld, width, dtype);
   if (bytes == 0) {
@@ -144,7 +185,7 @@ struct BwdPlan {
 BwdPlan plan_bwd(const void* dout, int dout_dtype, bool dact, const void* x, int64_t ldx, const void* w, int64_t ldw, bool dx, bool dw,
                  bool db, int64_t M, int64_t N, int64_t K, int dtype) {
   BwdPlan b = {};
-  if ((dx || dw) && (dact || dout_dtype != dtype || !gemm::in_chunks(dout, N, N, elem_bytes(dtype))))
+  if ((dx || dw) && (dact || dout_dtype != dtype || !gemm::in_words(dout, N, N, elem_bytes(dtype))))
     b.dz = up256((size_t)(M * padded(N, dtype)) * elem_bytes(dtype));
   if (db) b.part = up256((size_t)(ceil_div(M, kDzRows) * N) * sizeof(float));
   if (dx) b.w = pack_bytes(w, N, ldw, K, dtype);
@@ -157,11 +198,15 @@ BwdPlan plan_bwd(const void* dout, int dout_dtype, bool dact, const void* x, int
 template <typename T, typename G>
 int run_dz(const void* dout, const void* dact, void* dz, int64_t ld, float* part, void* db, int64_t M, int64_t N, hipStream_t s) {
   const int64_t blocks = ceil_div(M, kDzRows);
-  hipLaunchKernelGGL((dz_kernel<T, G>), dim3((unsigned)ceil_div(N, kDzCols), (unsigned)blocks), dim3(256), 0, s,
-                     static_cast<const G*>(dout), dact, static_cast<T*>(dz), ld, part, M, N);
+  const dim3 grid((unsigned)ceil_div(N, kDzCols), (unsigned)blocks);
+  const G* const g = static_cast<const G*>(dout);
+  if (N % 8 == 0 && aligned(dout, 16) && aligned(dact, 16))
+    hipLaunchKernelGGL((dz_kernel<T, G, true>), grid, dim3(256), 0, s, g, dact, static_cast<T*>(dz), ld, part, M, N);
+  else
+    hipLaunchKernelGGL((dz_kernel<T, G, false>), grid, dim3(256), 0, s, g, dact, static_cast<T*>(dz), ld, part, M, N);
   MHC_CHECK_LAUNCH("dz_kernel");
   if (db != nullptr) {
-    hipLaunchKernelGGL((db_kernel<T>), dim3((unsigned)ceil_div(N, 256)), dim3(256), 0, s, (const float*)part, static_cast<T*>(db),
+    hipLaunchKernelGGL((db_kernel<T>), dim3((unsigned)ceil_div(N, 32)), dim3(256), 0, s, (const float*)part, static_cast<T*>(db),
                        blocks, N);
     MHC_CHECK_LAUNCH("db_kernel");
   }
@@ -181,7 +226,7 @@ int check_shape(int64_t M, int64_t N, int64_t K, int dtype) {
 
 extern "C" size_t mhc_linear_act_fwd_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M,
                                                      int64_t N, int64_t K, int dtype) {
-  if (M <= 0 || N <= 0 || K <= 0 || mhc::few_rows(M, N, K, dtype)) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || mhc::gemm::few_rows(x, ldx, w, ldw, M, N, K, dtype)) return 0;
   return mhc::pack_bytes(x, M, ldx, K, dtype) + mhc::pack_bytes(w, N, ldw, K, dtype) + mhc::part_bytes(M, N, K, dtype);
 }
 
@@ -202,7 +247,7 @@ extern "C" int mhc_linear_act_fwd(const void* x, int64_t ldx, const void* w, int
   MHC_CHECK_ARG(aligned(workspace, 16), "workspace must be 16-byte aligned");
   hipStream_t s = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
-  if (few_rows(M, N, K, dtype)) {
+  if (gemm::few_rows(x, ldx, w, ldw, M, N, K, dtype)) {
     const gemm::Epilogue e = gemm::epilogue(bias, residual, out, dact, act, out_dtype, dtype, N);
     if (dtype == kF32) return gemm::run_few_rows_f32(x, ldx, w, ldw, M, N, K, e, s);
     if (dtype == kBF16) return gemm::run_few_rows_bf16(x, ldx, w, ldw, M, N, K, e, s);

@@ -6,6 +6,7 @@
 #pragma once
 
 #include <cmath>
+#include <type_traits>
 
 #include "mhc_device.hpp"
 #include "mhc_host.hpp"
@@ -27,15 +28,17 @@ struct Epilogue {
   void* dact;            // [M, N] as DactOf has it, or NULL; act is not none then
   int act;               // MHC_ACT_*
   int out_f32;           // out and residual are fp32, else of the operands' type
-  int vec;               // 8, 4 or 1: so many outputs, from a column that is a multiple of it, are whole vectors of each array
+  int vec;               // 8, 4, 2 or 1: so many outputs, from a column that is a multiple of it, are whole vectors of each array
 };
 
 // an epilogue whose `vec` goes by the row length and the addresses (residuals start anywhere)
 inline Epilogue epilogue(const void* bias, const void* residual, void* out, void* dact, int act, int out_dtype, int dtype,
                          int64_t N) {
-  const int v4 = out_dtype == kF32 ? 16 : 8, d4 = dtype == kF32 ? 16 : 8;  // bytes of four
-  const int vec = N % 8 == 0 && aligned(out, 16) && aligned(residual, 16) && aligned(dact, 16) ? 8
-                  : N % 4 == 0 && aligned(out, v4) && aligned(residual, v4) && aligned(dact, d4) ? 4 : 1;
+  const int eo = out_dtype == kF32 ? 4 : 2, ed = dtype == kF32 ? 4 : 2;
+  int vec = 8;
+  while (vec > 1 && (N % vec != 0 || !aligned(out, std::min(16, vec * eo)) || !aligned(residual, std::min(16, vec * eo)) ||
+                     !aligned(dact, std::min(16, vec * ed))))
+    vec /= 2;
   return Epilogue{bias, residual, out, dact, act, out_dtype == kF32, vec};
 }
 
@@ -43,25 +46,66 @@ struct Act {
   float y, d;
 };
 
-MHC_DEV float sigmoid(float x) { return 1.f / (1.f + expf(-x)); }
+// FAST (16-bit operands): the hardware's exponential and reciprocal, which are
+// good to 2^-22 of the value; else the library's.
+template <bool FAST>
+MHC_DEV float exp_of(float x) {
+  return FAST ? __builtin_amdgcn_exp2f(x * 1.44269504f) : expf(x);
+}
+template <bool FAST>
+MHC_DEV float sigmoid(float x) {
+  const float d = 1.f + exp_of<FAST>(-x);
+  return FAST ? __builtin_amdgcn_rcpf(d) : 1.f / d;
+}
+
+// Phi(z), with e = exp(-z^2 / 2).  FAST: Abramowitz and Stegun 7.1.26,
+// 1 - erf(x) = e^(-x^2) (a1 t + .. + a5 t^5), t = 1 / (1 + p x), to 1.5e-7,
+// which shares the exponential with the derivative.
+template <bool FAST>
+MHC_DEV float normal_cdf(float z, float e) {
+  if constexpr (!FAST) return 0.5f * (1.f + erff(z * 0.70710678f));
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * 0.70710678f * fabsf(z));
+  const float tail = 0.5f * e * (t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)))));
+  return z < 0.f ? tail : 1.f - tail;
+}
 
 // act(z) and act'(z).  NaN goes through each of them.
-MHC_DEV Act activate(float z, int act) {
+template <bool FAST, int ACT>
+MHC_DEV Act activate(float z) {
+  if constexpr (ACT == MHC_ACT_RELU) {
+    return {z < 0.f ? 0.f : z, z > 0.f ? 1.f : 0.f};
+  } else if constexpr (ACT == MHC_ACT_GELU) {
+    const float e = exp_of<FAST>(-0.5f * z * z), p = normal_cdf<FAST>(z, e);
+    return {z * p, p + z * e * 0.39894228f};
+  } else if constexpr (ACT == MHC_ACT_GELU_TANH) {  // (1 + tanh u) / 2 is sigmoid(2 u)
+    const float p = sigmoid<FAST>(1.59576912f * (z + 0.044715f * z * z * z));
+    return {z * p, p + z * p * (1.f - p) * 1.59576912f * (1.f + 0.134145f * z * z)};
+  } else {
+    const float p = sigmoid<FAST>(z);
+    return {z * p, p * (1.f + z * (1.f - p))};
+  }
+}
+
+template <bool FAST, int ACT, int R, int V>
+MHC_DEV void activate_each(float (&z)[R][V], float (&d)[R][V]) {
+#pragma unroll
+  for (int b = 0; b < R; ++b)
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const Act a = activate<FAST, ACT>(z[b][k]);
+      z[b][k] = a.y;
+      d[b][k] = a.d;
+    }
+}
+
+template <bool FAST, int R, int V>
+MHC_DEV void activate_all(int act, float (&z)[R][V], float (&d)[R][V]) {
   switch (act) {
-    case MHC_ACT_RELU: return {z < 0.f ? 0.f : z, z > 0.f ? 1.f : 0.f};
-    case MHC_ACT_GELU: {
-      const float p = 0.5f * (1.f + erff(z * 0.70710678f));
-      return {z * p, p + z * expf(-0.5f * z * z) * 0.39894228f};
-    }
-    case MHC_ACT_GELU_TANH: {  // (1 + tanh u) / 2 is sigmoid(2 u)
-      const float p = sigmoid(1.59576912f * (z + 0.044715f * z * z * z));
-      return {z * p, p + z * p * (1.f - p) * 1.59576912f * (1.f + 0.134145f * z * z)};
-    }
-    case MHC_ACT_SILU: {
-      const float p = sigmoid(z);
-      return {z * p, p * (1.f + z * (1.f - p))};
-    }
-    default: return {z, 1.f};
+    case MHC_ACT_RELU: return activate_each<FAST, MHC_ACT_RELU>(z, d);
+    case MHC_ACT_GELU: return activate_each<FAST, MHC_ACT_GELU>(z, d);
+    case MHC_ACT_GELU_TANH: return activate_each<FAST, MHC_ACT_GELU_TANH>(z, d);
+    case MHC_ACT_SILU: return activate_each<FAST, MHC_ACT_SILU>(z, d);
+    default: return;
   }
 }
 
@@ -85,6 +129,8 @@ MHC_DEV void put(O* p, const float (&z)[V]) {
   if constexpr (V == 1) {
     if constexpr (__is_same(O, int16_t)) *p = (int16_t)dact_code(z[0]);
     else store1(p, z[0]);
+  } else if constexpr (sizeof(O) == 4 && V == 2) {
+    *reinterpret_cast<f32x2*>(p) = f32x2{z[0], z[1]};
   } else if constexpr (sizeof(O) == 4) {
 #pragma unroll
     for (int k = 0; k < V; k += 4) *reinterpret_cast<f32x4*>(p + k) = f32x4{z[k], z[k + 1], z[k + 2], z[k + 3]};
@@ -101,37 +147,58 @@ MHC_DEV void put(O* p, const float (&z)[V]) {
 }
 
 template <typename O, int V>
-MHC_DEV void add(const O* p, float (&z)[V]) {
+MHC_DEV void take(const O* p, float (&z)[V]) {
   Vec<O, V> r;
   r.load(p);
 #pragma unroll
-  for (int k = 0; k < V; ++k) z[k] += r.get(k);
+  for (int k = 0; k < V; ++k) z[k] = r.get(k);
 }
 
-// V outputs of row m from column n on, from their sums; V > 1: each array's are whole vectors
-template <typename T, int V>
-MHC_DEV void finish(const Epilogue& e, int64_t m, int64_t n, int64_t N, float (&z)[V]) {
-  const int64_t at = m * N + n;
-  if (e.bias != nullptr) {
+// The residuals of V outputs from column n on, of R rows `step` apart from
+// row m on (of the last row past the end; zeros without a residual): all of
+// them loaded before the first is used.
+template <typename T, int V, int R>
+MHC_DEV void residual_of(const Epilogue& e, int64_t m, int step, int64_t M, int64_t n, int64_t N, float (&r)[R][V]) {
+  if (e.residual == nullptr) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) z[k] += load1(static_cast<const T*>(e.bias) + n + k);
-  }
-  if (e.act != MHC_ACT_NONE) {
-    float d[V];
+    for (int b = 0; b < R; ++b)
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const Act a = activate(z[k], e.act);
-      z[k] = a.y;
-      d[k] = a.d;
-    }
-    if (e.dact != nullptr) put(static_cast<typename DactOf<T>::Type*>(e.dact) + at, d);
-  }
-  if (e.out_f32) {
-    if (e.residual != nullptr) add(static_cast<const float*>(e.residual) + at, z);
-    put(static_cast<float*>(e.out) + at, z);
+      for (int k = 0; k < V; ++k) r[b][k] = 0.f;
+  } else if (e.out_f32) {
+#pragma unroll
+    for (int b = 0; b < R; ++b) take(static_cast<const float*>(e.residual) + min(m + b * step, M - 1) * N + n, r[b]);
   } else if constexpr (sizeof(T) == 2) {
-    if (e.residual != nullptr) add(static_cast<const T*>(e.residual) + at, z);
-    put(static_cast<T*>(e.out) + at, z);
+#pragma unroll
+    for (int b = 0; b < R; ++b) take(static_cast<const T*>(e.residual) + min(m + b * step, M - 1) * N + n, r[b]);
+  }
+}
+
+template <typename T, int V>
+MHC_DEV void bias_of(const Epilogue& e, int64_t n, float (&b)[V]) {
+#pragma unroll
+  for (int k = 0; k < V; ++k) b[k] = e.bias != nullptr ? load1(static_cast<const T*>(e.bias) + n + k) : 0.f;
+}
+
+// The outputs of R rows `step` apart from row m on, V from column n on, from
+// their sums; V > 1: each array's are whole vectors.
+template <typename T, int V, int R>
+MHC_DEV void finish(const Epilogue& e, int64_t m, int step, int64_t M, int64_t n, int64_t N, float (&z)[R][V], const float (&bias)[V],
+                    const float (&residual)[R][V]) {
+  float d[R][V];
+#pragma unroll
+  for (int b = 0; b < R; ++b)
+#pragma unroll
+    for (int k = 0; k < V; ++k) z[b][k] += bias[k];
+  activate_all<sizeof(T) == 2>(e.act, z, d);
+#pragma unroll
+  for (int b = 0; b < R; ++b) {
+    if (m + b * step >= M) break;
+    const int64_t at = (m + b * step) * N + n;
+    if (e.dact != nullptr) put(static_cast<typename DactOf<T>::Type*>(e.dact) + at, d[b]);
+#pragma unroll
+    for (int k = 0; k < V; ++k) z[b][k] += residual[b][k];
+    if (e.out_f32) put(static_cast<float*>(e.out) + at, z[b]);
+    else if constexpr (sizeof(T) == 2) put(static_cast<T*>(e.out) + at, z[b]);
   }
 }
 
@@ -162,7 +229,8 @@ MHC_DEV f32x4 mfma16(const u32x4& a, const u32x4& b, f32x4 c) {
 // --------------------------------------------------------------------------
 
 // An operand as it is stored: rows of `width` elements, `ld` elements apart.
-// Rows and width are a multiple of 16 bytes long and start on one.
+// Rows start on four bytes, as the loads to LDS ask, and are a multiple of
+// four bytes long, so that the end of the last one is the end of a word.
 struct Operand {
   const void* p;
   int64_t ld, width;
@@ -171,8 +239,8 @@ struct Operand {
 constexpr int64_t kMaxRowBytes = 1 << 23;  // between rows: 256 of them stay below 2^31
 
 // Whether rows of `width` elements, `ld` apart, can be an Operand as they are.
-inline bool in_chunks(const void* p, int64_t ld, int64_t width, int bytes) {
-  return aligned(p, 16) && ld * bytes % 16 == 0 && width * bytes % 16 == 0 && ld * bytes <= kMaxRowBytes;
+inline bool in_words(const void* p, int64_t ld, int64_t width, int bytes) {
+  return aligned(p, 4) && ld * bytes % 4 == 0 && width * bytes % 4 == 0 && ld * bytes <= kMaxRowBytes;
 }
 
 struct Product {
@@ -282,6 +350,19 @@ struct Loader {
     base += (uint64_t)step;
     left -= step;
   }
+
+  // Zeros after the last of the `kleft` k that a stage has, in the chunk that
+  // they end in: what follows them in memory is the next row.  (Whole chunks
+  // past the end were not loaded; for rows of k, whole rows.)
+  static MHC_DEV void clear_end(char* stage, int kleft, int thread, int threads) {
+    if constexpr (KM) {
+      const int c = kleft / S::kE;
+      for (int row = thread; row < R; row += threads) {
+        T* const p = reinterpret_cast<T*>(stage + row * 128 + ((c ^ (row & 7)) << 4));
+        for (int j = kleft % S::kE; j < S::kE; ++j) p[j] = (T)0;
+      }
+    }
+  }
 };
 
 // A wave's fragments of one operand: J times 16 indices from w0 of a tile
@@ -368,25 +449,34 @@ MHC_DEV void interleave() {
 }
 
 // ROWS rows of 64 sums in LDS, as tile_kernel puts them there, to the outputs
-// from (m0, n0) on: V columns a lane.
+// from (m0, n0) on: V columns a lane, 16 outputs of it at a time.
 template <typename T, int V, int ROWS>
 MHC_DEV void store_rows(const Epilogue& e, const char* sums, int lane, int64_t m0, int64_t M, int64_t n0, int64_t N) {
-  constexpr int kLanes = 64 / V;  // of a row
+  constexpr int kLanes = 64 / V, kPass = kWave / kLanes;  // lanes of a row, rows of a pass
+  constexpr int kBatch = ROWS / kPass < 16 / V ? ROWS / kPass : 16 / V;
   const int c = lane % kLanes * V;
   if (n0 + c >= N) return;
-  for (int r = lane / kLanes; r < ROWS && m0 + r < M; r += kWave / kLanes) {
-    float z[V];
-    if constexpr (V == 1) {
-      z[0] = *reinterpret_cast<const float*>(sums + r * 256 + (((c / 4) ^ (r % 16)) << 4) + c % 4 * 4);
-    } else {
+  float bias[V];
+  bias_of<T>(e, n0 + c, bias);
+  for (int r0 = lane / kLanes; r0 < ROWS && m0 + r0 < M; r0 += kPass * kBatch) {
+    float z[kBatch][V], res[kBatch][V];
+    residual_of<T>(e, m0 + r0, kPass, M, n0 + c, N, res);
 #pragma unroll
-      for (int k = 0; k < V / 4; ++k) {
-        const f32x4 u = *reinterpret_cast<const f32x4*>(sums + r * 256 + (((c / 4 + k) ^ (r % 16)) << 4));
+    for (int b = 0; b < kBatch; ++b) {
+      const int r = r0 + b * kPass;
+      if constexpr (V < 4) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) z[4 * k + j] = u[j];
+        for (int k = 0; k < V; ++k) z[b][k] = *reinterpret_cast<const float*>(sums + r * 256 + (((c / 4) ^ (r % 16)) << 4) + (c % 4 + k) * 4);
+      } else {
+#pragma unroll
+        for (int k = 0; k < V / 4; ++k) {
+          const f32x4 u = *reinterpret_cast<const f32x4*>(sums + r * 256 + (((c / 4 + k) ^ (r % 16)) << 4));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) z[b][4 * k + j] = u[j];
+        }
       }
     }
-    finish<T>(e, m0 + r, n0 + c, N, z);
+    finish<T>(e, m0 + r0, kPass, M, n0 + c, N, z, bias, res);
   }
 }
 
@@ -439,7 +529,14 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const Product p) {
   }
   wait_loads<(NS - 1) * kLoads>();
   __syncthreads();
+  const auto clear_end = [&](int stage, int left) {
+    if (left <= 0 || left >= S::kK || left % S::kE == 0) return;
+    la.clear_end(smem + stage, left, threadIdx.x, 64 * kWaves);
+    lb.clear_end(smem + stage + kA, left, threadIdx.x, 64 * kWaves);
+    __syncthreads();
+  };
   int cur = 0;
+  clear_end(cur, kleft);
   Fragments<JM, JN> f0, f1;
   f0.read(ra, rb, smem, smem + kA, 0);
   for (; kleft > 0; kleft -= S::kK) {
@@ -453,6 +550,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const Product p) {
     la.next();
     lb.next();
     cur = cur == (NS - 1) * kStage ? 0 : cur + kStage;
+    clear_end(cur, kleft - S::kK);
     f0.read(ra, rb, smem + cur, smem + cur + kA, 0);
     f1.template multiply<T>(acc);
     interleave<(JM * (AK ? 1 : S::kE / 4) + JN * (BK ? 1 : S::kE / 4)), JM * JN * (sizeof(T) == 4 ? 4 : 1)>();
@@ -467,33 +565,119 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const Product p) {
   constexpr int kRound = JM >= 4 && kFit >= 4 ? 4 : JM >= 2 && kFit >= 2 ? 2 : 1, kRows = kRound * 16;
   static_assert(JN == 4 && JM % kRound == 0 && kFit >= 1, "64 columns a wave");
   char* const mine = smem + wave * kRows * 256;
-#pragma unroll
-  for (int h = 0; h < JM; h += kRound) {
+  // (a round's sums have constant indices, and those of the first are gone before the second)
+  int at = lane;
+  asm volatile("" : "+v"(at));  // (or addresses of the outputs would be formed before the loop and held through it)
+  const auto round = [&](auto first) {
+    constexpr int h = decltype(first)::value;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kRound; ++j)
 #pragma unroll
       for (int i = 0; i < JN; ++i)
-        *reinterpret_cast<f32x4*>(mine + (j * 16 + lane % 16) * 256 + (((i * 4 + lane / 16) ^ (lane % 16)) << 4)) = acc[i][h + j];
+        *reinterpret_cast<f32x4*>(mine + (j * 16 + at % 16) * 256 + (((i * 4 + at / 16) ^ (at % 16)) << 4)) = acc[i][h + j];
     __syncthreads();
     const int64_t mh = m0 + wm + h * 16;
-    if (e.vec == 8) store_rows<T, 8, kRows>(e, mine, lane, mh, p.M, n0 + wn, p.N);
-    else if (e.vec == 4) store_rows<T, 4, kRows>(e, mine, lane, mh, p.M, n0 + wn, p.N);
-    else store_rows<T, 1, kRows>(e, mine, lane, mh, p.M, n0 + wn, p.N);
-  }
+    if (e.vec == 8) store_rows<T, 8, kRows>(e, mine, at, mh, p.M, n0 + wn, p.N);
+    else if (e.vec == 4) store_rows<T, 4, kRows>(e, mine, at, mh, p.M, n0 + wn, p.N);
+    else if (e.vec == 2) store_rows<T, 2, kRows>(e, mine, at, mh, p.M, n0 + wn, p.N);
+    else store_rows<T, 1, kRows>(e, mine, at, mh, p.M, n0 + wn, p.N);
+  };
+  static_assert(JM / kRound <= 2, "two rounds");
+  round(std::integral_constant<int, 0>{});
+  if constexpr (JM > kRound) round(std::integral_constant<int, kRound>{});
 }
 
 // --------------------------------------------------------------------------
 // Few rows: x W^T with M <= 64, bound by reading W
 // --------------------------------------------------------------------------
 
-// A workgroup has 16 rows of W and all of x; its eight waves take the k in
-// turn, straight from memory to the matrix instructions (each element of W is
-// used once, so LDS would only be a detour), with kDepth steps of loads under
-// way: 16 waves of a CU hold 64 KB of W in flight at M <= 16.  The waves'
-// sums meet in LDS, in order.  Rows may start anywhere.
+// A workgroup has 16 rows of W and all of x, and its eight waves take stages
+// of the k in turn: each wave has some of its own under way to LDS, so that
+// memory is read in whole lines (fragments read straight from memory are half
+// lines: 9.1 us for 16 rows of 4096 x 4096 bf16, 12.7 us for 32; so 6.0, 8.0).  No wave waits for another before the end, where their
+// sums meet in LDS, in order.
 constexpr int kFewWaves = 8;
 
+// the waves' sums, in order, and the epilogue
+template <typename T, int MT>
+MHC_DEV void join_waves(const f32x4 (&acc)[MT], float* sums, int M, int64_t n0, int64_t N, const Epilogue& e) {
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(sums + ((wave * MT + j) * 16 + lane % 16) * 16 + lane / 16 * 4) = acc[j];
+  __syncthreads();
+  for (int at = threadIdx.x; at < MT * 256; at += 64 * kFewWaves) {
+    const int m = at / 16, n = at % 16;
+    float z[1][1] = {};
+#pragma unroll
+    for (int v = 0; v < kFewWaves; ++v) z[0][0] += sums[(v * MT * 16 + m) * 16 + n];
+    if (m < M && n0 + n < N) {
+      float bias[1], residual[1][1];
+      bias_of<T>(e, n0 + n, bias);
+      residual_of<T>(e, m, 0, M, n0 + n, N, residual);
+      finish<T>(e, m, 0, M, n0 + n, N, z, bias, residual);
+    }
+  }
+}
+
+template <typename T, int MT, int NS>
+__global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const Operand x, const Operand w, int M, int64_t N, int K, const Epilogue e) {
+  using S = Stage<T>;
+  constexpr int kW = 2048, kStage = kW * (1 + MT), kLoads = 2 * (1 + MT);
+  __shared__ __attribute__((aligned(1024))) char smem[kFewWaves * NS * kStage];
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  char* const mine = smem + wave * NS * kStage;
+  Loader<T, true, 16, 1> lw;
+  Loader<T, true, 16 * MT, 1> lx;
+  lw.init(w, n0, N, wave * S::kK, K, 0, lane, lds_address(mine));
+  lx.init(x, 0, M, wave * S::kK, K, 0, lane, lds_address(mine) + kW);
+  lw.step = lx.step = kFewWaves * 128;
+  Reader<T, true, 16, 1> rw;
+  Reader<T, true, 16 * MT, MT> rx;
+  rw.init(0, lane);
+  rx.init(0, lane);
+  f32x4 acc[MT] = {};
+  int kleft = K - wave * S::kK;
+#pragma unroll
+  for (int q = 0; q < NS; ++q) {
+    lw.load(q * kStage, kleft - q * kFewWaves * S::kK, lane);
+    lx.load(q * kStage, kleft - q * kFewWaves * S::kK, lane);
+    lw.next();
+    lx.next();
+  }
+  int cur = 0;
+  for (; kleft > 0; kleft -= kFewWaves * S::kK) {
+    wait_loads<(NS - 1) * kLoads>();
+    if (kleft < S::kK && kleft % S::kE != 0) {
+      lw.clear_end(mine + cur, kleft, lane, kWave);
+      lx.clear_end(mine + cur + kW, kleft, lane, kWave);
+    }
+    u32x4 fw[2], fx[2][MT];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      fw[s] = rw.get(mine + cur, s, 0);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) fx[s][j] = rx.get(mine + cur + kW, s, j);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage is read: its place can be loaded again
+    lw.load(cur, kleft - NS * kFewWaves * S::kK, lane);
+    lx.load(cur, kleft - NS * kFewWaves * S::kK, lane);
+    lw.next();
+    lx.next();
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) acc[j] = mfma16<T>(fw[s], fx[s][j], acc[j]);
+    cur = cur == (NS - 1) * kStage ? 0 : cur + kStage;
+  }
+  wait_loads<0>();
+  __syncthreads();
+  join_waves<T, MT>(acc, reinterpret_cast<float*>(smem), M, n0, N, e);
+}
+
+// The same for rows that start anywhere: fragments straight from memory, with
+// kDepth steps of loads under way.
 template <typename T>
 MHC_DEV u32x4 load_any(const T* p) {
   u32x4 v;
@@ -512,11 +696,11 @@ MHC_DEV u32x4 load_end(const T* p, int left) {
 }
 
 template <typename T, int MT>
-__global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const T* x, int64_t ldx, const T* w, int64_t ldw, int M, int64_t N,
-                                                                  int K, const Epilogue e) {
+__global__ __launch_bounds__(64 * kFewWaves) void few_ragged_rows_kernel(const T* x, int64_t ldx, const T* w, int64_t ldw, int M,
+                                                                         int64_t N, int K, const Epilogue e) {
   constexpr int kE = 16 / (int)sizeof(T), kStep = 4 * kE;  // k of a step: a chunk for each of four groups of lanes
   constexpr int kDepth = MT == 1 ? 8 : MT == 2 ? 4 : 2;
-  __shared__ __attribute__((aligned(16))) float sums[kFewWaves][MT * 16][16];
+  __shared__ __attribute__((aligned(16))) float sums[kFewWaves * MT * 256];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, r = lane & 15, g = lane >> 4;
   const int64_t n0 = (int64_t)blockIdx.x * 16;
   // (lanes of rows that are not there read another one; their sums are not stored)
@@ -546,28 +730,28 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const T* x, in
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[j] = mfma16<T>(fw, full ? load_any(xr[j] + k) : load_end(xr[j] + k, left), acc[j]);
   }
-#pragma unroll
-  for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(&sums[wave][j * 16 + r][g * 4]) = acc[j];
-  __syncthreads();
-  for (int at = threadIdx.x; at < MT * 256; at += 64 * kFewWaves) {
-    const int m = at / 16, n = at % 16;
-    float z[1] = {0.f};
-#pragma unroll
-    for (int v = 0; v < kFewWaves; ++v) z[0] += sums[v][m][n];
-    if (m < M && n0 + n < N) finish<T>(e, m, n0 + n, N, z);
-  }
+  join_waves<T, MT>(acc, sums, M, n0, N, e);
+}
+
+template <typename T, int MT>
+int launch_few_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K, const Epilogue& e, hipStream_t s) {
+  const dim3 grid((unsigned)ceil_div(N, 16)), block(64 * kFewWaves);
+  // (more stages under way in fewer workgroups of a CU: 5.4 for 4.9 us at one row of 4096 x 4096, 10.1 for 8.6 at 32 of 8192 x 2048)
+  if (in_words(x, ldx, K, sizeof(T)) && in_words(w, ldw, K, sizeof(T)))
+    hipLaunchKernelGGL((few_rows_kernel<T, MT, MT == 1 ? 2 : 1>), grid, block, 0, s, Operand{x, ldx, K}, Operand{w, ldw, K}, (int)M, N,
+                       (int)K, e);
+  else
+    hipLaunchKernelGGL((few_ragged_rows_kernel<T, MT>), grid, block, 0, s, static_cast<const T*>(x), ldx, static_cast<const T*>(w), ldw,
+                       (int)M, N, (int)K, e);
+  MHC_CHECK_LAUNCH("few_rows_kernel");
+  return MHC_OK;
 }
 
 template <typename T>
 int run_few_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K, const Epilogue& e, hipStream_t s) {
-  const dim3 grid((unsigned)ceil_div(N, 16)), block(64 * kFewWaves);
-  const T* const xt = static_cast<const T*>(x);
-  const T* const wt = static_cast<const T*>(w);
-  if (M <= 16) hipLaunchKernelGGL((few_rows_kernel<T, 1>), grid, block, 0, s, xt, ldx, wt, ldw, (int)M, N, (int)K, e);
-  else if (M <= 32) hipLaunchKernelGGL((few_rows_kernel<T, 2>), grid, block, 0, s, xt, ldx, wt, ldw, (int)M, N, (int)K, e);
-  else hipLaunchKernelGGL((few_rows_kernel<T, 4>), grid, block, 0, s, xt, ldx, wt, ldw, (int)M, N, (int)K, e);
-  MHC_CHECK_LAUNCH("few_rows_kernel");
-  return MHC_OK;
+  if (M <= 16) return launch_few_rows<T, 1>(x, ldx, w, ldw, M, N, K, e, s);
+  if (M <= 32) return launch_few_rows<T, 2>(x, ldx, w, ldw, M, N, K, e, s);
+  return launch_few_rows<T, 4>(x, ldx, w, ldw, M, N, K, e, s);
 }
 
 // The sum over the splits, in order, and the epilogue.
@@ -576,13 +760,17 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, int splits
   const int64_t total = M * N / V;
   for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * 256) {
     const int64_t m = at * V / N, n = at * V % N;
-    float z[V] = {};
+    float z[1][V] = {}, bias[V], residual[1][V];
+    bias_of<T>(e, n, bias);
+    residual_of<T>(e, m, 0, M, n, N, residual);
+#pragma unroll 4
     for (int k = 0; k < splits; ++k) {
-      const float* const p = part + ((int64_t)k * M + m) * N + n;
-      if constexpr (V == 1) z[0] += *p;
-      else add(p, z);
+      float v[V];
+      take(part + ((int64_t)k * M + m) * N + n, v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) z[0][j] += v[j];
     }
-    finish<T>(e, m, n, N, z);
+    finish<T>(e, m, 0, M, n, N, z, bias, residual);
   }
 }
 
@@ -600,6 +788,7 @@ int launch_join(const Epilogue& e, const float* part, int splits, int64_t M, int
   const unsigned blocks = (unsigned)std::min(ceil_div(M * N / e.vec, 256), (int64_t)device_cu_count() * 16);
   if (e.vec == 8) hipLaunchKernelGGL((join_kernel<T, 8>), dim3(blocks), dim3(256), 0, s, part, splits, M, N, e);
   else if (e.vec == 4) hipLaunchKernelGGL((join_kernel<T, 4>), dim3(blocks), dim3(256), 0, s, part, splits, M, N, e);
+  else if (e.vec == 2) hipLaunchKernelGGL((join_kernel<T, 2>), dim3(blocks), dim3(256), 0, s, part, splits, M, N, e);
   else hipLaunchKernelGGL((join_kernel<T, 1>), dim3(blocks), dim3(256), 0, s, part, splits, M, N, e);
   MHC_CHECK_LAUNCH("join_kernel");
   return MHC_OK;
@@ -608,21 +797,23 @@ int launch_join(const Epilogue& e, const float* part, int splits, int64_t M, int
 // How a product is cut up: its tile, and into how many parts its reduction.
 struct Cut {
   int tile, splits, kper;
+  float us;  // estimated
 };
 
-// The tiles, and what a stage of them takes in us on an MI355X: `alone` with
+// The tiles, and what they take in us on an MI355X: `ends` for the launch, the
+// first loads and the outputs, and a stage `alone` with
 // few workgroups on the card (its latencies), `busy` for each workgroup of a
 // CU that has `fit` of them (its matrix instructions and LDS reads).  From
-// x W^T over 64 to 512 stages: 256 x 256 16-bit at 1.18 alone, 1.6 with all
+// x W^T over 16 to 512 stages: 256 x 256 16-bit at 1.12 alone, 1.6 with all
 // CUs at it (1.3 PFLOP/s); fp32 stages have half the k at 1/16 the rate.
 struct TileCost {
   int bm, bn, fit;
-  float alone16, busy16, alone32, busy32;
+  float ends, alone16, busy16, alone32, busy32;
 };
 constexpr TileCost kTiles[] = {
-    {256, 256, 1, 1.18f, 1.60f, 7.20f, 7.35f}, {128, 256, 1, 0.71f, 0.92f, 3.68f, 3.84f},
-    {128, 128, 2, 0.57f, 0.54f, 1.96f, 1.88f}, {64, 128, 2, 0.43f, 0.34f, 1.07f, 0.98f},
-    {64, 64, 3, 0.26f, 0.21f, 0.57f, 0.53f},
+    {256, 256, 1, 7.0f, 1.12f, 1.60f, 7.17f, 7.35f},   {128, 256, 1, 5.0f, 0.68f, 0.92f, 3.66f, 3.84f},
+    {128, 128, 2, 5.0f, 0.545f, 0.54f, 1.95f, 1.88f},  {64, 128, 2, 4.5f, 0.40f, 0.34f, 1.05f, 0.98f},
+    {64, 64, 3, 3.6f, 0.245f, 0.21f, 0.555f, 0.53f},
 };
 
 // The cut with the least estimated time.  Large tiles read least, small ones
@@ -633,8 +824,7 @@ inline Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype) {
   const int kK = f32 ? 32 : 64;
   const int stages = (int)ceil_div(K, kK);
   const float cus = (float)device_cu_count();
-  Cut best = {0, 1, stages * kK};
-  float least = 0.f;
+  Cut best = {0, 1, stages * kK, 0.f};
   for (int t = 0; t < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++t) {
     const TileCost& c = kTiles[t];
     const float tiles = (float)ceil_div(M, c.bm) * (float)ceil_div(N, c.bn);
@@ -645,15 +835,30 @@ inline Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype) {
       if (splits < want) continue;
       const float of_cu = tiles * splits / cus, q = ceilf(of_cu);  // workgroups of a CU
       const float stage = of_cu <= 1.f ? alone + std::max(0.f, busy - alone) * of_cu : std::max(alone * ceilf(q / c.fit), busy * q);
-      float us = 3.f + per * stage;
+      float us = c.ends + per * stage;
       if (splits > 1) us += 4.f + 2.f * splits * (float)M * (float)N / 1e6f;  // 8 bytes each at 4 TB/s
-      if (least == 0.f || us < least) {
-        least = us;
-        best = {t, splits, per * kK};
-      }
+      if (best.us == 0.f || us < best.us) best = {t, splits, per * kK, us};
     }
   }
   return best;
+}
+
+// Whether x W^T goes to the kernels for few rows: up to 64 of them, unless a
+// tile is estimated faster (33 to 64 rows of a W of over some 30 M elements,
+// or with short rows: 8192 x 8192 bf16 35 us here, 27 in tiles; 16384 x 1024
+// 14 and 8).  From one to four workgroups of a CU; per stage of a wave:
+// 0.35, 0.65, 1.05 us for 16, 32, 64 rows (fp32: 0.8, 1.1, 1.5).
+inline bool few_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K, int dtype) {
+  if (M > 64) return false;
+  const bool f32 = dtype == kF32;
+  const int bytes = f32 ? 4 : 2;
+  const bool words = in_words(x, ldx, K, bytes) && in_words(w, ldw, K, bytes);
+  const float stage = f32 ? (M <= 16 ? 0.8f : M <= 32 ? 1.1f : 1.5f) : (M <= 16 ? 0.35f : M <= 32 ? 0.65f : 1.05f);
+  const float of_cu = std::max(1.f, (float)N / 16.f / (float)device_cu_count());
+  const float few = 3.f + of_cu * (float)ceil_div(K * bytes, 128 * kFewWaves) * stage * (words ? 1.f : 1.8f);
+  // (tiles need copies of rows that are no whole words: two launches and the operands' way out and in)
+  const float copies = words ? 0.f : 9.f + 2.f * (float)((M + N) * K * bytes) / 4e6f;
+  return few <= cut_of(M, N, K, dtype).us + copies;
 }
 
 template <typename T, bool AK, bool BK>
