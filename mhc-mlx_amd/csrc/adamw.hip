@@ -13,7 +13,7 @@
 // to a few of millions.  Up to kMaxTensors of them go into one launch: their
 // pointers travel in the kernel arguments (no table in device memory that a
 // captured graph or a later step could find changed), and a workgroup finds
-// its tensor by bisection over the chunk counts, on the scalar unit.
+// its tensor with one load of the chunk counts, a lane each, and a vote.
 #include <cmath>
 
 #include "mhc_device.hpp"
@@ -25,7 +25,8 @@ namespace {
 constexpr int kMaxTensors = 60;   // 60 * (56 + 4) bytes of arguments: the limit is 4096
 constexpr int kThreads = 256;
 constexpr int kQuant = 256;       // elements that share a scale: one wave, four elements a lane
-constexpr int kChunk = 4096;      // elements of one workgroup
+constexpr int kPass = kThreads * 4;  // elements that a workgroup has at a time
+constexpr int kChunk = 4 * kPass; // elements of one workgroup (kPass in a call too small to fill the card: four passes take 5 us)
 constexpr int64_t kMaxChunks = 1 << 23;  // workgroups of a launch: its threads stay below 2^31
 constexpr float kCodeMax = 448.f; // largest e4m3 value
 constexpr float kMinTop = 0x1p-100f;  // least largest value of a block: its scale's inverse stays finite
@@ -38,7 +39,7 @@ struct Hyper {
 struct Table {
   mhc_adamw_tensor t[kMaxTensors];
   int32_t end[kMaxTensors];  // chunks of the tensors up to and with this one
-  int32_t count;
+  int32_t count, chunk;      // elements of a chunk
   Hyper h;
 };
 static_assert(sizeof(Table) <= 4096, "kernel arguments");
@@ -128,15 +129,12 @@ MHC_DEV bool lines_up(const void* p, int bytes) { return ((uintptr_t)p & (uintpt
 template <typename P, bool MASTER, bool Q8>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(const Table tab) {
 #pragma clang fp contract(off)
-  const int chunk = (int)blockIdx.x;
-  int lo = 0, hi = tab.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (tab.end[mid] > chunk) hi = mid;
-    else lo = mid + 1;
-  }
+  const int chunk = (int)blockIdx.x, lane = (int)threadIdx.x % kWave;
+  static_assert(kMaxTensors <= kWave, "a lane for each tensor");
+  const uint64_t past = __ballot(lane < tab.count && tab.end[min(lane, kMaxTensors - 1)] > chunk);
+  const int lo = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(past));
   const mhc_adamw_tensor& t = tab.t[lo];
-  const int64_t first = (int64_t)(chunk - (lo > 0 ? tab.end[lo - 1] : 0)) * kChunk;
+  const int64_t first = (int64_t)(chunk - (lo > 0 ? tab.end[lo - 1] : 0)) * tab.chunk;
   P* const p = static_cast<P*>(t.param);
   const P* const g = static_cast<const P*>(t.grad);
   const Hyper& h = tab.h;
@@ -147,7 +145,7 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Table tab) {
                        : lines_up(t.exp_avg, 16) && lines_up(t.exp_avg_sq, 16);
   const bool mvec = !MASTER || lines_up(t.master, 16);
 
-  for (int64_t i = first + threadIdx.x * 4; i < first + kChunk; i += kThreads * 4) {
+  for (int64_t i = first + threadIdx.x * 4; i < first + tab.chunk; i += kPass) {
     // a wave's 256 elements are one block of an 8-bit state; its lanes past the end take part with zeros
     const int left = (int)min((int64_t)4, t.numel - i);
     if (t.numel - (i - (threadIdx.x % kWave) * 4) <= 0) break;
@@ -253,11 +251,14 @@ extern "C" int mhc_adamw_step(const mhc_adamw_tensor* tensors, int64_t count, in
                 (float)(1.0 - beta2),             (float)(1.0 / std::sqrt(bc2)), (float)eps, (float)(lr / bc1),
                 (float)grad_scale,                grad_scale_ptr};
   tab.count = 0;
+  int64_t total = 0;
+  for (int64_t i = 0; i < count; ++i) total += tensors[i].numel;
+  tab.chunk = total < (int64_t)device_cu_count() * 8 * kChunk ? kPass : kChunk;
   hipStream_t s = static_cast<hipStream_t>(stream);
   int64_t chunks = 0;
   for (int64_t i = 0; i < count; ++i) {
     if (tensors[i].numel == 0) continue;
-    const int64_t mine = ceil_div(tensors[i].numel, kChunk);
+    const int64_t mine = ceil_div(tensors[i].numel, tab.chunk);
     if (tab.count == kMaxTensors || (tab.count > 0 && chunks + mine > kMaxChunks)) {
       if (const int rc = launch_table(tab, dtype, master, q8, s)) return rc;
       tab.count = 0;

@@ -10,7 +10,7 @@
 #include <torch/extension.h>
 
 #include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/VariableTypeUtils.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include "mhc_hip.h"
@@ -367,95 +367,126 @@ std::tuple<at::Tensor, at::Tensor> policy_loss(const at::Tensor& logits, const a
 // AdamW
 // ---------------------------------------------------------------------------
 
-using TensorList = std::vector<at::Tensor>;
-using OptList = c10::optional<std::vector<OptTensor>>;
+// A Python list or tuple of tensors, read in place: hundreds of them would
+// take longer to convert than the step takes.
+struct TensorSeq {
+  PyObject* seq = nullptr;  // borrowed from the caller's argument, or the fast sequence of it
+  py::object held;
+
+  TensorSeq(const py::object& o, const char* name) {
+    if (o.is_none()) return;
+    held = py::reinterpret_steal<py::object>(PySequence_Fast(o.ptr(), ""));
+    if (!held) {
+      PyErr_Clear();
+      TORCH_CHECK_VALUE(false, name, " must be a list of tensors");
+    }
+    seq = held.ptr();
+  }
+  bool given() const { return seq != nullptr; }
+  size_t size() const { return (size_t)PySequence_Fast_GET_SIZE(seq); }
+  // entry i, or nullptr for None
+  const at::Tensor* get(size_t i, const char* name) const {
+    PyObject* o = PySequence_Fast_GET_ITEM(seq, (Py_ssize_t)i);
+    if (o == Py_None) return nullptr;
+    TORCH_CHECK_VALUE(THPVariable_Check(o), name, "[", i, "] is no tensor");
+    return &THPVariable_Unpack(o);
+  }
+  const at::Tensor& at(size_t i, const char* name) const {
+    const at::Tensor* t = get(i, name);
+    TORCH_CHECK_VALUE(t != nullptr, name, "[", i, "] is None");
+    return *t;
+  }
+};
 
 // elements in the same order in memory, without holes
 bool same_layout(const at::Tensor& a, const at::Tensor& b) {
   return a.sizes() == b.sizes() && (a.strides() == b.strides() || (a.is_contiguous() && b.is_contiguous()));
 }
 
-// A tensor written by a kernel counts as modified, for graphs that saved it.
-void modified(const at::Tensor& t) {
-  if (!t.is_inference()) torch::autograd::impl::bump_version(t);
-}
 
-void adamw_step(const TensorList& params, const TensorList& grads, const TensorList& exp_avgs, const TensorList& exp_avg_sqs,
-                const OptList& masters, const OptList& scales, int64_t step, double lr, double beta1, double beta2, double eps,
+void adamw_step(const py::object& params_, const py::object& grads_, const py::object& exp_avgs_, const py::object& exp_avg_sqs_,
+                const py::object& masters_, const py::object& scales_, int64_t step, double lr, double beta1, double beta2, double eps,
                 double weight_decay, double grad_scale, const OptTensor& grad_scale_tensor) {
+  const TensorSeq params(params_, "params"), grads(grads_, "grads"), exp_avgs(exp_avgs_, "exp_avgs"),
+      exp_avg_sqs(exp_avg_sqs_, "exp_avg_sqs"), masters(masters_, "masters"), scales(scales_, "scales");
+  TORCH_CHECK_VALUE(params.given() && grads.given() && exp_avgs.given() && exp_avg_sqs.given(),
+                    "params, grads, exp_avgs and exp_avg_sqs must be lists of tensors");
   const size_t n = params.size();
-  const auto same = [&](size_t k, const char* name) {
-    TORCH_CHECK_VALUE(k == n, name, " must have one entry for each of the ", n, " params, got ", k);
+  const auto same = [&](const TensorSeq& s, const char* name) {
+    TORCH_CHECK_VALUE(!s.given() || s.size() == n, name, " must have one entry for each of the ", n, " params, got ", s.size());
   };
-  same(grads.size(), "grads");
-  same(exp_avgs.size(), "exp_avgs");
-  same(exp_avg_sqs.size(), "exp_avg_sqs");
-  if (masters.has_value()) same(masters->size(), "masters");
-  if (scales.has_value()) same(scales->size(), "scales");
+  same(grads, "grads");
+  same(exp_avgs, "exp_avgs");
+  same(exp_avg_sqs, "exp_avg_sqs");
+  same(masters, "masters");
+  same(scales, "scales");
   if (n == 0) return;
-  const at::Device dev = params[0].device();
+  const at::Device dev = params.at(0, "params").device();
   TORCH_CHECK_VALUE(dev.is_cuda(), "the HIP path needs GPU tensors (got params[0] on ", dev, ")");
-  const bool q8 = scales.has_value();
-  TensorList held;  // gradients brought into their parameter's layout
+  const bool q8 = scales.given();
+  const at::ScalarType st = q8 ? at::kFloat8_e4m3fn : at::kFloat;
+  std::vector<at::Tensor> held;  // gradients brought into their parameter's layout
   // one call of the library for each kind: dtype, and with or without a master copy
   std::vector<mhc_adamw_tensor> of[6];
+  std::vector<c10::TensorImpl*> written;
+  written.reserve(n * (3 + masters.given() + q8));
+  const auto bytes = [&](const at::Tensor& t) {  // of a tensor that the step writes
+    written.push_back(t.unsafeGetTensorImpl());
+    return t.unsafeGetTensorImpl()->mutable_data();
+  };
   for (size_t i = 0; i < n; ++i) {
-    const at::Tensor &p = params[i], &m = exp_avgs[i], &v = exp_avg_sqs[i];
-    at::Tensor g = grads[i];
+    const at::Tensor &p = params.at(i, "params"), &m = exp_avgs.at(i, "exp_avgs"), &v = exp_avg_sqs.at(i, "exp_avg_sqs");
+    const at::Tensor* g = &grads.at(i, "grads");
     const int code = dtype_code(p.scalar_type(), "params");
-    TORCH_CHECK_VALUE(p.layout() == at::kStrided && g.layout() == at::kStrided, "tensor ", i, ": params and grads must be dense");
-    TORCH_CHECK_VALUE(p.device() == dev && g.device() == dev && m.device() == dev && v.device() == dev, "tensor ", i,
+    TORCH_CHECK_VALUE(p.layout() == at::kStrided && g->layout() == at::kStrided, "tensor ", i, ": params and grads must be dense");
+    TORCH_CHECK_VALUE(p.device() == dev && g->device() == dev && m.device() == dev && v.device() == dev, "tensor ", i,
                       ": every tensor must be on ", dev);
     TORCH_CHECK_VALUE(p.is_non_overlapping_and_dense(), "tensor ", i, ": params must have their elements without holes or overlaps, got shape ",
                       p.sizes(), " with strides ", p.strides());
-    TORCH_CHECK_VALUE(g.sizes() == p.sizes() && g.scalar_type() == p.scalar_type(), "tensor ", i, ": the gradient must have the parameter's shape ",
-                      p.sizes(), " and dtype ", p.scalar_type(), ", got ", g.sizes(), " ", g.scalar_type());
-    const at::ScalarType st = q8 ? at::kFloat8_e4m3fn : at::kFloat;
+    TORCH_CHECK_VALUE(g->sizes() == p.sizes() && g->scalar_type() == p.scalar_type(), "tensor ", i,
+                      ": the gradient must have the parameter's shape ", p.sizes(), " and dtype ", p.scalar_type(), ", got ", g->sizes(), " ",
+                      g->scalar_type());
     TORCH_CHECK_VALUE(m.scalar_type() == st && v.scalar_type() == st && same_layout(p, m) && same_layout(p, v), "tensor ", i,
                       ": the states must be ", st, " in the parameter's shape and layout");
-    if (!same_layout(p, g)) {
-      g = at::empty_like(p).copy_(g);
-      held.push_back(g);
+    if (!same_layout(p, *g)) {
+      held.push_back(at::empty_like(p).copy_(*g));
+      g = &held.back();
     }
-    mhc_adamw_tensor t = {p.data_ptr(), g.data_ptr(), nullptr, m.data_ptr(), v.data_ptr(), nullptr, p.numel()};
-    if (masters.has_value() && (*masters)[i].has_value()) {
-      const at::Tensor& w = *(*masters)[i];
-      TORCH_CHECK_VALUE(code != MHC_DTYPE_F32, "tensor ", i, ": a master copy is for 16-bit parameters");
-      TORCH_CHECK_VALUE(w.device() == dev && w.scalar_type() == at::kFloat && same_layout(p, w), "tensor ", i,
-                        ": the master copy must be float32 in the parameter's shape and layout");
-      t.master = w.data_ptr<float>();
+    mhc_adamw_tensor t = {bytes(p), g->const_data_ptr(), nullptr, bytes(m), bytes(v), nullptr, p.numel()};
+    if (masters.given()) {
+      if (const at::Tensor* w = masters.get(i, "masters")) {
+        TORCH_CHECK_VALUE(code != MHC_DTYPE_F32, "tensor ", i, ": a master copy is for 16-bit parameters");
+        TORCH_CHECK_VALUE(w->device() == dev && w->scalar_type() == at::kFloat && same_layout(p, *w), "tensor ", i,
+                          ": the master copy must be float32 in the parameter's shape and layout");
+        t.master = static_cast<float*>(bytes(*w));
+      }
     }
     if (q8) {
       const int64_t want = 2 * ((p.numel() + 255) / 256);
-      TORCH_CHECK_VALUE((*scales)[i].has_value(), "tensor ", i, ": states in 8 bits need scales");
-      const at::Tensor& s = *(*scales)[i];
+      const at::Tensor& s = scales.at(i, "scales");
       TORCH_CHECK_VALUE(s.device() == dev && s.scalar_type() == at::kFloat && s.is_contiguous() && s.numel() == want, "tensor ", i,
                         ": scales must be contiguous float32 [ceil(numel / 256), 2] on ", dev);
-      t.scales = s.data_ptr<float>();
+      t.scales = static_cast<float*>(bytes(s));
     }
+    if (of[2 * code + (t.master != nullptr)].empty()) of[2 * code + (t.master != nullptr)].reserve(n);
     of[2 * code + (t.master != nullptr)].push_back(t);
   }
   const float* gs = nullptr;
-  at::Tensor gst;
   if (grad_scale_tensor.has_value()) {
-    gst = *grad_scale_tensor;
+    const at::Tensor& gst = *grad_scale_tensor;
     TORCH_CHECK_VALUE(gst.device() == dev && gst.numel() == 1 && gst.scalar_type() == at::kFloat, "grad_scale must be a number or one float32 on ",
                       dev);
     gs = gst.data_ptr<float>();
   }
   const at::DeviceGuard guard(dev);
+  void* const stream = c10::hip::getCurrentHIPStream(dev.index()).stream();
   for (int k = 0; k < 6; ++k)
     if (!of[k].empty())
       check(mhc_adamw_step(of[k].data(), (int64_t)of[k].size(), k / 2, q8 ? 8 : 32, lr, beta1, beta2, eps, weight_decay, step,
-                           grad_scale, gs, stream_of(params[0])),
+                           grad_scale, gs, stream),
             "mhc_adamw_step");
-  for (size_t i = 0; i < n; ++i) {
-    modified(params[i]);
-    modified(exp_avgs[i]);
-    modified(exp_avg_sqs[i]);
-    if (masters.has_value() && (*masters)[i].has_value()) modified(*(*masters)[i]);
-    if (q8) modified(*(*scales)[i]);
-  }
+  for (c10::TensorImpl* t : written)  // modified, for graphs that saved it
+    if (!t->is_inference()) t->bump_version();
 }
 
 }  // namespace
