@@ -13,74 +13,53 @@ using gemm::Operand;
 using gemm::Product;
 
 constexpr int kDzCols = 64 * 8;   // columns of a workgroup of dz_kernel: eight for each lane of a wave
-constexpr int kDzRows = 64;       // rows: sixteen for each wave
+
+// rows of a workgroup: sixteen for each wave, four where those would be too few to fill the card
+int dz_rows(int64_t M, int64_t N) { return ceil_div(M, 64) * ceil_div(N, kDzCols) < 2 * device_cu_count() ? 16 : 64; }
 
 // dz = dout dact (dact NULL: dout), rounded to T, in rows of N elements `ld`
-// apart with zeros between (not stored if dz is NULL), and sums of dz over
-// this workgroup's rows, before rounding, to part[block of rows][N] (if not
-// NULL).  One pass at the card's streaming rate: a lane has eight consecutive
-// columns (VEC: every array's are 16-byte vectors), else eight 64 apart, of
-// every fourth row, four of which are loaded at a time.
-template <typename T, typename G, bool VEC>
-__global__ __launch_bounds__(256) void dz_kernel(const G* dout, const void* dact, T* dz, int64_t ld, float* part, int64_t M,
-                                                 int64_t N) {
-  using D = typename gemm::DactOf<T>::Type;
-  __shared__ float lds[4][kDzCols];
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int64_t n0 = (int64_t)blockIdx.x * kDzCols, m0 = (int64_t)blockIdx.y * kDzRows;
-  const auto column = [&](int k) { return VEC ? lane * 8 + k : k * kWave + lane; };
-  const D* const d = static_cast<const D*>(dact);
-  float sum[8] = {};
-  const bool in = !VEC || n0 + lane * 8 < N;
-  for (int64_t m = m0 + wave; in && m < min(m0 + kDzRows, M); m += 16) {
+// (a multiple of eight) apart with zeros between (not stored if dz is NULL),
+// and sums of dz over this workgroup's rows, before rounding, to
+// part[block of rows][N] (if not NULL).  One pass at the card's streaming
+// rate: a lane has eight columns of every fourth row, and loads four rows at
+// a time.
+template <typename T, typename G, bool WHOLE>
+MHC_DEV void dz_columns(const G* dout, const typename gemm::DactOf<T>::Type* d, T* dz, int64_t ld, int64_t m0, int64_t m1, int64_t n,
+                        int64_t N, int left, float (&sum)[8]) {
+  for (int64_t m = m0; m < m1; m += 16) {
     float v[4][8], f[4][8];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int64_t row = min(m + 4 * q, M - 1);
-      if constexpr (VEC) {
-        gemm::take(dout + row * N + n0 + lane * 8, v[q]);
-        if (d != nullptr) {
-          if constexpr (sizeof(D) == 4) {
-            gemm::take(d + row * N + n0 + lane * 8, f[q]);
-          } else {
-            const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(d + row * N + n0 + lane * 8));
+    for (int q = 0; q < 4; ++q) gemm::take<WHOLE>(dout + min(m + 4 * q, m1 - 1) * N + n, v[q], left);
+    if (d != nullptr) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) f[q][k] = gemm::dact_value((int16_t)(w[k / 2] >> (16 * (k % 2))));
-          }
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int64_t at = row * N + min(n0 + column(k), N - 1);
-          v[q][k] = load1(dout + at);
-          if (d != nullptr) f[q][k] = gemm::dact_value(d[at]);
-        }
-      }
+      for (int q = 0; q < 4; ++q) gemm::take_dact<WHOLE>(d + min(m + 4 * q, m1 - 1) * N + n, f[q], left);
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int64_t row = m + 4 * q;
-      if (row >= min(m0 + kDzRows, M)) break;
+      if (m + 4 * q >= m1) break;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        if (d != nullptr) v[q][k] *= f[q][k];
+        if (d != nullptr) v[q][k] *= f[q][k];  // (not WHOLE: zeros from `left` on)
         sum[k] += v[q][k];
       }
-      if (dz == nullptr) continue;
-      if constexpr (VEC) {
-        gemm::put(dz + row * ld + n0 + lane * 8, v[q]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int64_t n = n0 + column(k);
-          if (n < ld) store1(dz + row * ld + n, n < N ? v[q][k] : 0.f);
-        }
-      }
+      if (dz != nullptr) gemm::put<true>(dz + (m + 4 * q) * ld + n, v[q], 8);
     }
   }
+}
+
+template <typename T, typename G>
+__global__ __launch_bounds__(256) void dz_kernel(const G* dout, const void* dact, T* dz, int64_t ld, float* part, int64_t M,
+                                                 int64_t N, int rows) {
+  __shared__ float lds[4][kDzCols];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int64_t n0 = (int64_t)blockIdx.x * kDzCols, n = n0 + lane * 8, m0 = (int64_t)blockIdx.y * rows, m1 = min(m0 + rows, M);
+  const auto* const d = static_cast<const typename gemm::DactOf<T>::Type*>(dact);
+  float sum[8] = {};
+  if (n + 8 <= N) dz_columns<T, G, true>(dout, d, dz, ld, m0 + wave, m1, n, N, 8, sum);
+  else if (n < N) dz_columns<T, G, false>(dout, d, dz, ld, m0 + wave, m1, n, N, (int)(N - n), sum);
   if (part == nullptr) return;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) lds[wave][column(k)] = sum[k];
+  for (int k = 0; k < 8; ++k) lds[wave][lane * 8 + k] = sum[k];
   __syncthreads();
   for (int c = threadIdx.x; c < kDzCols; c += 256)
     if (n0 + c < N) part[(int64_t)blockIdx.y * N + n0 + c] = (lds[0][c] + lds[1][c]) + (lds[2][c] + lds[3][c]);
@@ -142,15 +121,13 @@ size_t part_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
 
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
-int64_t padded(int64_t width, int dtype) {
-  const int64_t e = 16 / elem_bytes(dtype);
-  return (width + e - 1) / e * e;
-}
+// a row's length in a copy: a multiple of eight
+int64_t padded(int64_t width) { return (width + 7) / 8 * 8; }
 
 // bytes of an operand's copy in rows of whole chunks; 0: it is read as it is
 size_t pack_bytes(const void* p, int64_t rows, int64_t ld, int64_t width, int dtype) {
   if (gemm::in_words(p, ld, width, elem_bytes(dtype))) return 0;
-  return up256((size_t)(rows * padded(width, dtype)) * elem_bytes(dtype));
+  return up256((size_t)(rows * padded(width)) * elem_bytes(dtype));
 }
 
 template <typename T>
@@ -170,7 +147,7 @@ int operand(Operand& o, const void* p, int64_t rows, int64_t ld, int64_t width, 
     o = Operand{p, ld, width};
     return MHC_OK;
   }
-  const int64_t wide = padded(width, dtype);
+  const int64_t wide = padded(width);
   o = Operand{ws, wide, wide};
   const int rc = dtype == kF32 ? run_pack<float>(p, ld, ws, rows, width, wide, s)
                                : run_pack<uint16_t>(p, ld, ws, rows, width, wide, s);
@@ -186,8 +163,8 @@ BwdPlan plan_bwd(const void* dout, int dout_dtype, bool dact, const void* x, int
                  bool db, int64_t M, int64_t N, int64_t K, int dtype) {
   BwdPlan b = {};
   if ((dx || dw) && (dact || dout_dtype != dtype || !gemm::in_words(dout, N, N, elem_bytes(dtype))))
-    b.dz = up256((size_t)(M * padded(N, dtype)) * elem_bytes(dtype));
-  if (db) b.part = up256((size_t)(ceil_div(M, kDzRows) * N) * sizeof(float));
+    b.dz = up256((size_t)(M * padded(N)) * elem_bytes(dtype));
+  if (db) b.part = up256((size_t)(ceil_div(M, dz_rows(M, N)) * N) * sizeof(float));
   if (dx) b.w = pack_bytes(w, N, ldw, K, dtype);
   if (dw) b.x = pack_bytes(x, M, ldx, K, dtype);
   b.total = b.dz + b.part + b.x + b.w +
@@ -197,13 +174,10 @@ BwdPlan plan_bwd(const void* dout, int dout_dtype, bool dact, const void* x, int
 
 template <typename T, typename G>
 int run_dz(const void* dout, const void* dact, void* dz, int64_t ld, float* part, void* db, int64_t M, int64_t N, hipStream_t s) {
-  const int64_t blocks = ceil_div(M, kDzRows);
+  const int rows = dz_rows(M, N);
+  const int64_t blocks = ceil_div(M, rows);
   const dim3 grid((unsigned)ceil_div(N, kDzCols), (unsigned)blocks);
-  const G* const g = static_cast<const G*>(dout);
-  if (N % 8 == 0 && aligned(dout, 16) && aligned(dact, 16))
-    hipLaunchKernelGGL((dz_kernel<T, G, true>), grid, dim3(256), 0, s, g, dact, static_cast<T*>(dz), ld, part, M, N);
-  else
-    hipLaunchKernelGGL((dz_kernel<T, G, false>), grid, dim3(256), 0, s, g, dact, static_cast<T*>(dz), ld, part, M, N);
+  hipLaunchKernelGGL((dz_kernel<T, G>), grid, dim3(256), 0, s, static_cast<const G*>(dout), dact, static_cast<T*>(dz), ld, part, M, N, rows);
   MHC_CHECK_LAUNCH("dz_kernel");
   if (db != nullptr) {
     hipLaunchKernelGGL((db_kernel<T>), dim3((unsigned)ceil_div(N, 32)), dim3(256), 0, s, (const float*)part, static_cast<T*>(db),
@@ -248,12 +222,12 @@ extern "C" int mhc_linear_act_fwd(const void* x, int64_t ldx, const void* w, int
   hipStream_t s = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
   if (gemm::few_rows(x, ldx, w, ldw, M, N, K, dtype)) {
-    const gemm::Epilogue e = gemm::epilogue(bias, residual, out, dact, act, out_dtype, dtype, N);
+    const gemm::Epilogue e = gemm::Epilogue{bias, residual, out, dact, act, out_dtype == kF32};
     if (dtype == kF32) return gemm::run_few_rows_f32(x, ldx, w, ldw, M, N, K, e, s);
     if (dtype == kBF16) return gemm::run_few_rows_bf16(x, ldx, w, ldw, M, N, K, e, s);
     return gemm::run_few_rows_f16(x, ldx, w, ldw, M, N, K, e, s);
   }
-  Product p = {{}, {}, M, N, K, gemm::epilogue(bias, residual, out, dact, act, out_dtype, dtype, N), 1, 0};
+  Product p = {{}, {}, M, N, K, gemm::Epilogue{bias, residual, out, dact, act, out_dtype == kF32}, 1, 0};
   if (const int rc = operand(p.a, x, M, ldx, K, dtype, ws, s)) return rc;
   if (const int rc = operand(p.b, w, N, ldw, K, dtype, ws, s)) return rc;
   return run_product(p, true, true, dtype, ws, s);
@@ -287,24 +261,24 @@ extern "C" int mhc_linear_act_bwd(const void* dout, int dout_dtype, const void* 
   float* const part = b.part > 0 ? reinterpret_cast<float*>(ws + b.dz) : nullptr;
   if (dz != nullptr || db != nullptr) {
     int rc;
-    if (dtype == kF32) rc = run_dz<float, float>(dout, dact, dz, padded(N, dtype), part, db, M, N, s);
+    if (dtype == kF32) rc = run_dz<float, float>(dout, dact, dz, padded(N), part, db, M, N, s);
     else if (dtype == kBF16)
-      rc = dout_dtype == kF32 ? run_dz<__bf16, float>(dout, dact, dz, padded(N, dtype), part, db, M, N, s)
-                              : run_dz<__bf16, __bf16>(dout, dact, dz, padded(N, dtype), part, db, M, N, s);
+      rc = dout_dtype == kF32 ? run_dz<__bf16, float>(dout, dact, dz, padded(N), part, db, M, N, s)
+                              : run_dz<__bf16, __bf16>(dout, dact, dz, padded(N), part, db, M, N, s);
     else
-      rc = dout_dtype == kF32 ? run_dz<_Float16, float>(dout, dact, dz, padded(N, dtype), part, db, M, N, s)
-                              : run_dz<_Float16, _Float16>(dout, dact, dz, padded(N, dtype), part, db, M, N, s);
+      rc = dout_dtype == kF32 ? run_dz<_Float16, float>(dout, dact, dz, padded(N), part, db, M, N, s)
+                              : run_dz<_Float16, _Float16>(dout, dact, dz, padded(N), part, db, M, N, s);
     if (rc != MHC_OK) return rc;
   }
   ws += b.dz + b.part;
-  const Operand g = dz != nullptr ? Operand{dz, padded(N, dtype), padded(N, dtype)} : Operand{dout, N, N};
+  const Operand g = dz != nullptr ? Operand{dz, padded(N), padded(N)} : Operand{dout, N, N};
   if (dx != nullptr) {  // dx[m, k] = sum_n dz[m, n] W[n, k]
-    Product p = {g, {}, M, K, N, gemm::epilogue(nullptr, nullptr, dx, nullptr, MHC_ACT_NONE, dtype, dtype, K), 1, 0};
+    Product p = {g, {}, M, K, N, gemm::Epilogue{nullptr, nullptr, dx, nullptr, MHC_ACT_NONE, dtype == kF32}, 1, 0};
     if (const int rc = operand(p.b, w, N, ldw, K, dtype, ws, s)) return rc;
     if (const int rc = run_product(p, true, false, dtype, ws + (dw != nullptr ? b.x : 0), s)) return rc;
   }
   if (dw != nullptr) {  // dw[n, k] = sum_m dz[m, n] x[m, k]
-    Product p = {g, {}, N, K, M, gemm::epilogue(nullptr, nullptr, dw, nullptr, MHC_ACT_NONE, dtype, dtype, K), 1, 0};
+    Product p = {g, {}, N, K, M, gemm::Epilogue{nullptr, nullptr, dw, nullptr, MHC_ACT_NONE, dtype == kF32}, 1, 0};
     if (const int rc = operand(p.b, x, M, ldx, K, dtype, ws, s)) return rc;
     if (const int rc = run_product(p, false, false, dtype, ws, s)) return rc;
   }

@@ -16,6 +16,7 @@ namespace gemm {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));  // sixteen bytes that start at any element
 
 // --------------------------------------------------------------------------
 // Epilogue: out = act(sum + bias) + residual, and act' for a backward
@@ -28,19 +29,7 @@ struct Epilogue {
   void* dact;            // [M, N] as DactOf has it, or NULL; act is not none then
   int act;               // MHC_ACT_*
   int out_f32;           // out and residual are fp32, else of the operands' type
-  int vec;               // 8, 4, 2 or 1: so many outputs, from a column that is a multiple of it, are whole vectors of each array
 };
-
-// an epilogue whose `vec` goes by the row length and the addresses (residuals start anywhere)
-inline Epilogue epilogue(const void* bias, const void* residual, void* out, void* dact, int act, int out_dtype, int dtype,
-                         int64_t N) {
-  const int eo = out_dtype == kF32 ? 4 : 2, ed = dtype == kF32 ? 4 : 2;
-  int vec = 8;
-  while (vec > 1 && (N % vec != 0 || !aligned(out, std::min(16, vec * eo)) || !aligned(residual, std::min(16, vec * eo)) ||
-                     !aligned(dact, std::min(16, vec * ed))))
-    vec /= 2;
-  return Epilogue{bias, residual, out, dact, act, out_dtype == kF32, vec};
-}
 
 struct Act {
   float y, d;
@@ -123,42 +112,77 @@ MHC_DEV uint32_t dact_code(float d) {
 MHC_DEV float dact_value(int16_t q) { return q == -32768 ? __builtin_nanf("") : 0.5f + (float)q * 0x1p-15f; }
 MHC_DEV float dact_value(float d) { return d; }
 
-// V values to p, as vectors
-template <typename O, int V>
-MHC_DEV void put(O* p, const float (&z)[V]) {
+// Eight values to or from p, which starts anywhere, as 16-byte vectors (the
+// hardware takes them at any element), or (not WHOLE) those before `left` one
+// by one; or one value.  Callers branch on WHOLE around all of their loads:
+// a load under a condition of its own would be waited for there.
+template <bool WHOLE, typename O, int V>
+MHC_DEV void put(O* p, const float (&z)[V], int left) {
   if constexpr (V == 1) {
     if constexpr (__is_same(O, int16_t)) *p = (int16_t)dact_code(z[0]);
     else store1(p, z[0]);
-  } else if constexpr (sizeof(O) == 4 && V == 2) {
-    *reinterpret_cast<f32x2*>(p) = f32x2{z[0], z[1]};
-  } else if constexpr (sizeof(O) == 4) {
-#pragma unroll
-    for (int k = 0; k < V; k += 4) *reinterpret_cast<f32x4*>(p + k) = f32x4{z[k], z[k + 1], z[k + 2], z[k + 3]};
   } else {
-    typedef uint32_t words __attribute__((ext_vector_type(V / 2)));
-    words w;
+    uint32_t w[V * sizeof(O) / 4];
 #pragma unroll
-    for (int k = 0; k < V / 2; ++k) {
-      if constexpr (__is_same(O, int16_t)) w[k] = dact_code(z[2 * k]) | dact_code(z[2 * k + 1]) << 16;
+    for (int k = 0; k < (int)(V * sizeof(O) / 4); ++k) {
+      if constexpr (sizeof(O) == 4) w[k] = __builtin_bit_cast(uint32_t, (float)z[k]);
+      else if constexpr (__is_same(O, int16_t)) w[k] = dact_code(z[2 * k]) | dact_code(z[2 * k + 1]) << 16;
       else w[k] = pack2<O>(z[2 * k], z[2 * k + 1]);
     }
-    *reinterpret_cast<words*>(p) = w;
+    if constexpr (WHOLE) {
+      __builtin_memcpy(p, w, V * sizeof(O));
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        if (k >= left) break;
+        if constexpr (sizeof(O) == 4) p[k] = __builtin_bit_cast(O, w[k]);
+        else p[k] = __builtin_bit_cast(O, (uint16_t)(w[k / 2] >> (16 * (k % 2))));
+      }
+    }
   }
 }
 
-template <typename O, int V>
-MHC_DEV void take(const O* p, float (&z)[V]) {
-  Vec<O, V> r;
-  r.load(p);
+template <bool WHOLE, typename O, int V>
+MHC_DEV void take(const O* p, float (&z)[V], int left) {
+  if constexpr (V == 1) {
+    z[0] = load1(p);
+  } else {
+    Vec<O, V> r;
+    if constexpr (WHOLE) {
 #pragma unroll
-  for (int k = 0; k < V; ++k) z[k] = r.get(k);
+      for (int k = 0; k < (int)(V * sizeof(O) / 16); ++k) {
+        const u32x4 u = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p) + k);
+        r.w[4 * k] = u.x, r.w[4 * k + 1] = u.y, r.w[4 * k + 2] = u.z, r.w[4 * k + 3] = u.w;
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) z[k] = r.get(k);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k) z[k] = k < left ? load1(p + k) : 0.f;
+    }
+  }
 }
 
-// The residuals of V outputs from column n on, of R rows `step` apart from
-// row m on (of the last row past the end; zeros without a residual): all of
-// them loaded before the first is used.
-template <typename T, int V, int R>
-MHC_DEV void residual_of(const Epilogue& e, int64_t m, int step, int64_t M, int64_t n, int64_t N, float (&r)[R][V]) {
+// act' as put() stored it
+template <bool WHOLE, typename D, int V>
+MHC_DEV void take_dact(const D* p, float (&z)[V], int left) {
+  if constexpr (sizeof(D) == 4) {
+    take<WHOLE>(p, z, left);
+  } else if constexpr (WHOLE) {
+    const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
+#pragma unroll
+    for (int k = 0; k < V; ++k) z[k] = dact_value((int16_t)(w[k / 2] >> (16 * (k % 2))));
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) z[k] = k < left ? dact_value(p[k]) : 0.f;
+  }
+}
+
+// The residuals of V outputs from column n on (those before `left`), of R rows
+// `step` apart from row m on (of the last row past the end; zeros without a
+// residual): all of them loaded before the first is used.
+template <typename T, bool WHOLE, int V, int R>
+MHC_DEV void residual_of(const Epilogue& e, int64_t m, int step, int64_t M, int64_t n, int64_t N, int left, float (&r)[R][V]) {
   if (e.residual == nullptr) {
 #pragma unroll
     for (int b = 0; b < R; ++b)
@@ -166,24 +190,24 @@ MHC_DEV void residual_of(const Epilogue& e, int64_t m, int step, int64_t M, int6
       for (int k = 0; k < V; ++k) r[b][k] = 0.f;
   } else if (e.out_f32) {
 #pragma unroll
-    for (int b = 0; b < R; ++b) take(static_cast<const float*>(e.residual) + min(m + b * step, M - 1) * N + n, r[b]);
+    for (int b = 0; b < R; ++b) take<WHOLE>(static_cast<const float*>(e.residual) + min(m + b * step, M - 1) * N + n, r[b], left);
   } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int b = 0; b < R; ++b) take(static_cast<const T*>(e.residual) + min(m + b * step, M - 1) * N + n, r[b]);
+    for (int b = 0; b < R; ++b) take<WHOLE>(static_cast<const T*>(e.residual) + min(m + b * step, M - 1) * N + n, r[b], left);
   }
 }
 
 template <typename T, int V>
-MHC_DEV void bias_of(const Epilogue& e, int64_t n, float (&b)[V]) {
+MHC_DEV void bias_of(const Epilogue& e, int64_t n, int left, float (&b)[V]) {
 #pragma unroll
-  for (int k = 0; k < V; ++k) b[k] = e.bias != nullptr ? load1(static_cast<const T*>(e.bias) + n + k) : 0.f;
+  for (int k = 0; k < V; ++k) b[k] = e.bias != nullptr && k < left ? load1(static_cast<const T*>(e.bias) + n + k) : 0.f;
 }
 
-// The outputs of R rows `step` apart from row m on, V from column n on, from
-// their sums; V > 1: each array's are whole vectors.
-template <typename T, int V, int R>
-MHC_DEV void finish(const Epilogue& e, int64_t m, int step, int64_t M, int64_t n, int64_t N, float (&z)[R][V], const float (&bias)[V],
-                    const float (&residual)[R][V]) {
+// The outputs of R rows `step` apart from row m on, V from column n on (those
+// before `left`), from their sums.
+template <typename T, bool WHOLE, int V, int R>
+MHC_DEV void finish(const Epilogue& e, int64_t m, int step, int64_t M, int64_t n, int64_t N, int left, float (&z)[R][V],
+                    const float (&bias)[V], const float (&residual)[R][V]) {
   float d[R][V];
 #pragma unroll
   for (int b = 0; b < R; ++b)
@@ -194,11 +218,11 @@ MHC_DEV void finish(const Epilogue& e, int64_t m, int step, int64_t M, int64_t n
   for (int b = 0; b < R; ++b) {
     if (m + b * step >= M) break;
     const int64_t at = (m + b * step) * N + n;
-    if (e.dact != nullptr) put(static_cast<typename DactOf<T>::Type*>(e.dact) + at, d[b]);
+    if (e.dact != nullptr) put<WHOLE>(static_cast<typename DactOf<T>::Type*>(e.dact) + at, d[b], left);
 #pragma unroll
     for (int k = 0; k < V; ++k) z[b][k] += residual[b][k];
-    if (e.out_f32) put(static_cast<float*>(e.out) + at, z[b]);
-    else if constexpr (sizeof(T) == 2) put(static_cast<T*>(e.out) + at, z[b]);
+    if (e.out_f32) put<WHOLE>(static_cast<float*>(e.out) + at, z[b], left);
+    else if constexpr (sizeof(T) == 2) put<WHOLE>(static_cast<T*>(e.out) + at, z[b], left);
   }
 }
 
@@ -449,35 +473,66 @@ MHC_DEV void interleave() {
 }
 
 // ROWS rows of 64 sums in LDS, as tile_kernel puts them there, to the outputs
-// from (m0, n0) on: V columns a lane, 16 outputs of it at a time.
-template <typename T, int V, int ROWS>
-MHC_DEV void store_rows(const Epilogue& e, const char* sums, int lane, int64_t m0, int64_t M, int64_t n0, int64_t N) {
-  constexpr int kLanes = 64 / V, kPass = kWave / kLanes;  // lanes of a row, rows of a pass
-  constexpr int kBatch = ROWS / kPass < 16 / V ? ROWS / kPass : 16 / V;
-  const int c = lane % kLanes * V;
-  if (n0 + c >= N) return;
-  float bias[V];
-  bias_of<T>(e, n0 + c, bias);
-  for (int r0 = lane / kLanes; r0 < ROWS && m0 + r0 < M; r0 += kPass * kBatch) {
-    float z[kBatch][V], res[kBatch][V];
-    residual_of<T>(e, m0 + r0, kPass, M, n0 + c, N, res);
+// from (m0, n0) on: eight columns a lane, of two rows at a time.
+template <typename T, int ROWS, bool WHOLE>
+MHC_DEV void store_columns(const Epilogue& e, const char* sums, int lane, int64_t m0, int64_t M, int64_t n0, int64_t N, int left) {
+  const int c = lane % 8 * 8;
+  float bias[8];
+  bias_of<T>(e, n0 + c, left, bias);
+  for (int r0 = lane / 8; r0 < ROWS && m0 + r0 < M; r0 += 16) {
+    float z[2][8], res[2][8];
+    residual_of<T, WHOLE>(e, m0 + r0, 8, M, n0 + c, N, left, res);
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int r = r0 + b * kPass;
-      if constexpr (V < 4) {
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int k = 0; k < V; ++k) z[b][k] = *reinterpret_cast<const float*>(sums + r * 256 + (((c / 4) ^ (r % 16)) << 4) + (c % 4 + k) * 4);
-      } else {
+      for (int k = 0; k < 2; ++k) {
+        const int r = r0 + b * 8;
+        const f32x4 u = *reinterpret_cast<const f32x4*>(sums + r * 256 + (((c / 4 + k) ^ (r % 16)) << 4));
 #pragma unroll
-        for (int k = 0; k < V / 4; ++k) {
-          const f32x4 u = *reinterpret_cast<const f32x4*>(sums + r * 256 + (((c / 4 + k) ^ (r % 16)) << 4));
-#pragma unroll
-          for (int j = 0; j < 4; ++j) z[b][4 * k + j] = u[j];
-        }
+        for (int j = 0; j < 4; ++j) z[b][4 * k + j] = u[j];
       }
-    }
-    finish<T>(e, m0 + r0, kPass, M, n0 + c, N, z, bias, res);
+    finish<T, WHOLE>(e, m0 + r0, 8, M, n0 + c, N, left, z, bias, res);
   }
+}
+
+template <typename T, int ROWS>
+MHC_DEV void store_rows(const Epilogue& e, const char* sums, int lane, int64_t m0, int64_t M, int64_t n0, int64_t N) {
+  const int left = (int)max((int64_t)0, min((int64_t)8, N - n0 - lane % 8 * 8));
+  if (left == 8) store_columns<T, ROWS, true>(e, sums, lane, m0, M, n0, N, left);
+  else if (left > 0) store_columns<T, ROWS, false>(e, sums, lane, m0, M, n0, N, left);
+}
+
+// A wave's JM x JN sums of 16 x 16, in registers, to the outputs from (m0, n0)
+// on, through the workgroup's LDS (BYTES of it, free).
+template <typename T, int JM, int JN, int WAVES, int BYTES>
+MHC_DEV void store_tile(const Product& p, char* smem, const f32x4 (&acc)[JN][JM], int64_t m0, int64_t n0, int wave, int lane) {
+  Epilogue e = p.e;
+  if (p.splits > 1) e.out = static_cast<float*>(e.out) + (int64_t)blockIdx.y * p.M * p.N;
+  // The sums go through LDS, where each wave has room for up to 64 rows
+  // of 64 columns, so that rows of the outputs are written as whole vectors of
+  // consecutive lanes.  The 16-byte chunk c of row r is at c ^ (r % 16).
+  constexpr int kFit = BYTES / (WAVES * 4096);  // sets of 16 rows that every wave has room for
+  constexpr int kRound = JM >= 4 && kFit >= 4 ? 4 : JM >= 2 && kFit >= 2 ? 2 : 1, kRows = kRound * 16;
+  static_assert(JN == 4 && JM % kRound == 0 && kFit >= 1, "64 columns a wave");
+  char* const mine = smem + wave * kRows * 256;
+  // (a round's sums have constant indices, and those of the first are gone before the second)
+  int at = lane;
+  asm volatile("" : "+v"(at));  // (or addresses of the outputs would be formed before the loop and held through it)
+  const auto round = [&](auto first) {
+    constexpr int h = decltype(first)::value;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kRound; ++j)
+#pragma unroll
+      for (int i = 0; i < JN; ++i)
+        *reinterpret_cast<f32x4*>(mine + (j * 16 + at % 16) * 256 + (((i * 4 + at / 16) ^ (at % 16)) << 4)) = acc[i][h + j];
+    __syncthreads();
+    const int64_t mh = m0 + h * 16;
+    store_rows<T, kRows>(e, mine, at, mh, p.M, n0, p.N);
+  };
+  static_assert(JM / kRound <= 2, "two rounds");
+  round(std::integral_constant<int, 0>{});
+  if constexpr (JM > kRound) round(std::integral_constant<int, kRound>{});
 }
 
 // The tile of a workgroup.  Workgroups go round the eight XCDs, each with an
@@ -556,36 +611,106 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const Product p) {
     interleave<(JM * (AK ? 1 : S::kE / 4) + JN * (BK ? 1 : S::kE / 4)), JM * JN * (sizeof(T) == 4 ? 4 : 1)>();
   }
   wait_loads<0>();  // (the last ones store zeros where the sums go next)
-  Epilogue e = p.e;
-  if (p.splits > 1) e.out = static_cast<float*>(e.out) + (int64_t)blockIdx.y * p.M * p.N;
-  // The sums go through LDS, where each wave has room for up to 64 rows
-  // of 64 columns, so that rows of the outputs are written as whole vectors of
-  // consecutive lanes.  The 16-byte chunk c of row r is at c ^ (r % 16).
-  constexpr int kFit = NS * kStage / (kWaves * 4096);  // sets of 16 rows that every wave has room for
-  constexpr int kRound = JM >= 4 && kFit >= 4 ? 4 : JM >= 2 && kFit >= 2 ? 2 : 1, kRows = kRound * 16;
-  static_assert(JN == 4 && JM % kRound == 0 && kFit >= 1, "64 columns a wave");
-  char* const mine = smem + wave * kRows * 256;
-  // (a round's sums have constant indices, and those of the first are gone before the second)
-  int at = lane;
-  asm volatile("" : "+v"(at));  // (or addresses of the outputs would be formed before the loop and held through it)
-  const auto round = [&](auto first) {
-    constexpr int h = decltype(first)::value;
-    __syncthreads();
+  store_tile<T, JM, JN, kWaves, NS * kStage>(p, smem, acc, m0 + wm, n0 + wn, wave, lane);
+}
+
+// --------------------------------------------------------------------------
+// fp32 operands on the bf16 matrix instructions
+// --------------------------------------------------------------------------
+
+// Eight fp32 values as three bf16 values each: the leading eight bits of the
+// value, of what is left and of what is left then.  Cut off and not rounded,
+// they add up to the value exactly.  What is left of an infinity is 0.
+MHC_DEV void split8(const u32x4& lo, const u32x4& hi, u32x4 (&part)[3]) {
+  const f32x4 flo = __builtin_bit_cast(f32x4, lo), fhi = __builtin_bit_cast(f32x4, hi);
 #pragma unroll
-    for (int j = 0; j < kRound; ++j)
+  for (int w = 0; w < 4; ++w) {
+    uint32_t x[2], y[2], z[2];
 #pragma unroll
-      for (int i = 0; i < JN; ++i)
-        *reinterpret_cast<f32x4*>(mine + (j * 16 + at % 16) * 256 + (((i * 4 + at / 16) ^ (at % 16)) << 4)) = acc[i][h + j];
-    __syncthreads();
-    const int64_t mh = m0 + wm + h * 16;
-    if (e.vec == 8) store_rows<T, 8, kRows>(e, mine, at, mh, p.M, n0 + wn, p.N);
-    else if (e.vec == 4) store_rows<T, 4, kRows>(e, mine, at, mh, p.M, n0 + wn, p.N);
-    else if (e.vec == 2) store_rows<T, 2, kRows>(e, mine, at, mh, p.M, n0 + wn, p.N);
-    else store_rows<T, 1, kRows>(e, mine, at, mh, p.M, n0 + wn, p.N);
-  };
-  static_assert(JM / kRound <= 2, "two rounds");
-  round(std::integral_constant<int, 0>{});
-  if constexpr (JM > kRound) round(std::integral_constant<int, kRound>{});
+    for (int k = 0; k < 2; ++k) {
+      const float v = w < 2 ? flo[2 * w + k] : fhi[2 * w - 4 + k];
+      x[k] = __builtin_bit_cast(uint32_t, v);
+      float r = v - __builtin_bit_cast(float, x[k] & 0xffff0000u);
+      if (fabsf(v) == __builtin_inff()) r = 0.f;
+      y[k] = __builtin_bit_cast(uint32_t, r);
+      z[k] = __builtin_bit_cast(uint32_t, r - __builtin_bit_cast(float, y[k] & 0xffff0000u));
+    }
+    part[0][w] = __builtin_amdgcn_perm(x[1], x[0], 0x07060302);
+    part[1][w] = __builtin_amdgcn_perm(y[1], y[0], 0x07060302);
+    part[2][w] = __builtin_amdgcn_perm(z[1], z[0], 0x07060302);
+  }
+}
+
+// tile_kernel for fp32 with each product of two values as six of their parts.
+// The three that are left out are below 2^-21 of it, and 2^-24 on average, so
+// that the sums are as good as fp32's own (1000 x 1100 x 1536: 6.4e-7 of the
+// result either way).  Six bf16 products take 3/8 of the time of one in fp32;
+// the splits, on the vector unit, go on beside them in another wave.
+template <bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
+__global__ __launch_bounds__(64 * WM * WN) void split_kernel(const Product p) {
+  using S = Stage<float>;
+  constexpr int kWaves = WM * WN, JM = BM / WM / 16, JN = BN / WN / 16;
+  constexpr int kA = BM * 128, kStage = kA + BN * 128;
+  __shared__ __attribute__((aligned(1024))) char smem[NS * kStage];
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  uint32_t tm, tn;
+  tile_of(blockIdx.x, (uint32_t)ceil_div(p.M, BM), (uint32_t)ceil_div(p.N, BN), tm, tn);
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+  const int k0 = (int)blockIdx.y * p.kper, k1 = min((int)p.K, k0 + p.kper);
+  Loader<float, AK, BM, kWaves> la;
+  Loader<float, BK, BN, kWaves> lb;
+  constexpr int kLoads = decltype(la)::kLoads + decltype(lb)::kLoads;
+  const uint32_t lds = lds_address(smem);
+  la.init(p.a, m0, p.M, k0, k1, wave, lane, lds);
+  lb.init(p.b, n0, p.N, k0, k1, wave, lane, lds + kA);
+  Reader<float, AK, BM, JM> ra;
+  Reader<float, BK, BN, JN> rb;
+  ra.init(wm, lane);
+  rb.init(wn, lane);
+  f32x4 acc[JN][JM] = {};
+  int kleft = k1 - k0;
+#pragma unroll
+  for (int q = 0; q < NS - 1; ++q) {
+    la.load(q * kStage, kleft - q * S::kK, lane);
+    lb.load(q * kStage, kleft - q * S::kK, lane);
+    la.next();
+    lb.next();
+  }
+  int cur = 0, ahead = (NS - 1) * kStage;
+  for (; kleft > 0; kleft -= S::kK) {
+    wait_loads<(NS - 2) * kLoads>();
+    __syncthreads();  // this stage is there, and nobody reads the one before any more
+    la.load(ahead, kleft - (NS - 1) * S::kK, lane);
+    lb.load(ahead, kleft - (NS - 1) * S::kK, lane);
+    la.next();
+    lb.next();
+    char* const sa = smem + cur;
+    char* const sb = sa + kA;
+    if (kleft < S::kK && kleft % S::kE != 0) {
+      la.clear_end(sa, kleft, threadIdx.x, 64 * kWaves);
+      lb.clear_end(sb, kleft, threadIdx.x, 64 * kWaves);
+      __syncthreads();
+    }
+    u32x4 b[JN][3];
+#pragma unroll
+    for (int i = 0; i < JN; ++i) split8(rb.get(sb, 0, i), rb.get(sb, 1, i), b[i]);
+#pragma unroll
+    for (int j = 0; j < JM; ++j) {
+      u32x4 a[3];
+      split8(ra.get(sa, 0, j), ra.get(sa, 1, j), a);
+#pragma unroll
+      for (int q = 0; q < 6; ++q) {  // the small ones first
+        constexpr int kB[6] = {2, 0, 1, 1, 0, 0}, kAt[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+        for (int i = 0; i < JN; ++i) acc[i][j] = mfma16<__bf16>(b[i][kB[q]], a[kAt[q]], acc[i][j]);
+      }
+    }
+    cur = cur == (NS - 1) * kStage ? 0 : cur + kStage;
+    ahead = ahead == (NS - 1) * kStage ? 0 : ahead + kStage;
+  }
+  wait_loads<0>();
+  store_tile<float, JM, JN, kWaves, NS * kStage>(p, smem, acc, m0 + wm, n0 + wn, wave, lane);
 }
 
 // --------------------------------------------------------------------------
@@ -613,9 +738,9 @@ MHC_DEV void join_waves(const f32x4 (&acc)[MT], float* sums, int M, int64_t n0, 
     for (int v = 0; v < kFewWaves; ++v) z[0][0] += sums[(v * MT * 16 + m) * 16 + n];
     if (m < M && n0 + n < N) {
       float bias[1], residual[1][1];
-      bias_of<T>(e, n0 + n, bias);
-      residual_of<T>(e, m, 0, M, n0 + n, N, residual);
-      finish<T>(e, m, 0, M, n0 + n, N, z, bias, residual);
+      bias_of<T>(e, n0 + n, 1, bias);
+      residual_of<T, true>(e, m, 0, M, n0 + n, N, 1, residual);
+      finish<T, true>(e, m, 0, M, n0 + n, N, 1, z, bias, residual);
     }
   }
 }
@@ -754,42 +879,42 @@ int run_few_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t
   return launch_few_rows<T, 4>(x, ldx, w, ldw, M, N, K, e, s);
 }
 
-// The sum over the splits, in order, and the epilogue.
-template <typename T, int V>
-__global__ __launch_bounds__(256) void join_kernel(const float* part, int splits, int64_t M, int64_t N, const Epilogue e) {
-  const int64_t total = M * N / V;
-  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * 256) {
-    const int64_t m = at * V / N, n = at * V % N;
-    float z[1][V] = {}, bias[V], residual[1][V];
-    bias_of<T>(e, n, bias);
-    residual_of<T>(e, m, 0, M, n, N, residual);
+// The sum over the splits, in order, and the epilogue: eight columns a thread
+// (four of fp32 outputs, so that a wave reads and writes one piece).
+template <typename T> constexpr int kJoin = sizeof(T) == 4 ? 4 : 8;
+
+template <typename T, bool WHOLE>
+MHC_DEV void join_columns(const float* part, int splits, int64_t m, int64_t M, int64_t n, int64_t N, int left, const Epilogue& e) {
+  constexpr int V = kJoin<T>;
+  float z[1][V] = {}, bias[V], residual[1][V];
+  bias_of<T>(e, n, left, bias);
+  residual_of<T, WHOLE>(e, m, 0, M, n, N, left, residual);
 #pragma unroll 4
-    for (int k = 0; k < splits; ++k) {
-      float v[V];
-      take(part + ((int64_t)k * M + m) * N + n, v);
+  for (int k = 0; k < splits; ++k) {
+    float v[V];
+    take<WHOLE>(part + ((int64_t)k * M + m) * N + n, v, left);
 #pragma unroll
-      for (int j = 0; j < V; ++j) z[0][j] += v[j];
-    }
-    finish<T>(e, m, 0, M, n, N, z, bias, residual);
+    for (int j = 0; j < V; ++j) z[0][j] += v[j];
   }
+  finish<T, WHOLE>(e, m, 0, M, n, N, left, z, bias, residual);
 }
 
-template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
-int launch_tile(const Product& p, hipStream_t s) {
-  const int64_t tiles = ceil_div(p.M, BM) * ceil_div(p.N, BN);
-  hipLaunchKernelGGL((tile_kernel<T, AK, BK, BM, BN, WM, WN, NS>), dim3((unsigned)tiles, (unsigned)p.splits),
-                     dim3(64 * WM * WN), 0, s, p);
-  MHC_CHECK_LAUNCH("tile_kernel");
-  return MHC_OK;
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(const float* part, int splits, int64_t M, int64_t N, const Epilogue e) {
+  constexpr int V = kJoin<T>;
+  const uint32_t groups = (uint32_t)ceil_div(N, V);
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < M * groups; at += (int64_t)gridDim.x * 256) {
+    const int64_t m = at / groups, n = at % groups * V;
+    const int left = (int)min((int64_t)V, N - n);
+    if (left == V) join_columns<T, true>(part, splits, m, M, n, N, left, e);
+    else join_columns<T, false>(part, splits, m, M, n, N, left, e);
+  }
 }
 
 template <typename T>
 int launch_join(const Epilogue& e, const float* part, int splits, int64_t M, int64_t N, hipStream_t s) {
-  const unsigned blocks = (unsigned)std::min(ceil_div(M * N / e.vec, 256), (int64_t)device_cu_count() * 16);
-  if (e.vec == 8) hipLaunchKernelGGL((join_kernel<T, 8>), dim3(blocks), dim3(256), 0, s, part, splits, M, N, e);
-  else if (e.vec == 4) hipLaunchKernelGGL((join_kernel<T, 4>), dim3(blocks), dim3(256), 0, s, part, splits, M, N, e);
-  else if (e.vec == 2) hipLaunchKernelGGL((join_kernel<T, 2>), dim3(blocks), dim3(256), 0, s, part, splits, M, N, e);
-  else hipLaunchKernelGGL((join_kernel<T, 1>), dim3(blocks), dim3(256), 0, s, part, splits, M, N, e);
+  const unsigned blocks = (unsigned)std::min(ceil_div(M * ceil_div(N, kJoin<T>), 256), (int64_t)device_cu_count() * 16);
+  hipLaunchKernelGGL((join_kernel<T>), dim3(blocks), dim3(256), 0, s, part, splits, M, N, e);
   MHC_CHECK_LAUNCH("join_kernel");
   return MHC_OK;
 }
@@ -805,14 +930,14 @@ struct Cut {
 // few workgroups on the card (its latencies), `busy` for each workgroup of a
 // CU that has `fit` of them (its matrix instructions and LDS reads).  From
 // x W^T over 16 to 512 stages: 256 x 256 16-bit at 1.12 alone, 1.6 with all
-// CUs at it (1.3 PFLOP/s); fp32 stages have half the k at 1/16 the rate.
+// CUs at it (1.3 PFLOP/s); a stage of fp32 has half the k.
 struct TileCost {
   int bm, bn, fit;
   float ends, alone16, busy16, alone32, busy32;
 };
 constexpr TileCost kTiles[] = {
-    {256, 256, 1, 7.0f, 1.12f, 1.60f, 7.17f, 7.35f},   {128, 256, 1, 5.0f, 0.68f, 0.92f, 3.66f, 3.84f},
-    {128, 128, 2, 5.0f, 0.545f, 0.54f, 1.95f, 1.88f},  {64, 128, 2, 4.5f, 0.40f, 0.34f, 1.05f, 0.98f},
+    {256, 256, 1, 7.0f, 1.12f, 1.60f, 4.55f, 5.05f},   {128, 256, 1, 5.0f, 0.68f, 0.92f, 2.79f, 2.92f},
+    {128, 128, 2, 5.0f, 0.545f, 0.54f, 1.82f, 1.41f},  {64, 128, 2, 4.5f, 0.40f, 0.34f, 1.21f, 0.87f},
     {64, 64, 3, 3.6f, 0.245f, 0.21f, 0.555f, 0.53f},
 };
 
@@ -861,14 +986,27 @@ inline bool few_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, int
   return few <= cut_of(M, N, K, dtype).us + copies;
 }
 
+// BM x BN tiles; fp32 ones of at least 64 x 128 on the bf16 instructions (64 x 64
+// have too few products for each value that is split: 65 us so, 57 in fp32 at
+// 1000 x 1100 x 1536; 128 x 128 107 in fp32, 93 so; 8192 x 4096 x 4096 1889
+// and 1293 in 256 x 256, where the library's fp32 product takes 1800)
+template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
+int launch(const Product& p, hipStream_t s) {
+  const dim3 grid((unsigned)(ceil_div(p.M, BM) * ceil_div(p.N, BN)), (unsigned)p.splits), block(64 * WM * WN);
+  if constexpr (sizeof(T) == 4 && BN > 64) hipLaunchKernelGGL((split_kernel<AK, BK, BM, BN, WM, WN, NS>), grid, block, 0, s, p);
+  else hipLaunchKernelGGL((tile_kernel<T, AK, BK, BM, BN, WM, WN, NS>), grid, block, 0, s, p);
+  MHC_CHECK_LAUNCH("tile_kernel");
+  return MHC_OK;
+}
+
 template <typename T, bool AK, bool BK>
 int run_layout(const Product& p, int tile, hipStream_t s) {
   switch (tile) {
-    case 0: return launch_tile<T, AK, BK, 256, 256, 2, 4, 2>(p, s);
-    case 1: return launch_tile<T, AK, BK, 128, 256, 2, 4, 2>(p, s);
-    case 2: return launch_tile<T, AK, BK, 128, 128, 2, 2, 2>(p, s);
-    case 3: return launch_tile<T, AK, BK, 64, 128, 2, 2, 3>(p, s);
-    default: return launch_tile<T, AK, BK, 64, 64, 4, 1, 3>(p, s);
+    case 0: return launch<T, AK, BK, 256, 256, 2, 4, 2>(p, s);
+    case 1: return launch<T, AK, BK, 128, 256, 2, 4, 2>(p, s);
+    case 2: return launch<T, AK, BK, 128, 128, 2, 2, 2>(p, s);
+    case 3: return launch<T, AK, BK, 64, 128, 2, 2, 3>(p, s);
+    default: return launch<T, AK, BK, 64, 64, 4, 1, 3>(p, s);
   }
 }
 
@@ -878,7 +1016,7 @@ int run_product(Product p, bool a_k, bool b_k, const Cut& c, float* part, hipStr
   const Epilogue e = p.e;
   p.splits = c.splits;
   p.kper = c.kper;
-  if (c.splits > 1) p.e = epilogue(nullptr, nullptr, part, nullptr, MHC_ACT_NONE, kF32, kF32, p.N);
+  if (c.splits > 1) p.e = Epilogue{nullptr, nullptr, part, nullptr, MHC_ACT_NONE, 1};
   const int rc = a_k && b_k ? run_layout<T, true, true>(p, c.tile, s)
                  : a_k      ? run_layout<T, true, false>(p, c.tile, s)
                             : run_layout<T, false, false>(p, c.tile, s);
