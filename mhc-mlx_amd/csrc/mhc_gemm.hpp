@@ -546,35 +546,50 @@ MHC_DEV void tile_of(uint32_t id, uint32_t tm, uint32_t tn, uint32_t& m, uint32_
   n = (t % (8 * tn)) / rows;
 }
 
+// A workgroup's place: its tile, its part of the reduction, and its wave's corner of the tile.
+template <int BM, int BN, int WM, int WN>
+struct Place {
+  int64_t m0, n0;
+  int wm, wn, k0, k1, wave, lane;
+
+  MHC_DEV Place(const Product& p) {
+    lane = threadIdx.x % kWave;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    uint32_t tm, tn;
+    tile_of(blockIdx.x, (uint32_t)ceil_div(p.M, BM), (uint32_t)ceil_div(p.N, BN), tm, tn);
+    m0 = (int64_t)tm * BM;
+    n0 = (int64_t)tn * BN;
+    wm = wave / WN * (BM / WM);
+    wn = wave % WN * (BN / WN);
+    k0 = (int)blockIdx.y * p.kper;
+    k1 = min((int)p.K, k0 + p.kper);
+  }
+};
+
+// The sums of a workgroup's tile.  (The first operand's index, n, runs over a
+// lane's four values.)
 template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
-__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const Product p) {
+MHC_DEV void sum_tile(const Product& p, const Place<BM, BN, WM, WN>& at, char* smem, f32x4 (&acc)[BN / WN / 16][BM / WM / 16]) {
   using S = Stage<T>;
   constexpr int kWaves = WM * WN, JM = BM / WM / 16, JN = BN / WN / 16;
   constexpr int kA = BM * 128, kStage = kA + BN * 128;
-  __shared__ __attribute__((aligned(1024))) char smem[NS * kStage];
-  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  uint32_t tm, tn;
-  tile_of(blockIdx.x, (uint32_t)ceil_div(p.M, BM), (uint32_t)ceil_div(p.N, BN), tm, tn);
-  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
-  const int k0 = (int)blockIdx.y * p.kper, k1 = min((int)p.K, k0 + p.kper);
+  const int lane = at.lane;
   Loader<T, AK, BM, kWaves> la;
   Loader<T, BK, BN, kWaves> lb;
   constexpr int kLoads = decltype(la)::kLoads + decltype(lb)::kLoads;
   const uint32_t lds = lds_address(smem);
-  la.init(p.a, m0, p.M, k0, k1, wave, lane, lds);
-  lb.init(p.b, n0, p.N, k0, k1, wave, lane, lds + kA);
+  la.init(p.a, at.m0, p.M, at.k0, at.k1, at.wave, lane, lds);
+  lb.init(p.b, at.n0, p.N, at.k0, at.k1, at.wave, lane, lds + kA);
   Reader<T, AK, BM, JM> ra;
   Reader<T, BK, BN, JN> rb;
-  ra.init(wm, lane);
-  rb.init(wn, lane);
-  f32x4 acc[JN][JM] = {};  // the first operand's index, n, runs over a lane's four values
+  ra.init(at.wm, lane);
+  rb.init(at.wn, lane);
   // The fragments of half a stage are read while the products of the half
   // before are formed; in the middle of a stage its last reads are done, so
   // that the barrier there frees its place and hands over the next one.
   // NS stages are under way.  (Those past the end read nothing: every pass
   // issues the same number of loads.)
-  int kleft = k1 - k0;
+  int kleft = at.k1 - at.k0;
 #pragma unroll
   for (int q = 0; q < NS; ++q) {
     la.load(q * kStage, kleft - q * S::kK, lane);
@@ -610,8 +625,17 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const Product p) {
     f1.template multiply<T>(acc);
     interleave<(JM * (AK ? 1 : S::kE / 4) + JN * (BK ? 1 : S::kE / 4)), JM * JN * (sizeof(T) == 4 ? 4 : 1)>();
   }
-  wait_loads<0>();  // (the last ones store zeros where the sums go next)
-  store_tile<T, JM, JN, kWaves, NS * kStage>(p, smem, acc, m0 + wm, n0 + wn, wave, lane);
+  wait_loads<0>();  // (the last ones store zeros)
+}
+
+template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
+__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const Product p) {
+  constexpr int kBytes = NS * (BM + BN) * 128;
+  __shared__ __attribute__((aligned(1024))) char smem[kBytes];
+  const Place<BM, BN, WM, WN> at(p);
+  f32x4 acc[BN / WN / 16][BM / WM / 16] = {};
+  sum_tile<T, AK, BK, BM, BN, WM, WN, NS>(p, at, smem, acc);
+  store_tile<T, BM / WM / 16, BN / WN / 16, WM * WN, kBytes>(p, smem, acc, at.m0 + at.wm, at.n0 + at.wn, at.wave, at.lane);
 }
 
 // --------------------------------------------------------------------------
@@ -620,7 +644,7 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const Product p) {
 
 // Eight fp32 values as three bf16 values each: the leading eight bits of the
 // value, of what is left and of what is left then.  Cut off and not rounded,
-// they add up to the value exactly.  What is left of an infinity is 0.
+// they add up to the value exactly.  An infinity's second part is NaN.
 MHC_DEV void split8(const u32x4& lo, const u32x4& hi, u32x4 (&part)[3]) {
   const f32x4 flo = __builtin_bit_cast(f32x4, lo), fhi = __builtin_bit_cast(f32x4, hi);
 #pragma unroll
@@ -630,8 +654,7 @@ MHC_DEV void split8(const u32x4& lo, const u32x4& hi, u32x4 (&part)[3]) {
     for (int k = 0; k < 2; ++k) {
       const float v = w < 2 ? flo[2 * w + k] : fhi[2 * w - 4 + k];
       x[k] = __builtin_bit_cast(uint32_t, v);
-      float r = v - __builtin_bit_cast(float, x[k] & 0xffff0000u);
-      if (fabsf(v) == __builtin_inff()) r = 0.f;
+      const float r = v - __builtin_bit_cast(float, x[k] & 0xffff0000u);
       y[k] = __builtin_bit_cast(uint32_t, r);
       z[k] = __builtin_bit_cast(uint32_t, r - __builtin_bit_cast(float, y[k] & 0xffff0000u));
     }
@@ -641,35 +664,29 @@ MHC_DEV void split8(const u32x4& lo, const u32x4& hi, u32x4 (&part)[3]) {
   }
 }
 
-// tile_kernel for fp32 with each product of two values as six of their parts.
+// sum_tile for fp32 with each product of two values as six of their parts.
 // The three that are left out are below 2^-21 of it, and 2^-24 on average, so
-// that the sums are as good as fp32's own (1000 x 1100 x 1536: 6.4e-7 of the
-// result either way).  Six bf16 products take 3/8 of the time of one in fp32;
-// the splits, on the vector unit, go on beside them in another wave.
+// that the sums are as good as fp32's own (1000 x 1100 x 1536: 6.0e-7 of the
+// result off float64, 7.0e-7 with fp32 instructions).  Six bf16 products take
+// 3/8 of the time of one in fp32; the splits, on the vector unit, go on beside
+// them in another wave.
 template <bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
-__global__ __launch_bounds__(64 * WM * WN) void split_kernel(const Product p) {
+MHC_DEV void sum_tile_split(const Product& p, const Place<BM, BN, WM, WN>& at, char* smem, f32x4 (&acc)[BN / WN / 16][BM / WM / 16]) {
   using S = Stage<float>;
   constexpr int kWaves = WM * WN, JM = BM / WM / 16, JN = BN / WN / 16;
   constexpr int kA = BM * 128, kStage = kA + BN * 128;
-  __shared__ __attribute__((aligned(1024))) char smem[NS * kStage];
-  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  uint32_t tm, tn;
-  tile_of(blockIdx.x, (uint32_t)ceil_div(p.M, BM), (uint32_t)ceil_div(p.N, BN), tm, tn);
-  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
-  const int k0 = (int)blockIdx.y * p.kper, k1 = min((int)p.K, k0 + p.kper);
+  const int lane = at.lane;
   Loader<float, AK, BM, kWaves> la;
   Loader<float, BK, BN, kWaves> lb;
   constexpr int kLoads = decltype(la)::kLoads + decltype(lb)::kLoads;
   const uint32_t lds = lds_address(smem);
-  la.init(p.a, m0, p.M, k0, k1, wave, lane, lds);
-  lb.init(p.b, n0, p.N, k0, k1, wave, lane, lds + kA);
+  la.init(p.a, at.m0, p.M, at.k0, at.k1, at.wave, lane, lds);
+  lb.init(p.b, at.n0, p.N, at.k0, at.k1, at.wave, lane, lds + kA);
   Reader<float, AK, BM, JM> ra;
   Reader<float, BK, BN, JN> rb;
-  ra.init(wm, lane);
-  rb.init(wn, lane);
-  f32x4 acc[JN][JM] = {};
-  int kleft = k1 - k0;
+  ra.init(at.wm, lane);
+  rb.init(at.wn, lane);
+  int kleft = at.k1 - at.k0;
 #pragma unroll
   for (int q = 0; q < NS - 1; ++q) {
     la.load(q * kStage, kleft - q * S::kK, lane);
@@ -710,7 +727,41 @@ __global__ __launch_bounds__(64 * WM * WN) void split_kernel(const Product p) {
     ahead = ahead == (NS - 1) * kStage ? 0 : ahead + kStage;
   }
   wait_loads<0>();
-  store_tile<float, JM, JN, kWaves, NS * kStage>(p, smem, acc, m0 + wm, n0 + wn, wave, lane);
+}
+
+// A tile with a NaN is summed once more with fp32 instructions: they tell what
+// an infinity makes of it, whose parts make NaN of everything.
+template <bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
+__global__ __launch_bounds__(64 * WM * WN) void split_kernel(const Product p) {
+  constexpr int kBytes = NS * (BM + BN) * 128, JM = BM / WM / 16, JN = BN / WN / 16;
+  __shared__ __attribute__((aligned(1024))) char smem[kBytes];
+  const Place<BM, BN, WM, WN> at(p);
+  f32x4 acc[JN][JM] = {};
+  sum_tile_split<AK, BK, BM, BN, WM, WN, NS>(p, at, smem, acc);
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < JN; ++i)
+#pragma unroll
+    for (int j = 0; j < JM; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) nan |= acc[i][j][e] != acc[i][j][e];
+  int* const found = reinterpret_cast<int*>(smem);
+  const int mine = __ballot(nan) != 0;
+  __syncthreads();  // nobody reads the last stage any more
+  if (at.lane == 0) found[at.wave] = mine;
+  __syncthreads();
+  int again = 0;
+#pragma unroll
+  for (int w = 0; w < WM * WN; ++w) again |= found[w];
+  __syncthreads();
+  if (__builtin_amdgcn_readfirstlane(again)) {
+#pragma unroll
+    for (int i = 0; i < JN; ++i)
+#pragma unroll
+      for (int j = 0; j < JM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    sum_tile<float, AK, BK, BM, BN, WM, WN, NS>(p, at, smem, acc);
+  }
+  store_tile<float, JM, JN, WM * WN, kBytes>(p, smem, acc, at.m0 + at.wm, at.n0 + at.wn, at.wave, at.lane);
 }
 
 // --------------------------------------------------------------------------
@@ -989,7 +1040,7 @@ inline bool few_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, int
 // BM x BN tiles; fp32 ones of at least 64 x 128 on the bf16 instructions (64 x 64
 // have too few products for each value that is split: 65 us so, 57 in fp32 at
 // 1000 x 1100 x 1536; 128 x 128 107 in fp32, 93 so; 8192 x 4096 x 4096 1889
-// and 1293 in 256 x 256, where the library's fp32 product takes 1800)
+// and 1180 in 256 x 256, where the library's fp32 product takes 1800)
 template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
 int launch(const Product& p, hipStream_t s) {
   const dim3 grid((unsigned)(ceil_div(p.M, BM) * ceil_div(p.N, BN)), (unsigned)p.splits), block(64 * WM * WN);

@@ -200,6 +200,40 @@ def test_non_finite_values_stay_in_their_rows(M, N, K, dt):
     assert out[:, N - 1].isnan().all() and torch.equal(out[:, :N - 1], clean[:, :N - 1])
 
 
+@pytest.mark.parametrize("M,N,K", [(5, 64, 96), (100, 130, 96), (1024, 1600, 96), (2048, 2048, 104), (2100, 4300, 72)])
+def test_fp32_extremes(M, N, K):
+    """Infinities with their signs, and values near both ends of the range, in every row that has them and no other."""
+    x, w, _, _, _ = _inputs(M, N, K, "f32", 17)
+    x[1] *= 1e35
+    x[2] *= 1e-34
+    x[3, K - 1], x[4, 0] = float("inf"), -float("inf")
+    w[5] *= 1e4
+    w[6] *= 1e-4
+    out = linear_act(x, w)
+    ref, bound, *_ = linear64(x, w, None, None, "none", torch.float32)
+    fine = ref.abs() < 3e38
+    close(torch.where(fine, out.double(), 0.0), torch.where(fine, ref, 0.0), torch.where(fine, bound, 1.0), "finite")
+    assert torch.equal(out[3:5].isinf(), ref[3:5].isinf()) and torch.equal(out[3:5].sign(), ref[3:5].sign().float())
+    assert not out.isnan().any()
+
+
+@pytest.mark.parametrize("M", [9, 70, 150, 700])
+@pytest.mark.parametrize("dt,K", [("bf16", 4100), ("bf16", 4102), ("bf16", 4101), ("f32", 2049), ("f16", 1030)])
+def test_ends_of_long_rows(M, dt, K):
+    """Reductions that end inside a chunk, and inside a part where they are split; what follows each row in memory is NaN."""
+    x, w, b, r, g = _inputs(M, 140, K, dt, 18)
+    _check(_holed(x, 6), _holed(w, 10), b, r, g, "silu")
+
+
+@pytest.mark.parametrize("N", [512, 516, 514, 513])
+@pytest.mark.parametrize("dt,out", [("bf16", None), ("f16", torch.float32), ("f32", None)])
+@pytest.mark.parametrize("M,K", [(300, 1000), (1030, 264), (2100, 200), (4200, 1032)])
+def test_output_rows_of_any_length(M, N, K, dt, out):
+    """Every tile, forward and backward, with outputs that end inside a vector."""
+    N = N * 8 if M >= 2100 else N
+    _check(*_inputs(M, N - (8 - N % 8) % 8 if N > 4000 else N, K, dt, 19, out=out), "gelu", out)
+
+
 def test_more_than_2_31_elements():
     """Rows past 2^31 elements of x and past 2^32 bytes (a view of one allocation)."""
     M, K, N = 70000, 32768, 16
