@@ -987,9 +987,9 @@ struct TileCost {
   float ends, alone16, busy16, alone32, busy32;
 };
 constexpr TileCost kTiles[] = {
-    {256, 256, 1, 7.0f, 1.12f, 1.60f, 4.55f, 5.05f},   {128, 256, 1, 5.0f, 0.68f, 0.92f, 2.79f, 2.92f},
-    {128, 128, 2, 5.0f, 0.545f, 0.54f, 1.82f, 1.41f},  {64, 128, 2, 4.5f, 0.40f, 0.34f, 1.21f, 0.87f},
-    {64, 64, 3, 3.6f, 0.245f, 0.21f, 0.555f, 0.53f},
+    {256, 256, 1, 7.0f, 1.12f, 1.60f, 4.10f, 4.75f},   {128, 256, 1, 5.0f, 0.68f, 0.92f, 2.35f, 2.60f},
+    {128, 128, 2, 5.0f, 0.545f, 0.54f, 1.67f, 1.28f},  {64, 128, 2, 4.5f, 0.40f, 0.34f, 1.03f, 0.78f},
+    {64, 64, 3, 3.6f, 0.245f, 0.21f, 0.58f, 0.525f},
 };
 
 // The cut with the least estimated time.  Large tiles read least, small ones
