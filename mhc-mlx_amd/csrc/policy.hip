@@ -95,8 +95,9 @@ MHC_DEV Running join_workgroup(Running r, float (&lds)[32]) {
 }
 
 // a sum over a workgroup's threads, in every thread, in a fixed order
-template <int THREADS>
-MHC_DEV float sum_workgroup(float s, float (&lds)[32]) {
+template <int THREADS, typename S, int N>
+MHC_DEV S sum_workgroup(S s, S (&lds)[N]) {
+  static_assert(N >= THREADS / kWave);
   constexpr int kWaves = THREADS / kWave;
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
@@ -104,7 +105,7 @@ MHC_DEV float sum_workgroup(float s, float (&lds)[32]) {
   __syncthreads();
   if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = s;
   __syncthreads();
-  float all = 0.f;
+  S all = 0;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) all += lds[w];
   return all;
@@ -121,24 +122,31 @@ struct Token {
   float logit;
 };
 
+// The differences of log probabilities are small beside them, and the mean of
+// ratio times advantage is small beside its terms: lp's rounding to fp32 (5e-7
+// at -11) would be most of the loss's error.  So lp is put together in fp64,
+// from log sum = e log 2 + log m, whose fp32 part, of m around 1, is below 0.35.
 template <typename T>
 MHC_DEV Token token_of(const mhc_policy_args& a, int64_t t, const T* row, float top, float sum) {
   const int64_t at = a.actions[t];
   const float nan = __builtin_nanf("");
   const float z = at >= 0 && at < a.V ? load1(row + at) : nan;
-  const float lp = (z - top) - logf(sum);
-  const float ratio = expf(lp - a.old_logp[t]), adv = a.advantages[t];
+  int e;
+  float m = frexpf(sum, &e);
+  if (m < 0.70710678f) m *= 2.f, --e;
+  const double lp = (double)z - (double)top - ((double)e * 0.6931471805599453 + (double)logf(m));
+  const float ratio = expf((float)(lp - (double)a.old_logp[t])), adv = a.advantages[t];
   // (a NaN ratio stays one: fminf and fmaxf would drop it)
   const float held_ratio = ratio < 1.f - a.clip_low ? 1.f - a.clip_low : ratio > 1.f + a.clip_high ? 1.f + a.clip_high : ratio;
   const float free = ratio * adv, held = held_ratio * adv;
   Token r;
-  r.logp = lp;
+  r.logp = (float)lp;
   r.logit = z;
   r.loss = -(free <= held ? free : held);
   r.coef = free <= held ? -free : 0.f;
   if (!(free == free)) r.loss = r.coef = nan;
   if (a.ref_logp != nullptr) {
-    const float gap = a.ref_logp[t] - lp, over = expm1f(gap);  // q - 1 without cancellation near q = 1
+    const float gap = (float)((double)a.ref_logp[t] - lp), over = expm1f(gap);  // q - 1 without cancellation near q = 1
     r.loss += a.kl_coef * (over - gap);
     r.coef -= a.kl_coef * over;
   }
@@ -318,12 +326,13 @@ __global__ __launch_bounds__(kRowThreads) void policy_rows_kernel(const mhc_poli
 __global__ __launch_bounds__(kRowThreads) void policy_loss_kernel(const mhc_policy_args a, const float* terms, float* loss,
                                                                   float* inv) {
   __shared__ float lds[32];
-  float s = 0.f;
-  for (int64_t t = threadIdx.x; t < a.T; t += kRowThreads) s += terms[t];
-  s = sum_workgroup<kRowThreads>(s, lds);
+  __shared__ double lds_terms[kRowThreads / kWave];
+  double s = 0;  // (terms of both signs)
+  for (int64_t t = threadIdx.x; t < a.T; t += kRowThreads) s += (double)terms[t];
+  s = sum_workgroup<kRowThreads>(s, lds_terms);
   const float den = denominator_of<kRowThreads>(a, lds);
   if (threadIdx.x == 0) {
-    loss[0] = s / den;
+    loss[0] = (float)(s / (double)den);
     if (inv != nullptr) inv[0] = 1.f / den;
   }
 }
