@@ -1,8 +1,9 @@
-"""The torch binding of libmhc_hip (``_mhc_torch.so``, built from csrc/torch_ext.cpp).
+"""The torch binding of libmhc_hip (``_mhc_torch.so``, built from csrc/torch_ext.cpp and torch_train.cpp).
 
 It holds MHCLayer's forward and backward as a C++ autograd Function over the
 same C ABI that ops.py calls through ctypes, so the small-batch path makes
-the fewest host steps and the backward runs without Python.  Loaded once,
+the fewest host steps and the backward runs without Python, and likewise the
+linear layer, the policy loss and the AdamW step.  Loaded once,
 from this package directory, after libmhc_hip.so (whose symbols it uses).
 Like the library, it must be present where a GPU is: a missing build raises
 RuntimeError naming the build command.
