@@ -65,24 +65,14 @@ __global__ __launch_bounds__(256) void dz_kernel(const G* dout, const void* dact
     if (n0 + c < N) part[(int64_t)blockIdx.y * N + n0 + c] = (lds[0][c] + lds[1][c]) + (lds[2][c] + lds[3][c]);
 }
 
-// db[n] = sum over the blocks of rows: 32 columns a workgroup, each in eight parts that are joined in order
+// db[n] = sum over the blocks of rows
 template <typename T>
-__global__ __launch_bounds__(256) void db_kernel(const float* part, T* db, int64_t blocks, int64_t N) {
-  __shared__ float lds[8][32];
-  const int c = threadIdx.x % 32, q = threadIdx.x / 32;
-  const int64_t n = (int64_t)blockIdx.x * 32 + c;
-  float s = 0.f;
-#pragma unroll 8
-  for (int64_t b = q; b < blocks; b += 8) s += part[b * N + min(n, N - 1)];
-  lds[q][c] = s;
-  __syncthreads();
-  if (q != 0 || n >= N) return;
-#pragma unroll
-  for (int k = 1; k < 8; ++k) s += lds[k][c];
-  store1(db + n, s);
+__global__ __launch_bounds__(256) void db_kernel(const float* part, T* db, int64_t rows, int64_t N) {
+  __shared__ float lds[8][gemm::kSumCols];
+  gemm::sum_columns(lds, part, db, rows, N, blockIdx.x);
 }
 
-// rows of `width` elements, `ld` apart, into rows of a multiple of 16 bytes, with zeros after the last element
+// rows of `width` elements, `ld` apart, into rows of whole chunks of 16 bytes, with zeros after the last element
 template <typename T>
 __global__ __launch_bounds__(256) void pack_kernel(const T* src, int64_t ld, T* dst, int64_t rows, int64_t width, int64_t chunks) {
   constexpr int kE = 16 / (int)sizeof(T);
@@ -105,19 +95,15 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* src, int64_t ld, T* 
 int elem_bytes(int dtype) { return dtype == kF32 ? 4 : 2; }
 
 // ws: part_bytes of the product
-int run_product(const Product& p, bool a_k, bool b_k, int dtype, char* ws, hipStream_t s) {
-  const gemm::Cut c = gemm::cut_of(p.M, p.N, p.K, dtype);
+int run_product(const Product& p, bool a_k, bool b_k, const gemm::Cut& c, int dtype, char* ws, hipStream_t s) {
   float* const part = reinterpret_cast<float*>(ws);
   if (dtype == kF32) return gemm::run_product_f32(p, a_k, b_k, c, part, s);
   if (dtype == kBF16) return gemm::run_product_bf16(p, a_k, b_k, c, part, s);
   return gemm::run_product_f16(p, a_k, b_k, c, part, s);
 }
 
-// bytes of the sums of a product whose reduction is split
-size_t part_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
-  const gemm::Cut c = gemm::cut_of(M, N, K, dtype);
-  return c.splits > 1 ? (size_t)(c.splits * M * N) * sizeof(float) : 0;
-}
+// bytes of the sums of an M x N product whose reduction is split
+size_t part_bytes(const gemm::Cut& c, int64_t M, int64_t N) { return c.splits > 1 ? (size_t)(c.splits * M * N) * sizeof(float) : 0; }
 
 size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
@@ -156,7 +142,8 @@ int operand(Operand& o, const void* p, int64_t rows, int64_t ld, int64_t width, 
 }
 
 struct BwdPlan {
-  size_t dz, part, x, w, total;  // bytes; the products' sums, one after the other, come last
+  size_t dz, part, x, w, total;  // bytes; the products' sums (of one after the other, unless they go together) come last
+  gemm::PairCut cut;
 };
 
 BwdPlan plan_bwd(const void* dout, int dout_dtype, bool dact, const void* x, int64_t ldx, const void* w, int64_t ldw, bool dx, bool dw,
@@ -167,8 +154,11 @@ BwdPlan plan_bwd(const void* dout, int dout_dtype, bool dact, const void* x, int
   if (db) b.part = up256((size_t)(ceil_div(M, dz_rows(M, N)) * N) * sizeof(float));
   if (dx) b.w = pack_bytes(w, N, ldw, K, dtype);
   if (dw) b.x = pack_bytes(x, M, ldx, K, dtype);
-  b.total = b.dz + b.part + b.x + b.w +
-            std::max(dx ? part_bytes(M, K, N, dtype) : 0, dw ? part_bytes(N, K, M, dtype) : 0);
+  if (dx && dw) b.cut = gemm::pair_of(M, N, K, dtype);
+  else if (dx) b.cut.dx = gemm::cut_of(M, K, N, dtype);
+  else if (dw) b.cut.dw = gemm::cut_of(N, K, M, dtype);
+  const size_t of_dx = dx ? part_bytes(b.cut.dx, M, K) : 0, of_dw = dw ? part_bytes(b.cut.dw, N, K) : 0;
+  b.total = b.dz + b.part + b.x + b.w + (b.cut.together ? of_dx + of_dw : std::max(of_dx, of_dw));
   return b;
 }
 
@@ -180,8 +170,8 @@ int run_dz(const void* dout, const void* dact, void* dz, int64_t ld, float* part
   hipLaunchKernelGGL((dz_kernel<T, G>), grid, dim3(256), 0, s, static_cast<const G*>(dout), dact, static_cast<T*>(dz), ld, part, M, N, rows);
   MHC_CHECK_LAUNCH("dz_kernel");
   if (db != nullptr) {
-    hipLaunchKernelGGL((db_kernel<T>), dim3((unsigned)ceil_div(N, 32)), dim3(256), 0, s, (const float*)part, static_cast<T*>(db),
-                       blocks, N);
+    hipLaunchKernelGGL((db_kernel<T>), dim3((unsigned)ceil_div(N, gemm::kSumCols)), dim3(256), 0, s, (const float*)part,
+                       static_cast<T*>(db), blocks, N);
     MHC_CHECK_LAUNCH("db_kernel");
   }
   return MHC_OK;
@@ -201,7 +191,8 @@ int check_shape(int64_t M, int64_t N, int64_t K, int dtype) {
 extern "C" size_t mhc_linear_act_fwd_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M,
                                                      int64_t N, int64_t K, int dtype) {
   if (M <= 0 || N <= 0 || K <= 0 || mhc::gemm::few_rows(x, ldx, w, ldw, M, N, K, dtype)) return 0;
-  return mhc::pack_bytes(x, M, ldx, K, dtype) + mhc::pack_bytes(w, N, ldw, K, dtype) + mhc::part_bytes(M, N, K, dtype);
+  return mhc::pack_bytes(x, M, ldx, K, dtype) + mhc::pack_bytes(w, N, ldw, K, dtype) +
+         mhc::part_bytes(mhc::gemm::cut_of(M, N, K, dtype), M, N);
 }
 
 extern "C" int mhc_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
@@ -230,7 +221,7 @@ extern "C" int mhc_linear_act_fwd(const void* x, int64_t ldx, const void* w, int
   Product p = {{}, {}, M, N, K, gemm::Epilogue{bias, residual, out, dact, act, out_dtype == kF32}, 1, 0};
   if (const int rc = operand(p.a, x, M, ldx, K, dtype, ws, s)) return rc;
   if (const int rc = operand(p.b, w, N, ldw, K, dtype, ws, s)) return rc;
-  return run_product(p, true, true, dtype, ws, s);
+  return run_product(p, true, true, gemm::cut_of(M, N, K, dtype), dtype, ws, s);
 }
 
 extern "C" size_t mhc_linear_act_bwd_workspace_bytes(const void* dout, int dout_dtype, const void* dact, const void* x,
@@ -260,27 +251,39 @@ extern "C" int mhc_linear_act_bwd(const void* dout, int dout_dtype, const void* 
   void* const dz = b.dz > 0 ? ws : nullptr;
   float* const part = b.part > 0 ? reinterpret_cast<float*>(ws + b.dz) : nullptr;
   if (dz != nullptr || db != nullptr) {
+    void* const sum = b.cut.together ? nullptr : db;  // (else by the products' launch)
     int rc;
-    if (dtype == kF32) rc = run_dz<float, float>(dout, dact, dz, padded(N), part, db, M, N, s);
+    if (dtype == kF32) rc = run_dz<float, float>(dout, dact, dz, padded(N), part, sum, M, N, s);
     else if (dtype == kBF16)
-      rc = dout_dtype == kF32 ? run_dz<__bf16, float>(dout, dact, dz, padded(N), part, db, M, N, s)
-                              : run_dz<__bf16, __bf16>(dout, dact, dz, padded(N), part, db, M, N, s);
+      rc = dout_dtype == kF32 ? run_dz<__bf16, float>(dout, dact, dz, padded(N), part, sum, M, N, s)
+                              : run_dz<__bf16, __bf16>(dout, dact, dz, padded(N), part, sum, M, N, s);
     else
-      rc = dout_dtype == kF32 ? run_dz<_Float16, float>(dout, dact, dz, padded(N), part, db, M, N, s)
-                              : run_dz<_Float16, _Float16>(dout, dact, dz, padded(N), part, db, M, N, s);
+      rc = dout_dtype == kF32 ? run_dz<_Float16, float>(dout, dact, dz, padded(N), part, sum, M, N, s)
+                              : run_dz<_Float16, _Float16>(dout, dact, dz, padded(N), part, sum, M, N, s);
     if (rc != MHC_OK) return rc;
   }
   ws += b.dz + b.part;
   const Operand g = dz != nullptr ? Operand{dz, padded(N), padded(N)} : Operand{dout, N, N};
-  if (dx != nullptr) {  // dx[m, k] = sum_n dz[m, n] W[n, k]
-    Product p = {g, {}, M, K, N, gemm::Epilogue{nullptr, nullptr, dx, nullptr, MHC_ACT_NONE, dtype == kF32}, 1, 0};
-    if (const int rc = operand(p.b, w, N, ldw, K, dtype, ws, s)) return rc;
-    if (const int rc = run_product(p, true, false, dtype, ws + (dw != nullptr ? b.x : 0), s)) return rc;
+  Product px = {g, {}, M, K, N, gemm::Epilogue{nullptr, nullptr, dx, nullptr, MHC_ACT_NONE, dtype == kF32}, 1, 0};  // dx[m, k] = sum_n dz[m, n] W[n, k]
+  Product pw = {g, {}, N, K, M, gemm::Epilogue{nullptr, nullptr, dw, nullptr, MHC_ACT_NONE, dtype == kF32}, 1, 0};  // dw[n, k] = sum_m dz[m, n] x[m, k]
+  if (dx != nullptr) {
+    if (const int rc = operand(px.b, w, N, ldw, K, dtype, ws, s)) return rc;
   }
-  if (dw != nullptr) {  // dw[n, k] = sum_m dz[m, n] x[m, k]
-    Product p = {g, {}, N, K, M, gemm::Epilogue{nullptr, nullptr, dw, nullptr, MHC_ACT_NONE, dtype == kF32}, 1, 0};
-    if (const int rc = operand(p.b, x, M, ldx, K, dtype, ws, s)) return rc;
-    if (const int rc = run_product(p, false, false, dtype, ws, s)) return rc;
+  if (dw != nullptr) {
+    if (const int rc = operand(pw.b, x, M, ldx, K, dtype, ws, s)) return rc;
+  }
+  if (b.cut.together) {
+    const gemm::Pair p = {px, pw, 0, 0, 0, 0, part, db, ceil_div(M, dz_rows(M, N)), N};
+    float* const sums = reinterpret_cast<float*>(ws);
+    if (dtype == kF32) return gemm::run_pair_f32(p, b.cut, sums, s);
+    if (dtype == kBF16) return gemm::run_pair_bf16(p, b.cut, sums, s);
+    return gemm::run_pair_f16(p, b.cut, sums, s);
+  }
+  if (dx != nullptr) {
+    if (const int rc = run_product(px, true, false, b.cut.dx, dtype, ws, s)) return rc;
+  }
+  if (dw != nullptr) {
+    if (const int rc = run_product(pw, false, false, b.cut.dw, dtype, ws, s)) return rc;
   }
   return MHC_OK;
 }

@@ -8,6 +8,8 @@ int run_product_bf16(const Product& p, bool a_k, bool b_k, const Cut& c, float* 
   return run_product<__bf16>(p, a_k, b_k, c, part, s);
 }
 
+int run_pair_bf16(const Pair& p, const PairCut& c, float* part, hipStream_t s) { return run_pair<__bf16>(p, c, part, s); }
+
 int run_few_rows_bf16(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K, const Epilogue& e,
                  hipStream_t s) {
   return run_few_rows<__bf16>(x, ldx, w, ldw, M, N, K, e, s);

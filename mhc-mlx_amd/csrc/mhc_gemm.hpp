@@ -505,9 +505,9 @@ MHC_DEV void store_rows(const Epilogue& e, const char* sums, int lane, int64_t m
 // A wave's JM x JN sums of 16 x 16, in registers, to the outputs from (m0, n0)
 // on, through the workgroup's LDS (BYTES of it, free).
 template <typename T, int JM, int JN, int WAVES, int BYTES>
-MHC_DEV void store_tile(const Product& p, char* smem, const f32x4 (&acc)[JN][JM], int64_t m0, int64_t n0, int wave, int lane) {
+MHC_DEV void store_tile(const Product& p, char* smem, const f32x4 (&acc)[JN][JM], int64_t m0, int64_t n0, int wave, int lane, int split) {
   Epilogue e = p.e;
-  if (p.splits > 1) e.out = static_cast<float*>(e.out) + (int64_t)blockIdx.y * p.M * p.N;
+  if (p.splits > 1) e.out = static_cast<float*>(e.out) + (int64_t)split * p.M * p.N;
   // The sums go through LDS, where each wave has room for up to 64 rows
   // of 64 columns, so that rows of the outputs are written as whole vectors of
   // consecutive lanes.  The 16-byte chunk c of row r is at c ^ (r % 16).
@@ -552,16 +552,16 @@ struct Place {
   int64_t m0, n0;
   int wm, wn, k0, k1, wave, lane;
 
-  MHC_DEV Place(const Product& p) {
+  MHC_DEV Place(const Product& p, uint32_t tile, int split) {
     lane = threadIdx.x % kWave;
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     uint32_t tm, tn;
-    tile_of(blockIdx.x, (uint32_t)ceil_div(p.M, BM), (uint32_t)ceil_div(p.N, BN), tm, tn);
+    tile_of(tile, (uint32_t)ceil_div(p.M, BM), (uint32_t)ceil_div(p.N, BN), tm, tn);
     m0 = (int64_t)tm * BM;
     n0 = (int64_t)tn * BN;
     wm = wave / WN * (BM / WM);
     wn = wave % WN * (BN / WN);
-    k0 = (int)blockIdx.y * p.kper;
+    k0 = split * p.kper;
     k1 = min((int)p.K, k0 + p.kper);
   }
 };
@@ -626,16 +626,6 @@ MHC_DEV void sum_tile(const Product& p, const Place<BM, BN, WM, WN>& at, char* s
     interleave<(JM * (AK ? 1 : S::kE / 4) + JN * (BK ? 1 : S::kE / 4)), JM * JN * (sizeof(T) == 4 ? 4 : 1)>();
   }
   wait_loads<0>();  // (the last ones store zeros)
-}
-
-template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
-__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const Product p) {
-  constexpr int kBytes = NS * (BM + BN) * 128;
-  __shared__ __attribute__((aligned(1024))) char smem[kBytes];
-  const Place<BM, BN, WM, WN> at(p);
-  f32x4 acc[BN / WN / 16][BM / WM / 16] = {};
-  sum_tile<T, AK, BK, BM, BN, WM, WN, NS>(p, at, smem, acc);
-  store_tile<T, BM / WM / 16, BN / WN / 16, WM * WN, kBytes>(p, smem, acc, at.m0 + at.wm, at.n0 + at.wn, at.wave, at.lane);
 }
 
 // --------------------------------------------------------------------------
@@ -729,39 +719,103 @@ MHC_DEV void sum_tile_split(const Product& p, const Place<BM, BN, WM, WN>& at, c
   wait_loads<0>();
 }
 
-// A tile with a NaN is summed once more with fp32 instructions: they tell what
-// an infinity makes of it, whose parts make NaN of everything.
-template <bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
-__global__ __launch_bounds__(64 * WM * WN) void split_kernel(const Product p) {
+// --------------------------------------------------------------------------
+// The kernels of tiles
+// --------------------------------------------------------------------------
+
+// A tile of outputs, or (split) of one part of the reduction's sums.  fp32
+// tiles of at least 64 x 128 are summed on the bf16 instructions (64 x 64 have
+// too few products for each value that is split: 65 us so, 57 in fp32 at
+// 1000 x 1100 x 1536; 128 x 128 107 in fp32, 93 so; 8192 x 4096 x 4096 1889
+// and 1180 in 256 x 256, where the library's fp32 product takes 1800), and one
+// with a NaN once more with fp32 instructions: they tell what an infinity
+// makes of it, whose parts make NaN of everything.
+template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
+MHC_DEV void run_tile(const Product& p, char* smem, uint32_t tile, int split) {
   constexpr int kBytes = NS * (BM + BN) * 128, JM = BM / WM / 16, JN = BN / WN / 16;
-  __shared__ __attribute__((aligned(1024))) char smem[kBytes];
-  const Place<BM, BN, WM, WN> at(p);
+  const Place<BM, BN, WM, WN> at(p, tile, split);
   f32x4 acc[JN][JM] = {};
-  sum_tile_split<AK, BK, BM, BN, WM, WN, NS>(p, at, smem, acc);
-  bool nan = false;
-#pragma unroll
-  for (int i = 0; i < JN; ++i)
-#pragma unroll
-    for (int j = 0; j < JM; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) nan |= acc[i][j][e] != acc[i][j][e];
-  int* const found = reinterpret_cast<int*>(smem);
-  const int mine = __ballot(nan) != 0;
-  __syncthreads();  // nobody reads the last stage any more
-  if (at.lane == 0) found[at.wave] = mine;
-  __syncthreads();
-  int again = 0;
-#pragma unroll
-  for (int w = 0; w < WM * WN; ++w) again |= found[w];
-  __syncthreads();
-  if (__builtin_amdgcn_readfirstlane(again)) {
+  if constexpr (sizeof(T) == 4 && BN > 64) {
+    sum_tile_split<AK, BK, BM, BN, WM, WN, NS>(p, at, smem, acc);
+    bool nan = false;
 #pragma unroll
     for (int i = 0; i < JN; ++i)
 #pragma unroll
-      for (int j = 0; j < JM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    sum_tile<float, AK, BK, BM, BN, WM, WN, NS>(p, at, smem, acc);
+      for (int j = 0; j < JM; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) nan |= acc[i][j][e] != acc[i][j][e];
+    int* const found = reinterpret_cast<int*>(smem);
+    const int mine = __ballot(nan) != 0;
+    __syncthreads();  // nobody reads the last stage any more
+    if (at.lane == 0) found[at.wave] = mine;
+    __syncthreads();
+    int again = 0;
+#pragma unroll
+    for (int w = 0; w < WM * WN; ++w) again |= found[w];
+    __syncthreads();
+    if (__builtin_amdgcn_readfirstlane(again)) {
+#pragma unroll
+      for (int i = 0; i < JN; ++i)
+#pragma unroll
+        for (int j = 0; j < JM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      sum_tile<T, AK, BK, BM, BN, WM, WN, NS>(p, at, smem, acc);
+    }
+  } else {
+    sum_tile<T, AK, BK, BM, BN, WM, WN, NS>(p, at, smem, acc);
   }
-  store_tile<float, JM, JN, WM * WN, kBytes>(p, smem, acc, at.m0 + at.wm, at.n0 + at.wn, at.wave, at.lane);
+  store_tile<T, JM, JN, WM * WN, kBytes>(p, smem, acc, at.m0 + at.wm, at.n0 + at.wn, at.wave, at.lane, split);
+}
+
+template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
+__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const Product p) {
+  __shared__ __attribute__((aligned(1024))) char smem[NS * (BM + BN) * 128];
+  run_tile<T, AK, BK, BM, BN, WM, WN, NS>(p, smem, blockIdx.x, (int)blockIdx.y);
+}
+
+// Column sums of fp32 rows: 32 columns for 256 threads, each column in eight
+// parts that are joined in order.
+constexpr int kSumCols = 32;
+
+template <typename T>
+MHC_DEV void sum_columns(float (*lds)[kSumCols], const float* part, T* db, int64_t rows, int64_t N, uint32_t block) {
+  const int c = threadIdx.x % kSumCols, q = threadIdx.x / kSumCols;
+  const int64_t n = (int64_t)block * kSumCols + c;
+  float s = 0.f;
+#pragma unroll 8
+  for (int64_t b = q; b < rows; b += 8) s += part[b * N + min(n, N - 1)];
+  lds[q][c] = s;
+  __syncthreads();
+  if (q != 0 || n >= N) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) s += lds[k][c];
+  store1(db + n, s);
+}
+
+// A backward's two products and the last sums of db, none of which needs
+// another, as one launch: alone, neither product of a few hundred rows fills
+// the card.  The longer reductions go first.
+struct Pair {
+  Product dx, dw;
+  uint32_t dx0, dx_count, dw0, dw_count;  // the workgroups of each; those of db come last
+  const float* part;
+  void* db;
+  int64_t part_rows, N;
+};
+
+template <typename T, int BM, int BN, int WM, int WN, int NS>
+__global__ __launch_bounds__(256) void pair_kernel(const Pair p) {
+  static_assert(WM * WN == 4, "sum_columns has 256 threads");
+  __shared__ __attribute__((aligned(1024))) char smem[NS * (BM + BN) * 128];
+  const uint32_t id = blockIdx.x;
+  if (id - p.dx0 < p.dx_count) {
+    const uint32_t at = id - p.dx0, tiles = p.dx_count / p.dx.splits;
+    run_tile<T, true, false, BM, BN, WM, WN, NS>(p.dx, smem, at % tiles, (int)(at / tiles));
+  } else if (id - p.dw0 < p.dw_count) {
+    const uint32_t at = id - p.dw0, tiles = p.dw_count / p.dw.splits;
+    run_tile<T, false, false, BM, BN, WM, WN, NS>(p.dw, smem, at % tiles, (int)(at / tiles));
+  } else {
+    sum_columns(reinterpret_cast<float(*)[kSumCols]>(smem), p.part, static_cast<T*>(p.db), p.part_rows, p.N, id - p.dx_count - p.dw_count);
+  }
 }
 
 // --------------------------------------------------------------------------
@@ -992,28 +1046,72 @@ constexpr TileCost kTiles[] = {
     {64, 64, 3, 3.6f, 0.245f, 0.21f, 0.58f, 0.525f},
 };
 
+inline float stage_us(const TileCost& c, int dtype, float of_cu) {  // of_cu: workgroups of a CU
+  const float alone = dtype == kF32 ? c.alone32 : c.alone16, busy = dtype == kF32 ? c.busy32 : c.busy16;
+  const float q = ceilf(of_cu);
+  return of_cu <= 1.f ? alone + std::max(0.f, busy - alone) * of_cu : std::max(alone * ceilf(q / c.fit), busy * q);
+}
+
+inline float join_us(int splits, int64_t M, int64_t N) {  // a launch, and 8 bytes of each sum at 4 TB/s
+  return splits > 1 ? 4.f + 2.f * splits * (float)M * (float)N / 1e6f : 0.f;
+}
+
 // The cut with the least estimated time.  Large tiles read least, small ones
 // give every CU work; a reduction is split where even those are too few,
 // which costs a launch and its sums' way through memory.
 inline Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype) {
-  const bool f32 = dtype == kF32;
-  const int kK = f32 ? 32 : 64;
+  const int kK = dtype == kF32 ? 32 : 64;
   const int stages = (int)ceil_div(K, kK);
   const float cus = (float)device_cu_count();
   Cut best = {0, 1, stages * kK, 0.f};
   for (int t = 0; t < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++t) {
     const TileCost& c = kTiles[t];
     const float tiles = (float)ceil_div(M, c.bm) * (float)ceil_div(N, c.bn);
-    const float alone = f32 ? c.alone32 : c.alone16, busy = f32 ? c.busy32 : c.busy16;
     for (int want = 1; want <= 16; ++want) {
       if (want > 1 && (tiles * (want - 1) > 4.f * cus || stages < 2 * want)) break;
       const int per = (stages + want - 1) / want, splits = (stages + per - 1) / per;
       if (splits < want) continue;
-      const float of_cu = tiles * splits / cus, q = ceilf(of_cu);  // workgroups of a CU
-      const float stage = of_cu <= 1.f ? alone + std::max(0.f, busy - alone) * of_cu : std::max(alone * ceilf(q / c.fit), busy * q);
-      float us = c.ends + per * stage;
-      if (splits > 1) us += 4.f + 2.f * splits * (float)M * (float)N / 1e6f;  // 8 bytes each at 4 TB/s
+      const float us = c.ends + per * stage_us(c, dtype, tiles * splits / cus) + join_us(splits, M, N);
       if (best.us == 0.f || us < best.us) best = {t, splits, per * kK, us};
+    }
+  }
+  return best;
+}
+
+// Both products of a backward, dx = dz W and dw = dz^T x, in one launch of the
+// tiles of four waves, or (together false) one after the other.
+struct PairCut {
+  bool together;
+  Cut dx, dw;
+};
+
+inline PairCut pair_of(int64_t M, int64_t N, int64_t K, int dtype) {
+  PairCut best = {false, cut_of(M, K, N, dtype), cut_of(N, K, M, dtype)};
+  float least = best.dx.us + best.dw.us;
+  const float cus = (float)device_cu_count();
+  const int kK = dtype == kF32 ? 32 : 64;
+  const int stages1 = (int)ceil_div(N, kK), stages2 = (int)ceil_div(M, kK);
+  constexpr int kWant[] = {1, 2, 3, 4, 6, 8};
+  for (int t = 2; t < 5; ++t) {
+    const TileCost& c = kTiles[t];
+    const float tiles1 = (float)ceil_div(M, c.bm) * (float)ceil_div(K, c.bn), tiles2 = (float)ceil_div(N, c.bm) * (float)ceil_div(K, c.bn);
+    if (tiles1 + tiles2 > 16.f * cus) continue;  // (each fills the card)
+    for (int want1 : kWant) {
+      if (want1 > 1 && (tiles1 * want1 + tiles2 > 4.f * cus || stages1 < 2 * want1)) break;
+      const int per1 = (stages1 + want1 - 1) / want1, splits1 = (stages1 + per1 - 1) / per1;
+      for (int want2 : kWant) {
+        if (want2 > 1 && (tiles1 * want1 + tiles2 * want2 > 4.f * cus || stages2 < 2 * want2)) break;
+        const int per2 = (stages2 + want2 - 1) / want2, splits2 = (stages2 + per2 - 1) / per2;
+        const float n1 = tiles1 * splits1, n2 = tiles2 * splits2, of_cu = (n1 + n2) / cus;
+        // more than one a CU: of all lengths
+        const float per = of_cu <= 1.f ? (float)std::max(per1, per2) : (n1 * per1 + n2 * per2) / (n1 + n2);
+        const float us = c.ends + std::max(per * stage_us(c, dtype, of_cu), (float)std::max(per1, per2) * stage_us(c, dtype, 0.f)) +
+                         join_us(splits1, M, K) + join_us(splits2, N, K);
+        if (us < least) {
+          least = us;
+          best = {true, {t, splits1, per1 * kK, us}, {t, splits2, per2 * kK, us}};
+        }
+      }
     }
   }
   return best;
@@ -1037,15 +1135,10 @@ inline bool few_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, int
   return few <= cut_of(M, N, K, dtype).us + copies;
 }
 
-// BM x BN tiles; fp32 ones of at least 64 x 128 on the bf16 instructions (64 x 64
-// have too few products for each value that is split: 65 us so, 57 in fp32 at
-// 1000 x 1100 x 1536; 128 x 128 107 in fp32, 93 so; 8192 x 4096 x 4096 1889
-// and 1180 in 256 x 256, where the library's fp32 product takes 1800)
 template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
 int launch(const Product& p, hipStream_t s) {
   const dim3 grid((unsigned)(ceil_div(p.M, BM) * ceil_div(p.N, BN)), (unsigned)p.splits), block(64 * WM * WN);
-  if constexpr (sizeof(T) == 4 && BN > 64) hipLaunchKernelGGL((split_kernel<AK, BK, BM, BN, WM, WN, NS>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((tile_kernel<T, AK, BK, BM, BN, WM, WN, NS>), grid, block, 0, s, p);
+  hipLaunchKernelGGL((tile_kernel<T, AK, BK, BM, BN, WM, WN, NS>), grid, block, 0, s, p);
   MHC_CHECK_LAUNCH("tile_kernel");
   return MHC_OK;
 }
@@ -1059,6 +1152,36 @@ int run_layout(const Product& p, int tile, hipStream_t s) {
     case 3: return launch<T, AK, BK, 64, 128, 2, 2, 3>(p, s);
     default: return launch<T, AK, BK, 64, 64, 4, 1, 3>(p, s);
   }
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int NS>
+int launch_pair(Pair p, hipStream_t s) {
+  p.dx_count = (uint32_t)(ceil_div(p.dx.M, BM) * ceil_div(p.dx.N, BN) * p.dx.splits);
+  p.dw_count = (uint32_t)(ceil_div(p.dw.M, BM) * ceil_div(p.dw.N, BN) * p.dw.splits);
+  const bool first = p.dx.kper >= p.dw.kper;
+  p.dx0 = first ? 0 : p.dw_count;
+  p.dw0 = first ? p.dx_count : 0;
+  const unsigned sums = p.db != nullptr ? (unsigned)ceil_div(p.N, kSumCols) : 0;
+  hipLaunchKernelGGL((pair_kernel<T, BM, BN, WM, WN, NS>), dim3(p.dx_count + p.dw_count + sums), dim3(256), 0, s, p);
+  MHC_CHECK_LAUNCH("pair_kernel");
+  return MHC_OK;
+}
+
+// The products of a backward together.  part: the sums of dx's parts, if it is split, and then of dw's.
+template <typename T>
+int run_pair(Pair p, const PairCut& c, float* part, hipStream_t s) {
+  const Epilogue dx = p.dx.e, dw = p.dw.e;
+  float* const part2 = c.dx.splits > 1 ? part + c.dx.splits * p.dx.M * p.dx.N : part;
+  p.dx.splits = c.dx.splits, p.dx.kper = c.dx.kper;
+  p.dw.splits = c.dw.splits, p.dw.kper = c.dw.kper;
+  if (c.dx.splits > 1) p.dx.e = Epilogue{nullptr, nullptr, part, nullptr, MHC_ACT_NONE, 1};
+  if (c.dw.splits > 1) p.dw.e = Epilogue{nullptr, nullptr, part2, nullptr, MHC_ACT_NONE, 1};
+  int rc = c.dx.tile == 2   ? launch_pair<T, 128, 128, 2, 2, 2>(p, s)
+           : c.dx.tile == 3 ? launch_pair<T, 64, 128, 2, 2, 3>(p, s)
+                            : launch_pair<T, 64, 64, 4, 1, 3>(p, s);
+  if (rc == MHC_OK && c.dx.splits > 1) rc = launch_join<T>(dx, part, c.dx.splits, p.dx.M, p.dx.N, s);
+  if (rc == MHC_OK && c.dw.splits > 1) rc = launch_join<T>(dw, part2, c.dw.splits, p.dw.M, p.dw.N, s);
+  return rc;
 }
 
 // The product of one type; a_k / b_k: the operand's k are contiguous.  part: splits * M * N floats where it is split.
@@ -1078,6 +1201,9 @@ int run_product(Product p, bool a_k, bool b_k, const Cut& c, float* part, hipStr
 int run_few_rows_f32(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K, const Epilogue& e, hipStream_t s);
 int run_few_rows_bf16(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K, const Epilogue& e, hipStream_t s);
 int run_few_rows_f16(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K, const Epilogue& e, hipStream_t s);
+int run_pair_f32(const Pair& p, const PairCut& c, float* part, hipStream_t s);
+int run_pair_bf16(const Pair& p, const PairCut& c, float* part, hipStream_t s);
+int run_pair_f16(const Pair& p, const PairCut& c, float* part, hipStream_t s);
 int run_product_f32(const Product& p, bool a_k, bool b_k, const Cut& c, float* part, hipStream_t s);
 int run_product_bf16(const Product& p, bool a_k, bool b_k, const Cut& c, float* part, hipStream_t s);
 int run_product_f16(const Product& p, bool a_k, bool b_k, const Cut& c, float* part, hipStream_t s);
