@@ -793,7 +793,9 @@ MHC_DEV void sum_columns(float (*lds)[kSumCols], const float* part, T* db, int64
 
 // A backward's two products and the last sums of db, none of which needs
 // another, as one launch: alone, neither product of a few hundred rows fills
-// the card.  The longer reductions go first.
+// the card, and each launch is some 3 us of host time (backward of 1000 x 1100
+// x 1536 fp32: 99 us in four launches, 65 in two; 64 x 1024 x 1024 bf16 19 and
+// 14).  The longer reductions go first.
 struct Pair {
   Product dx, dw;
   uint32_t dx0, dx_count, dw0, dw_count;  // the workgroups of each; those of db come last
