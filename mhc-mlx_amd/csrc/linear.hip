@@ -69,7 +69,7 @@ __global__ __launch_bounds__(256) void dz_kernel(const G* dout, const void* dact
 template <typename T>
 __global__ __launch_bounds__(256) void db_kernel(const float* part, T* db, int64_t rows, int64_t N) {
   __shared__ float lds[8][gemm::kSumCols];
-  gemm::sum_columns(lds, part, db, rows, N, blockIdx.x);
+  gemm::sum_columns<256>(lds, part, db, rows, N, blockIdx.x);
 }
 
 // rows of `width` elements, `ld` apart, into rows of whole chunks of 16 bytes, with zeros after the last element

@@ -772,22 +772,23 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const Product p) {
   run_tile<T, AK, BK, BM, BN, WM, WN, NS>(p, smem, blockIdx.x, (int)blockIdx.y);
 }
 
-// Column sums of fp32 rows: 32 columns for 256 threads, each column in eight
-// parts that are joined in order.
+// Column sums of fp32 rows: 32 columns a workgroup, each column in eight parts
+// (sixteen with 512 threads) that are joined in order.
 constexpr int kSumCols = 32;
 
-template <typename T>
+template <int THREADS, typename T>
 MHC_DEV void sum_columns(float (*lds)[kSumCols], const float* part, T* db, int64_t rows, int64_t N, uint32_t block) {
+  constexpr int kParts = THREADS / kSumCols;
   const int c = threadIdx.x % kSumCols, q = threadIdx.x / kSumCols;
   const int64_t n = (int64_t)block * kSumCols + c;
   float s = 0.f;
 #pragma unroll 8
-  for (int64_t b = q; b < rows; b += 8) s += part[b * N + min(n, N - 1)];
+  for (int64_t b = q; b < rows; b += kParts) s += part[b * N + min(n, N - 1)];
   lds[q][c] = s;
   __syncthreads();
   if (q != 0 || n >= N) return;
 #pragma unroll
-  for (int k = 1; k < 8; ++k) s += lds[k][c];
+  for (int k = 1; k < kParts; ++k) s += lds[k][c];
   store1(db + n, s);
 }
 
@@ -805,8 +806,7 @@ struct Pair {
 };
 
 template <typename T, int BM, int BN, int WM, int WN, int NS>
-__global__ __launch_bounds__(256) void pair_kernel(const Pair p) {
-  static_assert(WM * WN == 4, "sum_columns has 256 threads");
+__global__ __launch_bounds__(64 * WM * WN) void pair_kernel(const Pair p) {
   __shared__ __attribute__((aligned(1024))) char smem[NS * (BM + BN) * 128];
   const uint32_t id = blockIdx.x;
   if (id - p.dx0 < p.dx_count) {
@@ -816,7 +816,7 @@ __global__ __launch_bounds__(256) void pair_kernel(const Pair p) {
     const uint32_t at = id - p.dw0, tiles = p.dw_count / p.dw.splits;
     run_tile<T, false, false, BM, BN, WM, WN, NS>(p.dw, smem, at % tiles, (int)(at / tiles));
   } else {
-    sum_columns(reinterpret_cast<float(*)[kSumCols]>(smem), p.part, static_cast<T*>(p.db), p.part_rows, p.N, id - p.dx_count - p.dw_count);
+    sum_columns<64 * WM * WN>(reinterpret_cast<float(*)[kSumCols]>(smem), p.part, static_cast<T*>(p.db), p.part_rows, p.N, id - p.dx_count - p.dw_count);
   }
 }
 
@@ -1044,8 +1044,8 @@ struct TileCost {
 };
 constexpr TileCost kTiles[] = {
     {256, 256, 1, 7.0f, 1.12f, 1.60f, 4.10f, 4.75f},   {128, 256, 1, 5.0f, 0.68f, 0.92f, 2.35f, 2.60f},
-    {128, 128, 2, 5.0f, 0.545f, 0.54f, 1.67f, 1.28f},  {64, 128, 2, 4.5f, 0.40f, 0.34f, 1.03f, 0.78f},
-    {64, 64, 3, 3.6f, 0.245f, 0.21f, 0.58f, 0.525f},
+    {128, 128, 2, 5.0f, 0.48f, 0.53f, 1.67f, 1.28f},   {64, 128, 2, 4.5f, 0.35f, 0.335f, 1.03f, 0.78f},
+    {64, 64, 3, 3.6f, 0.29f, 0.21f, 0.58f, 0.525f},
 };
 
 inline float stage_us(const TileCost& c, int dtype, float of_cu) {  // of_cu: workgroups of a CU
@@ -1081,7 +1081,7 @@ inline Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype) {
 }
 
 // Both products of a backward, dx = dz W and dw = dz^T x, in one launch of the
-// tiles of four waves, or (together false) one after the other.
+// smaller tiles, or (together false) one after the other.
 struct PairCut {
   bool together;
   Cut dx, dw;
@@ -1145,13 +1145,21 @@ int launch(const Product& p, hipStream_t s) {
   return MHC_OK;
 }
 
+// Rows of waves of the middle tiles: two waves for each SIMD, so that one has
+// products while the other waits for its fragments (bf16 2048 x 2048 x 2048 in
+// 128 x 128 28 us with four waves, 24 with eight; 1000 x 1024 x 1024 in
+// 64 x 128 11.2 and 9.8).  fp32, which has more products for each fragment,
+// stays with four (2048 x 2048 x 2048 in two parts 104 and 111).
+template <typename T>
+constexpr int kRowWaves = sizeof(T) == 2 ? 4 : 2;
+
 template <typename T, bool AK, bool BK>
 int run_layout(const Product& p, int tile, hipStream_t s) {
   switch (tile) {
     case 0: return launch<T, AK, BK, 256, 256, 2, 4, 2>(p, s);
     case 1: return launch<T, AK, BK, 128, 256, 2, 4, 2>(p, s);
-    case 2: return launch<T, AK, BK, 128, 128, 2, 2, 2>(p, s);
-    case 3: return launch<T, AK, BK, 64, 128, 2, 2, 3>(p, s);
+    case 2: return launch<T, AK, BK, 128, 128, kRowWaves<T>, 2, 2>(p, s);
+    case 3: return launch<T, AK, BK, 64, 128, kRowWaves<T>, 2, 3>(p, s);
     default: return launch<T, AK, BK, 64, 64, 4, 1, 3>(p, s);
   }
 }
@@ -1164,7 +1172,7 @@ int launch_pair(Pair p, hipStream_t s) {
   p.dx0 = first ? 0 : p.dw_count;
   p.dw0 = first ? p.dx_count : 0;
   const unsigned sums = p.db != nullptr ? (unsigned)ceil_div(p.N, kSumCols) : 0;
-  hipLaunchKernelGGL((pair_kernel<T, BM, BN, WM, WN, NS>), dim3(p.dx_count + p.dw_count + sums), dim3(256), 0, s, p);
+  hipLaunchKernelGGL((pair_kernel<T, BM, BN, WM, WN, NS>), dim3(p.dx_count + p.dw_count + sums), dim3(64 * WM * WN), 0, s, p);
   MHC_CHECK_LAUNCH("pair_kernel");
   return MHC_OK;
 }
@@ -1178,8 +1186,8 @@ int run_pair(Pair p, const PairCut& c, float* part, hipStream_t s) {
   p.dw.splits = c.dw.splits, p.dw.kper = c.dw.kper;
   if (c.dx.splits > 1) p.dx.e = Epilogue{nullptr, nullptr, part, nullptr, MHC_ACT_NONE, 1};
   if (c.dw.splits > 1) p.dw.e = Epilogue{nullptr, nullptr, part2, nullptr, MHC_ACT_NONE, 1};
-  int rc = c.dx.tile == 2   ? launch_pair<T, 128, 128, 2, 2, 2>(p, s)
-           : c.dx.tile == 3 ? launch_pair<T, 64, 128, 2, 2, 3>(p, s)
+  int rc = c.dx.tile == 2   ? launch_pair<T, 128, 128, kRowWaves<T>, 2, 2>(p, s)
+           : c.dx.tile == 3 ? launch_pair<T, 64, 128, kRowWaves<T>, 2, 3>(p, s)
                             : launch_pair<T, 64, 64, 4, 1, 3>(p, s);
   if (rc == MHC_OK && c.dx.splits > 1) rc = launch_join<T>(dx, part, c.dx.splits, p.dx.M, p.dx.N, s);
   if (rc == MHC_OK && c.dw.splits > 1) rc = launch_join<T>(dw, part2, c.dw.splits, p.dw.M, p.dw.N, s);
