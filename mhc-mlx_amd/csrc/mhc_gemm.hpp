@@ -824,25 +824,29 @@ __global__ __launch_bounds__(64 * WM * WN) void pair_kernel(const Pair p) {
 // Few rows: x W^T with M <= 64, bound by reading W
 // --------------------------------------------------------------------------
 
-// A workgroup has 16 rows of W and all of x, and its eight waves take stages
-// of the k in turn: each wave has some of its own under way to LDS, so that
-// memory is read in whole lines (fragments read straight from memory are half
-// lines: 9.1 us for 16 rows of 4096 x 4096 bf16, 12.7 us for 32; so 6.0, 8.0).  No wave waits for another before the end, where their
-// sums meet in LDS, in order.
+// A workgroup has 16 NT rows of W and all of x, and its eight waves take
+// stages of the k in turn: each wave has some of its own under way to LDS, so
+// that memory is read in whole lines (fragments read straight from memory are
+// half lines: 9.1 us for 16 rows of 4096 x 4096 bf16, 12.7 us for 32; so 6.0,
+// 8.0).  No wave waits for another before the end, where their sums meet in
+// LDS, in order.
 constexpr int kFewWaves = 8;
 
 // the waves' sums, in order, and the epilogue
-template <typename T, int MT>
-MHC_DEV void join_waves(const f32x4 (&acc)[MT], float* sums, int M, int64_t n0, int64_t N, const Epilogue& e) {
+template <typename T, int MT, int NT>
+MHC_DEV void join_waves(const f32x4 (&acc)[NT][MT], float* sums, int M, int64_t n0, int64_t N, const Epilogue& e) {
+  constexpr int kN = 16 * NT;
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
 #pragma unroll
-  for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(sums + ((wave * MT + j) * 16 + lane % 16) * 16 + lane / 16 * 4) = acc[j];
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(sums + ((wave * MT + j) * 16 + lane % 16) * kN + i * 16 + lane / 16 * 4) = acc[i][j];
   __syncthreads();
-  for (int at = threadIdx.x; at < MT * 256; at += 64 * kFewWaves) {
-    const int m = at / 16, n = at % 16;
+  for (int at = threadIdx.x; at < MT * 16 * kN; at += 64 * kFewWaves) {
+    const int m = at / kN, n = at % kN;
     float z[1][1] = {};
 #pragma unroll
-    for (int v = 0; v < kFewWaves; ++v) z[0][0] += sums[(v * MT * 16 + m) * 16 + n];
+    for (int v = 0; v < kFewWaves; ++v) z[0][0] += sums[(v * MT * 16 + m) * kN + n];
     if (m < M && n0 + n < N) {
       float bias[1], residual[1][1];
       bias_of<T>(e, n0 + n, 1, bias);
@@ -852,24 +856,24 @@ MHC_DEV void join_waves(const f32x4 (&acc)[MT], float* sums, int M, int64_t n0, 
   }
 }
 
-template <typename T, int MT, int NS>
+template <typename T, int MT, int NT, int NS>
 __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const Operand x, const Operand w, int M, int64_t N, int K, const Epilogue e) {
   using S = Stage<T>;
-  constexpr int kW = 2048, kStage = kW * (1 + MT), kLoads = 2 * (1 + MT);
+  constexpr int kW = 2048 * NT, kStage = 2048 * (NT + MT), kLoads = 2 * (NT + MT);
   __shared__ __attribute__((aligned(1024))) char smem[kFewWaves * NS * kStage];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int64_t n0 = (int64_t)blockIdx.x * (16 * NT);
   char* const mine = smem + wave * NS * kStage;
-  Loader<T, true, 16, 1> lw;
+  Loader<T, true, 16 * NT, 1> lw;
   Loader<T, true, 16 * MT, 1> lx;
   lw.init(w, n0, N, wave * S::kK, K, 0, lane, lds_address(mine));
   lx.init(x, 0, M, wave * S::kK, K, 0, lane, lds_address(mine) + kW);
   lw.step = lx.step = kFewWaves * 128;
-  Reader<T, true, 16, 1> rw;
+  Reader<T, true, 16 * NT, NT> rw;
   Reader<T, true, 16 * MT, MT> rx;
   rw.init(0, lane);
   rx.init(0, lane);
-  f32x4 acc[MT] = {};
+  f32x4 acc[NT][MT] = {};
   int kleft = K - wave * S::kK;
 #pragma unroll
   for (int q = 0; q < NS; ++q) {
@@ -885,10 +889,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const Operand 
       lw.clear_end(mine + cur, kleft, lane, kWave);
       lx.clear_end(mine + cur + kW, kleft, lane, kWave);
     }
-    u32x4 fw[2], fx[2][MT];
+    u32x4 fw[2][NT], fx[2][MT];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      fw[s] = rw.get(mine + cur, s, 0);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) fw[s][i] = rw.get(mine + cur, s, i);
 #pragma unroll
       for (int j = 0; j < MT; ++j) fx[s][j] = rx.get(mine + cur + kW, s, j);
     }
@@ -900,12 +905,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const Operand 
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int j = 0; j < MT; ++j) acc[j] = mfma16<T>(fw[s], fx[s][j], acc[j]);
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[i][j] = mfma16<T>(fw[s][i], fx[s][j], acc[i][j]);
     cur = cur == (NS - 1) * kStage ? 0 : cur + kStage;
   }
   wait_loads<0>();
   __syncthreads();
-  join_waves<T, MT>(acc, reinterpret_cast<float*>(smem), M, n0, N, e);
+  join_waves<T, MT, NT>(acc, reinterpret_cast<float*>(smem), M, n0, N, e);
 }
 
 // The same for rows that start anywhere: fragments straight from memory, with
@@ -940,7 +947,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_ragged_rows_kernel(const T
   const T* xr[MT];
 #pragma unroll
   for (int j = 0; j < MT; ++j) xr[j] = x + (int64_t)min(j * 16 + r, M - 1) * ldx + g * kE;
-  f32x4 acc[MT] = {};
+  f32x4 acc[1][MT] = {};
   const int whole = K / (kStep * kDepth) * (kStep * kDepth);
   for (int k = wave * kStep * kDepth; k < whole; k += kFewWaves * kStep * kDepth) {
     u32x4 fw[kDepth], fx[MT][kDepth];
@@ -953,37 +960,53 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_ragged_rows_kernel(const T
 #pragma unroll
     for (int q = 0; q < kDepth; ++q)
 #pragma unroll
-      for (int j = 0; j < MT; ++j) acc[j] = mfma16<T>(fw[q], fx[j][q], acc[j]);
+      for (int j = 0; j < MT; ++j) acc[0][j] = mfma16<T>(fw[q], fx[j][q], acc[0][j]);
   }
   for (int k = whole + wave * kStep; k < K; k += kFewWaves * kStep) {
     const int left = K - k - g * kE;
     const bool full = left >= kE;
     const u32x4 fw = full ? load_any(wr + k) : load_end(wr + k, left);
 #pragma unroll
-    for (int j = 0; j < MT; ++j) acc[j] = mfma16<T>(fw, full ? load_any(xr[j] + k) : load_end(xr[j] + k, left), acc[j]);
+    for (int j = 0; j < MT; ++j) acc[0][j] = mfma16<T>(fw, full ? load_any(xr[j] + k) : load_end(xr[j] + k, left), acc[0][j]);
   }
-  join_waves<T, MT>(acc, sums, M, n0, N, e);
+  join_waves<T, MT, 1>(acc, sums, M, n0, N, e);
 }
 
-template <typename T, int MT>
-int launch_few_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K, const Epilogue& e, hipStream_t s) {
-  const dim3 grid((unsigned)ceil_div(N, 16)), block(64 * kFewWaves);
-  // (more stages under way in fewer workgroups of a CU: 5.4 for 4.9 us at one row of 4096 x 4096, 10.1 for 8.6 at 32 of 8192 x 2048)
-  if (in_words(x, ldx, K, sizeof(T)) && in_words(w, ldw, K, sizeof(T)))
-    hipLaunchKernelGGL((few_rows_kernel<T, MT, MT == 1 ? 2 : 1>), grid, block, 0, s, Operand{x, ldx, K}, Operand{w, ldw, K}, (int)M, N,
-                       (int)K, e);
-  else
-    hipLaunchKernelGGL((few_ragged_rows_kernel<T, MT>), grid, block, 0, s, static_cast<const T*>(x), ldx, static_cast<const T*>(w), ldw,
-                       (int)M, N, (int)K, e);
+template <typename T, int MT, int NT, int NS>
+int launch_few_rows(const Operand& x, const Operand& w, int64_t M, int64_t N, int64_t K, const Epilogue& e, hipStream_t s) {
+  hipLaunchKernelGGL((few_rows_kernel<T, MT, NT, NS>), dim3((unsigned)ceil_div(N, 16 * NT)), dim3(64 * kFewWaves), 0, s, x, w, (int)M, N,
+                     (int)K, e);
   MHC_CHECK_LAUNCH("few_rows_kernel");
   return MHC_OK;
 }
 
+template <typename T, int MT>
+int launch_few(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K, const Epilogue& e, hipStream_t s) {
+  const dim3 grid((unsigned)ceil_div(N, 16)), block(64 * kFewWaves);
+  if (!in_words(x, ldx, K, sizeof(T)) || !in_words(w, ldw, K, sizeof(T))) {
+    hipLaunchKernelGGL((few_ragged_rows_kernel<T, MT>), grid, block, 0, s, static_cast<const T*>(x), ldx, static_cast<const T*>(w), ldw,
+                       (int)M, N, (int)K, e);
+    MHC_CHECK_LAUNCH("few_ragged_rows_kernel");
+    return MHC_OK;
+  }
+  const Operand ox = {x, ldx, K}, ow = {w, ldw, K};
+  // Each workgroup reads all of x: between one and two of 16 columns a CU, one
+  // of 32 columns reads it once (bf16, 8192 x 2048: 32 rows 11.6 for 10.0 us,
+  // 64 rows 13.9 for 12.4; but 4096 x 4096 9.5 for 12.4, and 8200 x 1000
+  // 7.5 for 8.4: some CUs have two; in fp32 17.0 for 20.0).
+  if constexpr (MT >= 2 && sizeof(T) == 2) {
+    const int64_t cus = device_cu_count();
+    if (N > 16 * cus && N <= 32 * cus) return launch_few_rows<T, MT, 2, MT == 2 ? 2 : 1>(ox, ow, M, N, K, e, s);
+  }
+  // (more stages under way in fewer workgroups of a CU: 5.4 for 4.9 us at one row of 4096 x 4096, 10.1 for 8.6 at 32 of 8192 x 2048)
+  return launch_few_rows<T, MT, 1, MT == 1 ? 2 : 1>(ox, ow, M, N, K, e, s);
+}
+
 template <typename T>
 int run_few_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K, const Epilogue& e, hipStream_t s) {
-  if (M <= 16) return launch_few_rows<T, 1>(x, ldx, w, ldw, M, N, K, e, s);
-  if (M <= 32) return launch_few_rows<T, 2>(x, ldx, w, ldw, M, N, K, e, s);
-  return launch_few_rows<T, 4>(x, ldx, w, ldw, M, N, K, e, s);
+  if (M <= 16) return launch_few<T, 1>(x, ldx, w, ldw, M, N, K, e, s);
+  if (M <= 32) return launch_few<T, 2>(x, ldx, w, ldw, M, N, K, e, s);
+  return launch_few<T, 4>(x, ldx, w, ldw, M, N, K, e, s);
 }
 
 // The sum over the splits, in order, and the epilogue: eight columns a thread

@@ -357,3 +357,29 @@ def test_module_forms():
     close(out, ref, bound)
     y, d = act64(ref, "none")
     assert y.shape == d.shape
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("M", [17, 32, 64])
+@pytest.mark.parametrize("columns,more", [(16, 0), (16, 2), (25, 7), (32, 0), (32, 1)])
+def test_few_rows_of_wide_layers(M, columns, more, dt):
+    """Around the widths that give each compute unit one workgroup of 16 or of 32 columns."""
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    _check(*_inputs(M, columns * cus + more, 200, dt, 21), "gelu")
+
+
+@pytest.mark.parametrize("M,N,K", [(70, 300, 200), (100, 2048, 72), (90, 72, 2048), (512, 512, 1024), (1000, 520, 1030), (1500, 1001, 260),
+                                   (2049, 1500, 1024), (3000, 200, 130)])
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("bias", [True, False])
+def test_backward_of_middle_sizes(M, N, K, dt, bias):
+    """Both products of the backward in one launch, whole and split, with and without the bias's sums."""
+    ts = _inputs(M, N, K, dt, 22, bias=bias)
+    _check(*ts, "silu")
+    x, w, b, _, g = ts
+
+    def grads():
+        return torch.autograd.grad(linear_act(x, w, b, activation="silu"), [t for t in (x, w, b) if t is not None], g)
+
+    for one, two in zip(grads(), grads()):
+        assert torch.equal(one, two)
