@@ -160,6 +160,7 @@ MHC_DEV float denominator_of(const mhc_policy_args& a, float (&lds)[32]) {
   float d = (float)a.T;
   if (a.weights != nullptr) {
     d = 0.f;
+#pragma unroll 8
     for (int64_t t = threadIdx.x; t < a.T; t += THREADS) d += weight_of(a, t);
     d = sum_workgroup<THREADS>(d, lds);
   }
@@ -328,6 +329,7 @@ __global__ __launch_bounds__(kRowThreads) void policy_loss_kernel(const mhc_poli
   __shared__ float lds[32];
   __shared__ double lds_terms[kRowThreads / kWave];
   double s = 0;  // (terms of both signs)
+#pragma unroll 8
   for (int64_t t = threadIdx.x; t < a.T; t += kRowThreads) s += (double)terms[t];
   s = sum_workgroup<kRowThreads>(s, lds_terms);
   const float den = denominator_of<kRowThreads>(a, lds);
