@@ -10,10 +10,14 @@
 // that of the same formula in elementary tensor operations.
 //
 // A model around mHC layers has hundreds of tensors of 4 to 4096 floats next
-// to a few of millions.  Up to kMaxTensors of them go into one launch: their
-// pointers travel in the kernel arguments (no table in device memory that a
+// to a few of millions.  As many of them go into one launch as the kernel
+// arguments hold (100 in fp32, 84 with master copies, 72 with both and states
+// in 8 bits): their pointers travel there (no table in device memory that a
 // captured graph or a later step could find changed), and a workgroup finds
-// its tensor with one load of the chunk counts, a lane each, and a vote.
+// its tensor with one or two loads of the chunk counts, a lane each, and
+// votes.  Large tensors are bound by memory (16 of 4096 x 4096 bf16 with
+// masters: 28 bytes an element at 5.3 TB/s; in 8 bits 5.2 TB/s), lists of
+// small ones by the host.
 #include <cmath>
 
 #include "mhc_device.hpp"
@@ -22,7 +26,6 @@
 namespace mhc {
 namespace {
 
-constexpr int kMaxTensors = 60;   // 60 * (56 + 4) bytes of arguments: the limit is 4096
 constexpr int kThreads = 256;
 constexpr int kQuant = 256;       // elements that share a scale: one wave, four elements a lane
 constexpr int kPass = kThreads * 4;  // elements that a workgroup has at a time
@@ -36,13 +39,18 @@ struct Hyper {
   const float* gscale_ptr;  // a factor of the gradients in device memory, or NULL
 };
 
+template <bool MASTER, bool Q8>
 struct Table {
-  mhc_adamw_tensor t[kMaxTensors];
-  int32_t end[kMaxTensors];  // chunks of the tensors up to and with this one
+  static constexpr int kPointers = 4 + MASTER + Q8;
+  static constexpr int kMax = (4096 - (int)sizeof(Hyper) - 16) / (8 * kPointers + 8);
+  void* p[kMax][kPointers];  // param, grad, exp_avg, exp_avg_sq, master, scales
+  int32_t end[kMax];         // chunks of the tensors up to and with this one
+  int32_t last[kMax];        // elements of the tensor's last chunk
   int32_t count, chunk;      // elements of a chunk
   Hyper h;
 };
-static_assert(sizeof(Table) <= 4096, "kernel arguments");
+static_assert(sizeof(Table<false, false>) <= 4096 && sizeof(Table<true, false>) <= 4096 && sizeof(Table<true, true>) <= 4096,
+              "kernel arguments");
 
 struct Quad {
   float v[4];
@@ -127,41 +135,51 @@ MHC_DEV uint32_t encode(const Quad& q, float top) {
 MHC_DEV bool lines_up(const void* p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
 
 template <typename P, bool MASTER, bool Q8>
-__global__ __launch_bounds__(kThreads) void adamw_kernel(const Table tab) {
+__global__ __launch_bounds__(kThreads) void adamw_kernel(const Table<MASTER, Q8> tab) {
 #pragma clang fp contract(off)
+  constexpr int kMax = Table<MASTER, Q8>::kMax;
+  static_assert(kMax > kWave && kMax <= 2 * kWave, "two tensors for each lane");
   const int chunk = (int)blockIdx.x, lane = (int)threadIdx.x % kWave;
-  static_assert(kMaxTensors <= kWave, "a lane for each tensor");
-  const uint64_t past = __ballot(lane < tab.count && tab.end[min(lane, kMaxTensors - 1)] > chunk);
-  const int lo = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(past));
-  const mhc_adamw_tensor& t = tab.t[lo];
+  int lo;
+  const uint64_t past = __ballot(lane < tab.count && tab.end[lane] > chunk);
+  if (past != 0) {
+    lo = __builtin_ctzll(past);
+  } else {
+    const int at = kWave + lane;
+    lo = kWave + __builtin_ctzll(__ballot(at < tab.count && tab.end[min(at, kMax - 1)] > chunk));
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  void* const* const t = tab.p[lo];
   const int64_t first = (int64_t)(chunk - (lo > 0 ? tab.end[lo - 1] : 0)) * tab.chunk;
-  P* const p = static_cast<P*>(t.param);
-  const P* const g = static_cast<const P*>(t.grad);
+  const int64_t end = first + (chunk + 1 == tab.end[lo] ? tab.last[lo] : tab.chunk);
+  P* const p = static_cast<P*>(t[0]);
+  const P* const g = static_cast<const P*>(t[1]);
+  float* const master = MASTER ? static_cast<float*>(t[3 + MASTER]) : nullptr;
+  float* const scales = Q8 ? static_cast<float*>(t[3 + MASTER + Q8]) : nullptr;
   const Hyper& h = tab.h;
   const float gs = h.gscale_ptr != nullptr ? h.gscale * *h.gscale_ptr : h.gscale;
   // four elements at a multiple of four from an aligned start are one vector
   const bool pvec = lines_up(p, 4 * sizeof(P)) && lines_up(g, 4 * sizeof(P));
-  const bool svec = Q8 ? lines_up(t.exp_avg, 4) && lines_up(t.exp_avg_sq, 4)
-                       : lines_up(t.exp_avg, 16) && lines_up(t.exp_avg_sq, 16);
-  const bool mvec = !MASTER || lines_up(t.master, 16);
+  const bool svec = Q8 ? lines_up(t[2], 4) && lines_up(t[3], 4) : lines_up(t[2], 16) && lines_up(t[3], 16);
+  const bool mvec = !MASTER || lines_up(master, 16);
 
-  for (int64_t i = first + threadIdx.x * 4; i < first + tab.chunk; i += kPass) {
+  for (int64_t i = first + threadIdx.x * 4; ; i += kPass) {
     // a wave's 256 elements are one block of an 8-bit state; its lanes past the end take part with zeros
-    const int left = (int)min((int64_t)4, t.numel - i);
-    if (t.numel - (i - (threadIdx.x % kWave) * 4) <= 0) break;
+    const int left = (int)min((int64_t)4, end - i);
+    if (i - lane * 4 >= end) break;
     Quad gq = load4(g + i, pvec, left), pq;
-    if constexpr (MASTER) pq = load4(t.master + i, mvec, left);
+    if constexpr (MASTER) pq = load4(master + i, mvec, left);
     else pq = load4(p + i, pvec, left);
     Quad mq, vq;
     const int64_t b = i / kQuant;
     if constexpr (Q8) {
-      mq = decode(load_codes(static_cast<const uint8_t*>(t.exp_avg) + i, svec, left), t.scales[2 * b]);
-      vq = decode(load_codes(static_cast<const uint8_t*>(t.exp_avg_sq) + i, svec, left), t.scales[2 * b + 1]);
+      mq = decode(load_codes(static_cast<const uint8_t*>(t[2]) + i, svec, left), scales[2 * b]);
+      vq = decode(load_codes(static_cast<const uint8_t*>(t[3]) + i, svec, left), scales[2 * b + 1]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) vq.v[k] = vq.v[k] * vq.v[k];
     } else {
-      mq = load4(static_cast<const float*>(t.exp_avg) + i, svec, left);
-      vq = load4(static_cast<const float*>(t.exp_avg_sq) + i, svec, left);
+      mq = load4(static_cast<const float*>(t[2]) + i, svec, left);
+      vq = load4(static_cast<const float*>(t[3]) + i, svec, left);
     }
     Quad rq;
 #pragma unroll
@@ -176,40 +194,62 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Table tab) {
     if constexpr (Q8) {
       // the second moment is held as its root: half the exponents, so 8 bits cover 2^35 of v below a block's largest
       const float mt = wave_top(mq), rt = wave_top(rq);
-      store_codes(static_cast<uint8_t*>(t.exp_avg) + i, encode(mq, mt), svec, left);
-      store_codes(static_cast<uint8_t*>(t.exp_avg_sq) + i, encode(rq, rt), svec, left);
+      store_codes(static_cast<uint8_t*>(t[2]) + i, encode(mq, mt), svec, left);
+      store_codes(static_cast<uint8_t*>(t[3]) + i, encode(rq, rt), svec, left);
       if (threadIdx.x % kWave == 0) {
-        t.scales[2 * b] = mt * (1.f / kCodeMax);
-        t.scales[2 * b + 1] = rt * (1.f / kCodeMax);
+        scales[2 * b] = mt * (1.f / kCodeMax);
+        scales[2 * b + 1] = rt * (1.f / kCodeMax);
       }
     } else {
-      store4(static_cast<float*>(t.exp_avg) + i, mq, svec, left);
-      store4(static_cast<float*>(t.exp_avg_sq) + i, vq, svec, left);
+      store4(static_cast<float*>(t[2]) + i, mq, svec, left);
+      store4(static_cast<float*>(t[3]) + i, vq, svec, left);
     }
-    if constexpr (MASTER) store4(t.master + i, pq, mvec, left);
+    if constexpr (MASTER) store4(master + i, pq, mvec, left);
     store4(p + i, pq, pvec, left);
   }
 }
 
 template <typename P, bool MASTER, bool Q8>
-int launch(const Table& tab, hipStream_t s) {
-  hipLaunchKernelGGL((adamw_kernel<P, MASTER, Q8>), dim3((unsigned)tab.end[tab.count - 1]), dim3(kThreads), 0, s, tab);
-  MHC_CHECK_LAUNCH("adamw_kernel");
-  return MHC_OK;
+int launch(const mhc_adamw_tensor* tensors, int64_t count, const Hyper& h, hipStream_t s) {
+  Table<MASTER, Q8> tab;
+  const auto run = [&] {
+    hipLaunchKernelGGL((adamw_kernel<P, MASTER, Q8>), dim3((unsigned)tab.end[tab.count - 1]), dim3(kThreads), 0, s, tab);
+    MHC_CHECK_LAUNCH("adamw_kernel");
+    return MHC_OK;
+  };
+  tab.h = h;
+  tab.count = 0;
+  int64_t total = 0;
+  for (int64_t i = 0; i < count; ++i) total += tensors[i].numel;
+  tab.chunk = total < (int64_t)device_cu_count() * 8 * kChunk ? kPass : kChunk;
+  int64_t chunks = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    const mhc_adamw_tensor& t = tensors[i];
+    if (t.numel == 0) continue;
+    const int64_t mine = ceil_div(t.numel, tab.chunk);
+    if (tab.count == Table<MASTER, Q8>::kMax || (tab.count > 0 && chunks + mine > kMaxChunks)) {
+      if (const int rc = run()) return rc;
+      tab.count = 0;
+      chunks = 0;
+    }
+    chunks += mine;
+    void** const p = tab.p[tab.count];
+    p[0] = t.param, p[1] = const_cast<void*>(t.grad), p[2] = t.exp_avg, p[3] = t.exp_avg_sq;
+    if constexpr (MASTER) p[4] = t.master;
+    if constexpr (Q8) p[4 + MASTER] = t.scales;
+    tab.end[tab.count] = (int32_t)chunks;
+    tab.last[tab.count] = (int32_t)(t.numel - (mine - 1) * tab.chunk);
+    ++tab.count;
+  }
+  return tab.count > 0 ? run() : MHC_OK;
 }
 
 template <typename P>
-int launch_for(const Table& tab, bool master, bool q8, hipStream_t s) {
+int launch_for(const mhc_adamw_tensor* tensors, int64_t count, const Hyper& h, bool master, bool q8, hipStream_t s) {
   if constexpr (sizeof(P) == 2) {
-    if (master) return q8 ? launch<P, true, true>(tab, s) : launch<P, true, false>(tab, s);
+    if (master) return q8 ? launch<P, true, true>(tensors, count, h, s) : launch<P, true, false>(tensors, count, h, s);
   }
-  return q8 ? launch<P, false, true>(tab, s) : launch<P, false, false>(tab, s);
-}
-
-int launch_table(const Table& tab, int dtype, bool master, bool q8, hipStream_t s) {
-  if (dtype == kF32) return launch_for<float>(tab, master, q8, s);
-  if (dtype == kBF16) return launch_for<__bf16>(tab, master, q8, s);
-  return launch_for<_Float16>(tab, master, q8, s);
+  return q8 ? launch<P, false, true>(tensors, count, h, s) : launch<P, false, false>(tensors, count, h, s);
 }
 
 }  // namespace
@@ -245,29 +285,12 @@ extern "C" int mhc_adamw_step(const mhc_adamw_tensor* tensors, int64_t count, in
     MHC_CHECK_ARG(t.numel <= kMaxChunks * kChunk, "tensor %lld: numel %lld is too large", (long long)i,
                   (long long)t.numel);
   }
-  Table tab;
   const double bc1 = 1.0 - std::pow(beta1, (double)step), bc2 = 1.0 - std::pow(beta2, (double)step);
-  tab.h = Hyper{(float)(1.0 - lr * weight_decay), (float)beta1, (float)(1.0 - beta1), (float)beta2,
-                (float)(1.0 - beta2),             (float)(1.0 / std::sqrt(bc2)), (float)eps, (float)(lr / bc1),
-                (float)grad_scale,                grad_scale_ptr};
-  tab.count = 0;
-  int64_t total = 0;
-  for (int64_t i = 0; i < count; ++i) total += tensors[i].numel;
-  tab.chunk = total < (int64_t)device_cu_count() * 8 * kChunk ? kPass : kChunk;
+  const Hyper h = {(float)(1.0 - lr * weight_decay), (float)beta1, (float)(1.0 - beta1), (float)beta2,
+                   (float)(1.0 - beta2),             (float)(1.0 / std::sqrt(bc2)), (float)eps, (float)(lr / bc1),
+                   (float)grad_scale,                grad_scale_ptr};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  int64_t chunks = 0;
-  for (int64_t i = 0; i < count; ++i) {
-    if (tensors[i].numel == 0) continue;
-    const int64_t mine = ceil_div(tensors[i].numel, tab.chunk);
-    if (tab.count == kMaxTensors || (tab.count > 0 && chunks + mine > kMaxChunks)) {
-      if (const int rc = launch_table(tab, dtype, master, q8, s)) return rc;
-      tab.count = 0;
-      chunks = 0;
-    }
-    chunks += mine;
-    tab.t[tab.count] = tensors[i];
-    tab.end[tab.count] = (int32_t)chunks;
-    ++tab.count;
-  }
-  return tab.count > 0 ? launch_table(tab, dtype, master, q8, s) : MHC_OK;
+  if (dtype == kF32) return launch_for<float>(tensors, count, h, master, q8, s);
+  if (dtype == kBF16) return launch_for<__bf16>(tensors, count, h, master, q8, s);
+  return launch_for<_Float16>(tensors, count, h, master, q8, s);
 }

@@ -311,3 +311,15 @@ def test_refusals():
         with pytest.raises(ValueError):
             step(**bad)
     adamw_step_hip([], [], [], [], step=1)
+
+
+@pytest.mark.parametrize("count", [63, 64, 65, 72, 73, 84, 85, 100, 101, 128, 129, 201])
+@pytest.mark.parametrize("dt,bits,master", [("f32", 32, False), ("f32", 8, False), ("bf16", 32, True), ("f16", 8, True)])
+def test_lists_around_the_length_of_a_launch(count, dt, bits, master):
+    """Tensors of one and of several workgroups, in numbers at which a launch's table or a vote ends."""
+    shapes = [((5, 1024, 1025, 300, 2048)[i % 5],) for i in range(count)]
+    a = _lists(shapes, dt, bits, master, 7)
+    b = _clone(a, "cpu")
+    adamw_step_hip(**a, **HYPER)
+    adamw_step_reference(**b, **HYPER)
+    _same(a, b)
