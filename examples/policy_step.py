@@ -62,7 +62,9 @@ def train(steps: int = 20, tokens: int = 2048, vocab: int = 512, width: int = 25
             old, ref = logp_of(logits, actions), logp_of(first(state), actions)
             reward = (actions == target).float()
             sampled = (torch.softmax(logits.float(), -1).gather(1, target[:, None])).mean()  # chance of the rewarded action
-            mask = torch.rand(tokens, device="cuda") < 0.9  # (the others stand for padding)
+            # some stand for padding; an imposed action that the policy all but excludes would be nearly all of the KL
+            # term, whose estimate exp(ref - lp) takes actions to be the policy's own
+            mask = (torch.rand(tokens, device="cuda") < 0.9) & (old > -10.0)
         for _ in range(2):  # two passes over the same actions: the second is off the acting policy, and clipped
             opt.zero_grad(set_to_none=True)
             loss, _ = policy_loss(model(state), actions, old, reward - reward.mean(), ref_logp=ref, mask=mask, kl_coef=0.001)
