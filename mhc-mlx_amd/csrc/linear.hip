@@ -155,8 +155,8 @@ BwdPlan plan_bwd(const void* dout, int dout_dtype, bool dact, const void* x, int
   if (dx) b.w = pack_bytes(w, N, ldw, K, dtype);
   if (dw) b.x = pack_bytes(x, M, ldx, K, dtype);
   if (dx && dw) b.cut = gemm::pair_of(M, N, K, dtype);
-  else if (dx) b.cut.dx = gemm::cut_of(M, K, N, dtype);
-  else if (dw) b.cut.dw = gemm::cut_of(N, K, M, dtype);
+  else if (dx) b.cut.dx = gemm::cut_of(M, K, N, dtype, true, false);
+  else if (dw) b.cut.dw = gemm::cut_of(N, K, M, dtype, false, false);
   const size_t of_dx = dx ? part_bytes(b.cut.dx, M, K) : 0, of_dw = dw ? part_bytes(b.cut.dw, N, K) : 0;
   b.total = b.dz + b.part + b.x + b.w + (b.cut.together ? of_dx + of_dw : std::max(of_dx, of_dw));
   return b;
@@ -192,7 +192,7 @@ extern "C" size_t mhc_linear_act_fwd_workspace_bytes(const void* x, int64_t ldx,
                                                      int64_t N, int64_t K, int dtype) {
   if (M <= 0 || N <= 0 || K <= 0 || mhc::gemm::few_rows(x, ldx, w, ldw, M, N, K, dtype)) return 0;
   return mhc::pack_bytes(x, M, ldx, K, dtype) + mhc::pack_bytes(w, N, ldw, K, dtype) +
-         mhc::part_bytes(mhc::gemm::cut_of(M, N, K, dtype), M, N);
+         mhc::part_bytes(mhc::gemm::cut_of(M, N, K, dtype, true, true), M, N);
 }
 
 extern "C" int mhc_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
@@ -221,7 +221,7 @@ extern "C" int mhc_linear_act_fwd(const void* x, int64_t ldx, const void* w, int
   Product p = {{}, {}, M, N, K, gemm::Epilogue{bias, residual, out, dact, act, out_dtype == kF32}, 1, 0};
   if (const int rc = operand(p.a, x, M, ldx, K, dtype, ws, s)) return rc;
   if (const int rc = operand(p.b, w, N, ldw, K, dtype, ws, s)) return rc;
-  return run_product(p, true, true, gemm::cut_of(M, N, K, dtype), dtype, ws, s);
+  return run_product(p, true, true, gemm::cut_of(M, N, K, dtype, true, true), dtype, ws, s);
 }
 
 extern "C" size_t mhc_linear_act_bwd_workspace_bytes(const void* dout, int dout_dtype, const void* dact, const void* x,

@@ -260,7 +260,9 @@ struct Operand {
   int64_t ld, width;
 };
 
-constexpr int64_t kMaxRowBytes = 1 << 23;  // between rows: 256 of them stay below 2^31
+// Offsets inside a tile, of up to 256 rows, stay below 2^31: rows are at most
+// this far apart, or the tile has half as many of them (most_rows).
+constexpr int64_t kMaxRowBytes = 1 << 23;
 
 // Whether rows of `width` elements, `ld` apart, can be an Operand as they are.
 inline bool in_words(const void* p, int64_t ld, int64_t width, int bytes) {
@@ -357,7 +359,7 @@ struct Loader {
 
   // the stage at base; kleft: k from it to the end
   MHC_DEV void load(uint32_t stage, int kleft, int lane) const {
-    // (offsets of the tile stay below 2^31, see kMaxRowBytes)
+    // (offsets of the tile stay below 2^31, see kMaxRowBytes and most_rows)
     const uint32_t n = left <= 0 ? 0u : left > 0x80000000ll ? 0x80000000u : (uint32_t)left;
     const u32x4 rs = {(uint32_t)base, (uint32_t)(base >> 32) & 0xffffu, n, 0x00020000u};
 #pragma unroll
@@ -1088,16 +1090,22 @@ inline float join_us(int splits, int64_t M, int64_t N) {  // a launch, and 8 byt
   return splits > 1 ? 4.f + 2.f * splits * (float)M * (float)N / 1e6f : 0.f;
 }
 
+// Rows that a tile may have of an operand.  A k-major one whose rows are longer
+// than kMaxRowBytes has been copied to rows of whole chunks; they are at most
+// 2^24 bytes long (K < 2^22), and 128 of them stay below 2^31.
+inline int most_rows(bool k_major, int64_t K, int dtype) { return k_major && K * (dtype == kF32 ? 4 : 2) > kMaxRowBytes ? 128 : 256; }
+
 // The cut with the least estimated time.  Large tiles read least, small ones
 // give every CU work; a reduction is split where even those are too few,
 // which costs a launch and its sums' way through memory.
-inline Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype) {
+inline Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool a_k, bool b_k) {
   const int kK = dtype == kF32 ? 32 : 64;
   const int stages = (int)ceil_div(K, kK);
   const float cus = (float)device_cu_count();
   Cut best = {0, 1, stages * kK, 0.f};
   for (int t = 0; t < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++t) {
     const TileCost& c = kTiles[t];
+    if (c.bm > most_rows(a_k, K, dtype) || c.bn > most_rows(b_k, K, dtype)) continue;
     const float tiles = (float)ceil_div(M, c.bm) * (float)ceil_div(N, c.bn);
     for (int want = 1; want <= 16; ++want) {
       if (want > 1 && (tiles * (want - 1) > 4.f * cus || stages < 2 * want)) break;
@@ -1118,13 +1126,13 @@ struct PairCut {
 };
 
 inline PairCut pair_of(int64_t M, int64_t N, int64_t K, int dtype) {
-  PairCut best = {false, cut_of(M, K, N, dtype), cut_of(N, K, M, dtype)};
+  PairCut best = {false, cut_of(M, K, N, dtype, true, false), cut_of(N, K, M, dtype, false, false)};
   float least = best.dx.us + best.dw.us;
   const float cus = (float)device_cu_count();
   const int kK = dtype == kF32 ? 32 : 64;
   const int stages1 = (int)ceil_div(N, kK), stages2 = (int)ceil_div(M, kK);
   constexpr int kWant[] = {1, 2, 3, 4, 6, 8};
-  for (int t = 2; t < 5; ++t) {
+  for (int t = 2; t < 5; ++t) {  // (at most 128 rows: see most_rows)
     const TileCost& c = kTiles[t];
     const float tiles1 = (float)ceil_div(M, c.bm) * (float)ceil_div(K, c.bn), tiles2 = (float)ceil_div(N, c.bm) * (float)ceil_div(K, c.bn);
     if (tiles1 + tiles2 > 16.f * cus) continue;  // (each fills the card)
@@ -1164,7 +1172,7 @@ inline bool few_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, int
   const float few = 3.f + of_cu * (float)ceil_div(K * bytes, 128 * kFewWaves) * stage * (words ? 1.f : 1.8f);
   // (tiles need copies of rows that are no whole words: two launches and the operands' way out and in)
   const float copies = words ? 0.f : 9.f + 2.f * (float)((M + N) * K * bytes) / 4e6f;
-  return few <= cut_of(M, N, K, dtype).us + copies;
+  return few <= cut_of(M, N, K, dtype, true, true).us + copies;
 }
 
 template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>

@@ -1,0 +1,34 @@
+"""linear_act / FusedLinear at the ends of what they take: very long rows, many rows, tiny values, mixed types."""
+
+import pytest
+import torch
+
+from tests._train import close, linear64, linear_grads64
+
+from mhc_mlx_amd import linear_act
+
+pytestmark = pytest.mark.gpu
+
+
+def test_rows_of_more_than_8_megabytes():
+    """fp32 reductions past 2^21 elements, forward and in dx, at sizes that large tiles would serve best.
+
+    The values are positive, so that a sum that lacks a part of its terms is far outside the bound.
+    """
+    M, N, K = 1024, 1024, 2_200_000
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x, w = (torch.rand(n, K, generator=g, device="cuda") for n in (M, N))
+    rows = torch.tensor([0, 127, 128, 190, 255, 256, 447, 1023], device="cuda")  # first, middle and last ones of tiles
+    out = linear_act(x, w)
+    ref, bound, *_ = linear64(x[rows], w[rows], None, None, "none", torch.float32)
+    close(out[rows][:, rows], ref, bound, "out")
+    del out
+    # dx [1024, 1024] = dout [1024, K] W [K, 1024]
+    wide = w.view(K, N)
+    a = torch.rand(M, N, generator=g, device="cuda").requires_grad_(True)
+    dx, = torch.autograd.grad(linear_act(a, wide), a, x)
+    del w
+    some = wide[:, rows]
+    ones = torch.ones(len(rows), K, dtype=torch.float64, device="cuda")
+    (ref, bound), _, _ = linear_grads64(a[rows][:, rows], some, x[rows], ones, torch.zeros_like(ones), torch.float32, False)
+    close(dx[rows][:, rows], ref, bound, "dx")
