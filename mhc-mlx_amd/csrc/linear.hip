@@ -49,10 +49,11 @@ MHC_DEV void dz_columns(const G* dout, const typename gemm::DactOf<T>::Type* d, 
 
 template <typename T, typename G>
 __global__ __launch_bounds__(256) void dz_kernel(const G* dout, const void* dact, T* dz, int64_t ld, float* part, int64_t M,
-                                                 int64_t N, int rows) {
+                                                 int64_t N, int rows, uint32_t wide) {
   __shared__ float lds[4][kDzCols];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int64_t n0 = (int64_t)blockIdx.x * kDzCols, n = n0 + lane * 8, m0 = (int64_t)blockIdx.y * rows, m1 = min(m0 + rows, M);
+  const uint32_t block = blockIdx.x / wide;  // of rows; `wide` workgroups have its columns
+  const int64_t n0 = (int64_t)(blockIdx.x % wide) * kDzCols, n = n0 + lane * 8, m0 = (int64_t)block * rows, m1 = min(m0 + rows, M);
   const auto* const d = static_cast<const typename gemm::DactOf<T>::Type*>(dact);
   float sum[8] = {};
   if (n + 8 <= N) dz_columns<T, G, true>(dout, d, dz, ld, m0 + wave, m1, n, N, 8, sum);
@@ -62,7 +63,7 @@ __global__ __launch_bounds__(256) void dz_kernel(const G* dout, const void* dact
   for (int k = 0; k < 8; ++k) lds[wave][lane * 8 + k] = sum[k];
   __syncthreads();
   for (int c = threadIdx.x; c < kDzCols; c += 256)
-    if (n0 + c < N) part[(int64_t)blockIdx.y * N + n0 + c] = (lds[0][c] + lds[1][c]) + (lds[2][c] + lds[3][c]);
+    if (n0 + c < N) part[(int64_t)block * N + n0 + c] = (lds[0][c] + lds[1][c]) + (lds[2][c] + lds[3][c]);
 }
 
 // db[n] = sum over the blocks of rows
@@ -166,8 +167,9 @@ template <typename T, typename G>
 int run_dz(const void* dout, const void* dact, void* dz, int64_t ld, float* part, void* db, int64_t M, int64_t N, hipStream_t s) {
   const int rows = dz_rows(M, N);
   const int64_t blocks = ceil_div(M, rows);
-  const dim3 grid((unsigned)ceil_div(N, kDzCols), (unsigned)blocks);
-  hipLaunchKernelGGL((dz_kernel<T, G>), grid, dim3(256), 0, s, static_cast<const G*>(dout), dact, static_cast<T*>(dz), ld, part, M, N, rows);
+  const uint32_t wide = (uint32_t)ceil_div(N, kDzCols);
+  hipLaunchKernelGGL((dz_kernel<T, G>), dim3(wide * (uint32_t)blocks), dim3(256), 0, s, static_cast<const G*>(dout), dact,
+                     static_cast<T*>(dz), ld, part, M, N, rows, wide);
   MHC_CHECK_LAUNCH("dz_kernel");
   if (db != nullptr) {
     hipLaunchKernelGGL((db_kernel<T>), dim3((unsigned)ceil_div(N, gemm::kSumCols)), dim3(256), 0, s, (const float*)part,
@@ -180,7 +182,9 @@ int run_dz(const void* dout, const void* dact, void* dz, int64_t ld, float* part
 int check_shape(int64_t M, int64_t N, int64_t K, int dtype) {
   MHC_CHECK_ARG(M >= 0 && N >= 1 && K >= 1, "M must be >= 0, N and K >= 1 (got %lld, %lld, %lld)", (long long)M,
                 (long long)N, (long long)K);
-  MHC_CHECK_ARG(M < ((int64_t)1 << 22) && N < ((int64_t)1 << 22) && K < ((int64_t)1 << 22), "M, N and K must be below 2^22");
+  // (M: the reduction of dW is counted in 32 bits, and a launch has fewer than 2^32 threads; N and K: see gemm::most_rows)
+  MHC_CHECK_ARG(M < ((int64_t)1 << 28) && N < ((int64_t)1 << 22) && K < ((int64_t)1 << 22),
+                "M must be below 2^28, N and K below 2^22 (got %lld, %lld, %lld)", (long long)M, (long long)N, (long long)K);
   MHC_CHECK_ARG(dtype == kF32 || dtype == kBF16 || dtype == kF16, "unsupported dtype %d", dtype);
   return MHC_OK;
 }

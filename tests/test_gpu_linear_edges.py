@@ -32,3 +32,19 @@ def test_rows_of_more_than_8_megabytes():
     ones = torch.ones(len(rows), K, dtype=torch.float64, device="cuda")
     (ref, bound), _, _ = linear_grads64(a[rows][:, rows], some, x[rows], ones, torch.zeros_like(ones), torch.float32, False)
     close(dx[rows][:, rows], ref, bound, "dx")
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_more_than_2_22_rows(dt):
+    """Zeros and ones, so that every sum over the rows is a whole number below 2^24: exact in fp32."""
+    M, N, K = (1 << 22) + 70, 24, 16
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x, w, up = (torch.randint(0, 2, s, generator=g, device="cuda").to(dt) for s in ((M, K), (N, K), (M, N)))
+    b = torch.ones(N, device="cuda", dtype=dt)
+    ts = [t.requires_grad_(True) for t in (x, w, b)]
+    out = linear_act(*ts, activation="relu")
+    xd, wd, ud = (t.detach().double() for t in (x, w, up))
+    assert torch.equal(out, (xd @ wd.t() + 1).to(dt))
+    dx, dw, db = torch.autograd.grad(out, ts, up)  # (every sum is positive: relu's derivative is 1)
+    assert torch.equal(dx, (ud @ wd).to(dt)) and torch.equal(dw, (ud.t() @ xd).to(dt))
+    assert torch.equal(db, (torch.ones(1, M, dtype=torch.float64, device="cuda") @ ud)[0].to(dt))
