@@ -8,8 +8,9 @@ residual) of that dtype or float32.  Sums are held in fp32.  The backward gives 
 residual; dz = dout act'(z) is rounded once to x's dtype as an operand of the two products (the bias's gradient is
 summed from it unrounded).  It is not twice differentiable.
 
-linear_act needs GPU tensors and the built library; FusedLinear hands a call that the HIP path cannot take (CPU
-tensors, a RuntimeError from the library) to ``linear_act_reference``, with one warning per process, as MHCLayer does.
+linear_act needs GPU tensors and the built library, fewer than 2^28 rows, and N and K below 2^22; FusedLinear hands a call
+that the HIP path cannot take (CPU tensors, a wider layer, a RuntimeError from the library) to ``linear_act_reference``,
+with one warning per process, as MHCLayer does.
 """
 
 from __future__ import annotations
@@ -26,6 +27,9 @@ __all__ = ["ACTIVATIONS", "FusedLinear", "linear_act", "linear_act_reference"]
 
 ACTIVATIONS = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "gelu": _lib.ACT_GELU, "gelu_tanh": _lib.ACT_GELU_TANH,
                "silu": _lib.ACT_SILU}
+
+
+_MAX_WIDTH = 1 << 22  # N and K stay below it
 
 
 def _act_code(activation: str) -> int:
@@ -110,6 +114,8 @@ class FusedLinear(nn.Linear):
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
         if not layer._disabled_by_env() and layer.hip_available():
             why = layer._off_gpu(x, self.weight, self.bias, residual)
+            if max(self.in_features, self.out_features) >= _MAX_WIDTH:
+                why = f"the HIP path needs N and K below {_MAX_WIDTH} (got {self.out_features} and {self.in_features})"
             if why is None:
                 try:
                     return linear_act(x, self.weight, self.bias, residual, self.activation, self.return_dtype)

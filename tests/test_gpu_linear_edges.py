@@ -5,7 +5,8 @@ import torch
 
 from tests._train import close, linear64, linear_grads64
 
-from mhc_mlx_amd import linear_act
+from mhc_mlx_amd import FusedLinear, linear_act
+from mhc_mlx_amd import layer as L
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +49,15 @@ def test_more_than_2_22_rows(dt):
     dx, dw, db = torch.autograd.grad(out, ts, up)  # (every sum is positive: relu's derivative is 1)
     assert torch.equal(dx, (ud @ wd).to(dt)) and torch.equal(dw, (ud.t() @ xd).to(dt))
     assert torch.equal(db, (torch.ones(1, M, dtype=torch.float64, device="cuda") @ ud)[0].to(dt))
+
+
+def test_wider_layers_than_the_kernels_take(monkeypatch):
+    """linear_act refuses them, FusedLinear computes them in the plain form."""
+    monkeypatch.setattr(L, "_METAL_FAILED", True)  # (the warning has been given)
+    for N, K in ((2, 1 << 22), (1 << 22, 2)):
+        m = FusedLinear(K, N, device="cuda")
+        x = torch.randn(3, K, device="cuda")
+        with pytest.raises(ValueError, match="2\\^22"):
+            linear_act(x, m.weight, m.bias)
+        ref, bound, *_ = linear64(x, m.weight, m.bias, None, "none", torch.float32)
+        close(m(x), ref, bound, "out")
