@@ -11,10 +11,14 @@ summed from it unrounded).  It is not twice differentiable.
 linear_act needs GPU tensors and the built library, fewer than 2^28 rows, and N and K below 2^22; FusedLinear hands a call
 that the HIP path cannot take (CPU tensors, a wider layer, a RuntimeError from the library) to ``linear_act_reference``,
 with one warning per process, as MHCLayer does.
+
+Under torch.autocast FusedLinear casts x, weight and bias to the autocast dtype, as nn.Linear does; linear_act takes its
+arguments as they are.
 """
 
 from __future__ import annotations
 
+import contextlib
 import math
 
 import torch
@@ -37,6 +41,11 @@ def _act_code(activation: str) -> int:
         return ACTIVATIONS[activation]
     except (KeyError, TypeError):
         raise ValueError(f"activation must be one of: {', '.join(ACTIVATIONS)} (got {activation!r})") from None
+
+
+def _autocast_dtype(x: torch.Tensor) -> torch.dtype | None:
+    device = x.device.type
+    return torch.get_autocast_dtype(device) if device in ("cuda", "cpu") and torch.is_autocast_enabled(device) else None
 
 
 class LinearActFn(torch.autograd.Function):
@@ -81,7 +90,8 @@ def linear_act_reference(x, weight, bias=None, residual=None, activation: str = 
     """linear_act in elementary torch operations (fp32 for half inputs, else the inputs' dtype), on any device."""
     _act_code(activation)
     up = torch.float64 if x.dtype == torch.float64 else torch.float32
-    z = torch.matmul(x.to(up), weight.to(up).t())
+    with torch.autocast(x.device.type, enabled=False) if _autocast_dtype(x) else contextlib.nullcontext():
+        z = torch.matmul(x.to(up), weight.to(up).t())
     if bias is not None:
         z = z + bias.to(up)
     if activation == "relu":
@@ -101,7 +111,8 @@ class FusedLinear(nn.Linear):
     """nn.Linear with an activation, and an optional residual of its output's shape, in the product's epilogue.
 
     ``return_dtype`` (torch.float32, or None for x's dtype) is the output's dtype.  Parameters, their names and their
-    initialisation are nn.Linear's, so checkpoints carry over and AutoPatcher wraps it like one.
+    initialisation are nn.Linear's, so checkpoints carry over and AutoPatcher wraps it like one.  Under autocast x's dtype
+    is the autocast one, and a float32 residual makes the output float32, as adding it would.
     """
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, activation: str = "none", *,
@@ -112,17 +123,24 @@ class FusedLinear(nn.Linear):
         self.return_dtype = return_dtype
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        weight, bias, return_dtype = self.weight, self.bias, self.return_dtype
+        cast = _autocast_dtype(x)
+        if cast is not None and x.dtype != torch.float64:  # (autocast leaves float64 alone)
+            x, weight, bias = x.to(cast), weight.to(cast), None if bias is None else bias.to(cast)
+            if residual is not None:
+                return_dtype = return_dtype or (torch.float32 if residual.dtype == torch.float32 else cast)
+                residual = residual.to(return_dtype)
         if not layer._disabled_by_env() and layer.hip_available():
-            why = layer._off_gpu(x, self.weight, self.bias, residual)
+            why = layer._off_gpu(x, weight, bias, residual)
             if max(self.in_features, self.out_features) >= _MAX_WIDTH:
                 why = f"the HIP path needs N and K below {_MAX_WIDTH} (got {self.out_features} and {self.in_features})"
             if why is None:
                 try:
-                    return linear_act(x, self.weight, self.bias, residual, self.activation, self.return_dtype)
+                    return linear_act(x, weight, bias, residual, self.activation, return_dtype)
                 except RuntimeError as e:
                     why = e
             layer._fallback_warning(" in FusedLinear", why)
-        return linear_act_reference(x, self.weight, self.bias, residual, self.activation, self.return_dtype)
+        return linear_act_reference(x, weight, bias, residual, self.activation, return_dtype)
 
     def extra_repr(self) -> str:
         return f"{super().extra_repr()}, activation={self.activation}"

@@ -61,3 +61,24 @@ def test_wider_layers_than_the_kernels_take(monkeypatch):
             linear_act(x, m.weight, m.bias)
         ref, bound, *_ = linear64(x, m.weight, m.bias, None, "none", torch.float32)
         close(m(x), ref, bound, "out")
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("given", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [5, 200])
+def test_fused_linear_under_autocast(dt, given, rows):
+    """The call and its gradients are those of the operands in the autocast dtype; parameters get float32 gradients."""
+    m = FusedLinear(72, 136, activation="gelu", device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.randn(rows, 72, generator=g, device="cuda").to(given).requires_grad_(True)
+    r = torch.randn(rows, 136, generator=g, device="cuda", requires_grad=True)
+    low = [t.detach().to(dt).requires_grad_(True) for t in (x, m.weight, m.bias)]
+    for residual, out_dtype in ((None, dt), (r, torch.float32), (r.detach().to(dt), dt)):
+        with torch.autocast("cuda", dt):
+            out = m(x, residual)
+        want = linear_act(*low, residual, activation="gelu", output_dtype=out_dtype)
+        assert out.dtype == out_dtype and torch.equal(out, want)
+        up = torch.randn(out.shape, generator=g, device="cuda").to(out_dtype)
+        grads = torch.autograd.grad(out, (x, m.weight, m.bias), up)
+        for got, ref, t in zip(grads, torch.autograd.grad(want, low, up), (x, m.weight, m.bias)):
+            assert got.dtype == t.dtype and torch.equal(got, ref.to(t.dtype))

@@ -61,6 +61,27 @@ def test_fused_linear_falls_back_on_the_cpu(monkeypatch):
         FusedLinear(8, 6, activation="swish")
 
 
+def test_fused_linear_under_autocast_on_the_cpu(monkeypatch):
+    """As nn.Linear: operands in the autocast dtype, whatever x's; a float32 residual keeps its precision."""
+    monkeypatch.setattr(L, "_METAL_FAILED", True)
+    m = FusedLinear(32, 24)
+    plain = torch.nn.Linear(32, 24)
+    plain.load_state_dict(m.state_dict())
+    r = torch.randn(5, 24)
+    for x in (torch.randn(5, 32), torch.randn(5, 32).to(torch.bfloat16)):
+        with torch.autocast("cpu", torch.bfloat16):
+            y, z, with_r = m(x), plain(x), m(x, r)
+        assert y.dtype == z.dtype == torch.bfloat16 and with_r.dtype == torch.float32
+        low = [t.detach().to(torch.bfloat16).double() for t in (x, m.weight, m.bias)]
+        exact = low[0] @ low[1].t() + low[2]
+        assert bool(((y.double() - exact).abs() <= 2.0 ** -8 * exact.abs() + 1e-5).all())  # one rounding to bf16
+        assert bool(((with_r.double() - exact - r).abs() <= 1e-5).all())  # fp32 sums of 32 products of size 1
+        y.float().sum().backward()
+        assert m.weight.grad.dtype == torch.float32
+    with torch.autocast("cpu", torch.bfloat16):
+        assert linear_act_reference(x.float(), m.weight).dtype == torch.float32
+
+
 def test_operators_never_fall_back():
     x = torch.randn(3, 8)
     if not _lib.LIB_PATH.exists():
