@@ -504,12 +504,28 @@ MHC_DEV void store_rows(const Epilogue& e, const char* sums, int lane, int64_t m
   else if (left > 0) store_columns<T, ROWS, false>(e, sums, lane, m0, M, n0, N, left);
 }
 
+// The same for those of the sums that are not kKeep, one by one: rarely used, so it is short.
+constexpr uint32_t kKeep = 0x7fc5a5a5u;  // (a NaN: a sum that comes to it by itself is NaN in the outputs already)
+
+template <typename T, int ROWS>
+MHC_DEV void store_some(const Epilogue& e, const char* sums, int lane, int64_t m0, int64_t M, int64_t n0, int64_t N) {
+  if (n0 + lane >= N) return;
+  float bias[1];
+  bias_of<T>(e, n0 + lane, 1, bias);
+  for (int r = 0; r < ROWS && m0 + r < M; ++r) {
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(sums + r * 256 + (((lane / 4) ^ (r % 16)) << 4) + lane % 4 * 4);
+    if (u == kKeep) continue;
+    float z[1][1] = {{__builtin_bit_cast(float, u)}}, residual[1][1];
+    residual_of<T, true>(e, m0 + r, 0, M, n0 + lane, N, 1, residual);
+    finish<T, true>(e, m0 + r, 0, M, n0 + lane, N, 1, z, bias, residual);
+  }
+}
+
 // A wave's JM x JN sums of 16 x 16, in registers, to the outputs from (m0, n0)
-// on, through the workgroup's LDS (BYTES of it, free).
-template <typename T, int JM, int JN, int WAVES, int BYTES>
-MHC_DEV void store_tile(const Product& p, char* smem, const f32x4 (&acc)[JN][JM], int64_t m0, int64_t n0, int wave, int lane, int split) {
-  Epilogue e = p.e;
-  if (p.splits > 1) e.out = static_cast<float*>(e.out) + (int64_t)split * p.M * p.N;
+// on, through the workgroup's LDS (BYTES of it, free).  SOME: those that are not kKeep.
+template <typename T, int JM, int JN, int WAVES, int BYTES, bool SOME = false>
+MHC_DEV void store_tile(const Epilogue& e, char* smem, const f32x4 (&acc)[JN][JM], int64_t m0, int64_t M, int64_t n0, int64_t N, int wave,
+                        int lane) {
   // The sums go through LDS, where each wave has room for up to 64 rows
   // of 64 columns, so that rows of the outputs are written as whole vectors of
   // consecutive lanes.  The 16-byte chunk c of row r is at c ^ (r % 16).
@@ -530,7 +546,8 @@ MHC_DEV void store_tile(const Product& p, char* smem, const f32x4 (&acc)[JN][JM]
         *reinterpret_cast<f32x4*>(mine + (j * 16 + at % 16) * 256 + (((i * 4 + at / 16) ^ (at % 16)) << 4)) = acc[i][h + j];
     __syncthreads();
     const int64_t mh = m0 + h * 16;
-    store_rows<T, kRows>(e, mine, at, mh, p.M, n0, p.N);
+    if constexpr (SOME) store_some<T, kRows>(e, mine, at, mh, M, n0, N);
+    else store_rows<T, kRows>(e, mine, at, mh, M, n0, N);
   };
   static_assert(JM / kRound <= 2, "two rounds");
   round(std::integral_constant<int, 0>{});
@@ -731,52 +748,108 @@ MHC_DEV void sum_tile_split(const Product& p, const Place<BM, BN, WM, WN>& at, c
 // The kernels of tiles
 // --------------------------------------------------------------------------
 
-// A tile of outputs, or (split) of one part of the reduction's sums.  fp32
-// tiles of at least 64 x 128 are summed on the bf16 instructions (1000 x 1100 x
-// 1536 in 128 x 128 107 us in fp32, 89 so; 8192 x 4096 x 4096 in 256 x 256
-// 1889 and 1180, where the library's fp32 product takes 1800; 64 x 64 have
-// too few products for each value that is split: 512 x 2048 x 2048 43 and 56),
-// and one with a NaN once more with fp32 instructions: they tell what an
-// infinity makes of it, whose parts make NaN of everything.
+// fp32 tiles of at least 64 x 128 are summed on the bf16 instructions (1000 x
+// 1100 x 1536 in 128 x 128 107 us in fp32, 89 so; 8192 x 4096 x 4096 in 256 x
+// 256 1889 and 1180, where the library's fp32 product takes 1800; 64 x 64 have
+// too few products for each value that is split: 512 x 2048 x 2048 43 and 56).
+template <typename T, int BN>
+constexpr bool kSplit = sizeof(T) == 4 && BN > 64;
+
+// LDS of a workgroup: its stages and, for sums on split values, a bit for each
+// sum of a thread, in words, and one word for each wave.
+template <typename T, int BM, int BN, int WM, int WN, int NS>
+struct TileBytes {
+  static constexpr int kStages = NS * (BM + BN) * 128, kThreads = 64 * WM * WN, kWords = BM * BN / kThreads / 32;
+  static constexpr int kAll = kStages + (kSplit<T, BN> ? (kWords * kThreads + WM * WN) * 4 : 0);
+};
+
+// A tile of outputs, or (split) of one part of the reduction's sums.  Sums on
+// split values that come out as NaN are formed once more with fp32
+// instructions: they tell what an infinity makes of a sum, whose parts make NaN
+// of everything.  The other sums of the tile stay as they are, so that a row's
+// outputs do not depend on what other rows hold.
 template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
 MHC_DEV void run_tile(const Product& p, char* smem, uint32_t tile, int split) {
-  constexpr int kBytes = NS * (BM + BN) * 128, JM = BM / WM / 16, JN = BN / WN / 16;
+  using B = TileBytes<T, BM, BN, WM, WN, NS>;
+  constexpr int kWaves = WM * WN, JM = BM / WM / 16, JN = BN / WN / 16;
   const Place<BM, BN, WM, WN> at(p, tile, split);
+  const int64_t m0 = at.m0 + at.wm, n0 = at.n0 + at.wn;
+  Epilogue e = p.e;
+  if (p.splits > 1) e.out = static_cast<float*>(e.out) + (int64_t)split * p.M * p.N;
   f32x4 acc[JN][JM] = {};
-  if constexpr (sizeof(T) == 4 && BN > 64) {
+  if constexpr (!kSplit<T, BN>) {
+    sum_tile<T, AK, BK, BM, BN, WM, WN, NS>(p, at, smem, acc);
+    store_tile<T, JM, JN, kWaves, B::kStages>(e, smem, acc, m0, p.M, n0, p.N, at.wave, at.lane);
+  } else {
+    static_assert(B::kWords * 32 == JM * JN * 4);
     sum_tile_split<AK, BK, BM, BN, WM, WN, NS>(p, at, smem, acc);
+    uint32_t* const marks = reinterpret_cast<uint32_t*>(smem + B::kStages);
+    uint32_t* const found = marks + B::kWords * B::kThreads;
     bool nan = false;
 #pragma unroll
     for (int i = 0; i < JN; ++i)
 #pragma unroll
       for (int j = 0; j < JM; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) nan |= acc[i][j][e] != acc[i][j][e];
-    int* const found = reinterpret_cast<int*>(smem);
-    const int mine = __ballot(nan) != 0;
-    __syncthreads();  // nobody reads the last stage any more
-    if (at.lane == 0) found[at.wave] = mine;
-    __syncthreads();
-    int again = 0;
-#pragma unroll
-    for (int w = 0; w < WM * WN; ++w) again |= found[w];
-    __syncthreads();
-    if (__builtin_amdgcn_readfirstlane(again)) {
+        for (int k = 0; k < 4; ++k) nan |= acc[i][j][k] != acc[i][j][k];
+    int mine = 0;
+    if (__ballot(nan) != 0) {  // those of outputs that are there
+      // bit 4 (i JM + j) + k of a thread is for acc[i][j][k], row j 16 + lane % 16, column i 16 + lane / 16 4 + k
+      uint32_t mark[B::kWords] = {}, any = 0;
+      const int rows = (int)min((int64_t)(JM * 16), p.M - m0) - at.lane % 16, cols = (int)min((int64_t)(JN * 16), p.N - n0) - at.lane / 16 * 4;
 #pragma unroll
       for (int i = 0; i < JN; ++i)
 #pragma unroll
-        for (int j = 0; j < JM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      sum_tile<T, AK, BK, BM, BN, WM, WN, NS>(p, at, smem, acc);
+        for (int j = 0; j < JM; ++j)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int bit = 4 * (i * JM + j) + k;
+            if (acc[i][j][k] != acc[i][j][k] && j * 16 < rows && i * 16 + k < cols) mark[bit / 32] |= 1u << bit % 32;
+          }
+#pragma unroll
+      for (int w = 0; w < B::kWords; ++w) {
+        marks[w * B::kThreads + threadIdx.x] = mark[w];
+        any |= mark[w];
+      }
+      mine = __ballot(any != 0) != 0;
     }
-  } else {
-    sum_tile<T, AK, BK, BM, BN, WM, WN, NS>(p, at, smem, acc);
+    if (at.lane == 0) found[at.wave] = mine;
+    __syncthreads();
+    uint32_t again = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) again |= found[w];
+    again = __builtin_amdgcn_readfirstlane(again);
+    store_tile<T, JM, JN, kWaves, B::kStages>(e, smem, acc, m0, p.M, n0, p.N, at.wave, at.lane);
+    if (!again) return;
+#pragma unroll
+    for (int i = 0; i < JN; ++i)
+#pragma unroll
+      for (int j = 0; j < JM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    __syncthreads();  // nobody reads the sums in LDS any more
+    Place<BM, BN, WM, WN> once_more = at;
+    asm volatile("" : "+v"(once_more.lane), "+s"(once_more.wave));  // (or registers would hold places from the first sums to these)
+    sum_tile<T, AK, BK, BM, BN, WM, WN, NS>(p, once_more, smem, acc);  // (it waits for the wave's stores, too)
+    uint32_t mark[B::kWords] = {};
+    if (mine) {
+#pragma unroll
+      for (int w = 0; w < B::kWords; ++w) mark[w] = marks[w * B::kThreads + threadIdx.x];
+    }
+#pragma unroll
+    for (int i = 0; i < JN; ++i)
+#pragma unroll
+      for (int j = 0; j < JM; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int bit = 4 * (i * JM + j) + k;
+          if (!(mark[bit / 32] >> bit % 32 & 1)) acc[i][j][k] = __builtin_bit_cast(float, kKeep);
+        }
+    store_tile<T, JM, JN, kWaves, B::kStages, true>(e, smem, acc, m0, p.M, n0, p.N, at.wave, at.lane);
   }
-  store_tile<T, JM, JN, WM * WN, kBytes>(p, smem, acc, at.m0 + at.wm, at.n0 + at.wn, at.wave, at.lane, split);
 }
 
 template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
 __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const Product p) {
-  __shared__ __attribute__((aligned(1024))) char smem[NS * (BM + BN) * 128];
+  __shared__ __attribute__((aligned(1024))) char smem[TileBytes<T, BM, BN, WM, WN, NS>::kAll];
   run_tile<T, AK, BK, BM, BN, WM, WN, NS>(p, smem, blockIdx.x, (int)blockIdx.y);
 }
 
@@ -815,7 +888,7 @@ struct Pair {
 
 template <typename T, int BM, int BN, int WM, int WN, int NS>
 __global__ __launch_bounds__(64 * WM * WN) void pair_kernel(const Pair p) {
-  __shared__ __attribute__((aligned(1024))) char smem[NS * (BM + BN) * 128];
+  __shared__ __attribute__((aligned(1024))) char smem[TileBytes<T, BM, BN, WM, WN, NS>::kAll];
   const uint32_t id = blockIdx.x;
   if (id - p.dx0 < p.dx_count) {
     const uint32_t at = id - p.dx0, tiles = p.dx_count / p.dx.splits;

@@ -82,3 +82,57 @@ def test_fused_linear_under_autocast(dt, given, rows):
         grads = torch.autograd.grad(out, (x, m.weight, m.bias), up)
         for got, ref, t in zip(grads, torch.autograd.grad(want, low, up), (x, m.weight, m.bias)):
             assert got.dtype == t.dtype and torch.equal(got, ref.to(t.dtype))
+
+
+def _holed(t, fill, pad=12):
+    """t's values in rows `pad` elements longer, whose extra elements are `fill`."""
+    wide = torch.full((t.shape[0], t.shape[1] + pad), fill, dtype=t.dtype, device=t.device)
+    wide[:, :t.shape[1]] = t
+    return wide[:, :t.shape[1]]
+
+
+# fp32 sizes whose products, of the call and of its backward, are summed in tiles of every height and width from 64 x 128 on
+SPLIT = [(2048, 2048, 104), (1000, 1100, 1540), (2048, 2048, 2048), (1500, 2048, 4100), (4096, 4096, 264), (6000, 6000, 1100)]
+
+
+def _normal(seed, *shapes):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return [torch.randn(*s, generator=g, device="cuda") * (s[-1] ** -0.5 if len(s) == 2 and k == 1 else 1.0) for k, s in enumerate(shapes)]
+
+
+@pytest.mark.parametrize("M,N,K", SPLIT)
+def test_fp32_results_do_not_depend_on_what_lies_between_rows(M, N, K):
+    x, w, g = _normal(8, (M, K), (N, K), (M, N))
+    runs = []
+    for fill in (0.0, float("nan"), float("inf")):
+        ts = [_holed(t, fill).requires_grad_(True) for t in (x, w)]
+        out = linear_act(*ts)
+        runs.append((out.detach(), *torch.autograd.grad(out, ts, g)))
+    assert all(torch.equal(p, q) for run in runs[1:] for p, q in zip(run, runs[0]))
+
+
+@pytest.mark.parametrize("M,N,K", SPLIT)
+def test_fp32_results_do_not_depend_on_other_rows(M, N, K):
+    """Bit by bit: NaN and infinities in some rows of every operand leave every other sum as it was."""
+    x, w, g = _normal(9, (M, K), (N, K), (M, N))
+    rows, cols = torch.tensor([1, M // 2, M - 1], device="cuda"), torch.tensor([0, N - 3], device="cuda")
+    x2, w2 = x.clone(), w.clone()
+    x2[1, K // 2], x2[M // 2, 0], x2[M - 1, K - 1] = float("nan"), float("inf"), -float("inf")
+    w2[0, K - 1], w2[N - 3, 1] = float("inf"), float("nan")
+    clean, out = linear_act(x, w), linear_act(x2, w2)
+    keep = torch.ones_like(clean, dtype=torch.bool)
+    keep[rows], keep[:, cols] = False, False
+    assert torch.equal(out[keep], clean[keep])
+    ref = x2.double() @ w2.double().t()
+    assert torch.equal(out.isnan(), ref.isnan()) and torch.equal(out.isinf(), ref.isinf())
+    assert torch.equal(out[out.isinf()].sign().double(), ref[ref.isinf()].sign())
+    # dx = g W: a row of g; dW = g^T x: a column of g and a column of x
+    ts = [t.requires_grad_(True) for t in (x, w)]
+    y = linear_act(*ts)
+    dx, dw = torch.autograd.grad(y, ts, g, retain_graph=True)
+    g2 = g.clone()
+    g2[3, 5] = float("nan")
+    dx2, dw2 = torch.autograd.grad(y, ts, g2)
+    assert dx2[3].isnan().all() and dw2[5].isnan().all()
+    dx2[3], dw2[5] = dx[3], dw[5]
+    assert torch.equal(dx2, dx) and torch.equal(dw2, dw)
