@@ -657,9 +657,15 @@ MHC_DEV void sum_tile(const Product& p, const Place<BM, BN, WM, WN>& at, char* s
 // fp32 operands on the bf16 matrix instructions
 // --------------------------------------------------------------------------
 
-// Eight fp32 values as three bf16 values each: the leading eight bits of the
-// value, of what is left and of what is left then.  Cut off and not rounded,
-// they add up to the value exactly.  An infinity's second part is NaN.
+// Eight fp32 values, times kLift, as three bf16 values each: the leading eight
+// bits of the value, of what is left and of what is left then.  Cut off and not
+// rounded, they add up to the value exactly: the last bit of an fp32 value is
+// 2^-149 or more, and of a bf16 one 2^-133 or more, which is why values are
+// lifted (unlifted, a value around 2^-120 would keep 2^-13 of itself too
+// little).  Lifted values past the range are infinite, and the second part of
+// an infinity is NaN.
+constexpr float kLift = 0x1p16f;
+
 MHC_DEV void split8(const u32x4& lo, const u32x4& hi, u32x4 (&part)[3]) {
   const f32x4 flo = __builtin_bit_cast(f32x4, lo), fhi = __builtin_bit_cast(f32x4, hi);
 #pragma unroll
@@ -667,7 +673,7 @@ MHC_DEV void split8(const u32x4& lo, const u32x4& hi, u32x4 (&part)[3]) {
     uint32_t x[2], y[2], z[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const float v = w < 2 ? flo[2 * w + k] : fhi[2 * w - 4 + k];
+      const float v = kLift * (w < 2 ? flo[2 * w + k] : fhi[2 * w - 4 + k]);
       x[k] = __builtin_bit_cast(uint32_t, v);
       const float r = v - __builtin_bit_cast(float, x[k] & 0xffff0000u);
       y[k] = __builtin_bit_cast(uint32_t, r);
@@ -742,6 +748,10 @@ MHC_DEV void sum_tile_split(const Product& p, const Place<BM, BN, WM, WN>& at, c
     ahead = ahead == (NS - 1) * kStage ? 0 : ahead + kStage;
   }
   wait_loads<0>();
+#pragma unroll
+  for (int i = 0; i < JN; ++i)
+#pragma unroll
+    for (int j = 0; j < JM; ++j) acc[i][j] *= 1.f / (kLift * kLift);
 }
 
 // --------------------------------------------------------------------------
@@ -764,9 +774,9 @@ struct TileBytes {
 };
 
 // A tile of outputs, or (split) of one part of the reduction's sums.  Sums on
-// split values that come out as NaN are formed once more with fp32
-// instructions: they tell what an infinity makes of a sum, whose parts make NaN
-// of everything.  The other sums of the tile stay as they are, so that a row's
+// split values that come out infinite or as NaN are formed once more with fp32
+// instructions: their values or lifted sums were past the range (2^111, 2^95),
+// or had an infinity, whose parts make NaN of everything.  The other sums of the tile stay as they are, so that a row's
 // outputs do not depend on what other rows hold.
 template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
 MHC_DEV void run_tile(const Product& p, char* smem, uint32_t tile, int split) {
@@ -785,15 +795,16 @@ MHC_DEV void run_tile(const Product& p, char* smem, uint32_t tile, int split) {
     sum_tile_split<AK, BK, BM, BN, WM, WN, NS>(p, at, smem, acc);
     uint32_t* const marks = reinterpret_cast<uint32_t*>(smem + B::kStages);
     uint32_t* const found = marks + B::kWords * B::kThreads;
-    bool nan = false;
+    const auto past = [](float v) { return !(fabsf(v) < __builtin_inff()); };
+    bool one = false;
 #pragma unroll
     for (int i = 0; i < JN; ++i)
 #pragma unroll
       for (int j = 0; j < JM; ++j)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) nan |= acc[i][j][k] != acc[i][j][k];
+        for (int k = 0; k < 4; ++k) one |= past(acc[i][j][k]);
     int mine = 0;
-    if (__ballot(nan) != 0) {  // those of outputs that are there
+    if (__ballot(one) != 0) {  // those of outputs that are there
       // bit 4 (i JM + j) + k of a thread is for acc[i][j][k], row j 16 + lane % 16, column i 16 + lane / 16 4 + k
       uint32_t mark[B::kWords] = {}, any = 0;
       const int rows = (int)min((int64_t)(JM * 16), p.M - m0) - at.lane % 16, cols = (int)min((int64_t)(JN * 16), p.N - n0) - at.lane / 16 * 4;
@@ -804,7 +815,7 @@ MHC_DEV void run_tile(const Product& p, char* smem, uint32_t tile, int split) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int bit = 4 * (i * JM + j) + k;
-            if (acc[i][j][k] != acc[i][j][k] && j * 16 < rows && i * 16 + k < cols) mark[bit / 32] |= 1u << bit % 32;
+            if (past(acc[i][j][k]) && j * 16 < rows && i * 16 + k < cols) mark[bit / 32] |= 1u << bit % 32;
           }
 #pragma unroll
       for (int w = 0; w < B::kWords; ++w) {

@@ -136,3 +136,31 @@ def test_fp32_results_do_not_depend_on_other_rows(M, N, K):
     assert dx2[3].isnan().all() and dw2[5].isnan().all()
     dx2[3], dw2[5] = dx[3], dw[5]
     assert torch.equal(dx2, dx) and torch.equal(dw2, dw)
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 64, 96), (100, 130, 96)] + SPLIT)
+def test_fp32_values_near_both_ends_of_the_range(M, N, K):
+    """Rows of values down to subnormal ones against weights that make ordinary numbers of them, and large results."""
+    x, w = _normal(10, (M, K), (N, K))
+    for row, size in ((0, 1e-34), (1, 1e-36), (2, 1e-37), (3, 1e-39), (M - 1, 1e30)):
+        x[row] *= size
+    w[1::2] *= 1e36
+    w[2] *= 1e-36
+    out = linear_act(x, w)
+    ref, bound, *_ = linear64(x, w, None, None, "none", torch.float32)
+    fine = ref.abs() < 3e38
+    close(torch.where(fine, out.double(), 0.0), torch.where(fine, ref, 0.0), torch.where(fine, bound, 1.0), "out")
+    assert not out[:4].isinf().any()
+
+
+def test_fp32_gradients_of_tiny_values():
+    """Both products of the backward with a gradient that is as small, in tiles of several sizes."""
+    for M, N, K in SPLIT:
+        x, w, g = _normal(11, (M, K), (N, K), (M, N))
+        x, w, g = x * 1e30, w * 1e28, g * 1e-37
+        ts = [t.requires_grad_(True) for t in (x, w)]
+        dx, dw = torch.autograd.grad(linear_act(*ts), ts, g)
+        one = torch.ones(M, N, dtype=torch.float64, device="cuda")
+        px, pw, _ = linear_grads64(x, w, g, one, torch.zeros_like(one), torch.float32, False)
+        close(dx, *px, f"dx {M} {N} {K}")
+        close(dw, *pw, f"dw {M} {N} {K}")
