@@ -414,9 +414,9 @@ size_t mhc_linear_act_fwd_workspace_bytes(const void* x, int64_t ldx, const void
  * apart, w [N, K] with rows ldw apart, bias [N] or NULL, all of `dtype`;
  * residual [M, N] or NULL and out of out_dtype (`dtype` or fp32), contiguous.
  * dact [M, N] or NULL (only NULL for MHC_ACT_NONE) receives act'(x W^T +
- * bias) for the backward: fp32 for fp32, else int16, (act' - 1/2) 2^15 with
- * -2^15 for NaN.  Sums are held in fp32.  M is below 2^28, N and K are below
- * 2^22. */
+ * bias) for the backward: fp32 for fp32, else 16-bit codes, which hold it to
+ * 2^-16 and to 2^-10 of itself.  Sums are held in fp32.  M is below 2^28, N
+ * and K are below 2^22. */
 int mhc_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
                        const void* residual, void* out, int out_dtype, void* dact, int act,
                        int64_t M, int64_t N, int64_t K, int dtype, void* workspace,

@@ -98,18 +98,37 @@ MHC_DEV void activate_all(int act, float (&z)[R][V], float (&d)[R][V]) {
   }
 }
 
-// act'(z) as a backward reads it: fp32 for fp32 operands, else 16 bits in fixed
-// point, (act' - 1/2) 2^15.  All of the derivatives lie in [-0.13, 1.13], so
-// that 2^-16 is the largest error, where fp16 has 2^-11 of the value and more
-// of the gradients' error would be act's than the one rounding of dz; 0 and 1
-// are exact.  The lowest code is NaN.
-template <typename T> struct DactOf { using Type = int16_t; };
+// act'(z) as a backward reads it: fp32 for fp32 operands, else 16 bits.  All of
+// the derivatives lie in [-0.13, 1.13], and most of fp16's codes are for numbers
+// that they never are: with 2^-11 of the value, fp16 would add to the one
+// rounding of dz.  From 1/32 on the code is fixed point in steps of 2^-15, below
+// it has nine bits after the leading one, down to 2^-29 and evenly from there:
+// the error is at most 2^-16, and 2^-10 of the value (a unit far below zero has
+// a derivative of 1e-5 and less, and still its gradient), 0 and 1 are exact.
+// Codes rise with the value from 16384 for 0; the largest is NaN.
+template <typename T> struct DactOf { using Type = uint16_t; };
 template <> struct DactOf<float> { using Type = float; };
 
+constexpr uint32_t kDactZero = 16384, kDactNan = 0xffff;
+constexpr uint32_t kDactEven = 25 << 9;     // code of 1/32: 24 powers of two of 512 codes, and what is below them
+constexpr float kDactLeast = 0x1p-97f;      // 2^-29, the least with nine bits of its own, to the least normal number
+constexpr uint32_t kDactFixed = kDactEven - 1024;  // fixed point counts 1/32 as 1024
+
 MHC_DEV uint32_t dact_code(float d) {
-  return (uint32_t)(d == d ? (int)rintf((d - 0.5f) * 32768.f) : -32768) & 0xffffu;
+  const float a = fabsf(d);
+  const uint32_t low = (__builtin_bit_cast(uint32_t, a * kDactLeast) + 0x2000u) >> 14;  // (of NaN: far above the codes)
+  const uint32_t high = (uint32_t)fmaf(a, 32768.f, (float)kDactFixed + 0.5f);
+  const uint32_t c = !(a >= 0x1p-5f) ? low : high, sign = (uint32_t)(__builtin_bit_cast(int32_t, d) >> 31);
+  return min((c ^ sign) + (kDactZero - sign), kDactNan);
 }
-MHC_DEV float dact_value(int16_t q) { return q == -32768 ? __builtin_nanf("") : 0.5f + (float)q * 0x1p-15f; }
+MHC_DEV float dact_value(uint16_t q) {
+  const int32_t c = (int32_t)q - (int32_t)kDactZero;
+  const uint32_t a = (uint32_t)max(c, -c);
+  const float low = __builtin_bit_cast(float, a << 14) * (1.f / kDactLeast);
+  const float high = fmaf((float)a, 0x1p-15f, -(float)kDactFixed * 0x1p-15f);
+  const float v = __builtin_copysignf(a < kDactEven ? low : high, __builtin_bit_cast(float, c));
+  return q == kDactNan ? __builtin_nanf("") : v;
+}
 MHC_DEV float dact_value(float d) { return d; }
 
 // Eight values to or from p, which starts anywhere, as 16-byte vectors (the
@@ -119,14 +138,14 @@ MHC_DEV float dact_value(float d) { return d; }
 template <bool WHOLE, typename O, int V>
 MHC_DEV void put(O* p, const float (&z)[V], int left) {
   if constexpr (V == 1) {
-    if constexpr (__is_same(O, int16_t)) *p = (int16_t)dact_code(z[0]);
+    if constexpr (__is_same(O, uint16_t)) *p = (uint16_t)dact_code(z[0]);
     else store1(p, z[0]);
   } else {
     uint32_t w[V * sizeof(O) / 4];
 #pragma unroll
     for (int k = 0; k < (int)(V * sizeof(O) / 4); ++k) {
       if constexpr (sizeof(O) == 4) w[k] = __builtin_bit_cast(uint32_t, (float)z[k]);
-      else if constexpr (__is_same(O, int16_t)) w[k] = dact_code(z[2 * k]) | dact_code(z[2 * k + 1]) << 16;
+      else if constexpr (__is_same(O, uint16_t)) w[k] = dact_code(z[2 * k]) | dact_code(z[2 * k + 1]) << 16;
       else w[k] = pack2<O>(z[2 * k], z[2 * k + 1]);
     }
     if constexpr (WHOLE) {
@@ -171,7 +190,7 @@ MHC_DEV void take_dact(const D* p, float (&z)[V], int left) {
   } else if constexpr (WHOLE) {
     const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
 #pragma unroll
-    for (int k = 0; k < V; ++k) z[k] = dact_value((int16_t)(w[k / 2] >> (16 * (k % 2))));
+    for (int k = 0; k < V; ++k) z[k] = dact_value((uint16_t)(w[k / 2] >> (16 * (k % 2))));
   } else {
 #pragma unroll
     for (int k = 0; k < V; ++k) z[k] = k < left ? dact_value(p[k]) : 0.f;

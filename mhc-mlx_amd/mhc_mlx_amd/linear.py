@@ -6,7 +6,9 @@ It is the layer that MHCRewire wraps and AutoPatcher finds (FusedLinear is an ``
 [N, K], bias [N], residual [..., N]; float32, bfloat16 or float16, x, weight and bias of one dtype; the output (and the
 residual) of that dtype or float32.  Sums are held in fp32.  The backward gives the gradients of x, weight, bias and
 residual; dz = dout act'(z) is rounded once to x's dtype as an operand of the two products (the bias's gradient is
-summed from it unrounded).  It is not twice differentiable.
+summed from it unrounded).  The forward keeps act'(z) for it, of 16-bit operands in 16 bits (to 2^-16, and to 2^-10 of
+itself down to 2^-29), and forms their activations to about 2^-21 of z, for float32 outputs too.  It is not twice
+differentiable.
 
 linear_act needs GPU tensors and the built library, fewer than 2^28 rows, and N and K below 2^22; FusedLinear hands a call
 that the HIP path cannot take (CPU tensors, a wider layer, a RuntimeError from the library) to ``linear_act_reference``,

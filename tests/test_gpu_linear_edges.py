@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from tests._train import close, linear64, linear_grads64
+from tests._train import U32, UNIT, act64, close, linear64, linear_grads64
 
 from mhc_mlx_amd import FusedLinear, linear_act
 from mhc_mlx_amd import layer as L
@@ -164,3 +164,37 @@ def test_fp32_gradients_of_tiny_values():
         px, pw, _ = linear_grads64(x, w, g, one, torch.zeros_like(one), torch.float32, False)
         close(dx, *px, f"dx {M} {N} {K}")
         close(dw, *pw, f"dw {M} {N} {K}")
+
+
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M", [3, 300])
+def test_gradients_of_units_far_below_zero(act, dt, M):
+    """act' keeps its precision where it is small: x is 0, so that z is the bias and db a sum of equal values."""
+    b = torch.linspace(-14, 8, 1001, device="cuda").to(dt).requires_grad_(True)
+    x, w = torch.zeros(M, 16, device="cuda", dtype=dt), torch.ones(1001, 16, device="cuda", dtype=dt)
+    out = linear_act(x, w, b, activation=act)
+    db, = torch.autograd.grad(out, b, torch.ones_like(out))
+    z = b.detach().double()
+    _, d = act64(z, act)
+    # its code: 2^-10 of it, down to 2^-39; its formula: roundings of the exponent's argument (up to 2^7, 16 where act' is
+    # above 2^-39) and a few more of each term, and the error function's polynomial, 1.5e-7 / 2
+    phi = torch.exp(-z * z / 2)
+    terms = {"gelu": z.abs() * phi + torch.special.ndtr(z), "silu": torch.sigmoid(z) * (1 + z.abs()),
+             "gelu_tanh": d.abs() + 4 * torch.sigmoid(1.6 * z + 0.0714 * z ** 3) * (1 + z.abs() ** 3)}[act]
+    bound = 2.0 ** -10 * d.abs() + 2.0 ** -39 + 256 * U32 * terms + (0.75e-7 if act == "gelu" else 0.0)
+    close(db, M * d, M * bound + UNIT[dt] * M * d.abs() + 2.0 ** -25, act)
+
+
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("M", [3, 300])
+def test_nan_goes_through_the_derivative(act, M):
+    x, w, b, g = (t.to(torch.bfloat16) for t in _normal(12, (M, 40), (136, 40), (136,), (M, 136)))
+    x[1, 7], b[5] = float("nan"), -float("nan")
+    ts = [t.requires_grad_(True) for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(linear_act(*ts, activation=act), ts, g)
+    assert dx.isnan().all() and dw.isnan().all() and db.isnan().all()  # (every row has column 5, every column row 1)
+    with torch.no_grad():
+        b[5] = 0
+    dx, _, db = torch.autograd.grad(linear_act(*ts, activation=act), ts, g)
+    assert dx[1].isnan().all() and dx[[k for k in range(M) if k != 1]].isfinite().all() and db.isnan().all()
