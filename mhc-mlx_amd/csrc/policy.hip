@@ -141,14 +141,15 @@ MHC_DEV Token token_of(const mhc_policy_args& a, int64_t t, const T* row, float 
   const float ratio = expf((float)(lp - (double)a.old_logp[t])), adv = a.advantages[t];
   // (a NaN ratio stays one: fminf and fmaxf would drop it)
   const float held_ratio = ratio < 1.f - a.clip_low ? 1.f - a.clip_low : ratio > 1.f + a.clip_high ? 1.f + a.clip_high : ratio;
-  const float free = ratio * adv, held = held_ratio * adv;
+  // (a ratio past fp32's range is still nothing without an advantage, and so is a KL term without a coefficient)
+  const float free = adv == 0.f && ratio == __builtin_inff() ? 0.f : ratio * adv, held = held_ratio * adv;
   Token r;
   r.logp = (float)lp;
   r.logit = z;
   r.loss = -(free <= held ? free : held);
   r.coef = free <= held ? -free : 0.f;
   if (!(free == free)) r.loss = r.coef = nan;
-  if (a.ref_logp != nullptr) {
+  if (a.ref_logp != nullptr && a.kl_coef != 0.f) {
     const float gap = (float)((double)a.ref_logp[t] - lp), over = expm1f(gap);  // q - 1 without cancellation near q = 1
     r.loss += a.kl_coef * (over - gap);
     r.coef -= a.kl_coef * over;

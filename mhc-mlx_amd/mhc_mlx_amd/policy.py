@@ -64,7 +64,7 @@ def policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logp: torch.Ten
     """(loss, logp): the scalar loss, differentiable in ``logits``, and each token's log probability (no gradient).
 
     logits [..., V] float32, bfloat16 or float16; the others [...]: actions int64 or int32, old_logp, advantages and
-    ref_logp floating, mask bool, uint8 or floating weights.  Without ref_logp there is no KL term.
+    ref_logp floating, mask bool, uint8 or floating weights.  Without ref_logp, or with kl_coef 0, there is no KL term.
     """
     den = _check(clip_low, clip_high, denominator)
     numbers = float(clip_low), float(clip_high), float(kl_coef), den

@@ -109,6 +109,20 @@ def test_tokens_left_out(dt, V):
     assert g.isfinite().all() and not g[~mask].any()
 
 
+@pytest.mark.parametrize("V", [40, 5000, 140000])
+def test_exponentials_past_fp32_without_a_factor(V):
+    """exp(lp - old) of a token without an advantage, and exp(ref - lp) with kl_coef 0, count for nothing when they overflow."""
+    z, a, old, adv, ref, mask = _inputs(8, V, "f32", 12)
+    mask[:4] = True
+    z[torch.arange(2), a[:2]] = -150.0  # lp about -160, against a reference of about -8
+    old[:2] = torch.log_softmax(z[:2].double(), 1).gather(1, a[:2, None])[:, 0].float() - 0.05
+    old[2], adv[2] = -200.0, 0.0
+    old[3], adv[3] = -200.0, 1.0  # held by the clip
+    assert torch.exp(ref[0] + 150.0).isinf()
+    _check(z, a, old, adv, ref, mask, kl=0.0)
+    _check(z[2:], a[2:], old[2:], adv[2:], ref[2:], mask[2:], kl=0.1)
+
+
 def test_nothing_counts():
     z, a, old, adv, ref, mask = _inputs(6, 50, "bf16", 4)
     z.requires_grad_(True)
