@@ -409,7 +409,12 @@ int run_held(const mhc_policy_args& a, float* logp, float* stats, float* terms, 
     return wide ? launch_held<T, 1024, 4, GRAD>(a, logp, stats, terms, scale, dlogits, s)
                 : launch_held<T, 512, 8, GRAD>(a, logp, stats, terms, scale, dlogits, s);
   }
-  if (vecs <= 6656 && !wide) return launch_held<T, 512, 13, GRAD>(a, logp, stats, terms, scale, dlogits, s);
+  if constexpr (!GRAD) {
+    // 13 vectors a thread are the most that leave room for a third workgroup of a CU (78 of 80 registers): the loss of 8192
+    // rows of 34000 bf16 120 us, with 16 vectors 134; of 50257 158 and 175; of 53000 158 and 167.  (With the gradient two fit
+    // either way, and the time is the same.)
+    if (vecs <= 13 * 512 && !wide) return launch_held<T, 512, 13, GRAD>(a, logp, stats, terms, scale, dlogits, s);
+  }
   if (vecs <= 8192) {
     return wide ? launch_held<T, 1024, 8, GRAD>(a, logp, stats, terms, scale, dlogits, s)
                 : launch_held<T, 512, 16, GRAD>(a, logp, stats, terms, scale, dlogits, s);

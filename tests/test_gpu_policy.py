@@ -86,6 +86,16 @@ def test_more_rows_than_workgroups_at_once():
     _check(z, a, old, adv, ref, mask, kl=0.1)
 
 
+@pytest.mark.parametrize("vecs", [1025, 4096, 4097, 6656, 6657, 8192, 8193])
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+def test_long_rows_of_more_tokens_than_compute_units(vecs, dt):
+    """Vocabularies around the lengths at which a workgroup's threads hold more vectors of a row."""
+    T = torch.cuda.get_device_properties(0).multi_processor_count + 5
+    e = 4 if dt == "f32" else 8
+    z, a, old, adv, ref, mask = _inputs(T, vecs * e + (vecs % 2) * 3, dt, 13)  # (odd ones: rows that end inside a vector)
+    _check(z, a, old, adv, ref, mask, kl=0.1, scale=1024.0 if dt == "f16" else 1.0)
+
+
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("V", [40, 1024, 33000])
 def test_tokens_left_out(dt, V):
