@@ -349,10 +349,10 @@ int mhc_adamw_step(const mhc_adamw_tensor* tensors, int64_t count, int dtype, in
 
 /* Arguments shared by the policy-loss calls.  logits [T, V] of `dtype` with
  * rows row_stride elements apart; actions [T] int64 in [0, V); old_logp,
- * advantages [T] fp32; ref_logp [T] fp32 or NULL (no KL term, nor with kl_coef 0); weights [T] of
- * weights_dtype (fp32, or MHC_DTYPE_U8: 0 or 1) or NULL (all one), and 0
- * leaves a token out: none of its other inputs counts.  denominator > 0
- * divides the sum; 0: the sum of the weights (1 if that is 0). */
+ * advantages [T] fp32; ref_logp [T] fp32 or NULL (no KL term, nor is there one
+ * with kl_coef 0); weights [T] of weights_dtype (fp32, or MHC_DTYPE_U8: 0 or 1)
+ * or NULL (all one), and 0 leaves a token out: none of its other inputs counts.
+ * denominator > 0 divides the sum; 0: the sum of the weights (1 if that is 0). */
 typedef struct {
   const void* logits;
   int64_t row_stride;

@@ -58,7 +58,8 @@ MHC_DEV float normal_cdf(float z, float e) {
   return z < 0.f ? tail : 1.f - tail;
 }
 
-// act(z) and act'(z).  NaN goes through each of them.
+// act(z) and act'(z).  NaN goes through each of them, but for relu', which is 0
+// wherever z is not above 0.
 template <bool FAST, int ACT>
 MHC_DEV Act activate(float z) {
   if constexpr (ACT == MHC_ACT_RELU) {
