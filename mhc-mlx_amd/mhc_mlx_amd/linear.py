@@ -7,8 +7,8 @@ It is the layer that MHCRewire wraps and AutoPatcher finds (FusedLinear is an ``
 residual) of that dtype or float32.  Sums are held in fp32.  The backward gives the gradients of x, weight, bias and
 residual; dz = dout act'(z) is rounded once to x's dtype as an operand of the two products (the bias's gradient is
 summed from it unrounded).  The forward keeps act'(z) for it, of 16-bit operands in 16 bits (to 2^-16, and to 2^-10 of
-itself down to 2^-29), and forms their activations to about 2^-21 of z, for float32 outputs too.  It is not twice
-differentiable.
+itself down to 2^-29), and forms their activations to about 2^-21 of z and 2^-15 of themselves, for float32 outputs too.
+It is not twice differentiable.
 
 linear_act needs GPU tensors and the built library, fewer than 2^28 rows, and N and K below 2^22; FusedLinear hands a call
 that the HIP path cannot take (CPU tensors, a wider layer, a RuntimeError from the library) to ``linear_act_reference``,
@@ -99,7 +99,7 @@ def linear_act_reference(x, weight, bias=None, residual=None, activation: str = 
     if activation == "relu":
         z = torch.clamp(z, min=0.0)
     elif activation == "gelu":
-        z = z * (0.5 * (1.0 + torch.erf(z * math.sqrt(0.5))))
+        z = z * (0.5 * torch.erfc(z * -math.sqrt(0.5)))
     elif activation == "gelu_tanh":
         z = 0.5 * z * (1.0 + torch.tanh(math.sqrt(2.0 / math.pi) * (z + 0.044715 * z ** 3)))
     elif activation == "silu":

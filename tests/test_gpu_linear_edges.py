@@ -178,12 +178,26 @@ def test_gradients_of_units_far_below_zero(act, dt, M):
     z = b.detach().double()
     _, d = act64(z, act)
     # its code: 2^-10 of it, down to 2^-39; its formula: roundings of the exponent's argument (up to 2^7, 16 where act' is
-    # above 2^-39) and a few more of each term, and the error function's polynomial, 1.5e-7 / 2
+    # above 2^-39) and a few more of each term, and the normal distribution's polynomial
     phi = torch.exp(-z * z / 2)
     terms = {"gelu": z.abs() * phi + torch.special.ndtr(z), "silu": torch.sigmoid(z) * (1 + z.abs()),
              "gelu_tanh": d.abs() + 4 * torch.sigmoid(1.6 * z + 0.0714 * z ** 3) * (1 + z.abs() ** 3)}[act]
-    bound = 2.0 ** -10 * d.abs() + 2.0 ** -39 + 256 * U32 * terms + (0.75e-7 if act == "gelu" else 0.0)
+    bound = 2.0 ** -10 * d.abs() + 2.0 ** -39 + 256 * U32 * terms + (7e-6 * torch.special.ndtr(z) if act == "gelu" else 0.0)
     close(db, M * d, M * bound + UNIT[dt] * M * d.abs() + 2.0 ** -25, act)
+
+
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M", [3, 300])
+def test_values_of_units_far_below_zero(act, dt, M):
+    """float32 outputs hold 2^-14 of an activation however small it is."""
+    b = torch.linspace(-9, 9, 1001, device="cuda").to(dt)
+    x, w = torch.zeros(M, 16, device="cuda", dtype=dt), torch.ones(1001, 16, device="cuda", dtype=dt)
+    z = b.double()
+    y = z * 0.5 * torch.special.erfc(-z * 0.5 ** 0.5) if act == "gelu" else act64(z, act)[0]  # (ndtr is 1 + erf: 0 from -8.3 on)
+    y = y.expand(M, 1001)
+    # Phi's fit 7e-6; the exponent's argument, up to 75 (gelu_tanh at -9), rounded three times
+    close(linear_act(x, w, b, activation=act, output_dtype=torch.float32), y, (7e-6 + 256 * U32 + 16 * U32) * y.abs() + 2.0 ** -126, act)
 
 
 @pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
