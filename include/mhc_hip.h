@@ -412,7 +412,8 @@ size_t mhc_linear_act_fwd_workspace_bytes(const void* x, int64_t ldx, const void
 
 /* out [M, N] = act(x W^T + bias) + residual.  x [M, K] with rows ldx elements
  * apart, w [N, K] with rows ldw apart, bias [N] or NULL, all of `dtype`;
- * residual [M, N] or NULL and out of out_dtype (`dtype` or fp32), contiguous.
+ * residual [M, N] or NULL and out of out_dtype (`dtype` or fp32), contiguous;
+ * out and dact overlap nothing else.
  * dact [M, N] or NULL (only NULL for MHC_ACT_NONE) receives act'(x W^T +
  * bias) for the backward: fp32 for fp32, else 16-bit codes, which hold it to
  * 2^-16 and to 2^-10 of itself.  Sums are held in fp32.  M is below 2^28, N

@@ -16,7 +16,7 @@
 // captured graph or a later step could find changed), and a workgroup finds
 // its tensor with one or two loads of the chunk counts, a lane each, and
 // votes.  Large tensors are bound by memory (16 of 4096 x 4096 bf16 with
-// masters: 28 bytes an element at 5.3 TB/s; in 8 bits 5.2 TB/s), lists of
+// masters: 28 bytes an element at 5.2 TB/s; in 8 bits the same), lists of
 // small ones by the host.
 #include <cmath>
 

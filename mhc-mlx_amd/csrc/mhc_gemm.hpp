@@ -712,10 +712,11 @@ MHC_DEV void split8(const u32x4& lo, const u32x4& hi, u32x4 (&part)[3]) {
 
 // sum_tile for fp32 with each product of two values as six of their parts.
 // The three that are left out are below 2^-21 of it, and 2^-24 on average, so
-// that the sums are as good as fp32's own (1000 x 1100 x 1536: 6.0e-7 of the
-// result off float64, 7.0e-7 with fp32 instructions).  Six bf16 products take
+// that the sums are as good as fp32's own (2048 x 2048 x 2048: 7.0e-7 of the
+// result off float64, 8.1e-7 with fp32 instructions).  Six bf16 products take
 // 3/8 of the time of one in fp32; the splits, on the vector unit, go on beside
-// them in another wave.
+// them in another wave (the lift is one of their 6.5 instructions for a value,
+// and 5 % of the time).
 template <bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
 MHC_DEV void sum_tile_split(const Product& p, const Place<BM, BN, WM, WN>& at, char* smem, f32x4 (&acc)[BN / WN / 16][BM / WM / 16]) {
   using S = Stage<float>;
@@ -783,10 +784,11 @@ MHC_DEV void sum_tile_split(const Product& p, const Place<BM, BN, WM, WN>& at, c
 // The kernels of tiles
 // --------------------------------------------------------------------------
 
-// fp32 tiles of at least 64 x 128 are summed on the bf16 instructions (1000 x
-// 1100 x 1536 in 128 x 128 107 us in fp32, 89 so; 8192 x 4096 x 4096 in 256 x
-// 256 1889 and 1180, where the library's fp32 product takes 1800; 64 x 64 have
-// too few products for each value that is split: 512 x 2048 x 2048 43 and 56).
+// fp32 tiles of at least 64 x 128 are summed on the bf16 instructions (us in
+// fp32, and so: 8192 x 4096 x 4096 in 256 x 256 1950 and 1370, 2048 x 2048 x 2048
+// in 64 x 128 136 and 119, its backward in 128 x 128 268 and 200; a library's
+// fp32 product takes 1800 for the first.  64 x 64 have too few products for each
+// value that is split: 512 x 2048 x 2048 43 and 56).
 template <typename T, int BN>
 constexpr bool kSplit = sizeof(T) == 4 && BN > 64;
 
@@ -1178,7 +1180,8 @@ struct Cut {
 // few workgroups on the card (its latencies), `busy` for each workgroup of a
 // CU that has `fit` of them (its matrix instructions and LDS reads).  From
 // x W^T over 16 to 512 stages: 256 x 256 16-bit at 1.12 alone, 1.6 with all
-// CUs at it (1.3 PFLOP/s); a stage of fp32 has half the k.
+// CUs at it (1.3 PFLOP/s); a stage of fp32 has half the k (timed before values
+// were lifted, which takes 5 % more of a stage from 64 x 128 on).
 struct TileCost {
   int bm, bn, fit;
   float ends, alone16, busy16, alone32, busy32;
