@@ -110,7 +110,8 @@ class AdamW(torch.optim.Optimizer):
 
     ``state_bits`` 8 keeps the states of tensors with at least ``min_8bit_size`` elements in 8 bits (those of smaller ones,
     the mHC parameters among them, in 32).  ``master_weights`` gives every 16-bit parameter a float32 master copy, made from
-    it at its first step.  CPU parameters are updated by ``adamw_step_reference``.  ``step(grad_scale=...)`` multiplies
+    it at its first step; the parameter is the copy's rounding from then on, so that one who sets a parameter's values
+    later sets ``state[p]["master"]`` too.  CPU parameters are updated by ``adamw_step_reference``.  ``step(grad_scale=...)`` multiplies
     the gradients.
     """
 
