@@ -438,6 +438,110 @@ int mhc_linear_act_bwd(const void* dout, int dout_dtype, const void* dact, const
                        int64_t M, int64_t N, int64_t K, int dtype, void* workspace,
                        size_t workspace_bytes, void* stream);
 
+/* --------------------------------------------------------------------- */
+/* RMS norm with the residual's addition                                   */
+/* --------------------------------------------------------------------- */
+
+/* h = x + residual, rounded to `dtype` (h [T, C], contiguous; without a
+ * residual, NULL, h is x and nothing is written to it);
+ *   s = 1 / sqrt(mean h^2 + eps);  y [T, C] = h s w
+ * x and residual [T, C] of `dtype` with rows ldx and ldr elements apart; w [C]
+ * of w_dtype (`dtype` or fp32), or NULL: ones; y contiguous.  rstd [T] (or
+ * NULL) receives s for the backward.  eps > 0, C < 2^24. */
+int mhc_add_rms_norm_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                         const void* w, int w_dtype, void* h, void* y, float* rstd, int64_t T,
+                         int64_t C, int dtype, float eps, void* stream);
+
+/* The same with y as int8 codes and a scale for each row:
+ *   a = max |h w|;  codes = rint(127 h w / a);  scales = a s / 127
+ * A row of zeros has the scale 0, one with an infinity or NaN in h w the scale
+ * NaN and codes of 0. */
+int mhc_add_rms_norm_int8(const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                          const void* w, int w_dtype, void* h, int8_t* codes, float* scales,
+                          int64_t T, int64_t C, int dtype, float eps, void* stream);
+
+/* x [T, C] itself as codes and scales (a = max |x|, scales = a / 127). */
+int mhc_quantize_int8(const void* x, int64_t ldx, int8_t* codes, float* scales, int64_t T,
+                      int64_t C, int dtype, void* stream);
+
+size_t mhc_add_rms_norm_bwd_workspace_bytes(int64_t T, int64_t C, int dtype);
+
+/* Gradients for dy and dh (or NULL: none) of y and h, from h (or x) and rstd:
+ *   g = dy w;  n = h rstd;  dx [T, C] = rstd (g - n mean(g n)) + dh
+ *   dw [C] = sum_t dy n, of w_dtype
+ * each written if not NULL; dx is the residual's gradient too.  dy, dh and h
+ * have rows lddy, lddh and ldh elements apart.  The workspace is for dw. */
+int mhc_add_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, int64_t lddh,
+                         const void* h, int64_t ldh, const float* rstd, const void* w,
+                         int w_dtype, void* dx, void* dw, int64_t T, int64_t C, int dtype,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* --------------------------------------------------------------------- */
+/* Product of int8 rows with scales                                        */
+/* --------------------------------------------------------------------- */
+
+/* Bytes of workspace of mhc_linear_int8 for these operands. */
+size_t mhc_linear_int8_workspace_bytes(const int8_t* x, int64_t ldx, const int8_t* w,
+                                       int64_t ldw, int64_t M, int64_t N, int64_t K);
+
+/* out [M, N] = act(x_scales[m] w_scales[n] sum_k x[m, k] w[n, k] + bias[n]) +
+ * residual[m, n].  x [M, K] and w [N, K] int8 with rows ldx and ldw apart;
+ * scales and bias (or NULL) fp32; residual [M, N] (or NULL) and out of
+ * out_dtype, contiguous; act is one of MHC_ACT_*.  The products' sums are
+ * exact, in 32 bits: K < 2^17.  M < 2^28, N < 2^22. */
+int mhc_linear_int8(const int8_t* x, int64_t ldx, const float* x_scales, const int8_t* w,
+                    int64_t ldw, const float* w_scales, const float* bias, const void* residual,
+                    void* out, int out_dtype, int act, int64_t M, int64_t N, int64_t K,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* --------------------------------------------------------------------- */
+/* Softmax cross entropy of logits that are not stored                     */
+/* --------------------------------------------------------------------- */
+
+/* Arguments shared by the calls.  x [T, C] and w [V, C] of `dtype` with rows
+ * ldx and ldw elements apart; targets [T] int64; weights [T] of weights_dtype
+ * (fp32, or MHC_DTYPE_U8: 0 or 1) or NULL (all one).  A token of weight 0 or
+ * with the target ignore_index is left out: its row of x is not read.
+ * denominator > 0 divides the sum; 0: the sum of the weights of the tokens
+ * that are not left out (1 if that is 0). */
+typedef struct {
+  const void* x;
+  int64_t ldx;
+  const void* w;
+  int64_t ldw;
+  const int64_t* targets;
+  const void* weights;
+  int weights_dtype;
+  int64_t T;
+  int64_t V;
+  int64_t C;
+  int dtype;
+  int64_t ignore_index;
+  float denominator;
+} mhc_linear_ce_args;
+
+/* Bytes of what the forward leaves for the backward. */
+size_t mhc_linear_ce_state_bytes(int64_t T);
+
+size_t mhc_linear_ce_fwd_workspace_bytes(const mhc_linear_ce_args* args);
+
+/* With z = x W^T: logp [T] = z[t, y_t] - log sum_v exp z[t, v] (0 for a token
+ * left out), loss[0] = -sum_t w_t logp_t / D.  A target outside [0, V) makes
+ * its token's values NaN.  T < 2^28, V and C < 2^22. */
+int mhc_linear_ce_fwd(const mhc_linear_ce_args* args, float* loss, float* logp, void* state,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+size_t mhc_linear_ce_bwd_workspace_bytes(const mhc_linear_ce_args* args, int want_dx,
+                                         int want_dw);
+
+/* grad_scale (times *dloss, if not NULL) times the gradients of the loss:
+ * dx [T, C] (0 for tokens left out) and dw [V, C], contiguous, of `dtype`, each
+ * written if not NULL.  dz = softmax - onehot, times the tokens' weights over
+ * the largest of them, is rounded to `dtype` as an operand of the products. */
+int mhc_linear_ce_bwd(const mhc_linear_ce_args* args, const void* state, const float* dloss,
+                      float grad_scale, void* dx, void* dw, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,381 @@
+// Softmax cross entropy of logits z = x W^T that are never stored whole, and
+// its gradient.
+//
+//   lp_t = z[t, y_t] - log sum_v exp z[t, v];  loss = -sum_t w_t lp_t / D
+//   dz = w_t / D (softmax(z) - [v = y_t]);  dx = dz W;  dW = dz^T x
+//
+// Tokens that count for nothing (weight 0, or the ignored target) are left out
+// at the start: the others' rows of x are brought together, and every product
+// below takes as many rows as there are of them, which only the device knows.
+//
+// Forward: the logits' product keeps of each tile a largest value and a sum of
+// exponentials for each row, which are joined.  Backward: the vocabulary goes
+// by in pieces; the logits of a piece are formed again and become its dz, of
+// which dx (summed up in fp32 over the pieces) and the piece's rows of dW are
+// products.  That is four products of T V C where three would do if the logits
+// were kept.
+#include "mhc_ce.hpp"
+#include "mhc_operand.hpp"
+#include "mhc_plan.hpp"
+
+namespace mhc {
+namespace {
+
+using ce::Gradient;
+using ce::ScaledBy;
+using ce::State;
+using gemm::Cut;
+using gemm::Epilogue;
+using gemm::Operand;
+using gemm::Product;
+using gemm::padded;
+using gemm::up256;
+
+constexpr int kOne = 1024;  // threads of the kernels of one workgroup
+
+// dz of a piece of the vocabulary takes at most about this much.
+constexpr int64_t kPieceBytes = 256 << 20;
+
+MHC_DEV float weight_of(const mhc_linear_ce_args& a, int64_t t) {
+  if (a.targets[t] == a.ignore_index) return 0.f;
+  if (a.weights == nullptr) return 1.f;
+  return a.weights_dtype == MHC_DTYPE_U8 ? (static_cast<const uint8_t*>(a.weights)[t] != 0 ? 1.f : 0.f)
+                                         : static_cast<const float*>(a.weights)[t];
+}
+
+// The live tokens, in order, and D: one workgroup, whose threads each have a run of the tokens.
+__global__ __launch_bounds__(kOne) void ce_live_kernel(const mhc_linear_ce_args a, float* logp, const State s) {
+  __shared__ int counts[kOne / kWave];
+  __shared__ double sums[kOne / kWave];
+  __shared__ float tops[kOne / kWave];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int64_t per = ceil_div(a.T, kOne), t0 = min(a.T, threadIdx.x * per), t1 = min(a.T, t0 + per);
+  int count = 0;
+  double sum = 0;
+  float top = 0.f;
+  for (int64_t t = t0; t < t1; ++t) {
+    const float w = weight_of(a, t);
+    count += w != 0.f;
+    sum += (double)w;
+    top = fmaxf(top, fabsf(w));
+  }
+  int before = count;  // of the wave's lanes up to this one
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int up = __shfl_up(before, d);
+    if (lane >= d) before += up;
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+  top = group_max<kWave>(top);
+  if (lane == kWave - 1) {
+    counts[wave] = before;
+    sums[wave] = sum;
+    tops[wave] = top;
+  }
+  __syncthreads();
+  int first = before - count, total = 0;
+  sum = 0;
+#pragma unroll
+  for (int w = 0; w < kOne / kWave; ++w) {
+    if (w < wave) first += counts[w];
+    total += counts[w];
+    sum += sums[w];
+    top = fmaxf(top, tops[w]);
+  }
+  for (int64_t t = t0; t < t1; ++t) {
+    const float w = weight_of(a, t);
+    if (w == 0.f) {
+      s.pos[t] = -1;
+      logp[t] = 0.f;
+      continue;
+    }
+    const int64_t y = a.targets[t];
+    s.pos[t] = first;
+    s.index[first] = (int)t;
+    s.target[first] = y >= 0 && y < a.V ? (int)y : -1;
+    s.coef[first] = w / top;
+    ++first;
+  }
+  if (threadIdx.x == 0) {
+    const double d = a.denominator > 0.f ? (double)a.denominator : sum != 0 ? sum : 1.0;
+    s.head[0] = total;
+    reinterpret_cast<float*>(s.head)[1] = (float)((double)top / d);
+    reinterpret_cast<float*>(s.head)[2] = top;
+    *reinterpret_cast<double*>(s.head + 4) = d;
+  }
+}
+
+// the live rows of x, one after the other, in whole chunks of 16 bytes with zeros after the last element
+template <typename T>
+__global__ __launch_bounds__(256) void ce_gather_kernel(const T* x, int64_t ld, T* to, const int* live, const int* index, int64_t C, uint32_t chunks) {
+  constexpr int kE = 16 / (int)sizeof(T);
+  const int64_t total = (int64_t)*live * chunks;
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * 256) {
+    const int64_t row = at / chunks, k = at % chunks * kE;
+    const T* const p = x + index[row] * ld + k;
+    u32x4 v = {0, 0, 0, 0};
+    if (k + kE <= C) {
+      __builtin_memcpy(&v, p, 16);
+    } else {
+      T e[kE];
+#pragma unroll
+      for (int j = 0; j < kE; ++j) e[j] = k + j < C ? p[j] : (T)0;
+      __builtin_memcpy(&v, e, 16);
+    }
+    reinterpret_cast<u32x4*>(to)[at] = v;
+  }
+}
+
+// A row's parts to its sums, and its log probability, put together in fp64
+// (log sum = e log 2 + log m with m around 1: the fp32 part stays below 0.35):
+// a wave for each row.
+__global__ __launch_bounds__(256) void ce_rows_kernel(const State s, const float2* part, const float* at_target, int64_t tiles, float* logp,
+                                                      double* terms) {
+  const int lane = threadIdx.x % kWave;
+  const int64_t rows = *s.head;
+  for (int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave; r < rows; r += (int64_t)gridDim.x * 4) {
+    float top = -__builtin_inff();
+    for (int64_t k = lane; k < tiles; k += kWave) top = fmaxf(top, part[r * tiles + k].x);
+    top = group_max<kWave>(top);
+    const float base = ce::base_of(top);
+    float sum = 0.f;
+    for (int64_t k = lane; k < tiles; k += kWave) {
+      const float2 one = part[r * tiles + k];
+      sum += one.y * expf(one.x - base);
+    }
+    sum = wave_sum(sum);
+    if (lane != 0) continue;
+    const float z = s.target[r] < 0 ? __builtin_nanf("") : at_target[r];
+    int e;
+    float m = frexpf(sum, &e);
+    if (m < 0.70710678f) m *= 2.f, --e;
+    const double lp = (double)z - (double)top - ((double)e * 0.6931471805599453 + (double)logf(m));
+    s.top[r] = top;
+    s.inv[r] = 1.f / sum;
+    logp[s.index[r]] = (float)lp;
+    terms[r] = (double)s.coef[r] * lp;
+  }
+}
+
+// loss = -(largest weight / D) sum of the terms: one workgroup, a fixed order
+__global__ __launch_bounds__(kOne) void ce_loss_kernel(const State s, const double* terms, float* loss) {
+  __shared__ double lds[kOne / kWave];
+  const int rows = *s.head;
+  double sum = 0;
+#pragma unroll 8
+  for (int r = threadIdx.x; r < rows; r += kOne) sum += terms[r];
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+  if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = sum;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  sum = 0;
+#pragma unroll
+  for (int w = 0; w < kOne / kWave; ++w) sum += lds[w];
+  loss[0] = rows == 0 ? 0.f : (float)(-sum * (double)reinterpret_cast<float*>(s.head)[2] / *reinterpret_cast<double*>(s.head + 4));
+}
+
+// dx of every token from the live ones' sums, scaled: zeros for the others
+template <typename T>
+__global__ __launch_bounds__(256) void ce_scatter_kernel(const float* sums, const State s, const float* dloss, float scale, T* dx, int64_t tokens,
+                                                         int64_t C, uint32_t groups) {
+  constexpr int V = 8;
+  const float by = reinterpret_cast<const float*>(s.head)[1] * (dloss != nullptr ? dloss[0] : 1.f) * scale;
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < tokens * groups; at += (int64_t)gridDim.x * 256) {
+    const int64_t t = at / groups, n = at % groups * V;
+    const int left = (int)min((int64_t)V, C - n), pos = s.pos[t];
+    float z[V] = {};
+    if (pos >= 0) {
+      if (left == V) gemm::take<true>(sums + pos * C + n, z, V);
+      else gemm::take<false>(sums + pos * C + n, z, left);
+#pragma unroll
+      for (int k = 0; k < V; ++k) z[k] *= by;
+    }
+    if (left == V) gemm::put<true>(dx + t * C + n, z, V);
+    else gemm::put<false>(dx + t * C + n, z, left);
+  }
+}
+
+struct FwdPlan {
+  Cut cut;
+  int64_t tiles;
+  size_t x, w, part, at_target, total;  // bytes; terms come last
+};
+
+FwdPlan plan_fwd(const mhc_linear_ce_args& a) {
+  constexpr int kBn[] = {256, 256, 128, 128, 64};
+  FwdPlan p;
+  p.cut = gemm::cut_of(a.T, a.V, a.C, a.dtype, true, true, 1);
+  p.tiles = ceil_div(a.V, kBn[p.cut.tile]);
+  p.x = up256((size_t)(a.T * padded(a.C, a.dtype)) * gemm::elem_bytes(a.dtype));
+  p.w = gemm::pack_bytes(a.w, a.V, a.ldw, a.C, a.dtype);
+  p.part = up256((size_t)(a.T * p.tiles) * sizeof(float2));
+  p.at_target = up256((size_t)a.T * sizeof(float));
+  p.total = p.x + p.w + p.part + p.at_target + (size_t)a.T * sizeof(double);
+  return p;
+}
+
+struct BwdPlan {
+  int64_t piece;                        // columns of the vocabulary
+  Cut dz, dx, dw;
+  size_t x, w, of_dz, sums, part, total;  // bytes
+};
+
+BwdPlan plan_bwd(const mhc_linear_ce_args& a, bool dx, bool dw) {
+  BwdPlan p = {};
+  const int64_t e = gemm::elem_bytes(a.dtype), pieces = std::max<int64_t>(1, ceil_div(a.T * a.V * e, kPieceBytes));
+  p.piece = std::min(a.V, ceil_div(ceil_div(a.V, pieces), 256) * 256);
+  p.dz = gemm::cut_of(a.T, p.piece, a.C, a.dtype, true, true, 1);
+  if (dx) p.dx = gemm::cut_of(a.T, a.C, p.piece, a.dtype, true, false);
+  if (dw) p.dw = gemm::cut_of(p.piece, a.C, a.T, a.dtype, false, false);
+  p.x = up256((size_t)(a.T * padded(a.C, a.dtype) * e));
+  p.w = gemm::pack_bytes(a.w, a.V, a.ldw, a.C, a.dtype);
+  p.of_dz = up256((size_t)(a.T * padded(p.piece, a.dtype) * e));
+  if (dx) p.sums = up256((size_t)(a.T * a.C) * sizeof(float));
+  p.part = std::max(dx ? gemm::part_bytes(p.dx, a.T, a.C) : 0, dw ? gemm::part_bytes(p.dw, p.piece, a.C) : 0);
+  p.total = p.x + p.w + p.of_dz + p.sums + p.part;
+  return p;
+}
+
+int run_gather(const mhc_linear_ce_args& a, const State& st, void* to, hipStream_t s) {
+  const uint32_t chunks = (uint32_t)(padded(a.C, a.dtype) * gemm::elem_bytes(a.dtype) / 16);
+  const dim3 grid((unsigned)std::min(ceil_div(a.T * chunks, 256), (int64_t)device_cu_count() * 16));
+  if (a.dtype == kF32)
+    hipLaunchKernelGGL((ce_gather_kernel<float>), grid, dim3(256), 0, s, static_cast<const float*>(a.x), a.ldx, static_cast<float*>(to),
+                       (const int*)st.head, (const int*)st.index, a.C, chunks);
+  else
+    hipLaunchKernelGGL((ce_gather_kernel<uint16_t>), grid, dim3(256), 0, s, static_cast<const uint16_t*>(a.x), a.ldx, static_cast<uint16_t*>(to),
+                       (const int*)st.head, (const int*)st.index, a.C, chunks);
+  MHC_CHECK_LAUNCH("ce_gather_kernel");
+  return MHC_OK;
+}
+
+template <typename T>
+int run_scatter(const mhc_linear_ce_args& a, const float* sums, const State& st, const float* dloss, float scale, void* dx, hipStream_t s) {
+  const uint32_t groups = (uint32_t)ceil_div(a.C, 8);
+  const dim3 grid((unsigned)std::min(ceil_div(a.T * groups, 256), (int64_t)device_cu_count() * 16));
+  hipLaunchKernelGGL((ce_scatter_kernel<T>), grid, dim3(256), 0, s, sums, st, dloss, scale * (1.f / ce::kDzUnit<T>), static_cast<T*>(dx), a.T, a.C,
+                     groups);
+  MHC_CHECK_LAUNCH("ce_scatter_kernel");
+  return MHC_OK;
+}
+
+int check_args(const mhc_linear_ce_args* a) {
+  MHC_CHECK_ARG(a != nullptr, "null pointer: args");
+  MHC_CHECK_ARG(a->T >= 0 && a->V >= 1 && a->C >= 1, "T must be >= 0, V and C >= 1 (got %lld, %lld, %lld)", (long long)a->T, (long long)a->V,
+                (long long)a->C);
+  MHC_CHECK_ARG(a->T < ((int64_t)1 << 28) && a->V < ((int64_t)1 << 22) && a->C < ((int64_t)1 << 22),
+                "T must be below 2^28, V and C below 2^22 (got %lld, %lld, %lld)", (long long)a->T, (long long)a->V, (long long)a->C);
+  MHC_CHECK_ARG(a->dtype == kF32 || a->dtype == kBF16 || a->dtype == kF16, "unsupported dtype %d", a->dtype);
+  MHC_CHECK_ARG(a->denominator >= 0, "denominator must be >= 0");
+  if (a->T == 0) return MHC_OK;
+  MHC_CHECK_ARG(a->x && a->w && a->targets, "null pointer");
+  MHC_CHECK_ARG((a->ldx >= a->C || a->T == 1) && (a->ldw >= a->C || a->V == 1), "ldx and ldw must be at least C");
+  MHC_CHECK_ARG(a->weights == nullptr || a->weights_dtype == MHC_DTYPE_F32 || a->weights_dtype == MHC_DTYPE_U8, "weights must be fp32 or bytes");
+  return MHC_OK;
+}
+
+}  // namespace
+}  // namespace mhc
+
+extern "C" size_t mhc_linear_ce_state_bytes(int64_t T) { return T < 0 ? 0 : mhc::ce::State::bytes(T); }
+
+extern "C" size_t mhc_linear_ce_fwd_workspace_bytes(const mhc_linear_ce_args* a) {
+  if (a == nullptr || a->T <= 0 || a->V <= 0 || a->C <= 0) return 0;
+  return mhc::plan_fwd(*a).total;
+}
+
+extern "C" int mhc_linear_ce_fwd(const mhc_linear_ce_args* args, float* loss, float* logp, void* state, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
+  using namespace mhc;
+  clear_error();
+  if (const int rc = check_args(args)) return rc;
+  const mhc_linear_ce_args& a = *args;
+  MHC_CHECK_ARG(loss != nullptr && state != nullptr && (logp != nullptr || a.T == 0), "null pointer");
+  MHC_CHECK_ARG(aligned(state, 16) && aligned(workspace, 16), "state and workspace must be 16-byte aligned");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const State st(state, a.T);
+  FwdPlan p = {};
+  if (a.T > 0) p = plan_fwd(a);
+  MHC_CHECK_ARG(workspace_bytes >= p.total && (p.total == 0 || workspace != nullptr), "workspace too small");
+  hipLaunchKernelGGL(ce_live_kernel, dim3(1), dim3(kOne), 0, s, a, logp, st);
+  MHC_CHECK_LAUNCH("ce_live_kernel");
+  char* ws = static_cast<char*>(workspace);
+  double* terms = nullptr;
+  if (a.T > 0) {
+    char* const x = ws;
+    ws += p.x;
+    if (const int rc = run_gather(a, st, x, s)) return rc;
+    const int64_t wide = padded(a.C, a.dtype);
+    Product q = {Operand{x, wide, wide}, {}, a.T, a.V, a.C, {}, 1, 0};
+    if (const int rc = gemm::operand(q.b, a.w, a.V, a.ldw, a.C, a.dtype, ws, s)) return rc;
+    float2* const part = reinterpret_cast<float2*>(ws);
+    float* const at_target = reinterpret_cast<float*>(ws + p.part);
+    terms = reinterpret_cast<double*>(ws + p.part + p.at_target);
+    const auto run = a.dtype == kF32 ? ce::run_sums_f32 : a.dtype == kBF16 ? ce::run_sums_bf16 : ce::run_sums_f16;
+    if (const int rc = run(q, p.cut, st.head, st.target, part, at_target, s)) return rc;
+    hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)std::min(ceil_div(a.T, 4), kMaxGrid)), dim3(256), 0, s, st, (const float2*)part,
+                       (const float*)at_target, p.tiles, logp, terms);
+    MHC_CHECK_LAUNCH("ce_rows_kernel");
+  }
+  hipLaunchKernelGGL(ce_loss_kernel, dim3(1), dim3(kOne), 0, s, st, (const double*)terms, loss);
+  MHC_CHECK_LAUNCH("ce_loss_kernel");
+  return MHC_OK;
+}
+
+extern "C" size_t mhc_linear_ce_bwd_workspace_bytes(const mhc_linear_ce_args* a, int want_dx, int want_dw) {
+  if (a == nullptr || a->T <= 0 || a->V <= 0 || a->C <= 0) return 0;
+  return mhc::plan_bwd(*a, want_dx != 0, want_dw != 0).total;
+}
+
+extern "C" int mhc_linear_ce_bwd(const mhc_linear_ce_args* args, const void* state, const float* dloss, float grad_scale, void* dx, void* dw,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace mhc;
+  clear_error();
+  if (const int rc = check_args(args)) return rc;
+  const mhc_linear_ce_args& a = *args;
+  MHC_CHECK_ARG(a.T > 0, "T must be > 0");
+  MHC_CHECK_ARG(state != nullptr, "null pointer");
+  MHC_CHECK_ARG(aligned(state, 16) && aligned(workspace, 16), "state and workspace must be 16-byte aligned");
+  if (dx == nullptr && dw == nullptr) return MHC_OK;
+  const BwdPlan p = plan_bwd(a, dx != nullptr, dw != nullptr);
+  MHC_CHECK_ARG(workspace_bytes >= p.total && workspace != nullptr, "workspace too small");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const State st(const_cast<void*>(state), a.T);
+  const int64_t e = gemm::elem_bytes(a.dtype), wide = padded(a.C, a.dtype);
+  char* ws = static_cast<char*>(workspace);
+  const Operand x = {ws, wide, wide};
+  if (const int rc = run_gather(a, st, ws, s)) return rc;
+  ws += p.x;
+  Operand w;
+  if (const int rc = gemm::operand(w, a.w, a.V, a.ldw, a.C, a.dtype, ws, s)) return rc;
+  char* const dz = ws;
+  float* const sums = reinterpret_cast<float*>(dz + p.of_dz);
+  float* const part = reinterpret_cast<float*>(dz + p.of_dz + p.sums);
+  const float* const unit = reinterpret_cast<const float*>(st.head) + 1;
+  const float lift = a.dtype == kF16 ? ce::kDzUnit<_Float16> : 1.f;
+  const auto run_dz = a.dtype == kF32 ? ce::run_dz_f32 : a.dtype == kBF16 ? ce::run_dz_bf16 : ce::run_dz_f16;
+  const auto run_dx = a.dtype == kF32 ? ce::run_dx_f32 : a.dtype == kBF16 ? ce::run_dx_bf16 : ce::run_dx_f16;
+  const auto run_dw = a.dtype == kF32 ? ce::run_dw_f32 : a.dtype == kBF16 ? ce::run_dw_bf16 : ce::run_dw_f16;
+  for (int64_t v0 = 0; v0 < a.V; v0 += p.piece) {
+    const int64_t n = std::min(p.piece, a.V - v0), pitch = padded(n, a.dtype);
+    const Operand piece = {static_cast<const char*>(w.p) + v0 * w.ld * e, w.ld, w.width};
+    const Operand d = {dz, pitch, pitch};
+    const Product pz = {x, piece, a.T, n, a.C, Epilogue{nullptr, nullptr, dz, nullptr, MHC_ACT_NONE, a.dtype == kF32}, 1, 0};
+    if (const int rc = run_dz(pz, p.dz, st.head, pitch, Gradient{st.target, st.coef, st.top, st.inv, v0, lift}, s)) return rc;
+    if (dx != nullptr) {
+      const Product px = {d, piece, a.T, a.C, n, Epilogue{nullptr, v0 > 0 ? sums : nullptr, sums, nullptr, MHC_ACT_NONE, 1}, 1, 0};
+      if (const int rc = run_dx(px, p.dx, st.head, part, s)) return rc;
+    }
+    if (dw != nullptr) {
+      char* const out = static_cast<char*>(dw) + v0 * a.C * e;
+      const Product pw = {d, x, n, a.C, a.T, Epilogue{nullptr, nullptr, out, nullptr, MHC_ACT_NONE, a.dtype == kF32}, 1, 0};
+      if (const int rc = run_dw(pw, p.dw, st.head, ScaledBy{unit, dloss, grad_scale / lift}, part, s)) return rc;
+    }
+  }
+  if (dx == nullptr) return MHC_OK;
+  if (a.dtype == kF32) return run_scatter<float>(a, sums, st, dloss, grad_scale, dx, s);
+  if (a.dtype == kBF16) return run_scatter<__bf16>(a, sums, st, dloss, grad_scale, dx, s);
+  return run_scatter<_Float16>(a, sums, st, dloss, grad_scale, dx, s);
+}

@@ -4,13 +4,18 @@
 // step it also stores d = act'(z), so that the backward needs neither z nor
 // an exponential: dz = dout d is one streaming pass, which also forms db from
 // the unrounded dz, and dx = dz W and dW = dz^T x are two more products.
-#include "mhc_gemm.hpp"
+#include "mhc_operand.hpp"
 
 namespace mhc {
 namespace {
 
+using gemm::operand;
 using gemm::Operand;
+using gemm::pack_bytes;
+using gemm::padded;
+using gemm::part_bytes;
 using gemm::Product;
+using gemm::up256;
 
 constexpr int kDzCols = 64 * 8;   // columns of a workgroup of dz_kernel: eight for each lane of a wave
 
@@ -73,73 +78,12 @@ __global__ __launch_bounds__(256) void db_kernel(const float* part, T* db, int64
   gemm::sum_columns<256>(lds, part, db, rows, N, blockIdx.x);
 }
 
-// rows of `width` elements, `ld` apart, into rows of whole chunks of 16 bytes, with zeros after the last element
-template <typename T>
-__global__ __launch_bounds__(256) void pack_kernel(const T* src, int64_t ld, T* dst, int64_t rows, int64_t width, int64_t chunks) {
-  constexpr int kE = 16 / (int)sizeof(T);
-  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < rows * chunks; at += (int64_t)gridDim.x * 256) {
-    const int64_t row = at / chunks, k = at % chunks * kE;
-    const T* const p = src + row * ld + k;
-    u32x4 v = {0, 0, 0, 0};
-    if (k + kE <= width) {
-      __builtin_memcpy(&v, p, 16);
-    } else {
-      T e[kE];
-#pragma unroll
-      for (int j = 0; j < kE; ++j) e[j] = k + j < width ? p[j] : (T)0;
-      __builtin_memcpy(&v, e, 16);
-    }
-    reinterpret_cast<u32x4*>(dst)[at] = v;
-  }
-}
-
-int elem_bytes(int dtype) { return dtype == kF32 ? 4 : 2; }
-
 // ws: part_bytes of the product
 int run_product(const Product& p, bool a_k, bool b_k, const gemm::Cut& c, int dtype, char* ws, hipStream_t s) {
   float* const part = reinterpret_cast<float*>(ws);
   if (dtype == kF32) return gemm::run_product_f32(p, a_k, b_k, c, part, s);
   if (dtype == kBF16) return gemm::run_product_bf16(p, a_k, b_k, c, part, s);
   return gemm::run_product_f16(p, a_k, b_k, c, part, s);
-}
-
-// bytes of the sums of an M x N product whose reduction is split
-size_t part_bytes(const gemm::Cut& c, int64_t M, int64_t N) { return c.splits > 1 ? (size_t)(c.splits * M * N) * sizeof(float) : 0; }
-
-size_t up256(size_t b) { return (b + 255) / 256 * 256; }
-
-// a row's length in a copy: a multiple of eight
-int64_t padded(int64_t width) { return (width + 7) / 8 * 8; }
-
-// bytes of an operand's copy in rows of whole chunks; 0: it is read as it is
-size_t pack_bytes(const void* p, int64_t rows, int64_t ld, int64_t width, int dtype) {
-  if (gemm::in_words(p, ld, width, elem_bytes(dtype))) return 0;
-  return up256((size_t)(rows * padded(width)) * elem_bytes(dtype));
-}
-
-template <typename T>
-int run_pack(const void* p, int64_t ld, void* to, int64_t rows, int64_t width, int64_t wide, hipStream_t s) {
-  const int64_t chunks = wide * (int64_t)sizeof(T) / 16;
-  const int64_t blocks = std::min(ceil_div(rows * chunks, 256), (int64_t)device_cu_count() * 16);
-  hipLaunchKernelGGL((pack_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, s, static_cast<const T*>(p), ld,
-                     static_cast<T*>(to), rows, width, chunks);
-  MHC_CHECK_LAUNCH("pack_kernel");
-  return MHC_OK;
-}
-
-// The operand, copied to `ws` first (which moves on) where its rows are no whole words.
-int operand(Operand& o, const void* p, int64_t rows, int64_t ld, int64_t width, int dtype, char*& ws, hipStream_t s) {
-  const size_t bytes = pack_bytes(p, rows, ld, width, dtype);
-  if (bytes == 0) {
-    o = Operand{p, ld, width};
-    return MHC_OK;
-  }
-  const int64_t wide = padded(width);
-  o = Operand{ws, wide, wide};
-  const int rc = dtype == kF32 ? run_pack<float>(p, ld, ws, rows, width, wide, s)
-                               : run_pack<uint16_t>(p, ld, ws, rows, width, wide, s);
-  ws += bytes;
-  return rc;
 }
 
 struct BwdPlan {
@@ -150,8 +94,8 @@ struct BwdPlan {
 BwdPlan plan_bwd(const void* dout, int dout_dtype, bool dact, const void* x, int64_t ldx, const void* w, int64_t ldw, bool dx, bool dw,
                  bool db, int64_t M, int64_t N, int64_t K, int dtype) {
   BwdPlan b = {};
-  if ((dx || dw) && (dact || dout_dtype != dtype || !gemm::in_words(dout, N, N, elem_bytes(dtype))))
-    b.dz = up256((size_t)(M * padded(N)) * elem_bytes(dtype));
+  if ((dx || dw) && (dact || dout_dtype != dtype || !gemm::in_words(dout, N, N, gemm::elem_bytes(dtype))))
+    b.dz = up256((size_t)(M * padded(N, dtype)) * gemm::elem_bytes(dtype));
   if (db) b.part = up256((size_t)(ceil_div(M, dz_rows(M, N)) * N) * sizeof(float));
   if (dx) b.w = pack_bytes(w, N, ldw, K, dtype);
   if (dw) b.x = pack_bytes(x, M, ldx, K, dtype);
@@ -195,8 +139,8 @@ int check_shape(int64_t M, int64_t N, int64_t K, int dtype) {
 extern "C" size_t mhc_linear_act_fwd_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M,
                                                      int64_t N, int64_t K, int dtype) {
   if (M <= 0 || N <= 0 || K <= 0 || mhc::gemm::few_rows(x, ldx, w, ldw, M, N, K, dtype)) return 0;
-  return mhc::pack_bytes(x, M, ldx, K, dtype) + mhc::pack_bytes(w, N, ldw, K, dtype) +
-         mhc::part_bytes(mhc::gemm::cut_of(M, N, K, dtype, true, true), M, N);
+  return mhc::gemm::pack_bytes(x, M, ldx, K, dtype) + mhc::gemm::pack_bytes(w, N, ldw, K, dtype) +
+         mhc::gemm::part_bytes(mhc::gemm::cut_of(M, N, K, dtype, true, true), M, N);
 }
 
 extern "C" int mhc_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
@@ -257,17 +201,17 @@ extern "C" int mhc_linear_act_bwd(const void* dout, int dout_dtype, const void* 
   if (dz != nullptr || db != nullptr) {
     void* const sum = b.cut.together ? nullptr : db;  // (else by the products' launch)
     int rc;
-    if (dtype == kF32) rc = run_dz<float, float>(dout, dact, dz, padded(N), part, sum, M, N, s);
+    if (dtype == kF32) rc = run_dz<float, float>(dout, dact, dz, padded(N, dtype), part, sum, M, N, s);
     else if (dtype == kBF16)
-      rc = dout_dtype == kF32 ? run_dz<__bf16, float>(dout, dact, dz, padded(N), part, sum, M, N, s)
-                              : run_dz<__bf16, __bf16>(dout, dact, dz, padded(N), part, sum, M, N, s);
+      rc = dout_dtype == kF32 ? run_dz<__bf16, float>(dout, dact, dz, padded(N, dtype), part, sum, M, N, s)
+                              : run_dz<__bf16, __bf16>(dout, dact, dz, padded(N, dtype), part, sum, M, N, s);
     else
-      rc = dout_dtype == kF32 ? run_dz<_Float16, float>(dout, dact, dz, padded(N), part, sum, M, N, s)
-                              : run_dz<_Float16, _Float16>(dout, dact, dz, padded(N), part, sum, M, N, s);
+      rc = dout_dtype == kF32 ? run_dz<_Float16, float>(dout, dact, dz, padded(N, dtype), part, sum, M, N, s)
+                              : run_dz<_Float16, _Float16>(dout, dact, dz, padded(N, dtype), part, sum, M, N, s);
     if (rc != MHC_OK) return rc;
   }
   ws += b.dz + b.part;
-  const Operand g = dz != nullptr ? Operand{dz, padded(N), padded(N)} : Operand{dout, N, N};
+  const Operand g = dz != nullptr ? Operand{dz, padded(N, dtype), padded(N, dtype)} : Operand{dout, N, N};
   // dx[m, k] = sum_n dz[m, n] W[n, k],  dw[n, k] = sum_m dz[m, n] x[m, k]
   Product px = {g, {}, M, K, N, gemm::Epilogue{nullptr, nullptr, dx, nullptr, MHC_ACT_NONE, dtype == kF32}, 1, 0};
   Product pw = {g, {}, N, K, M, gemm::Epilogue{nullptr, nullptr, dw, nullptr, MHC_ACT_NONE, dtype == kF32}, 1, 0};

@@ -1,0 +1,186 @@
+// linear_int8: out = act(xs ws (x W^T) + bias) + residual for int8 codes x and
+// W with a scale for each row (of tokens, and of channels).
+//
+// The products' sums are whole numbers in 32 bits, exact: a term is at most
+// 2^14, and there are fewer than 2^17 of them.  They are scaled in registers
+// on their way to the epilogue, each of the two scales and the sum's way to
+// fp32 one rounding.
+#include "mhc_operand.hpp"
+
+namespace mhc {
+namespace {
+
+using gemm::Cut;
+using gemm::Epilogue;
+using gemm::Operand;
+using gemm::Product;
+
+constexpr int64_t kMaxK = 1 << 17;
+
+struct Scales {
+  const float* x;     // [M]
+  const float* w;     // [N]
+  const float* bias;  // [N], or NULL
+};
+
+// four values from column n on, of those before N; zeros after
+MHC_DEV f32x4 four_of(const float* p, int64_t n, int64_t N) {
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (n + 4 <= N) {
+    __builtin_memcpy(&v, p + n, 16);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (n + k < N) v[k] = p[n + k];
+  }
+  return v;
+}
+
+// int32 sums to fp32 values, with the bias (in the first of a reduction's parts)
+struct Scaled {
+  Scales s;
+  template <typename P, int JM, int JN>
+  MHC_DEV void operator()(const Product& p, const P& at, int split, f32x4 (&acc)[JN][JM]) const {
+    const int64_t m0 = at.m0 + at.wm + at.lane % 16, n0 = at.n0 + at.wn + at.lane / 16 * 4;
+    float x[JM];
+#pragma unroll
+    for (int j = 0; j < JM; ++j) x[j] = s.x[min(m0 + j * 16, p.M - 1)];
+    const bool biased = s.bias != nullptr && split == 0;
+#pragma unroll
+    for (int i = 0; i < JN; ++i) {
+      const f32x4 w = four_of(s.w, n0 + i * 16, p.N);
+      f32x4 b = {0.f, 0.f, 0.f, 0.f};
+      if (biased) b = four_of(s.bias, n0 + i * 16, p.N);
+#pragma unroll
+      for (int j = 0; j < JM; ++j) {
+        const i32x4 sum = __builtin_bit_cast(i32x4, acc[i][j]);
+        f32x4 v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = fmaf((float)sum[k] * x[j], w[k], b[k]);
+        acc[i][j] = v;
+      }
+    }
+  }
+  using i32x4 = gemm::i32x4;
+};
+
+template <typename O, int BM, int BN, int WM, int WN, int NS>
+__global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(const Product p, const Scaled then) {
+  __shared__ __attribute__((aligned(1024))) char smem[gemm::TileBytes<int8_t, BM, BN, WM, WN, NS>::kAll];
+  gemm::run_tile<int8_t, true, true, BM, BN, WM, WN, NS, O>(p, smem, blockIdx.x, (int)blockIdx.y, p.M * p.N, p.N, then);
+}
+
+// Up to 64 rows: as few_rows_kernel, with the waves' sums joined as whole numbers.
+template <typename O, int MT, int NT, int NS>
+__global__ __launch_bounds__(64 * gemm::kFewWaves) void int8_few_rows_kernel(const Operand x, const Operand w, int M, int64_t N, int K,
+                                                                            const Scales s, const Epilogue e) {
+  constexpr int kN = 16 * NT, kSums = MT * 16 * kN;
+  __shared__ __attribute__((aligned(1024))) char smem[std::max(gemm::kFewBytes<MT, NT, NS>, gemm::kFewWaves * kSums * 4)];
+  const int64_t n0 = (int64_t)blockIdx.x * kN;
+  f32x4 acc[NT][MT] = {};
+  gemm::sum_few_rows<int8_t, MT, NT, NS>(x, w, M, n0, N, K, smem, acc);
+  int* const sums = reinterpret_cast<int*>(smem);
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(sums + ((wave * MT + j) * 16 + lane % 16) * kN + i * 16 + lane / 16 * 4) = acc[i][j];
+  __syncthreads();
+  for (int at = threadIdx.x; at < kSums; at += 64 * gemm::kFewWaves) {
+    const int m = at / kN;
+    const int64_t n = n0 + at % kN;
+    int sum = 0;
+#pragma unroll
+    for (int v = 0; v < gemm::kFewWaves; ++v) sum += sums[v * kSums + at];
+    if (m < M && n < N) {
+      const float none[1] = {};
+      float z[1][1] = {{fmaf((float)sum * s.x[m], s.w[n], s.bias != nullptr ? s.bias[n] : 0.f)}}, residual[1][1];
+      gemm::residual_of<O, true>(e, m, 0, M, n, N, 1, residual);
+      gemm::finish<O, true>(e, m, 0, M, n, N, 1, z, none, residual);
+    }
+  }
+}
+
+template <typename O, int BM, int BN, int WM, int WN, int NS>
+int launch_tile(const Product& p, const Scaled& then, hipStream_t s) {
+  const dim3 grid((unsigned)(ceil_div(p.M, BM) * ceil_div(p.N, BN)), (unsigned)p.splits), block(64 * WM * WN);
+  hipLaunchKernelGGL((int8_tile_kernel<O, BM, BN, WM, WN, NS>), grid, block, 0, s, p, then);
+  MHC_CHECK_LAUNCH("int8_tile_kernel");
+  return MHC_OK;
+}
+
+template <typename O>
+int run_tiles(Product p, const Cut& c, const Scaled& then, float* part, hipStream_t s) {
+  const Epilogue e = p.e;
+  p.splits = c.splits;
+  p.kper = c.kper;
+  if (c.splits > 1) p.e = Epilogue{nullptr, nullptr, part, nullptr, MHC_ACT_NONE, 1};
+  int rc;
+  switch (c.tile) {
+    case 0: rc = launch_tile<O, 256, 256, 2, 4, 2>(p, then, s); break;
+    case 1: rc = launch_tile<O, 128, 256, 2, 4, 2>(p, then, s); break;
+    case 2: rc = launch_tile<O, 128, 128, 4, 2, 2>(p, then, s); break;
+    case 3: rc = launch_tile<O, 64, 128, 4, 2, 3>(p, then, s); break;
+    default: rc = launch_tile<O, 64, 64, 4, 1, 3>(p, then, s); break;
+  }
+  if (rc != MHC_OK || c.splits == 1) return rc;
+  return gemm::launch_join<O>(e, part, c.splits, p.M, p.N, s);
+}
+
+template <typename O, int MT>
+int run_few(const Operand& x, const Operand& w, int64_t M, int64_t N, int64_t K, const Scales& scales, const Epilogue& e, hipStream_t s) {
+  hipLaunchKernelGGL((int8_few_rows_kernel<O, MT, 1, MT == 1 ? 2 : 1>), dim3((unsigned)ceil_div(N, 16)), dim3(64 * gemm::kFewWaves), 0, s, x, w,
+                     (int)M, N, (int)K, scales, e);
+  MHC_CHECK_LAUNCH("int8_few_rows_kernel");
+  return MHC_OK;
+}
+
+bool few_rows(int64_t M) { return M <= 64; }
+
+template <typename O>
+int run(const Product& p, const Scales& scales, float* part, hipStream_t s) {
+  if (few_rows(p.M)) {
+    if (p.M <= 16) return run_few<O, 1>(p.a, p.b, p.M, p.N, p.K, scales, p.e, s);
+    if (p.M <= 32) return run_few<O, 2>(p.a, p.b, p.M, p.N, p.K, scales, p.e, s);
+    return run_few<O, 4>(p.a, p.b, p.M, p.N, p.K, scales, p.e, s);
+  }
+  return run_tiles<O>(p, gemm::cut_of(p.M, p.N, p.K, kI8, true, true), Scaled{scales}, part, s);
+}
+
+}  // namespace
+}  // namespace mhc
+
+extern "C" size_t mhc_linear_int8_workspace_bytes(const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, int64_t M, int64_t N, int64_t K) {
+  using namespace mhc;
+  if (M <= 0 || N <= 0 || K <= 0 || K >= kMaxK) return 0;
+  return gemm::pack_bytes(x, M, ldx, K, kI8) + gemm::pack_bytes(w, N, ldw, K, kI8) +
+         (few_rows(M) ? 0 : gemm::part_bytes(gemm::cut_of(M, N, K, kI8, true, true), M, N));
+}
+
+extern "C" int mhc_linear_int8(const int8_t* x, int64_t ldx, const float* x_scales, const int8_t* w, int64_t ldw, const float* w_scales,
+                               const float* bias, const void* residual, void* out, int out_dtype, int act, int64_t M, int64_t N, int64_t K,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace mhc;
+  clear_error();
+  MHC_CHECK_ARG(M >= 0 && N >= 1 && K >= 1, "M must be >= 0, N and K >= 1 (got %lld, %lld, %lld)", (long long)M, (long long)N, (long long)K);
+  MHC_CHECK_ARG(M < ((int64_t)1 << 28) && N < ((int64_t)1 << 22), "M must be below 2^28, N below 2^22 (got %lld, %lld)", (long long)M, (long long)N);
+  MHC_CHECK_ARG(K < kMaxK, "K must be below 2^17, so that sums stay in 32 bits (got %lld)", (long long)K);
+  MHC_CHECK_ARG(out_dtype == kF32 || out_dtype == kBF16 || out_dtype == kF16, "unsupported out_dtype %d", out_dtype);
+  MHC_CHECK_ARG(act >= MHC_ACT_NONE && act <= MHC_ACT_SILU, "unknown activation %d", act);
+  if (M == 0) return MHC_OK;
+  MHC_CHECK_ARG(x && x_scales && w && w_scales && out, "null pointer");
+  MHC_CHECK_ARG((ldx >= K || M == 1) && (ldw >= K || N == 1), "ldx and ldw must be at least K");
+  MHC_CHECK_ARG(workspace_bytes >= mhc_linear_int8_workspace_bytes(x, ldx, w, ldw, M, N, K), "workspace too small");
+  MHC_CHECK_ARG(workspace_bytes == 0 || workspace != nullptr, "null workspace");
+  MHC_CHECK_ARG(aligned(workspace, 16), "workspace must be 16-byte aligned");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  Product p = {{}, {}, M, N, K, Epilogue{nullptr, residual, out, nullptr, act, out_dtype == kF32}, 1, 0};
+  if (const int rc = gemm::operand(p.a, x, M, ldx, K, kI8, ws, s)) return rc;
+  if (const int rc = gemm::operand(p.b, w, N, ldw, K, kI8, ws, s)) return rc;
+  const Scales scales = {x_scales, w_scales, bias};
+  float* const part = reinterpret_cast<float*>(ws);
+  if (out_dtype == kF32) return run<float>(p, scales, part, s);
+  if (out_dtype == kBF16) return run<__bf16>(p, scales, part, s);
+  return run<_Float16>(p, scales, part, s);
+}

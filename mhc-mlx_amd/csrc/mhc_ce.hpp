@@ -1,0 +1,262 @@
+// Products of linear_cross_entropy, whose rows of tokens are counted on the
+// device: logits' sums, their gradient, and that gradient's two products.
+#pragma once
+
+#include "mhc_gemm.hpp"
+
+namespace mhc {
+namespace ce {
+
+using gemm::Cut;
+using gemm::Epilogue;
+using gemm::Operand;
+using gemm::Product;
+
+// What the forward leaves for the backward, in words: the tokens that count
+// ("live"), in order, and what is known of each.
+struct State {
+  int* head;     // how many are live; then, as floats, the largest weight over D, and D
+  int* index;    // [T] their tokens
+  int* pos;      // [T] of each token: its place among them, or -1
+  int* target;   // [T] by place: -1 where it is no column
+  float* coef;   // [T] by place: weight / largest weight
+  float* top;    // [T] by place: largest logit
+  float* inv;    // [T] by place: 1 / sum of exp(logit - top)
+
+  static constexpr int kHead = 16;
+  static size_t bytes(int64_t T) { return (size_t)(kHead + 6 * T) * 4; }
+  State(void* p, int64_t T) {
+    head = static_cast<int*>(p);
+    index = head + kHead;
+    pos = index + T;
+    target = pos + T;
+    coef = reinterpret_cast<float*>(target + T);
+    top = coef + T;
+    inv = top + T;
+  }
+};
+
+// dz in fp16 is held times 2^14: a probability below 2^-14 would lose bits
+// there, and one of 2^-24 be 0.
+template <typename T> inline constexpr float kDzUnit = 1.f;
+template <> inline constexpr float kDzUnit<_Float16> = 0x1p14f;
+
+// Logits to dz = coef (softmax - [v = target]), zeros past the last column.
+struct Gradient {
+  const int* target;
+  const float *coef, *top, *inv;
+  int64_t v0;  // the vocabulary's index of the first column
+  float unit;
+
+  template <bool FAST, typename P, int JM, int JN>
+  MHC_DEV void apply(const Product& p, const P& at, f32x4 (&acc)[JN][JM]) const {
+    const int64_t m0 = at.m0 + at.wm + at.lane % 16, n0 = at.n0 + at.wn + at.lane / 16 * 4;
+#pragma unroll
+    for (int j = 0; j < JM; ++j) {
+      const int64_t m = min(m0 + j * 16, p.M - 1);
+      const int to = target[m];
+      const float c = to < 0 ? __builtin_nanf("") : coef[m] * unit, t = top[m], each = c * inv[m];
+      const int64_t mine = to < 0 ? -1 : to - v0 - n0;  // the target's place among the lane's columns
+#pragma unroll
+      for (int i = 0; i < JN; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float d = each * gemm::exp_of<FAST>(acc[i][j][k] - t) - (mine == i * 16 + k ? c : 0.f);
+          acc[i][j][k] = n0 + i * 16 + k < p.N ? d : 0.f;
+        }
+    }
+  }
+};
+
+template <bool FAST>
+struct GradientOf : Gradient {
+  template <typename P, int JM, int JN>
+  MHC_DEV void operator()(const Product& p, const P& at, int, f32x4 (&acc)[JN][JM]) const {
+    this->template apply<FAST>(p, at, acc);
+  }
+};
+
+// sums times a * b * c, a and b in memory (b may be NULL)
+struct ScaledBy {
+  const float *a, *b;
+  float c;
+  template <typename P, int JM, int JN>
+  MHC_DEV void operator()(const Product&, const P&, int, f32x4 (&acc)[JN][JM]) const {
+    const float s = a[0] * (b != nullptr ? b[0] : 1.f) * c;
+#pragma unroll
+    for (int i = 0; i < JN; ++i)
+#pragma unroll
+      for (int j = 0; j < JM; ++j) acc[i][j] *= s;
+  }
+};
+
+// The product with as many rows of tokens as there are: they are rows of the
+// outputs, or (AK false) what is summed over.  False: not this workgroup's.
+template <bool AK, int BM, int BN>
+MHC_DEV bool limit(Product& p, const int* live, uint32_t tile) {
+  const int64_t n = __builtin_amdgcn_readfirstlane(*live);
+  if constexpr (AK) {
+    p.M = min(p.M, n);
+    return tile < ceil_div(p.M, BM) * ceil_div(p.N, BN);
+  } else {
+    p.K = min(p.K, n);
+    return true;
+  }
+}
+
+template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS, typename Then>
+__global__ __launch_bounds__(64 * WM * WN) void live_tile_kernel(Product p, const int* live, int64_t width, const Then then) {
+  __shared__ __attribute__((aligned(1024))) char smem[gemm::TileBytes<T, BM, BN, WM, WN, NS>::kAll];
+  const int64_t part = p.M * p.N;
+  if (!limit<AK, BM, BN>(p, live, blockIdx.x)) return;
+  gemm::run_tile<T, AK, BK, BM, BN, WM, WN, NS, T>(p, smem, blockIdx.x, (int)blockIdx.y, part, width, then);
+}
+
+// exp(x - top) below `top`; a part of a row that is -inf alone has no top, and -inf - -inf would be NaN
+MHC_DEV float base_of(float top) { return top == -__builtin_inff() ? 0.f : top; }
+
+// A tile of logits, of which only each row's largest and the sum of
+// exp(logit - largest) are kept, and the target's: to part[row][column of
+// tiles] and at_target[row].
+template <typename T, int BM, int BN, int WM, int WN, int NS>
+__global__ __launch_bounds__(64 * WM * WN) void sums_tile_kernel(Product p, const int* live, const int* target, float2* part, float* at_target) {
+  __shared__ __attribute__((aligned(1024))) char smem[NS * (BM + BN) * 128];
+  if (!limit<true, BM, BN>(p, live, blockIdx.x)) return;
+  constexpr int JM = BM / WM / 16, JN = BN / WN / 16, kThreads = 64 * WM * WN;
+  constexpr bool kFast = sizeof(T) == 2;
+  const gemm::Place<BM, BN, WM, WN> at(p, blockIdx.x, 0);
+  f32x4 acc[JN][JM] = {};
+  if constexpr (gemm::kSplit<T, BN>) gemm::sum_tile_split<true, true, BM, BN, WM, WN, NS>(p, at, smem, acc);
+  else gemm::sum_tile<T, true, true, BM, BN, WM, WN, NS>(p, at, smem, acc);
+  const int64_t m0 = at.m0 + at.wm + at.lane % 16, n0 = at.n0 + at.wn + at.lane / 16 * 4;
+  if (at.n0 + BN > p.N) {
+#pragma unroll
+    for (int i = 0; i < JN; ++i)
+#pragma unroll
+      for (int j = 0; j < JM; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (n0 + i * 16 + k >= p.N) acc[i][j][k] = -__builtin_inff();
+  }
+  __syncthreads();  // nobody reads the stages any more
+  float2* const of_waves = reinterpret_cast<float2*>(smem);  // [columns of waves][BM]
+#pragma unroll
+  for (int j = 0; j < JM; ++j) {
+    float top = acc[0][j][0];
+#pragma unroll
+    for (int i = 0; i < JN; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top = fmaxf(top, acc[i][j][k]);
+    top = xor_allreduce<16>(top, MaxOp{});
+    top = xor_allreduce<32>(top, MaxOp{});
+    const float base = base_of(top);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < JN; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum += gemm::exp_of<kFast>(acc[i][j][k] - base);
+    sum = xor_allreduce<16>(sum, SumOp{});
+    sum = xor_allreduce<32>(sum, SumOp{});
+    if (at.lane < 16) of_waves[at.wave % WN * BM + at.wm + j * 16 + at.lane] = float2{top, sum};
+    const int64_t m = m0 + j * 16;
+    const int mine = m < p.M ? target[m] - (int)n0 : -1;
+#pragma unroll
+    for (int i = 0; i < JN; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (mine == i * 16 + k) at_target[m] = acc[i][j][k];
+  }
+  __syncthreads();
+  const int64_t tiles = ceil_div(p.N, BN);
+  for (int r = threadIdx.x; r < BM; r += kThreads) {
+    if (at.m0 + r >= p.M) break;
+    float2 all = of_waves[r];
+#pragma unroll
+    for (int w = 1; w < WN; ++w) {
+      const float2 one = of_waves[w * BM + r];
+      const float top = fmaxf(all.x, one.x), base = base_of(top);
+      all.y = all.y * gemm::exp_of<kFast>(all.x - base) + one.y * gemm::exp_of<kFast>(one.x - base);
+      all.x = top;
+    }
+    part[(at.m0 + r) * tiles + at.n0 / BN] = all;
+  }
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int NS>
+int launch_sums(const Product& p, const int* live, const int* target, float2* part, float* at_target, hipStream_t s) {
+  hipLaunchKernelGGL((sums_tile_kernel<T, BM, BN, WM, WN, NS>), dim3((unsigned)(ceil_div(p.M, BM) * ceil_div(p.N, BN))), dim3(64 * WM * WN), 0, s,
+                     p, live, target, part, at_target);
+  MHC_CHECK_LAUNCH("sums_tile_kernel");
+  return MHC_OK;
+}
+
+template <typename T>
+int run_sums(Product p, const Cut& c, const int* live, const int* target, float2* part, float* at_target, hipStream_t s) {
+  using gemm::kRowWaves;
+  p.splits = 1;
+  p.kper = c.kper;
+  switch (c.tile) {
+    case 0: return launch_sums<T, 256, 256, 2, 4, 2>(p, live, target, part, at_target, s);
+    case 1: return launch_sums<T, 128, 256, 2, 4, 2>(p, live, target, part, at_target, s);
+    case 2: return launch_sums<T, 128, 128, kRowWaves<T>, 2, 2>(p, live, target, part, at_target, s);
+    case 3: return launch_sums<T, 64, 128, kRowWaves<T>, 2, 3>(p, live, target, part, at_target, s);
+    default: return launch_sums<T, 64, 64, 4, 1, 3>(p, live, target, part, at_target, s);
+  }
+}
+
+template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS, typename Then>
+int launch_live(const Product& p, const int* live, int64_t width, const Then& then, hipStream_t s) {
+  const dim3 grid((unsigned)(ceil_div(p.M, BM) * ceil_div(p.N, BN)), (unsigned)p.splits), block(64 * WM * WN);
+  hipLaunchKernelGGL((live_tile_kernel<T, AK, BK, BM, BN, WM, WN, NS, Then>), grid, block, 0, s, p, live, width, then);
+  MHC_CHECK_LAUNCH("live_tile_kernel");
+  return MHC_OK;
+}
+
+// width: of the outputs' rows; part: the sums of a reduction's parts, if it is split
+template <typename T, bool AK, bool BK, typename Then>
+int run_live(Product p, const Cut& c, const int* live, int64_t width, const Then& then, float* part, hipStream_t s) {
+  using gemm::kRowWaves;
+  const Epilogue e = p.e;
+  p.splits = c.splits;
+  p.kper = c.kper;
+  if (c.splits > 1) p.e = Epilogue{nullptr, nullptr, part, nullptr, MHC_ACT_NONE, 1};
+  int rc;
+  switch (c.tile) {
+    case 0: rc = launch_live<T, AK, BK, 256, 256, 2, 4, 2>(p, live, width, then, s); break;
+    case 1: rc = launch_live<T, AK, BK, 128, 256, 2, 4, 2>(p, live, width, then, s); break;
+    case 2: rc = launch_live<T, AK, BK, 128, 128, kRowWaves<T>, 2, 2>(p, live, width, then, s); break;
+    case 3: rc = launch_live<T, AK, BK, 64, 128, kRowWaves<T>, 2, 3>(p, live, width, then, s); break;
+    default: rc = launch_live<T, AK, BK, 64, 64, 4, 1, 3>(p, live, width, then, s); break;
+  }
+  if (rc != MHC_OK || c.splits == 1) return rc;
+  return gemm::launch_join<T>(e, part, c.splits, p.M, p.N, s);
+}
+
+#define MHC_CE_DECLARE(NAME)                                                                                                         \
+  int run_sums_##NAME(const Product& p, const Cut& c, const int* live, const int* target, float2* part, float* at_target, hipStream_t s); \
+  int run_dz_##NAME(const Product& p, const Cut& c, const int* live, int64_t width, const Gradient& g, hipStream_t s);                              \
+  int run_dx_##NAME(const Product& p, const Cut& c, const int* live, float* part, hipStream_t s);                                    \
+  int run_dw_##NAME(const Product& p, const Cut& c, const int* live, const ScaledBy& by, float* part, hipStream_t s);
+
+MHC_CE_DECLARE(f32)
+MHC_CE_DECLARE(bf16)
+MHC_CE_DECLARE(f16)
+
+// the functions above for a type, in a file of its own
+#define MHC_CE_DEFINE(NAME, T)                                                                                                       \
+  int run_sums_##NAME(const Product& p, const Cut& c, const int* live, const int* target, float2* part, float* at_target,            \
+                      hipStream_t s) {                                                                                               \
+    return run_sums<T>(p, c, live, target, part, at_target, s);                                                                      \
+  }                                                                                                                                  \
+  int run_dz_##NAME(const Product& p, const Cut& c, const int* live, int64_t width, const Gradient& g, hipStream_t s) {                             \
+    return run_live<T, true, true>(p, c, live, width, GradientOf<sizeof(T) == 2>{g}, nullptr, s);                                           \
+  }                                                                                                                                  \
+  int run_dx_##NAME(const Product& p, const Cut& c, const int* live, float* part, hipStream_t s) {                                   \
+    return run_live<T, true, false>(p, c, live, p.N, gemm::AsTheyAre{}, part, s);                                                         \
+  }                                                                                                                                  \
+  int run_dw_##NAME(const Product& p, const Cut& c, const int* live, const ScaledBy& by, float* part, hipStream_t s) {               \
+    return run_live<T, false, false>(p, c, live, p.N, by, part, s);                                                                       \
+  }
+
+}  // namespace ce
+}  // namespace mhc

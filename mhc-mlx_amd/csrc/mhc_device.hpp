@@ -25,7 +25,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 // Element type codes shared with the C ABI (include/mhc_hip.h).
-enum DType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
+enum DType : int { kF32 = 0, kBF16 = 1, kF16 = 2, kI8 = 4 };
 
 // --------------------------------------------------------------------------
 // scalar conversions

@@ -1,5 +1,5 @@
 // Matrix products out[m, n] = sum_k A(m, k) B(n, k) on MFMA with a fused
-// epilogue (gfx950), for fp32, bf16 and fp16 operands.
+// epilogue (gfx950), for fp32, bf16, fp16 and int8 operands.
 //
 // Each operand is either "k-major" (its k are contiguous: x and W of x W^T)
 // or not (its rows are k: W of dz W, and both operands of dz^T x).
@@ -16,6 +16,7 @@ namespace gemm {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));  // sixteen bytes that start at any element
 
 // --------------------------------------------------------------------------
@@ -260,7 +261,10 @@ MHC_DEV void finish(const Epilogue& e, int64_t m, int step, int64_t M, int64_t n
 // both operands agree.
 template <typename T>
 MHC_DEV f32x4 mfma16(const u32x4& a, const u32x4& b, f32x4 c) {
-  if constexpr (sizeof(T) == 4) {
+  if constexpr (sizeof(T) == 1) {  // (the sums are int32, and a lane's sixteen k go with those of its group)
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b),
+                                                                           __builtin_bit_cast(i32x4, c), 0, 0, 0));
+  } else if constexpr (sizeof(T) == 4) {
     // (the vectors are cast whole: a bit cast of one element of a vector takes its first)
     const f32x4 af = __builtin_bit_cast(f32x4, a), bf = __builtin_bit_cast(f32x4, b);
 #pragma unroll
@@ -800,23 +804,31 @@ struct TileBytes {
   static constexpr int kAll = kStages + (kSplit<T, BN> ? (kWords * kThreads + WM * WN) * 4 : 0);
 };
 
-// A tile of outputs, or (split) of one part of the reduction's sums.  Sums on
+// What becomes of a tile's sums before they are stored: nothing here.
+struct AsTheyAre {
+  template <typename P, int JM, int JN>
+  MHC_DEV void operator()(const Product&, const P&, int, f32x4 (&)[JN][JM]) const {}
+};
+
+// A tile of outputs, or (split) of one part of the reduction's sums, which
+// `then` changes; T: of the operands, O: of the epilogue.  Sums on
 // split values that come out infinite or as NaN are formed once more with fp32
 // instructions: their values or lifted sums were past the range (2^111, 2^95),
 // or had an infinity, whose parts make NaN of everything.  The other sums of the tile stay as they are, so that a row's
 // outputs do not depend on what other rows hold.
-template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
-MHC_DEV void run_tile(const Product& p, char* smem, uint32_t tile, int split) {
+template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS, typename O = T, typename Then = AsTheyAre>
+MHC_DEV void run_tile(const Product& p, char* smem, uint32_t tile, int split, int64_t part, int64_t width, const Then& then = {}) {
   using B = TileBytes<T, BM, BN, WM, WN, NS>;
   constexpr int kWaves = WM * WN, JM = BM / WM / 16, JN = BN / WN / 16;
   const Place<BM, BN, WM, WN> at(p, tile, split);
   const int64_t m0 = at.m0 + at.wm, n0 = at.n0 + at.wn;
   Epilogue e = p.e;
-  if (p.splits > 1) e.out = static_cast<float*>(e.out) + (int64_t)split * p.M * p.N;
+  if (p.splits > 1) e.out = static_cast<float*>(e.out) + split * part;
   f32x4 acc[JN][JM] = {};
   if constexpr (!kSplit<T, BN>) {
     sum_tile<T, AK, BK, BM, BN, WM, WN, NS>(p, at, smem, acc);
-    store_tile<T, JM, JN, kWaves, B::kStages>(e, smem, acc, m0, p.M, n0, p.N, at.wave, at.lane);
+    then(p, at, split, acc);
+    store_tile<O, JM, JN, kWaves, B::kStages>(e, smem, acc, m0, p.M, n0, width, at.wave, at.lane);
   } else {
     static_assert(B::kWords * 32 == JM * JN * 4);
     sum_tile_split<AK, BK, BM, BN, WM, WN, NS>(p, at, smem, acc);
@@ -857,7 +869,8 @@ MHC_DEV void run_tile(const Product& p, char* smem, uint32_t tile, int split) {
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) again |= found[w];
     again = __builtin_amdgcn_readfirstlane(again);
-    store_tile<T, JM, JN, kWaves, B::kStages>(e, smem, acc, m0, p.M, n0, p.N, at.wave, at.lane);
+    then(p, at, split, acc);
+    store_tile<O, JM, JN, kWaves, B::kStages>(e, smem, acc, m0, p.M, n0, width, at.wave, at.lane);
     if (!again) return;
 #pragma unroll
     for (int i = 0; i < JN; ++i)
@@ -867,6 +880,7 @@ MHC_DEV void run_tile(const Product& p, char* smem, uint32_t tile, int split) {
     Place<BM, BN, WM, WN> once_more = at;
     asm volatile("" : "+v"(once_more.lane), "+s"(once_more.wave));  // (or registers would hold places from the first sums to these)
     sum_tile<T, AK, BK, BM, BN, WM, WN, NS>(p, once_more, smem, acc);  // (it waits for the wave's stores, too)
+    then(p, once_more, split, acc);
     uint32_t mark[B::kWords] = {};
     if (mine) {
 #pragma unroll
@@ -881,14 +895,14 @@ MHC_DEV void run_tile(const Product& p, char* smem, uint32_t tile, int split) {
           const int bit = 4 * (i * JM + j) + k;
           if (!(mark[bit / 32] >> bit % 32 & 1)) acc[i][j][k] = __builtin_bit_cast(float, kKeep);
         }
-    store_tile<T, JM, JN, kWaves, B::kStages, true>(e, smem, acc, m0, p.M, n0, p.N, at.wave, at.lane);
+    store_tile<O, JM, JN, kWaves, B::kStages, true>(e, smem, acc, m0, p.M, n0, width, at.wave, at.lane);
   }
 }
 
 template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
 __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(const Product p) {
   __shared__ __attribute__((aligned(1024))) char smem[TileBytes<T, BM, BN, WM, WN, NS>::kAll];
-  run_tile<T, AK, BK, BM, BN, WM, WN, NS>(p, smem, blockIdx.x, (int)blockIdx.y);
+  run_tile<T, AK, BK, BM, BN, WM, WN, NS>(p, smem, blockIdx.x, (int)blockIdx.y, p.M * p.N, p.N);
 }
 
 // Column sums of fp32 rows: 32 columns a workgroup, each column in eight parts
@@ -930,10 +944,10 @@ __global__ __launch_bounds__(64 * WM * WN) void pair_kernel(const Pair p) {
   const uint32_t id = blockIdx.x;
   if (id - p.dx0 < p.dx_count) {
     const uint32_t at = id - p.dx0, tiles = p.dx_count / p.dx.splits;
-    run_tile<T, true, false, BM, BN, WM, WN, NS>(p.dx, smem, at % tiles, (int)(at / tiles));
+    run_tile<T, true, false, BM, BN, WM, WN, NS>(p.dx, smem, at % tiles, (int)(at / tiles), p.dx.M * p.dx.N, p.dx.N);
   } else if (id - p.dw0 < p.dw_count) {
     const uint32_t at = id - p.dw0, tiles = p.dw_count / p.dw.splits;
-    run_tile<T, false, false, BM, BN, WM, WN, NS>(p.dw, smem, at % tiles, (int)(at / tiles));
+    run_tile<T, false, false, BM, BN, WM, WN, NS>(p.dw, smem, at % tiles, (int)(at / tiles), p.dw.M * p.dw.N, p.dw.N);
   } else {
     sum_columns<64 * WM * WN>(reinterpret_cast<float(*)[kSumCols]>(smem), p.part, static_cast<T*>(p.db), p.part_rows, p.N,
                               id - p.dx_count - p.dw_count);
@@ -976,13 +990,15 @@ MHC_DEV void join_waves(const f32x4 (&acc)[NT][MT], float* sums, int M, int64_t 
   }
 }
 
+template <int MT, int NT, int NS>
+constexpr int kFewBytes = kFewWaves * NS * 2048 * (NT + MT);  // of LDS
+
+// a wave's sums, over its part of the k; the workgroup is together at the end and LDS free
 template <typename T, int MT, int NT, int NS>
-__global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const Operand x, const Operand w, int M, int64_t N, int K, const Epilogue e) {
+MHC_DEV void sum_few_rows(const Operand& x, const Operand& w, int M, int64_t n0, int64_t N, int K, char* smem, f32x4 (&acc)[NT][MT]) {
   using S = Stage<T>;
   constexpr int kW = 2048 * NT, kStage = 2048 * (NT + MT), kLoads = 2 * (NT + MT);
-  __shared__ __attribute__((aligned(1024))) char smem[kFewWaves * NS * kStage];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int64_t n0 = (int64_t)blockIdx.x * (16 * NT);
   char* const mine = smem + wave * NS * kStage;
   Loader<T, true, 16 * NT, 1> lw;
   Loader<T, true, 16 * MT, 1> lx;
@@ -993,7 +1009,6 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const Operand 
   Reader<T, true, 16 * MT, MT> rx;
   rw.init(0, lane);
   rx.init(0, lane);
-  f32x4 acc[NT][MT] = {};
   int kleft = K - wave * S::kK;
 #pragma unroll
   for (int q = 0; q < NS; ++q) {
@@ -1032,6 +1047,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const Operand 
   }
   wait_loads<0>();
   __syncthreads();
+}
+
+template <typename T, int MT, int NT, int NS>
+__global__ __launch_bounds__(64 * kFewWaves) void few_rows_kernel(const Operand x, const Operand w, int M, int64_t N, int K, const Epilogue e) {
+  __shared__ __attribute__((aligned(1024))) char smem[kFewBytes<MT, NT, NS>];
+  const int64_t n0 = (int64_t)blockIdx.x * (16 * NT);
+  f32x4 acc[NT][MT] = {};
+  sum_few_rows<T, MT, NT, NS>(x, w, M, n0, N, K, smem, acc);
   join_waves<T, MT, NT>(acc, reinterpret_cast<float*>(smem), M, n0, N, e);
 }
 
@@ -1202,16 +1225,19 @@ inline float join_us(int splits, int64_t M, int64_t N) {  // a launch, and 8 byt
   return splits > 1 ? 4.f + 2.f * splits * (float)M * (float)N / 1e6f : 0.f;
 }
 
+inline int elem_bytes(int dtype) { return dtype == kF32 ? 4 : dtype == kI8 ? 1 : 2; }
+inline int stage_k(int dtype) { return 128 / elem_bytes(dtype); }  // (a stage of int8 has twice the k of a 16-bit one, and takes its time)
+
 // Rows that a tile may have of an operand.  A k-major one whose rows are longer
 // than kMaxRowBytes has been copied to rows of whole chunks; they are at most
 // 2^24 bytes long (K < 2^22), and 128 of them stay below 2^31.
-inline int most_rows(bool k_major, int64_t K, int dtype) { return k_major && K * (dtype == kF32 ? 4 : 2) > kMaxRowBytes ? 128 : 256; }
+inline int most_rows(bool k_major, int64_t K, int dtype) { return k_major && K * elem_bytes(dtype) > kMaxRowBytes ? 128 : 256; }
 
 // The cut with the least estimated time.  Large tiles read least, small ones
 // give every CU work; a reduction is split where even those are too few,
 // which costs a launch and its sums' way through memory.
-inline Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool a_k, bool b_k) {
-  const int kK = dtype == kF32 ? 32 : 64;
+inline Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool a_k, bool b_k, int most_splits = 16) {
+  const int kK = stage_k(dtype);
   const int stages = (int)ceil_div(K, kK);
   const float cus = (float)device_cu_count();
   Cut best = {0, 1, stages * kK, 0.f};
@@ -1219,7 +1245,7 @@ inline Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool a_k, bool b_k
     const TileCost& c = kTiles[t];
     if (c.bm > most_rows(a_k, K, dtype) || c.bn > most_rows(b_k, K, dtype)) continue;
     const float tiles = (float)ceil_div(M, c.bm) * (float)ceil_div(N, c.bn);
-    for (int want = 1; want <= 16; ++want) {
+    for (int want = 1; want <= most_splits; ++want) {
       if (want > 1 && (tiles * (want - 1) > 4.f * cus || stages < 2 * want)) break;
       const int per = (stages + want - 1) / want, splits = (stages + per - 1) / per;
       if (splits < want) continue;
@@ -1241,7 +1267,7 @@ inline PairCut pair_of(int64_t M, int64_t N, int64_t K, int dtype) {
   PairCut best = {false, cut_of(M, K, N, dtype, true, false), cut_of(N, K, M, dtype, false, false)};
   float least = best.dx.us + best.dw.us;
   const float cus = (float)device_cu_count();
-  const int kK = dtype == kF32 ? 32 : 64;
+  const int kK = stage_k(dtype);
   const int stages1 = (int)ceil_div(N, kK), stages2 = (int)ceil_div(M, kK);
   constexpr int kWant[] = {1, 2, 3, 4, 6, 8};
   for (int t = 2; t < 5; ++t) {  // (at most 128 rows: see most_rows)
@@ -1301,7 +1327,7 @@ int launch(const Product& p, hipStream_t s) {
 // 64 x 128 11.2 and 9.8).  fp32, which has more products for each fragment,
 // stays with four (2048 x 2048 x 2048 in two parts 104 and 111).
 template <typename T>
-constexpr int kRowWaves = sizeof(T) == 2 ? 4 : 2;
+constexpr int kRowWaves = sizeof(T) <= 2 ? 4 : 2;
 
 template <typename T, bool AK, bool BK>
 int run_layout(const Product& p, int tile, hipStream_t s) {

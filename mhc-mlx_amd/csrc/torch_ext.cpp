@@ -474,6 +474,7 @@ at::Tensor module_call(py::handle mod, py::handle x_obj, py::handle rd_obj) {
 }  // namespace
 
 void bind_train(py::module_& m);  // torch_train.cpp
+void bind_block(py::module_& m);  // torch_block.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "torch binding of libmhc_hip for MHCLayer's forward and backward";
@@ -485,4 +486,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("module_forward", &module_forward, "MHCLayer.forward's accelerated path (None: take the general path)");
   m.def("module_call", &module_call, "module_forward with the arguments read from the MHCLayer instance");
   bind_train(m);
+  bind_block(m);
 }

@@ -26,9 +26,10 @@ SOURCES = ["capi.hip", "sinkhorn.hip", "fused_fwd.hip", "fused_bwd.hip", "stream
            "mfma32.hip", "mix32.hip", "lf32_fwd.hip",
            "lf32_bwd_f32.hip", "lf32_bwd_bf16.hip", "lf32_bwd_f16.hip", "mxf32_f32.hip", "mxf32_bf16.hip", "mxf32_f16.hip",
            "lv_fwd_f32.hip", "lv_fwd_bf16.hip", "lv_fwd_f16.hip", "lv_bwd_f32.hip", "lv_bwd_bf16.hip", "lv_bwd_f16.hip",
-           "noalloc.hip", "adamw.hip", "policy.hip", "linear.hip", "linear_f32.hip", "linear_bf16.hip", "linear_f16.hip"]
+           "noalloc.hip", "adamw.hip", "policy.hip", "linear.hip", "linear_f32.hip", "linear_bf16.hip", "linear_f16.hip", "norm.hip", "linear_int8.hip",
+           "cross_entropy.hip", "ce_f32.hip", "ce_bf16.hip", "ce_f16.hip"]
 
-EXT_SOURCES = ["torch_ext.cpp", "torch_train.cpp"]
+EXT_SOURCES = ["torch_ext.cpp", "torch_train.cpp", "torch_block.cpp"]
 
 # Packed-FP32 VALU forms are disabled for every device pass (hipcc only; the
 # host pass prints a harmless "not a recognized feature" warning).

@@ -1,0 +1,101 @@
+"""Softmax cross entropy over a vocabulary, from the last hidden states and the head's weight, without keeping the logits.
+
+For a token with hidden state x and target y, and the logits z = weight x:
+
+    logp = log_softmax(z)[y];  loss = -sum w logp / D,   D = denominator, or the sum of the weights (1 if that is 0)
+
+Tokens of weight 0 (a prompt, padding) and those whose target is ``ignore_index`` are left out whatever their hidden states
+hold, NaN among them: they add nothing to the loss, their log probability is given as 0, their gradient is 0, and the
+products are formed without their rows.  A target outside [0, V) of a token that counts makes the loss, that token's
+gradient and the weight's NaN (it cannot be refused without waiting for the GPU).
+
+The logits are formed in pieces, in fp32 of exact products (fp32 operands: as linear_act has them, but logits past 2^95 are
+NaN), and again for the gradients, where softmax - onehot, times the token's weight over the largest one, is rounded once to x's dtype
+as an operand of two more products.  A call takes some 256 MB of workspace beside the sums of x's gradient, whatever the
+vocabulary.
+
+``linear_cross_entropy`` is differentiable in x and weight (once); ``linear_cross_entropy_and_grad`` returns the gradients with
+the loss, for a caller without autograd.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import ops
+from .profiling import timed
+
+__all__ = ["linear_cross_entropy", "linear_cross_entropy_and_grad", "linear_cross_entropy_reference"]
+
+
+def _check(denominator, ignore_index):
+    if denominator is not None and not denominator > 0:
+        raise ValueError(f"denominator must be positive (got {denominator})")
+    return 0.0 if denominator is None else float(denominator), int(ignore_index)
+
+
+class LinearCrossEntropyFn(torch.autograd.Function):
+    """linear_cross_entropy with its host steps in Python: under a kernel timer, and for torch.jit.trace, which records it."""
+
+    @staticmethod
+    def forward(ctx, x, weight, targets, mask, *numbers):
+        with timed("linear_cross_entropy_fwd"):
+            loss, logp, state = ops._binding().linear_ce_fwd(x, weight, targets, mask, *numbers)
+        ctx.save_for_backward(x, weight, targets, mask, state)
+        ctx.numbers = numbers
+        ctx.mark_non_differentiable(logp)
+        ctx.set_materialize_grads(False)
+        return loss, logp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss, _dlogp):
+        if dloss is None:
+            return (None,) * 6
+        *tensors, state = ctx.saved_tensors
+        with timed("linear_cross_entropy_bwd"):
+            dx, dw = ops._binding().linear_ce_bwd(*tensors, *ctx.numbers, state, dloss, *ctx.needs_input_grad[:2])
+        return dx, dw, None, None, None, None
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, mask: torch.Tensor | None = None,
+                         denominator: float | None = None, ignore_index: int = -100):
+    """(loss, logp): the scalar loss, differentiable in ``x`` and ``weight``, and each token's log probability (no gradient).
+
+    x [..., C] and weight [V, C] float32, bfloat16 or float16, of one dtype; targets [...] int64 or int32; mask [...] bool,
+    uint8 or floating weights.
+    """
+    numbers = _check(denominator, ignore_index)
+    if ops._use_binding() and torch.autograd.forward_ad._current_level < 0:  # (forward mode is refused by the Function)
+        return ops._binding().linear_ce(x, weight, targets, mask, *numbers)
+    return LinearCrossEntropyFn.apply(x, weight, targets, mask, *numbers)
+
+
+@torch.no_grad()
+def linear_cross_entropy_and_grad(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, mask: torch.Tensor | None = None,
+                                  denominator: float | None = None, ignore_index: int = -100, grad_scale: float = 1.0):
+    """(loss, logp, dx, dweight): linear_cross_entropy and grad_scale times its gradients, in x's dtype. No autograd.
+
+    ``grad_scale`` is the loss scale of float16 training (the loss itself is not scaled).
+    """
+    numbers = _check(denominator, ignore_index)
+    with timed("linear_cross_entropy_and_grad"):
+        return ops._binding().linear_ce_and_grad(x, weight, targets, mask, *numbers, float(grad_scale))
+
+
+def linear_cross_entropy_reference(x, weight, targets, mask=None, denominator=None, ignore_index: int = -100):
+    """linear_cross_entropy in elementary torch operations (fp32 for half inputs, else the inputs' dtype), on any device."""
+    den, ignored = _check(denominator, ignore_index)
+    up = torch.float64 if x.dtype == torch.float64 else torch.float32
+    w = torch.ones(targets.shape, dtype=up, device=x.device) if mask is None else mask.to(up)
+    w = torch.where(targets == ignored, 0.0, w)
+    live = w != 0
+    z = torch.matmul(torch.where(live[..., None], x.to(up), 0.0), weight.to(up).t())
+    at = torch.where(live, targets, 0).long()
+    bad = (at < 0) | (at >= weight.shape[0])
+    picked = z.gather(-1, torch.where(bad, 0, at)[..., None])[..., 0]
+    logp = torch.where(bad, float("nan"), picked - torch.logsumexp(z, -1))
+    logp = torch.where(live, logp, 0.0)
+    total = den or w.sum()
+    loss = -torch.where(live, w * logp, 0.0).sum() / (total if den else torch.where(total != 0, total, 1.0))
+    return loss, logp.detach()

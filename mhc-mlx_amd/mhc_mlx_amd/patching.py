@@ -31,13 +31,14 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
+from .int8 import Int8Linear
 from .layer import MHCRewire
 
 __all__ = ["AutoPatcher"]
 
 
 def _quantized_linear_types() -> tuple:
-    types = []
+    types = [Int8Linear]
     try:
         import torch.ao.nn.quantized as nnq
         import torch.ao.nn.quantized.dynamic as nnqd
@@ -52,6 +53,8 @@ _QUANTIZED = _quantized_linear_types()
 
 
 def _module_device_dtype(module: nn.Module):
+    if isinstance(module, Int8Linear):  # (its buffers are no dtype that activations have)
+        return module.weight.device, module.return_dtype
     for t in list(module.parameters(recurse=False)) + list(module.buffers(recurse=False)):
         return t.device, t.dtype
     return None, None
