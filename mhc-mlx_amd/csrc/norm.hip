@@ -124,6 +124,159 @@ MHC_DEV float factor_of(float squares, int C, float eps, Sum sum, Largest larges
 }
 
 // --------------------------------------------------------------------------
+// Rows that registers hold
+// --------------------------------------------------------------------------
+
+// A row in the registers of THREADS threads (a wave, and then four rows a
+// workgroup, or a workgroup): NV vectors each, and the C % V elements after the
+// last whole vector one for each of the first threads.  Threads past the last
+// vector read it once more (a load under a condition would wait for itself) and
+// count it as zeros.
+template <typename T, int THREADS, int NV>
+struct Held {
+  static constexpr int V = kV<T>, kRows = THREADS == kWave ? 4 : 1, kBlock = THREADS * kRows;
+  int tid, vecs, tail, C;
+  bool on_tail;
+
+  MHC_DEV explicit Held(int C_) : C(C_) {
+    tid = threadIdx.x % THREADS;
+    vecs = C / V;
+    tail = vecs * V + tid;
+    on_tail = tail < C;
+  }
+  MHC_DEV int vec(int i) const { return i * THREADS + tid; }
+  MHC_DEV bool has(int i) const { return vec(i) < vecs; }
+
+  template <typename S>
+  MHC_DEV void load(const S* p, float (&z)[NV][V], float& last) const {
+    if (vecs > 0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) gemm::take<true>(p + min(vec(i), vecs - 1) * V, z[i], V);
+    }
+    last = on_tail ? load1(p + tail) : 0.f;
+  }
+  template <typename S>
+  MHC_DEV void store(S* p, const float (&z)[NV][V], float last) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (has(i)) gemm::put<true>(p + vec(i) * V, z[i], V);
+    if (on_tail) store1(p + tail, last);
+  }
+  // zeros in the place of vectors that are not there
+  MHC_DEV void clear(float (&z)[NV][V]) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) z[i][k] = has(i) ? z[i][k] : 0.f;
+  }
+  MHC_DEV void load_weights(const void* w, bool f32, float (&z)[NV][V], float& last) const {
+    if (w == nullptr) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) z[i][k] = 1.f;
+      last = 1.f;
+    } else if (f32) {
+      load_cached(static_cast<const float*>(w), z, last);
+    } else if constexpr (sizeof(T) == 2) {
+      load_cached(static_cast<const T*>(w), z, last);
+    }
+  }
+  // (every row reads the weights)
+  template <typename S>
+  MHC_DEV void load_cached(const S* p, float (&z)[NV][V], float& last) const {
+    if (vecs > 0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        Vec<S, V> r;
+        __builtin_memcpy(r.w, p + min(vec(i), vecs - 1) * V, sizeof(r.w));
+#pragma unroll
+        for (int k = 0; k < V; ++k) z[i][k] = r.get(k);
+      }
+    }
+    last = on_tail ? load1(p + tail) : 0.f;
+  }
+};
+
+template <typename T, int MODE, int THREADS, int NV>
+__global__ __launch_bounds__((Held<T, THREADS, NV>::kBlock)) void norm_held_kernel(const NormArgs a, int w_f32) {
+  using H = Held<T, THREADS, NV>;
+  constexpr int V = H::V;
+  __shared__ float lds[2][16];
+  const H at(a.C);
+  const int64_t t = (int64_t)blockIdx.x * H::kRows + (H::kRows > 1 ? threadIdx.x / THREADS : 0);
+  if (t >= a.T) return;  // (a wave with its row)
+  float z[NV][V] = {}, w[NV][V] = {}, z1, w1;
+  at.load(static_cast<const T*>(a.x) + t * a.ldx, z, z1);
+  if (a.r != nullptr) {
+    float r[NV][V] = {}, r1;
+    at.load(static_cast<const T*>(a.r) + t * a.ldr, r, r1);
+    if constexpr (MODE != kCodesOnly) at.load_weights(a.w, w_f32, w, w1);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        z[i][k] += r[i][k];
+        if constexpr (sizeof(T) == 2) z[i][k] = from16<T>(bits16<T>(z[i][k]));
+      }
+    z1 += r1;
+    if constexpr (sizeof(T) == 2) z1 = from16<T>(bits16<T>(z1));
+    at.store(static_cast<T*>(a.h) + t * a.C, z, z1);
+  } else if constexpr (MODE != kCodesOnly) {
+    at.load_weights(a.w, w_f32, w, w1);
+  }
+  at.clear(z);
+  float s = 1.f, top = 0.f;
+  if constexpr (MODE != kCodesOnly) {
+    const auto squares = [&](float by) {
+      float q = z1 * by * (z1 * by);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) q = fmaf(z[i][k] * by, z[i][k] * by, q);
+      return join_threads<THREADS>(q, SumOp{}, lds[0]);
+    };
+    s = factor_of(squares(1.f), a.C, a.eps, squares, [&] {
+      float m = fabsf(z1);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) m = LargerOp{}(m, fabsf(z[i][k]));
+      return join_threads<THREADS>(m, LargerOp{}, lds[1]);
+    });
+  }
+  if constexpr (MODE == kPlain) {
+    if (at.tid == 0 && a.rstd != nullptr) a.rstd[t] = s;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) z[i][k] = z[i][k] * s * w[i][k];
+    at.store(static_cast<T*>(a.y) + t * a.C, z, z1 * s * w1);
+  } else {
+    if constexpr (MODE == kCodes) {
+      z1 = at.on_tail ? z1 * w1 : 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) z[i][k] = at.has(i) ? z[i][k] * w[i][k] : 0.f;  // (0 times a weight that is not finite)
+    }
+    top = fabsf(z1);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) top = LargerOp{}(top, fabsf(z[i][k]));
+    top = join_threads<THREADS>(top, LargerOp{}, lds[1]);
+    if (at.tid == 0) a.scales[t] = Coder::scale(top, s);
+    const Coder coder(top);
+    int8_t* const codes = static_cast<int8_t*>(a.y) + t * a.C;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (at.has(i)) put_codes<true>(codes + at.vec(i) * V, coder, z[i], V);
+    if (at.on_tail) codes[at.tail] = (int8_t)coder.code(z1);
+  }
+}
+
+// --------------------------------------------------------------------------
 // Rows of any length: a workgroup goes over a row twice
 // --------------------------------------------------------------------------
 
@@ -227,10 +380,13 @@ struct NormBwdArgs {
   const void* w;   // or NULL
   int64_t lddy, lddh, ldh;
   void* dx;        // [T, C], or NULL
-  float* part;     // sums of dw, [workgroups, C], or NULL
+  float* part;     // sums of dw, [workgroups, part_pitch], or NULL
   int64_t T;
   int C;
 };
+
+// A row of the sums of dw: C, and up to three more, so that every row is in whole vectors.
+__host__ __device__ inline int64_t part_pitch(int64_t C) { return (C + 3) / 4 * 4; }
 
 template <typename T>
 __global__ __launch_bounds__(kLongThreads) void norm_bwd_long_kernel(const NormBwdArgs a, int w_f32) {
@@ -277,6 +433,72 @@ __global__ __launch_bounds__(kLongThreads) void norm_bwd_long_kernel(const NormB
   }
 }
 
+// Rows that registers hold: dx, and this workgroup's sums of dw, to
+// part[workgroup].  A workgroup takes rows in turn and keeps the weights and
+// the sums in registers.
+template <typename T, int THREADS, int NV>
+__global__ __launch_bounds__((Held<T, THREADS, NV>::kBlock)) void norm_bwd_held_kernel(const NormBwdArgs a, int w_f32) {
+  using H = Held<T, THREADS, NV>;
+  constexpr int V = H::V, kRows = H::kRows;
+  __shared__ float lds[16];
+  const H at(a.C);
+  const int row = kRows > 1 ? threadIdx.x / THREADS : 0;
+  float w[NV][V] = {}, w1 = 0.f, sum[NV][V] = {}, sum1 = 0.f;
+  at.load_weights(a.w, w_f32, w, w1);
+  for (int64_t t = (int64_t)blockIdx.x * kRows + row; t < a.T; t += (int64_t)gridDim.x * kRows) {
+    float g[NV][V] = {}, n[NV][V] = {}, d[NV][V] = {}, g1, n1, d1 = 0.f;
+    at.load(static_cast<const T*>(a.dy) + t * a.lddy, g, g1);
+    at.load(static_cast<const T*>(a.h) + t * a.ldh, n, n1);
+    if (a.dh != nullptr && a.dx != nullptr) at.load(static_cast<const T*>(a.dh) + t * a.lddh, d, d1);
+    const float s = a.rstd[t];
+    float along = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        n[i][k] *= s;
+        const float dn = at.has(i) ? g[i][k] * n[i][k] : 0.f;  // dy n, of which dw is the sum over rows and along over columns, times w
+        sum[i][k] += dn;
+        along = at.has(i) ? fmaf(dn, w[i][k], along) : along;
+        g[i][k] *= w[i][k];
+      }
+    n1 *= s;
+    sum1 = fmaf(g1, n1, sum1);
+    g1 *= w1;
+    if (at.on_tail) along = fmaf(g1, n1, along);
+    if (a.dx == nullptr) continue;
+    along = join_threads<THREADS>(along, SumOp{}, lds) / (float)a.C;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) d[i][k] = fmaf(s, g[i][k] - n[i][k] * along, d[i][k]);
+    at.store(static_cast<T*>(a.dx) + t * a.C, d, fmaf(s, g1 - n1 * along, d1));
+  }
+  if (a.part == nullptr) return;
+  float* const part = a.part + blockIdx.x * part_pitch(a.C);
+  if constexpr (kRows == 1) {
+    at.store(part, sum, sum1);
+  } else {
+    __shared__ float sums[kRows][THREADS * NV * V + THREADS];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) sums[row][(i * V + k) * THREADS + at.tid] = sum[i][k];
+    sums[row][NV * V * THREADS + at.tid] = sum1;
+    __syncthreads();
+    if (row != 0) return;
+#pragma unroll
+    for (int q = 1; q < kRows; ++q) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) sum[i][k] += sums[q][(i * V + k) * THREADS + at.tid];
+      sum1 += sums[q][NV * V * THREADS + at.tid];
+    }
+    at.store(part, sum, sum1);
+  }
+}
+
 constexpr int kDwCols = 64 * 8;  // columns of a workgroup of norm_dw_kernel
 
 int dw_rows(int64_t T, int C) { return (int)std::max<int64_t>(16, ceil_div(T * ceil_div(C, kDwCols), 4 * device_cu_count())); }
@@ -309,19 +531,100 @@ __global__ __launch_bounds__(256) void norm_dw_kernel(const NormBwdArgs a, int r
   for (int k = 0; k < 8; ++k) lds[wave][lane * 8 + k] = sum[k];
   __syncthreads();
   for (int c = threadIdx.x; c < kDwCols; c += 256)
-    if (n0 + c < a.C) a.part[(int64_t)block * a.C + n0 + c] = (lds[0][c] + lds[1][c]) + (lds[2][c] + lds[3][c]);
+    if (n0 + c < a.C) a.part[block * part_pitch(a.C) + n0 + c] = (lds[0][c] + lds[1][c]) + (lds[2][c] + lds[3][c]);
 }
 
+// dw from the rows of its sums: sixteen columns a workgroup, each of 64 groups
+// of threads with every 64th row, eight of them under way, joined in order.
+constexpr int kJoinCols = 4, kJoinParts = 64;
+
 template <typename W>
-__global__ __launch_bounds__(256) void norm_dw_join_kernel(const float* part, W* dw, int64_t rows, int64_t C) {
-  __shared__ float lds[8][gemm::kSumCols];
-  gemm::sum_columns<256>(lds, part, dw, rows, C, blockIdx.x);
+__global__ __launch_bounds__(kJoinCols* kJoinParts) void norm_dw_join_kernel(const float* part, W* dw, int rows, int C) {
+  __shared__ f32x4 lds[kJoinParts][kJoinCols];
+  const int col = threadIdx.x % kJoinCols, q = threadIdx.x / kJoinCols;
+  const int64_t pitch = part_pitch(C);
+  const int c = (blockIdx.x * kJoinCols + col) * 4;
+  const float* const p = part + min((int64_t)c, pitch - 4);
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int r = q; r < rows; r += 8 * kJoinParts) {
+    f32x4 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const f32x4*>(p + min(r + k * kJoinParts, rows - 1) * pitch);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (r + k * kJoinParts < rows) s += v[k];
+  }
+  lds[q][col] = s;
+  __syncthreads();
+  if (threadIdx.x >= kJoinCols * 4) return;  // a thread for each column
+  const float* const mine = reinterpret_cast<const float*>(lds) + threadIdx.x;
+  const int n = blockIdx.x * kJoinCols * 4 + threadIdx.x;
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < kJoinParts; ++k) sum += mine[k * kJoinCols * 4];
+  if (n < C) store1(dw + n, sum);
 }
 
 unsigned grid_of(int64_t T) { return (unsigned)std::min<int64_t>(T, kMaxRows); }
 
+// How a row of C elements is held: by how many threads, and how many vectors
+// each; none: it is not.
+struct Hold {
+  int threads, vecs;
+};
+
+Hold hold_of(int C, int dtype) {
+  const int vecs = std::max(1, C * gemm::elem_bytes(dtype) / 16);
+  if (vecs <= 64) return {64, 1};
+  if (vecs <= 128) return {64, 2};
+  if (vecs <= 256) return {64, 4};
+  if (vecs <= 512) return {256, 2};
+  if (vecs <= 1024) return {256, 4};
+  if (vecs <= 2048) return {1024, 2};
+  if (vecs <= 4096) return {1024, 4};
+  return {0, 0};
+}
+
+// The same in the backward, which has five vectors of numbers for each of a row's.
+Hold bwd_hold_of(int C, int dtype) {
+  const int vecs = std::max(1, C * gemm::elem_bytes(dtype) / 16);
+  if (vecs <= 64) return {64, 1};
+  if (vecs <= 128) return {64, 2};
+  if (vecs <= 256) return {256, 1};
+  if (vecs <= 512) return {256, 2};
+  if (vecs <= 1024) return {512, 2};
+  if (vecs <= 2048) return {512, 4};
+  return {0, 0};
+}
+
+template <int THREADS, int VECS>
+struct HoldOf {
+  static constexpr int kThreads = THREADS, kVecs = VECS;
+  static bool is(const Hold& h) { return h.threads == THREADS && h.vecs == VECS; }
+};
+
+// f(HoldOf<...>{}) for the one of the list that h is
+template <typename F>
+int with_hold(const Hold&, F) { return MHC_OK; }
+template <typename H, typename... Hs, typename F>
+int with_hold(const Hold& h, F f) {
+  if (H::is(h)) return f(H{});
+  return with_hold<Hs...>(h, f);
+}
+
 template <typename T, int MODE>
 int run_norm(const NormArgs& a, int w_f32, hipStream_t s) {
+  const Hold hold = hold_of(a.C, dtype_code<T>());
+  if (hold.threads > 0) {
+    return with_hold<HoldOf<64, 1>, HoldOf<64, 2>, HoldOf<64, 4>, HoldOf<256, 2>, HoldOf<256, 4>, HoldOf<1024, 2>, HoldOf<1024, 4>>(
+        hold, [&](auto of) {
+          using O = decltype(of);
+          using H = Held<T, O::kThreads, O::kVecs>;
+          hipLaunchKernelGGL((norm_held_kernel<T, MODE, O::kThreads, O::kVecs>), dim3((unsigned)ceil_div(a.T, H::kRows)), dim3(H::kBlock), 0, s, a, w_f32);
+          MHC_CHECK_LAUNCH("norm_held_kernel");
+          return (int)MHC_OK;
+        });
+  }
   hipLaunchKernelGGL((norm_long_kernel<T, MODE>), dim3(grid_of(a.T)), dim3(kLongThreads), 0, s, a, w_f32);
   MHC_CHECK_LAUNCH("norm_long_kernel");
   return MHC_OK;
@@ -334,25 +637,51 @@ int run_norm(const NormArgs& a, int dtype, int w_f32, hipStream_t s) {
   return run_norm<_Float16, MODE>(a, w_f32, s);
 }
 
+// Workgroups of norm_bwd_held_kernel: as many as a CU has room for, with four rows each if there are so many.
+int64_t bwd_blocks(const Hold& h, int64_t T) {
+  const int64_t cus = device_cu_count(), most = cus * (h.threads == 512 ? 2 : 4), rows = h.threads == 64 ? ceil_div(T, 4) : T;
+  return std::min(std::min(rows, most), std::max(cus, ceil_div(rows, 4)));
+}
+
 // rows of the sums of dw
-int64_t part_rows(int64_t T, int C) { return ceil_div(T, dw_rows(T, C)); }
+int64_t part_rows(int64_t T, int C, int dtype) {
+  const Hold hold = bwd_hold_of(C, dtype);
+  return hold.threads > 0 ? bwd_blocks(hold, T) : ceil_div(T, dw_rows(T, C));
+}
 
 template <typename T>
-int run_bwd(const NormBwdArgs& a, int w_f32, void* dw, hipStream_t s) {
+int run_dw_join(const float* part, void* dw, int w_f32, int64_t rows, int64_t C, hipStream_t s) {
+  const dim3 grid((unsigned)ceil_div(C, kJoinCols * 4)), block(kJoinCols * kJoinParts);
+  if (w_f32) hipLaunchKernelGGL((norm_dw_join_kernel<float>), grid, block, 0, s, part, static_cast<float*>(dw), (int)rows, (int)C);
+  else hipLaunchKernelGGL((norm_dw_join_kernel<T>), grid, block, 0, s, part, static_cast<T*>(dw), (int)rows, (int)C);
+  MHC_CHECK_LAUNCH("norm_dw_join_kernel");
+  return MHC_OK;
+}
+
+template <typename T>
+int run_bwd(NormBwdArgs a, int w_f32, void* dw, hipStream_t s) {
+  if (dw == nullptr) a.part = nullptr;
+  const Hold hold = bwd_hold_of(a.C, dtype_code<T>());
+  const int64_t blocks = part_rows(a.T, a.C, dtype_code<T>());
+  if (hold.threads > 0) {
+    const int rc = with_hold<HoldOf<64, 1>, HoldOf<64, 2>, HoldOf<256, 1>, HoldOf<256, 2>, HoldOf<512, 2>, HoldOf<512, 4>>(hold, [&](auto of) {
+      using O = decltype(of);
+      using H = Held<T, O::kThreads, O::kVecs>;
+      hipLaunchKernelGGL((norm_bwd_held_kernel<T, O::kThreads, O::kVecs>), dim3((unsigned)blocks), dim3(H::kBlock), 0, s, a, w_f32);
+      MHC_CHECK_LAUNCH("norm_bwd_held_kernel");
+      return (int)MHC_OK;
+    });
+    return rc != MHC_OK || dw == nullptr ? rc : run_dw_join<T>(a.part, dw, w_f32, blocks, a.C, s);
+  }
   if (a.dx != nullptr) {
     hipLaunchKernelGGL((norm_bwd_long_kernel<T>), dim3(grid_of(a.T)), dim3(kLongThreads), 0, s, a, w_f32);
     MHC_CHECK_LAUNCH("norm_bwd_long_kernel");
   }
   if (dw == nullptr) return MHC_OK;
-  const int64_t blocks = part_rows(a.T, a.C);
   const uint32_t wide = (uint32_t)ceil_div(a.C, kDwCols);
   hipLaunchKernelGGL((norm_dw_kernel<T>), dim3(wide * (uint32_t)blocks), dim3(256), 0, s, a, dw_rows(a.T, a.C), wide);
   MHC_CHECK_LAUNCH("norm_dw_kernel");
-  const dim3 grid((unsigned)ceil_div(a.C, gemm::kSumCols));
-  if (w_f32) hipLaunchKernelGGL((norm_dw_join_kernel<float>), grid, dim3(256), 0, s, (const float*)a.part, static_cast<float*>(dw), blocks, a.C);
-  else hipLaunchKernelGGL((norm_dw_join_kernel<T>), grid, dim3(256), 0, s, (const float*)a.part, static_cast<T*>(dw), blocks, a.C);
-  MHC_CHECK_LAUNCH("norm_dw_join_kernel");
-  return MHC_OK;
+  return run_dw_join<T>(a.part, dw, w_f32, blocks, a.C, s);
 }
 
 int check_shape(int64_t T, int64_t C, int dtype) {
@@ -410,9 +739,8 @@ extern "C" int mhc_quantize_int8(const void* x, int64_t ldx, int8_t* codes, floa
 }
 
 extern "C" size_t mhc_add_rms_norm_bwd_workspace_bytes(int64_t T, int64_t C, int dtype) {
-  (void)dtype;
   if (T <= 0 || C <= 0 || C >= ((int64_t)1 << 24)) return 0;
-  return (size_t)(mhc::part_rows(T, (int)C) * C) * sizeof(float);
+  return (size_t)(mhc::part_rows(T, (int)C, dtype) * mhc::part_pitch(C)) * sizeof(float);
 }
 
 extern "C" int mhc_add_rms_norm_bwd(const void* dy, int64_t lddy, const void* dh, int64_t lddh, const void* h, int64_t ldh, const float* rstd,
