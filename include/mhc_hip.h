@@ -464,6 +464,11 @@ int mhc_add_rms_norm_int8(const void* x, int64_t ldx, const void* residual, int6
 int mhc_quantize_int8(const void* x, int64_t ldx, int8_t* codes, float* scales, int64_t T,
                       int64_t C, int dtype, void* stream);
 
+/* The values that rows of codes [T, C], ld apart, stand for: out [T, C] =
+ * codes * scales, contiguous, of out_dtype. */
+int mhc_dequantize_int8(const int8_t* codes, int64_t ld, const float* scales, void* out,
+                        int out_dtype, int64_t T, int64_t C, void* stream);
+
 size_t mhc_add_rms_norm_bwd_workspace_bytes(int64_t T, int64_t C, int dtype);
 
 /* Gradients for dy and dh (or NULL: none) of y and h, from h (or x) and rstd:

@@ -565,6 +565,41 @@ __global__ __launch_bounds__(kJoinCols* kJoinParts) void norm_dw_join_kernel(con
   if (n < C) store1(dw + n, sum);
 }
 
+// codes times their row's scale, eight a thread
+template <typename O, bool WHOLE>
+MHC_DEV void values_of(const int8_t* codes, float scale, O* out, int left) {
+  float v[8];
+  if constexpr (WHOLE) {
+    int8_t c[8];
+    __builtin_memcpy(c, codes, 8);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = (float)c[k] * scale;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = k < left ? (float)codes[k] * scale : 0.f;
+  }
+  gemm::put<WHOLE>(out, v, left);
+}
+
+template <typename O>
+__global__ __launch_bounds__(256) void values_kernel(const int8_t* codes, int64_t ld, const float* scales, O* out, int64_t T, int C, uint32_t groups) {
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < T * groups; at += (int64_t)gridDim.x * 256) {
+    const int64_t t = at / groups;
+    const int n = (int)(at % groups) * 8, left = min(8, C - n);
+    if (left == 8) values_of<O, true>(codes + t * ld + n, scales[t], out + t * C + n, 8);
+    else values_of<O, false>(codes + t * ld + n, scales[t], out + t * C + n, left);
+  }
+}
+
+template <typename O>
+int run_values(const int8_t* codes, int64_t ld, const float* scales, void* out, int64_t T, int C, hipStream_t s) {
+  const uint32_t groups = (uint32_t)ceil_div(C, 8);
+  const dim3 grid((unsigned)std::min(ceil_div(T * groups, 256), (int64_t)device_cu_count() * 32));
+  hipLaunchKernelGGL((values_kernel<O>), grid, dim3(256), 0, s, codes, ld, scales, static_cast<O*>(out), T, C, groups);
+  MHC_CHECK_LAUNCH("values_kernel");
+  return MHC_OK;
+}
+
 unsigned grid_of(int64_t T) { return (unsigned)std::min<int64_t>(T, kMaxRows); }
 
 // How a row of C elements is held: by how many threads, and how many vectors
@@ -736,6 +771,20 @@ extern "C" int mhc_quantize_int8(const void* x, int64_t ldx, int8_t* codes, floa
   MHC_CHECK_ARG(ldx >= C || T == 1, "ldx must be at least C");
   const NormArgs a = {x, nullptr, nullptr, ldx, 0, nullptr, codes, scales, nullptr, T, (int)C, 1.f};
   return run_norm<kCodesOnly>(a, dtype, 0, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int mhc_dequantize_int8(const int8_t* codes, int64_t ld, const float* scales, void* out, int out_dtype, int64_t T, int64_t C,
+                                   void* stream) {
+  using namespace mhc;
+  clear_error();
+  if (const int rc = check_shape(T, C, out_dtype)) return rc;
+  if (T == 0) return MHC_OK;
+  MHC_CHECK_ARG(codes != nullptr && scales != nullptr && out != nullptr, "null pointer");
+  MHC_CHECK_ARG(ld >= C || T == 1, "ld must be at least C");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (out_dtype == kF32) return run_values<float>(codes, ld, scales, out, T, (int)C, s);
+  if (out_dtype == kBF16) return run_values<__bf16>(codes, ld, scales, out, T, (int)C, s);
+  return run_values<_Float16>(codes, ld, scales, out, T, (int)C, s);
 }
 
 extern "C" size_t mhc_add_rms_norm_bwd_workspace_bytes(int64_t T, int64_t C, int dtype) {

@@ -133,6 +133,7 @@ std::tuple<at::Tensor, at::Tensor> add_rms_norm(const at::Tensor& x, const OptTe
 
 // (codes, scales, h)
 std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_int8(const at::Tensor& x, const OptTensor& r, const OptTensor& w, double eps) {
+  const at::AutoGradMode plain_mode(false);
   const NormInputs n = norm_inputs(x, get(r), get(w));
   const at::DeviceGuard guard(x.device());
   const auto plain = x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous);
@@ -150,6 +151,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_int8(const at::Tenso
 
 // (codes, scales)
 std::tuple<at::Tensor, at::Tensor> quantize_int8(const at::Tensor& x) {
+  const at::AutoGradMode plain_mode(false);
   const NormInputs n = norm_inputs(x, at::Tensor(), at::Tensor());
   const at::DeviceGuard guard(x.device());
   at::Tensor codes = at::empty(x.sizes(), x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous).dtype(at::kChar));
@@ -169,8 +171,20 @@ void check_rows(const at::Tensor& like, const at::Tensor& codes, const at::Tenso
                     codes.sizes().slice(0, codes.dim() - 1), ", got ", scales.sizes());
 }
 
+at::Tensor dequantize_int8(const at::Tensor& codes, const at::Tensor& scales, int64_t out_code) {
+  check_rows(codes, codes, scales, "rows");
+  const at::DeviceGuard guard(codes.device());
+  const int64_t C = codes.size(-1), T = codes.numel() / C;
+  const at::Tensor rows = rows_of(codes, C), s = scales.contiguous();
+  at::Tensor out = at::empty(codes.sizes(), codes.options().memory_format(at::MemoryFormat::Contiguous).dtype(scalar_type(out_code)));
+  check(mhc_dequantize_int8(rows.data_ptr<int8_t>(), row_stride(rows), s.data_ptr<float>(), out.data_ptr(), (int)out_code, T, C, stream_of(codes)),
+        "mhc_dequantize_int8");
+  return out;
+}
+
 at::Tensor linear_int8(const at::Tensor& x, const at::Tensor& x_scales, const at::Tensor& w, const at::Tensor& w_scales, const OptTensor& bias_,
                        const OptTensor& residual_, int64_t act, int64_t out_code) {
+  const at::AutoGradMode plain_mode(false);
   check_rows(x, x, x_scales, "x");
   check_rows(x, w, w_scales, "weight");
   TORCH_CHECK_VALUE(w.dim() == 2 && w.size(0) >= 1, "weight: codes must be [N, K], got shape ", w.sizes());
@@ -194,8 +208,8 @@ at::Tensor linear_int8(const at::Tensor& x, const at::Tensor& x_scales, const at
   const at::DeviceGuard guard(x.device());
   at::Tensor out = at::empty(shape, x.options().dtype(scalar_type(out_code)));
   if (M == 0) return out;
-  if (bias.defined()) bias = bias.detach().to(at::kFloat).contiguous();
-  if (residual.defined()) residual = residual.detach().contiguous();
+  if (bias.defined()) bias = bias.to(at::kFloat).contiguous();
+  if (residual.defined()) residual = residual.contiguous();
   const at::Tensor xr = rows_of(x, K), wr = rows_of(w, K), xs = x_scales.contiguous(), wsc = w_scales.contiguous();
   const int8_t *xp = xr.data_ptr<int8_t>(), *wp = wr.data_ptr<int8_t>();
   const size_t nb = mhc_linear_int8_workspace_bytes(xp, row_stride(xr), wp, row_stride(wr), M, N, K);
@@ -306,6 +320,7 @@ std::tuple<at::Tensor, at::Tensor> linear_ce_bwd(const at::Tensor& x, const at::
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_ce_and_grad(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets,
                                                                               const OptTensor& mask, double denominator, int64_t ignore_index,
                                                                               double grad_scale) {
+  const at::AutoGradMode plain_mode(false);
   const CeInputs c = ce_inputs(x, w, targets, get(mask), denominator, ignore_index);
   const at::DeviceGuard guard(x.device());
   const CeResult r = ce_forward(c, x);
@@ -355,6 +370,7 @@ void bind_block(py::module_& m) {
   m.def("add_rms_norm_bwd", &add_rms_norm_bwd, "gradients of x (and the residual) and of the weight (None where not asked for)");
   m.def("add_rms_norm_int8", &add_rms_norm_int8, "codes and scales of the normed rows, and the sum");
   m.def("quantize_int8", &quantize_int8, "codes and scales of rows");
+  m.def("dequantize_int8", &dequantize_int8, "the values of int8 rows");
   m.def("linear_int8", &linear_int8, "product of int8 rows with scales, bias, activation and residual");
   m.def("linear_ce", &linear_ce, "cross entropy from hidden states with the backward in C++");
   m.def("linear_ce_fwd", &linear_ce_fwd, "the loss, the log probabilities and what the backward reads, without autograd");

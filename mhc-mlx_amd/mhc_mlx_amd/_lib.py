@@ -128,6 +128,7 @@ SIGNATURES = {
     "mhc_add_rms_norm_fwd": ([_VP, _I64, _VP, _I64, _VP, _I32, _VP, _VP, _VP, _I64, _I64, _I32, _F32, _VP], _I32),
     "mhc_add_rms_norm_int8": ([_VP, _I64, _VP, _I64, _VP, _I32, _VP, _VP, _VP, _I64, _I64, _I32, _F32, _VP], _I32),
     "mhc_quantize_int8": ([_VP, _I64, _VP, _VP, _I64, _I64, _I32, _VP], _I32),
+    "mhc_dequantize_int8": ([_VP, _I64, _VP, _VP, _I32, _I64, _I64, _VP], _I32),
     "mhc_add_rms_norm_bwd_workspace_bytes": ([_I64, _I64, _I32], _SZ),
     "mhc_add_rms_norm_bwd": ([_VP, _I64, _VP, _I64, _VP, _I64, _VP, _VP, _I32, _VP, _VP, _I64, _I64, _I32, _VP, _SZ, _VP], _I32),
     "mhc_linear_int8_workspace_bytes": ([_VP, _I64, _VP, _I64, _I64, _I64, _I64], _SZ),

@@ -71,7 +71,6 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     return LinearCrossEntropyFn.apply(x, weight, targets, mask, *numbers)
 
 
-@torch.no_grad()
 def linear_cross_entropy_and_grad(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, mask: torch.Tensor | None = None,
                                   denominator: float | None = None, ignore_index: int = -100, grad_scale: float = 1.0):
     """(loss, logp, dx, dweight): linear_cross_entropy and grad_scale times its gradients, in x's dtype. No autograd.

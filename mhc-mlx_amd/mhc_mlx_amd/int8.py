@@ -37,18 +37,19 @@ class Int8Rows(NamedTuple):
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values that the rows stand for."""
+        if self.codes.is_cuda and dtype != torch.float64:
+            with timed("dequantize_int8"):
+                return ops._binding().dequantize_int8(self.codes, self.scales, ops._code(dtype))
         out = torch.empty(self.codes.shape, dtype=dtype, device=self.codes.device)
         return torch.mul(self.codes, self.scales.unsqueeze(-1), out=out)
 
 
-@torch.no_grad()
 def quantize_int8(x: torch.Tensor) -> Int8Rows:
     """x [..., K] in 8 bits, with a scale for each row. Rows may lie any distance apart; other strides are copied."""
     with timed("quantize_int8"):
         return Int8Rows(*ops._binding().quantize_int8(x))
 
 
-@torch.no_grad()
 def linear_int8(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None, residual: torch.Tensor | None = None,
                 activation: str = "none", output_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """act(x weight^T + bias) + residual of rows in 8 bits: x [..., K], weight [N, K], bias [N], residual [..., N].

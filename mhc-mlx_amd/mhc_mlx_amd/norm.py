@@ -72,7 +72,6 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None = None, weight: 
     return (out, x) if residual is None else out
 
 
-@torch.no_grad()
 def add_rms_norm_int8(x: torch.Tensor, residual: torch.Tensor | None = None, weight: torch.Tensor | None = None, eps: float = 1e-6):
     """(Int8Rows of y, h): add_rms_norm with its output in 8 bits. No autograd."""
     eps = _check_eps(eps)

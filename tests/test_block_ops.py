@@ -139,6 +139,9 @@ def test_norm_refusals_at_the_c_abi(lib):
     assert int8(s=None) == -1 and b"null" in lib.mhc_last_error()
     assert lib.mhc_quantize_int8(None, 8, p, p, 2, 8, 0, None) == -1 and lib.mhc_quantize_int8(p, 7, p, p, 2, 8, 0, None) == -1
     assert lib.mhc_quantize_int8(None, 8, None, None, 0, 8, 0, None) == 0
+    for bad in ((None, 8, p, p, 1, 2, 8), (p, 8, None, p, 1, 2, 8), (p, 8, p, None, 1, 2, 8), (p, 7, p, p, 1, 2, 8), (p, 8, p, p, 3, 2, 8), (p, 8, p, p, 1, 2, 0)):
+        assert lib.mhc_dequantize_int8(*bad, None) == -1
+    assert lib.mhc_dequantize_int8(None, 8, None, None, 1, 0, 8, None) == 0
     nb = lib.mhc_add_rms_norm_bwd_workspace_bytes(100, 64, 1)
     assert nb > 0 and lib.mhc_add_rms_norm_bwd_workspace_bytes(0, 64, 1) == 0
 

@@ -44,6 +44,32 @@ def test_products(dt, M):
         check(g, M, N, K, dt, bias=N % 2 == 0, residual=K % 2 == 0)
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+def test_values(dt):
+    g = gen(2)
+    for shape in ((1, 1), (3, 7), (2, 5, 64), (40, 1001), (9, 16384)):
+        rows = rows_of(g, *shape, low=-128)
+        want = rows.codes.float() * rows.scales[..., None]
+        assert torch.equal(rows.dequantize(dt), want.to(dt)) and torch.equal(rows.dequantize(torch.float64), want.double())
+    part = Int8Rows(rows.codes[:, 3:999], rows.scales)
+    assert torch.equal(part.dequantize(dt), want[:, 3:999].to(dt))
+    assert Int8Rows(rows.codes[:0], rows.scales[:0]).dequantize(dt).shape == (0, 16384)
+    with pytest.raises(ValueError):
+        rows.dequantize(torch.int32)
+    with pytest.raises(ValueError):
+        Int8Rows(rows.codes, rows.scales[:3]).dequantize(dt)
+
+
+def test_results_carry_no_gradient():
+    g = gen(3)
+    x = torch.randn(4, 64, generator=g, device="cuda", requires_grad=True)
+    w = rows_of(g, 8, 64)
+    rows, h = add_rms_norm_int8(x.t().contiguous().t(), x, torch.ones(64, device="cuda", requires_grad=True))
+    out = linear_int8(quantize_int8(x[:, ::2][:, :32].contiguous().repeat(1, 2)), w, torch.zeros(8, device="cuda", requires_grad=True),
+                      torch.zeros(4, 8, device="cuda", requires_grad=True).t().contiguous().t(), output_dtype=torch.float32)
+    assert not any(t.requires_grad for t in (rows.codes, rows.scales, h, out, rows.dequantize()))
+
+
 @pytest.mark.parametrize("act", ACTIVATIONS)
 @pytest.mark.parametrize("dt", DTYPES)
 def test_activations(act, dt):
