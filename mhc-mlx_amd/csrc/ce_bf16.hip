@@ -4,7 +4,7 @@
 namespace mhc {
 namespace ce {
 
-MHC_CE_DEFINE(bf16, __bf16)
+const Runs& runs_bf16() { return runs_of<__bf16>(); }
 
 }  // namespace ce
 }  // namespace mhc

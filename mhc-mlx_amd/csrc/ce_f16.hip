@@ -4,7 +4,7 @@
 namespace mhc {
 namespace ce {
 
-MHC_CE_DEFINE(f16, _Float16)
+const Runs& runs_f16() { return runs_of<_Float16>(); }
 
 }  // namespace ce
 }  // namespace mhc

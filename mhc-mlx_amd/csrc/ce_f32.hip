@@ -4,7 +4,7 @@
 namespace mhc {
 namespace ce {
 
-MHC_CE_DEFINE(f32, float)
+const Runs& runs_f32() { return runs_of<float>(); }
 
 }  // namespace ce
 }  // namespace mhc

@@ -176,9 +176,9 @@ __global__ __launch_bounds__(kOne) void ce_loss_kernel(const State s, const doub
   loss[0] = rows == 0 ? 0.f : (float)(-sum * (double)reinterpret_cast<float*>(s.head)[2] / *reinterpret_cast<double*>(s.head + 4));
 }
 
-// dx of every token from the live ones' sums, scaled: zeros for the others
+// dx of every token from the live ones' sums, of each part of the reduction, scaled: zeros for the others
 template <typename T>
-__global__ __launch_bounds__(256) void ce_scatter_kernel(const float* sums, const State s, const float* dloss, float scale, T* dx, int64_t tokens,
+__global__ __launch_bounds__(256) void ce_scatter_kernel(const float* sums, int parts, const State s, const float* dloss, float scale, T* dx, int64_t tokens,
                                                          int64_t C, uint32_t groups) {
   constexpr int V = 8;
   const float by = reinterpret_cast<const float*>(s.head)[1] * (dloss != nullptr ? dloss[0] : 1.f) * scale;
@@ -187,8 +187,15 @@ __global__ __launch_bounds__(256) void ce_scatter_kernel(const float* sums, cons
     const int left = (int)min((int64_t)V, C - n), pos = s.pos[t];
     float z[V] = {};
     if (pos >= 0) {
-      if (left == V) gemm::take<true>(sums + pos * C + n, z, V);
-      else gemm::take<false>(sums + pos * C + n, z, left);
+#pragma unroll 4
+      for (int q = 0; q < parts; ++q) {
+        const float* const p = sums + (q * tokens + pos) * C + n;
+        float v[V];
+        if (left == V) gemm::take<true>(p, v, V);
+        else gemm::take<false>(p, v, left);
+#pragma unroll
+        for (int k = 0; k < V; ++k) z[k] += v[k];
+      }
 #pragma unroll
       for (int k = 0; k < V; ++k) z[k] *= by;
     }
@@ -196,6 +203,8 @@ __global__ __launch_bounds__(256) void ce_scatter_kernel(const float* sums, cons
     else gemm::put<false>(dx + t * C + n, z, left);
   }
 }
+
+const ce::Runs& runs_of(int dtype) { return dtype == kF32 ? ce::runs_f32() : dtype == kBF16 ? ce::runs_bf16() : ce::runs_f16(); }
 
 struct FwdPlan {
   Cut cut;
@@ -217,9 +226,10 @@ FwdPlan plan_fwd(const mhc_linear_ce_args& a) {
 }
 
 struct BwdPlan {
-  int64_t piece;                        // columns of the vocabulary
-  Cut dz, dx, dw;
-  size_t x, w, of_dz, sums, part, total;  // bytes
+  int64_t piece;   // columns of the vocabulary
+  bool joint;      // a piece's dx and dW go with the next one's dz
+  Cut dz, dx, dw;  // dx.splits: parts of its reduction, each with sums of its own over all pieces
+  size_t x, w, of_dz, sums, part, total;  // bytes; two of of_dz where joint
 };
 
 BwdPlan plan_bwd(const mhc_linear_ce_args& a, bool dx, bool dw) {
@@ -227,14 +237,29 @@ BwdPlan plan_bwd(const mhc_linear_ce_args& a, bool dx, bool dw) {
   const int64_t e = gemm::elem_bytes(a.dtype), pieces = std::max<int64_t>(1, ceil_div(a.T * a.V * e, kPieceBytes));
   p.piece = std::min(a.V, ceil_div(ceil_div(a.V, pieces), 256) * 256);
   p.dz = gemm::cut_of(a.T, p.piece, a.C, a.dtype, true, true, 1);
-  if (dx) p.dx = gemm::cut_of(a.T, a.C, p.piece, a.dtype, true, false);
-  if (dw) p.dw = gemm::cut_of(p.piece, a.C, a.T, a.dtype, false, false);
+  // (whichever is asked for: a gradient does not depend on that)
+  p.dx = gemm::cut_of(a.T, a.C, p.piece, a.dtype, true, false);
+  p.dw = gemm::cut_of(p.piece, a.C, a.T, a.dtype, false, false);
+  if (a.dtype != kF32 && gemm::most_rows(true, a.C, a.dtype) >= 256) {
+    // One launch of 256 x 256 tiles: as long as all of its stages take on all CUs (a twentieth more for its end), if dx's
+    // reduction is cut so that no tile takes more than half of that, and at least as long as its longest tile.
+    const gemm::TileCost& c = gemm::kTiles[0];
+    const float cus = (float)device_cu_count();
+    const int kK = gemm::stage_k(a.dtype), deep = (int)ceil_div(p.piece, kK), low = (int)ceil_div(a.T, kK), of_c = (int)ceil_div(a.C, kK);
+    const float mt = (float)ceil_div(a.T, 256), mv = (float)ceil_div(p.piece, 256), mc = (float)ceil_div(a.C, 256);
+    const float units = mt * mc * deep + mv * mc * low + (p.piece < a.V ? mt * mv * of_c : 0.f);
+    const int splits = std::min(16, std::max(1, (int)ceilf(2.f * deep * cus / units))), per = (int)ceil_div(deep, splits);
+    const float us = c.ends + std::max(1.05f * units / cus * gemm::stage_us(c, a.dtype, 1.f), std::max(std::max(per, low), of_c) * gemm::stage_us(c, a.dtype, 0.f));
+    const float apart = p.dx.us + p.dw.us + (p.piece < a.V ? p.dz.us : 0.f);
+    p.joint = us < apart;
+    if (p.joint) p.dx.splits = (int)ceil_div(deep, per), p.dx.kper = per * kK;
+  }
   p.x = up256((size_t)(a.T * padded(a.C, a.dtype) * e));
   p.w = gemm::pack_bytes(a.w, a.V, a.ldw, a.C, a.dtype);
   p.of_dz = up256((size_t)(a.T * padded(p.piece, a.dtype) * e));
-  if (dx) p.sums = up256((size_t)(a.T * a.C) * sizeof(float));
-  p.part = std::max(dx ? gemm::part_bytes(p.dx, a.T, a.C) : 0, dw ? gemm::part_bytes(p.dw, p.piece, a.C) : 0);
-  p.total = p.x + p.w + p.of_dz + p.sums + p.part;
+  if (dx) p.sums = up256((size_t)(p.dx.splits * a.T * a.C) * sizeof(float));
+  p.part = dw && !p.joint ? gemm::part_bytes(p.dw, p.piece, a.C) : 0;
+  p.total = p.x + p.w + p.of_dz * (p.joint && p.piece < a.V ? 2 : 1) + p.sums + p.part;
   return p;
 }
 
@@ -252,10 +277,10 @@ int run_gather(const mhc_linear_ce_args& a, const State& st, void* to, hipStream
 }
 
 template <typename T>
-int run_scatter(const mhc_linear_ce_args& a, const float* sums, const State& st, const float* dloss, float scale, void* dx, hipStream_t s) {
+int run_scatter(const mhc_linear_ce_args& a, const float* sums, int parts, const State& st, const float* dloss, float scale, void* dx, hipStream_t s) {
   const uint32_t groups = (uint32_t)ceil_div(a.C, 8);
   const dim3 grid((unsigned)std::min(ceil_div(a.T * groups, 256), (int64_t)device_cu_count() * 16));
-  hipLaunchKernelGGL((ce_scatter_kernel<T>), grid, dim3(256), 0, s, sums, st, dloss, scale * (1.f / ce::kDzUnit<T>), static_cast<T*>(dx), a.T, a.C,
+  hipLaunchKernelGGL((ce_scatter_kernel<T>), grid, dim3(256), 0, s, sums, parts, st, dloss, scale * (1.f / ce::kDzUnit<T>), static_cast<T*>(dx), a.T, a.C,
                      groups);
   MHC_CHECK_LAUNCH("ce_scatter_kernel");
   return MHC_OK;
@@ -313,8 +338,7 @@ extern "C" int mhc_linear_ce_fwd(const mhc_linear_ce_args* args, float* loss, fl
     float2* const part = reinterpret_cast<float2*>(ws);
     float* const at_target = reinterpret_cast<float*>(ws + p.part);
     terms = reinterpret_cast<double*>(ws + p.part + p.at_target);
-    const auto run = a.dtype == kF32 ? ce::run_sums_f32 : a.dtype == kBF16 ? ce::run_sums_bf16 : ce::run_sums_f16;
-    if (const int rc = run(q, p.cut, st.head, st.target, part, at_target, s)) return rc;
+    if (const int rc = runs_of(a.dtype).sums(q, p.cut, st.head, st.target, part, at_target, s)) return rc;
     hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)std::min(ceil_div(a.T, 4), kMaxGrid)), dim3(256), 0, s, st, (const float2*)part,
                        (const float*)at_target, p.tiles, logp, terms);
     MHC_CHECK_LAUNCH("ce_rows_kernel");
@@ -350,32 +374,60 @@ extern "C" int mhc_linear_ce_bwd(const mhc_linear_ce_args* args, const void* sta
   ws += p.x;
   Operand w;
   if (const int rc = gemm::operand(w, a.w, a.V, a.ldw, a.C, a.dtype, ws, s)) return rc;
-  char* const dz = ws;
-  float* const sums = reinterpret_cast<float*>(dz + p.of_dz);
-  float* const part = reinterpret_cast<float*>(dz + p.of_dz + p.sums);
+  char* const dz[2] = {ws, ws + (p.joint && p.piece < a.V ? p.of_dz : 0)};
+  float* const sums = reinterpret_cast<float*>(dz[1] + p.of_dz);
+  float* const part = reinterpret_cast<float*>(dz[1] + p.of_dz + p.sums);
   const float* const unit = reinterpret_cast<const float*>(st.head) + 1;
   const float lift = a.dtype == kF16 ? ce::kDzUnit<_Float16> : 1.f;
-  const auto run_dz = a.dtype == kF32 ? ce::run_dz_f32 : a.dtype == kBF16 ? ce::run_dz_bf16 : ce::run_dz_f16;
-  const auto run_dx = a.dtype == kF32 ? ce::run_dx_f32 : a.dtype == kBF16 ? ce::run_dx_bf16 : ce::run_dx_f16;
-  const auto run_dw = a.dtype == kF32 ? ce::run_dw_f32 : a.dtype == kBF16 ? ce::run_dw_bf16 : ce::run_dw_f16;
+  const ce::Runs& run = runs_of(a.dtype);
+  const ScaledBy by = {unit, dloss, grad_scale / lift};
+  // the products of the piece from column v0 on, whose dz is in buffer b
+  const auto columns = [&](int64_t v0) { return std::min(p.piece, a.V - v0); };
+  const auto rows_of = [&](int64_t v0) { return Operand{static_cast<const char*>(w.p) + v0 * w.ld * e, w.ld, w.width}; };
+  const auto pitch = [&](int64_t v0) { return padded(columns(v0), a.dtype); };
+  const auto of_dz = [&](int64_t v0, int b) {
+    return Product{x, rows_of(v0), a.T, columns(v0), a.C, Epilogue{nullptr, nullptr, dz[b], nullptr, MHC_ACT_NONE, a.dtype == kF32}, 1, p.dz.kper};
+  };
+  const auto gradient = [&](int64_t v0) { return Gradient{st.target, st.coef, st.top, st.inv, v0, lift}; };
+  const auto of_dx = [&](int64_t v0, int b) {
+    return Product{Operand{dz[b], pitch(v0), pitch(v0)}, rows_of(v0), a.T, a.C, columns(v0),
+                   Epilogue{nullptr, v0 > 0 ? sums : nullptr, sums, nullptr, MHC_ACT_NONE, 1}, p.dx.splits, p.dx.kper};
+  };
+  const auto of_dw = [&](int64_t v0, int b) {
+    char* const out = static_cast<char*>(dw) + v0 * a.C * e;
+    return Product{Operand{dz[b], pitch(v0), pitch(v0)}, x, columns(v0), a.C, a.T,
+                   Epilogue{nullptr, nullptr, out, nullptr, MHC_ACT_NONE, a.dtype == kF32}, 1, p.dw.kper};
+  };
+  int b = 0;
   for (int64_t v0 = 0; v0 < a.V; v0 += p.piece) {
-    const int64_t n = std::min(p.piece, a.V - v0), pitch = padded(n, a.dtype);
-    const Operand piece = {static_cast<const char*>(w.p) + v0 * w.ld * e, w.ld, w.width};
-    const Operand d = {dz, pitch, pitch};
-    const Product pz = {x, piece, a.T, n, a.C, Epilogue{nullptr, nullptr, dz, nullptr, MHC_ACT_NONE, a.dtype == kF32}, 1, 0};
-    if (const int rc = run_dz(pz, p.dz, st.head, pitch, Gradient{st.target, st.coef, st.top, st.inv, v0, lift}, s)) return rc;
+    if (v0 == 0 || !p.joint) {
+      if (const int rc = run.dz(of_dz(v0, b), p.dz, st.head, pitch(v0), gradient(v0), s)) return rc;
+    }
+    if (p.joint) {
+      ce::Joint j = {of_dx(v0, b), of_dw(v0, b), {}, a.T * a.C, 0, by, {}};
+      if (dx == nullptr) j.dx.M = 0;
+      if (dw == nullptr) j.dw.M = 0;
+      const int all = (int)ceil_div(a.T, gemm::stage_k(a.dtype)) * gemm::stage_k(a.dtype);
+      j.dw.kper = all;
+      j.dz.splits = 1;
+      if (const int64_t next = v0 + p.piece; next < a.V) {
+        j.dz = of_dz(next, b ^ 1);
+        j.width = pitch(next);
+        j.g = gradient(next);
+      }
+      if (const int rc = run.joint(j, st.head, s)) return rc;
+      b ^= 1;
+      continue;
+    }
     if (dx != nullptr) {
-      const Product px = {d, piece, a.T, a.C, n, Epilogue{nullptr, v0 > 0 ? sums : nullptr, sums, nullptr, MHC_ACT_NONE, 1}, 1, 0};
-      if (const int rc = run_dx(px, p.dx, st.head, part, s)) return rc;
+      if (const int rc = run.dx(of_dx(v0, b), p.dx, st.head, s)) return rc;
     }
     if (dw != nullptr) {
-      char* const out = static_cast<char*>(dw) + v0 * a.C * e;
-      const Product pw = {d, x, n, a.C, a.T, Epilogue{nullptr, nullptr, out, nullptr, MHC_ACT_NONE, a.dtype == kF32}, 1, 0};
-      if (const int rc = run_dw(pw, p.dw, st.head, ScaledBy{unit, dloss, grad_scale / lift}, part, s)) return rc;
+      if (const int rc = run.dw(of_dw(v0, b), p.dw, st.head, by, part, s)) return rc;
     }
   }
   if (dx == nullptr) return MHC_OK;
-  if (a.dtype == kF32) return run_scatter<float>(a, sums, st, dloss, grad_scale, dx, s);
-  if (a.dtype == kBF16) return run_scatter<__bf16>(a, sums, st, dloss, grad_scale, dx, s);
-  return run_scatter<_Float16>(a, sums, st, dloss, grad_scale, dx, s);
+  if (a.dtype == kF32) return run_scatter<float>(a, sums, p.dx.splits, st, dloss, grad_scale, dx, s);
+  if (a.dtype == kBF16) return run_scatter<__bf16>(a, sums, p.dx.splits, st, dloss, grad_scale, dx, s);
+  return run_scatter<_Float16>(a, sums, p.dx.splits, st, dloss, grad_scale, dx, s);
 }

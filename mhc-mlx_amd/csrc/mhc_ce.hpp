@@ -104,12 +104,86 @@ MHC_DEV bool limit(Product& p, const int* live, uint32_t tile) {
   }
 }
 
-template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS, typename Then>
+// One part of a reduction whose parts have outputs of their own, one after the
+// other, which sum up what the calls for pieces of it add.
+MHC_DEV void move_to_part(Epilogue& e, int64_t at) {
+  e.out = static_cast<float*>(e.out) + at;
+  if (e.residual != nullptr) e.residual = static_cast<const float*>(e.residual) + at;
+}
+
+// (SUMS: the parts of a reduction add to sums of their own)
+template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS, bool SUMS, typename Then>
 __global__ __launch_bounds__(64 * WM * WN) void live_tile_kernel(Product p, const int* live, int64_t width, const Then then) {
   __shared__ __attribute__((aligned(1024))) char smem[gemm::TileBytes<T, BM, BN, WM, WN, NS>::kAll];
   const int64_t part = p.M * p.N;
   if (!limit<AK, BM, BN>(p, live, blockIdx.x)) return;
+  if constexpr (SUMS) {
+    move_to_part(p.e, blockIdx.y * part);
+    p.splits = 1;
+  }
   gemm::run_tile<T, AK, BK, BM, BN, WM, WN, NS, T>(p, smem, blockIdx.x, (int)blockIdx.y, part, width, then);
+}
+
+// dx and dW of one piece of the vocabulary and dz of the next, none of which
+// needs another, as one launch, so that the card is full to its end: their
+// tiles are few and long (6144 tokens, 50257 columns in four pieces, C = 4096:
+// 384 of 196 stages on 256 CUs, 800 of 96 and 1200 of 64; 1.62 ms in one launch,
+// 1.88 in three).  The longest go first.  fp32 tiles gain nothing by it (1000
+// tokens, 32768 columns, C = 1024: 0.79 ms for dx and dW, 0.74 apart).
+struct Joint {
+  Product dx, dw, dz;   // M = 0: not there
+  int64_t part, width;  // of a part of dx's sums, and of dz's rows
+  ScaledBy by;
+  Gradient g;
+};
+
+// A kernel's first argument where it lies, to be read when it is needed: those
+// of all three products at once are more than there are scalar registers.
+template <typename A>
+MHC_DEV const A& first_argument() {
+  auto* p = (const __attribute__((address_space(4))) A*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const A*)p;
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int NS>
+__global__ __launch_bounds__(64 * WM * WN) void joint_kernel(const Joint, const int* live) {
+  __shared__ __attribute__((aligned(1024))) char smem[gemm::TileBytes<T, BM, BN, WM, WN, NS>::kAll];
+  const int64_t n = __builtin_amdgcn_readfirstlane(*live);
+  const auto tiles = [](int64_t M, int64_t N) { return (uint32_t)(ceil_div(M, BM) * ceil_div(N, BN)); };
+  const Joint& j = first_argument<Joint>();
+  uint32_t id = blockIdx.x;
+  const uint32_t of_dx = tiles(min(j.dx.M, n), j.dx.N), all_dx = of_dx * j.dx.splits, of_dw = tiles(j.dw.M, j.dw.N);
+  if (id < all_dx) {
+    const Joint& k = first_argument<Joint>();
+    Product p = k.dx;
+    p.M = min(p.M, n);
+    p.splits = 1;
+    move_to_part(p.e, id / of_dx * k.part);
+    gemm::run_tile<T, true, false, BM, BN, WM, WN, NS, T>(p, smem, id % of_dx, (int)(id / of_dx), 0, p.N);
+  } else if (id - all_dx < of_dw) {
+    const Joint& k = first_argument<Joint>();
+    Product p = k.dw;
+    p.K = min(p.K, n);
+    gemm::run_tile<T, false, false, BM, BN, WM, WN, NS, T>(p, smem, id - all_dx, 0, 0, p.N, ScaledBy(k.by));
+  } else {
+    const Joint& k = first_argument<Joint>();
+    Product p = k.dz;
+    p.M = min(p.M, n);
+    id -= all_dx + of_dw;
+    if (id >= tiles(p.M, p.N)) return;
+    gemm::run_tile<T, true, true, BM, BN, WM, WN, NS, T>(p, smem, id, 0, 0, k.width, GradientOf<sizeof(T) == 2>{k.g});
+  }
+}
+
+template <typename T>
+int run_joint(const Joint& j, const int* live, hipStream_t s) {
+  constexpr int kB = 256;
+  const auto tiles = [](int64_t M, int64_t N) { return ceil_div(M, kB) * ceil_div(N, kB); };
+  const int64_t grid = tiles(j.dx.M, j.dx.N) * j.dx.splits + tiles(j.dw.M, j.dw.N) + tiles(j.dz.M, j.dz.N);
+  hipLaunchKernelGGL((joint_kernel<T, kB, kB, 2, 4, 2>), dim3((unsigned)grid), dim3(512), 0, s, j, live);
+  MHC_CHECK_LAUNCH("joint_kernel");
+  return MHC_OK;
 }
 
 // exp(x - top) below `top`; a part of a row that is -inf alone has no top, and -inf - -inf would be NaN
@@ -204,59 +278,69 @@ int run_sums(Product p, const Cut& c, const int* live, const int* target, float2
   }
 }
 
-template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS, typename Then>
+template <typename T, bool AK, bool BK, bool SUMS, int BM, int BN, int WM, int WN, int NS, typename Then>
 int launch_live(const Product& p, const int* live, int64_t width, const Then& then, hipStream_t s) {
   const dim3 grid((unsigned)(ceil_div(p.M, BM) * ceil_div(p.N, BN)), (unsigned)p.splits), block(64 * WM * WN);
-  hipLaunchKernelGGL((live_tile_kernel<T, AK, BK, BM, BN, WM, WN, NS, Then>), grid, block, 0, s, p, live, width, then);
+  hipLaunchKernelGGL((live_tile_kernel<T, AK, BK, BM, BN, WM, WN, NS, SUMS, Then>), grid, block, 0, s, p, live, width, then);
   MHC_CHECK_LAUNCH("live_tile_kernel");
   return MHC_OK;
 }
 
-// width: of the outputs' rows; part: the sums of a reduction's parts, if it is split
-template <typename T, bool AK, bool BK, typename Then>
+// width: of the outputs' rows; part: the sums of a reduction's parts, if it is split (and not SUMS)
+template <typename T, bool AK, bool BK, bool SUMS, typename Then>
 int run_live(Product p, const Cut& c, const int* live, int64_t width, const Then& then, float* part, hipStream_t s) {
   using gemm::kRowWaves;
   const Epilogue e = p.e;
   p.splits = c.splits;
   p.kper = c.kper;
-  if (c.splits > 1) p.e = Epilogue{nullptr, nullptr, part, nullptr, MHC_ACT_NONE, 1};
+  if (c.splits > 1 && !SUMS) p.e = Epilogue{nullptr, nullptr, part, nullptr, MHC_ACT_NONE, 1};
   int rc;
   switch (c.tile) {
-    case 0: rc = launch_live<T, AK, BK, 256, 256, 2, 4, 2>(p, live, width, then, s); break;
-    case 1: rc = launch_live<T, AK, BK, 128, 256, 2, 4, 2>(p, live, width, then, s); break;
-    case 2: rc = launch_live<T, AK, BK, 128, 128, kRowWaves<T>, 2, 2>(p, live, width, then, s); break;
-    case 3: rc = launch_live<T, AK, BK, 64, 128, kRowWaves<T>, 2, 3>(p, live, width, then, s); break;
-    default: rc = launch_live<T, AK, BK, 64, 64, 4, 1, 3>(p, live, width, then, s); break;
+    case 0: rc = launch_live<T, AK, BK, SUMS, 256, 256, 2, 4, 2>(p, live, width, then, s); break;
+    case 1: rc = launch_live<T, AK, BK, SUMS, 128, 256, 2, 4, 2>(p, live, width, then, s); break;
+    case 2: rc = launch_live<T, AK, BK, SUMS, 128, 128, kRowWaves<T>, 2, 2>(p, live, width, then, s); break;
+    case 3: rc = launch_live<T, AK, BK, SUMS, 64, 128, kRowWaves<T>, 2, 3>(p, live, width, then, s); break;
+    default: rc = launch_live<T, AK, BK, SUMS, 64, 64, 4, 1, 3>(p, live, width, then, s); break;
   }
-  if (rc != MHC_OK || c.splits == 1) return rc;
+  if (rc != MHC_OK || c.splits == 1 || SUMS) return rc;
   return gemm::launch_join<T>(e, part, c.splits, p.M, p.N, s);
 }
 
-#define MHC_CE_DECLARE(NAME)                                                                                                         \
-  int run_sums_##NAME(const Product& p, const Cut& c, const int* live, const int* target, float2* part, float* at_target, hipStream_t s); \
-  int run_dz_##NAME(const Product& p, const Cut& c, const int* live, int64_t width, const Gradient& g, hipStream_t s);                              \
-  int run_dx_##NAME(const Product& p, const Cut& c, const int* live, float* part, hipStream_t s);                                    \
-  int run_dw_##NAME(const Product& p, const Cut& c, const int* live, const ScaledBy& by, float* part, hipStream_t s);
+// The launches of one type, each compiled in a file of its own.
+struct Runs {
+  int (*sums)(Product p, const Cut& c, const int* live, const int* target, float2* part, float* at_target, hipStream_t s);
+  int (*dz)(const Product& p, const Cut& c, const int* live, int64_t width, const Gradient& g, hipStream_t s);
+  int (*dx)(const Product& p, const Cut& c, const int* live, hipStream_t s);
+  int (*dw)(const Product& p, const Cut& c, const int* live, const ScaledBy& by, float* part, hipStream_t s);
+  int (*joint)(const Joint& j, const int* live, hipStream_t s);  // of 16-bit operands
+};
+const Runs& runs_f32();
+const Runs& runs_bf16();
+const Runs& runs_f16();
 
-MHC_CE_DECLARE(f32)
-MHC_CE_DECLARE(bf16)
-MHC_CE_DECLARE(f16)
+template <typename T>
+int run_dz(const Product& p, const Cut& c, const int* live, int64_t width, const Gradient& g, hipStream_t s) {
+  return run_live<T, true, true, false>(p, c, live, width, GradientOf<sizeof(T) == 2>{g}, nullptr, s);
+}
+template <typename T>
+int run_dx(const Product& p, const Cut& c, const int* live, hipStream_t s) {
+  return run_live<T, true, false, true>(p, c, live, p.N, gemm::AsTheyAre{}, nullptr, s);
+}
+template <typename T>
+int run_dw(const Product& p, const Cut& c, const int* live, const ScaledBy& by, float* part, hipStream_t s) {
+  return run_live<T, false, false, false>(p, c, live, p.N, by, part, s);
+}
 
-// the functions above for a type, in a file of its own
-#define MHC_CE_DEFINE(NAME, T)                                                                                                       \
-  int run_sums_##NAME(const Product& p, const Cut& c, const int* live, const int* target, float2* part, float* at_target,            \
-                      hipStream_t s) {                                                                                               \
-    return run_sums<T>(p, c, live, target, part, at_target, s);                                                                      \
-  }                                                                                                                                  \
-  int run_dz_##NAME(const Product& p, const Cut& c, const int* live, int64_t width, const Gradient& g, hipStream_t s) {                             \
-    return run_live<T, true, true>(p, c, live, width, GradientOf<sizeof(T) == 2>{g}, nullptr, s);                                           \
-  }                                                                                                                                  \
-  int run_dx_##NAME(const Product& p, const Cut& c, const int* live, float* part, hipStream_t s) {                                   \
-    return run_live<T, true, false>(p, c, live, p.N, gemm::AsTheyAre{}, part, s);                                                         \
-  }                                                                                                                                  \
-  int run_dw_##NAME(const Product& p, const Cut& c, const int* live, const ScaledBy& by, float* part, hipStream_t s) {               \
-    return run_live<T, false, false>(p, c, live, p.N, by, part, s);                                                                       \
+template <typename T>
+const Runs& runs_of() {
+  if constexpr (sizeof(T) == 2) {
+    static const Runs r = {run_sums<T>, run_dz<T>, run_dx<T>, run_dw<T>, run_joint<T>};
+    return r;
+  } else {
+    static const Runs r = {run_sums<T>, run_dz<T>, run_dx<T>, run_dw<T>, nullptr};
+    return r;
   }
+}
 
 }  // namespace ce
 }  // namespace mhc
