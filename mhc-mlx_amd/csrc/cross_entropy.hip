@@ -31,79 +31,96 @@ using gemm::Product;
 using gemm::padded;
 using gemm::up256;
 
-constexpr int kOne = 1024;  // threads of the kernels of one workgroup
+// Threads of the kernels of one workgroup: few for few tokens.
+constexpr int kFew = 256, kMany = 1024;
 
 // dz of a piece of the vocabulary takes at most about this much.
 constexpr int64_t kPieceBytes = 256 << 20;
 
 MHC_DEV float weight_of(const mhc_linear_ce_args& a, int64_t t) {
-  if (a.targets[t] == a.ignore_index) return 0.f;
   if (a.weights == nullptr) return 1.f;
   return a.weights_dtype == MHC_DTYPE_U8 ? (static_cast<const uint8_t*>(a.weights)[t] != 0 ? 1.f : 0.f)
                                          : static_cast<const float*>(a.weights)[t];
 }
 
-// The live tokens, in order, and D: one workgroup, whose threads each have a run of the tokens.
-__global__ __launch_bounds__(kOne) void ce_live_kernel(const mhc_linear_ce_args a, float* logp, const State s) {
-  __shared__ int counts[kOne / kWave];
-  __shared__ double sums[kOne / kWave];
-  __shared__ float tops[kOne / kWave];
+// The live tokens, in order, with their weights, and D: one workgroup, whose
+// threads have kRun tokens each of a chunk.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void ce_live_kernel(const mhc_linear_ce_args a, float* logp, const State s) {
+  constexpr int kRun = 8, kWaves = THREADS / kWave;
+  __shared__ int counts[kWaves];
+  __shared__ double sums[kWaves];
+  __shared__ float tops[kWaves];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int64_t per = ceil_div(a.T, kOne), t0 = min(a.T, threadIdx.x * per), t1 = min(a.T, t0 + per);
-  int count = 0;
+  int total = 0;  // of the chunks before
   double sum = 0;
   float top = 0.f;
-  for (int64_t t = t0; t < t1; ++t) {
-    const float w = weight_of(a, t);
-    count += w != 0.f;
-    sum += (double)w;
-    top = fmaxf(top, fabsf(w));
-  }
-  int before = count;  // of the wave's lanes up to this one
+  for (int64_t first = 0; first < a.T; first += THREADS * kRun) {
+    const int64_t t0 = first + threadIdx.x * kRun;
+    float w[kRun];
+    int64_t y[kRun];
 #pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const int up = __shfl_up(before, d);
-    if (lane >= d) before += up;
+    for (int k = 0; k < kRun; ++k) {  // (tokens past the last one read it once more: a load under a condition would wait for itself)
+      const int64_t t = min(t0 + k, a.T - 1);
+      w[k] = weight_of(a, t);
+      y[k] = a.targets[t];
+    }
+    int count = 0;
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+      if (t0 + k >= a.T || y[k] == a.ignore_index) w[k] = 0.f;
+      count += w[k] != 0.f;
+      sum += (double)w[k];
+      top = fmaxf(top, fabsf(w[k]));
+    }
+    int before = count;  // of the wave's lanes up to this one
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int up = __shfl_up(before, d);
+      if (lane >= d) before += up;
+    }
+    __syncthreads();
+    if (lane == kWave - 1) counts[wave] = before;
+    __syncthreads();
+    int place = total + before - count;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+      if (v < wave) place += counts[v];
+      total += counts[v];
+    }
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+      if (t0 + k >= a.T) break;
+      const bool live = w[k] != 0.f;
+      s.pos[t0 + k] = live ? place : -1;
+      if (!live) {
+        logp[t0 + k] = 0.f;
+        continue;
+      }
+      s.index[place] = (int)(t0 + k);
+      s.target[place] = y[k] >= 0 && y[k] < a.V ? (int)y[k] : -1;
+      s.coef[place] = w[k];
+      ++place;
+    }
   }
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
   top = group_max<kWave>(top);
-  if (lane == kWave - 1) {
-    counts[wave] = before;
+  if (lane == 0) {
     sums[wave] = sum;
     tops[wave] = top;
   }
   __syncthreads();
-  int first = before - count, total = 0;
-  sum = 0;
-#pragma unroll
-  for (int w = 0; w < kOne / kWave; ++w) {
-    if (w < wave) first += counts[w];
-    total += counts[w];
-    sum += sums[w];
-    top = fmaxf(top, tops[w]);
+  if (threadIdx.x != 0) return;
+  for (int v = 1; v < kWaves; ++v) {
+    sum += sums[v];
+    top = fmaxf(top, tops[v]);
   }
-  for (int64_t t = t0; t < t1; ++t) {
-    const float w = weight_of(a, t);
-    if (w == 0.f) {
-      s.pos[t] = -1;
-      logp[t] = 0.f;
-      continue;
-    }
-    const int64_t y = a.targets[t];
-    s.pos[t] = first;
-    s.index[first] = (int)t;
-    s.target[first] = y >= 0 && y < a.V ? (int)y : -1;
-    s.coef[first] = w / top;
-    ++first;
-  }
-  if (threadIdx.x == 0) {
-    const double d = a.denominator > 0.f ? (double)a.denominator : sum != 0 ? sum : 1.0;
-    s.head[0] = total;
-    reinterpret_cast<float*>(s.head)[1] = (float)((double)top / d);
-    reinterpret_cast<float*>(s.head)[2] = top;
-    *reinterpret_cast<double*>(s.head + 4) = d;
-  }
+  const double d = a.denominator > 0.f ? (double)a.denominator : sum != 0 ? sum : 1.0;
+  s.head[0] = total;
+  reinterpret_cast<float*>(s.head)[1] = (float)((double)top / d);
+  reinterpret_cast<float*>(s.head)[2] = top;
+  *reinterpret_cast<double*>(s.head + 4) = d;
 }
 
 // the live rows of x, one after the other, in whole chunks of 16 bytes with zeros after the last element
@@ -129,7 +146,7 @@ __global__ __launch_bounds__(256) void ce_gather_kernel(const T* x, int64_t ld, 
 
 // A row's parts to its sums, and its log probability, put together in fp64
 // (log sum = e log 2 + log m with m around 1: the fp32 part stays below 0.35):
-// a wave for each row.
+// a wave for each row.  (The weights become those over the largest one here.)
 __global__ __launch_bounds__(256) void ce_rows_kernel(const State s, const float2* part, const float* at_target, int64_t tiles, float* logp,
                                                       double* terms) {
   const int lane = threadIdx.x % kWave;
@@ -154,17 +171,22 @@ __global__ __launch_bounds__(256) void ce_rows_kernel(const State s, const float
     s.top[r] = top;
     s.inv[r] = 1.f / sum;
     logp[s.index[r]] = (float)lp;
-    terms[r] = (double)s.coef[r] * lp;
+    const float coef = s.coef[r] / reinterpret_cast<const float*>(s.head)[2];
+    s.coef[r] = coef;
+    terms[r] = (double)coef * lp;
   }
 }
 
-// loss = -(largest weight / D) sum of the terms: one workgroup, a fixed order
-__global__ __launch_bounds__(kOne) void ce_loss_kernel(const State s, const double* terms, float* loss) {
-  __shared__ double lds[kOne / kWave];
+// loss = -(largest weight / D) sum of the terms: one workgroup, a fixed order.
+// (A launch of its own: counting the workgroups of the one before, so that its
+// last one goes on, takes a fence of each, and 200 us for 8192 rows.)
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void ce_loss_kernel(const State s, const double* terms, float* loss) {
+  __shared__ double lds[THREADS / kWave];
   const int rows = *s.head;
   double sum = 0;
 #pragma unroll 8
-  for (int r = threadIdx.x; r < rows; r += kOne) sum += terms[r];
+  for (int r = threadIdx.x; r < rows; r += THREADS) sum += terms[r];
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
   if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = sum;
@@ -172,7 +194,7 @@ __global__ __launch_bounds__(kOne) void ce_loss_kernel(const State s, const doub
   if (threadIdx.x != 0) return;
   sum = 0;
 #pragma unroll
-  for (int w = 0; w < kOne / kWave; ++w) sum += lds[w];
+  for (int w = 0; w < THREADS / kWave; ++w) sum += lds[w];
   loss[0] = rows == 0 ? 0.f : (float)(-sum * (double)reinterpret_cast<float*>(s.head)[2] / *reinterpret_cast<double*>(s.head + 4));
 }
 
@@ -209,6 +231,7 @@ const ce::Runs& runs_of(int dtype) { return dtype == kF32 ? ce::runs_f32() : dty
 struct FwdPlan {
   Cut cut;
   int64_t tiles;
+  bool direct;  // the live rows of x are read where they lie
   size_t x, w, part, at_target, total;  // bytes; terms come last
 };
 
@@ -217,7 +240,9 @@ FwdPlan plan_fwd(const mhc_linear_ce_args& a) {
   FwdPlan p;
   p.cut = gemm::cut_of(a.T, a.V, a.C, a.dtype, true, true, 1);
   p.tiles = ceil_div(a.V, kBn[p.cut.tile]);
-  p.x = up256((size_t)(a.T * padded(a.C, a.dtype)) * gemm::elem_bytes(a.dtype));
+  const int e = gemm::elem_bytes(a.dtype);
+  p.direct = gemm::in_words(a.x, a.ldx, a.C, e) && ((a.T - 1) * a.ldx + a.C) * e < ((int64_t)1 << 31);
+  p.x = p.direct ? 0 : up256((size_t)(a.T * padded(a.C, a.dtype)) * e);
   p.w = gemm::pack_bytes(a.w, a.V, a.ldw, a.C, a.dtype);
   p.part = up256((size_t)(a.T * p.tiles) * sizeof(float2));
   p.at_target = up256((size_t)a.T * sizeof(float));
@@ -324,26 +349,33 @@ extern "C" int mhc_linear_ce_fwd(const mhc_linear_ce_args* args, float* loss, fl
   FwdPlan p = {};
   if (a.T > 0) p = plan_fwd(a);
   MHC_CHECK_ARG(workspace_bytes >= p.total && (p.total == 0 || workspace != nullptr), "workspace too small");
-  hipLaunchKernelGGL(ce_live_kernel, dim3(1), dim3(kOne), 0, s, a, logp, st);
+  if (a.T <= kFew) hipLaunchKernelGGL((ce_live_kernel<kFew>), dim3(1), dim3(kFew), 0, s, a, logp, st);
+  else hipLaunchKernelGGL((ce_live_kernel<kMany>), dim3(1), dim3(kMany), 0, s, a, logp, st);
   MHC_CHECK_LAUNCH("ce_live_kernel");
   char* ws = static_cast<char*>(workspace);
+  float2* part = nullptr;
+  float* at_target = nullptr;
   double* terms = nullptr;
   if (a.T > 0) {
     char* const x = ws;
     ws += p.x;
-    if (const int rc = run_gather(a, st, x, s)) return rc;
-    const int64_t wide = padded(a.C, a.dtype);
-    Product q = {Operand{x, wide, wide}, {}, a.T, a.V, a.C, {}, 1, 0};
+    Product q = {Operand{a.x, a.ldx, a.C}, {}, a.T, a.V, a.C, {}, 1, 0};
+    if (!p.direct) {
+      if (const int rc = run_gather(a, st, x, s)) return rc;
+      const int64_t wide = padded(a.C, a.dtype);
+      q.a = Operand{x, wide, wide};
+    }
     if (const int rc = gemm::operand(q.b, a.w, a.V, a.ldw, a.C, a.dtype, ws, s)) return rc;
-    float2* const part = reinterpret_cast<float2*>(ws);
-    float* const at_target = reinterpret_cast<float*>(ws + p.part);
+    part = reinterpret_cast<float2*>(ws);
+    at_target = reinterpret_cast<float*>(ws + p.part);
     terms = reinterpret_cast<double*>(ws + p.part + p.at_target);
-    if (const int rc = runs_of(a.dtype).sums(q, p.cut, st.head, st.target, part, at_target, s)) return rc;
+    if (const int rc = runs_of(a.dtype).sums(q, ce::RowsOf{p.direct ? st.index : nullptr, a.T}, p.cut, st.head, st.target, part, at_target, s)) return rc;
     hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)std::min(ceil_div(a.T, 4), kMaxGrid)), dim3(256), 0, s, st, (const float2*)part,
                        (const float*)at_target, p.tiles, logp, terms);
     MHC_CHECK_LAUNCH("ce_rows_kernel");
   }
-  hipLaunchKernelGGL(ce_loss_kernel, dim3(1), dim3(kOne), 0, s, st, (const double*)terms, loss);
+  if (a.T <= kFew) hipLaunchKernelGGL((ce_loss_kernel<kFew>), dim3(1), dim3(kFew), 0, s, st, (const double*)terms, loss);
+  else hipLaunchKernelGGL((ce_loss_kernel<kMany>), dim3(1), dim3(kMany), 0, s, st, (const double*)terms, loss);
   MHC_CHECK_LAUNCH("ce_loss_kernel");
   return MHC_OK;
 }

@@ -15,7 +15,7 @@ using gemm::Product;
 // What the forward leaves for the backward, in words: the tokens that count
 // ("live"), in order, and what is known of each.
 struct State {
-  int* head;     // how many are live; then, as floats, the largest weight over D, and D
+  int* head;     // how many are live; as floats, the largest weight over D, and the largest weight; as a double from word 4 on, D
   int* index;    // [T] their tokens
   int* pos;      // [T] of each token: its place among them, or -1
   int* target;   // [T] by place: -1 where it is no column
@@ -189,19 +189,30 @@ int run_joint(const Joint& j, const int* live, hipStream_t s) {
 // exp(x - top) below `top`; a part of a row that is -inf alone has no top, and -inf - -inf would be NaN
 MHC_DEV float base_of(float top) { return top == -__builtin_inff() ? 0.f : top; }
 
+// The live tokens' rows: where they lie in x, or one after the other.
+struct RowsOf {
+  const int* index;  // or NULL
+  int64_t rows;
+  template <typename L, typename P>
+  MHC_DEV void init(L& l, const Product& p, const P& at, uint32_t lds) const {
+    l.init(p.a, index != nullptr ? 0 : at.m0, index != nullptr ? rows : p.M, at.k0, at.k1, at.wave, at.lane, lds);
+    if (index != nullptr) l.take_rows(p.a, index, at.m0, p.M, at.wave, at.lane);
+  }
+};
+
 // A tile of logits, of which only each row's largest and the sum of
 // exp(logit - largest) are kept, and the target's: to part[row][column of
 // tiles] and at_target[row].
 template <typename T, int BM, int BN, int WM, int WN, int NS>
-__global__ __launch_bounds__(64 * WM * WN) void sums_tile_kernel(Product p, const int* live, const int* target, float2* part, float* at_target) {
+__global__ __launch_bounds__(64 * WM * WN) void sums_tile_kernel(Product p, const RowsOf rows, const int* live, const int* target, float2* part, float* at_target) {
   __shared__ __attribute__((aligned(1024))) char smem[NS * (BM + BN) * 128];
   if (!limit<true, BM, BN>(p, live, blockIdx.x)) return;
   constexpr int JM = BM / WM / 16, JN = BN / WN / 16, kThreads = 64 * WM * WN;
   constexpr bool kFast = sizeof(T) == 2;
   const gemm::Place<BM, BN, WM, WN> at(p, blockIdx.x, 0);
   f32x4 acc[JN][JM] = {};
-  if constexpr (gemm::kSplit<T, BN>) gemm::sum_tile_split<true, true, BM, BN, WM, WN, NS>(p, at, smem, acc);
-  else gemm::sum_tile<T, true, true, BM, BN, WM, WN, NS>(p, at, smem, acc);
+  if constexpr (gemm::kSplit<T, BN>) gemm::sum_tile_split<true, true, BM, BN, WM, WN, NS>(p, at, smem, acc, rows);
+  else gemm::sum_tile<T, true, true, BM, BN, WM, WN, NS>(p, at, smem, acc, rows);
   const int64_t m0 = at.m0 + at.wm + at.lane % 16, n0 = at.n0 + at.wn + at.lane / 16 * 4;
   if (at.n0 + BN > p.N) {
 #pragma unroll
@@ -257,24 +268,24 @@ __global__ __launch_bounds__(64 * WM * WN) void sums_tile_kernel(Product p, cons
 }
 
 template <typename T, int BM, int BN, int WM, int WN, int NS>
-int launch_sums(const Product& p, const int* live, const int* target, float2* part, float* at_target, hipStream_t s) {
+int launch_sums(const Product& p, const RowsOf& rows, const int* live, const int* target, float2* part, float* at_target, hipStream_t s) {
   hipLaunchKernelGGL((sums_tile_kernel<T, BM, BN, WM, WN, NS>), dim3((unsigned)(ceil_div(p.M, BM) * ceil_div(p.N, BN))), dim3(64 * WM * WN), 0, s,
-                     p, live, target, part, at_target);
+                     p, rows, live, target, part, at_target);
   MHC_CHECK_LAUNCH("sums_tile_kernel");
   return MHC_OK;
 }
 
 template <typename T>
-int run_sums(Product p, const Cut& c, const int* live, const int* target, float2* part, float* at_target, hipStream_t s) {
+int run_sums(Product p, const RowsOf& rows, const Cut& c, const int* live, const int* target, float2* part, float* at_target, hipStream_t s) {
   using gemm::kRowWaves;
   p.splits = 1;
   p.kper = c.kper;
   switch (c.tile) {
-    case 0: return launch_sums<T, 256, 256, 2, 4, 2>(p, live, target, part, at_target, s);
-    case 1: return launch_sums<T, 128, 256, 2, 4, 2>(p, live, target, part, at_target, s);
-    case 2: return launch_sums<T, 128, 128, kRowWaves<T>, 2, 2>(p, live, target, part, at_target, s);
-    case 3: return launch_sums<T, 64, 128, kRowWaves<T>, 2, 3>(p, live, target, part, at_target, s);
-    default: return launch_sums<T, 64, 64, 4, 1, 3>(p, live, target, part, at_target, s);
+    case 0: return launch_sums<T, 256, 256, 2, 4, 2>(p, rows, live, target, part, at_target, s);
+    case 1: return launch_sums<T, 128, 256, 2, 4, 2>(p, rows, live, target, part, at_target, s);
+    case 2: return launch_sums<T, 128, 128, kRowWaves<T>, 2, 2>(p, rows, live, target, part, at_target, s);
+    case 3: return launch_sums<T, 64, 128, kRowWaves<T>, 2, 3>(p, rows, live, target, part, at_target, s);
+    default: return launch_sums<T, 64, 64, 4, 1, 3>(p, rows, live, target, part, at_target, s);
   }
 }
 
@@ -308,7 +319,7 @@ int run_live(Product p, const Cut& c, const int* live, int64_t width, const Then
 
 // The launches of one type, each compiled in a file of its own.
 struct Runs {
-  int (*sums)(Product p, const Cut& c, const int* live, const int* target, float2* part, float* at_target, hipStream_t s);
+  int (*sums)(Product p, const RowsOf& rows, const Cut& c, const int* live, const int* target, float2* part, float* at_target, hipStream_t s);
   int (*dz)(const Product& p, const Cut& c, const int* live, int64_t width, const Gradient& g, hipStream_t s);
   int (*dx)(const Product& p, const Cut& c, const int* live, hipStream_t s);
   int (*dw)(const Product& p, const Cut& c, const int* live, const ScaledBy& by, float* part, hipStream_t s);

@@ -386,6 +386,17 @@ struct Loader {
     lds = lds0 + wave * kLoads * 1024;
   }
 
+  // After init with i0 = 0 and all of the operand's rows as its count: index i of the tile is row index[i0 + i] instead, of
+  // which `count` are there.  No row ends 2^31 bytes from the first or further.
+  MHC_DEV void take_rows(const Operand& o, const int* index, int64_t i0, int64_t count, int wave, int lane) {
+    static_assert(KM, "rows of an index");
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int at = (wave * kLoads + i) * 64 + lane, row = at >> 3;
+      off[i] = i0 + row < count ? (uint32_t)(index[i0 + row] * o.ld * (int64_t)sizeof(T)) + (((at & 7) ^ (row & 7)) << 4) : 0xfffffff0u;
+    }
+  }
+
   // the stage at base; kleft: k from it to the end
   MHC_DEV void load(uint32_t stage, int kleft, int lane) const {
     // (offsets of the tile stay below 2^31, see kMaxRowBytes and most_rows)
@@ -614,6 +625,14 @@ struct Place {
   }
 };
 
+// Where a tile's rows of A are: one after the other.
+struct InOrder {
+  template <typename L, typename P>
+  MHC_DEV void init(L& l, const Product& p, const P& at, uint32_t lds) const {
+    l.init(p.a, at.m0, p.M, at.k0, at.k1, at.wave, at.lane, lds);
+  }
+};
+
 // The sums of a workgroup's tile.  (The first operand's index, n, runs over a
 // lane's four values.)  Bound by the matrix instructions and, beside them, the
 // LDS reads of the fragments: a wave of a 256 x 256 tile reads 24 KB for 64
@@ -622,8 +641,9 @@ struct Place {
 // library's 178).  Smaller tiles read more for each product and serve where
 // large ones would leave CUs idle; their stages are as long as their chain of
 // wait, barrier, reads and products, which more stages under way don't shorten.
-template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
-MHC_DEV void sum_tile(const Product& p, const Place<BM, BN, WM, WN>& at, char* smem, f32x4 (&acc)[BN / WN / 16][BM / WM / 16]) {
+template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS, typename Rows = InOrder>
+MHC_DEV void sum_tile(const Product& p, const Place<BM, BN, WM, WN>& at, char* smem, f32x4 (&acc)[BN / WN / 16][BM / WM / 16],
+                      const Rows& rows = {}) {
   using S = Stage<T>;
   constexpr int kWaves = WM * WN, JM = BM / WM / 16, JN = BN / WN / 16;
   constexpr int kA = BM * 128, kStage = kA + BN * 128;
@@ -632,7 +652,7 @@ MHC_DEV void sum_tile(const Product& p, const Place<BM, BN, WM, WN>& at, char* s
   Loader<T, BK, BN, kWaves> lb;
   constexpr int kLoads = decltype(la)::kLoads + decltype(lb)::kLoads;
   const uint32_t lds = lds_address(smem);
-  la.init(p.a, at.m0, p.M, at.k0, at.k1, at.wave, lane, lds);
+  rows.init(la, p, at, lds);
   lb.init(p.b, at.n0, p.N, at.k0, at.k1, at.wave, lane, lds + kA);
   Reader<T, AK, BM, JM> ra;
   Reader<T, BK, BN, JN> rb;
@@ -721,8 +741,9 @@ MHC_DEV void split8(const u32x4& lo, const u32x4& hi, u32x4 (&part)[3]) {
 // 3/8 of the time of one in fp32; the splits, on the vector unit, go on beside
 // them in another wave (the lift is one of their 6.5 instructions for a value,
 // and 5 % of the time).
-template <bool AK, bool BK, int BM, int BN, int WM, int WN, int NS>
-MHC_DEV void sum_tile_split(const Product& p, const Place<BM, BN, WM, WN>& at, char* smem, f32x4 (&acc)[BN / WN / 16][BM / WM / 16]) {
+template <bool AK, bool BK, int BM, int BN, int WM, int WN, int NS, typename Rows = InOrder>
+MHC_DEV void sum_tile_split(const Product& p, const Place<BM, BN, WM, WN>& at, char* smem, f32x4 (&acc)[BN / WN / 16][BM / WM / 16],
+                            const Rows& rows = {}) {
   using S = Stage<float>;
   constexpr int kWaves = WM * WN, JM = BM / WM / 16, JN = BN / WN / 16;
   constexpr int kA = BM * 128, kStage = kA + BN * 128;
@@ -731,7 +752,7 @@ MHC_DEV void sum_tile_split(const Product& p, const Place<BM, BN, WM, WN>& at, c
   Loader<float, BK, BN, kWaves> lb;
   constexpr int kLoads = decltype(la)::kLoads + decltype(lb)::kLoads;
   const uint32_t lds = lds_address(smem);
-  la.init(p.a, at.m0, p.M, at.k0, at.k1, at.wave, lane, lds);
+  rows.init(la, p, at, lds);
   lb.init(p.b, at.n0, p.N, at.k0, at.k1, at.wave, lane, lds + kA);
   Reader<float, AK, BM, JM> ra;
   Reader<float, BK, BN, JN> rb;
