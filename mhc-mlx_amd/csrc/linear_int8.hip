@@ -23,37 +23,46 @@ struct Scales {
   const float* bias;  // [N], or NULL
 };
 
-// four values from column n on, of those before N; zeros after
-MHC_DEV f32x4 four_of(const float* p, int64_t n, int64_t N) {
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  if (n + 4 <= N) {
-    __builtin_memcpy(&v, p + n, 16);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (n + k < N) v[k] = p[n + k];
-  }
-  return v;
-}
-
-// int32 sums to fp32 values, with the bias (in the first of a reduction's parts)
+// int32 sums to fp32 values, with the bias (in the first of a reduction's
+// parts).  The tile's scales are loaded before its sums are formed, one or two
+// numbers a thread, and shared through LDS after them.
 struct Scaled {
   Scales s;
-  template <typename P, int JM, int JN>
-  MHC_DEV void operator()(const Product& p, const P& at, int split, f32x4 (&acc)[JN][JM]) const {
-    const int64_t m0 = at.m0 + at.wm + at.lane % 16, n0 = at.n0 + at.wn + at.lane / 16 * 4;
+
+  struct Own {
+    float scale, bias;
+  };
+
+  template <int BM, int BN, int WM, int WN>
+  MHC_DEV Own ahead(const Product& p, const gemm::Place<BM, BN, WM, WN>& at) const {
+    static_assert(BM + BN <= 64 * WM * WN, "a scale for each thread");
+    const int t = threadIdx.x;
+    const int64_t n = min(at.n0 + (t < BM ? 0 : t - BM), p.N - 1);
+    const float* const from = t < BM ? s.x + min(at.m0 + t, p.M - 1) : s.w + n;
+    return {*from, s.bias != nullptr && t >= BM ? s.bias[n] : 0.f};
+  }
+
+  template <int BM, int BN, int WM, int WN, int JM, int JN>
+  MHC_DEV void operator()(const Product&, const gemm::Place<BM, BN, WM, WN>& at, int split, char* smem, const Own& own,
+                          f32x4 (&acc)[JN][JM]) const {
+    float* const lds = reinterpret_cast<float*>(smem);  // of rows, of columns, biases
+    const int t = threadIdx.x;
+    lds_barrier();  // nobody reads the stages any more
+    if (t < BM + BN) lds[t] = own.scale;
+    if (t >= BM && t < BM + BN) lds[BN + t] = own.bias;
+    lds_barrier();
     float x[JM];
 #pragma unroll
-    for (int j = 0; j < JM; ++j) x[j] = s.x[min(m0 + j * 16, p.M - 1)];
-    const bool biased = s.bias != nullptr && split == 0;
+    for (int j = 0; j < JM; ++j) x[j] = lds[at.wm + j * 16 + at.lane % 16];
 #pragma unroll
     for (int i = 0; i < JN; ++i) {
-      const f32x4 w = four_of(s.w, n0 + i * 16, p.N);
+      const float* const of_columns = lds + BM + at.wn + i * 16 + at.lane / 16 * 4;
+      const f32x4 w = *reinterpret_cast<const f32x4*>(of_columns);
       f32x4 b = {0.f, 0.f, 0.f, 0.f};
-      if (biased) b = four_of(s.bias, n0 + i * 16, p.N);
+      if (split == 0) b = *reinterpret_cast<const f32x4*>(of_columns + BN);
 #pragma unroll
       for (int j = 0; j < JM; ++j) {
-        const i32x4 sum = __builtin_bit_cast(i32x4, acc[i][j]);
+        const gemm::i32x4 sum = __builtin_bit_cast(gemm::i32x4, acc[i][j]);
         f32x4 v;
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = fmaf((float)sum[k] * x[j], w[k], b[k]);
@@ -61,13 +70,16 @@ struct Scaled {
       }
     }
   }
-  using i32x4 = gemm::i32x4;
 };
 
 template <typename O, int BM, int BN, int WM, int WN, int NS>
 __global__ __launch_bounds__(64 * WM * WN) void int8_tile_kernel(const Product p, const Scaled then) {
   __shared__ __attribute__((aligned(1024))) char smem[gemm::TileBytes<int8_t, BM, BN, WM, WN, NS>::kAll];
-  gemm::run_tile<int8_t, true, true, BM, BN, WM, WN, NS, O>(p, smem, blockIdx.x, (int)blockIdx.y, p.M * p.N, p.N, then);
+  Product q = p;
+  q.e.dact = nullptr;  // (known here, so that no derivative is formed)
+  // (without a derivative, large tiles have the registers for four rows at a time: with a residual and gelu_tanh 2048 x 8192 x
+  // 4096 79 to 72 us)
+  gemm::run_tile<int8_t, true, true, BM, BN, WM, WN, NS, O, BM * BN == 65536 ? 4 : 2>(q, smem, blockIdx.x, (int)blockIdx.y, p.M * p.N, p.N, then);
 }
 
 // Up to 64 rows: as few_rows_kernel, with the waves' sums joined as whole numbers.
@@ -95,8 +107,10 @@ __global__ __launch_bounds__(64 * gemm::kFewWaves) void int8_few_rows_kernel(con
     if (m < M && n < N) {
       const float none[1] = {};
       float z[1][1] = {{fmaf((float)sum * s.x[m], s.w[n], s.bias != nullptr ? s.bias[n] : 0.f)}}, residual[1][1];
-      gemm::residual_of<O, true>(e, m, 0, M, n, N, 1, residual);
-      gemm::finish<O, true>(e, m, 0, M, n, N, 1, z, none, residual);
+      Epilogue f = e;
+      f.dact = nullptr;  // (known here, so that no derivative is formed)
+      gemm::residual_of<O, true>(f, m, 0, M, n, N, 1, residual);
+      gemm::finish<O, true>(f, m, 0, M, n, N, 1, z, none, residual);
     }
   }
 }
@@ -135,11 +149,21 @@ int run_few(const Operand& x, const Operand& w, int64_t M, int64_t N, int64_t K,
   return MHC_OK;
 }
 
-bool few_rows(int64_t M) { return M <= 64; }
+// Whether the product goes to the kernel for few rows: up to 64 of them, unless
+// tiles are estimated faster.  A workgroup of it has 16 columns and reads all of
+// x, and takes 0.35, 0.65 or 1.05 us for 1024 k of 16, 32 or 64 rows (64 x 4096 x
+// 4096 8.1 us, tiles 11.7; 64 x 16384 x 1024 10.0 and 6.3); W's bytes go by at 5
+// TB/s there, in tiles at 6 (16 x 32000 x 4096 25.5 and 21.9, 48 rows 37.6 and 22.5).
+bool few_rows(int64_t M, int64_t N, int64_t K) {
+  if (M > 64) return false;
+  const float of_cu = std::max(1.f, (float)N / 16.f / (float)device_cu_count()), bytes = (float)(N * K) * 1e-6f;
+  const float few = 2.5f + of_cu * (float)ceil_div(K, 1024) * (M <= 16 ? 0.35f : M <= 32 ? 0.65f : 1.05f);
+  return std::max(few, bytes / 5.f) <= std::max(gemm::cut_of(M, N, K, kI8, true, true).us, bytes / 6.f);
+}
 
 template <typename O>
 int run(const Product& p, const Scales& scales, float* part, hipStream_t s) {
-  if (few_rows(p.M)) {
+  if (few_rows(p.M, p.N, p.K)) {
     if (p.M <= 16) return run_few<O, 1>(p.a, p.b, p.M, p.N, p.K, scales, p.e, s);
     if (p.M <= 32) return run_few<O, 2>(p.a, p.b, p.M, p.N, p.K, scales, p.e, s);
     return run_few<O, 4>(p.a, p.b, p.M, p.N, p.K, scales, p.e, s);
@@ -154,7 +178,7 @@ extern "C" size_t mhc_linear_int8_workspace_bytes(const int8_t* x, int64_t ldx, 
   using namespace mhc;
   if (M <= 0 || N <= 0 || K <= 0 || K >= kMaxK) return 0;
   return gemm::pack_bytes(x, M, ldx, K, kI8) + gemm::pack_bytes(w, N, ldw, K, kI8) +
-         (few_rows(M) ? 0 : gemm::part_bytes(gemm::cut_of(M, N, K, kI8, true, true), M, N));
+         (few_rows(M, N, K) ? 0 : gemm::part_bytes(gemm::cut_of(M, N, K, kI8, true, true), M, N));
 }
 
 extern "C" int mhc_linear_int8(const int8_t* x, int64_t ldx, const float* x_scales, const int8_t* w, int64_t ldw, const float* w_scales,

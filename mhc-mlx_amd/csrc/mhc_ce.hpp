@@ -70,8 +70,11 @@ struct Gradient {
 
 template <bool FAST>
 struct GradientOf : Gradient {
+  using Own = gemm::AsTheyAre::Own;
+  template <typename P>
+  MHC_DEV Own ahead(const Product&, const P&) const { return {}; }
   template <typename P, int JM, int JN>
-  MHC_DEV void operator()(const Product& p, const P& at, int, f32x4 (&acc)[JN][JM]) const {
+  MHC_DEV void operator()(const Product& p, const P& at, int, char*, const Own&, f32x4 (&acc)[JN][JM]) const {
     this->template apply<FAST>(p, at, acc);
   }
 };
@@ -80,8 +83,11 @@ struct GradientOf : Gradient {
 struct ScaledBy {
   const float *a, *b;
   float c;
+  using Own = gemm::AsTheyAre::Own;
+  template <typename P>
+  MHC_DEV Own ahead(const Product&, const P&) const { return {}; }
   template <typename P, int JM, int JN>
-  MHC_DEV void operator()(const Product&, const P&, int, f32x4 (&acc)[JN][JM]) const {
+  MHC_DEV void operator()(const Product&, const P&, int, char*, const Own&, f32x4 (&acc)[JN][JM]) const {
     const float s = a[0] * (b != nullptr ? b[0] : 1.f) * c;
 #pragma unroll
     for (int i = 0; i < JN; ++i)
@@ -104,6 +110,13 @@ MHC_DEV bool limit(Product& p, const int* live, uint32_t tile) {
   }
 }
 
+// The epilogue's sums alone, known here, so that nothing else is compiled.
+MHC_DEV void only_sums(Epilogue& e) {
+  e.bias = nullptr;
+  e.dact = nullptr;
+  e.act = MHC_ACT_NONE;
+}
+
 // One part of a reduction whose parts have outputs of their own, one after the
 // other, which sum up what the calls for pieces of it add.
 MHC_DEV void move_to_part(Epilogue& e, int64_t at) {
@@ -117,6 +130,7 @@ __global__ __launch_bounds__(64 * WM * WN) void live_tile_kernel(Product p, cons
   __shared__ __attribute__((aligned(1024))) char smem[gemm::TileBytes<T, BM, BN, WM, WN, NS>::kAll];
   const int64_t part = p.M * p.N;
   if (!limit<AK, BM, BN>(p, live, blockIdx.x)) return;
+  only_sums(p.e);
   if constexpr (SUMS) {
     move_to_part(p.e, blockIdx.y * part);
     p.splits = 1;
@@ -157,6 +171,7 @@ __global__ __launch_bounds__(64 * WM * WN) void joint_kernel(const Joint, const 
   if (id < all_dx) {
     const Joint& k = first_argument<Joint>();
     Product p = k.dx;
+    only_sums(p.e);
     p.M = min(p.M, n);
     p.splits = 1;
     move_to_part(p.e, id / of_dx * k.part);
@@ -164,11 +179,13 @@ __global__ __launch_bounds__(64 * WM * WN) void joint_kernel(const Joint, const 
   } else if (id - all_dx < of_dw) {
     const Joint& k = first_argument<Joint>();
     Product p = k.dw;
+    only_sums(p.e);
     p.K = min(p.K, n);
     gemm::run_tile<T, false, false, BM, BN, WM, WN, NS, T>(p, smem, id - all_dx, 0, 0, p.N, ScaledBy(k.by));
   } else {
     const Joint& k = first_argument<Joint>();
     Product p = k.dz;
+    only_sums(p.e);
     p.M = min(p.M, n);
     id -= all_dx + of_dw;
     if (id >= tiles(p.M, p.N)) return;

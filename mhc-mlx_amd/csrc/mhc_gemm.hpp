@@ -514,18 +514,18 @@ MHC_DEV void interleave() {
   }
 }
 
-// ROWS rows of 64 sums in LDS, as tile_kernel puts them there, to the outputs
-// from (m0, n0) on: eight columns a lane, of two rows at a time.
-template <typename T, int ROWS, bool WHOLE>
+// ROWS rows of 64 sums in LDS, as store_tile puts them there, to the outputs
+// from (m0, n0) on: eight columns a lane, of EACH rows at a time.
+template <typename T, int ROWS, int EACH, bool WHOLE>
 MHC_DEV void store_columns(const Epilogue& e, const char* sums, int lane, int64_t m0, int64_t M, int64_t n0, int64_t N, int left) {
   const int c = lane % 8 * 8;
   float bias[8];
   bias_of<T>(e, n0 + c, left, bias);
-  for (int r0 = lane / 8; r0 < ROWS && m0 + r0 < M; r0 += 16) {
-    float z[2][8], res[2][8];
+  for (int r0 = lane / 8; r0 < ROWS && m0 + r0 < M; r0 += 8 * EACH) {
+    float z[EACH][8], res[EACH][8];
     residual_of<T, WHOLE>(e, m0 + r0, 8, M, n0 + c, N, left, res);
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < EACH; ++b)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int r = r0 + b * 8;
@@ -537,11 +537,11 @@ MHC_DEV void store_columns(const Epilogue& e, const char* sums, int lane, int64_
   }
 }
 
-template <typename T, int ROWS>
+template <typename T, int ROWS, int EACH>
 MHC_DEV void store_rows(const Epilogue& e, const char* sums, int lane, int64_t m0, int64_t M, int64_t n0, int64_t N) {
   const int left = (int)max((int64_t)0, min((int64_t)8, N - n0 - lane % 8 * 8));
-  if (left == 8) store_columns<T, ROWS, true>(e, sums, lane, m0, M, n0, N, left);
-  else if (left > 0) store_columns<T, ROWS, false>(e, sums, lane, m0, M, n0, N, left);
+  if (left == 8) store_columns<T, ROWS, EACH, true>(e, sums, lane, m0, M, n0, N, left);
+  else if (left > 0) store_columns<T, ROWS, EACH, false>(e, sums, lane, m0, M, n0, N, left);
 }
 
 // The same for those of the sums that are not kKeep, one by one: rarely used, so it is short.
@@ -563,7 +563,7 @@ MHC_DEV void store_some(const Epilogue& e, const char* sums, int lane, int64_t m
 
 // A wave's JM x JN sums of 16 x 16, in registers, to the outputs from (m0, n0)
 // on, through the workgroup's LDS (BYTES of it, free).  SOME: those that are not kKeep.
-template <typename T, int JM, int JN, int WAVES, int BYTES, bool SOME = false>
+template <typename T, int JM, int JN, int WAVES, int BYTES, int EACH, bool SOME = false>
 MHC_DEV void store_tile(const Epilogue& e, char* smem, const f32x4 (&acc)[JN][JM], int64_t m0, int64_t M, int64_t n0, int64_t N, int wave,
                         int lane) {
   // The sums go through LDS, where each wave has room for up to 64 rows
@@ -576,18 +576,19 @@ MHC_DEV void store_tile(const Epilogue& e, char* smem, const f32x4 (&acc)[JN][JM
   // (a round's sums have constant indices, and those of the first are gone before the second)
   int at = lane;
   asm volatile("" : "+v"(at));  // (or addresses of the outputs would be formed before the loop and held through it)
+  // (Barriers of LDS alone: the second round does not wait for the stores of the first.)
   const auto round = [&](auto first) {
     constexpr int h = decltype(first)::value;
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (int j = 0; j < kRound; ++j)
 #pragma unroll
       for (int i = 0; i < JN; ++i)
         *reinterpret_cast<f32x4*>(mine + (j * 16 + at % 16) * 256 + (((i * 4 + at / 16) ^ (at % 16)) << 4)) = acc[i][h + j];
-    __syncthreads();
+    lds_barrier();
     const int64_t mh = m0 + h * 16;
     if constexpr (SOME) store_some<T, kRows>(e, mine, at, mh, M, n0, N);
-    else store_rows<T, kRows>(e, mine, at, mh, M, n0, N);
+    else store_rows<T, kRows, EACH>(e, mine, at, mh, M, n0, N);
   };
   static_assert(JM / kRound <= 2, "two rounds");
   round(std::integral_constant<int, 0>{});
@@ -825,19 +826,26 @@ struct TileBytes {
   static constexpr int kAll = kStages + (kSplit<T, BN> ? (kWords * kThreads + WM * WN) * 4 : 0);
 };
 
-// What becomes of a tile's sums before they are stored: nothing here.
+// What becomes of a tile's sums before they are stored: nothing here.  What
+// ahead() loads is on its way while the sums are formed; the workgroup's LDS is
+// free for a kernel that uses it after a barrier.
 struct AsTheyAre {
+  struct Own {};
+  template <typename P>
+  MHC_DEV Own ahead(const Product&, const P&) const { return {}; }
   template <typename P, int JM, int JN>
-  MHC_DEV void operator()(const Product&, const P&, int, f32x4 (&)[JN][JM]) const {}
+  MHC_DEV void operator()(const Product&, const P&, int, char*, const Own&, f32x4 (&)[JN][JM]) const {}
 };
 
 // A tile of outputs, or (split) of one part of the reduction's sums, which
-// `then` changes; T: of the operands, O: of the epilogue.  Sums on
+// `then` changes; T: of the operands, O: of the epilogue; part: sums of one
+// part; width: of the outputs' rows (N, or more, whose columns are stored too);
+// EACH: rows that a lane finishes at a time.  Sums on
 // split values that come out infinite or as NaN are formed once more with fp32
 // instructions: their values or lifted sums were past the range (2^111, 2^95),
 // or had an infinity, whose parts make NaN of everything.  The other sums of the tile stay as they are, so that a row's
 // outputs do not depend on what other rows hold.
-template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS, typename O = T, typename Then = AsTheyAre>
+template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS, typename O = T, int EACH = 2, typename Then = AsTheyAre>
 MHC_DEV void run_tile(const Product& p, char* smem, uint32_t tile, int split, int64_t part, int64_t width, const Then& then = {}) {
   using B = TileBytes<T, BM, BN, WM, WN, NS>;
   constexpr int kWaves = WM * WN, JM = BM / WM / 16, JN = BN / WN / 16;
@@ -846,10 +854,11 @@ MHC_DEV void run_tile(const Product& p, char* smem, uint32_t tile, int split, in
   Epilogue e = p.e;
   if (p.splits > 1) e.out = static_cast<float*>(e.out) + split * part;
   f32x4 acc[JN][JM] = {};
+  const auto own = then.ahead(p, at);
   if constexpr (!kSplit<T, BN>) {
     sum_tile<T, AK, BK, BM, BN, WM, WN, NS>(p, at, smem, acc);
-    then(p, at, split, acc);
-    store_tile<O, JM, JN, kWaves, B::kStages>(e, smem, acc, m0, p.M, n0, width, at.wave, at.lane);
+    then(p, at, split, smem, own, acc);
+    store_tile<O, JM, JN, kWaves, B::kStages, EACH>(e, smem, acc, m0, p.M, n0, width, at.wave, at.lane);
   } else {
     static_assert(B::kWords * 32 == JM * JN * 4);
     sum_tile_split<AK, BK, BM, BN, WM, WN, NS>(p, at, smem, acc);
@@ -890,8 +899,8 @@ MHC_DEV void run_tile(const Product& p, char* smem, uint32_t tile, int split, in
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) again |= found[w];
     again = __builtin_amdgcn_readfirstlane(again);
-    then(p, at, split, acc);
-    store_tile<O, JM, JN, kWaves, B::kStages>(e, smem, acc, m0, p.M, n0, width, at.wave, at.lane);
+    then(p, at, split, smem, own, acc);
+    store_tile<O, JM, JN, kWaves, B::kStages, EACH>(e, smem, acc, m0, p.M, n0, width, at.wave, at.lane);
     if (!again) return;
 #pragma unroll
     for (int i = 0; i < JN; ++i)
@@ -901,7 +910,7 @@ MHC_DEV void run_tile(const Product& p, char* smem, uint32_t tile, int split, in
     Place<BM, BN, WM, WN> once_more = at;
     asm volatile("" : "+v"(once_more.lane), "+s"(once_more.wave));  // (or registers would hold places from the first sums to these)
     sum_tile<T, AK, BK, BM, BN, WM, WN, NS>(p, once_more, smem, acc);  // (it waits for the wave's stores, too)
-    then(p, once_more, split, acc);
+    then(p, once_more, split, smem, own, acc);
     uint32_t mark[B::kWords] = {};
     if (mine) {
 #pragma unroll
@@ -916,7 +925,7 @@ MHC_DEV void run_tile(const Product& p, char* smem, uint32_t tile, int split, in
           const int bit = 4 * (i * JM + j) + k;
           if (!(mark[bit / 32] >> bit % 32 & 1)) acc[i][j][k] = __builtin_bit_cast(float, kKeep);
         }
-    store_tile<O, JM, JN, kWaves, B::kStages, true>(e, smem, acc, m0, p.M, n0, width, at.wave, at.lane);
+    store_tile<O, JM, JN, kWaves, B::kStages, EACH, true>(e, smem, acc, m0, p.M, n0, width, at.wave, at.lane);
   }
 }
 
@@ -1225,15 +1234,18 @@ struct Cut {
 // CU that has `fit` of them (its matrix instructions and LDS reads).  From
 // x W^T over 16 to 512 stages: 256 x 256 16-bit at 1.12 alone, 1.6 with all
 // CUs at it (1.3 PFLOP/s); a stage of fp32 has half the k (timed before values
-// were lifted, which takes 5 % more of a stage from 64 x 128 on).
+// were lifted, which takes 5 % more of a stage from 64 x 128 on).  A stage of
+// int8 has twice the k of a 16-bit one and takes its time, so that the outputs
+// count for more: `more8` for each further tile of a CU (from 1001 x 2050 x 1100
+// and 16384 x 16384 x 4096).
 struct TileCost {
   int bm, bn, fit;
-  float ends, alone16, busy16, alone32, busy32;
+  float ends, alone16, busy16, alone32, busy32, more8;
 };
 constexpr TileCost kTiles[] = {
-    {256, 256, 1, 7.0f, 1.12f, 1.60f, 4.10f, 4.75f},   {128, 256, 1, 5.0f, 0.68f, 0.92f, 2.35f, 2.60f},
-    {128, 128, 2, 5.0f, 0.48f, 0.53f, 1.67f, 1.28f},   {64, 128, 2, 4.5f, 0.35f, 0.335f, 1.03f, 0.78f},
-    {64, 64, 3, 3.6f, 0.29f, 0.21f, 0.58f, 0.525f},
+    {256, 256, 1, 7.0f, 1.12f, 1.60f, 4.10f, 4.75f, 7.0f},   {128, 256, 1, 5.0f, 0.68f, 0.92f, 2.35f, 2.60f, 6.0f},
+    {128, 128, 2, 5.0f, 0.48f, 0.53f, 1.67f, 1.28f, 0.5f},   {64, 128, 2, 4.5f, 0.35f, 0.335f, 1.03f, 0.78f, 1.5f},
+    {64, 64, 3, 3.6f, 0.29f, 0.21f, 0.58f, 0.525f, 1.4f},
 };
 
 inline float stage_us(const TileCost& c, int dtype, float of_cu) {  // of_cu: workgroups of a CU
@@ -1270,7 +1282,8 @@ inline Cut cut_of(int64_t M, int64_t N, int64_t K, int dtype, bool a_k, bool b_k
       if (want > 1 && (tiles * (want - 1) > 4.f * cus || stages < 2 * want)) break;
       const int per = (stages + want - 1) / want, splits = (stages + per - 1) / per;
       if (splits < want) continue;
-      const float us = c.ends + per * stage_us(c, dtype, tiles * splits / cus) + join_us(splits, M, N);
+      const float more = dtype == kI8 ? c.more8 * std::max(0.f, ceilf(tiles * splits / cus) - 1.f) : 0.f;
+      const float us = c.ends + per * stage_us(c, dtype, tiles * splits / cus) + join_us(splits, M, N) + more;
       if (best.us == 0.f || us < best.us) best = {t, splits, per * kK, us};
     }
   }
