@@ -144,6 +144,68 @@ __global__ __launch_bounds__(256) void ce_gather_kernel(const T* x, int64_t ld, 
   }
 }
 
+// four values of a row from element k on, zeros past its end
+MHC_DEV f32x4 four_of(const float* row, int k, int C) {
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (k + 4 <= C) {
+    __builtin_memcpy(&v, row + k, 16);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (k + j < C) v[j] = row[k + j];
+  }
+  return v;
+}
+
+// Rows of fp32 as rows of fp16 parts (see ce::Halves): [high, low, high] or
+// (LAST_LOW) [high, high, low], each part in `wide` elements, zeros after the
+// last.  The live rows of x (index given), or all of `rows`.  A wave for each
+// row, which it keeps in registers up to 1024 elements and reads again beyond.
+template <bool LAST_LOW>
+__global__ __launch_bounds__(256) void ce_halves_kernel(const float* x, int64_t ld, _Float16* to, float* scales, const int* live, const int* index,
+                                                        int64_t rows, int C, int wide) {
+  constexpr int kHeld = 4, kStep = 4 * kWave;
+  const int k0 = threadIdx.x % kWave * 4;
+  if (live != nullptr) rows = *live;
+  for (int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave; r < rows; r += (int64_t)gridDim.x * 4) {
+    const float* const row = x + (index != nullptr ? index[r] : r) * ld;
+    f32x4 held[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) held[i] = four_of(row, k0 + i * kStep, C);
+    float top = 0.f;
+    const auto look = [&](const f32x4& v) {  // (as bit patterns, of which NaN's are the largest)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = __builtin_bit_cast(float, max(__builtin_bit_cast(uint32_t, top), __builtin_bit_cast(uint32_t, fabsf(v[j]))));
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) look(held[i]);
+    for (int k = k0 + kHeld * kStep; k < C; k += kStep) look(four_of(row, k, C));
+    uint32_t bits = __builtin_bit_cast(uint32_t, top);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) bits = max(bits, (uint32_t)__shfl_xor((int)bits, d));
+    // 2^14 over the largest value's power of two, if both are normal numbers (a row with an infinity: 1, and its logits are NaN)
+    const uint32_t e = bits >> 23, up = e == 255 ? 127 : min(268u - max(e, 15u), 253u);
+    const float by = __builtin_bit_cast(float, up << 23);
+    if (k0 == 0) scales[r] = __builtin_bit_cast(float, (254u - up) << 23);
+    _Float16* const out = to + r * 3 * wide;
+    const auto store = [&](int k, const f32x4& v) {
+      f16x4 high, low;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        high[j] = (_Float16)(v[j] * by);
+        low[j] = (_Float16)(v[j] * by - (float)high[j]);
+      }
+      *reinterpret_cast<f16x4*>(out + k) = high;  // (wide is a multiple of eight)
+      *reinterpret_cast<f16x4*>(out + wide + k) = LAST_LOW ? high : low;
+      *reinterpret_cast<f16x4*>(out + 2 * wide + k) = LAST_LOW ? low : high;
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (k0 + i * kStep < wide) store(k0 + i * kStep, held[i]);
+    for (int k = k0 + kHeld * kStep; k < wide; k += kStep) store(k, four_of(row, k, C));
+  }
+}
+
 // A row's parts to its sums, and its log probability, put together in fp64
 // (log sum = e log 2 + log m with m around 1: the fp32 part stays below 0.35):
 // a wave for each row.  (The weights become those over the largest one here.)
@@ -228,32 +290,79 @@ __global__ __launch_bounds__(256) void ce_scatter_kernel(const float* sums, int 
 
 const ce::Runs& runs_of(int dtype) { return dtype == kF32 ? ce::runs_f32() : dtype == kBF16 ? ce::runs_bf16() : ce::runs_f16(); }
 
+// Whether fp32 logits are formed of fp16 parts: bringing W into them takes the
+// time of some 400 rows' products.
+bool in_halves(const mhc_linear_ce_args& a) { return a.dtype == kF32 && a.T >= 512; }
+
+// What the parts of x's rows and of a piece's rows of W take.
+struct HalvesPlan {
+  int64_t wide;  // elements of a part of a row
+  size_t x, w;   // bytes, with the rows' scales
+};
+
+HalvesPlan plan_halves(const mhc_linear_ce_args& a, int64_t piece) {
+  const int64_t wide = padded(a.C, kF16);
+  const auto bytes = [&](int64_t rows) { return up256((size_t)(rows * 3 * wide) * 2) + up256((size_t)rows * 4); };
+  return {wide, bytes(a.T), bytes(piece)};
+}
+
+// columns of the vocabulary whose parts take at most kPieceBytes
+int64_t halves_piece(const mhc_linear_ce_args& a) {
+  const int64_t most = std::max<int64_t>(256, kPieceBytes / (6 * padded(a.C, kF16)) / 256 * 256);
+  return std::min(a.V, ceil_div(ceil_div(a.V, ceil_div(a.V, most)), 256) * 256);
+}
+
 struct FwdPlan {
   Cut cut;
   int64_t tiles;
-  bool direct;  // the live rows of x are read where they lie
+  int64_t piece;  // columns of the vocabulary at a time
+  bool direct;    // the live rows of x are read where they lie
   size_t x, w, part, at_target, total;  // bytes; terms come last
 };
 
 FwdPlan plan_fwd(const mhc_linear_ce_args& a) {
   constexpr int kBn[] = {256, 256, 128, 128, 64};
   FwdPlan p;
-  p.cut = gemm::cut_of(a.T, a.V, a.C, a.dtype, true, true, 1);
-  p.tiles = ceil_div(a.V, kBn[p.cut.tile]);
   const int e = gemm::elem_bytes(a.dtype);
-  p.direct = gemm::in_words(a.x, a.ldx, a.C, e) && ((a.T - 1) * a.ldx + a.C) * e < ((int64_t)1 << 31);
-  p.x = p.direct ? 0 : up256((size_t)(a.T * padded(a.C, a.dtype)) * e);
-  p.w = gemm::pack_bytes(a.w, a.V, a.ldw, a.C, a.dtype);
+  p.direct = false;
+  if (in_halves(a)) {
+    p.piece = halves_piece(a);
+    const HalvesPlan h = plan_halves(a, p.piece);
+    p.cut = gemm::cut_of(a.T, p.piece, 3 * h.wide, kF16, true, true, 1);
+    p.x = h.x;
+    p.w = h.w;
+  } else {
+    p.piece = a.V;
+    p.cut = gemm::cut_of(a.T, a.V, a.C, a.dtype, true, true, 1);
+    p.direct = gemm::in_words(a.x, a.ldx, a.C, e) && ((a.T - 1) * a.ldx + a.C) * e < ((int64_t)1 << 31);
+    p.x = p.direct ? 0 : up256((size_t)(a.T * padded(a.C, a.dtype)) * e);
+    p.w = gemm::pack_bytes(a.w, a.V, a.ldw, a.C, a.dtype);
+  }
+  p.tiles = ceil_div(a.V, kBn[p.cut.tile]);  // (pieces are whole tiles, but for the last)
   p.part = up256((size_t)(a.T * p.tiles) * sizeof(float2));
   p.at_target = up256((size_t)a.T * sizeof(float));
   p.total = p.x + p.w + p.part + p.at_target + (size_t)a.T * sizeof(double);
   return p;
 }
 
+// the parts of rows to `to`, their scales after them
+int run_halves(bool last_low, const void* x, int64_t ld, char* to, const float** scales, const State* live, int64_t rows, int64_t C, int64_t wide,
+               hipStream_t s) {
+  float* const at = reinterpret_cast<float*>(to + up256((size_t)(rows * 3 * wide) * 2));
+  *scales = at;
+  const dim3 grid((unsigned)std::min<int64_t>(ceil_div(rows, 4), device_cu_count() * 16));
+  const int *const count = live != nullptr ? live->head : nullptr, *const index = live != nullptr ? live->index : nullptr;
+  hipLaunchKernelGGL(last_low ? ce_halves_kernel<true> : ce_halves_kernel<false>, grid, dim3(256), 0, s, static_cast<const float*>(x), ld,
+                     reinterpret_cast<_Float16*>(to), at, count, index, rows, (int)C, (int)wide);
+  MHC_CHECK_LAUNCH("ce_halves_kernel");
+  return MHC_OK;
+}
+
 struct BwdPlan {
   int64_t piece;   // columns of the vocabulary
   bool joint;      // a piece's dx and dW go with the next one's dz
   Cut dz, dx, dw;  // dx.splits: parts of its reduction, each with sums of its own over all pieces
+  HalvesPlan halves;
   size_t x, w, of_dz, sums, part, total;  // bytes; two of of_dz where joint
 };
 
@@ -261,7 +370,13 @@ BwdPlan plan_bwd(const mhc_linear_ce_args& a, bool dx, bool dw) {
   BwdPlan p = {};
   const int64_t e = gemm::elem_bytes(a.dtype), pieces = std::max<int64_t>(1, ceil_div(a.T * a.V * e, kPieceBytes));
   p.piece = std::min(a.V, ceil_div(ceil_div(a.V, pieces), 256) * 256);
-  p.dz = gemm::cut_of(a.T, p.piece, a.C, a.dtype, true, true, 1);
+  if (in_halves(a)) {
+    p.piece = std::min(p.piece, halves_piece(a));
+    p.halves = plan_halves(a, p.piece);
+    p.dz = gemm::cut_of(a.T, p.piece, 3 * p.halves.wide, kF16, true, true, 1);
+  } else {
+    p.dz = gemm::cut_of(a.T, p.piece, a.C, a.dtype, true, true, 1);
+  }
   // (whichever is asked for: a gradient does not depend on that)
   p.dx = gemm::cut_of(a.T, a.C, p.piece, a.dtype, true, false);
   p.dw = gemm::cut_of(p.piece, a.C, a.T, a.dtype, false, false);
@@ -284,7 +399,7 @@ BwdPlan plan_bwd(const mhc_linear_ce_args& a, bool dx, bool dw) {
   p.of_dz = up256((size_t)(a.T * padded(p.piece, a.dtype) * e));
   if (dx) p.sums = up256((size_t)(p.dx.splits * a.T * a.C) * sizeof(float));
   p.part = dw && !p.joint ? gemm::part_bytes(p.dw, p.piece, a.C) : 0;
-  p.total = p.x + p.w + p.of_dz * (p.joint && p.piece < a.V ? 2 : 1) + p.sums + p.part;
+  p.total = p.x + p.w + p.of_dz * (p.joint && p.piece < a.V ? 2 : 1) + p.sums + p.halves.x + p.halves.w + p.part;
   return p;
 }
 
@@ -357,19 +472,32 @@ extern "C" int mhc_linear_ce_fwd(const mhc_linear_ce_args* args, float* loss, fl
   float* at_target = nullptr;
   double* terms = nullptr;
   if (a.T > 0) {
-    char* const x = ws;
-    ws += p.x;
-    Product q = {Operand{a.x, a.ldx, a.C}, {}, a.T, a.V, a.C, {}, 1, 0};
-    if (!p.direct) {
-      if (const int rc = run_gather(a, st, x, s)) return rc;
-      const int64_t wide = padded(a.C, a.dtype);
-      q.a = Operand{x, wide, wide};
+    char *const x = ws, *const w = ws + p.x;
+    part = reinterpret_cast<float2*>(ws + p.x + p.w);
+    at_target = reinterpret_cast<float*>(ws + p.x + p.w + p.part);
+    terms = reinterpret_cast<double*>(ws + p.x + p.w + p.part + p.at_target);
+    ce::SumsOf of = {st.target, part, at_target, p.tiles, 0};
+    if (in_halves(a)) {
+      const int64_t wide = padded(a.C, kF16);
+      ce::Halves halves;
+      if (const int rc = run_halves(false, a.x, a.ldx, x, &halves.x, &st, a.T, a.C, wide, s)) return rc;
+      for (of.v0 = 0; of.v0 < a.V; of.v0 += p.piece) {
+        const int64_t n = std::min(p.piece, a.V - of.v0);
+        if (const int rc = run_halves(true, static_cast<const float*>(a.w) + of.v0 * a.ldw, a.ldw, w, &halves.w, nullptr, n, a.C, wide, s)) return rc;
+        const Product q = {Operand{x, 3 * wide, 3 * wide}, Operand{w, 3 * wide, 3 * wide}, a.T, n, 3 * wide, {}, 1, 0};
+        if (const int rc = ce::run_sums_halves(q, p.cut, st.head, of, halves, s)) return rc;
+      }
+    } else {
+      Product q = {Operand{a.x, a.ldx, a.C}, {}, a.T, a.V, a.C, {}, 1, 0};
+      if (!p.direct) {
+        if (const int rc = run_gather(a, st, x, s)) return rc;
+        const int64_t wide = padded(a.C, a.dtype);
+        q.a = Operand{x, wide, wide};
+      }
+      ws = w;
+      if (const int rc = gemm::operand(q.b, a.w, a.V, a.ldw, a.C, a.dtype, ws, s)) return rc;
+      if (const int rc = runs_of(a.dtype).sums(q, ce::RowsOf{p.direct ? st.index : nullptr, a.T}, p.cut, st.head, of, {}, s)) return rc;
     }
-    if (const int rc = gemm::operand(q.b, a.w, a.V, a.ldw, a.C, a.dtype, ws, s)) return rc;
-    part = reinterpret_cast<float2*>(ws);
-    at_target = reinterpret_cast<float*>(ws + p.part);
-    terms = reinterpret_cast<double*>(ws + p.part + p.at_target);
-    if (const int rc = runs_of(a.dtype).sums(q, ce::RowsOf{p.direct ? st.index : nullptr, a.T}, p.cut, st.head, st.target, part, at_target, s)) return rc;
     hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)std::min(ceil_div(a.T, 4), kMaxGrid)), dim3(256), 0, s, st, (const float2*)part,
                        (const float*)at_target, p.tiles, logp, terms);
     MHC_CHECK_LAUNCH("ce_rows_kernel");
@@ -408,7 +536,12 @@ extern "C" int mhc_linear_ce_bwd(const mhc_linear_ce_args* args, const void* sta
   if (const int rc = gemm::operand(w, a.w, a.V, a.ldw, a.C, a.dtype, ws, s)) return rc;
   char* const dz[2] = {ws, ws + (p.joint && p.piece < a.V ? p.of_dz : 0)};
   float* const sums = reinterpret_cast<float*>(dz[1] + p.of_dz);
-  float* const part = reinterpret_cast<float*>(dz[1] + p.of_dz + p.sums);
+  char* const of_halves = dz[1] + p.of_dz + p.sums;
+  float* const part = reinterpret_cast<float*>(of_halves + p.halves.x + p.halves.w);
+  ce::Halves halves = {};
+  if (in_halves(a)) {
+    if (const int rc = run_halves(false, a.x, a.ldx, of_halves, &halves.x, &st, a.T, a.C, p.halves.wide, s)) return rc;
+  }
   const float* const unit = reinterpret_cast<const float*>(st.head) + 1;
   const float lift = a.dtype == kF16 ? ce::kDzUnit<_Float16> : 1.f;
   const ce::Runs& run = runs_of(a.dtype);
@@ -432,7 +565,14 @@ extern "C" int mhc_linear_ce_bwd(const mhc_linear_ce_args* args, const void* sta
   };
   int b = 0;
   for (int64_t v0 = 0; v0 < a.V; v0 += p.piece) {
-    if (v0 == 0 || !p.joint) {
+    if (in_halves(a)) {
+      const int64_t wide = 3 * p.halves.wide;
+      char* const w_halves = of_halves + p.halves.x;
+      if (const int rc = run_halves(true, rows_of(v0).p, w.ld, w_halves, &halves.w, nullptr, columns(v0), a.C, p.halves.wide, s)) return rc;
+      Product q = of_dz(v0, b);
+      q.a = Operand{of_halves, wide, wide}, q.b = Operand{w_halves, wide, wide}, q.K = wide;
+      if (const int rc = ce::run_dz_halves(q, p.dz, st.head, pitch(v0), gradient(v0), halves, s)) return rc;
+    } else if (v0 == 0 || !p.joint) {
       if (const int rc = run.dz(of_dz(v0, b), p.dz, st.head, pitch(v0), gradient(v0), s)) return rc;
     }
     if (p.joint) {

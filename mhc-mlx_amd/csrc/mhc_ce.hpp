@@ -41,6 +41,34 @@ struct State {
 template <typename T> inline constexpr float kDzUnit = 1.f;
 template <> inline constexpr float kDzUnit<_Float16> = 0x1p14f;
 
+// fp32 rows as pairs of fp16 parts: each row times a power of two that brings its
+// largest value to 2^14, each value the sum of the nearest fp16 number and of
+// the one nearest to what is left, which is the value to 2^-24 of itself (and to
+// 2^-40 of the row's largest).  Of the products of two values three parts are
+// formed (the fourth is below 2^-24): rows of [high, low, high] against rows of
+// [high, high, low], 3 C long, half of what linear_act's fp32 tiles do.
+struct Halves {
+  const float *x, *w;  // of each row: what its parts are to be multiplied by
+
+  template <int BM, int BN, int WM, int WN, int JM, int JN>
+  MHC_DEV void scale(const Product& p, const gemm::Place<BM, BN, WM, WN>& at, f32x4 (&acc)[JN][JM]) const {
+    const int64_t m0 = at.m0 + at.wm + at.lane % 16, n0 = at.n0 + at.wn + at.lane / 16 * 4;
+    float row[JM];
+#pragma unroll
+    for (int j = 0; j < JM; ++j) row[j] = x[min(m0 + j * 16, p.M - 1)];
+#pragma unroll
+    for (int i = 0; i < JN; ++i) {
+      f32x4 column;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) column[k] = w[min(n0 + i * 16 + k, p.N - 1)];
+#pragma unroll
+      for (int j = 0; j < JM; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[i][j][k] = acc[i][j][k] * row[j] * column[k];
+    }
+  }
+};
+
 // Logits to dz = coef (softmax - [v = target]), zeros past the last column.
 struct Gradient {
   const int* target;
@@ -76,6 +104,19 @@ struct GradientOf : Gradient {
   template <typename P, int JM, int JN>
   MHC_DEV void operator()(const Product& p, const P& at, int, char*, const Own&, f32x4 (&acc)[JN][JM]) const {
     this->template apply<FAST>(p, at, acc);
+  }
+};
+
+// the same of logits that are products of halves
+struct GradientOfHalves : Gradient {
+  Halves halves;
+  using Own = gemm::AsTheyAre::Own;
+  template <typename P>
+  MHC_DEV Own ahead(const Product&, const P&) const { return {}; }
+  template <typename P, int JM, int JN>
+  MHC_DEV void operator()(const Product& p, const P& at, int, char*, const Own&, f32x4 (&acc)[JN][JM]) const {
+    halves.scale(p, at, acc);
+    this->template apply<false>(p, at, acc);
   }
 };
 
@@ -124,8 +165,8 @@ MHC_DEV void move_to_part(Epilogue& e, int64_t at) {
   if (e.residual != nullptr) e.residual = static_cast<const float*>(e.residual) + at;
 }
 
-// (SUMS: the parts of a reduction add to sums of their own)
-template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS, bool SUMS, typename Then>
+// (SUMS: the parts of a reduction add to sums of their own; O: of the outputs)
+template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS, bool SUMS, typename O, typename Then>
 __global__ __launch_bounds__(64 * WM * WN) void live_tile_kernel(Product p, const int* live, int64_t width, const Then then) {
   __shared__ __attribute__((aligned(1024))) char smem[gemm::TileBytes<T, BM, BN, WM, WN, NS>::kAll];
   const int64_t part = p.M * p.N;
@@ -135,7 +176,7 @@ __global__ __launch_bounds__(64 * WM * WN) void live_tile_kernel(Product p, cons
     move_to_part(p.e, blockIdx.y * part);
     p.splits = 1;
   }
-  gemm::run_tile<T, AK, BK, BM, BN, WM, WN, NS, T>(p, smem, blockIdx.x, (int)blockIdx.y, part, width, then);
+  gemm::run_tile<T, AK, BK, BM, BN, WM, WN, NS, O>(p, smem, blockIdx.x, (int)blockIdx.y, part, width, then);
 }
 
 // dx and dW of one piece of the vocabulary and dz of the next, none of which
@@ -218,18 +259,27 @@ struct RowsOf {
 };
 
 // A tile of logits, of which only each row's largest and the sum of
-// exp(logit - largest) are kept, and the target's: to part[row][column of
-// tiles] and at_target[row].
-template <typename T, int BM, int BN, int WM, int WN, int NS>
-__global__ __launch_bounds__(64 * WM * WN) void sums_tile_kernel(Product p, const RowsOf rows, const int* live, const int* target, float2* part, float* at_target) {
+// exp(logit - largest) are kept, and the target's: to part[row][tile] and
+// at_target[row].  The tile is one of the vocabulary's from v0 on, of which a
+// row has `tiles`.
+struct SumsOf {
+  const int* target;
+  float2* part;
+  float* at_target;
+  int64_t tiles, v0;
+};
+
+template <typename T, bool HALVES, int BM, int BN, int WM, int WN, int NS>
+__global__ __launch_bounds__(64 * WM * WN) void sums_tile_kernel(Product p, const RowsOf rows, const int* live, const SumsOf of, const Halves halves) {
   __shared__ __attribute__((aligned(1024))) char smem[NS * (BM + BN) * 128];
   if (!limit<true, BM, BN>(p, live, blockIdx.x)) return;
   constexpr int JM = BM / WM / 16, JN = BN / WN / 16, kThreads = 64 * WM * WN;
-  constexpr bool kFast = sizeof(T) == 2;
+  constexpr bool kFast = sizeof(T) == 2 && !HALVES;
   const gemm::Place<BM, BN, WM, WN> at(p, blockIdx.x, 0);
   f32x4 acc[JN][JM] = {};
   if constexpr (gemm::kSplit<T, BN>) gemm::sum_tile_split<true, true, BM, BN, WM, WN, NS>(p, at, smem, acc, rows);
   else gemm::sum_tile<T, true, true, BM, BN, WM, WN, NS>(p, at, smem, acc, rows);
+  if constexpr (HALVES) halves.scale(p, at, acc);
   const int64_t m0 = at.m0 + at.wm + at.lane % 16, n0 = at.n0 + at.wn + at.lane / 16 * 4;
   if (at.n0 + BN > p.N) {
 #pragma unroll
@@ -261,15 +311,14 @@ __global__ __launch_bounds__(64 * WM * WN) void sums_tile_kernel(Product p, cons
     sum = xor_allreduce<32>(sum, SumOp{});
     if (at.lane < 16) of_waves[at.wave % WN * BM + at.wm + j * 16 + at.lane] = float2{top, sum};
     const int64_t m = m0 + j * 16;
-    const int mine = m < p.M ? target[m] - (int)n0 : -1;
+    const int64_t mine = m < p.M ? of.target[m] - of.v0 - n0 : -1;
 #pragma unroll
     for (int i = 0; i < JN; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (mine == i * 16 + k) at_target[m] = acc[i][j][k];
+        if (mine == i * 16 + k) of.at_target[m] = acc[i][j][k];
   }
   __syncthreads();
-  const int64_t tiles = ceil_div(p.N, BN);
   for (int r = threadIdx.x; r < BM; r += kThreads) {
     if (at.m0 + r >= p.M) break;
     float2 all = of_waves[r];
@@ -280,42 +329,42 @@ __global__ __launch_bounds__(64 * WM * WN) void sums_tile_kernel(Product p, cons
       all.y = all.y * gemm::exp_of<kFast>(all.x - base) + one.y * gemm::exp_of<kFast>(one.x - base);
       all.x = top;
     }
-    part[(at.m0 + r) * tiles + at.n0 / BN] = all;
+    of.part[(at.m0 + r) * of.tiles + (of.v0 + at.n0) / BN] = all;
   }
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int NS>
-int launch_sums(const Product& p, const RowsOf& rows, const int* live, const int* target, float2* part, float* at_target, hipStream_t s) {
-  hipLaunchKernelGGL((sums_tile_kernel<T, BM, BN, WM, WN, NS>), dim3((unsigned)(ceil_div(p.M, BM) * ceil_div(p.N, BN))), dim3(64 * WM * WN), 0, s,
-                     p, rows, live, target, part, at_target);
+template <typename T, bool HALVES, int BM, int BN, int WM, int WN, int NS>
+int launch_sums(const Product& p, const RowsOf& rows, const int* live, const SumsOf& of, const Halves& halves, hipStream_t s) {
+  hipLaunchKernelGGL((sums_tile_kernel<T, HALVES, BM, BN, WM, WN, NS>), dim3((unsigned)(ceil_div(p.M, BM) * ceil_div(p.N, BN))), dim3(64 * WM * WN),
+                     0, s, p, rows, live, of, halves);
   MHC_CHECK_LAUNCH("sums_tile_kernel");
   return MHC_OK;
 }
 
-template <typename T>
-int run_sums(Product p, const RowsOf& rows, const Cut& c, const int* live, const int* target, float2* part, float* at_target, hipStream_t s) {
+template <typename T, bool HALVES = false>
+int run_sums(Product p, const RowsOf& rows, const Cut& c, const int* live, const SumsOf& of, const Halves& halves, hipStream_t s) {
   using gemm::kRowWaves;
   p.splits = 1;
   p.kper = c.kper;
   switch (c.tile) {
-    case 0: return launch_sums<T, 256, 256, 2, 4, 2>(p, rows, live, target, part, at_target, s);
-    case 1: return launch_sums<T, 128, 256, 2, 4, 2>(p, rows, live, target, part, at_target, s);
-    case 2: return launch_sums<T, 128, 128, kRowWaves<T>, 2, 2>(p, rows, live, target, part, at_target, s);
-    case 3: return launch_sums<T, 64, 128, kRowWaves<T>, 2, 3>(p, rows, live, target, part, at_target, s);
-    default: return launch_sums<T, 64, 64, 4, 1, 3>(p, rows, live, target, part, at_target, s);
+    case 0: return launch_sums<T, HALVES, 256, 256, 2, 4, 2>(p, rows, live, of, halves, s);
+    case 1: return launch_sums<T, HALVES, 128, 256, 2, 4, 2>(p, rows, live, of, halves, s);
+    case 2: return launch_sums<T, HALVES, 128, 128, kRowWaves<T>, 2, 2>(p, rows, live, of, halves, s);
+    case 3: return launch_sums<T, HALVES, 64, 128, kRowWaves<T>, 2, 3>(p, rows, live, of, halves, s);
+    default: return launch_sums<T, HALVES, 64, 64, 4, 1, 3>(p, rows, live, of, halves, s);
   }
 }
 
-template <typename T, bool AK, bool BK, bool SUMS, int BM, int BN, int WM, int WN, int NS, typename Then>
+template <typename T, bool AK, bool BK, bool SUMS, typename O, int BM, int BN, int WM, int WN, int NS, typename Then>
 int launch_live(const Product& p, const int* live, int64_t width, const Then& then, hipStream_t s) {
   const dim3 grid((unsigned)(ceil_div(p.M, BM) * ceil_div(p.N, BN)), (unsigned)p.splits), block(64 * WM * WN);
-  hipLaunchKernelGGL((live_tile_kernel<T, AK, BK, BM, BN, WM, WN, NS, SUMS, Then>), grid, block, 0, s, p, live, width, then);
+  hipLaunchKernelGGL((live_tile_kernel<T, AK, BK, BM, BN, WM, WN, NS, SUMS, O, Then>), grid, block, 0, s, p, live, width, then);
   MHC_CHECK_LAUNCH("live_tile_kernel");
   return MHC_OK;
 }
 
 // width: of the outputs' rows; part: the sums of a reduction's parts, if it is split (and not SUMS)
-template <typename T, bool AK, bool BK, bool SUMS, typename Then>
+template <typename T, bool AK, bool BK, bool SUMS, typename O = T, typename Then>
 int run_live(Product p, const Cut& c, const int* live, int64_t width, const Then& then, float* part, hipStream_t s) {
   using gemm::kRowWaves;
   const Epilogue e = p.e;
@@ -324,11 +373,11 @@ int run_live(Product p, const Cut& c, const int* live, int64_t width, const Then
   if (c.splits > 1 && !SUMS) p.e = Epilogue{nullptr, nullptr, part, nullptr, MHC_ACT_NONE, 1};
   int rc;
   switch (c.tile) {
-    case 0: rc = launch_live<T, AK, BK, SUMS, 256, 256, 2, 4, 2>(p, live, width, then, s); break;
-    case 1: rc = launch_live<T, AK, BK, SUMS, 128, 256, 2, 4, 2>(p, live, width, then, s); break;
-    case 2: rc = launch_live<T, AK, BK, SUMS, 128, 128, kRowWaves<T>, 2, 2>(p, live, width, then, s); break;
-    case 3: rc = launch_live<T, AK, BK, SUMS, 64, 128, kRowWaves<T>, 2, 3>(p, live, width, then, s); break;
-    default: rc = launch_live<T, AK, BK, SUMS, 64, 64, 4, 1, 3>(p, live, width, then, s); break;
+    case 0: rc = launch_live<T, AK, BK, SUMS, O, 256, 256, 2, 4, 2>(p, live, width, then, s); break;
+    case 1: rc = launch_live<T, AK, BK, SUMS, O, 128, 256, 2, 4, 2>(p, live, width, then, s); break;
+    case 2: rc = launch_live<T, AK, BK, SUMS, O, 128, 128, kRowWaves<T>, 2, 2>(p, live, width, then, s); break;
+    case 3: rc = launch_live<T, AK, BK, SUMS, O, 64, 128, kRowWaves<T>, 2, 3>(p, live, width, then, s); break;
+    default: rc = launch_live<T, AK, BK, SUMS, O, 64, 64, 4, 1, 3>(p, live, width, then, s); break;
   }
   if (rc != MHC_OK || c.splits == 1 || SUMS) return rc;
   return gemm::launch_join<T>(e, part, c.splits, p.M, p.N, s);
@@ -336,7 +385,7 @@ int run_live(Product p, const Cut& c, const int* live, int64_t width, const Then
 
 // The launches of one type, each compiled in a file of its own.
 struct Runs {
-  int (*sums)(Product p, const RowsOf& rows, const Cut& c, const int* live, const int* target, float2* part, float* at_target, hipStream_t s);
+  int (*sums)(Product p, const RowsOf& rows, const Cut& c, const int* live, const SumsOf& of, const Halves& halves, hipStream_t s);
   int (*dz)(const Product& p, const Cut& c, const int* live, int64_t width, const Gradient& g, hipStream_t s);
   int (*dx)(const Product& p, const Cut& c, const int* live, hipStream_t s);
   int (*dw)(const Product& p, const Cut& c, const int* live, const ScaledBy& by, float* part, hipStream_t s);
@@ -345,6 +394,10 @@ struct Runs {
 const Runs& runs_f32();
 const Runs& runs_bf16();
 const Runs& runs_f16();
+
+// of rows of fp16 parts for fp32 logits
+int run_sums_halves(const Product& p, const Cut& c, const int* live, const SumsOf& of, const Halves& halves, hipStream_t s);
+int run_dz_halves(const Product& p, const Cut& c, const int* live, int64_t width, const Gradient& g, const Halves& halves, hipStream_t s);
 
 template <typename T>
 int run_dz(const Product& p, const Cut& c, const int* live, int64_t width, const Gradient& g, hipStream_t s) {
@@ -362,10 +415,10 @@ int run_dw(const Product& p, const Cut& c, const int* live, const ScaledBy& by, 
 template <typename T>
 const Runs& runs_of() {
   if constexpr (sizeof(T) == 2) {
-    static const Runs r = {run_sums<T>, run_dz<T>, run_dx<T>, run_dw<T>, run_joint<T>};
+    static const Runs r = {run_sums<T, false>, run_dz<T>, run_dx<T>, run_dw<T>, run_joint<T>};
     return r;
   } else {
-    static const Runs r = {run_sums<T>, run_dz<T>, run_dx<T>, run_dw<T>, nullptr};
+    static const Runs r = {run_sums<T, false>, run_dz<T>, run_dx<T>, run_dw<T>, nullptr};
     return r;
   }
 }
