@@ -160,26 +160,27 @@ MHC_DEV f32x4 four_of(const float* row, int k, int C) {
 // Rows of fp32 as rows of fp16 parts (see ce::Halves): [high, low, high] or
 // (LAST_LOW) [high, high, low], each part in `wide` elements, zeros after the
 // last.  The live rows of x (index given), or all of `rows`.  A wave for each
-// row, which it keeps in registers up to 1024 elements and reads again beyond.
-template <bool LAST_LOW>
+// row, of which it keeps HELD times 256 elements in registers and reads those
+// beyond again (32768 x 1024: 335 MB in 51 us, 6.5 TB/s).
+template <bool LAST_LOW, int HELD>
 __global__ __launch_bounds__(256) void ce_halves_kernel(const float* x, int64_t ld, _Float16* to, float* scales, const int* live, const int* index,
                                                         int64_t rows, int C, int wide) {
-  constexpr int kHeld = 4, kStep = 4 * kWave;
+  constexpr int kStep = 4 * kWave;
   const int k0 = threadIdx.x % kWave * 4;
   if (live != nullptr) rows = *live;
   for (int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave; r < rows; r += (int64_t)gridDim.x * 4) {
     const float* const row = x + (index != nullptr ? index[r] : r) * ld;
-    f32x4 held[kHeld];
+    f32x4 held[HELD];
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) held[i] = four_of(row, k0 + i * kStep, C);
+    for (int i = 0; i < HELD; ++i) held[i] = four_of(row, k0 + i * kStep, C);
     float top = 0.f;
     const auto look = [&](const f32x4& v) {  // (as bit patterns, of which NaN's are the largest)
 #pragma unroll
       for (int j = 0; j < 4; ++j) top = __builtin_bit_cast(float, max(__builtin_bit_cast(uint32_t, top), __builtin_bit_cast(uint32_t, fabsf(v[j]))));
     };
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) look(held[i]);
-    for (int k = k0 + kHeld * kStep; k < C; k += kStep) look(four_of(row, k, C));
+    for (int i = 0; i < HELD; ++i) look(held[i]);
+    for (int k = k0 + HELD * kStep; k < C; k += kStep) look(four_of(row, k, C));
     uint32_t bits = __builtin_bit_cast(uint32_t, top);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) bits = max(bits, (uint32_t)__shfl_xor((int)bits, d));
@@ -200,9 +201,9 @@ __global__ __launch_bounds__(256) void ce_halves_kernel(const float* x, int64_t 
       *reinterpret_cast<f16x4*>(out + 2 * wide + k) = LAST_LOW ? low : high;
     };
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i)
+    for (int i = 0; i < HELD; ++i)
       if (k0 + i * kStep < wide) store(k0 + i * kStep, held[i]);
-    for (int k = k0 + kHeld * kStep; k < wide; k += kStep) store(k, four_of(row, k, C));
+    for (int k = k0 + HELD * kStep; k < wide; k += kStep) store(k, four_of(row, k, C));
   }
 }
 
@@ -290,9 +291,23 @@ __global__ __launch_bounds__(256) void ce_scatter_kernel(const float* sums, int 
 
 const ce::Runs& runs_of(int dtype) { return dtype == kF32 ? ce::runs_f32() : dtype == kBF16 ? ce::runs_bf16() : ce::runs_f16(); }
 
-// Whether fp32 logits are formed of fp16 parts: bringing W into them takes the
-// time of some 400 rows' products.
-bool in_halves(const mhc_linear_ce_args& a) { return a.dtype == kF32 && a.T >= 512; }
+// columns of the vocabulary whose parts take at most kPieceBytes
+int64_t halves_piece(const mhc_linear_ce_args& a) {
+  const int64_t most = std::max<int64_t>(256, kPieceBytes / (6 * padded(a.C, kF16)) / 256 * 256);
+  return std::min(a.V, ceil_div(ceil_div(a.V, ceil_div(a.V, most)), 256) * 256);
+}
+
+// Whether fp32 logits are formed of fp16 parts: where their products and the
+// way of W into them (ten bytes for each of its elements at 4.5 TB/s) are
+// estimated shorter than fp32 products (512 x 32768 x 1024 165 and 176 us, 4096 x
+// 8000 x 2048 387 and 696; but 256 x 32768 x 1024 149 and 111).
+bool in_halves(const mhc_linear_ce_args& a) {
+  if (a.dtype != kF32) return false;
+  const int64_t piece = halves_piece(a), wide = padded(a.C, kF16);
+  const float pieces = (float)ceil_div(a.V, piece);
+  const float halves = 4.f + pieces * (4.f + gemm::cut_of(a.T, piece, 3 * wide, kF16, true, true, 1).us) + (float)(a.V * wide) * 10e-6f / 4.5f;
+  return halves < gemm::cut_of(a.T, a.V, a.C, kF32, true, true, 1).us;
+}
 
 // What the parts of x's rows and of a piece's rows of W take.
 struct HalvesPlan {
@@ -304,12 +319,6 @@ HalvesPlan plan_halves(const mhc_linear_ce_args& a, int64_t piece) {
   const int64_t wide = padded(a.C, kF16);
   const auto bytes = [&](int64_t rows) { return up256((size_t)(rows * 3 * wide) * 2) + up256((size_t)rows * 4); };
   return {wide, bytes(a.T), bytes(piece)};
-}
-
-// columns of the vocabulary whose parts take at most kPieceBytes
-int64_t halves_piece(const mhc_linear_ce_args& a) {
-  const int64_t most = std::max<int64_t>(256, kPieceBytes / (6 * padded(a.C, kF16)) / 256 * 256);
-  return std::min(a.V, ceil_div(ceil_div(a.V, ceil_div(a.V, most)), 256) * 256);
 }
 
 struct FwdPlan {
@@ -352,7 +361,9 @@ int run_halves(bool last_low, const void* x, int64_t ld, char* to, const float**
   *scales = at;
   const dim3 grid((unsigned)std::min<int64_t>(ceil_div(rows, 4), device_cu_count() * 16));
   const int *const count = live != nullptr ? live->head : nullptr, *const index = live != nullptr ? live->index : nullptr;
-  hipLaunchKernelGGL(last_low ? ce_halves_kernel<true> : ce_halves_kernel<false>, grid, dim3(256), 0, s, static_cast<const float*>(x), ld,
+  const auto kernel = last_low ? (C <= 1024 ? ce_halves_kernel<true, 4> : ce_halves_kernel<true, 16>)
+                               : (C <= 1024 ? ce_halves_kernel<false, 4> : ce_halves_kernel<false, 16>);
+  hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, static_cast<const float*>(x), ld,
                      reinterpret_cast<_Float16*>(to), at, count, index, rows, (int)C, (int)wide);
   MHC_CHECK_LAUNCH("ce_halves_kernel");
   return MHC_OK;

@@ -9,10 +9,12 @@ hold, NaN among them: they add nothing to the loss, their log probability is giv
 products are formed without their rows.  A target outside [0, V) of a token that counts makes the loss, that token's
 gradient and the weight's NaN (it cannot be refused without waiting for the GPU).
 
-The logits are formed in pieces, in fp32 of exact products (fp32 operands: as linear_act has them, but logits past 2^95 are
-NaN), and again for the gradients, where softmax - onehot, times the token's weight over the largest one, is rounded once to x's dtype
-as an operand of two more products.  A call takes some 256 MB of workspace beside the sums of x's gradient, whatever the
-vocabulary.
+The logits are formed in pieces, in fp32 of exact products, and again for the gradients, where softmax - onehot, times the
+token's weight over the largest one, is rounded once to x's dtype as an operand of two more products.  Of float32 operands
+the products are those of linear_act, but logits past 2^95 are NaN; of many tokens they are formed of fp16 parts, which hold
+a value to 2^-24 of itself and to 2^-40 of its row's largest.  Beside copies of operands whose rows are no whole four-byte
+words, a call takes workspace in proportion to the tokens (their rows of x, the sums of its gradient, twelve bytes for each
+64 to 256 columns) and up to some 0.5 GB for pieces of the vocabulary, whatever its size.
 
 ``linear_cross_entropy`` is differentiable in x and weight (once); ``linear_cross_entropy_and_grad`` returns the gradients with
 the loss, for a caller without autograd.

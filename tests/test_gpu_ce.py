@@ -118,6 +118,22 @@ def test_logits_far_apart(dt):
     check(torch.zeros_like(x), w, y, what="alike")
 
 
+@pytest.mark.parametrize("T,V,C", [(40, 300, 64), (1024, 4096, 256), (1500, 4096, 1100)])
+def test_fp32_rows_of_many_magnitudes(T, V, C):
+    """Few tokens and many (whose logits are products of fp16 parts): rows from 2^-60 to 2^8 times the usual, one of zeros, one subnormal."""
+    x, w, y, g = inputs(15, T, V, C, torch.float32)
+    x = x * 2.0 ** torch.randint(-60, 9, (T, 1), generator=g, device="cuda").float()
+    w = w * 2.0 ** torch.randint(-40, 3, (V, 1), generator=g, device="cuda").float()
+    x = x * 2.0 ** torch.randint(-10, 1, (1, C), generator=g, device="cuda").float()  # (and values of a row)
+    x[3], w[7] = 0.0, 0.0
+    x[4], w[8] = x[4] * 2.0 ** -100, w[8] * 2.0 ** -90
+    check(x, w, y, what="magnitudes")
+    x[5, 1] = float("inf")
+    loss, logp, dx, _ = linear_cross_entropy_and_grad(x, w, y)
+    others = torch.arange(T, device="cuda") != 5
+    assert bool(loss.isnan()) and bool(logp[5].isnan()) and bool(logp[others].isfinite().all()) and bool(dx[others].isfinite().all())
+
+
 def test_strides_and_shapes():
     x, w, y, g = inputs(8, 60, 90, 64, torch.bfloat16)
     want = linear_cross_entropy_and_grad(x, w, y)
