@@ -304,6 +304,7 @@ int64_t halves_piece(const mhc_linear_ce_args& a) {
 bool in_halves(const mhc_linear_ce_args& a) {
   if (a.dtype != kF32) return false;
   const int64_t piece = halves_piece(a), wide = padded(a.C, kF16);
+  if (6 * wide > gemm::kMaxRowBytes) return false;
   const float pieces = (float)ceil_div(a.V, piece);
   const float halves = 4.f + pieces * (4.f + gemm::cut_of(a.T, piece, 3 * wide, kF16, true, true, 1).us) + (float)(a.V * wide) * 10e-6f / 4.5f;
   return halves < gemm::cut_of(a.T, a.V, a.C, kF32, true, true, 1).us;
@@ -443,6 +444,9 @@ int check_args(const mhc_linear_ce_args* a) {
                 (long long)a->C);
   MHC_CHECK_ARG(a->T < ((int64_t)1 << 28) && a->V < ((int64_t)1 << 22) && a->C < ((int64_t)1 << 22),
                 "T must be below 2^28, V and C below 2^22 (got %lld, %lld, %lld)", (long long)a->T, (long long)a->V, (long long)a->C);
+  // (a launch has fewer than 2^32 threads: tiles of 256 x 256 with 512 each, or of 64 x 64 with 256 for small T or V)
+  MHC_CHECK_ARG((a->T / 256 + 1) * (std::max(a->V, a->C) / 256 + 1) < ((int64_t)1 << 22), "T times V is too large (got %lld, %lld)",
+                (long long)a->T, (long long)a->V);
   MHC_CHECK_ARG(a->dtype == kF32 || a->dtype == kBF16 || a->dtype == kF16, "unsupported dtype %d", a->dtype);
   MHC_CHECK_ARG(a->denominator >= 0, "denominator must be >= 0");
   if (a->T == 0) return MHC_OK;
@@ -509,7 +513,7 @@ extern "C" int mhc_linear_ce_fwd(const mhc_linear_ce_args* args, float* loss, fl
       if (const int rc = gemm::operand(q.b, a.w, a.V, a.ldw, a.C, a.dtype, ws, s)) return rc;
       if (const int rc = runs_of(a.dtype).sums(q, ce::RowsOf{p.direct ? st.index : nullptr, a.T}, p.cut, st.head, of, {}, s)) return rc;
     }
-    hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)std::min(ceil_div(a.T, 4), kMaxGrid)), dim3(256), 0, s, st, (const float2*)part,
+    hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(a.T, 4), 1 << 20)), dim3(256), 0, s, st, (const float2*)part,
                        (const float*)at_target, p.tiles, logp, terms);
     MHC_CHECK_LAUNCH("ce_rows_kernel");
   }

@@ -188,6 +188,8 @@ extern "C" int mhc_linear_int8(const int8_t* x, int64_t ldx, const float* x_scal
   clear_error();
   MHC_CHECK_ARG(M >= 0 && N >= 1 && K >= 1, "M must be >= 0, N and K >= 1 (got %lld, %lld, %lld)", (long long)M, (long long)N, (long long)K);
   MHC_CHECK_ARG(M < ((int64_t)1 << 28) && N < ((int64_t)1 << 22), "M must be below 2^28, N below 2^22 (got %lld, %lld)", (long long)M, (long long)N);
+  // (a launch has fewer than 2^32 threads: tiles of 256 x 256 with 512 each, or of 64 x 64 with 256 for small M or N)
+  MHC_CHECK_ARG((M / 256 + 1) * (N / 256 + 1) < ((int64_t)1 << 22), "M times N is too large (got %lld, %lld)", (long long)M, (long long)N);
   MHC_CHECK_ARG(K < kMaxK, "K must be below 2^17, so that sums stay in 32 bits (got %lld)", (long long)K);
   MHC_CHECK_ARG(out_dtype == kF32 || out_dtype == kBF16 || out_dtype == kF16, "unsupported out_dtype %d", out_dtype);
   MHC_CHECK_ARG(act >= MHC_ACT_NONE && act <= MHC_ACT_SILU, "unknown activation %d", act);

@@ -204,7 +204,7 @@ __global__ __launch_bounds__((Held<T, THREADS, NV>::kBlock)) void norm_held_kern
   constexpr int V = H::V;
   __shared__ float lds[2][16];
   const H at(a.C);
-  const int64_t t = (int64_t)blockIdx.x * H::kRows + (H::kRows > 1 ? threadIdx.x / THREADS : 0);
+  const int64_t t = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * H::kRows + (H::kRows > 1 ? threadIdx.x / THREADS : 0);
   if (t >= a.T) return;  // (a wave with its row)
   float z[NV][V] = {}, w[NV][V] = {}, z1, w1;
   at.load(static_cast<const T*>(a.x) + t * a.ldx, z, z1);
@@ -655,7 +655,8 @@ int run_norm(const NormArgs& a, int w_f32, hipStream_t s) {
         hold, [&](auto of) {
           using O = decltype(of);
           using H = Held<T, O::kThreads, O::kVecs>;
-          hipLaunchKernelGGL((norm_held_kernel<T, MODE, O::kThreads, O::kVecs>), dim3((unsigned)ceil_div(a.T, H::kRows)), dim3(H::kBlock), 0, s, a, w_f32);
+          const int64_t groups = ceil_div(a.T, H::kRows);  // (in two dimensions: a launch has fewer than 2^32 threads in one)
+          hipLaunchKernelGGL((norm_held_kernel<T, MODE, O::kThreads, O::kVecs>), dim3(grid_of(groups), (unsigned)ceil_div(groups, kMaxRows)), dim3(H::kBlock), 0, s, a, w_f32);
           MHC_CHECK_LAUNCH("norm_held_kernel");
           return (int)MHC_OK;
         });

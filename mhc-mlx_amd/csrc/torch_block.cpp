@@ -131,7 +131,7 @@ std::tuple<at::Tensor, at::Tensor> add_rms_norm(const at::Tensor& x, const OptTe
   return {out[0], out.size() > 1 ? out[1] : x};
 }
 
-// (codes, scales, h)
+// (codes, scales, h or undefined without a residual)
 std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_int8(const at::Tensor& x, const OptTensor& r, const OptTensor& w, double eps) {
   const at::AutoGradMode plain_mode(false);
   const NormInputs n = norm_inputs(x, get(r), get(w));
@@ -142,7 +142,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_int8(const at::Tenso
   check(mhc_add_rms_norm_int8(ptr(n.x), stride_of(n.x), ptr(n.r), stride_of(n.r), ptr(n.w), n.w_code, ptr(h), codes.data_ptr<int8_t>(),
                               scales.data_ptr<float>(), n.T, n.C, n.code, (float)eps, stream_of(x)),
         "mhc_add_rms_norm_int8");
-  return {codes, scales, h.defined() ? h : x.detach()};
+  return {codes, scales, h};
 }
 
 // ---------------------------------------------------------------------------

@@ -16,6 +16,8 @@ a value to 2^-24 of itself and to 2^-40 of its row's largest.  Beside copies of 
 words, a call takes workspace in proportion to the tokens (their rows of x, the sums of its gradient, twelve bytes for each
 64 to 256 columns) and up to some 0.5 GB for pieces of the vocabulary, whatever its size.
 
+x and weight are taken as they are, under torch.autocast too.
+
 ``linear_cross_entropy`` is differentiable in x and weight (once); ``linear_cross_entropy_and_grad`` returns the gradients with
 the loss, for a caller without autograd.
 """
@@ -25,6 +27,7 @@ from __future__ import annotations
 import torch
 
 from . import ops
+from .int8 import call
 from .profiling import timed
 
 __all__ = ["linear_cross_entropy", "linear_cross_entropy_and_grad", "linear_cross_entropy_reference"]
@@ -80,8 +83,7 @@ def linear_cross_entropy_and_grad(x: torch.Tensor, weight: torch.Tensor, targets
     ``grad_scale`` is the loss scale of float16 training (the loss itself is not scaled).
     """
     numbers = _check(denominator, ignore_index)
-    with timed("linear_cross_entropy_and_grad"):
-        return ops._binding().linear_ce_and_grad(x, weight, targets, mask, *numbers, float(grad_scale))
+    return call("linear_ce_and_grad", x, weight, targets, mask, *numbers, float(grad_scale))
 
 
 def linear_cross_entropy_reference(x, weight, targets, mask=None, denominator=None, ignore_index: int = -100):

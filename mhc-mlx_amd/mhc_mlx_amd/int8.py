@@ -38,16 +38,38 @@ class Int8Rows(NamedTuple):
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values that the rows stand for."""
         if self.codes.is_cuda and dtype != torch.float64:
-            with timed("dequantize_int8"):
-                return ops._binding().dequantize_int8(self.codes, self.scales, ops._code(dtype))
+            return call("dequantize_int8", self.codes, self.scales, ops._code(dtype))
         out = torch.empty(self.codes.shape, dtype=dtype, device=self.codes.device)
         return torch.mul(self.codes, self.scales.unsqueeze(-1), out=out)
 
 
+class RecordedFn(torch.autograd.Function):
+    """A call of the binding without a gradient, as a node that torch.jit.trace keeps and runs again."""
+
+    @staticmethod
+    def forward(ctx, name, *args):
+        out = getattr(ops._binding(), name)(*args)
+        ctx.mark_non_differentiable(*(out if isinstance(out, tuple) else (out,)))
+        return out
+
+    @staticmethod
+    def backward(ctx, *grads):  # pragma: no cover - its results are not differentiable
+        return None
+
+
+def call(name: str, *args):
+    """A call of the binding without a gradient, under a kernel timer or while torch.jit.trace records."""
+    if torch._C._is_tracing():
+        return RecordedFn.apply(name, *args)
+    with timed(name):
+        return getattr(ops._binding(), name)(*args)
+
+
 def quantize_int8(x: torch.Tensor) -> Int8Rows:
     """x [..., K] in 8 bits, with a scale for each row. Rows may lie any distance apart; other strides are copied."""
-    with timed("quantize_int8"):
+    if ops._use_binding():
         return Int8Rows(*ops._binding().quantize_int8(x))
+    return Int8Rows(*call("quantize_int8", x))
 
 
 def linear_int8(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None, residual: torch.Tensor | None = None,
@@ -58,8 +80,9 @@ def linear_int8(x: Int8Rows, weight: Int8Rows, bias: torch.Tensor | None = None,
     four-byte words (an odd K) are copied in every call.
     """
     act, out_code = _act_code(activation), ops._code(output_dtype)
-    with timed("linear_int8"):
+    if ops._use_binding():
         return ops._binding().linear_int8(x[0], x[1], weight[0], weight[1], bias, residual, act, out_code)
+    return call("linear_int8", x[0], x[1], weight[0], weight[1], bias, residual, act, out_code)
 
 
 @torch.no_grad()

@@ -23,7 +23,7 @@ import torch
 import torch.nn as nn
 
 from . import layer, ops
-from .int8 import Int8Rows, quantize_int8_reference
+from .int8 import Int8Rows, call, quantize_int8_reference
 from .profiling import timed
 
 __all__ = ["AddRMSNorm", "add_rms_norm", "add_rms_norm_int8", "add_rms_norm_reference"]
@@ -75,9 +75,11 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None = None, weight: 
 def add_rms_norm_int8(x: torch.Tensor, residual: torch.Tensor | None = None, weight: torch.Tensor | None = None, eps: float = 1e-6):
     """(Int8Rows of y, h): add_rms_norm with its output in 8 bits. No autograd."""
     eps = _check_eps(eps)
-    with timed("add_rms_norm_int8"):
+    if ops._use_binding():
         codes, scales, h = ops._binding().add_rms_norm_int8(x, residual, weight, eps)
-    return Int8Rows(codes, scales), h
+    else:
+        codes, scales, h = call("add_rms_norm_int8", x, residual, weight, eps)
+    return Int8Rows(codes, scales), x.detach() if residual is None else h
 
 
 def add_rms_norm_reference(x, residual=None, weight=None, eps: float = 1e-6, int8: bool = False):
@@ -96,6 +98,7 @@ class AddRMSNorm(nn.Module):
     """add_rms_norm with a weight of its own (ones at the start; ``dtype`` may be the rows' or float32).
 
     ``forward(x, residual=None)`` gives (y, h); with ``int8`` y is Int8Rows, without autograd, for an Int8Linear behind it.
+    x and a residual of different dtypes (one of them from an autocast region) are brought to the one that their sum has.
     """
 
     def __init__(self, dim: int, eps: float = 1e-6, *, int8: bool = False, device=None, dtype=None):
@@ -104,6 +107,9 @@ class AddRMSNorm(nn.Module):
         self.weight = nn.Parameter(torch.ones(self.dim, device=device, dtype=dtype))
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
+        if residual is not None and residual.dtype != x.dtype:
+            both = torch.promote_types(x.dtype, residual.dtype)
+            x, residual = x.to(both), residual.to(both)
         if not layer._disabled_by_env() and layer.hip_available():
             why = layer._off_gpu(x, residual, self.weight)
             if why is None:

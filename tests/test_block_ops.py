@@ -160,7 +160,7 @@ def test_int8_refusals_at_the_c_abi(lib):
     def call(x=p, ldx=32, xs=p, w=p, ldw=32, ws=p, out=p, od=1, act=0, M=100, N=8, K=32, buf=None, n=0):
         return lib.mhc_linear_int8(x, ldx, xs, w, ldw, ws, None, None, out, od, act, M, N, K, buf, n, None)
 
-    for bad in (dict(M=-1), dict(N=0), dict(K=0), dict(M=1 << 28), dict(N=1 << 22), dict(K=1 << 17, ldx=1 << 17, ldw=1 << 17), dict(od=3), dict(act=5),
+    for bad in (dict(M=-1), dict(N=0), dict(K=0), dict(M=1 << 28), dict(N=1 << 22), dict(M=1 << 27, N=1 << 21), dict(K=1 << 17, ldx=1 << 17, ldw=1 << 17), dict(od=3), dict(act=5),
                 dict(act=-1), dict(x=None), dict(xs=None), dict(w=None), dict(ws=None), dict(out=None), dict(ldx=31), dict(ldw=31)):
         assert call(**bad) == -1, bad
     assert call(M=0, x=None) == 0
@@ -182,7 +182,7 @@ def test_cross_entropy_refusals_at_the_c_abi(lib):
     def bwd(a, state=p, dx=p, dw=p, ws=p, n=1 << 40):
         return lib.mhc_linear_ce_bwd(ctypes.byref(a) if a else None, state, None, ctypes.c_float(1.0), dx, dw, ws, n, None)
 
-    for kw in (dict(T=-1), dict(V=0), dict(C=0), dict(T=1 << 28), dict(V=1 << 22), dict(C=1 << 22), dict(dtype=3), dict(denominator=-1.0), dict(x=None),
+    for kw in (dict(T=-1), dict(V=0), dict(C=0), dict(T=1 << 28), dict(V=1 << 22), dict(C=1 << 22), dict(T=1 << 27, V=1 << 21), dict(dtype=3), dict(denominator=-1.0), dict(x=None),
                dict(w=None), dict(targets=None), dict(ldx=15), dict(ldw=15), dict(weights=p, weights_dtype=1)):
         assert fwd(args(**kw)) == -1 and bwd(args(**kw)) == -1, kw
     a = args()

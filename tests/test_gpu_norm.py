@@ -83,6 +83,31 @@ def test_int8(dt, C):
         check_codes(q.codes, q.scales, x.double(), 0.0)
 
 
+@pytest.mark.parametrize("T,C", [((1 << 22) + 7, 6), ((1 << 20) + 9, 2056)])
+def test_more_rows_than_a_launch_has_workgroups(T, C):
+    """Rows that go round again: first, middle and last ones against float64, and every scale."""
+    g = gen(T)
+    x = torch.empty(T, C, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    w = (1 + 0.3 * rand(g, C)).bfloat16()
+    at = torch.tensor([0, 1, 255, (1 << 20) - 1, 1 << 20, (1 << 20) + 1, T - 2, T - 1], device="cuda")
+    y, _ = add_rms_norm(x, None, w, eps=EPS)
+    _, y0, bound = normed64(x[at], None, w, EPS)
+    close(y[at], y0, bound, "y")
+    del y
+    q = quantize_int8(x)
+    check_codes(q.codes[at], q.scales[at], x[at].double(), 0.0)
+    assert torch.allclose(q.scales, x.abs().amax(1).float() / 127, rtol=1e-6, atol=0)
+    del q
+    if C > 6:
+        return
+    xs, ws = x.requires_grad_(True), w.requires_grad_(True)
+    dx, dw = torch.autograd.grad(add_rms_norm(xs, None, ws, eps=EPS)[0], [xs, ws], torch.ones_like(x))
+    h, z, s, off = norm64(x, None, w, EPS)
+    (rdx, bdx), (rdw, bdw) = norm_grads64(h, z, s, off, w, torch.ones_like(x), None, x.dtype, w.dtype)
+    close(dx, rdx, bdx, "dx")
+    close(dw, rdw, bdw, "dw")
+
+
 def test_codes_of_ties_and_of_extreme_values():
     """Halves go to the even code, and the largest and smallest values of fp32 have their codes."""
     x = torch.tensor([[127.0, 0.5, 1.5, 2.5, -0.5, -1.5, -126.5, 126.5]], device="cuda")
@@ -216,6 +241,8 @@ def test_module_and_refusals():
     m8 = AddRMSNorm(96, int8=True, device="cuda", dtype=torch.bfloat16)
     rows, h = m8(x)
     assert torch.equal(rows.codes, quantize_int8(x).codes) and h is not None
+    mixed = AddRMSNorm(96, device="cuda")(x, x.float())
+    assert all(a.dtype == torch.float32 and torch.equal(a, b) for a, b in zip(mixed, add_rms_norm(x.float(), x.float(), m.weight)))
     for bad in (dict(residual=x[:2]), dict(residual=x.float()), dict(weight=torch.ones(95, device="cuda")), dict(eps=0.0), dict(eps=float("nan")),
                 dict(weight=torch.ones(96, device="cuda", dtype=torch.float16)), dict(weight=torch.ones(96)), dict(residual=x.cpu())):
         with pytest.raises(ValueError):
@@ -225,6 +252,38 @@ def test_module_and_refusals():
     for bad in (x.double(), x.cpu(), torch.ones(3, 0, device="cuda"), torch.ones(3, 8, device="cuda", dtype=torch.int32)):
         with pytest.raises(ValueError):
             quantize_int8(bad)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_traced_calls_run_the_kernels_again(grad):
+    """torch.jit.trace keeps the calls as nodes, those without a gradient too."""
+    from mhc_mlx_amd import Int8Linear, linear_cross_entropy_and_grad
+
+    g = gen(12)
+    targets = torch.randint(0, 50, (6,), generator=g, device="cuda")
+
+    class Block(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.norm, self.lin = AddRMSNorm(64, device="cuda"), Int8Linear.from_linear(torch.nn.Linear(64, 32, device="cuda"))
+            self.register_buffer("head", torch.randn(50, 64, generator=g, device="cuda"))
+
+        def forward(self, x, r):
+            y, h = self.norm(x, r)
+            rows, _ = add_rms_norm_int8(x, r, self.norm.weight)
+            loss, logp, dx, dw = linear_cross_entropy_and_grad(y.detach(), self.head, targets)
+            return y, h, self.lin(rows), self.lin(x), rows.dequantize(torch.bfloat16), quantize_int8(h).scales, loss, logp, dx, dw
+
+    f = Block()
+    traced = torch.jit.trace(f, (rand(g, 6, 64).requires_grad_(grad), rand(g, 6, 64)), check_trace=False)
+    for _ in range(2):
+        x, r = rand(g, 6, 64).requires_grad_(grad), rand(g, 6, 64)
+        with torch.set_grad_enabled(grad):
+            got, want = traced(x, r), f(x, r)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        if grad:
+            up = rand(g, 6, 64)
+            assert torch.equal(*(torch.autograd.grad(o[0], x, up)[0] for o in (got, want)))
 
 
 def test_captured_calls_and_other_streams():
