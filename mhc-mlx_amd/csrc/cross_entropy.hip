@@ -37,12 +37,6 @@ constexpr int kFew = 256, kMany = 1024;
 // dz of a piece of the vocabulary takes at most about this much.
 constexpr int64_t kPieceBytes = 256 << 20;
 
-MHC_DEV float weight_of(const mhc_linear_ce_args& a, int64_t t) {
-  if (a.weights == nullptr) return 1.f;
-  return a.weights_dtype == MHC_DTYPE_U8 ? (static_cast<const uint8_t*>(a.weights)[t] != 0 ? 1.f : 0.f)
-                                         : static_cast<const float*>(a.weights)[t];
-}
-
 // The live tokens, in order, with their weights, and D: one workgroup, whose
 // threads have kRun tokens each of a chunk.
 template <int THREADS>
@@ -62,7 +56,7 @@ __global__ __launch_bounds__(THREADS) void ce_live_kernel(const mhc_linear_ce_ar
 #pragma unroll
     for (int k = 0; k < kRun; ++k) {  // (tokens past the last one read it once more: a load under a condition would wait for itself)
       const int64_t t = min(t0 + k, a.T - 1);
-      w[k] = weight_of(a, t);
+      w[k] = ce::weight_of(a, t);
       y[k] = a.targets[t];
     }
     int count = 0;
@@ -116,11 +110,7 @@ __global__ __launch_bounds__(THREADS) void ce_live_kernel(const mhc_linear_ce_ar
     sum += sums[v];
     top = fmaxf(top, tops[v]);
   }
-  const double d = a.denominator > 0.f ? (double)a.denominator : sum != 0 ? sum : 1.0;
-  s.head[0] = total;
-  reinterpret_cast<float*>(s.head)[1] = (float)((double)top / d);
-  reinterpret_cast<float*>(s.head)[2] = top;
-  *reinterpret_cast<double*>(s.head + 4) = d;
+  ce::store_head(a, s, total, sum, top);
 }
 
 // the live rows of x, one after the other, in whole chunks of 16 bytes with zeros after the last element
@@ -327,6 +317,7 @@ struct FwdPlan {
   int64_t tiles;
   int64_t piece;  // columns of the vocabulary at a time
   bool direct;    // the live rows of x are read where they lie
+  bool few;       // and found by the products' launch
   size_t x, w, part, at_target, total;  // bytes; terms come last
 };
 
@@ -334,7 +325,7 @@ FwdPlan plan_fwd(const mhc_linear_ce_args& a) {
   constexpr int kBn[] = {256, 256, 128, 128, 64};
   FwdPlan p;
   const int e = gemm::elem_bytes(a.dtype);
-  p.direct = false;
+  p.direct = p.few = false;
   if (in_halves(a)) {
     p.piece = halves_piece(a);
     const HalvesPlan h = plan_halves(a, p.piece);
@@ -345,6 +336,7 @@ FwdPlan plan_fwd(const mhc_linear_ce_args& a) {
     p.piece = a.V;
     p.cut = gemm::cut_of(a.T, a.V, a.C, a.dtype, true, true, 1);
     p.direct = gemm::in_words(a.x, a.ldx, a.C, e) && ((a.T - 1) * a.ldx + a.C) * e < ((int64_t)1 << 31);
+    p.few = p.direct && a.T <= 64 && p.cut.tile >= 3;
     p.x = p.direct ? 0 : up256((size_t)(a.T * padded(a.C, a.dtype)) * e);
     p.w = gemm::pack_bytes(a.w, a.V, a.ldw, a.C, a.dtype);
   }
@@ -479,9 +471,11 @@ extern "C" int mhc_linear_ce_fwd(const mhc_linear_ce_args* args, float* loss, fl
   FwdPlan p = {};
   if (a.T > 0) p = plan_fwd(a);
   MHC_CHECK_ARG(workspace_bytes >= p.total && (p.total == 0 || workspace != nullptr), "workspace too small");
-  if (a.T <= kFew) hipLaunchKernelGGL((ce_live_kernel<kFew>), dim3(1), dim3(kFew), 0, s, a, logp, st);
-  else hipLaunchKernelGGL((ce_live_kernel<kMany>), dim3(1), dim3(kMany), 0, s, a, logp, st);
-  MHC_CHECK_LAUNCH("ce_live_kernel");
+  if (!p.few) {
+    if (a.T <= 8 * kFew) hipLaunchKernelGGL((ce_live_kernel<kFew>), dim3(1), dim3(kFew), 0, s, a, logp, st);
+    else hipLaunchKernelGGL((ce_live_kernel<kMany>), dim3(1), dim3(kMany), 0, s, a, logp, st);
+    MHC_CHECK_LAUNCH("ce_live_kernel");
+  }
   char* ws = static_cast<char*>(workspace);
   float2* part = nullptr;
   float* at_target = nullptr;
@@ -511,7 +505,10 @@ extern "C" int mhc_linear_ce_fwd(const mhc_linear_ce_args* args, float* loss, fl
       }
       ws = w;
       if (const int rc = gemm::operand(q.b, a.w, a.V, a.ldw, a.C, a.dtype, ws, s)) return rc;
-      if (const int rc = runs_of(a.dtype).sums(q, ce::RowsOf{p.direct ? st.index : nullptr, a.T}, p.cut, st.head, of, {}, s)) return rc;
+      const ce::Runs& run = runs_of(a.dtype);
+      const int rc = p.few ? run.sums_few(q, p.cut, of, ce::FewTokens{a, st, logp}, s)
+                           : run.sums(q, ce::RowsOf{p.direct ? st.index : nullptr, a.T}, p.cut, st.head, of, {}, s);
+      if (rc != MHC_OK) return rc;
     }
     hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(a.T, 4), 1 << 20)), dim3(256), 0, s, st, (const float2*)part,
                        (const float*)at_target, p.tiles, logp, terms);
