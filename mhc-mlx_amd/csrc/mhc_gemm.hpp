@@ -884,7 +884,10 @@ MHC_DEV void run_tile(const Product& p, char* smem, uint32_t tile, int split, in
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int bit = 4 * (i * JM + j) + k;
-            if (past(acc[i][j][k]) && j * 16 < rows && i * 16 + k < cols) mark[bit / 32] |= 1u << bit % 32;
+            if (past(acc[i][j][k]) && j * 16 < rows && i * 16 + k < cols) {
+              mark[bit / 32] |= 1u << bit % 32;
+              acc[i][j][k] = 0.f;  // (a residual that is the output stays as it is for the second time)
+            }
           }
 #pragma unroll
       for (int w = 0; w < B::kWords; ++w) {

@@ -65,6 +65,12 @@ def test_vocabularies_of_several_pieces(dt):
     check(x, w, y, torch.rand(5000, generator=g, device="cuda") < 0.9)
 
 
+def test_gradients_of_huge_weights_over_several_pieces():
+    """Weights around 2^112, whose sums in dx are formed a second time, are added to those of the pieces before."""
+    x, w, y, _ = inputs(16, 5000, 30011, 256, torch.float32)
+    check(x * 2.0 ** -112, w * 2.0 ** 112, y)
+
+
 @pytest.mark.parametrize("dt", DTYPES)
 def test_tokens_left_out(dt):
     x, w, y, g = inputs(5, 200, 333, 48, dt)
