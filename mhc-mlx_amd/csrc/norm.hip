@@ -114,16 +114,18 @@ MHC_DEV void weights_of(const void* w, bool f32, int64_t n, int left, float (&v)
   }
 }
 
-// s of a row from its sum of squares.  Squares past fp32's range are summed
-// once more, of values scaled by the row's largest (sum(k) gives that of the
-// values times k, largest() their largest magnitude).
+// s of a row from its sum of squares, over `by`, which is 1.  Squares past fp32's
+// range are summed once more, of values times a power of two that brings the
+// row's largest to 1, and that is `by` (sum(k) gives the sum for values times k,
+// largest() their largest magnitude).
 template <typename Sum, typename Largest>
-MHC_DEV float factor_of(float squares, int C, float eps, Sum sum, Largest largest) {
+MHC_DEV float factor_of(float squares, int C, float eps, float& by, Sum sum, Largest largest) {
+  by = 1.f;
   if (squares < __builtin_inff()) return 1.f / sqrtf(squares / (float)C + eps);
   const float top = largest();
   if (!(top < __builtin_inff())) return top == __builtin_inff() ? 0.f : top;
-  const float k = __builtin_bit_cast(float, (254u - min(__builtin_bit_cast(uint32_t, top) >> 23, 253u)) << 23);
-  return k / sqrtf(sum(k) / (float)C + eps * k * k);
+  by = __builtin_bit_cast(float, (254u - min(__builtin_bit_cast(uint32_t, top) >> 23, 253u)) << 23);
+  return 1.f / sqrtf(sum(by) / (float)C + eps * by * by);
 }
 
 // --------------------------------------------------------------------------
@@ -239,7 +241,8 @@ __global__ __launch_bounds__((Held<T, THREADS, NV>::kBlock)) void norm_held_kern
         for (int k = 0; k < V; ++k) q = fmaf(z[i][k] * by, z[i][k] * by, q);
       return join_threads<THREADS>(q, SumOp{}, lds[0]);
     };
-    s = factor_of(squares(1.f), a.C, a.eps, squares, [&] {
+    float by;
+    s = factor_of(squares(1.f), a.C, a.eps, by, squares, [&] {
       float m = fabsf(z1);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
@@ -247,6 +250,15 @@ __global__ __launch_bounds__((Held<T, THREADS, NV>::kBlock)) void norm_held_kern
         for (int k = 0; k < V; ++k) m = LargerOp{}(m, fabsf(z[i][k]));
       return join_threads<THREADS>(m, LargerOp{}, lds[1]);
     });
+    if constexpr (MODE == kPlain) {
+      s *= by;
+    } else if (by != 1.f) {  // (products with the weights may be past the range, too)
+      z1 *= by;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) z[i][k] *= by;
+    }
   }
   if constexpr (MODE == kPlain) {
     if (at.tid == 0 && a.rstd != nullptr) a.rstd[t] = s;
@@ -326,11 +338,11 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(const NormArgs 
       }
     });
     if (a.r != nullptr) row = h;  // (each thread reads what it wrote)
-    float s = 1.f;
+    float s = 1.f, by = 1.f;
     if constexpr (MODE != kCodesOnly) {
       squares = join_threads<kLongThreads>(squares, SumOp{}, lds);
       s = factor_of(
-          squares, C, a.eps,
+          squares, C, a.eps, by,
           [&](float by) {
             float q = 0.f;
             each(row, [&](int, int, float(&z)[V], auto) {
@@ -347,6 +359,17 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(const NormArgs 
             });
             return join_threads<kLongThreads>(m, LargerOp{}, lds);
           });
+      if constexpr (MODE == kPlain) {
+        s *= by;
+      } else if (by != 1.f) {  // (products with the weights may be past the range, too)
+        top = 0.f;
+        each(row, [&](int n, int left, float(&z)[V], auto whole) {
+          float w[V];
+          weights_of<decltype(whole)::value, T>(a.w, w_f32, n, left, w);
+#pragma unroll
+          for (int k = 0; k < V; ++k) top = LargerOp{}(top, fabsf(z[k] * by * w[k]));
+        });
+      }
     }
     if constexpr (MODE != kPlain) top = join_threads<kLongThreads>(top, LargerOp{}, lds);
     if (threadIdx.x == 0) {
@@ -364,7 +387,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(const NormArgs 
         gemm::put<W>(static_cast<T*>(a.y) + t * C + n, z, left);
       } else {
 #pragma unroll
-        for (int k = 0; k < V; ++k) z[k] *= w[k];
+        for (int k = 0; k < V; ++k) z[k] = z[k] * by * w[k];
         put_codes<W>(static_cast<int8_t*>(a.y) + t * C + n, coder, z, left);
       }
     });

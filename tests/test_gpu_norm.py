@@ -162,6 +162,19 @@ def test_squares_past_the_range(dt, C):
         check_codes(rows.codes, rows.scales, y, (C + 8) * U32 + 2.0 ** -149 * scale * 4)
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("C", [48, 1024, 9000, 50000])
+def test_codes_of_products_past_the_range(dt, C):
+    """Rows up to 1.2e38 times weights around 20: the products are past fp32's range, the normed values are around 20."""
+    x = rand(gen(C), 3, C, dt=dt).clamp(-4, 4) * 3e37
+    x[1] = 1.0  # (a row beside them is not touched)
+    w = (20 * (1 + 0.3 * rand(gen(C + 1), C))).to(dt)
+    h, z, s, _ = norm64(x, None, w, EPS)
+    rows, _ = add_rms_norm_int8(x, None, w, eps=EPS)
+    # (eps is nothing beside those squares)
+    check_codes(rows.codes, rows.scales, z * s * ones(w, z), (C + 8) * U32)
+
+
 def test_strides_and_shapes():
     g = gen(3)
     wide = rand(g, 6, 5, 300, dt=torch.bfloat16)
