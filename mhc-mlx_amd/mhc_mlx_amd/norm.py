@@ -98,7 +98,8 @@ class AddRMSNorm(nn.Module):
     """add_rms_norm with a weight of its own (ones at the start; ``dtype`` may be the rows' or float32).
 
     ``forward(x, residual=None)`` gives (y, h); with ``int8`` y is Int8Rows, without autograd, for an Int8Linear behind it.
-    x and a residual of different dtypes (one of them from an autocast region) are brought to the one that their sum has.
+    x and a residual of different dtypes (one of them from an autocast region) are brought to the one that their sum has,
+    and a weight of neither that dtype nor float32 to float32.
     """
 
     def __init__(self, dim: int, eps: float = 1e-6, *, int8: bool = False, device=None, dtype=None):
@@ -110,18 +111,19 @@ class AddRMSNorm(nn.Module):
         if residual is not None and residual.dtype != x.dtype:
             both = torch.promote_types(x.dtype, residual.dtype)
             x, residual = x.to(both), residual.to(both)
+        weight = self.weight if self.weight.dtype in (x.dtype, torch.float32) else self.weight.float()
         if not layer._disabled_by_env() and layer.hip_available():
             why = layer._off_gpu(x, residual, self.weight)
             if why is None:
                 try:
-                    return (add_rms_norm_int8 if self.int8 else add_rms_norm)(x, residual, self.weight, self.eps)
+                    return (add_rms_norm_int8 if self.int8 else add_rms_norm)(x, residual, weight, self.eps)
                 except RuntimeError as e:
                     why = e
             layer._fallback_warning(" in AddRMSNorm", why)
         if self.int8:
             with torch.no_grad():
-                return add_rms_norm_reference(x, residual, self.weight, self.eps, int8=True)
-        return add_rms_norm_reference(x, residual, self.weight, self.eps)
+                return add_rms_norm_reference(x, residual, weight, self.eps, int8=True)
+        return add_rms_norm_reference(x, residual, weight, self.eps)
 
     def extra_repr(self) -> str:
         return f"{self.dim}, eps={self.eps}" + (", int8=True" if self.int8 else "")

@@ -256,6 +256,13 @@ def test_module_and_refusals():
     assert torch.equal(rows.codes, quantize_int8(x).codes) and h is not None
     mixed = AddRMSNorm(96, device="cuda")(x, x.float())
     assert all(a.dtype == torch.float32 and torch.equal(a, b) for a, b in zip(mixed, add_rms_norm(x.float(), x.float(), m.weight)))
+    half = AddRMSNorm(96, device="cuda", dtype=torch.bfloat16)
+    with torch.no_grad():
+        half.weight.copy_(rand(g, 96))
+    y, h = half(x, x.float())  # (the sum has float32, the weight neither that nor the rows' dtype of before)
+    assert torch.equal(y, add_rms_norm(h, None, half.weight.float())[0]) and h.dtype == torch.float32
+    d, = torch.autograd.grad(y, half.weight, torch.ones_like(y))
+    assert d.dtype == torch.bfloat16 and bool(d.isfinite().all())
     for bad in (dict(residual=x[:2]), dict(residual=x.float()), dict(weight=torch.ones(95, device="cuda")), dict(eps=0.0), dict(eps=float("nan")),
                 dict(weight=torch.ones(96, device="cuda", dtype=torch.float16)), dict(weight=torch.ones(96)), dict(residual=x.cpu())):
         with pytest.raises(ValueError):
