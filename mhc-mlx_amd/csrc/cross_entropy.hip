@@ -37,8 +37,8 @@ constexpr int kFew = 256, kMany = 1024;
 // dz of a piece of the vocabulary takes at most about this much: the two of
 // them under way then stay near what the last-level cache holds, and few pieces
 // read and write dx's sums (6144 of 8192 tokens, 50257 columns, C = 4096 bf16: 64
-// MB a piece 9.44 ms, 128 8.27, 256 8.27, 512 8.64, 1024 9.39; 3072 of 4096, 131072,
-// 1024: 3.54, 3.39, 3.28, 3.35, 3.41).
+// MB a piece 9.44 ms, 128 8.27, 256 8.27, 512 8.64, 1024 9.39; three in four of 4096,
+// 131072, 1024: 3.54, 3.39, 3.28, 3.35, 3.41).
 constexpr int64_t kPieceBytes = 256 << 20;
 
 // The live tokens, in order, with their weights, and D: one workgroup, whose

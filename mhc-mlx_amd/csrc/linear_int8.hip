@@ -4,7 +4,8 @@
 // The products' sums are whole numbers in 32 bits, exact: a term is at most
 // 2^14, and there are fewer than 2^17 of them.  They are scaled in registers
 // on their way to the epilogue, each of the two scales and the sum's way to
-// fp32 one rounding.
+// fp32 one rounding.  (Where few outputs leave CUs idle, the reduction is cut
+// into up to 16 parts, which are scaled each and added in fp32.)
 #include "mhc_operand.hpp"
 
 namespace mhc {

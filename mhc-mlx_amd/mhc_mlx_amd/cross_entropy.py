@@ -11,10 +11,10 @@ gradient and the weight's NaN (it cannot be refused without waiting for the GPU)
 
 The logits are formed in pieces, in fp32 of exact products, and again for the gradients, where softmax - onehot, times the
 token's weight over the largest one, is rounded once to x's dtype as an operand of two more products.  Of float32 operands
-the products are those of linear_act, but logits past 2^95 are NaN; of many tokens they are formed of fp16 parts, which hold
-a value to 2^-24 of itself and to 2^-40 of its row's largest.  Beside copies of operands whose rows are no whole four-byte
-words, a call takes workspace in proportion to the tokens (their rows of x, the sums of its gradient, twelve bytes for each
-64 to 256 columns) and up to some 0.5 GB for pieces of the vocabulary, whatever its size.
+the products are those of linear_act, but values from 2^111 on and logits past 2^95 make NaN; of many tokens the logits are
+formed of fp16 parts, which hold a value to 2^-24 of itself and to 2^-40 of its row's largest.  Beside copies of operands
+whose rows are no whole four-byte words, a call takes workspace in proportion to the tokens (their rows of x, the sums of its
+gradient, eight bytes for each 64 to 256 columns) and up to some 0.5 GB for pieces of the vocabulary, whatever its size.
 
 x and weight are taken as they are, under torch.autocast too.
 
