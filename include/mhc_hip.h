@@ -523,10 +523,16 @@ typedef struct {
   int dtype;
   int64_t ignore_index;
   float denominator;
+  float* logits; /* or NULL; see mhc_linear_ce_logits_bytes */
 } mhc_linear_ce_args;
 
 /* Bytes of what the forward leaves for the backward. */
 size_t mhc_linear_ce_state_bytes(int64_t T);
+
+/* Bytes of the logits, for args->logits, in which the forward then keeps them
+ * and the backward finds them; 0 where they are more than it is worth to keep
+ * (2 GiB).  With args->logits NULL the backward forms them again. */
+size_t mhc_linear_ce_logits_bytes(const mhc_linear_ce_args* args);
 
 size_t mhc_linear_ce_fwd_workspace_bytes(const mhc_linear_ce_args* args);
 

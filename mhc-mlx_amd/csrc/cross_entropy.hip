@@ -366,6 +366,9 @@ int run_halves(bool last_low, const void* x, int64_t ld, char* to, const float**
   return MHC_OK;
 }
 
+// Logits are kept for the backward where they take up to this much.
+constexpr int64_t kKeepBytes = (int64_t)2 << 30;
+
 struct BwdPlan {
   int64_t piece;   // columns of the vocabulary
   bool joint;      // a piece's dx and dW go with the next one's dz
@@ -378,7 +381,9 @@ BwdPlan plan_bwd(const mhc_linear_ce_args& a, bool dx, bool dw) {
   BwdPlan p = {};
   const int64_t e = gemm::elem_bytes(a.dtype), pieces = std::max<int64_t>(1, ceil_div(a.T * a.V * e, kPieceBytes));
   p.piece = std::min(a.V, ceil_div(ceil_div(a.V, pieces), 256) * 256);
-  if (in_halves(a)) {
+  if (a.logits != nullptr) {
+    p.dz = Cut{};
+  } else if (in_halves(a)) {
     p.piece = std::min(p.piece, halves_piece(a));
     p.halves = plan_halves(a, p.piece);
     p.dz = gemm::cut_of(a.T, p.piece, 3 * p.halves.wide, kF16, true, true, 1);
@@ -395,7 +400,7 @@ BwdPlan plan_bwd(const mhc_linear_ce_args& a, bool dx, bool dw) {
     const float cus = (float)device_cu_count();
     const int kK = gemm::stage_k(a.dtype), deep = (int)ceil_div(p.piece, kK), low = (int)ceil_div(a.T, kK), of_c = (int)ceil_div(a.C, kK);
     const float mt = (float)ceil_div(a.T, 256), mv = (float)ceil_div(p.piece, 256), mc = (float)ceil_div(a.C, 256);
-    const float units = mt * mc * deep + mv * mc * low + (p.piece < a.V ? mt * mv * of_c : 0.f);
+    const float units = mt * mc * deep + mv * mc * low + (p.piece < a.V && a.logits == nullptr ? mt * mv * of_c : 0.f);
     const int splits = std::min(16, std::max(1, (int)ceilf(2.f * deep * cus / units))), per = (int)ceil_div(deep, splits);
     const float us = c.ends + std::max(1.05f * units / cus * gemm::stage_us(c, a.dtype, 1.f), std::max(std::max(per, low), of_c) * gemm::stage_us(c, a.dtype, 0.f));
     const float apart = p.dx.us + p.dw.us + (p.piece < a.V ? p.dz.us : 0.f);
@@ -448,6 +453,7 @@ int check_args(const mhc_linear_ce_args* a) {
   if (a->T == 0) return MHC_OK;
   MHC_CHECK_ARG(a->x && a->w && a->targets, "null pointer");
   MHC_CHECK_ARG((a->ldx >= a->C || a->T == 1) && (a->ldw >= a->C || a->V == 1), "ldx and ldw must be at least C");
+  MHC_CHECK_ARG(aligned(a->logits, 16), "logits must be 16-byte aligned");
   MHC_CHECK_ARG(a->weights == nullptr || a->weights_dtype == MHC_DTYPE_F32 || a->weights_dtype == MHC_DTYPE_U8, "weights must be fp32 or bytes");
   return MHC_OK;
 }
@@ -456,6 +462,12 @@ int check_args(const mhc_linear_ce_args* a) {
 }  // namespace mhc
 
 extern "C" size_t mhc_linear_ce_state_bytes(int64_t T) { return T < 0 ? 0 : mhc::ce::State::bytes(T); }
+
+extern "C" size_t mhc_linear_ce_logits_bytes(const mhc_linear_ce_args* a) {
+  if (a == nullptr || a->T <= 0 || a->V <= 0 || a->T >= ((int64_t)1 << 28) || a->V >= ((int64_t)1 << 22)) return 0;
+  const int64_t bytes = a->T * mhc::ce::kept_pitch(a->V) * 4;
+  return bytes <= mhc::kKeepBytes ? (size_t)bytes : 0;
+}
 
 extern "C" size_t mhc_linear_ce_fwd_workspace_bytes(const mhc_linear_ce_args* a) {
   if (a == nullptr || a->T <= 0 || a->V <= 0 || a->C <= 0) return 0;
@@ -489,7 +501,7 @@ extern "C" int mhc_linear_ce_fwd(const mhc_linear_ce_args* args, float* loss, fl
     part = reinterpret_cast<float2*>(ws + p.x + p.w);
     at_target = reinterpret_cast<float*>(ws + p.x + p.w + p.part);
     terms = reinterpret_cast<double*>(ws + p.x + p.w + p.part + p.at_target);
-    ce::SumsOf of = {st.target, part, at_target, p.tiles, 0};
+    ce::SumsOf of = {st.target, part, at_target, p.tiles, 0, {a.logits, ce::kept_pitch(a.V)}};
     if (in_halves(a)) {
       const int64_t wide = padded(a.C, kF16);
       ce::Halves halves;
@@ -555,7 +567,8 @@ extern "C" int mhc_linear_ce_bwd(const mhc_linear_ce_args* args, const void* sta
   char* const of_halves = dz[1] + p.of_dz + p.sums;
   float* const part = reinterpret_cast<float*>(of_halves + p.halves.x + p.halves.w);
   ce::Halves halves = {};
-  if (in_halves(a)) {
+  const ce::Kept kept = {a.logits, ce::kept_pitch(a.V)};
+  if (kept.z == nullptr && in_halves(a)) {
     if (const int rc = run_halves(false, a.x, a.ldx, of_halves, &halves.x, &st, a.T, a.C, p.halves.wide, s)) return rc;
   }
   const float* const unit = reinterpret_cast<const float*>(st.head) + 1;
@@ -581,7 +594,11 @@ extern "C" int mhc_linear_ce_bwd(const mhc_linear_ce_args* args, const void* sta
   };
   int b = 0;
   for (int64_t v0 = 0; v0 < a.V; v0 += p.piece) {
-    if (in_halves(a)) {
+    if (kept.z != nullptr) {
+      if (v0 == 0 || !p.joint) {
+        if (const int rc = run.dz_of_kept(gradient(v0), kept, dz[b], pitch(v0), a.T, columns(v0), st.head, s)) return rc;
+      }
+    } else if (in_halves(a)) {
       const int64_t wide = 3 * p.halves.wide;
       char* const w_halves = of_halves + p.halves.x;
       if (const int rc = run_halves(true, rows_of(v0).p, w.ld, w_halves, &halves.w, nullptr, columns(v0), a.C, p.halves.wide, s)) return rc;
@@ -592,7 +609,7 @@ extern "C" int mhc_linear_ce_bwd(const mhc_linear_ce_args* args, const void* sta
       if (const int rc = run.dz(of_dz(v0, b), p.dz, st.head, pitch(v0), gradient(v0), s)) return rc;
     }
     if (p.joint) {
-      ce::Joint j = {of_dx(v0, b), of_dw(v0, b), {}, a.T * a.C, 0, by, {}};
+      ce::Joint j = {of_dx(v0, b), of_dw(v0, b), {}, a.T * a.C, 0, by, {}, kept};
       if (dx == nullptr) j.dx.M = 0;
       if (dw == nullptr) j.dw.M = 0;
       const int all = (int)ceil_div(a.T, gemm::stage_k(a.dtype)) * gemm::stage_k(a.dtype);

@@ -69,6 +69,13 @@ struct Halves {
   }
 };
 
+// The logits that a forward keeps: of each live token a row of `pitch`.
+struct Kept {
+  float* z;  // or NULL
+  int64_t pitch;
+};
+inline int64_t kept_pitch(int64_t V) { return (V + 63) / 64 * 64; }
+
 // Logits to dz = coef (softmax - [v = target]), zeros past the last column.
 struct Gradient {
   const int* target;
@@ -76,25 +83,75 @@ struct Gradient {
   int64_t v0;  // the vocabulary's index of the first column
   float unit;
 
+  // a token's numbers
+  struct Row {
+    float c, t, each;
+    int to;
+  };
+  MHC_DEV Row row(int64_t m) const {
+    const int to = target[m];
+    const float c = to < 0 ? __builtin_nanf("") : coef[m] * unit;
+    return {c, top[m], c * inv[m], to};
+  }
+
   template <bool FAST, typename P, int JM, int JN>
   MHC_DEV void apply(const Product& p, const P& at, f32x4 (&acc)[JN][JM]) const {
     const int64_t m0 = at.m0 + at.wm + at.lane % 16, n0 = at.n0 + at.wn + at.lane / 16 * 4;
 #pragma unroll
     for (int j = 0; j < JM; ++j) {
-      const int64_t m = min(m0 + j * 16, p.M - 1);
-      const int to = target[m];
-      const float c = to < 0 ? __builtin_nanf("") : coef[m] * unit, t = top[m], each = c * inv[m];
-      const int64_t mine = to < 0 ? -1 : to - v0 - n0;  // the target's place among the lane's columns
+      const Row r = row(min(m0 + j * 16, p.M - 1));
+      const int64_t mine = r.to < 0 ? -1 : r.to - v0 - n0;  // the target's place among the lane's columns
 #pragma unroll
       for (int i = 0; i < JN; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float d = each * gemm::exp_of<FAST>(acc[i][j][k] - t) - (mine == i * 16 + k ? c : 0.f);
+          const float d = r.each * gemm::exp_of<FAST>(acc[i][j][k] - r.t) - (mine == i * 16 + k ? r.c : 0.f);
           acc[i][j][k] = n0 + i * 16 + k < p.N ? d : 0.f;
         }
     }
   }
 };
+
+// The same from logits that were kept: ROWS rows of 256 columns, eight a lane,
+// of dz [rows, width], of which N columns are there.
+template <typename T, int THREADS, int ROWS>
+MHC_DEV void dz_of_kept(const Gradient& g, const Kept& kept, T* dz, int64_t width, int64_t N, int64_t rows, int64_t m0, int64_t n0) {
+  constexpr int kEach = THREADS / 32, kAhead = 4;
+  const int64_t n = n0 + threadIdx.x % 32 * 8;
+  if (n >= width) return;
+  const float* const from = kept.z + g.v0 + n;
+  const int64_t m1 = min(m0 + ROWS, rows);
+  for (int64_t m = m0 + threadIdx.x / 32; m < m1; m += kEach * kAhead) {
+    f32x4 z[kAhead][2];
+    Gradient::Row r[kAhead];
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {  // (rows past the last one read it once more: a load under a condition would wait for itself)
+      const int64_t at = min(m + q * kEach, m1 - 1);
+      const f32x4* const p = reinterpret_cast<const f32x4*>(from + at * kept.pitch);
+      z[q][0] = __builtin_nontemporal_load(p);
+      z[q][1] = __builtin_nontemporal_load(p + 1);
+      r[q] = g.row(at);
+    }
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q) {
+      if (m + q * kEach >= m1) break;
+      const int64_t mine = r[q].to < 0 ? -1 : r[q].to - g.v0 - n;
+      float d[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        d[k] = r[q].each * gemm::exp_of<sizeof(T) == 2>(z[q][k / 4][k % 4] - r[q].t) - (mine == k ? r[q].c : 0.f);
+        d[k] = n + k < N ? d[k] : 0.f;
+      }
+      gemm::put<true>(dz + (m + q * kEach) * width + n, d, 8);
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void dz_kernel(const Gradient g, const Kept kept, T* dz, int64_t width, int64_t N, const int* live) {
+  const uint32_t wide = (uint32_t)ceil_div(width, 256);
+  dz_of_kept<T, 256, 32>(g, kept, dz, width, N, *live, (int64_t)(blockIdx.x / wide) * 32, (int64_t)(blockIdx.x % wide) * 256);
+}
 
 template <bool FAST>
 struct GradientOf : Gradient {
@@ -190,6 +247,7 @@ struct Joint {
   int64_t part, width;  // of a part of dx's sums, and of dz's rows
   ScaledBy by;
   Gradient g;
+  Kept kept;            // what dz is of, if there is any
 };
 
 // A kernel's first argument where it lies, to be read when it is needed: those
@@ -230,6 +288,12 @@ __global__ __launch_bounds__(64 * WM * WN) void joint_kernel(const Joint, const 
     p.M = min(p.M, n);
     id -= all_dx + of_dw;
     if (id >= tiles(p.M, p.N)) return;
+    if (k.kept.z != nullptr) {
+      const uint32_t wide = (uint32_t)ceil_div(p.N, BN);
+      dz_of_kept<T, 64 * WM * WN, BM>(Gradient(k.g), Kept(k.kept), static_cast<T*>(p.e.out), k.width, p.N, p.M, (int64_t)(id / wide) * BM,
+                                      (int64_t)(id % wide) * BN);
+      return;
+    }
     gemm::run_tile<T, true, true, BM, BN, WM, WN, NS, T>(p, smem, id, 0, 0, k.width, GradientOf<sizeof(T) == 2>{k.g});
   }
 }
@@ -315,13 +379,14 @@ struct FewTokens {
 
 // A tile of logits, of which only each row's largest and the sum of
 // exp(logit - largest) are kept, and the target's: to part[row][tile] and
-// at_target[row].  The tile is one of the vocabulary's from v0 on, of which a
-// row has `tiles`.
+// at_target[row]; and the logits themselves, if there is a place for them.  The
+// tile is one of the vocabulary's from v0 on, of which a row has `tiles`.
 struct SumsOf {
   const int* target;
   float2* part;
   float* at_target;
   int64_t tiles, v0;
+  Kept kept;
 };
 
 template <typename T, bool HALVES, int BM, int BN, int WM, int WN, int NS>
@@ -334,6 +399,15 @@ MHC_DEV void sums_tile(const Product& p, const RowsOf& rows, const SumsOf& of, c
   else gemm::sum_tile<T, true, true, BM, BN, WM, WN, NS>(p, at, smem, acc, rows);
   if constexpr (HALVES) halves.scale(p, at, acc);
   const int64_t m0 = at.m0 + at.wm + at.lane % 16, n0 = at.n0 + at.wn + at.lane / 16 * 4;
+  if (of.kept.z != nullptr) {
+    float* const to = of.kept.z + of.v0 + n0;
+#pragma unroll
+    for (int j = 0; j < JM; ++j)
+#pragma unroll
+      for (int i = 0; i < JN; ++i)
+        if (m0 + j * 16 < p.M && of.v0 + n0 + i * 16 < of.kept.pitch)
+          *reinterpret_cast<f32x4*>(to + (m0 + j * 16) * of.kept.pitch + i * 16) = acc[i][j];
+  }
   if (at.n0 + BN > p.N) {
 #pragma unroll
     for (int i = 0; i < JN; ++i)
@@ -473,6 +547,7 @@ struct Runs {
   int (*sums)(Product p, const RowsOf& rows, const Cut& c, const int* live, const SumsOf& of, const Halves& halves, hipStream_t s);
   int (*sums_few)(Product p, const Cut& c, const SumsOf& of, const FewTokens& few, hipStream_t s);
   int (*dz)(const Product& p, const Cut& c, const int* live, int64_t width, const Gradient& g, hipStream_t s);
+  int (*dz_of_kept)(const Gradient& g, const Kept& kept, void* dz, int64_t width, int64_t T, int64_t N, const int* live, hipStream_t s);
   int (*dx)(const Product& p, const Cut& c, const int* live, hipStream_t s);
   int (*dw)(const Product& p, const Cut& c, const int* live, const ScaledBy& by, float* part, hipStream_t s);
   int (*joint)(const Joint& j, const int* live, hipStream_t s);  // of 16-bit operands
@@ -490,6 +565,13 @@ int run_dz(const Product& p, const Cut& c, const int* live, int64_t width, const
   return run_live<T, true, true, false>(p, c, live, width, GradientOf<sizeof(T) == 2>{g}, nullptr, s);
 }
 template <typename T>
+int run_dz_of_kept(const Gradient& g, const Kept& kept, void* dz, int64_t width, int64_t rows, int64_t N, const int* live, hipStream_t s) {
+  const dim3 grid((unsigned)(ceil_div(rows, 32) * ceil_div(width, 256)));
+  hipLaunchKernelGGL((dz_kernel<T>), grid, dim3(256), 0, s, g, kept, static_cast<T*>(dz), width, N, live);
+  MHC_CHECK_LAUNCH("dz_kernel");
+  return MHC_OK;
+}
+template <typename T>
 int run_dx(const Product& p, const Cut& c, const int* live, hipStream_t s) {
   return run_live<T, true, false, true>(p, c, live, p.N, gemm::AsTheyAre{}, nullptr, s);
 }
@@ -501,10 +583,10 @@ int run_dw(const Product& p, const Cut& c, const int* live, const ScaledBy& by, 
 template <typename T>
 const Runs& runs_of() {
   if constexpr (sizeof(T) == 2) {
-    static const Runs r = {run_sums<T, false>, run_sums_few<T>, run_dz<T>, run_dx<T>, run_dw<T>, run_joint<T>};
+    static const Runs r = {run_sums<T, false>, run_sums_few<T>, run_dz<T>, run_dz_of_kept<T>, run_dx<T>, run_dw<T>, run_joint<T>};
     return r;
   } else {
-    static const Runs r = {run_sums<T, false>, run_sums_few<T>, run_dz<T>, run_dx<T>, run_dw<T>, nullptr};
+    static const Runs r = {run_sums<T, false>, run_sums_few<T>, run_dz<T>, run_dz_of_kept<T>, run_dx<T>, run_dw<T>, nullptr};
     return r;
   }
 }

@@ -273,16 +273,21 @@ struct CeResult {
   at::Tensor loss, logp, state;
 };
 
-CeResult ce_forward(const CeInputs& c, const at::Tensor& x) {
+// What the forward leaves: its state and, after it, the logits that are kept.
+size_t ce_state_bytes(const CeInputs& c) { return (mhc_linear_ce_state_bytes(c.args.T) + 255) / 256 * 256; }
+
+CeResult ce_forward(CeInputs& c, const at::Tensor& x, bool keep) {
   const auto opt = f32_options(x);
-  CeResult r = {at::empty({}, opt), at::empty(x.sizes().slice(0, x.dim() - 1), opt), workspace(mhc_linear_ce_state_bytes(c.args.T), x)};
+  const size_t kept = keep ? mhc_linear_ce_logits_bytes(&c.args) : 0;
+  CeResult r = {at::empty({}, opt), at::empty(x.sizes().slice(0, x.dim() - 1), opt), workspace(ce_state_bytes(c) + kept, x)};
+  if (kept > 0) c.args.logits = reinterpret_cast<float*>(static_cast<char*>(r.state.data_ptr()) + ce_state_bytes(c));
   const size_t nb = mhc_linear_ce_fwd_workspace_bytes(&c.args);
   const at::Tensor ws = workspace(nb, x);
   check(mhc_linear_ce_fwd(&c.args, fptr(r.loss), fptr(r.logp), r.state.data_ptr(), ws.data_ptr(), nb, stream_of(x)), "mhc_linear_ce_fwd");
   return r;
 }
 
-std::tuple<at::Tensor, at::Tensor> ce_backward(const CeInputs& c, const at::Tensor& x, const at::Tensor& w, const at::Tensor& state,
+std::tuple<at::Tensor, at::Tensor> ce_backward(CeInputs& c, const at::Tensor& x, const at::Tensor& w, const at::Tensor& state,
                                                const at::Tensor& dloss, double grad_scale, bool want_dx, bool want_dw) {
   at::Tensor dx, dw;
   if (want_dx) dx = at::empty(x.sizes(), x.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
@@ -291,6 +296,7 @@ std::tuple<at::Tensor, at::Tensor> ce_backward(const CeInputs& c, const at::Tens
     if (want_dw) dw.zero_();
     return {dx, dw};
   }
+  if ((size_t)state.numel() > ce_state_bytes(c)) c.args.logits = reinterpret_cast<float*>(static_cast<char*>(state.data_ptr()) + ce_state_bytes(c));
   const size_t nb = mhc_linear_ce_bwd_workspace_bytes(&c.args, want_dx, want_dw);
   const at::Tensor ws = workspace(nb, x);
   check(mhc_linear_ce_bwd(&c.args, state.data_ptr(), fptr(dloss), (float)grad_scale, ptr(dx), ptr(dw), ws.data_ptr(), nb, stream_of(x)),
@@ -298,12 +304,12 @@ std::tuple<at::Tensor, at::Tensor> ce_backward(const CeInputs& c, const at::Tens
   return {dx, dw};
 }
 
-// (loss [], logp [...], what the backward reads)
+// (loss [], logp [...], what the backward reads: of a call that will have one, with `keep`)
 std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_ce_fwd(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets,
-                                                             const OptTensor& mask, double denominator, int64_t ignore_index) {
-  const CeInputs c = ce_inputs(x, w, targets, get(mask), denominator, ignore_index);
+                                                             const OptTensor& mask, double denominator, int64_t ignore_index, bool keep) {
+  CeInputs c = ce_inputs(x, w, targets, get(mask), denominator, ignore_index);
   const at::DeviceGuard guard(x.device());
-  const CeResult r = ce_forward(c, x);
+  const CeResult r = ce_forward(c, x, keep);
   return {r.loss, r.logp, r.state};
 }
 
@@ -311,7 +317,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_ce_fwd(const at::Tensor& x
 std::tuple<at::Tensor, at::Tensor> linear_ce_bwd(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, const OptTensor& mask,
                                                  double denominator, int64_t ignore_index, const at::Tensor& state, const at::Tensor& dloss,
                                                  bool want_dx, bool want_dw) {
-  const CeInputs c = ce_inputs(x, w, targets, get(mask), denominator, ignore_index);
+  CeInputs c = ce_inputs(x, w, targets, get(mask), denominator, ignore_index);
   const at::DeviceGuard guard(x.device());
   return ce_backward(c, x, w, state, dloss.to(at::kFloat).contiguous(), 1.0, want_dx, want_dw);
 }
@@ -321,9 +327,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_ce_and_grad(co
                                                                               const OptTensor& mask, double denominator, int64_t ignore_index,
                                                                               double grad_scale) {
   const at::AutoGradMode plain_mode(false);
-  const CeInputs c = ce_inputs(x, w, targets, get(mask), denominator, ignore_index);
+  CeInputs c = ce_inputs(x, w, targets, get(mask), denominator, ignore_index);
   const at::DeviceGuard guard(x.device());
-  const CeResult r = ce_forward(c, x);
+  const CeResult r = ce_forward(c, x, true);
   auto [dx, dw] = ce_backward(c, x, w, r.state, at::Tensor(), grad_scale, true, true);
   return {r.loss, r.logp, dx, dw};
 }
@@ -331,7 +337,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_ce_and_grad(co
 struct LinearCeFn : public torch::autograd::Function<LinearCeFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, const OptTensor& mask,
                                double denominator, int64_t ignore_index) {
-    auto [loss, logp, state] = linear_ce_fwd(x, w, targets, mask, denominator, ignore_index);
+    auto [loss, logp, state] = linear_ce_fwd(x, w, targets, mask, denominator, ignore_index, true);
     ctx->save_for_backward({x, w, targets, get(mask), state});
     ctx->saved_data["denominator"] = denominator;
     ctx->saved_data["ignore_index"] = ignore_index;
@@ -355,7 +361,7 @@ struct LinearCeFn : public torch::autograd::Function<LinearCeFn> {
 std::tuple<at::Tensor, at::Tensor> linear_ce(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, const OptTensor& mask,
                                              double denominator, int64_t ignore_index) {
   if (!needs_grad({&x, &w})) {
-    auto [loss, logp, state] = linear_ce_fwd(x, w, targets, mask, denominator, ignore_index);
+    auto [loss, logp, state] = linear_ce_fwd(x, w, targets, mask, denominator, ignore_index, false);
     return {loss, logp};
   }
   variable_list r = LinearCeFn::apply(x, w, targets, mask.has_value() ? OptTensor(mask->detach()) : mask, denominator, ignore_index);

@@ -61,7 +61,8 @@ class LinearCeArgs(ctypes.Structure):
     """mhc_linear_ce_args: the inputs of the calls for the cross entropy from hidden states."""
 
     _fields_ = [("x", _VP), ("ldx", _I64), ("w", _VP), ("ldw", _I64), ("targets", _VP), ("weights", _VP), ("weights_dtype", _I32),
-                ("T", _I64), ("V", _I64), ("C", _I64), ("dtype", _I32), ("ignore_index", _I64), ("denominator", _F32)]
+                ("T", _I64), ("V", _I64), ("C", _I64), ("dtype", _I32), ("ignore_index", _I64), ("denominator", _F32),
+                ("logits", _VP)]
 
 
 _PCE = ctypes.POINTER(LinearCeArgs)
@@ -133,6 +134,7 @@ SIGNATURES = {
     "mhc_add_rms_norm_bwd": ([_VP, _I64, _VP, _I64, _VP, _I64, _VP, _VP, _I32, _VP, _VP, _I64, _I64, _I32, _VP, _SZ, _VP], _I32),
     "mhc_linear_int8_workspace_bytes": ([_VP, _I64, _VP, _I64, _I64, _I64, _I64], _SZ),
     "mhc_linear_int8": ([_VP, _I64, _VP, _VP, _I64, _VP, _VP, _VP, _VP, _I32, _I32, _I64, _I64, _I64, _VP, _SZ, _VP], _I32),
+    "mhc_linear_ce_logits_bytes": ([_PCE], _SZ),
     "mhc_linear_ce_state_bytes": ([_I64], _SZ),
     "mhc_linear_ce_fwd_workspace_bytes": ([_PCE], _SZ),
     "mhc_linear_ce_fwd": ([_PCE, _VP, _VP, _VP, _VP, _SZ, _VP], _I32),

@@ -45,7 +45,7 @@ class LinearCrossEntropyFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, targets, mask, *numbers):
         with timed("linear_cross_entropy_fwd"):
-            loss, logp, state = ops._binding().linear_ce_fwd(x, weight, targets, mask, *numbers)
+            loss, logp, state = ops._binding().linear_ce_fwd(x, weight, targets, mask, *numbers, any(ctx.needs_input_grad[:2]))
         ctx.save_for_backward(x, weight, targets, mask, state)
         ctx.numbers = numbers
         ctx.mark_non_differentiable(logp)

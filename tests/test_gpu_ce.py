@@ -1,9 +1,11 @@
 """linear_cross_entropy on the GPU against float64 (tests/_block.py)."""
 
+import ctypes
+
 import pytest
 import torch
 
-from mhc_mlx_amd import AddRMSNorm, FusedLinear, kernel_timer, linear_cross_entropy, linear_cross_entropy_and_grad, policy_loss
+from mhc_mlx_amd import AddRMSNorm, FusedLinear, _lib, kernel_timer, linear_cross_entropy, linear_cross_entropy_and_grad, ops, policy_loss
 from tests._block import ce64
 from tests._train import close
 
@@ -63,6 +65,41 @@ def test_vocabularies_of_several_pieces(dt):
     x, w, y, g = inputs(3, 5000, 30011, 40, dt)
     y[:7] = torch.tensor([0, 30010, 255, 256, 15103, 15104, 30000], device="cuda")
     check(x, w, y, torch.rand(5000, generator=g, device="cuda") < 0.9)
+
+
+def at_the_c_abi(x, w, y, mask, keep, scale=1.0):
+    """The two calls with the logits kept between them or formed again, whatever the sizes."""
+    lib, byref, T, V = _lib.load(), ctypes.byref, len(x), len(w)
+    pitch = -(-V // 64) * 64
+    logits = torch.full((T * pitch + 64,), float("nan"), device="cuda") if keep else None
+    a = _lib.LinearCeArgs(x=x.data_ptr(), ldx=x.stride(0), w=w.data_ptr(), ldw=w.stride(0), targets=y.data_ptr(), weights=mask.data_ptr(), weights_dtype=3, T=T, V=V,
+                          C=x.shape[1], dtype=ops._code(x.dtype), ignore_index=-100, denominator=0.0, logits=logits.data_ptr() if keep else None)
+    new = lambda n: torch.empty(max(n, 1), dtype=torch.uint8, device="cuda")  # noqa: E731
+    s, loss, logp = torch.cuda.current_stream().cuda_stream, torch.empty((), device="cuda"), torch.empty(T, device="cuda")
+    state = new(lib.mhc_linear_ce_state_bytes(T))
+    nf, nb = lib.mhc_linear_ce_fwd_workspace_bytes(byref(a)), lib.mhc_linear_ce_bwd_workspace_bytes(byref(a), 1, 1)
+    assert lib.mhc_linear_ce_logits_bytes(byref(a)) == T * pitch * 4
+    assert lib.mhc_linear_ce_fwd(byref(a), loss.data_ptr(), logp.data_ptr(), state.data_ptr(), new(nf).data_ptr(), nf, s) == 0
+    outs = []
+    for _ in range(2):  # (the backward leaves the logits as they are)
+        dx, dw = torch.empty_like(x), torch.empty_like(w)
+        assert lib.mhc_linear_ce_bwd(byref(a), state.data_ptr(), None, ctypes.c_float(scale), dx.data_ptr(), dw.data_ptr(), new(nb).data_ptr(), nb, s) == 0
+        outs.append((dx, dw))
+    assert all(torch.equal(p, q) for p, q in zip(*outs))
+    assert not keep or bool(logits[T * pitch:].isnan().all())
+    return dict(loss=loss, logp=logp, dx=dx, dw=dw)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("T,V,C", [(1, 2, 8), (2, 65, 8), (17, 1000, 40), (64, 257, 64), (130, 515, 72), (300, 2050, 128), (700, 1003, 256), (1024, 4096, 256),
+                                   (2050, 3001, 512), (520, 20000, 64), (3000, 500, 1000), (5000, 30011, 40), (4500, 30011, 256)])
+def test_logits_kept_and_formed_again(dt, T, V, C):
+    x, w, y, g = inputs(T + V, T, V, C, dt)
+    mask = (torch.rand(T, generator=g, device="cuda") < 0.8).to(torch.uint8)
+    ref = ce64(x, w, y, mask, scale=16.0)
+    for keep in (True, False):
+        for k, v in at_the_c_abi(x, w, y, mask, keep, 16.0).items():
+            close(v, *ref[k], f"{k} kept {keep}")
 
 
 def test_gradients_of_huge_weights_over_several_pieces():
