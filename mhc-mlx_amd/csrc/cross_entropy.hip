@@ -12,8 +12,8 @@
 // exponentials for each row, which are joined.  Backward: the vocabulary goes
 // by in pieces; the logits of a piece are formed again and become its dz, of
 // which dx (summed up in fp32 over the pieces) and the piece's rows of dW are
-// products.  That is four products of T V C where three would do if the logits
-// were kept.
+// products.  Where the logits are wide and few enough to be kept (keeps_logits),
+// dz is read from them, which saves the fourth product.
 #include "mhc_ce.hpp"
 #include "mhc_operand.hpp"
 #include "mhc_plan.hpp"
@@ -38,7 +38,8 @@ constexpr int kFew = 256, kMany = 1024;
 // them under way then stay near what the last-level cache holds, and few pieces
 // read and write dx's sums (6144 of 8192 tokens, 50257 columns, C = 4096 bf16: 64
 // MB a piece 9.44 ms, 128 8.27, 256 8.27, 512 8.64, 1024 9.39; three in four of 4096,
-// 131072, 1024: 3.54, 3.39, 3.28, 3.35, 3.41).
+// 131072, 1024: 3.54, 3.39, 3.28, 3.35, 3.41; from logits that were kept, 6144
+// tokens: 128 6.80, 256 6.91, 512 7.00, and 4096 x 100000 x 1024 3.17, 3.13, 3.11).
 constexpr int64_t kPieceBytes = 256 << 20;
 
 // The live tokens, in order, with their weights, and D: one workgroup, whose
@@ -366,8 +367,17 @@ int run_halves(bool last_low, const void* x, int64_t ld, char* to, const float**
   return MHC_OK;
 }
 
-// Logits are kept for the backward where they take up to this much.
+// Whether the forward keeps the logits for the backward, which forms them again
+// else: from a width on at which their way through memory and back is shorter
+// than their product (4096 x 100000 bf16 kept and formed again, C = 512 2.20
+// and 2.04 ms, 1024 3.13 and 3.34, 2048 5.02 and 5.88; 6144 x 50257, 4096 6.9
+// and 8.3; 2000 x 32768 fp32, C = 64 0.449 and 0.433, 256 0.75 and 0.81, 2048
+// 3.69 and 4.43), and up to an amount that a card of 288 GB does not miss.
 constexpr int64_t kKeepBytes = (int64_t)2 << 30;
+
+bool keeps_logits(const mhc_linear_ce_args& a) {
+  return a.C >= (a.dtype == kF32 ? 256 : 768) && a.T * ce::kept_pitch(a.V) * 4 <= kKeepBytes;
+}
 
 struct BwdPlan {
   int64_t piece;   // columns of the vocabulary
@@ -465,8 +475,7 @@ extern "C" size_t mhc_linear_ce_state_bytes(int64_t T) { return T < 0 ? 0 : mhc:
 
 extern "C" size_t mhc_linear_ce_logits_bytes(const mhc_linear_ce_args* a) {
   if (a == nullptr || a->T <= 0 || a->V <= 0 || a->T >= ((int64_t)1 << 28) || a->V >= ((int64_t)1 << 22)) return 0;
-  const int64_t bytes = a->T * mhc::ce::kept_pitch(a->V) * 4;
-  return bytes <= mhc::kKeepBytes ? (size_t)bytes : 0;
+  return mhc::keeps_logits(*a) ? (size_t)(a->T * mhc::ce::kept_pitch(a->V) * 4) : 0;
 }
 
 extern "C" size_t mhc_linear_ce_fwd_workspace_bytes(const mhc_linear_ce_args* a) {

@@ -1,4 +1,4 @@
-"""Softmax cross entropy over a vocabulary, from the last hidden states and the head's weight, without keeping the logits.
+"""Softmax cross entropy over a vocabulary, from the last hidden states and the head's weight, without the logits as a tensor.
 
 For a token with hidden state x and target y, and the logits z = weight x:
 
@@ -9,12 +9,14 @@ hold, NaN among them: they add nothing to the loss, their log probability is giv
 products are formed without their rows.  A target outside [0, V) of a token that counts makes the loss, that token's
 gradient and the weight's NaN (it cannot be refused without waiting for the GPU).
 
-The logits are formed in pieces, in fp32 of exact products, and again for the gradients, where softmax - onehot, times the
-token's weight over the largest one, is rounded once to x's dtype as an operand of two more products.  Of float32 operands
-the products are those of linear_act, but values from 2^111 on and logits past 2^95 make NaN; of many tokens the logits are
-formed of fp16 parts, which hold a value to 2^-24 of itself and to 2^-40 of its row's largest.  Beside copies of operands
-whose rows are no whole four-byte words, a call takes workspace in proportion to the tokens (their rows of x, the sums of its
-gradient, eight bytes for each 64 to 256 columns) and up to some 0.5 GB for pieces of the vocabulary, whatever its size.
+The logits are formed in fp32 of exact products. For the gradients, softmax - onehot, times the token's weight over the
+largest one, is rounded once to x's dtype as an operand of two more products, in pieces of the vocabulary; it is formed of
+the logits that the forward kept, where they take up to 2 GiB (and C is 768 or more, of float32 256), or of logits that are
+formed again. Of float32 operands the products are those of linear_act, but values from 2^111 on and logits past 2^95 make
+NaN; of many tokens the logits are formed of fp16 parts, which hold a value to 2^-24 of itself and to 2^-40 of its row's
+largest. Beside copies of operands whose rows are no whole four-byte words, a call takes workspace in proportion to the
+tokens (their rows of x, the sums of its gradient, eight bytes for each 64 to 256 columns) and up to some 0.5 GB for pieces
+of the vocabulary, whatever its size. Kept logits are held until the backward's graph is freed; without gradients none are.
 
 x and weight are taken as they are, under torch.autocast too.
 

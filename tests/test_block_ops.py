@@ -186,9 +186,9 @@ def test_cross_entropy_refusals_at_the_c_abi(lib):
                dict(w=None), dict(targets=None), dict(ldx=15), dict(ldw=15), dict(weights=p, weights_dtype=1)):
         assert fwd(args(**kw)) == -1 and bwd(args(**kw)) == -1, kw
     a = args()
-    assert lib.mhc_linear_ce_logits_bytes(ctypes.byref(a)) == 10 * 64 * 4 and lib.mhc_linear_ce_logits_bytes(None) == 0
-    assert lib.mhc_linear_ce_logits_bytes(ctypes.byref(args(T=1 << 14, V=1 << 15))) == 1 << 31
-    assert lib.mhc_linear_ce_logits_bytes(ctypes.byref(args(T=1 << 14, V=(1 << 15) + 1))) == 0
+    kept = lambda **kw: lib.mhc_linear_ce_logits_bytes(ctypes.byref(args(**kw)))  # noqa: E731
+    assert kept(C=1024) == kept(C=256, dtype=0) == 10 * 64 * 4 and kept() == 0 and lib.mhc_linear_ce_logits_bytes(None) == 0
+    assert kept(T=1 << 14, V=1 << 15, C=1024) == 1 << 31 and kept(T=1 << 14, V=(1 << 15) + 1, C=1024) == 0
     assert fwd(args(logits=4100)) == -1 and bwd(args(logits=4100)) == -1
     nf, nb = lib.mhc_linear_ce_fwd_workspace_bytes(ctypes.byref(a)), lib.mhc_linear_ce_bwd_workspace_bytes(ctypes.byref(a), 1, 1)
     assert nf > 0 and nb > 0 and lib.mhc_linear_ce_state_bytes(10) >= 24 * 10

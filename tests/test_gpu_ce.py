@@ -78,7 +78,7 @@ def at_the_c_abi(x, w, y, mask, keep, scale=1.0):
     s, loss, logp = torch.cuda.current_stream().cuda_stream, torch.empty((), device="cuda"), torch.empty(T, device="cuda")
     state = new(lib.mhc_linear_ce_state_bytes(T))
     nf, nb = lib.mhc_linear_ce_fwd_workspace_bytes(byref(a)), lib.mhc_linear_ce_bwd_workspace_bytes(byref(a), 1, 1)
-    assert lib.mhc_linear_ce_logits_bytes(byref(a)) == T * pitch * 4
+    assert lib.mhc_linear_ce_logits_bytes(byref(a)) in (0, T * pitch * 4)
     assert lib.mhc_linear_ce_fwd(byref(a), loss.data_ptr(), logp.data_ptr(), state.data_ptr(), new(nf).data_ptr(), nf, s) == 0
     outs = []
     for _ in range(2):  # (the backward leaves the logits as they are)
@@ -270,9 +270,23 @@ def test_the_same_call_twice_and_on_another_stream():
     assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
-def test_captured_calls_with_other_masks():
+@pytest.mark.parametrize("dt", DTYPES)
+def test_a_backward_twice(dt):
+    """Logits that are kept stay as they are until the graph is freed; without a gradient the loss is the same."""
+    x, w, y, _ = inputs(17, 130, 700, 776, dt)
+    xs, ws = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss, logp = linear_cross_entropy(xs, ws, y)
+    a = torch.autograd.grad(loss, [xs, ws], retain_graph=True)
+    b = torch.autograd.grad(loss, [xs, ws])
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    plain = linear_cross_entropy(x, w, y)
+    assert torch.equal(plain[0], loss) and torch.equal(plain[1], logp)
+
+
+@pytest.mark.parametrize("C", [128, 800])
+def test_captured_calls_with_other_masks(C):
     """How many tokens count is found on the device: a graph's replays follow the mask."""
-    x, w, y, g = inputs(14, 300, 1000, 128, torch.bfloat16)
+    x, w, y, g = inputs(14, 300, 1000, C, torch.bfloat16)
     mask = torch.ones(300, device="cuda")
 
     def step():
