@@ -113,7 +113,8 @@ struct Gradient {
 };
 
 // The same from logits that were kept: ROWS rows of 256 columns, eight a lane,
-// of dz [rows, width], of which N columns are there.
+// of dz [rows, width], of which N columns are there (6144 x 12800 bf16: 97 us
+// for 472 MB, 4.9 TB/s).
 template <typename T, int THREADS, int ROWS>
 MHC_DEV void dz_of_kept(const Gradient& g, const Kept& kept, T* dz, int64_t width, int64_t N, int64_t rows, int64_t m0, int64_t n0) {
   constexpr int kEach = THREADS / 32, kAhead = 4;
@@ -240,7 +241,8 @@ __global__ __launch_bounds__(64 * WM * WN) void live_tile_kernel(Product p, cons
 // needs another, as one launch, so that the card is full to its end: their
 // tiles are few and long (6144 tokens, 50257 columns in four pieces, C = 4096:
 // 384 of 196 stages on 256 CUs, 800 of 96 and 1200 of 64; 1.62 ms in one launch,
-// 1.88 in three).  The longest go first.  fp32 tiles gain nothing by it (1000
+// 1.88 in three; the whole call, from logits that were kept, 6.8 ms and 7.6).
+// The longest go first.  fp32 tiles gain nothing by it (1000
 // tokens, 32768 columns, C = 1024: 0.79 ms for dx and dW, 0.74 apart).
 struct Joint {
   Product dx, dw, dz;   // M = 0: not there
