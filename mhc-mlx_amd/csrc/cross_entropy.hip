@@ -179,10 +179,9 @@ __global__ __launch_bounds__(256) void ce_halves_kernel(const float* x, int64_t 
     uint32_t bits = __builtin_bit_cast(uint32_t, top);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) bits = max(bits, (uint32_t)__shfl_xor((int)bits, d));
-    // 2^14 over the largest value's power of two, if both are normal numbers (a row with an infinity: 1, and its logits are NaN)
-    const uint32_t e = bits >> 23, up = e == 255 ? 127 : min(268u - max(e, 15u), 253u);
-    const float by = __builtin_bit_cast(float, up << 23);
-    if (k0 == 0) scales[r] = __builtin_bit_cast(float, (254u - up) << 23);
+    const uint32_t up = ce::lift_of(bits);  // (the logits of a row with an infinity are NaN)
+    const float by = ce::lift_by(up);
+    if (k0 == 0) scales[r] = ce::lower_by(up);
     _Float16* const out = to + r * 3 * wide;
     const auto store = [&](int k, const f32x4& v) {
       f16x4 high, low;
@@ -381,6 +380,7 @@ bool keeps_logits(const mhc_linear_ce_args& a) {
 
 struct BwdPlan {
   int64_t piece;   // columns of the vocabulary
+  bool parts;      // dx and dW are formed of fp16 parts
   bool joint;      // a piece's dx and dW go with the next one's dz
   Cut dz, dx, dw;  // dx.splits: parts of its reduction, each with sums of its own over all pieces
   HalvesPlan halves;
@@ -389,11 +389,31 @@ struct BwdPlan {
 
 BwdPlan plan_bwd(const mhc_linear_ce_args& a, bool dx, bool dw) {
   BwdPlan p = {};
-  const int64_t e = gemm::elem_bytes(a.dtype), pieces = std::max<int64_t>(1, ceil_div(a.T * a.V * e, kPieceBytes));
+  const bool in_parts = in_halves(a);
+  p.parts = in_parts && a.logits != nullptr;
+  const int64_t e = gemm::elem_bytes(a.dtype), of_dz = p.parts ? 8 : e, pieces = std::max<int64_t>(1, ceil_div(a.T * a.V * of_dz, kPieceBytes));
   p.piece = std::min(a.V, ceil_div(ceil_div(a.V, pieces), 256) * 256);
+  if (p.parts) {
+    p.piece = std::min(p.piece, halves_piece(a));
+    p.halves = plan_halves(a, p.piece);
+    p.dx = gemm::cut_of(a.T, a.C, 3 * p.piece, kF16, true, false);
+    p.dw = gemm::cut_of(p.piece, a.C, 3 * a.T, kF16, false, false);
+    // (a part of a reduction takes its k of all three products)
+    const auto third = [](Cut& c, int64_t K) {
+      const int kK = gemm::stage_k(kF16), deep = (int)ceil_div(K, kK), per = (int)ceil_div(deep, std::min(c.splits, deep));
+      c.splits = (int)ceil_div(deep, per), c.kper = per * kK;
+    };
+    third(p.dx, p.piece);
+    third(p.dw, a.T);
+    p.of_dz = up256((size_t)(a.T * padded(p.piece, kF16)) * 2);
+    if (dx) p.sums = up256((size_t)(p.dx.splits * a.T * a.C) * sizeof(float));
+    p.part = dw ? up256(gemm::part_bytes(p.dw, p.piece, a.C)) : 0;
+    p.total = 4 * p.of_dz + p.sums + p.halves.x + p.halves.w + p.part + (size_t)(a.T + p.piece) * sizeof(uint32_t);
+    return p;
+  }
   if (a.logits != nullptr) {
     p.dz = Cut{};
-  } else if (in_halves(a)) {
+  } else if (in_parts) {
     p.piece = std::min(p.piece, halves_piece(a));
     p.halves = plan_halves(a, p.piece);
     p.dz = gemm::cut_of(a.T, p.piece, 3 * p.halves.wide, kF16, true, true, 1);
@@ -424,6 +444,43 @@ BwdPlan plan_bwd(const mhc_linear_ce_args& a, bool dx, bool dw) {
   p.part = dw && !p.joint ? gemm::part_bytes(p.dw, p.piece, a.C) : 0;
   p.total = p.x + p.w + p.of_dz * (p.joint && p.piece < a.V ? 2 : 1) + p.sums + p.halves.x + p.halves.w + p.part;
   return p;
+}
+
+// The gradients from logits that were kept, all products of fp16 parts; sums: dx's, of every part of its reduction.
+int run_bwd_parts(const mhc_linear_ce_args& a, const BwdPlan& p, const State& st, const float* dloss, float grad_scale, bool dx, void* dw, char* ws,
+                  float*& sums, hipStream_t s) {
+  const auto next = [&ws](size_t bytes) { return ws += bytes, ws - bytes; };
+  const auto halves_of_dz = [&] { return reinterpret_cast<_Float16*>(next(p.of_dz)); };
+  ce::Parts parts = {halves_of_dz(), halves_of_dz(), halves_of_dz(), halves_of_dz(), nullptr, nullptr, 0};
+  sums = reinterpret_cast<float*>(next(p.sums));
+  char *const of_x = next(p.halves.x), *const of_w = next(p.halves.w);
+  float* const part = reinterpret_cast<float*>(next(p.part));
+  parts.row = reinterpret_cast<uint32_t*>(ws);
+  parts.col = parts.row + a.T;
+  const int64_t wide = p.halves.wide;
+  const ScaledBy by = {reinterpret_cast<const float*>(st.head) + 1, dloss, grad_scale};
+  const ce::Kept kept = {a.logits, ce::kept_pitch(a.V)};
+  ce::Halves halves;
+  if (const int rc = run_halves(false, a.x, a.ldx, of_x, &halves.x, &st, a.T, a.C, wide, s)) return rc;
+  for (int64_t v0 = 0; v0 < a.V; v0 += p.piece) {
+    const int64_t n = std::min(p.piece, a.V - v0);
+    if (const int rc = run_halves(true, static_cast<const float*>(a.w) + v0 * a.ldw, a.ldw, of_w, &halves.w, nullptr, n, a.C, wide, s)) return rc;
+    parts.pitch = padded(n, kF16);
+    const ce::Gradient g = {st.target, st.coef, st.top, st.inv, v0, 1.f};
+    if (const int rc = ce::run_parts(g, kept, halves, parts, a.T, n, st.head, s)) return rc;
+    const auto low = [](const char* rows, int64_t at) { return rows + at * 2; };  // (x: high, low, high; W: high, high, low)
+    if (dx) {
+      const Product q = {Operand{parts.x_high, parts.pitch, parts.pitch}, Operand{of_w, 3 * wide, wide}, a.T, a.C, n,
+                         Epilogue{nullptr, v0 > 0 ? sums : nullptr, sums, nullptr, MHC_ACT_NONE, 1}, p.dx.splits, p.dx.kper};
+      if (const int rc = ce::run_dx_halves(q, parts.x_low, low(of_w, 2 * wide), parts.row, p.dx, st.head, s)) return rc;
+    }
+    if (dw != nullptr) {
+      const Product q = {Operand{parts.w_high, parts.pitch, parts.pitch}, Operand{of_x, 3 * wide, wide}, n, a.C, a.T,
+                         Epilogue{nullptr, nullptr, static_cast<float*>(dw) + v0 * a.C, nullptr, MHC_ACT_NONE, 1}, 1, p.dw.kper};
+      if (const int rc = ce::run_dw_halves(q, parts.w_low, low(of_x, wide), parts.col, p.dw, st.head, by, part, s)) return rc;
+    }
+  }
+  return MHC_OK;
 }
 
 int run_gather(const mhc_linear_ce_args& a, const State& st, void* to, hipStream_t s) {
@@ -566,6 +623,11 @@ extern "C" int mhc_linear_ce_bwd(const mhc_linear_ce_args* args, const void* sta
   const State st(const_cast<void*>(state), a.T);
   const int64_t e = gemm::elem_bytes(a.dtype), wide = padded(a.C, a.dtype);
   char* ws = static_cast<char*>(workspace);
+  if (p.parts) {
+    float* sums;
+    const int rc = run_bwd_parts(a, p, st, dloss, grad_scale, dx != nullptr, dw, ws, sums, s);
+    return rc != MHC_OK || dx == nullptr ? rc : run_scatter<float>(a, sums, p.dx.splits, st, dloss, grad_scale, dx, s);
+  }
   const Operand x = {ws, wide, wide};
   if (const int rc = run_gather(a, st, ws, s)) return rc;
   ws += p.x;

@@ -47,6 +47,11 @@ template <> inline constexpr float kDzUnit<_Float16> = 0x1p14f;
 // 2^-40 of the row's largest).  Of the products of two values three parts are
 // formed (the fourth is below 2^-24): rows of [high, low, high] against rows of
 // [high, high, low], 3 C long, half of what linear_act's fp32 tiles do.
+//
+// dz's two products are formed so, too, from logits that were kept.  Their k are
+// tokens and columns, whose powers of two go to dz: dx's rows are sums of dz w[v]
+// over the parts of W, each row of dz w lifted as one of x is, dW's of dz x[t]
+// over the parts of x, each column lifted.
 struct Halves {
   const float *x, *w;  // of each row: what its parts are to be multiplied by
 
@@ -67,6 +72,25 @@ struct Halves {
         for (int k = 0; k < 4; ++k) acc[i][j][k] = acc[i][j][k] * row[j] * column[k];
     }
   }
+};
+
+// The power of two, as its exponent's bits, that brings a row of the largest
+// magnitude `top` to 2^14, if both are normal numbers (a row with an infinity or
+// NaN: 1), and its reciprocal.
+MHC_DEV uint32_t lift_of(uint32_t top) {
+  const uint32_t e = top >> 23;
+  return e == 255 ? 127 : min(268u - max(e, 15u), 253u);
+}
+MHC_DEV float lift_by(uint32_t up) { return __builtin_bit_cast(float, up << 23); }
+MHC_DEV float lower_by(uint32_t up) { return __builtin_bit_cast(float, (254u - up) << 23); }
+
+// dz of a piece of the vocabulary as fp16 parts, in rows of `pitch`, for each of
+// its products, and the largest magnitudes by which they are lifted, as bits.
+struct Parts {
+  _Float16 *x_high, *x_low;  // for dx
+  _Float16 *w_high, *w_low;  // for dW
+  uint32_t *row, *col;
+  int64_t pitch;
 };
 
 // The logits that a forward keeps: of each live token a row of `pitch`.
@@ -561,6 +585,11 @@ const Runs& runs_f16();
 // of rows of fp16 parts for fp32 logits
 int run_sums_halves(const Product& p, const Cut& c, const int* live, const SumsOf& of, const Halves& halves, hipStream_t s);
 int run_dz_halves(const Product& p, const Cut& c, const int* live, int64_t width, const Gradient& g, const Halves& halves, hipStream_t s);
+// of logits that were kept: dz's parts of `rows` tokens and N columns, and its products, whose operands are the high parts
+int run_parts(const Gradient& g, const Kept& kept, const Halves& halves, const Parts& parts, int64_t rows, int64_t N, const int* live, hipStream_t s);
+int run_dx_halves(const Product& p, const void* a_low, const void* b_low, const uint32_t* tops, const Cut& c, const int* live, hipStream_t s);
+int run_dw_halves(const Product& p, const void* a_low, const void* b_low, const uint32_t* tops, const Cut& c, const int* live, const ScaledBy& by,
+                  float* part, hipStream_t s);
 
 template <typename T>
 int run_dz(const Product& p, const Cut& c, const int* live, int64_t width, const Gradient& g, hipStream_t s) {
