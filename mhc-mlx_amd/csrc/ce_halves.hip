@@ -4,8 +4,15 @@
 namespace mhc {
 namespace ce {
 
+// The larger of two bit patterns.
+struct MoreOp {
+  MHC_DEV float operator()(float a, float b) const {
+    return __builtin_bit_cast(float, max(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)));
+  }
+};
+
 // dz from logits that were kept, 8 columns of a row a thread: what both kernels below do with it
-template <int ROWS, typename Use>
+template <bool FAST, int ROWS, typename Use>
 MHC_DEV void each_dz(const Gradient& g, const Kept& kept, int64_t N, int64_t rows, int64_t m0, int64_t n, Use use) {
   constexpr int kEach = 8, kAhead = 4;
   const float* const from = kept.z + g.v0 + n;
@@ -28,7 +35,7 @@ MHC_DEV void each_dz(const Gradient& g, const Kept& kept, int64_t N, int64_t row
       float d[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        d[k] = r[q].each * gemm::exp_of<false>(z[q][k / 4][k % 4] - r[q].t) - (mine == k ? r[q].c : 0.f);
+        d[k] = r[q].each * gemm::exp_of<FAST>(z[q][k / 4][k % 4] - r[q].t) - (mine == k ? r[q].c : 0.f);
         d[k] = n + k < N ? d[k] : 0.f;
       }
       use(m + q * kEach, d);
@@ -36,19 +43,16 @@ MHC_DEV void each_dz(const Gradient& g, const Kept& kept, int64_t N, int64_t row
   }
 }
 
-constexpr int kTopRows = 64;
-
-__global__ __launch_bounds__(256) void clear_kernel(uint32_t* p, int64_t n) {
-  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < n; at += (int64_t)gridDim.x * 256) p[at] = 0;
-}
-
-// The largest magnitude of each row of dz w[v], and of each column of dz x[t]
-// (as bits, of which NaN's are the largest; the order of atomic maxima does not
-// matter), of 64 rows and 256 columns a workgroup.
+// The largest magnitudes of a workgroup's part of each row of dz w[v], to
+// rows[row][part], and of each column of dz x[t], to cols[part][column].  (As
+// bits, of which NaN's are the largest; put together by a launch of their own:
+// atomic maxima of 128 workgroups at the same lines took twice the time.)  The
+// hardware's exponential does: what is lifted to 2^14 has a factor of four to
+// fp16's range.
 __global__ __launch_bounds__(256) void tops_kernel(const Gradient g, const Kept kept, const Halves halves, const Parts parts, int64_t N, const int* live) {
   __shared__ uint32_t lds[8][256];
-  const uint32_t wide = (uint32_t)ceil_div(N, 256);
-  const int64_t rows = *live, m0 = (int64_t)(blockIdx.x / wide) * kTopRows, n = (int64_t)(blockIdx.x % wide) * 256 + threadIdx.x % 32 * 8;
+  const uint32_t wide = (uint32_t)ceil_div(N, 256), part = blockIdx.x % wide;
+  const int64_t rows = *live, m0 = (int64_t)(blockIdx.x / wide) * Parts::kRows, n = (int64_t)part * 256 + threadIdx.x % 32 * 8;
   if (m0 >= rows) return;
   const auto bits = [](float v) { return __builtin_bit_cast(uint32_t, fabsf(v)); };
   float w[8];
@@ -56,7 +60,7 @@ __global__ __launch_bounds__(256) void tops_kernel(const Gradient g, const Kept 
   for (int k = 0; k < 8; ++k) w[k] = halves.w[min(n + k, N - 1)];
   uint32_t col[8] = {};
   const int64_t from = min(n, (N - 1) / 8 * 8);  // (threads past the last column read it once more, and count nothing)
-  each_dz<kTopRows>(g, kept, n < N ? N : 0, rows, m0, from, [&](int64_t m, const float(&d)[8]) {
+  each_dz<true, Parts::kRows>(g, kept, n < N ? N : 0, rows, m0, from, [&](int64_t m, const float(&d)[8]) {
     const float x = halves.x[m];
     uint32_t row = 0;
 #pragma unroll
@@ -64,9 +68,8 @@ __global__ __launch_bounds__(256) void tops_kernel(const Gradient g, const Kept 
       row = max(row, bits(d[k] * w[k]));
       col[k] = max(col[k], bits(d[k] * x));
     }
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) row = max(row, (uint32_t)__shfl_xor((int)row, s));
-    if (threadIdx.x % 32 == 0) atomicMax(parts.row + m, row);
+    row = __builtin_bit_cast(uint32_t, group_reduce<32>(__builtin_bit_cast(float, row), MoreOp{}));
+    if (threadIdx.x % 32 == 0) parts.rows[m * wide + part] = row;
   });
 #pragma unroll
   for (int k = 0; k < 8; ++k) lds[threadIdx.x / 32][threadIdx.x % 32 * 8 + k] = col[k];
@@ -74,8 +77,28 @@ __global__ __launch_bounds__(256) void tops_kernel(const Gradient g, const Kept 
   uint32_t top = 0;
 #pragma unroll
   for (int q = 0; q < 8; ++q) top = max(top, lds[q][threadIdx.x]);
-  const int64_t mine = (int64_t)(blockIdx.x % wide) * 256 + threadIdx.x;
-  if (mine < N) atomicMax(parts.col + mine, top);
+  const int64_t mine = (int64_t)part * 256 + threadIdx.x;
+  if (mine < N) parts.cols[m0 / Parts::kRows * N + mine] = top;
+}
+
+// the largest of each row's and each column's parts: a wave for a row, a thread for a column
+__global__ __launch_bounds__(256) void join_tops_kernel(const Parts parts, int64_t N, uint32_t of_rows, const int* live) {
+  const int64_t rows = *live;
+  if (blockIdx.x < of_rows) {
+    const int64_t m = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave, wide = ceil_div(N, 256);
+    if (m >= rows) return;
+    float top = 0.f;
+    for (int64_t k = threadIdx.x % kWave; k < wide; k += kWave) top = MoreOp{}(top, __builtin_bit_cast(float, parts.rows[m * wide + k]));
+    top = group_reduce<kWave>(top, MoreOp{});
+    if (threadIdx.x % kWave == 0) parts.row[m] = __builtin_bit_cast(uint32_t, top);
+  } else {
+    const int64_t n = (int64_t)(blockIdx.x - of_rows) * 256 + threadIdx.x, high = ceil_div(rows, Parts::kRows);
+    if (n >= N) return;
+    uint32_t top = 0;
+#pragma unroll 8
+    for (int64_t k = 0; k < high; ++k) top = max(top, parts.cols[k * N + n]);
+    parts.col[n] = top;
+  }
 }
 
 // a vector of parts: the nearest fp16 numbers, and those nearest to what is left
@@ -100,7 +123,7 @@ __global__ __launch_bounds__(256) void parts_kernel(const Gradient g, const Kept
     w[k] = halves.w[min(n + k, N - 1)];
     col[k] = lift_by(lift_of(parts.col[min(n + k, N - 1)]));
   }
-  each_dz<32>(g, kept, N, rows, m0, n, [&](int64_t m, const float(&d)[8]) {
+  each_dz<false, 32>(g, kept, N, rows, m0, n, [&](int64_t m, const float(&d)[8]) {
     const float x = halves.x[m], row = lift_by(lift_of(parts.row[m]));
     float v[8];
 #pragma unroll
@@ -113,11 +136,11 @@ __global__ __launch_bounds__(256) void parts_kernel(const Gradient g, const Kept
 }
 
 int run_parts(const Gradient& g, const Kept& kept, const Halves& halves, const Parts& parts, int64_t rows, int64_t N, const int* live, hipStream_t s) {
-  const int64_t tops = parts.col + N - parts.row;
-  hipLaunchKernelGGL(clear_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(tops, 256), 4096)), dim3(256), 0, s, parts.row, tops);
-  MHC_CHECK_LAUNCH("clear_kernel");
-  hipLaunchKernelGGL(tops_kernel, dim3((unsigned)(ceil_div(rows, kTopRows) * ceil_div(N, 256))), dim3(256), 0, s, g, kept, halves, parts, N, live);
+  hipLaunchKernelGGL(tops_kernel, dim3((unsigned)(ceil_div(rows, Parts::kRows) * ceil_div(N, 256))), dim3(256), 0, s, g, kept, halves, parts, N, live);
   MHC_CHECK_LAUNCH("tops_kernel");
+  const uint32_t of_rows = (uint32_t)ceil_div(rows, 4);
+  hipLaunchKernelGGL(join_tops_kernel, dim3(of_rows + (unsigned)ceil_div(N, 256)), dim3(256), 0, s, parts, N, of_rows, live);
+  MHC_CHECK_LAUNCH("join_tops_kernel");
   hipLaunchKernelGGL(parts_kernel, dim3((unsigned)(ceil_div(rows, 32) * ceil_div(parts.pitch, 256))), dim3(256), 0, s, g, kept, halves, parts, N, live);
   MHC_CHECK_LAUNCH("parts_kernel");
   return MHC_OK;

@@ -152,12 +152,14 @@ MHC_DEV f32x4 four_of(const float* row, int k, int C) {
   return v;
 }
 
-// Rows of fp32 as rows of fp16 parts (see ce::Halves): [high, low, high] or
-// (LAST_LOW) [high, high, low], each part in `wide` elements, zeros after the
-// last.  The live rows of x (index given), or all of `rows`.  A wave for each
+// Rows of fp32 as rows of fp16 parts (see ce::Halves) in an order: of x or W for
+// the logits, whose products of parts are one, or each part once; each in `wide`
+// elements, zeros after the last.  The live rows of x (index given), or all of `rows`.  A wave for each
 // row, of which it keeps HELD times 256 elements in registers and reads those
 // beyond again (32768 x 1024: 335 MB in 51 us, 6.5 TB/s).
-template <bool LAST_LOW, int HELD>
+enum Order { kOfX, kOfW, kOnce };  // [high, low, high], [high, high, low], [high, low]
+
+template <int ORDER, int HELD>
 __global__ __launch_bounds__(256) void ce_halves_kernel(const float* x, int64_t ld, _Float16* to, float* scales, const int* live, const int* index,
                                                         int64_t rows, int C, int wide) {
   constexpr int kStep = 4 * kWave;
@@ -182,7 +184,7 @@ __global__ __launch_bounds__(256) void ce_halves_kernel(const float* x, int64_t 
     const uint32_t up = ce::lift_of(bits);  // (the logits of a row with an infinity are NaN)
     const float by = ce::lift_by(up);
     if (k0 == 0) scales[r] = ce::lower_by(up);
-    _Float16* const out = to + r * 3 * wide;
+    _Float16* const out = to + r * (ORDER == kOnce ? 2 : 3) * wide;
     const auto store = [&](int k, const f32x4& v) {
       f16x4 high, low;
 #pragma unroll
@@ -191,8 +193,8 @@ __global__ __launch_bounds__(256) void ce_halves_kernel(const float* x, int64_t 
         low[j] = (_Float16)(v[j] * by - (float)high[j]);
       }
       *reinterpret_cast<f16x4*>(out + k) = high;  // (wide is a multiple of eight)
-      *reinterpret_cast<f16x4*>(out + wide + k) = LAST_LOW ? high : low;
-      *reinterpret_cast<f16x4*>(out + 2 * wide + k) = LAST_LOW ? low : high;
+      *reinterpret_cast<f16x4*>(out + wide + k) = ORDER == kOfW ? high : low;
+      if constexpr (ORDER != kOnce) *reinterpret_cast<f16x4*>(out + 2 * wide + k) = ORDER == kOfW ? low : high;
     };
 #pragma unroll
     for (int i = 0; i < HELD; ++i)
@@ -304,15 +306,15 @@ bool in_halves(const mhc_linear_ce_args& a) {
   return halves < gemm::cut_of(a.T, a.V, a.C, kF32, true, true, 1).us;
 }
 
-// What the parts of x's rows and of a piece's rows of W take.
+// What `count` parts of each of x's rows and of a piece's rows of W take.
 struct HalvesPlan {
   int64_t wide;  // elements of a part of a row
   size_t x, w;   // bytes, with the rows' scales
 };
 
-HalvesPlan plan_halves(const mhc_linear_ce_args& a, int64_t piece) {
+HalvesPlan plan_halves(const mhc_linear_ce_args& a, int64_t piece, int count) {
   const int64_t wide = padded(a.C, kF16);
-  const auto bytes = [&](int64_t rows) { return up256((size_t)(rows * 3 * wide) * 2) + up256((size_t)rows * 4); };
+  const auto bytes = [&](int64_t rows) { return up256((size_t)(rows * count * wide) * 2) + up256((size_t)rows * 4); };
   return {wide, bytes(a.T), bytes(piece)};
 }
 
@@ -332,7 +334,7 @@ FwdPlan plan_fwd(const mhc_linear_ce_args& a) {
   p.direct = p.few = false;
   if (in_halves(a)) {
     p.piece = halves_piece(a);
-    const HalvesPlan h = plan_halves(a, p.piece);
+    const HalvesPlan h = plan_halves(a, p.piece, 3);
     p.cut = gemm::cut_of(a.T, p.piece, 3 * h.wide, kF16, true, true, 1);
     p.x = h.x;
     p.w = h.w;
@@ -352,14 +354,16 @@ FwdPlan plan_fwd(const mhc_linear_ce_args& a) {
 }
 
 // the parts of rows to `to`, their scales after them
-int run_halves(bool last_low, const void* x, int64_t ld, char* to, const float** scales, const State* live, int64_t rows, int64_t C, int64_t wide,
+int run_halves(Order order, const void* x, int64_t ld, char* to, const float** scales, const State* live, int64_t rows, int64_t C, int64_t wide,
                hipStream_t s) {
-  float* const at = reinterpret_cast<float*>(to + up256((size_t)(rows * 3 * wide) * 2));
+  float* const at = reinterpret_cast<float*>(to + up256((size_t)(rows * (order == kOnce ? 2 : 3) * wide) * 2));
   *scales = at;
   const dim3 grid((unsigned)std::min<int64_t>(ceil_div(rows, 4), device_cu_count() * 16));
   const int *const count = live != nullptr ? live->head : nullptr, *const index = live != nullptr ? live->index : nullptr;
-  const auto kernel = last_low ? (C <= 1024 ? ce_halves_kernel<true, 4> : ce_halves_kernel<true, 16>)
-                               : (C <= 1024 ? ce_halves_kernel<false, 4> : ce_halves_kernel<false, 16>);
+  const auto held = [&](auto kernel4, auto kernel16) { return C <= 1024 ? kernel4 : kernel16; };
+  const auto kernel = order == kOfX   ? held(ce_halves_kernel<kOfX, 4>, ce_halves_kernel<kOfX, 16>)
+                      : order == kOfW ? held(ce_halves_kernel<kOfW, 4>, ce_halves_kernel<kOfW, 16>)
+                                      : held(ce_halves_kernel<kOnce, 4>, ce_halves_kernel<kOnce, 16>);
   hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, static_cast<const float*>(x), ld,
                      reinterpret_cast<_Float16*>(to), at, count, index, rows, (int)C, (int)wide);
   MHC_CHECK_LAUNCH("ce_halves_kernel");
@@ -395,7 +399,7 @@ BwdPlan plan_bwd(const mhc_linear_ce_args& a, bool dx, bool dw) {
   p.piece = std::min(a.V, ceil_div(ceil_div(a.V, pieces), 256) * 256);
   if (p.parts) {
     p.piece = std::min(p.piece, halves_piece(a));
-    p.halves = plan_halves(a, p.piece);
+    p.halves = plan_halves(a, p.piece, 2);
     p.dx = gemm::cut_of(a.T, a.C, 3 * p.piece, kF16, true, false);
     p.dw = gemm::cut_of(p.piece, a.C, 3 * a.T, kF16, false, false);
     // (a part of a reduction takes its k of all three products)
@@ -408,14 +412,14 @@ BwdPlan plan_bwd(const mhc_linear_ce_args& a, bool dx, bool dw) {
     p.of_dz = up256((size_t)(a.T * padded(p.piece, kF16)) * 2);
     if (dx) p.sums = up256((size_t)(p.dx.splits * a.T * a.C) * sizeof(float));
     p.part = dw ? up256(gemm::part_bytes(p.dw, p.piece, a.C)) : 0;
-    p.total = 4 * p.of_dz + p.sums + p.halves.x + p.halves.w + p.part + (size_t)(a.T + p.piece) * sizeof(uint32_t);
+    p.total = 4 * p.of_dz + p.sums + p.halves.x + p.halves.w + p.part + ce::Parts::top_words(a.T, p.piece) * sizeof(uint32_t);
     return p;
   }
   if (a.logits != nullptr) {
     p.dz = Cut{};
   } else if (in_parts) {
     p.piece = std::min(p.piece, halves_piece(a));
-    p.halves = plan_halves(a, p.piece);
+    p.halves = plan_halves(a, p.piece, 3);
     p.dz = gemm::cut_of(a.T, p.piece, 3 * p.halves.wide, kF16, true, true, 1);
   } else {
     p.dz = gemm::cut_of(a.T, p.piece, a.C, a.dtype, true, true, 1);
@@ -451,33 +455,34 @@ int run_bwd_parts(const mhc_linear_ce_args& a, const BwdPlan& p, const State& st
                   float*& sums, hipStream_t s) {
   const auto next = [&ws](size_t bytes) { return ws += bytes, ws - bytes; };
   const auto halves_of_dz = [&] { return reinterpret_cast<_Float16*>(next(p.of_dz)); };
-  ce::Parts parts = {halves_of_dz(), halves_of_dz(), halves_of_dz(), halves_of_dz(), nullptr, nullptr, 0};
+  ce::Parts parts = {halves_of_dz(), halves_of_dz(), halves_of_dz(), halves_of_dz(), nullptr, nullptr, nullptr, nullptr, 0};
   sums = reinterpret_cast<float*>(next(p.sums));
   char *const of_x = next(p.halves.x), *const of_w = next(p.halves.w);
   float* const part = reinterpret_cast<float*>(next(p.part));
   parts.row = reinterpret_cast<uint32_t*>(ws);
   parts.col = parts.row + a.T;
+  parts.rows = parts.col + p.piece;
+  parts.cols = parts.rows + a.T * ceil_div(p.piece, 256);
   const int64_t wide = p.halves.wide;
   const ScaledBy by = {reinterpret_cast<const float*>(st.head) + 1, dloss, grad_scale};
   const ce::Kept kept = {a.logits, ce::kept_pitch(a.V)};
   ce::Halves halves;
-  if (const int rc = run_halves(false, a.x, a.ldx, of_x, &halves.x, &st, a.T, a.C, wide, s)) return rc;
+  if (const int rc = run_halves(kOnce, a.x, a.ldx, of_x, &halves.x, &st, a.T, a.C, wide, s)) return rc;
   for (int64_t v0 = 0; v0 < a.V; v0 += p.piece) {
     const int64_t n = std::min(p.piece, a.V - v0);
-    if (const int rc = run_halves(true, static_cast<const float*>(a.w) + v0 * a.ldw, a.ldw, of_w, &halves.w, nullptr, n, a.C, wide, s)) return rc;
+    if (const int rc = run_halves(kOnce, static_cast<const float*>(a.w) + v0 * a.ldw, a.ldw, of_w, &halves.w, nullptr, n, a.C, wide, s)) return rc;
     parts.pitch = padded(n, kF16);
     const ce::Gradient g = {st.target, st.coef, st.top, st.inv, v0, 1.f};
     if (const int rc = ce::run_parts(g, kept, halves, parts, a.T, n, st.head, s)) return rc;
-    const auto low = [](const char* rows, int64_t at) { return rows + at * 2; };  // (x: high, low, high; W: high, high, low)
     if (dx) {
-      const Product q = {Operand{parts.x_high, parts.pitch, parts.pitch}, Operand{of_w, 3 * wide, wide}, a.T, a.C, n,
+      const Product q = {Operand{parts.x_high, parts.pitch, parts.pitch}, Operand{of_w, 2 * wide, wide}, a.T, a.C, n,
                          Epilogue{nullptr, v0 > 0 ? sums : nullptr, sums, nullptr, MHC_ACT_NONE, 1}, p.dx.splits, p.dx.kper};
-      if (const int rc = ce::run_dx_halves(q, parts.x_low, low(of_w, 2 * wide), parts.row, p.dx, st.head, s)) return rc;
+      if (const int rc = ce::run_dx_halves(q, parts.x_low, of_w + wide * 2, parts.row, p.dx, st.head, s)) return rc;
     }
     if (dw != nullptr) {
-      const Product q = {Operand{parts.w_high, parts.pitch, parts.pitch}, Operand{of_x, 3 * wide, wide}, n, a.C, a.T,
+      const Product q = {Operand{parts.w_high, parts.pitch, parts.pitch}, Operand{of_x, 2 * wide, wide}, n, a.C, a.T,
                          Epilogue{nullptr, nullptr, static_cast<float*>(dw) + v0 * a.C, nullptr, MHC_ACT_NONE, 1}, 1, p.dw.kper};
-      if (const int rc = ce::run_dw_halves(q, parts.w_low, low(of_x, wide), parts.col, p.dw, st.head, by, part, s)) return rc;
+      if (const int rc = ce::run_dw_halves(q, parts.w_low, of_x + wide * 2, parts.col, p.dw, st.head, by, part, s)) return rc;
     }
   }
   return MHC_OK;
@@ -571,10 +576,10 @@ extern "C" int mhc_linear_ce_fwd(const mhc_linear_ce_args* args, float* loss, fl
     if (in_halves(a)) {
       const int64_t wide = padded(a.C, kF16);
       ce::Halves halves;
-      if (const int rc = run_halves(false, a.x, a.ldx, x, &halves.x, &st, a.T, a.C, wide, s)) return rc;
+      if (const int rc = run_halves(kOfX, a.x, a.ldx, x, &halves.x, &st, a.T, a.C, wide, s)) return rc;
       for (of.v0 = 0; of.v0 < a.V; of.v0 += p.piece) {
         const int64_t n = std::min(p.piece, a.V - of.v0);
-        if (const int rc = run_halves(true, static_cast<const float*>(a.w) + of.v0 * a.ldw, a.ldw, w, &halves.w, nullptr, n, a.C, wide, s)) return rc;
+        if (const int rc = run_halves(kOfW, static_cast<const float*>(a.w) + of.v0 * a.ldw, a.ldw, w, &halves.w, nullptr, n, a.C, wide, s)) return rc;
         const Product q = {Operand{x, 3 * wide, 3 * wide}, Operand{w, 3 * wide, 3 * wide}, a.T, n, 3 * wide, {}, 1, 0};
         if (const int rc = ce::run_sums_halves(q, p.cut, st.head, of, halves, s)) return rc;
       }
@@ -640,7 +645,7 @@ extern "C" int mhc_linear_ce_bwd(const mhc_linear_ce_args* args, const void* sta
   ce::Halves halves = {};
   const ce::Kept kept = {a.logits, ce::kept_pitch(a.V)};
   if (kept.z == nullptr && in_halves(a)) {
-    if (const int rc = run_halves(false, a.x, a.ldx, of_halves, &halves.x, &st, a.T, a.C, p.halves.wide, s)) return rc;
+    if (const int rc = run_halves(kOfX, a.x, a.ldx, of_halves, &halves.x, &st, a.T, a.C, p.halves.wide, s)) return rc;
   }
   const float* const unit = reinterpret_cast<const float*>(st.head) + 1;
   const float lift = a.dtype == kF16 ? ce::kDzUnit<_Float16> : 1.f;
@@ -672,7 +677,7 @@ extern "C" int mhc_linear_ce_bwd(const mhc_linear_ce_args* args, const void* sta
     } else if (in_halves(a)) {
       const int64_t wide = 3 * p.halves.wide;
       char* const w_halves = of_halves + p.halves.x;
-      if (const int rc = run_halves(true, rows_of(v0).p, w.ld, w_halves, &halves.w, nullptr, columns(v0), a.C, p.halves.wide, s)) return rc;
+      if (const int rc = run_halves(kOfW, rows_of(v0).p, w.ld, w_halves, &halves.w, nullptr, columns(v0), a.C, p.halves.wide, s)) return rc;
       Product q = of_dz(v0, b);
       q.a = Operand{of_halves, wide, wide}, q.b = Operand{w_halves, wide, wide}, q.K = wide;
       if (const int rc = ce::run_dz_halves(q, p.dz, st.head, pitch(v0), gradient(v0), halves, s)) return rc;

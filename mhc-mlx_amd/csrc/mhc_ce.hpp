@@ -90,7 +90,11 @@ struct Parts {
   _Float16 *x_high, *x_low;  // for dx
   _Float16 *w_high, *w_low;  // for dW
   uint32_t *row, *col;
+  uint32_t *rows, *cols;     // of parts of each, see tops_kernel
   int64_t pitch;
+
+  static constexpr int kRows = 64;  // of a part of a column
+  static size_t top_words(int64_t T, int64_t N) { return T + N + T * ceil_div(N, 256) + ceil_div(T, kRows) * N; }
 };
 
 // The logits that a forward keeps: of each live token a row of `pitch`.
