@@ -373,9 +373,9 @@ int run_halves(Order order, const void* x, int64_t ld, char* to, const float** s
 // Whether the forward keeps the logits for the backward, which forms them again
 // else: from a width on at which their way through memory and back is shorter
 // than their product (4096 x 100000 bf16 kept and formed again, C = 512 2.20
-// and 2.04 ms, 1024 3.13 and 3.34, 2048 5.02 and 5.88; 6144 x 50257, 4096 6.9
-// and 8.3; 2000 x 32768 fp32, C = 64 0.449 and 0.433, 256 0.75 and 0.81, 2048
-// 3.69 and 4.43), and up to an amount that a card of 288 GB does not miss.
+// and 2.04 ms, 1024 3.13 and 3.34, 2048 5.02 and 5.88; 6144 x 50257, 4096 6.8
+// and 8.3; 2000 x 32768 fp32, C = 64 0.449 and 0.433, 256 0.71 and 0.83, 2048
+// 2.62 and 4.25), and up to an amount that a card of 288 GB does not miss.
 constexpr int64_t kKeepBytes = (int64_t)2 << 30;
 
 bool keeps_logits(const mhc_linear_ce_args& a) {
@@ -391,12 +391,32 @@ struct BwdPlan {
   size_t x, w, of_dz, sums, part, total;  // bytes; two of of_dz where joint
 };
 
+// columns of a piece whose dz takes kPieceBytes, at e bytes
+int64_t piece_of(const mhc_linear_ce_args& a, int64_t e) {
+  const int64_t pieces = std::max<int64_t>(1, ceil_div(a.T * a.V * e, kPieceBytes));
+  return std::min(a.V, ceil_div(ceil_div(a.V, pieces), 256) * 256);
+}
+
+// Whether dx and dW of fp32 operands are formed of fp16 parts, from logits that
+// were kept: where that is estimated shorter, with eight bytes more of each of
+// dz's elements and eight of each of W's, and three launches (the whole call in
+// parts and in fp32 tiles, C = 1024 and 32768 columns: 128 tokens 294 and 282 us,
+// 520 665 and 742, 1000 887 and 1080; 2000 x 32768 x 256 890 and 713; 500 x 500 x
+// 4096 169 and 155; 4096 x 100000 x 1024 9.9 and 11.8 ms).
+bool in_parts(const mhc_linear_ce_args& a) {
+  if (a.dtype != kF32 || a.logits == nullptr || 6 * padded(a.C, kF16) > gemm::kMaxRowBytes) return false;
+  const int64_t wide = padded(a.C, kF16), of_parts = std::min(piece_of(a, 8), halves_piece(a)), plain = piece_of(a, 4);
+  const float pieces = (float)ceil_div(a.V, of_parts);
+  const float parts = pieces * (20.f + gemm::cut_of(a.T, a.C, 3 * of_parts, kF16, true, false).us + gemm::cut_of(of_parts, a.C, 3 * a.T, kF16, false, false).us) +
+                      (float)(a.V * wide) * 8e-6f / 5.5f + (float)(a.T * a.V) * 8e-6f / 3.f;
+  return parts < (float)ceil_div(a.V, plain) * (gemm::cut_of(a.T, a.C, plain, kF32, true, false).us + gemm::cut_of(plain, a.C, a.T, kF32, false, false).us);
+}
+
 BwdPlan plan_bwd(const mhc_linear_ce_args& a, bool dx, bool dw) {
   BwdPlan p = {};
-  const bool in_parts = in_halves(a);
-  p.parts = in_parts && a.logits != nullptr;
-  const int64_t e = gemm::elem_bytes(a.dtype), of_dz = p.parts ? 8 : e, pieces = std::max<int64_t>(1, ceil_div(a.T * a.V * of_dz, kPieceBytes));
-  p.piece = std::min(a.V, ceil_div(ceil_div(a.V, pieces), 256) * 256);
+  const int64_t e = gemm::elem_bytes(a.dtype);
+  p.parts = in_parts(a);
+  p.piece = piece_of(a, p.parts ? 8 : e);
   if (p.parts) {
     p.piece = std::min(p.piece, halves_piece(a));
     p.halves = plan_halves(a, p.piece, 2);
@@ -417,7 +437,7 @@ BwdPlan plan_bwd(const mhc_linear_ce_args& a, bool dx, bool dw) {
   }
   if (a.logits != nullptr) {
     p.dz = Cut{};
-  } else if (in_parts) {
+  } else if (in_halves(a)) {
     p.piece = std::min(p.piece, halves_piece(a));
     p.halves = plan_halves(a, p.piece, 3);
     p.dz = gemm::cut_of(a.T, p.piece, 3 * p.halves.wide, kF16, true, true, 1);

@@ -92,7 +92,7 @@ def at_the_c_abi(x, w, y, mask, keep, scale=1.0):
 
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("T,V,C", [(1, 2, 8), (2, 65, 8), (17, 1000, 40), (64, 257, 64), (130, 515, 72), (300, 2050, 128), (700, 1003, 256), (1024, 4096, 256),
-                                   (2050, 3001, 512), (520, 20000, 64), (3000, 500, 1000), (5000, 30011, 40), (4500, 30011, 256)])
+                                   (2050, 3001, 512), (520, 20000, 64), (3000, 500, 1000), (5000, 30011, 40), (4500, 30011, 256), (700, 5003, 1030), (2500, 30011, 520), (300, 9000, 2051)])
 def test_logits_kept_and_formed_again(dt, T, V, C):
     x, w, y, g = inputs(T + V, T, V, C, dt)
     mask = (torch.rand(T, generator=g, device="cuda") < 0.8).to(torch.uint8)
@@ -105,7 +105,11 @@ def test_logits_kept_and_formed_again(dt, T, V, C):
 def test_gradients_of_huge_weights_over_several_pieces():
     """Weights around 2^112, whose sums in dx are formed a second time, are added to those of the pieces before."""
     x, w, y, _ = inputs(16, 5000, 30011, 256, torch.float32)
-    check(x * 2.0 ** -112, w * 2.0 ** 112, y)
+    x, w = x * 2.0 ** -112, w * 2.0 ** 112
+    check(x, w, y)
+    ref = ce64(x, w, y)
+    for k, v in at_the_c_abi(x, w, y, torch.ones(5000, dtype=torch.uint8, device="cuda"), False).items():
+        close(v, *ref[k], f"{k} of logits formed again")
 
 
 @pytest.mark.parametrize("dt", DTYPES)
