@@ -69,7 +69,7 @@ struct Halves {
 #pragma unroll
       for (int j = 0; j < JM; ++j)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) acc[i][j][k] = acc[i][j][k] * row[j] * column[k];
+        for (int k = 0; k < 4; ++k) acc[i][j][k] *= row[j] * column[k];  // (the sum times one of them may be past the range)
     }
   }
 };
@@ -419,24 +419,21 @@ struct SumsOf {
   Kept kept;
 };
 
-template <typename T, bool HALVES, int BM, int BN, int WM, int WN, int NS>
-MHC_DEV void sums_tile(const Product& p, const RowsOf& rows, const SumsOf& of, const Halves& halves, char* smem) {
-  constexpr int JM = BM / WM / 16, JN = BN / WN / 16, kThreads = 64 * WM * WN;
-  constexpr bool kFast = sizeof(T) == 2 && !HALVES;
-  const gemm::Place<BM, BN, WM, WN> at(p, blockIdx.x, 0);
-  f32x4 acc[JN][JM] = {};
-  if constexpr (gemm::kSplit<T, BN>) gemm::sum_tile_split<true, true, BM, BN, WM, WN, NS>(p, at, smem, acc, rows);
-  else gemm::sum_tile<T, true, true, BM, BN, WM, WN, NS>(p, at, smem, acc, rows);
-  if constexpr (HALVES) halves.scale(p, at, acc);
+// What becomes of a tile of logits; `rows`: a bit for each of the rows that it is for.
+template <bool FAST, int BM, int BN, int WM, int WN, int JM, int JN>
+MHC_DEV void store_sums(const Product& p, const gemm::Place<BM, BN, WM, WN>& at, const SumsOf& of, f32x4 (&acc)[JN][JM], const uint32_t* rows, char* smem) {
+  constexpr int kThreads = 64 * WM * WN;
   const int64_t m0 = at.m0 + at.wm + at.lane % 16, n0 = at.n0 + at.wn + at.lane / 16 * 4;
+  const auto is_for = [&](int r) { return rows == nullptr || (rows[r / 32] >> r % 32 & 1) != 0; };
   if (of.kept.z != nullptr) {
     float* const to = of.kept.z + of.v0 + n0;
 #pragma unroll
-    for (int j = 0; j < JM; ++j)
+    for (int j = 0; j < JM; ++j) {
+      if (m0 + j * 16 >= p.M || !is_for(at.wm + at.lane % 16 + j * 16)) continue;
 #pragma unroll
       for (int i = 0; i < JN; ++i)
-        if (m0 + j * 16 < p.M && of.v0 + n0 + i * 16 < of.kept.pitch)
-          *reinterpret_cast<f32x4*>(to + (m0 + j * 16) * of.kept.pitch + i * 16) = acc[i][j];
+        if (of.v0 + n0 + i * 16 < of.kept.pitch) *reinterpret_cast<f32x4*>(to + (m0 + j * 16) * of.kept.pitch + i * 16) = acc[i][j];
+    }
   }
   if (at.n0 + BN > p.N) {
 #pragma unroll
@@ -447,7 +444,6 @@ MHC_DEV void sums_tile(const Product& p, const RowsOf& rows, const SumsOf& of, c
         for (int k = 0; k < 4; ++k)
           if (n0 + i * 16 + k >= p.N) acc[i][j][k] = -__builtin_inff();
   }
-  __syncthreads();  // nobody reads the stages any more
   float2* const of_waves = reinterpret_cast<float2*>(smem);  // [columns of waves][BM]
 #pragma unroll
   for (int j = 0; j < JM; ++j) {
@@ -463,12 +459,12 @@ MHC_DEV void sums_tile(const Product& p, const RowsOf& rows, const SumsOf& of, c
 #pragma unroll
     for (int i = 0; i < JN; ++i)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) sum += gemm::exp_of<kFast>(acc[i][j][k] - base);
+      for (int k = 0; k < 4; ++k) sum += gemm::exp_of<FAST>(acc[i][j][k] - base);
     sum = xor_allreduce<16>(sum, SumOp{});
     sum = xor_allreduce<32>(sum, SumOp{});
     if (at.lane < 16) of_waves[at.wave % WN * BM + at.wm + j * 16 + at.lane] = float2{top, sum};
     const int64_t m = m0 + j * 16;
-    const int64_t mine = m < p.M ? of.target[m] - of.v0 - n0 : -1;
+    const int64_t mine = m < p.M && is_for(at.wm + at.lane % 16 + j * 16) ? of.target[m] - of.v0 - n0 : -1;
 #pragma unroll
     for (int i = 0; i < JN; ++i)
 #pragma unroll
@@ -478,15 +474,64 @@ MHC_DEV void sums_tile(const Product& p, const RowsOf& rows, const SumsOf& of, c
   __syncthreads();
   for (int r = threadIdx.x; r < BM; r += kThreads) {
     if (at.m0 + r >= p.M) break;
+    if (!is_for(r)) continue;
     float2 all = of_waves[r];
 #pragma unroll
     for (int w = 1; w < WN; ++w) {
       const float2 one = of_waves[w * BM + r];
       const float top = fmaxf(all.x, one.x), base = base_of(top);
-      all.y = all.y * gemm::exp_of<kFast>(all.x - base) + one.y * gemm::exp_of<kFast>(one.x - base);
+      all.y = all.y * gemm::exp_of<FAST>(all.x - base) + one.y * gemm::exp_of<FAST>(one.x - base);
       all.x = top;
     }
     of.part[(at.m0 + r) * of.tiles + (of.v0 + at.n0) / BN] = all;
+  }
+}
+
+// (fp32: the rows of a tile that have a sum past the range of parts are formed
+// once more with fp32 instructions, as run_tile does it for single sums)
+template <typename T, bool HALVES, int BM, int BN, int WM, int WN, int NS>
+MHC_DEV void sums_tile(const Product& p, const RowsOf& rows, const SumsOf& of, const Halves& halves, char* smem) {
+  constexpr int JM = BM / WM / 16, JN = BN / WN / 16;
+  constexpr bool kFast = sizeof(T) == 2 && !HALVES;
+  const gemm::Place<BM, BN, WM, WN> at(p, blockIdx.x, 0);
+  f32x4 acc[JN][JM] = {};
+  if constexpr (!gemm::kSplit<T, BN>) {
+    gemm::sum_tile<T, true, true, BM, BN, WM, WN, NS>(p, at, smem, acc, rows);
+    if constexpr (HALVES) halves.scale(p, at, acc);
+    __syncthreads();  // nobody reads the stages any more
+    store_sums<kFast>(p, at, of, acc, nullptr, smem);
+  } else {
+    __shared__ uint32_t past[BM / 32];
+    if (threadIdx.x < BM / 32) past[threadIdx.x] = 0;
+    gemm::sum_tile_split<true, true, BM, BN, WM, WN, NS>(p, at, smem, acc, rows);
+    const int n0 = (int)min(p.N - at.n0, (int64_t)BN) - at.wn - at.lane / 16 * 4;  // columns from the lane's first on
+#pragma unroll
+    for (int j = 0; j < JM; ++j) {
+      bool one = false;
+#pragma unroll
+      for (int i = 0; i < JN; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) one |= !(fabsf(acc[i][j][k]) < __builtin_inff()) && i * 16 + k < n0;
+      const int r = at.wm + j * 16 + at.lane % 16;
+      if (one && at.m0 + r < p.M) atomicOr(past + r / 32, 1u << r % 32);
+    }
+    __syncthreads();  // nobody reads the stages any more
+    uint32_t again = 0;
+#pragma unroll
+    for (int k = 0; k < BM / 32; ++k) again |= past[k];
+    again = __builtin_amdgcn_readfirstlane(again);
+    store_sums<kFast>(p, at, of, acc, nullptr, smem);
+    if (!again) return;
+#pragma unroll
+    for (int i = 0; i < JN; ++i)
+#pragma unroll
+      for (int j = 0; j < JM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    gemm::Place<BM, BN, WM, WN> once_more = at;
+    asm volatile("" : "+v"(once_more.lane), "+s"(once_more.wave));  // (or registers would hold places from the first sums to these)
+    __syncthreads();  // nobody reads the rows' numbers in LDS any more
+    gemm::sum_tile<T, true, true, BM, BN, WM, WN, NS>(p, once_more, smem, acc, rows);
+    __syncthreads();
+    store_sums<kFast>(p, once_more, of, acc, past, smem);
   }
 }
 

@@ -181,6 +181,14 @@ def test_fp32_rows_of_many_magnitudes(T, V, C):
     assert bool(loss.isnan()) and bool(logp[5].isnan()) and bool(logp[others].isfinite().all()) and bool(dx[others].isfinite().all())
 
 
+@pytest.mark.parametrize("T,V,C,by", [(40, 300, 64, 105), (1024, 4096, 256, 118), (1500, 4096, 1100, 118)])
+def test_fp32_operands_that_are_large_and_small(T, V, C, by):
+    """Logits of the usual size from rows around 2^by and weights around 2^-by, and the other way round."""
+    x, w, y, _ = inputs(18, T, V, C, torch.float32)
+    for up in (by, -by):
+        check(x * 2.0 ** up, w * 2.0 ** -up, y, what=f"{up}")
+
+
 def test_strides_and_shapes():
     x, w, y, g = inputs(8, 60, 90, 64, torch.bfloat16)
     want = linear_cross_entropy_and_grad(x, w, y)
