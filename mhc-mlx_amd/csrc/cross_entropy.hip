@@ -379,7 +379,7 @@ int run_halves(Order order, const void* x, int64_t ld, char* to, const float** s
 constexpr int64_t kKeepBytes = (int64_t)2 << 30;
 
 bool keeps_logits(const mhc_linear_ce_args& a) {
-  return a.C >= (a.dtype == kF32 ? 256 : 768) && a.T * ce::kept_pitch(a.V) * 4 <= kKeepBytes;
+  return (a.T <= ce::kFewTokens || a.C >= (a.dtype == kF32 ? 256 : 768)) && a.T * ce::kept_pitch(a.V) * 4 <= kKeepBytes;
 }
 
 struct BwdPlan {
@@ -412,9 +412,15 @@ bool in_parts(const mhc_linear_ce_args& a) {
   return parts < (float)ceil_div(a.V, plain) * (gemm::cut_of(a.T, a.C, plain, kF32, true, false).us + gemm::cut_of(plain, a.C, a.T, kF32, false, false).us);
 }
 
+bool few(const mhc_linear_ce_args& a) { return a.logits != nullptr && a.T <= ce::kFewTokens; }
+
 BwdPlan plan_bwd(const mhc_linear_ce_args& a, bool dx, bool dw) {
   BwdPlan p = {};
   const int64_t e = gemm::elem_bytes(a.dtype);
+  if (few(a)) {
+    p.total = ce::few_bytes(a);
+    return p;
+  }
   p.parts = in_parts(a);
   p.piece = piece_of(a, p.parts ? 8 : e);
   if (p.parts) {
@@ -648,6 +654,7 @@ extern "C" int mhc_linear_ce_bwd(const mhc_linear_ce_args* args, const void* sta
   const State st(const_cast<void*>(state), a.T);
   const int64_t e = gemm::elem_bytes(a.dtype), wide = padded(a.C, a.dtype);
   char* ws = static_cast<char*>(workspace);
+  if (few(a)) return ce::run_few(a, st, dloss, grad_scale, dx, dw, ws, s);
   if (p.parts) {
     float* sums;
     const int rc = run_bwd_parts(a, p, st, dloss, grad_scale, dx != nullptr, dw, ws, sums, s);

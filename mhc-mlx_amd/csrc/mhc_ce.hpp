@@ -488,22 +488,24 @@ MHC_DEV void store_sums(const Product& p, const gemm::Place<BM, BN, WM, WN>& at,
 }
 
 // (fp32: the rows of a tile that have a sum past the range of parts are formed
-// once more with fp32 instructions, as run_tile does it for single sums)
+// once more with fp32 instructions, as run_tile does it for single sums.  Tiles
+// for few tokens, which have few sums and time, set them aside every four
+// stages: of 12 tokens, C = 2285, log probabilities are XXX off.)
 template <typename T, bool HALVES, int BM, int BN, int WM, int WN, int NS>
 MHC_DEV void sums_tile(const Product& p, const RowsOf& rows, const SumsOf& of, const Halves& halves, char* smem) {
-  constexpr int JM = BM / WM / 16, JN = BN / WN / 16;
+  constexpr int JM = BM / WM / 16, JN = BN / WN / 16, kEvery = BM == 64 ? 4 : 0;
   constexpr bool kFast = sizeof(T) == 2 && !HALVES;
   const gemm::Place<BM, BN, WM, WN> at(p, blockIdx.x, 0);
   f32x4 acc[JN][JM] = {};
   if constexpr (!gemm::kSplit<T, BN>) {
-    gemm::sum_tile<T, true, true, BM, BN, WM, WN, NS>(p, at, smem, acc, rows);
+    gemm::sum_tile<T, true, true, BM, BN, WM, WN, NS, RowsOf, kEvery>(p, at, smem, acc, rows);
     if constexpr (HALVES) halves.scale(p, at, acc);
     __syncthreads();  // nobody reads the stages any more
     store_sums<kFast>(p, at, of, acc, nullptr, smem);
   } else {
     __shared__ uint32_t past[BM / 32];
     if (threadIdx.x < BM / 32) past[threadIdx.x] = 0;
-    gemm::sum_tile_split<true, true, BM, BN, WM, WN, NS>(p, at, smem, acc, rows);
+    gemm::sum_tile_split<true, true, BM, BN, WM, WN, NS, RowsOf, kEvery>(p, at, smem, acc, rows);
     const int n0 = (int)min(p.N - at.n0, (int64_t)BN) - at.wn - at.lane / 16 * 4;  // columns from the lane's first on
 #pragma unroll
     for (int j = 0; j < JM; ++j) {
@@ -529,7 +531,7 @@ MHC_DEV void sums_tile(const Product& p, const RowsOf& rows, const SumsOf& of, c
     gemm::Place<BM, BN, WM, WN> once_more = at;
     asm volatile("" : "+v"(once_more.lane), "+s"(once_more.wave));  // (or registers would hold places from the first sums to these)
     __syncthreads();  // nobody reads the rows' numbers in LDS any more
-    gemm::sum_tile<T, true, true, BM, BN, WM, WN, NS>(p, once_more, smem, acc, rows);
+    gemm::sum_tile<T, true, true, BM, BN, WM, WN, NS, RowsOf, kEvery>(p, once_more, smem, acc, rows);
     __syncthreads();
     store_sums<kFast>(p, once_more, of, acc, past, smem);
   }
@@ -630,6 +632,11 @@ struct Runs {
 const Runs& runs_f32();
 const Runs& runs_bf16();
 const Runs& runs_f16();
+
+// Up to kFewTokens tokens whose logits were kept: dx and dW by the vector unit.
+inline constexpr int kFewTokens = 16;
+size_t few_bytes(const mhc_linear_ce_args& a);
+int run_few(const mhc_linear_ce_args& a, const State& st, const float* dloss, float grad_scale, void* dx, void* dw, char* ws, hipStream_t s);
 
 // of rows of fp16 parts for fp32 logits
 int run_sums_halves(const Product& p, const Cut& c, const int* live, const SumsOf& of, const Halves& halves, hipStream_t s);

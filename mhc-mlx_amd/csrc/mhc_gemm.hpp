@@ -634,6 +634,32 @@ struct InOrder {
   }
 };
 
+// Sums set aside after every EVERY stages, which keeps long ones closer (0: never).
+template <int EVERY, int JM, int JN>
+struct Aside {
+  f32x4 all[JN][JM] = {};
+  int left = EVERY;
+  MHC_DEV void stage(f32x4 (&acc)[JN][JM]) {
+    if (--left > 0) return;
+    left = EVERY;
+#pragma unroll
+    for (int i = 0; i < JN; ++i)
+#pragma unroll
+      for (int j = 0; j < JM; ++j) all[i][j] += acc[i][j], acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  MHC_DEV void end(f32x4 (&acc)[JN][JM]) const {
+#pragma unroll
+    for (int i = 0; i < JN; ++i)
+#pragma unroll
+      for (int j = 0; j < JM; ++j) acc[i][j] += all[i][j];
+  }
+};
+template <int JM, int JN>
+struct Aside<0, JM, JN> {
+  MHC_DEV void stage(f32x4 (&)[JN][JM]) {}
+  MHC_DEV void end(f32x4 (&)[JN][JM]) const {}
+};
+
 // The sums of a workgroup's tile.  (The first operand's index, n, runs over a
 // lane's four values.)  Bound by the matrix instructions and, beside them, the
 // LDS reads of the fragments: a wave of a 256 x 256 tile reads 24 KB for 64
@@ -642,7 +668,7 @@ struct InOrder {
 // library's 178).  Smaller tiles read more for each product and serve where
 // large ones would leave CUs idle; their stages are as long as their chain of
 // wait, barrier, reads and products, which more stages under way don't shorten.
-template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS, typename Rows = InOrder>
+template <typename T, bool AK, bool BK, int BM, int BN, int WM, int WN, int NS, typename Rows = InOrder, int EVERY = 0>
 MHC_DEV void sum_tile(const Product& p, const Place<BM, BN, WM, WN>& at, char* smem, f32x4 (&acc)[BN / WN / 16][BM / WM / 16],
                       const Rows& rows = {}) {
   using S = Stage<T>;
@@ -684,6 +710,7 @@ MHC_DEV void sum_tile(const Product& p, const Place<BM, BN, WM, WN>& at, char* s
   clear_end(cur, kleft);
   Fragments<JM, JN> f0, f1;
   f0.read(ra, rb, smem, smem + kA, 0);
+  Aside<EVERY, JM, JN> aside;
   for (; kleft > 0; kleft -= S::kK) {
     f1.read(ra, rb, smem + cur, smem + cur + kA, 1);
     f0.template multiply<T>(acc);
@@ -699,7 +726,9 @@ MHC_DEV void sum_tile(const Product& p, const Place<BM, BN, WM, WN>& at, char* s
     f0.read(ra, rb, smem + cur, smem + cur + kA, 0);
     f1.template multiply<T>(acc);
     interleave<(JM * (AK ? 1 : S::kE / 4) + JN * (BK ? 1 : S::kE / 4)), JM * JN * (sizeof(T) == 4 ? 4 : 1)>();
+    aside.stage(acc);
   }
+  aside.end(acc);
   wait_loads<0>();  // (the last ones store zeros)
 }
 
@@ -742,7 +771,7 @@ MHC_DEV void split8(const u32x4& lo, const u32x4& hi, u32x4 (&part)[3]) {
 // 3/8 of the time of one in fp32; the splits, on the vector unit, go on beside
 // them in another wave (the lift is one of their 6.5 instructions for a value,
 // and 5 % of the time).
-template <bool AK, bool BK, int BM, int BN, int WM, int WN, int NS, typename Rows = InOrder>
+template <bool AK, bool BK, int BM, int BN, int WM, int WN, int NS, typename Rows = InOrder, int EVERY = 0>
 MHC_DEV void sum_tile_split(const Product& p, const Place<BM, BN, WM, WN>& at, char* smem, f32x4 (&acc)[BN / WN / 16][BM / WM / 16],
                             const Rows& rows = {}) {
   using S = Stage<float>;
@@ -768,6 +797,7 @@ MHC_DEV void sum_tile_split(const Product& p, const Place<BM, BN, WM, WN>& at, c
     lb.next();
   }
   int cur = 0, ahead = (NS - 1) * kStage;
+  Aside<EVERY, JM, JN> aside;
   for (; kleft > 0; kleft -= S::kK) {
     wait_loads<(NS - 2) * kLoads>();
     __syncthreads();  // this stage is there, and nobody reads the one before any more
@@ -798,7 +828,9 @@ MHC_DEV void sum_tile_split(const Product& p, const Place<BM, BN, WM, WN>& at, c
     }
     cur = cur == (NS - 1) * kStage ? 0 : cur + kStage;
     ahead = ahead == (NS - 1) * kStage ? 0 : ahead + kStage;
+    aside.stage(acc);
   }
+  aside.end(acc);
   wait_loads<0>();
 #pragma unroll
   for (int i = 0; i < JN; ++i)

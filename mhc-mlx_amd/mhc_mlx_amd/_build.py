@@ -27,7 +27,7 @@ SOURCES = ["capi.hip", "sinkhorn.hip", "fused_fwd.hip", "fused_bwd.hip", "stream
            "lf32_bwd_f32.hip", "lf32_bwd_bf16.hip", "lf32_bwd_f16.hip", "mxf32_f32.hip", "mxf32_bf16.hip", "mxf32_f16.hip",
            "lv_fwd_f32.hip", "lv_fwd_bf16.hip", "lv_fwd_f16.hip", "lv_bwd_f32.hip", "lv_bwd_bf16.hip", "lv_bwd_f16.hip",
            "noalloc.hip", "adamw.hip", "policy.hip", "linear.hip", "linear_f32.hip", "linear_bf16.hip", "linear_f16.hip", "norm.hip", "linear_int8.hip",
-           "cross_entropy.hip", "ce_f32.hip", "ce_bf16.hip", "ce_f16.hip", "ce_halves.hip"]
+           "cross_entropy.hip", "ce_f32.hip", "ce_bf16.hip", "ce_f16.hip", "ce_halves.hip", "ce_few.hip"]
 
 EXT_SOURCES = ["torch_ext.cpp", "torch_train.cpp", "torch_block.cpp"]
 

@@ -67,6 +67,30 @@ def test_vocabularies_of_several_pieces(dt):
     check(x, w, y, torch.rand(5000, generator=g, device="cuda") < 0.9)
 
 
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("T", [1, 2, 3, 5, 8, 9, 16])
+def test_few_tokens(dt, T):
+    """dx and dW in one pass over W: widths off every vector's length, rows that start anywhere, one column of the vocabulary."""
+    for V, C in ((1000, 2285), (5003, 300), (40, 4100), (1, 33), (33, 1), (70001, 24)):
+        x, w, y, g = inputs(T + C, T, V, C, dt)
+        mask = torch.rand(T, generator=g, device="cuda") < 0.7
+        check(x, w, y, scale=64.0, what=f"{V} {C}")
+        got = check(x, w, y, mask, what=f"{V} {C} mask")
+        # what lies between rows and behind them is not looked at
+        wide = torch.full((V + 1, C + 5), float("nan"), device="cuda", dtype=dt)
+        wv, xv = wide[:V, 3:C + 3].copy_(w), torch.full((T, C + 7), float("nan"), device="cuda", dtype=dt)[:, 1:C + 1].copy_(x)
+        assert all(torch.equal(a, b) for a, b in zip(linear_cross_entropy_and_grad(xv, wv, y, mask), got.values()))
+        xs, ws = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        assert torch.equal(torch.autograd.grad(linear_cross_entropy(xs, w, y, mask)[0], xs)[0], got["dx"])
+        assert torch.equal(torch.autograd.grad(linear_cross_entropy(x, ws, y, mask)[0], ws)[0], got["dw"])
+        none = check(x, w, y, torch.zeros(T, device="cuda"), what="no token")
+        assert not none["dx"].any() and not none["dw"].any()
+    y2 = y.clone()
+    y2[0] = V
+    loss, logp, dx, dw = linear_cross_entropy_and_grad(x, w, y2)
+    assert bool(loss.isnan()) and bool(dx[0].isnan().all()) and bool(dx[1:].isfinite().all()) and bool(dw.isnan().all())
+
+
 def at_the_c_abi(x, w, y, mask, keep, scale=1.0):
     """The two calls with the logits kept between them or formed again, whatever the sizes."""
     lib, byref, T, V = _lib.load(), ctypes.byref, len(x), len(w)
