@@ -4,8 +4,9 @@
 //
 // One pass over W and dW by the vector unit, with dz in fp32 (rounded to 16
 // bits, the few elements at the targets would be most of dW's error).  A wave
-// has 4 or 8 columns a lane: x's values there and dx's sums in registers, dz from
-// scalar loads, a row of W and of dW at a time.  Bound by memory (XXX).
+// has four columns a lane: x's values there and dx's sums in registers, dz from
+// scalar loads, a row of W and of dW at a time.  Bound by memory (2 x 72999 x 2624
+// fp32: 1.53 GB in 289 us, 5.3 TB/s; 4 x 32000 x 4096 bf16 524 MB in 135, 3.9).
 #include "mhc_ce.hpp"
 #include "mhc_plan.hpp"
 
@@ -13,9 +14,9 @@ namespace mhc {
 namespace ce {
 namespace {
 
-constexpr int kWaves = 8, kAhead = 4;  // of a workgroup, which shares its columns; rows of a wave under way
+constexpr int kWaves = 4, kVec = 4;  // of a workgroup, which shares its columns; columns of a lane
 
-template <typename T, int TP> constexpr int kVec = sizeof(T) == 4 || TP > 8 ? 4 : 8;
+template <int TP> constexpr int kAhead = TP > 8 ? 4 : 8;  // rows of a wave under way
 
 struct Few {
   const void *x, *w;
@@ -46,9 +47,24 @@ __global__ __launch_bounds__(256) void few_dz_kernel(const Gradient g, const Kep
   for (int t = 0; t < TP; ++t) dz[v * TP + t] = d[t];
 }
 
+// four elements, past the caches: dW is not read soon (2 x 72999 x 2624 fp32 327 us, through the caches 390)
+template <typename T>
+MHC_DEV void store_past(T* p, const float (&v)[kVec]) {
+  typedef uint32_t words __attribute__((ext_vector_type(sizeof(T)), aligned(sizeof(T))));
+  words w;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) w[k] = __builtin_bit_cast(uint32_t, v[k]);
+  } else {
+    w[0] = pack2<T>(v[0], v[1]);
+    w[1] = pack2<T>(v[2], v[3]);
+  }
+  __builtin_nontemporal_store(w, reinterpret_cast<words*>(p));
+}
+
 template <typename T, int TP>
 __global__ __launch_bounds__(64 * kWaves) void few_kernel(const Few a, const int* live, const int* index) {
-  constexpr int V = kVec<T, TP>;
+  constexpr int V = kVec, A = kAhead<TP>;
   __shared__ float lds[kWaves - 1][kWave * V];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c = (blockIdx.x * kWave + lane) * V, left = min(V, a.C - c);
@@ -76,31 +92,32 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(const Few a, const int
   // rows of the workgroup, its waves one after the other
   const int64_t v0 = a.V * blockIdx.y / gridDim.y, v1 = a.V * (blockIdx.y + 1) / gridDim.y;
   const auto* const dz = (const __attribute__((address_space(4))) float*)(uintptr_t)a.dz;
-  for (int64_t v = v0 + wave; v < v1; v += kWaves * kAhead) {
-    float w[kAhead][V] = {};
-    if (a.part != nullptr) {
+  for (int64_t v = v0 + wave; v < v1; v += kWaves * A) {
+    float w[A][V] = {}, d[A][TP];
 #pragma unroll
-      for (int q = 0; q < kAhead; ++q) take(static_cast<const T*>(a.w) + min(v + q * kWaves, v1 - 1) * a.ldw + c, w[q]);
+    for (int q = 0; q < A; ++q) {  // (rows past the last one read it once more)
+      const int64_t row = min(v + q * kWaves, v1 - 1);
+      if (a.part != nullptr) take(static_cast<const T*>(a.w) + row * a.ldw + c, w[q]);
+#pragma unroll
+      for (int t = 0; t < TP; ++t) d[q][t] = dz[row * TP + t];
     }
 #pragma unroll
-    for (int q = 0; q < kAhead; ++q) {
+    for (int q = 0; q < A; ++q) {
       const int64_t row = v + q * kWaves;
       if (row >= v1) break;
-      float out[V] = {}, d[TP];
-#pragma unroll
-      for (int t = 0; t < TP; ++t) d[t] = dz[row * TP + t];
+      float out[V] = {};
 #pragma unroll
       for (int t = 0; t < TP; ++t)
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          sum[t][k] = fmaf(d[t], w[q][k], sum[t][k]);
-          out[k] = fmaf(d[t], x[t][k], out[k]);
+          sum[t][k] = fmaf(d[q][t], w[q][k], sum[t][k]);
+          out[k] = fmaf(d[q][t], x[t][k], out[k]);
         }
       if (a.dw != nullptr) {
 #pragma unroll
         for (int k = 0; k < V; ++k) out[k] *= scale;
         T* const to = static_cast<T*>(a.dw) + row * a.C + c;
-        if (left == V) gemm::put<true>(to, out, V);
+        if (left == V) store_past(to, out);
         else if (left > 0) gemm::put<false>(to, out, left);
       }
     }
@@ -120,9 +137,7 @@ __global__ __launch_bounds__(64 * kWaves) void few_kernel(const Few a, const int
 #pragma unroll
       for (int k = 0; k < V; ++k) sum[t][k] += lds[q][k * kWave + lane];
     float* const to = a.part + ((int64_t)blockIdx.y * TP + t) * a.pitch + c;
-#pragma unroll
-    for (int k = 0; k < V; k += 4)
-      if (c + k < a.pitch) *reinterpret_cast<f32x4*>(to + k) = f32x4{sum[t][k], sum[t][k + 1], sum[t][k + 2], sum[t][k + 3]};
+    if (c < a.pitch) *reinterpret_cast<f32x4*>(to) = f32x4{sum[t][0], sum[t][1], sum[t][2], sum[t][3]};
   }
 }
 
@@ -154,11 +169,10 @@ struct Grid {
   int64_t columns, parts, pitch;
 };
 
-// Some 1024 workgroups, each with 32 rows at least.
+// Some 2048 workgroups, each with 64 rows at least.
 Grid grid_of(const mhc_linear_ce_args& a) {
-  const int tp = padded_tokens(a.T), vec = a.dtype == kF32 || tp > 8 ? 4 : 8;
-  const int64_t columns = ceil_div(a.C, kWave * vec);
-  return {columns, std::max<int64_t>(1, std::min(ceil_div(a.V, kWaves * kAhead), (int64_t)device_cu_count() * 4 / columns)), ceil_div(a.C, 4) * 4};
+  const int64_t columns = ceil_div(a.C, kWave * kVec);
+  return {columns, std::max<int64_t>(1, std::min(ceil_div(a.V, 64), (int64_t)device_cu_count() * 8 / columns)), ceil_div(a.C, 4) * 4};
 }
 
 template <typename T, int TP>

@@ -205,23 +205,41 @@ __global__ __launch_bounds__(256) void ce_halves_kernel(const float* x, int64_t 
 
 // A row's parts to its sums, and its log probability, put together in fp64
 // (log sum = e log 2 + log m with m around 1: the fp32 part stays below 0.35):
-// a wave for each row.  (The weights become those over the largest one here.)
-__global__ __launch_bounds__(256) void ce_rows_kernel(const State s, const float2* part, const float* at_target, int64_t tiles, float* logp,
-                                                      double* terms) {
-  const int lane = threadIdx.x % kWave;
+// WAVES for each row, more for a few rows of many parts.  (The weights become those over the largest one here.)
+template <int WAVES>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * kWave) void ce_rows_kernel(const State s, const float2* part, const float* at_target, int64_t tiles,
+                                                                                 float* logp, double* terms) {
+  constexpr int kRows = WAVES == 1 ? 4 : 1, kThreads = WAVES * kWave;  // of a workgroup, and of a row
+  __shared__ float lds[2][WAVES];
+  const int at = threadIdx.x % kThreads, wave = at / kWave;
   const int64_t rows = *s.head;
-  for (int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave; r < rows; r += (int64_t)gridDim.x * 4) {
+  for (int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / kThreads; r < rows; r += (int64_t)gridDim.x * kRows) {
     float top = -__builtin_inff();
-    for (int64_t k = lane; k < tiles; k += kWave) top = fmaxf(top, part[r * tiles + k].x);
+#pragma unroll 4
+    for (int64_t k = at; k < tiles; k += kThreads) top = fmaxf(top, part[r * tiles + k].x);
     top = group_max<kWave>(top);
+    if constexpr (WAVES > 1) {
+      lds[0][wave] = top;
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v < WAVES; ++v) top = fmaxf(top, lds[0][v]);
+    }
     const float base = ce::base_of(top);
     float sum = 0.f;
-    for (int64_t k = lane; k < tiles; k += kWave) {
+#pragma unroll 4
+    for (int64_t k = at; k < tiles; k += kThreads) {
       const float2 one = part[r * tiles + k];
       sum += one.y * expf(one.x - base);
     }
     sum = wave_sum(sum);
-    if (lane != 0) continue;
+    if constexpr (WAVES > 1) {
+      lds[1][wave] = sum;
+      __syncthreads();
+      sum = 0.f;
+#pragma unroll
+      for (int v = 0; v < WAVES; ++v) sum += lds[1][v];
+    }
+    if (at != 0) continue;
     const float z = s.target[r] < 0 ? __builtin_nanf("") : at_target[r];
     int e;
     float m = frexpf(sum, &e);
@@ -298,7 +316,7 @@ int64_t halves_piece(const mhc_linear_ce_args& a) {
 // estimated shorter than fp32 products (512 x 32768 x 1024 165 and 176 us, 4096 x
 // 8000 x 2048 387 and 696; but 256 x 32768 x 1024 149 and 111).
 bool in_halves(const mhc_linear_ce_args& a) {
-  if (a.dtype != kF32) return false;
+  if (a.dtype != kF32 || a.T <= ce::kFewRows) return false;
   const int64_t piece = halves_piece(a), wide = padded(a.C, kF16);
   if (6 * wide > gemm::kMaxRowBytes) return false;
   const float pieces = (float)ceil_div(a.V, piece);
@@ -324,6 +342,7 @@ struct FwdPlan {
   int64_t piece;  // columns of the vocabulary at a time
   bool direct;    // the live rows of x are read where they lie
   bool few;       // and found by the products' launch
+  bool rows;      // which is that for up to kFewRows tokens
   size_t x, w, part, at_target, total;  // bytes; terms come last
 };
 
@@ -332,7 +351,13 @@ FwdPlan plan_fwd(const mhc_linear_ce_args& a) {
   FwdPlan p;
   const int e = gemm::elem_bytes(a.dtype);
   p.direct = p.few = false;
-  if (in_halves(a)) {
+  p.rows = a.T <= ce::kFewRows;
+  if (p.rows) {
+    p.few = true;
+    p.piece = a.V;
+    p.x = gemm::pack_bytes(a.x, a.T, a.ldx, a.C, a.dtype);
+    p.w = gemm::pack_bytes(a.w, a.V, a.ldw, a.C, a.dtype);
+  } else if (in_halves(a)) {
     p.piece = halves_piece(a);
     const HalvesPlan h = plan_halves(a, p.piece, 3);
     p.cut = gemm::cut_of(a.T, p.piece, 3 * h.wide, kF16, true, true, 1);
@@ -346,7 +371,7 @@ FwdPlan plan_fwd(const mhc_linear_ce_args& a) {
     p.x = p.direct ? 0 : up256((size_t)(a.T * padded(a.C, a.dtype)) * e);
     p.w = gemm::pack_bytes(a.w, a.V, a.ldw, a.C, a.dtype);
   }
-  p.tiles = ceil_div(a.V, kBn[p.cut.tile]);  // (pieces are whole tiles, but for the last)
+  p.tiles = ceil_div(a.V, p.rows ? ce::kRowsColumns : kBn[p.cut.tile]);  // (pieces are whole tiles, but for the last)
   p.part = up256((size_t)(a.T * p.tiles) * sizeof(float2));
   p.at_target = up256((size_t)a.T * sizeof(float));
   p.total = p.x + p.w + p.part + p.at_target + (size_t)a.T * sizeof(double);
@@ -379,7 +404,7 @@ int run_halves(Order order, const void* x, int64_t ld, char* to, const float** s
 constexpr int64_t kKeepBytes = (int64_t)2 << 30;
 
 bool keeps_logits(const mhc_linear_ce_args& a) {
-  return (a.T <= ce::kFewTokens || a.C >= (a.dtype == kF32 ? 256 : 768)) && a.T * ce::kept_pitch(a.V) * 4 <= kKeepBytes;
+  return (a.T <= ce::few_tokens(a.dtype) || a.C >= (a.dtype == kF32 ? 256 : 768)) && a.T * ce::kept_pitch(a.V) * 4 <= kKeepBytes;
 }
 
 struct BwdPlan {
@@ -412,7 +437,7 @@ bool in_parts(const mhc_linear_ce_args& a) {
   return parts < (float)ceil_div(a.V, plain) * (gemm::cut_of(a.T, a.C, plain, kF32, true, false).us + gemm::cut_of(plain, a.C, a.T, kF32, false, false).us);
 }
 
-bool few(const mhc_linear_ce_args& a) { return a.logits != nullptr && a.T <= ce::kFewTokens; }
+bool few(const mhc_linear_ce_args& a) { return a.logits != nullptr && a.T <= ce::few_tokens(a.dtype); }
 
 BwdPlan plan_bwd(const mhc_linear_ce_args& a, bool dx, bool dw) {
   BwdPlan p = {};
@@ -611,7 +636,10 @@ extern "C" int mhc_linear_ce_fwd(const mhc_linear_ce_args* args, float* loss, fl
       }
     } else {
       Product q = {Operand{a.x, a.ldx, a.C}, {}, a.T, a.V, a.C, {}, 1, 0};
-      if (!p.direct) {
+      if (p.rows) {
+        char* to = x;
+        if (const int rc = gemm::operand(q.a, a.x, a.T, a.ldx, a.C, a.dtype, to, s)) return rc;
+      } else if (!p.direct) {
         if (const int rc = run_gather(a, st, x, s)) return rc;
         const int64_t wide = padded(a.C, a.dtype);
         q.a = Operand{x, wide, wide};
@@ -619,12 +647,17 @@ extern "C" int mhc_linear_ce_fwd(const mhc_linear_ce_args* args, float* loss, fl
       ws = w;
       if (const int rc = gemm::operand(q.b, a.w, a.V, a.ldw, a.C, a.dtype, ws, s)) return rc;
       const ce::Runs& run = runs_of(a.dtype);
-      const int rc = p.few ? run.sums_few(q, p.cut, of, ce::FewTokens{a, st, logp}, s)
-                           : run.sums(q, ce::RowsOf{p.direct ? st.index : nullptr, a.T}, p.cut, st.head, of, {}, s);
+      const int rc = p.rows  ? run.sums_rows(q, of, ce::FewTokens{a, st, logp}, s)
+                     : p.few ? run.sums_few(q, p.cut, of, ce::FewTokens{a, st, logp}, s)
+                             : run.sums(q, ce::RowsOf{p.direct ? st.index : nullptr, a.T}, p.cut, st.head, of, {}, s);
       if (rc != MHC_OK) return rc;
     }
-    hipLaunchKernelGGL(ce_rows_kernel, dim3((unsigned)std::min<int64_t>(ceil_div(a.T, 4), 1 << 20)), dim3(256), 0, s, st, (const float2*)part,
-                       (const float*)at_target, p.tiles, logp, terms);
+    if (p.rows)
+      hipLaunchKernelGGL((ce_rows_kernel<16>), dim3((unsigned)a.T), dim3(16 * kWave), 0, s, st, (const float2*)part, (const float*)at_target, p.tiles, logp,
+                         terms);
+    else
+      hipLaunchKernelGGL((ce_rows_kernel<1>), dim3((unsigned)std::min<int64_t>(ceil_div(a.T, 4), 1 << 20)), dim3(256), 0, s, st, (const float2*)part,
+                         (const float*)at_target, p.tiles, logp, terms);
     MHC_CHECK_LAUNCH("ce_rows_kernel");
   }
   if (a.T <= kFew) hipLaunchKernelGGL((ce_loss_kernel<kFew>), dim3(1), dim3(kFew), 0, s, st, (const double*)terms, loss);

@@ -490,7 +490,8 @@ MHC_DEV void store_sums(const Product& p, const gemm::Place<BM, BN, WM, WN>& at,
 // (fp32: the rows of a tile that have a sum past the range of parts are formed
 // once more with fp32 instructions, as run_tile does it for single sums.  Tiles
 // for few tokens, which have few sums and time, set them aside every four
-// stages: of 12 tokens, C = 2285, log probabilities are XXX off.)
+// stages: of 40 tokens, C = 2285, fp32 log probabilities are 5e-8 off, without
+// 3.4e-7.)
 template <typename T, bool HALVES, int BM, int BN, int WM, int WN, int NS>
 MHC_DEV void sums_tile(const Product& p, const RowsOf& rows, const SumsOf& of, const Halves& halves, char* smem) {
   constexpr int JM = BM / WM / 16, JN = BN / WN / 16, kEvery = BM == 64 ? 4 : 0;
@@ -553,6 +554,52 @@ __global__ __launch_bounds__(64 * WM * WN) void sums_few_kernel(Product p, SumsO
   __syncthreads();
   of.target = target;
   sums_tile<T, false, 64, BN, WM, WN, NS>(p, RowsOf{index, rows}, of, {}, smem);
+}
+
+inline constexpr int kFewRows = 16, kRowsColumns = 32;
+
+// Up to 16 tokens: 32 columns a workgroup, whose waves split k as few_rows_kernel's
+// do, so that a small vocabulary's products take no longer than their loads, and
+// 16 rows are multiplied instead of 64 (fp32 12 x 9376 x 2285 62 to 29 us, 2 x 72999
+// x 2624 288 to 147; bf16 2 x 4524 x 2240 22 to 13, 2 x 128000 x 2048 114 to 106,
+// but 4 x 32000 x 4096, whose 1000 workgroups are a little more than there is room
+// for at once, 47 to 62).  All tokens' logits are formed, and
+// those of the live ones looked at, 32 threads for each.
+template <typename T, int NS>
+__global__ __launch_bounds__(64 * gemm::kFewWaves) void sums_rows_kernel(const Product p, const SumsOf of, const FewTokens few) {
+  constexpr int NT = kRowsColumns / 16, kN = kRowsColumns, kSums = gemm::kFewWaves * kFewRows * kN * 4;
+  __shared__ __attribute__((aligned(1024))) char smem[std::max(gemm::kFewBytes<1, NT, NS>, kSums)];
+  __shared__ int index[64], target[64];
+  const int count = __builtin_amdgcn_readfirstlane(few.live(index, target));
+  if (count == 0) return;
+  const int64_t n0 = (int64_t)blockIdx.x * kN;
+  f32x4 acc[NT][1] = {};
+  gemm::sum_few_rows<T, 1, NT, NS>(p.a, p.b, (int)p.M, n0, p.N, (int)p.K, smem, acc);
+  float* const sums = reinterpret_cast<float*>(smem);  // [waves][rows][columns]
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int i = 0; i < NT; ++i) *reinterpret_cast<f32x4*>(sums + (wave * kFewRows + lane % 16) * kN + i * 16 + lane / 16 * 4) = acc[i][0];
+  __syncthreads();
+  const int place = threadIdx.x / kN, col = threadIdx.x % kN;
+  const bool mine = place < count;
+  const int64_t n = n0 + col;
+  const float* const from = sums + index[mine ? place : 0] * kN + col;
+  float z = 0.f;
+#pragma unroll
+  for (int v = 0; v < gemm::kFewWaves; ++v) z += from[v * kFewRows * kN];
+  if (mine && of.kept.z != nullptr && n < of.kept.pitch) of.kept.z[place * of.kept.pitch + n] = z;
+  if (mine && n == target[place]) of.at_target[place] = z;
+  if (n >= p.N) z = -__builtin_inff();
+  const float top = group_max<32>(z), sum = group_sum<32>(gemm::exp_of<sizeof(T) == 2>(z - base_of(top)));
+  if (mine && col == 0) of.part[place * of.tiles + blockIdx.x] = float2{top, sum};
+}
+
+template <typename T>
+int run_sums_rows(const Product& p, const SumsOf& of, const FewTokens& few, hipStream_t s) {
+  static_assert(kFewRows * kRowsColumns == 64 * gemm::kFewWaves, "a thread for each sum");
+  hipLaunchKernelGGL((sums_rows_kernel<T, 1>), dim3((unsigned)ceil_div(p.N, kRowsColumns)), dim3(64 * gemm::kFewWaves), 0, s, p, of, few);
+  MHC_CHECK_LAUNCH("sums_rows_kernel");
+  return MHC_OK;
 }
 
 template <typename T, bool HALVES, int BM, int BN, int WM, int WN, int NS>
@@ -622,6 +669,7 @@ int run_live(Product p, const Cut& c, const int* live, int64_t width, const Then
 // The launches of one type, each compiled in a file of its own.
 struct Runs {
   int (*sums)(Product p, const RowsOf& rows, const Cut& c, const int* live, const SumsOf& of, const Halves& halves, hipStream_t s);
+  int (*sums_rows)(const Product& p, const SumsOf& of, const FewTokens& few, hipStream_t s);
   int (*sums_few)(Product p, const Cut& c, const SumsOf& of, const FewTokens& few, hipStream_t s);
   int (*dz)(const Product& p, const Cut& c, const int* live, int64_t width, const Gradient& g, hipStream_t s);
   int (*dz_of_kept)(const Gradient& g, const Kept& kept, void* dz, int64_t width, int64_t T, int64_t N, const int* live, hipStream_t s);
@@ -633,8 +681,9 @@ const Runs& runs_f32();
 const Runs& runs_bf16();
 const Runs& runs_f16();
 
-// Up to kFewTokens tokens whose logits were kept: dx and dW by the vector unit.
-inline constexpr int kFewTokens = 16;
+// dx and dW of up to few_tokens() tokens whose logits were kept by the vector unit
+// (16 x 32000 x 4096 fp32 417 and 507 us, bf16 285 and 250, 8 tokens 209 and 238).
+inline int few_tokens(int dtype) { return dtype == kF32 ? 16 : 8; }
 size_t few_bytes(const mhc_linear_ce_args& a);
 int run_few(const mhc_linear_ce_args& a, const State& st, const float* dloss, float grad_scale, void* dx, void* dw, char* ws, hipStream_t s);
 
@@ -670,10 +719,10 @@ int run_dw(const Product& p, const Cut& c, const int* live, const ScaledBy& by, 
 template <typename T>
 const Runs& runs_of() {
   if constexpr (sizeof(T) == 2) {
-    static const Runs r = {run_sums<T, false>, run_sums_few<T>, run_dz<T>, run_dz_of_kept<T>, run_dx<T>, run_dw<T>, run_joint<T>};
+    static const Runs r = {run_sums<T, false>, run_sums_rows<T>, run_sums_few<T>, run_dz<T>, run_dz_of_kept<T>, run_dx<T>, run_dw<T>, run_joint<T>};
     return r;
   } else {
-    static const Runs r = {run_sums<T, false>, run_sums_few<T>, run_dz<T>, run_dz_of_kept<T>, run_dx<T>, run_dw<T>, nullptr};
+    static const Runs r = {run_sums<T, false>, run_sums_rows<T>, run_sums_few<T>, run_dz<T>, run_dz_of_kept<T>, run_dx<T>, run_dw<T>, nullptr};
     return r;
   }
 }

@@ -10,14 +10,15 @@ products are formed without their rows.  A target outside [0, V) of a token that
 gradient and the weight's NaN (it cannot be refused without waiting for the GPU).
 
 The logits are formed in fp32 of exact products. For the gradients, softmax - onehot, times the token's weight over the
-largest one, is rounded once to x's dtype as an operand of two more products, in pieces of the vocabulary; it is formed of
-the logits that the forward kept, where they take up to 2 GiB (and C is 768 or more, of float32 256), or of logits that are
-formed again. Of float32 operands the products are those of linear_act; of many tokens the logits, and from kept logits the
-gradients, are formed of fp16 parts, which hold a value to 2^-24 of itself and to 2^-40 of its row's largest (of the
-gradients' sums, of the largest term in their row of x or column of the vocabulary). Beside copies of operands whose rows
-are no whole four-byte words, a call takes workspace in proportion to the tokens (their rows of x, the sums of its gradient,
-eight bytes for each 64 to 256 columns) and up to some 0.5 GB for pieces of the vocabulary, whatever its size. Kept logits
-are held until the backward's graph is freed; without gradients none are.
+largest one, is rounded once to x's dtype as an operand of two more products, in pieces of the vocabulary (of up to 8 tokens
+it is not rounded); it is formed of the logits that the forward kept, where they take up to 2 GiB (and C is 768 or more, of
+float32 256, or the tokens are few), or of logits that are formed again. Of float32 operands the products are those of
+linear_act; of many tokens the logits, and from kept logits the gradients, are formed of fp16 parts, which hold a value to
+2^-24 of itself and to 2^-40 of its row's largest (of the gradients' sums, of the largest term in their row of x or column
+of the vocabulary). Beside copies of operands whose rows are no whole four-byte words, a call takes workspace in proportion
+to the tokens (their rows of x, the sums of its gradient, eight bytes for each 64 to 256 columns) and up to some 0.5 GB for
+pieces of the vocabulary, whatever its size. Kept logits are held until the backward's graph is freed; without gradients
+none are.
 
 x and weight are taken as they are, under torch.autocast too.
 
