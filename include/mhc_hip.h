@@ -531,8 +531,8 @@ size_t mhc_linear_ce_state_bytes(int64_t T);
 
 /* Bytes of the logits, for args->logits, in which the forward then keeps them
  * and the backward finds them; 0 where that does not pay (C below 768, of fp32
- * below 256, and more than 8 tokens, of fp32 16) or they are more than 2 GiB.  With args->logits NULL the backward
- * forms them again. */
+ * below 256, and more than 8 tokens, of fp32 16) or they are more than 2 GiB.
+ * With args->logits NULL the backward forms them again. */
 size_t mhc_linear_ce_logits_bytes(const mhc_linear_ce_args* args);
 
 size_t mhc_linear_ce_fwd_workspace_bytes(const mhc_linear_ce_args* args);
