@@ -346,3 +346,58 @@ def test_captured_calls_with_other_masks(C):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, step())), share
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,V,C", [(6, 1000, 300), (16, 3001, 129), (900, 4000, 1024)])
+def test_captured_calls_of_few_tokens_and_of_parts(dt, T, V, C):
+    x, w, y, g = inputs(19, T, V, C, dt)
+    mask = torch.ones(T, device="cuda")
+
+    def step():
+        xs, ws = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        loss, logp = linear_cross_entropy(xs, ws, y, mask)
+        return [loss.detach(), logp, *torch.autograd.grad(loss, [xs, ws])]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for share in (0.5, 0.0, 1.0):
+        mask.copy_(torch.rand(T, generator=g, device="cuda") < share)
+        x.normal_(generator=g)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, step())), share
+
+
+def test_calls_from_two_threads():
+    """Each on a stream of its own, with operands of its own."""
+    import threading
+
+    cases = [inputs(20, 5, 3000, 512, torch.float32)[:3], inputs(21, 900, 2000, 1024, torch.float32)[:3], inputs(22, 700, 3000, 800, torch.bfloat16)[:3]]
+    want = [linear_cross_entropy_and_grad(*c) for c in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(order):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                for k in order:
+                    got = linear_cross_entropy_and_grad(*cases[k])
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[k])):
+                        wrong.append(k)
+
+    threads = [threading.Thread(target=work, args=(o,)) for o in ((0, 1, 2), (2, 1, 0))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
