@@ -1,4 +1,5 @@
-// linear_cross_entropy's gradients of up to 16 tokens, from logits that were kept:
+// linear_cross_entropy's gradients of up to 16 tokens (8 of 16-bit rows), from
+// logits that were kept:
 //
 //   dx[t] = sum_v dz[t, v] W[v];  dW[v] = sum_t dz[t, v] x[t]
 //
@@ -200,8 +201,9 @@ int run(const mhc_linear_ce_args& a, const State& st, const ScaledBy& by, void* 
     case 2: return run<T, 2>(a, st, by, dx, dw, ws, s);
     case 4: return run<T, 4>(a, st, by, dx, dw, ws, s);
     case 8: return run<T, 8>(a, st, by, dx, dw, ws, s);
-    default: return run<T, 16>(a, st, by, dx, dw, ws, s);
   }
+  if constexpr (sizeof(T) == 4) return run<T, 16>(a, st, by, dx, dw, ws, s);
+  return MHC_OK;  // (not reached: few_tokens())
 }
 
 }  // namespace
