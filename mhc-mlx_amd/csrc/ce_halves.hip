@@ -11,7 +11,9 @@ struct MoreOp {
   }
 };
 
-// dz from logits that were kept, 8 columns of a row a thread: what both kernels below do with it
+// dz from logits that were kept, 8 columns of a row a thread: what both kernels
+// below do with it.  FAST: a bound of its magnitude; the hardware's exponential
+// is 0 where the other one gives subnormal numbers, which are below 2^-126.
 template <bool FAST, int ROWS, typename Use>
 MHC_DEV void each_dz(const Gradient& g, const Kept& kept, int64_t N, int64_t rows, int64_t m0, int64_t n, Use use) {
   constexpr int kEach = 8, kAhead = 4;
@@ -35,7 +37,8 @@ MHC_DEV void each_dz(const Gradient& g, const Kept& kept, int64_t N, int64_t row
       float d[8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        d[k] = r[q].each * gemm::exp_of<FAST>(z[q][k / 4][k % 4] - r[q].t) - (mine == k ? r[q].c : 0.f);
+        const float e = gemm::exp_of<FAST>(z[q][k / 4][k % 4] - r[q].t);  // (where it is NaN, so is `each`)
+        d[k] = r[q].each * (FAST ? fmaxf(e, 0x1p-126f) : e) - (mine == k ? r[q].c : 0.f);
         d[k] = n + k < N ? d[k] : 0.f;
       }
       use(m + q * kEach, d);
@@ -119,20 +122,20 @@ __global__ __launch_bounds__(256) void parts_kernel(const Gradient g, const Kept
   const uint32_t wide = (uint32_t)ceil_div(parts.pitch, 256);
   const int64_t rows = *live, m0 = (int64_t)(blockIdx.x / wide) * 32, n = (int64_t)(blockIdx.x % wide) * 256 + threadIdx.x % 32 * 8;
   if (n >= parts.pitch) return;
-  float w[8], col[8];
+  int w[8], col[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    w[k] = halves.w[min(n + k, N - 1)];
-    col[k] = lift_by(lift_of(parts.col[min(n + k, N - 1)]));
+    w[k] = power_of(halves.w[min(n + k, N - 1)]);
+    col[k] = power_of(lift_by(lift_of(parts.col[min(n + k, N - 1)])));
   }
   each_dz<false, 32>(g, kept, N, rows, m0, n, [&](int64_t m, const float(&d)[8]) {
-    const float x = halves.x[m], row = lift_by(lift_of(parts.row[m]));
+    const int x = power_of(halves.x[m]), row = power_of(lift_by(lift_of(parts.row[m])));
     float v[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = d[k] * (w[k] * row);
+    for (int k = 0; k < 8; ++k) v[k] = times_power(d[k], w[k] + row);
     put_parts(parts.x_high + m * parts.pitch + n, parts.x_low + m * parts.pitch + n, v);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = d[k] * (x * col[k]);
+    for (int k = 0; k < 8; ++k) v[k] = times_power(d[k], x + col[k]);
     put_parts(parts.w_high + m * parts.pitch + n, parts.w_low + m * parts.pitch + n, v);
   });
 }

@@ -52,24 +52,31 @@ template <> inline constexpr float kDzUnit<_Float16> = 0x1p14f;
 // tokens and columns, whose powers of two go to dz: dx's rows are sums of dz w[v]
 // over the parts of W, each row of dz w lifted as one of x is, dW's of dz x[t]
 // over the parts of x, each column lifted.
+//
+// Powers of two are put together as their exponents: the product of two of them
+// may be past fp32's range where the value that they go to is 0, or brings it
+// back into it, and so may the value times one of them.
+MHC_DEV int power_of(float two) { return (int)(__builtin_bit_cast(uint32_t, two) >> 23) - 127; }
+MHC_DEV float times_power(float v, int e) { return __builtin_ldexpf(v, e); }
+
 struct Halves {
   const float *x, *w;  // of each row: what its parts are to be multiplied by
 
   template <int BM, int BN, int WM, int WN, int JM, int JN>
   MHC_DEV void scale(const Product& p, const gemm::Place<BM, BN, WM, WN>& at, f32x4 (&acc)[JN][JM]) const {
     const int64_t m0 = at.m0 + at.wm + at.lane % 16, n0 = at.n0 + at.wn + at.lane / 16 * 4;
-    float row[JM];
+    int row[JM];
 #pragma unroll
-    for (int j = 0; j < JM; ++j) row[j] = x[min(m0 + j * 16, p.M - 1)];
+    for (int j = 0; j < JM; ++j) row[j] = power_of(x[min(m0 + j * 16, p.M - 1)]);
 #pragma unroll
     for (int i = 0; i < JN; ++i) {
-      f32x4 column;
+      int column[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) column[k] = w[min(n0 + i * 16 + k, p.N - 1)];
+      for (int k = 0; k < 4; ++k) column[k] = power_of(w[min(n0 + i * 16 + k, p.N - 1)]);
 #pragma unroll
       for (int j = 0; j < JM; ++j)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) acc[i][j][k] *= row[j] * column[k];  // (the sum times one of them may be past the range)
+        for (int k = 0; k < 4; ++k) acc[i][j][k] = times_power(acc[i][j][k], row[j] + column[k]);
     }
   }
 };

@@ -1,0 +1,81 @@
+"""linear_cross_entropy at the ends of fp32's range, where its products are of fp16 parts: against float64 (tests/_block.py)."""
+
+import pytest
+import torch
+
+from mhc_mlx_amd import linear_cross_entropy_and_grad
+from tests._block import ce64
+from tests._train import close
+
+pytestmark = pytest.mark.gpu
+
+# fp32 sizes whose logits are kept and whose gradients are formed of parts
+PARTS = [(900, 4000, 1024), (1100, 32768, 1024)]
+
+
+def rand(seed, *shapes):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return [torch.randn(*s, generator=g, device="cuda") for s in shapes]
+
+
+def check(x, w, y, what, scale=1.0):
+    """Against ce64, and what parts cannot hold: terms are lifted by at most 2^126 to fp16 parts, whose least step is 2^-24, and meet
+    parts of up to 2^15, so that each of a sum's products is off by half of 2^-24 2^-126 2^15 at most, for each of two operands."""
+    got = dict(zip(("loss", "logp", "dx", "dw"), linear_cross_entropy_and_grad(x, w, y, grad_scale=scale)))
+    least = scale / len(y) * 2.0 ** -135
+    for k, (value, bound) in ce64(x, w, y, scale=scale).items():
+        close(got[k], value, bound + {"dx": len(w), "dw": len(y)}.get(k, 0) * least, f"{what} {k}")
+
+
+@pytest.mark.parametrize("T,V,C", PARTS)
+@pytest.mark.parametrize("up", [15, 16, 20, 40])
+def test_columns_without_probability(T, V, C, up):
+    """Rows of x around 2^up: nearly every column's probabilities are 0, and its gradient with them."""
+    x, w = rand(up, (T, C), (V, C))
+    y = torch.arange(T, device="cuda") % V
+    check(x * 2.0 ** (up - 1), w * C ** -0.5, y, f"x {up}")
+
+
+@pytest.mark.parametrize("T,V,C", PARTS)
+@pytest.mark.parametrize("up", [16, 20, 40])
+def test_tokens_that_are_certain(T, V, C, up):
+    """Rows of W around 2^up, some tokens near their targets' rows: their probability is 1, their dz 0 everywhere."""
+    x, w = rand(up, (T, C), (V, C))
+    y = torch.arange(T, device="cuda") * 3 % V
+    w = w * 2.0 ** (up - 1)
+    x[::2] += 4.0 * 2.0 ** (1 - up) * w[y[::2]]
+    check(x, w, y, f"w {up}")
+
+
+@pytest.mark.parametrize("up", [0, 16, 40, 100, -100])
+def test_probabilities_that_are_subnormal(up):
+    """All tokens' probabilities of each column but one between e^-83 and e^-105, beside rows of x or of W around 2^|up|."""
+    T, V, C = 900, 4000, 1024
+    noise, = rand(7, (T, C))
+    along = torch.ones(C, device="cuda") / C ** 0.5
+    below = -(85.0 + 18.0 * torch.arange(V, device="cuda") / V)
+    below[0] = 0.0
+    x = (along + 0.001 * noise) * 2.0 ** up
+    w = (below[:, None] * along) * 2.0 ** -up
+    y = torch.zeros(T, dtype=torch.int64, device="cuda")
+    scale = 1.0 if abs(up) == 100 else 2.0 ** 40  # (so that gradients are neither past the range nor subnormal)
+    check(x, w, y, f"{up}", scale)
+    y[::3] = 1 + torch.arange(T, device="cuda")[::3]
+    check(x, w, y, f"{up} with unlikely targets", scale)
+
+
+@pytest.mark.parametrize("T,V,C", PARTS + [(700, 32768, 128)])
+def test_large_rows_that_meet_in_no_element(T, V, C):
+    """Rows of x around 2^100 and of W around 2^80 whose products are 0, beside ordinary ones: logits are those of the formula.  (dx and
+    dW hold their terms to 2^-40 of the largest ones, which the large rows' are.)"""
+    x, w = rand(3, (T, C), (V, C))
+    w *= C ** -0.5
+    x[:, :2], w[:, :2] = 0.0, 0.0
+    x[5], w[7] = 0.0, 0.0
+    x[5, 0], w[7, 1] = 2.0 ** 100, -2.0 ** 80
+    y = torch.arange(T, device="cuda")
+    loss, logp, dx, dw = linear_cross_entropy_and_grad(x, w, y)
+    ref = ce64(x, w, y)
+    close(loss, *ref["loss"], "loss")
+    close(logp, *ref["logp"], "logp")
+    assert bool(dx.isfinite().all()) and bool(dw.isfinite().all())
