@@ -6,8 +6,8 @@
 //   g = dy w;  n = h s;  dx = dr = s (g - n mean(g n)) + dh;  dw = sum_t dy n
 //
 // s cancels in the codes, so that they need only a row's largest product: of
-// 16-bit values and weights the products and 127 times them are exact in fp32,
-// and so is the code, ties included.
+// 16-bit values and weights the products are exact in fp32, and so is the code,
+// ties included (see Coder).
 //
 // Bound by memory: a row is read once and written once, held in registers
 // between (8192 x 4096 bf16, with a residual: forward 45 us for 268 MB, 6.0 TB/s;
@@ -67,6 +67,13 @@ struct LargerOp {
 // quotient is corrected by its remainder, which makes it the nearest number to
 // 127 p / top.  A row of zeros has codes of 0 and the scale 0, one with an
 // infinity or NaN codes of 0 and the scale NaN.
+//
+// 127 p is exact for a p of up to 17 bits (bf16 times bf16 has 16), and no such
+// quotient that is not a tie rounds to one.  A product of two fp16 numbers has 22
+// bits, of which 127 p may lose up to five, and quotients lie as near as 2^-31
+// to a tie: codes whose quotient is within its error of one (one in 2^15) are put
+// right by their distance from 127 p, which is a number, and by what was lost
+// (2048 x 4096 fp16 13.3 to 14.1 us, all codes put right so 15.5).
 struct Coder {
   float up, top, inv;
   bool some;
@@ -78,20 +85,47 @@ struct Coder {
     top = some ? t * up : 1.f;
     inv = 1.f / top;
   }
-  MHC_DEV int code(float p) const {
+  MHC_DEV float quotient(float p) const {
     const float a = 127.f * (p * up), q = a * inv;
-    return some ? (int)rintf(fmaf(fmaf(-q, top, a), inv, q)) : 0;
+    return fmaf(fmaf(-q, top, a), inv, q);
+  }
+  MHC_DEV int code(float p) const { return some ? (int)rintf(quotient(p)) : 0; }
+  // the same, and how far a quotient is from its code at most: of a long product the code may not be the nearest if that is near 1/2
+  static constexpr float kUnsure = 0.5f - 0x1p-16f;
+  MHC_DEV int code(float p, float& far) const {
+    const float q = quotient(p), c = rintf(q);
+    far = fmaxf(far, fabsf(q - c));
+    return some ? (int)c : 0;
+  }
+  MHC_DEV int sure_code(float p) const {
+    const float u = p * up, a = 127.f * u, lost = fmaf(127.f, u, -a);
+    float c = rintf(quotient(p));
+    const float d = fmaf(-c, top, a), past = (fabsf(d) - 0.5f * top) + (d < 0.f ? -lost : lost);  // the middle between c and its neighbour
+    if (past > 0.f || (past == 0.f && ((int)c & 1) != 0)) c += d < 0.f ? -1.f : 1.f;
+    return some ? (int)c : 0;
   }
   static MHC_DEV float scale(float t, float s) { return t < __builtin_inff() ? t * s / 127.f : __builtin_nanf(""); }
 };
 
-template <bool WHOLE, int V>
+// whether rows of T in this mode are such products
+template <typename T, int MODE> constexpr bool kLong = MODE == kCodes && __is_same(T, _Float16);
+
+template <bool WHOLE, bool LONG, int V>
 MHC_DEV void put_codes(int8_t* p, const Coder& c, const float (&v)[V], int left) {
   uint32_t w[V / 4];
+  const auto each = [&](auto code) {
 #pragma unroll
-  for (int k = 0; k < V / 4; ++k)
-    w[k] = (uint32_t)(c.code(v[4 * k]) & 255) | (uint32_t)(c.code(v[4 * k + 1]) & 255) << 8 | (uint32_t)(c.code(v[4 * k + 2]) & 255) << 16 |
-           (uint32_t)c.code(v[4 * k + 3]) << 24;
+    for (int k = 0; k < V / 4; ++k)
+      w[k] = (uint32_t)(code(v[4 * k]) & 255) | (uint32_t)(code(v[4 * k + 1]) & 255) << 8 | (uint32_t)(code(v[4 * k + 2]) & 255) << 16 |
+             (uint32_t)code(v[4 * k + 3]) << 24;
+  };
+  if constexpr (LONG) {
+    float far = 0.f;
+    each([&](float z) { return c.code(z, far); });
+    if (far > Coder::kUnsure) [[unlikely]] each([&](float z) { return c.sure_code(z); });
+  } else {
+    each([&](float z) { return c.code(z); });
+  }
   if constexpr (WHOLE) {
     __builtin_memcpy(p, w, V);
   } else {
@@ -286,8 +320,8 @@ __global__ __launch_bounds__((Held<T, THREADS, NV>::kBlock)) void norm_held_kern
     int8_t* const codes = static_cast<int8_t*>(a.y) + t * a.C;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (at.has(i)) put_codes<true>(codes + at.vec(i) * V, coder, z[i], V);
-    if (at.on_tail) codes[at.tail] = (int8_t)coder.code(z1);
+      if (at.has(i)) put_codes<true, kLong<T, MODE>>(codes + at.vec(i) * V, coder, z[i], V);
+    if (at.on_tail) codes[at.tail] = (int8_t)(kLong<T, MODE> ? coder.sure_code(z1) : coder.code(z1));
   }
 }
 
@@ -388,7 +422,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(const NormArgs 
       } else {
 #pragma unroll
         for (int k = 0; k < V; ++k) z[k] = z[k] * by * w[k];
-        put_codes<W>(static_cast<int8_t*>(a.y) + t * C + n, coder, z, left);
+        put_codes<W, kLong<T, MODE>>(static_cast<int8_t*>(a.y) + t * C + n, coder, z, left);
       }
     });
   }
