@@ -27,7 +27,7 @@ struct Scales {
 // int32 sums to fp32 values, with the bias (in the first of a reduction's
 // parts).  The tile's scales are loaded before its sums are formed, one or two
 // numbers a thread, and shared through LDS after them.  So that the residuals
-// are in L2 by then, a word of each of their lines is loaded too, and dropped
+// are in L2 by then, one of each of their lines is loaded too, and dropped
 // (1001 x 2050 x 1100, operands from memory: 15.4 to 14.3 us).
 template <typename O>
 struct Scaled {
@@ -47,16 +47,16 @@ struct Scaled {
     static_assert(kTouch <= kMost, "lines of a tile's residuals");
     const int t = threadIdx.x;
     const int64_t n = min(at.n0 + (t < BM ? 0 : t - BM), p.N - 1);
-    const float* const from = t < BM ? s.x + min(at.m0 + t, p.M - 1) : s.w + n;
-    Own own = {*from, s.bias != nullptr && t >= BM ? s.bias[n] : 0.f, {}};
+    const float* const scale = t < BM ? s.x + min(at.m0 + t, p.M - 1) : s.w + n;
+    Own own = {*scale, s.bias != nullptr && t >= BM ? s.bias[n] : 0.f, {}};
 #pragma unroll
     for (int i = 0; i < kTouch; ++i) {
       const int line = i * kThreads + t;
       const int64_t m = min(at.m0 + line / kLines, p.M - 1), c = min(at.n0 + line % kLines * (kLine / (int)sizeof(O)), p.N - 1);
-      // (whole words of the residual or, without one, of the scales: a load under a condition would wait for itself)
-      const uintptr_t place = p.e.residual != nullptr ? reinterpret_cast<uintptr_t>(static_cast<const O*>(p.e.residual) + m * p.N + c)
-                                                      : reinterpret_cast<uintptr_t>(s.x);
-      own.touched[i] = *reinterpret_cast<const uint32_t*>(place & ~(uintptr_t)3);
+      // (without residuals a scale: a load under a condition would wait for itself)
+      const void* const from = p.e.residual != nullptr ? static_cast<const void*>(static_cast<const O*>(p.e.residual) + m * p.N + c) : s.x;
+      if constexpr (sizeof(O) == 4) own.touched[i] = *static_cast<const uint32_t*>(from);
+      else own.touched[i] = *static_cast<const uint16_t*>(from);
     }
     return own;
   }
