@@ -32,15 +32,14 @@ import torch
 
 from . import ops
 from .int8 import call
+from .policy import _check_denominator
 from .profiling import timed
 
 __all__ = ["linear_cross_entropy", "linear_cross_entropy_and_grad", "linear_cross_entropy_reference"]
 
 
 def _check(denominator, ignore_index):
-    if denominator is not None and not denominator > 0:
-        raise ValueError(f"denominator must be positive (got {denominator})")
-    return 0.0 if denominator is None else float(denominator), int(ignore_index)
+    return _check_denominator(denominator), int(ignore_index)
 
 
 class LinearCrossEntropyFn(torch.autograd.Function):

@@ -26,12 +26,19 @@ from .profiling import timed
 __all__ = ["policy_loss", "policy_loss_and_grad"]
 
 
+def _check_denominator(denominator) -> float:
+    """As the kernels take it: a float32, or 0 for the sum of the weights."""
+    if denominator is None:
+        return 0.0
+    if not 2.0 ** -126 <= denominator <= torch.finfo(torch.float32).max:
+        raise ValueError(f"denominator must be positive, at least 2^-126 and a finite float32 (got {denominator})")
+    return float(denominator)
+
+
 def _check(clip_low, clip_high, denominator) -> float:
     if not (clip_low >= 0 and clip_high >= 0):
         raise ValueError(f"clip_low and clip_high must be >= 0 (got {clip_low}, {clip_high})")
-    if denominator is not None and not denominator > 0:
-        raise ValueError(f"denominator must be positive (got {denominator})")
-    return 0.0 if denominator is None else float(denominator)
+    return _check_denominator(denominator)
 
 
 class PolicyLossFn(torch.autograd.Function):

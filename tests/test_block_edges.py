@@ -1,0 +1,28 @@
+"""The cross entropy's and the policy loss's numbers and masks at their ends, without a GPU."""
+
+import math
+
+import pytest
+import torch
+
+from mhc_mlx_amd import linear_cross_entropy, linear_cross_entropy_and_grad, policy_loss, policy_loss_and_grad
+
+
+@pytest.mark.parametrize("bad", [1e-50, 1e-40, 2.0 ** -127, 1e39, math.inf, math.nan])
+def test_denominators_that_are_no_float32_are_refused(bad):
+    """1e-50 is 0 there, and 0 asks for the sum of the weights."""
+    x, y, t = torch.zeros(2, 4), torch.zeros(2, dtype=torch.long), torch.zeros(2)
+    for call in (linear_cross_entropy, linear_cross_entropy_and_grad):
+        with pytest.raises(ValueError, match="denominator"):
+            call(x, x, y, denominator=bad)
+    for call in (policy_loss, policy_loss_and_grad):
+        with pytest.raises(ValueError, match="denominator"):
+            call(x, y, t, t, denominator=bad)
+
+
+def test_denominators_that_are_taken():
+    x, y, t = torch.zeros(2, 4), torch.zeros(2, dtype=torch.long), torch.zeros(2)
+    for good in (2.0 ** -126, 3, torch.finfo(torch.float32).max):
+        for call in (lambda: linear_cross_entropy(x, x, y, denominator=good), lambda: policy_loss(x, y, t, t, denominator=good)):
+            with pytest.raises(ValueError, match="GPU"):  # (the next check)
+                call()
