@@ -70,8 +70,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
                          denominator: float | None = None, ignore_index: int = -100):
     """(loss, logp): the scalar loss, differentiable in ``x`` and ``weight``, and each token's log probability (no gradient).
 
-    x [..., C] and weight [V, C] float32, bfloat16 or float16, of one dtype; targets [...] int64 or int32; mask [...] bool,
-    uint8 or floating weights.
+    x [..., C] and weight [V, C] float32, bfloat16 or float16, of one dtype; targets [...] int64 or int32; mask [...] bool
+    or uint8 (a token counts where it is not 0), or floating weights.
     """
     numbers = _check(denominator, ignore_index)
     if ops._use_binding() and torch.autograd.forward_ad._current_level < 0:  # (forward mode is refused by the Function)
@@ -93,6 +93,8 @@ def linear_cross_entropy_reference(x, weight, targets, mask=None, denominator=No
     """linear_cross_entropy in elementary torch operations (fp32 for half inputs, else the inputs' dtype), on any device."""
     den, ignored = _check(denominator, ignore_index)
     up = torch.float64 if x.dtype == torch.float64 else torch.float32
+    if mask is not None and mask.dtype == torch.uint8:
+        mask = mask != 0
     w = torch.ones(targets.shape, dtype=up, device=x.device) if mask is None else mask.to(up)
     w = torch.where(targets == ignored, 0.0, w)
     live = w != 0
