@@ -20,7 +20,8 @@ to the tokens (their rows of x, the sums of its gradient, eight bytes for each 6
 pieces of the vocabulary, whatever its size. Kept logits are held until the backward's graph is freed; without gradients
 none are.
 
-x and weight are taken as they are, under torch.autocast too.
+x and weight are taken as they are, under torch.autocast too; there, where their dtypes differ (a 16-bit hidden state and a
+head's float32 weight), both are brought to the autocast dtype, as nn.Linear does, and gradients have the tensors' own.
 
 ``linear_cross_entropy`` is differentiable in x and weight (once); ``linear_cross_entropy_and_grad`` returns the gradients with
 the loss, for a caller without autograd.
@@ -28,10 +29,13 @@ the loss, for a caller without autograd.
 
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import ops
 from .int8 import call
+from .linear import _autocast_dtype
 from .policy import _check_denominator
 from .profiling import timed
 
@@ -40,6 +44,14 @@ __all__ = ["linear_cross_entropy", "linear_cross_entropy_and_grad", "linear_cros
 
 def _check(denominator, ignore_index):
     return _check_denominator(denominator), int(ignore_index)
+
+
+def _as_one(x, weight):
+    """x and weight in one dtype, where autocast has one for them."""
+    cast = _autocast_dtype(x) if x.dtype != weight.dtype else None
+    if cast is None or torch.float64 in (x.dtype, weight.dtype) or not (x.is_floating_point() and weight.is_floating_point()):
+        return x, weight
+    return x.to(cast), weight.to(cast)
 
 
 class LinearCrossEntropyFn(torch.autograd.Function):
@@ -74,6 +86,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
     or uint8 (a token counts where it is not 0), or floating weights.
     """
     numbers = _check(denominator, ignore_index)
+    x, weight = _as_one(x, weight)
     if ops._use_binding() and torch.autograd.forward_ad._current_level < 0:  # (forward mode is refused by the Function)
         return ops._binding().linear_ce(x, weight, targets, mask, *numbers)
     return LinearCrossEntropyFn.apply(x, weight, targets, mask, *numbers)
@@ -81,12 +94,14 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.T
 
 def linear_cross_entropy_and_grad(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, mask: torch.Tensor | None = None,
                                   denominator: float | None = None, ignore_index: int = -100, grad_scale: float = 1.0):
-    """(loss, logp, dx, dweight): linear_cross_entropy and grad_scale times its gradients, in x's dtype. No autograd.
+    """(loss, logp, dx, dweight): linear_cross_entropy and grad_scale times its gradients, in the tensors' dtypes. No autograd.
 
     ``grad_scale`` is the loss scale of float16 training (the loss itself is not scaled).
     """
     numbers = _check(denominator, ignore_index)
-    return call("linear_ce_and_grad", x, weight, targets, mask, *numbers, float(grad_scale))
+    xs, ws = _as_one(x, weight)
+    loss, logp, dx, dw = call("linear_ce_and_grad", xs, ws, targets, mask, *numbers, float(grad_scale))
+    return loss, logp, dx.to(x.dtype), dw.to(weight.dtype)
 
 
 def linear_cross_entropy_reference(x, weight, targets, mask=None, denominator=None, ignore_index: int = -100):
@@ -98,7 +113,8 @@ def linear_cross_entropy_reference(x, weight, targets, mask=None, denominator=No
     w = torch.ones(targets.shape, dtype=up, device=x.device) if mask is None else mask.to(up)
     w = torch.where(targets == ignored, 0.0, w)
     live = w != 0
-    z = torch.matmul(torch.where(live[..., None], x.to(up), 0.0), weight.to(up).t())
+    with torch.autocast(x.device.type, enabled=False) if _autocast_dtype(x) else contextlib.nullcontext():
+        z = torch.matmul(torch.where(live[..., None], x.to(up), 0.0), weight.to(up).t())
     at = torch.where(live, targets, 0).long()
     bad = (at < 0) | (at >= weight.shape[0])
     picked = z.gather(-1, torch.where(bad, 0, at)[..., None])[..., 0]

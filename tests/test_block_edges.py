@@ -37,3 +37,13 @@ def test_byte_masks_of_the_plain_form():
     want = linear_cross_entropy_reference(x, w, y, mask != 0)
     got = linear_cross_entropy_reference(x, w, y, mask)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_the_plain_form_under_autocast():
+    """Its logits stay in float32."""
+    g = torch.Generator().manual_seed(1)
+    x, w = torch.randn(6, 50, generator=g), torch.randn(7, 50, generator=g)
+    want = linear_cross_entropy_reference(x, w, torch.arange(6))
+    with torch.autocast("cpu", torch.bfloat16):
+        got = linear_cross_entropy_reference(x, w, torch.arange(6))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from mhc_mlx_amd import linear_cross_entropy_and_grad
+from mhc_mlx_amd import linear_cross_entropy, linear_cross_entropy_and_grad
 from tests._block import ce64
 from tests._train import close
 
@@ -79,3 +79,38 @@ def test_large_rows_that_meet_in_no_element(T, V, C):
     close(loss, *ref["loss"], "loss")
     close(logp, *ref["logp"], "logp")
     assert bool(dx.isfinite().all()) and bool(dw.isfinite().all())
+
+
+@pytest.mark.parametrize("given", [(torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16), (torch.float16, torch.float32), (torch.float32, torch.float32)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_under_autocast(dt, given):
+    """Operands of two dtypes are taken in the autocast one; gradients come in their own."""
+    x, w = rand(9, (70, 96), (300, 96))
+    x, w = x.to(given[0]).requires_grad_(True), (w * 0.1).to(given[1]).requires_grad_(True)
+    y = torch.arange(70, device="cuda")
+    cast = dt if given[0] != given[1] else given[0]
+    xs, ws = x.detach().to(cast).requires_grad_(True), w.detach().to(cast).requires_grad_(True)
+    want = linear_cross_entropy(xs, ws, y)
+    dx, dw = torch.autograd.grad(want[0], [xs, ws])
+    with torch.autocast("cuda", dt):
+        got = linear_cross_entropy(x, w, y)
+        fused = linear_cross_entropy_and_grad(x, w, y)
+    grads = torch.autograd.grad(got[0], [x, w])
+    assert grads[0].dtype == x.dtype and grads[1].dtype == w.dtype
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert torch.equal(grads[0], dx.to(x.dtype)) and torch.equal(grads[1], dw.to(w.dtype))
+    assert all(torch.equal(a, b) for a, b in zip(fused, (want[0], want[1], *grads)))
+    if cast != given[0] or cast != given[1]:
+        with pytest.raises(ValueError, match="dtype"):
+            linear_cross_entropy(x, w, y)
+
+
+def test_other_operands_under_autocast_are_refused():
+    x, w = rand(10, (4, 16), (8, 16))
+    y = torch.arange(4, device="cuda")
+    with torch.autocast("cuda", torch.bfloat16):
+        for a, b in ((x, w.double()), (x.double(), w), (x, w.int()), (x.bfloat16(), w.to(torch.float8_e4m3fn).view(torch.uint8))):
+            with pytest.raises(ValueError):
+                linear_cross_entropy(a, b, y)
+            with pytest.raises(ValueError):
+                linear_cross_entropy_and_grad(a, b, y)
