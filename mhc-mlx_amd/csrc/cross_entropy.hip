@@ -342,18 +342,43 @@ struct FwdPlan {
   int64_t piece;  // columns of the vocabulary at a time
   bool direct;    // the live rows of x are read where they lie
   bool few;       // and found by the products' launch
-  bool rows;      // which is that for up to kFewRows tokens
+  bool rows;      // which is that for up to kFewRows tokens, else one of tiles
   size_t x, w, part, at_target, total;  // bytes; terms come last
 };
+
+// What reading `bytes` at a rate in GB/ms takes of `blocks` workgroups, of which
+// `room` are on the card at once: a last round that is not full costs `share` of
+// what it is not full by.
+float reading_us(int64_t bytes, float rate, int64_t blocks, int64_t room, float share) {
+  const float rounds = (float)blocks / (float)room, full = std::max(1.f, ceilf(rounds) / std::max(1.f, rounds));
+  return (float)bytes / (rate * 1e6f) * (1.f + share * (full - 1.f));
+}
+
+// Whether up to kFewRows tokens go to sums_rows_kernel: all of fp32 rows, whose
+// tiles are bound by their products (the call's kernels, 8 tokens: 32000 x 2048 56
+// us, tiles 98), and 16-bit ones unless tiles of 64 rows, whose start is longer
+// and of which fewer are on the card at once, are estimated faster (rows and
+// tiles, 8 tokens bf16: 4524 x 2240 11 and 23 us, 16384 x 1024 13 and 17, 72999 x
+// 2624 73 and 83, 151936 x 2048 118 and 137, 256000 x 2048 191 and 209; but 32000 x
+// 2048 31 and 29, 32000 x 4096 57 and 47, 50257 x 4096 90 and 83, 128256 x 4096 203
+// and 192.  Of 35 sizes three take the one that is more than 3 % slower, by a
+// tenth at most: 16384 x 4096 35 and 33, 24576 x 2048 27 and 25, 256000 x 768 87 and 82).
+bool takes_rows(const mhc_linear_ce_args& a, const Cut& c) {
+  if (a.dtype == kF32 || c.tile < 3) return true;
+  const int64_t cus = device_cu_count(), bytes = a.V * a.C * gemm::elem_bytes(a.dtype);
+  const float rows = std::max(4.f, reading_us(bytes, 5.7f, ceil_div(a.V, ce::kRowsColumns), 3 * cus, 0.25f));
+  return rows <= std::max(c.us + 2.f, reading_us(bytes, 5.6f, ceil_div(a.V, c.tile == 3 ? 128 : 64), 2 * cus, 0.5f));
+}
 
 FwdPlan plan_fwd(const mhc_linear_ce_args& a) {
   constexpr int kBn[] = {256, 256, 128, 128, 64};
   FwdPlan p;
   const int e = gemm::elem_bytes(a.dtype);
-  p.direct = p.few = false;
-  p.rows = a.T <= ce::kFewRows;
-  if (p.rows) {
-    p.few = true;
+  p.direct = p.few = p.rows = false;
+  if (a.T <= ce::kFewRows) {
+    p.cut = gemm::cut_of(a.T, a.V, a.C, a.dtype, true, true, 1);
+    p.rows = takes_rows(a, p.cut);
+    p.few = p.direct = true;
     p.piece = a.V;
     p.x = gemm::pack_bytes(a.x, a.T, a.ldx, a.C, a.dtype);
     p.w = gemm::pack_bytes(a.w, a.V, a.ldw, a.C, a.dtype);
@@ -636,7 +661,7 @@ extern "C" int mhc_linear_ce_fwd(const mhc_linear_ce_args* args, float* loss, fl
       }
     } else {
       Product q = {Operand{a.x, a.ldx, a.C}, {}, a.T, a.V, a.C, {}, 1, 0};
-      if (p.rows) {
+      if (a.T <= ce::kFewRows) {
         char* to = x;
         if (const int rc = gemm::operand(q.a, a.x, a.T, a.ldx, a.C, a.dtype, to, s)) return rc;
       } else if (!p.direct) {

@@ -567,11 +567,10 @@ inline constexpr int kFewRows = 16, kRowsColumns = 32;
 
 // Up to 16 tokens: 32 columns a workgroup, whose waves split k as few_rows_kernel's
 // do, so that a small vocabulary's products take no longer than their loads, and
-// 16 rows are multiplied instead of 64 (fp32 12 x 9376 x 2285 62 to 29 us, 2 x 72999
-// x 2624 288 to 147; bf16 2 x 4524 x 2240 22 to 13, 2 x 128000 x 2048 114 to 106,
-// but 4 x 32000 x 4096, whose 1000 workgroups are a little more than there is room
-// for at once, 47 to 62).  All tokens' logits are formed, and
-// those of the live ones looked at, 32 threads for each.
+// 16 rows are multiplied instead of 64 (12 x 9376 x 2285 fp32 62 to 29 us, 2 x 72999
+// x 2624 251 to 143; bf16 2 x 4524 x 2240 21 to 10).  takes_rows says when.  All
+// tokens' logits are formed, and those of the live ones looked at, 32 threads for
+// each.
 template <typename T, int NS>
 __global__ __launch_bounds__(64 * gemm::kFewWaves) void sums_rows_kernel(const Product p, const SumsOf of, const FewTokens few) {
   constexpr int NT = kRowsColumns / 16, kN = kRowsColumns, kSums = gemm::kFewWaves * kFewRows * kN * 4;

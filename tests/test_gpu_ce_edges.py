@@ -114,3 +114,38 @@ def test_other_operands_under_autocast_are_refused():
                 linear_cross_entropy(a, b, y)
             with pytest.raises(ValueError):
                 linear_cross_entropy_and_grad(a, b, y)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("T", [1, 3, 8, 9, 16])
+def test_few_tokens_over_a_vocabulary_that_tiles_read_faster(T, dt):
+    """Strides, tokens left out, none at all, and a captured call that follows its mask."""
+    V, C = 32000, 2048
+    x, w = rand(T, (T, C), (V, C))
+    w = (w * C ** -0.5).to(dt)
+    y = (torch.arange(T, device="cuda") * 1999 + 7) % V
+    x = (x + 3.0 * w[y].float()).to(dt)
+    mask = torch.arange(T, device="cuda") % 3 != 1
+    want = linear_cross_entropy_and_grad(x, w, y, mask, grad_scale=64.0)
+    for got, (value, bound) in zip(want, ce64(x, w, y, mask, scale=64.0).values()):
+        close(got, value, bound)
+    wide = torch.full((T, C + 9), float("nan"), device="cuda", dtype=dt)
+    for at in (0, 1, 4):
+        xv = wide[:, at:at + C].copy_(x)
+        assert all(torch.equal(a, b) for a, b in zip(linear_cross_entropy_and_grad(xv, w, y, mask, grad_scale=64.0), want))
+    xm = torch.where(mask[:, None], x, float("nan"))
+    assert all(torch.equal(a, b) for a, b in zip(linear_cross_entropy_and_grad(xm, w, y, mask, grad_scale=64.0), want))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        linear_cross_entropy(x, w, y, mask)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = linear_cross_entropy(x, w, y, mask)
+    for m in (mask, ~mask, torch.zeros_like(mask), torch.ones_like(mask)):
+        mask.copy_(m.clone())
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, linear_cross_entropy(x, w, y, mask)))
