@@ -325,19 +325,19 @@ std::tuple<at::Tensor, at::Tensor> linear_ce_bwd(const at::Tensor& x, const at::
 // (loss, logp, dx, dw)
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_ce_and_grad(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets,
                                                                               const OptTensor& mask, double denominator, int64_t ignore_index,
-                                                                              double grad_scale) {
+                                                                              double grad_scale, bool keep) {
   const at::AutoGradMode plain_mode(false);
   CeInputs c = ce_inputs(x, w, targets, get(mask), denominator, ignore_index);
   const at::DeviceGuard guard(x.device());
-  const CeResult r = ce_forward(c, x, true);
+  const CeResult r = ce_forward(c, x, keep);
   auto [dx, dw] = ce_backward(c, x, w, r.state, at::Tensor(), grad_scale, true, true);
   return {r.loss, r.logp, dx, dw};
 }
 
 struct LinearCeFn : public torch::autograd::Function<LinearCeFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, const OptTensor& mask,
-                               double denominator, int64_t ignore_index) {
-    auto [loss, logp, state] = linear_ce_fwd(x, w, targets, mask, denominator, ignore_index, true);
+                               double denominator, int64_t ignore_index, bool keep) {
+    auto [loss, logp, state] = linear_ce_fwd(x, w, targets, mask, denominator, ignore_index, keep);
     ctx->save_for_backward({x, w, targets, get(mask), state});
     ctx->saved_data["denominator"] = denominator;
     ctx->saved_data["ignore_index"] = ignore_index;
@@ -347,7 +347,7 @@ struct LinearCeFn : public torch::autograd::Function<LinearCeFn> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    variable_list r(6);
+    variable_list r(7);
     if (!grads[0].defined()) return r;
     const auto sv = ctx->get_saved_variables();
     auto [dx, dw] = linear_ce_bwd(sv[0], sv[1], sv[2], sv[3].defined() ? OptTensor(sv[3]) : OptTensor(), ctx->saved_data["denominator"].toDouble(),
@@ -359,12 +359,12 @@ struct LinearCeFn : public torch::autograd::Function<LinearCeFn> {
 };
 
 std::tuple<at::Tensor, at::Tensor> linear_ce(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, const OptTensor& mask,
-                                             double denominator, int64_t ignore_index) {
+                                             double denominator, int64_t ignore_index, bool keep) {
   if (!needs_grad({&x, &w})) {
     auto [loss, logp, state] = linear_ce_fwd(x, w, targets, mask, denominator, ignore_index, false);
     return {loss, logp};
   }
-  variable_list r = LinearCeFn::apply(x, w, targets, mask.has_value() ? OptTensor(mask->detach()) : mask, denominator, ignore_index);
+  variable_list r = LinearCeFn::apply(x, w, targets, mask.has_value() ? OptTensor(mask->detach()) : mask, denominator, ignore_index, keep);
   return {r[0], r[1]};
 }
 

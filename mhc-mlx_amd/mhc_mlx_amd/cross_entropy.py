@@ -17,8 +17,8 @@ linear_act; of many tokens the logits, and from kept logits the gradients, are f
 2^-24 of itself and to 2^-40 of its row's largest (of the gradients' sums, of the largest term in their row of x or column
 of the vocabulary). Beside copies of operands whose rows are no whole four-byte words, a call takes workspace in proportion
 to the tokens (their rows of x, the sums of its gradient, eight bytes for each 64 to 256 columns) and up to some 0.5 GB for
-pieces of the vocabulary, whatever its size. Kept logits are held until the backward's graph is freed; without gradients
-none are.
+pieces of the vocabulary, whatever its size. Kept logits (float32, [T, V]) are held until the backward's graph is
+freed; without gradients, or with ``keep_logits`` false, none are.
 
 x and weight are taken as they are, under torch.autocast too; there, where their dtypes differ (a 16-bit hidden state and a
 head's float32 weight), both are brought to the autocast dtype, as nn.Linear does, and gradients have the tensors' own.
@@ -58,9 +58,10 @@ class LinearCrossEntropyFn(torch.autograd.Function):
     """linear_cross_entropy with its host steps in Python: under a kernel timer, and for torch.jit.trace, which records it."""
 
     @staticmethod
-    def forward(ctx, x, weight, targets, mask, *numbers):
+    def forward(ctx, x, weight, targets, mask, keep_logits, *numbers):
         with timed("linear_cross_entropy_fwd"):
-            loss, logp, state = ops._binding().linear_ce_fwd(x, weight, targets, mask, *numbers, any(ctx.needs_input_grad[:2]))
+            keep = keep_logits and any(ctx.needs_input_grad[:2])
+            loss, logp, state = ops._binding().linear_ce_fwd(x, weight, targets, mask, *numbers, keep)
         ctx.save_for_backward(x, weight, targets, mask, state)
         ctx.numbers = numbers
         ctx.mark_non_differentiable(logp)
@@ -71,36 +72,38 @@ class LinearCrossEntropyFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss, _dlogp):
         if dloss is None:
-            return (None,) * 6
+            return (None,) * 7
         *tensors, state = ctx.saved_tensors
         with timed("linear_cross_entropy_bwd"):
             dx, dw = ops._binding().linear_ce_bwd(*tensors, *ctx.numbers, state, dloss, *ctx.needs_input_grad[:2])
-        return dx, dw, None, None, None, None
+        return dx, dw, None, None, None, None, None
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, mask: torch.Tensor | None = None,
-                         denominator: float | None = None, ignore_index: int = -100):
+                         denominator: float | None = None, ignore_index: int = -100, keep_logits: bool = True):
     """(loss, logp): the scalar loss, differentiable in ``x`` and ``weight``, and each token's log probability (no gradient).
 
     x [..., C] and weight [V, C] float32, bfloat16 or float16, of one dtype; targets [...] int64 or int32; mask [...] bool
-    or uint8 (a token counts where it is not 0), or floating weights.
+    or uint8 (a token counts where it is not 0), or floating weights.  With ``keep_logits`` false none are held for the
+    backward, which then forms them again.
     """
     numbers = _check(denominator, ignore_index)
     x, weight = _as_one(x, weight)
     if ops._use_binding() and torch.autograd.forward_ad._current_level < 0:  # (forward mode is refused by the Function)
-        return ops._binding().linear_ce(x, weight, targets, mask, *numbers)
-    return LinearCrossEntropyFn.apply(x, weight, targets, mask, *numbers)
+        return ops._binding().linear_ce(x, weight, targets, mask, *numbers, bool(keep_logits))
+    return LinearCrossEntropyFn.apply(x, weight, targets, mask, bool(keep_logits), *numbers)
 
 
 def linear_cross_entropy_and_grad(x: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, mask: torch.Tensor | None = None,
-                                  denominator: float | None = None, ignore_index: int = -100, grad_scale: float = 1.0):
+                                  denominator: float | None = None, ignore_index: int = -100, grad_scale: float = 1.0,
+                                  keep_logits: bool = True):
     """(loss, logp, dx, dweight): linear_cross_entropy and grad_scale times its gradients, in the tensors' dtypes. No autograd.
 
-    ``grad_scale`` is the loss scale of float16 training (the loss itself is not scaled).
+    ``grad_scale`` is the loss scale of float16 training (the loss itself is not scaled); ``keep_logits`` as there.
     """
     numbers = _check(denominator, ignore_index)
     xs, ws = _as_one(x, weight)
-    loss, logp, dx, dw = call("linear_ce_and_grad", xs, ws, targets, mask, *numbers, float(grad_scale))
+    loss, logp, dx, dw = call("linear_ce_and_grad", xs, ws, targets, mask, *numbers, float(grad_scale), bool(keep_logits))
     return loss, logp, dx.to(x.dtype), dw.to(weight.dtype)
 
 

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from mhc_mlx_amd import linear_cross_entropy, linear_cross_entropy_and_grad
+from mhc_mlx_amd import kernel_timer, linear_cross_entropy, linear_cross_entropy_and_grad
 from tests._block import ce64
 from tests._train import close
 
@@ -149,3 +149,31 @@ def test_few_tokens_over_a_vocabulary_that_tiles_read_faster(T, dt):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, linear_cross_entropy(x, w, y, mask)))
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T", [6, 700])
+def test_logits_that_are_not_to_be_kept(dt, T):
+    """What lies between forward and backward does not grow with the vocabulary; gradients are within the same bounds."""
+    V, C = 20000, 1024
+    x, w = rand(T, (T, C), (V, C))
+    w = (w * C ** -0.5).to(dt)
+    y = torch.arange(T, device="cuda") * 17 % V
+    x = (x + 3.0 * w[y].float()).to(dt)
+    ref = ce64(x, w, y)
+    xs, ws = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    held = {}
+    for keep in (True, False):
+        before = torch.cuda.memory_allocated()
+        loss, logp = linear_cross_entropy(xs, ws, y, keep_logits=keep)
+        held[keep] = torch.cuda.memory_allocated() - before
+        dx, dw = torch.autograd.grad(loss, [xs, ws])
+        fused = linear_cross_entropy_and_grad(x, w, y, keep_logits=keep)
+        with kernel_timer():
+            timed = linear_cross_entropy(xs, ws, y, keep_logits=keep)
+            grads = torch.autograd.grad(timed[0], [xs, ws])
+        for k, (value, bound) in ref.items():
+            close(dict(loss=loss, logp=logp, dx=dx, dw=dw)[k], value, bound, f"{k} {keep}")
+        assert all(torch.equal(a, b) for a, b in zip(fused, (loss, logp, dx, dw)))
+        assert all(torch.equal(a, b) for a, b in zip((*timed, *grads), (loss, logp, dx, dw)))
+    assert held[True] >= T * V * 4 and held[False] < 64 * T + 4096
