@@ -500,15 +500,15 @@ int mhc_linear_int8(const int8_t* x, int64_t ldx, const float* x_scales, const i
                     void* workspace, size_t workspace_bytes, void* stream);
 
 /* --------------------------------------------------------------------- */
-/* Softmax cross entropy of logits that are not stored                     */
+/* Softmax cross entropy from hidden states                                */
 /* --------------------------------------------------------------------- */
 
 /* Arguments shared by the calls.  x [T, C] and w [V, C] of `dtype` with rows
  * ldx and ldw elements apart; targets [T] int64; weights [T] of weights_dtype
- * (fp32, or MHC_DTYPE_U8: 0 or 1) or NULL (all one).  A token of weight 0 or
- * with the target ignore_index is left out: its row of x is not read.
- * denominator > 0 divides the sum; 0: the sum of the weights of the tokens
- * that are not left out (1 if that is 0). */
+ * (fp32, or MHC_DTYPE_U8: 0 or not) or NULL (all one).  A token of weight 0 or
+ * with the target ignore_index is left out: what its row of x holds has no
+ * effect (of up to 16 tokens it is read).  denominator > 0 divides the sum; 0:
+ * the sum of the weights of the tokens that are not left out (1 if that is 0). */
 typedef struct {
   const void* x;
   int64_t ldx;
@@ -529,9 +529,10 @@ typedef struct {
 /* Bytes of what the forward leaves for the backward. */
 size_t mhc_linear_ce_state_bytes(int64_t T);
 
-/* Bytes of the logits, for args->logits, in which the forward then keeps them
- * and the backward finds them; 0 where that does not pay (C below 768, of fp32
- * below 256, and more than 8 tokens, of fp32 16) or they are more than 2 GiB.
+/* Bytes of the logits, fp32 for all T tokens, for args->logits, in which the
+ * forward then keeps them and the backward finds them; 0 where that does not
+ * pay (C below 768, of fp32 below 256, and more than 8 tokens, of fp32 16) or
+ * they are more than 2 GiB.
  * With args->logits NULL the backward forms them again. */
 size_t mhc_linear_ce_logits_bytes(const mhc_linear_ce_args* args);
 
@@ -549,7 +550,8 @@ size_t mhc_linear_ce_bwd_workspace_bytes(const mhc_linear_ce_args* args, int wan
 /* grad_scale (times *dloss, if not NULL) times the gradients of the loss:
  * dx [T, C] (0 for tokens left out) and dw [V, C], contiguous, of `dtype`, each
  * written if not NULL.  dz = softmax - onehot, times the tokens' weights over
- * the largest of them, is rounded to `dtype` as an operand of the products. */
+ * the largest of them, is rounded to `dtype` as an operand of the products (not
+ * of up to 8 tokens whose logits were kept). */
 int mhc_linear_ce_bwd(const mhc_linear_ce_args* args, const void* state, const float* dloss,
                       float grad_scale, void* dx, void* dw, void* workspace,
                       size_t workspace_bytes, void* stream);

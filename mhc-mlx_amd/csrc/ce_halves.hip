@@ -117,7 +117,7 @@ MHC_DEV void put_parts(_Float16* high, _Float16* low, const float (&v)[8]) {
 }
 
 // dz, each element as two parts for each of its two products: 12 bytes go by for
-// each (900 x 32768: 354 MB in 72 us, 4.9 TB/s).
+// each (900 x 32768: 354 MB in 73 us, 4.8 TB/s).
 __global__ __launch_bounds__(256) void parts_kernel(const Gradient g, const Kept kept, const Halves halves, const Parts parts, int64_t N, const int* live) {
   const uint32_t wide = (uint32_t)ceil_div(parts.pitch, 256);
   const int64_t rows = *live, m0 = (int64_t)(blockIdx.x / wide) * 32, n = (int64_t)(blockIdx.x % wide) * 256 + threadIdx.x % 32 * 8;

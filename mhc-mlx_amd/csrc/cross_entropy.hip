@@ -1,12 +1,13 @@
-// Softmax cross entropy of logits z = x W^T that are never stored whole, and
-// its gradient.
+// Softmax cross entropy of logits z = x W^T, and its gradient.  Without gradients
+// the logits are not stored; with them up to 2 GiB are, in fp32.
 //
 //   lp_t = z[t, y_t] - log sum_v exp z[t, v];  loss = -sum_t w_t lp_t / D
 //   dz = w_t / D (softmax(z) - [v = y_t]);  dx = dz W;  dW = dz^T x
 //
 // Tokens that count for nothing (weight 0, or the ignored target) are left out
 // at the start: the others' rows of x are brought together, and every product
-// below takes as many rows as there are of them, which only the device knows.
+// below takes as many rows as there are of them, which only the device knows
+// (sums_rows_kernel multiplies all of up to 16 and takes the live ones' sums).
 //
 // Forward: the logits' product keeps of each tile a largest value and a sum of
 // exponentials for each row, which are joined.  Backward: the vocabulary goes

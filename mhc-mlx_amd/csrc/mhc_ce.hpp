@@ -112,6 +112,15 @@ struct Kept {
 inline int64_t kept_pitch(int64_t V) { return (V + 63) / 64 * 64; }
 
 // Logits to dz = coef (softmax - [v = target]), zeros past the last column.
+//
+// dz of 16-bit operands is rounded to their type, since it is an operand of two
+// products of that type: with the largest weight brought to 1 (and fp16's 2^14)
+// an element is off by 2^-8 (2^-11) of itself at most, which a product's sums
+// average out where many elements count; a row of dW that one token's element
+// makes up is off by as much as its own rounding adds (8192 x 50257 x 4096 bf16:
+// dx and dW 2.0e-3 off in the root mean square, 1.7e-3 from dz in fp32, which is
+// the outputs' rounding alone).  Two parts of dz, as fp32's, would double both
+// products (4.4 ms of 6.8).  The exponential is the hardware's, 2^-22 of itself.
 struct Gradient {
   const int* target;
   const float *coef, *top, *inv;

@@ -1271,8 +1271,11 @@ struct Cut {
 // CUs at it (1.3 PFLOP/s); a stage of fp32 has half the k (timed before values
 // were lifted, which takes 5 % more of a stage from 64 x 128 on).  A stage of
 // int8 has twice the k of a 16-bit one and takes its time, so that the outputs
-// count for more: `more8` for each further tile of a CU (from 1001 x 2050 x 1100
-// and 16384 x 16384 x 4096).
+// count for more: `more8` for each further tile of a CU, fitted.  Of 140 sizes,
+// 65 to 16384 rows by ten layers of 512 x 512 to 16384 x 4096, the choice with it
+// is within 5 % of the fastest tile in all and 0.3 % from it in the mean; without
+// it 11 are further off, by up to 26 % (8192 x 512 x 512 12.7 and 10.1 us, 16384 x
+// 1024 x 1024 33.7 and 27.4, 1001 x 2050 x 1100 14.7 and 12.1).
 struct TileCost {
   int bm, bn, fit;
   float ends, alone16, busy16, alone32, busy32, more8;

@@ -1,24 +1,24 @@
-"""Softmax cross entropy over a vocabulary, from the last hidden states and the head's weight, without the logits as a tensor.
+"""Softmax cross entropy over a vocabulary, from the last hidden states and the head's weight.
 
 For a token with hidden state x and target y, and the logits z = weight x:
 
     logp = log_softmax(z)[y];  loss = -sum w logp / D,   D = denominator, or the sum of the weights (1 if that is 0)
 
 Tokens of weight 0 (a prompt, padding) and those whose target is ``ignore_index`` are left out whatever their hidden states
-hold, NaN among them: they add nothing to the loss, their log probability is given as 0, their gradient is 0, and the
-products are formed without their rows.  A target outside [0, V) of a token that counts makes the loss, that token's
-gradient and the weight's NaN (it cannot be refused without waiting for the GPU).
+hold, NaN among them: they add nothing to the loss, their log probability is given as 0, their gradient is 0, and the products
+of more than 16 tokens are formed without their rows.  A target outside [0, V) of a token that counts makes the loss, that
+token's gradient and the weight's NaN (it cannot be refused without waiting for the GPU).
 
-The logits are formed in fp32 of exact products. For the gradients, softmax - onehot, times the token's weight over the
-largest one, is rounded once to x's dtype as an operand of two more products, in pieces of the vocabulary (of up to 8 tokens
-it is not rounded); it is formed of the logits that the forward kept, where they take up to 2 GiB (and C is 768 or more, of
-float32 256, or the tokens are few), or of logits that are formed again. Of float32 operands the products are those of
-linear_act; of many tokens the logits, and from kept logits the gradients, are formed of fp16 parts, which hold a value to
-2^-24 of itself and to 2^-40 of its row's largest (of the gradients' sums, of the largest term in their row of x or column
-of the vocabulary). Beside copies of operands whose rows are no whole four-byte words, a call takes workspace in proportion
-to the tokens (their rows of x, the sums of its gradient, eight bytes for each 64 to 256 columns) and up to some 0.5 GB for
-pieces of the vocabulary, whatever its size. Kept logits (float32, [T, V]) are held until the backward's graph is
-freed; without gradients, or with ``keep_logits`` false, none are.
+The logits are formed in fp32 of exact products. For the gradients, softmax - onehot, times the token's weight over the largest
+one, is rounded once to x's dtype as an operand of two more products, in pieces of the vocabulary (of up to 8 tokens whose
+logits were kept it is not rounded); it is formed of the logits that the forward kept, where they take up to 2 GiB (and C is
+768 or more, of float32 256, or the tokens are few), or of logits that are formed again. Of float32 operands the products are
+those of linear_act; of many tokens the logits, and from kept logits the gradients, are formed of fp16 parts, which hold a
+value to 2^-24 of itself and to 2^-40 of its row's largest (of the gradients' sums, of the largest term in their row of x or
+column of the vocabulary). Beside copies of operands whose rows are no whole four-byte words, a call takes workspace in
+proportion to the tokens (their rows of x, the sums of its gradient, eight bytes for each 32 to 256 columns) and up to some 0.5
+GB for pieces of the vocabulary, whatever its size. Kept logits (float32, [T, V]) are held until the backward's graph is freed;
+without gradients, or with ``keep_logits`` false, none are.
 
 x and weight are taken as they are, under torch.autocast too; there, where their dtypes differ (a 16-bit hidden state and a
 head's float32 weight), both are brought to the autocast dtype, as nn.Linear does, and gradients have the tensors' own.

@@ -4,9 +4,9 @@
 
 ``Int8Rows`` holds codes (int8, [..., K]) and scales (float32, [...]): a row's values are its codes times its scale.
 ``quantize_int8`` makes them of float32, bfloat16 or float16 rows (codes are rint(127 x / max|x|)), ``add_rms_norm_int8`` of
-normed ones.  The products' sums are exact (32-bit whole numbers, K below 2^17), or those of up to 16 parts of them where
-there are few outputs, and are scaled and added up in fp32; the output is float32, bfloat16 or float16, the residual of its
-dtype, the bias of any floating dtype (read as float32).
+normed ones.  The products' sums are exact (32-bit whole numbers, K below 2^17), or those of up to 16 parts of them where there
+are few outputs, and are scaled and added up in fp32 (times x's scale they have to stay in its range); the output is float32,
+bfloat16 or float16, the residual of its dtype, the bias of any floating dtype (read as float32).
 
 All of it is for serving: nothing here has a gradient, and results of inputs that require one carry none.
 
