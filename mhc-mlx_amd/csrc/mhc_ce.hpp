@@ -120,7 +120,8 @@ inline int64_t kept_pitch(int64_t V) { return (V + 63) / 64 * 64; }
 // makes up is off by as much as its own rounding adds (8192 x 50257 x 4096 bf16:
 // dx and dW 2.0e-3 off in the root mean square, 1.7e-3 from dz in fp32, which is
 // the outputs' rounding alone).  Two parts of dz, as fp32's, would double both
-// products (4.4 ms of 6.8).  The exponential is the hardware's, 2^-22 of itself.
+// products (4.4 ms of 6.8).  The exponential is the hardware's: 2^-22 of itself, and
+// 0 below 2^-126.
 struct Gradient {
   const int* target;
   const float *coef, *top, *inv;
